@@ -495,6 +495,7 @@ void register_attention(pybind11::module& m);
 void register_inference(pybind11::module& m);
 void register_moe(pybind11::module& m);
 void register_comm(pybind11::module& m);
+void register_qk_norm(pybind11::module& m);
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "astrai_b200 sm_100a kernels";
@@ -557,4 +558,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   register_inference(m);
   register_moe(m);
   register_comm(m);
+  register_qk_norm(m);
 }

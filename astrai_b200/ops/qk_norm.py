@@ -1,0 +1,200 @@
+"""RMS norm of every query and key head together with the rotation of its position.
+
+The reference rotates q and k with elementwise ops and then normalises each head
+(astrai/model/components/rope.py:26-33, attention.py:79-84). :func:`qk_norm_rope` does both in one
+pass over the fused projection output, forward and backward, and knows what other checkpoints need:
+the norm before the rotation, the half layout (channel ``i`` rotates with ``i + rot_dim / 2``),
+a rotation of part of each head, and tables scaled for long contexts
+(:func:`astrai_b200.ops.rope.scaled_rope_table`).
+
+With ``z`` one head, ``R`` the rotation and ``n(z) = z / sqrt(mean z^2 + eps) * w``:
+
+* ``norm="after"``  ``y = n(R x)`` (the reference's order)
+* ``norm="before"`` ``y = R n(x)``
+* ``norm="none"``   ``y = R x``
+
+On CUDA bfloat16, float16 and float32 run on the kernels of ``csrc/qk_norm.cu`` (fp32 inside, one
+rounding at the end); CPU tensors take the plain PyTorch math of :func:`qk_norm_rope_reference`.
+"""
+
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from astrai_b200.ops._ext import native
+
+NORM_MODES = {"none": 0, "after": 1, "before": 2}
+LAYOUTS = ("interleaved", "half")
+
+
+def rotate_reference(x: torch.Tensor, cs: torch.Tensor, layout: str, rot_dim: int, rot_off: int = 0) -> torch.Tensor:
+    """x ``[..., H, D]`` rotated in its own type; cs ``[..., rot_dim / 2, 2]``, one row per token."""
+    c, s = cs[..., 0].unsqueeze(-2), cs[..., 1].unsqueeze(-2)
+    part = x[..., rot_off: rot_off + rot_dim]
+    if layout == "half":
+        a, b = part.chunk(2, -1)
+        turned = torch.cat([a * c - b * s, a * s + b * c], -1)
+    else:
+        a, b = part[..., 0::2], part[..., 1::2]
+        turned = torch.stack([a * c - b * s, a * s + b * c], -1).flatten(-2)
+    return torch.cat([x[..., :rot_off], turned, x[..., rot_off + rot_dim:]], -1)
+
+
+def qk_norm_rope_reference(x, n_heads, n_kv_heads, head_dim, table, q_weight=None, k_weight=None, positions=None,
+                           seq_len=None, eps=1e-6, layout="interleaved", norm="after", rot_dim=None, rot_off=0):
+    """Plain PyTorch math (at least fp32, rounded once); same arguments as :func:`qk_norm_rope`."""
+    rot = head_dim if rot_dim is None else rot_dim
+    H = n_heads + n_kv_heads
+    wide = torch.float64 if x.dtype == torch.float64 else torch.float32
+    z = x[:, : H * head_dim].to(wide).reshape(-1, H, head_dim)
+    if positions is None:
+        positions = torch.arange(z.shape[0], device=x.device) % seq_len
+    cs = table.to(wide)[positions.long()]
+    if norm != "none":
+        w = torch.cat([q_weight.to(wide).expand(n_heads, head_dim), k_weight.to(wide).expand(n_kv_heads, head_dim)])
+
+    def n(t):
+        return t * torch.rsqrt((t * t).mean(-1, keepdim=True) + eps) * w
+
+    if norm == "before":
+        z = n(z)
+    z = rotate_reference(z, cs, layout, rot, rot_off)
+    if norm == "after":
+        z = n(z)
+    return z.reshape(-1, H * head_dim).to(x.dtype)
+
+
+def _rows(t: torch.Tensor) -> torch.Tensor:
+    """A row view that the kernels can read (unit inner stride, 16-byte aligned rows), copied if it is none."""
+    if t.stride(1) != 1 or (t.stride(0) * t.element_size()) % 16 or t.data_ptr() % 16:
+        return t.contiguous()
+    return t
+
+
+def qk_norm_backward(dy, x, dx, n_heads, n_kv_heads, head_dim, table, q_weight, k_weight, positions, seq_len, eps,
+                     half, mode, rot_dim, rot_off):
+    """Backward kernels on row buffers: fills the q and k columns of ``dx``; -> (dq_weight, dk_weight)."""
+    C = native()
+    if mode == 0:  # the transposed rotation
+        C.qk_norm_fwd(dy, dx, n_heads, n_kv_heads, head_dim, table, positions, seq_len, None, None, rot_dim, rot_off,
+                      half, 0, True, eps)
+        return None, None
+    dwq, dwk = torch.empty_like(q_weight), torch.empty_like(k_weight)
+    scratch = torch.empty(C.qk_norm_bwd_scratch(x.shape[0], head_dim, x.device.index), device=x.device,
+                          dtype=torch.float32)
+    if x.shape[0] == 0:
+        return dwq.zero_(), dwk.zero_()
+    C.qk_norm_bwd(dy, x, dx, n_heads, n_kv_heads, head_dim, table, positions, seq_len, q_weight, k_weight, rot_dim,
+                  rot_off, half, mode, eps, dwq, dwk, scratch)
+    return dwq, dwk
+
+
+class _QKNormRopeFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, q_weight, k_weight, table, positions, dims):
+        hq, hkv, D, seq_len, eps, half, mode, rot, off = dims
+        y = torch.empty((x.shape[0], (hq + hkv) * D), device=x.device, dtype=x.dtype)
+        xr = _rows(x)
+        native().qk_norm_fwd(xr, y, hq, hkv, D, table, positions, seq_len, q_weight, k_weight, rot, off, half, mode,
+                             False, eps)
+        ctx.save_for_backward(xr, q_weight, k_weight, table, positions)
+        ctx.dims, ctx.width = dims, x.shape[1]
+        return y
+
+    @staticmethod
+    def backward(ctx, dy):
+        x, q_weight, k_weight, table, positions = ctx.saved_tensors
+        hq, hkv, D, seq_len, eps, half, mode, rot, off = ctx.dims
+        used = (hq + hkv) * D
+        dx = torch.empty((x.shape[0], ctx.width), device=x.device, dtype=x.dtype)
+        if ctx.width > used:  # columns behind the keys are not an input
+            dx[:, used:].zero_()
+        dwq, dwk = qk_norm_backward(_rows(dy), x, dx, hq, hkv, D, table, q_weight, k_weight, positions, seq_len, eps,
+                                    half, mode, rot, off)
+        return dx, dwq, dwk, None, None, None
+
+
+def _check(x, n_heads, n_kv_heads, head_dim, table, q_weight, k_weight, positions, seq_len, layout, norm, rot, off):
+    if layout not in LAYOUTS:
+        raise ValueError(f"layout must be one of {LAYOUTS}, got {layout!r}")
+    if norm not in NORM_MODES:
+        raise ValueError(f"norm must be one of {tuple(NORM_MODES)}, got {norm!r}")
+    if x.dim() != 2 or x.shape[1] < (n_heads + n_kv_heads) * head_dim:
+        raise ValueError(f"x must be [rows, >= {(n_heads + n_kv_heads) * head_dim}], got {tuple(x.shape)}")
+    if rot <= 0 or rot % 2 or off < 0 or rot + off > head_dim:
+        raise ValueError(f"rot_dim {rot} at offset {off} does not fit an even part of head_dim {head_dim}")
+    if table.dim() != 3 or table.shape[1] * 2 != rot or table.shape[2] != 2:
+        raise ValueError(f"table must be [max_pos, {rot // 2}, 2], got {tuple(table.shape)}")
+    if norm != "none" and (q_weight is None or k_weight is None or q_weight.numel() != head_dim
+                           or k_weight.numel() != head_dim):
+        raise ValueError(f"norm={norm!r} needs q_weight and k_weight of {head_dim} entries")
+    if positions is None and not seq_len:
+        raise ValueError("positions or seq_len must be given")
+    if positions is not None and positions.numel() != x.shape[0]:
+        raise ValueError(f"positions must have one entry per row ({x.shape[0]}), got {positions.numel()}")
+
+
+def _kernel_positions(positions: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    if positions is None:
+        return None
+    if positions.dtype == torch.int32 and positions.dim() == 1 and positions.is_contiguous():
+        return positions
+    return positions.reshape(-1).to(torch.int32).contiguous()
+
+
+def qk_norm_rope(x: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: int, table: torch.Tensor,
+                 q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None,
+                 positions: Optional[torch.Tensor] = None, seq_len: Optional[int] = None, eps: float = 1e-6,
+                 layout: str = "interleaved", norm: str = "after", rot_dim: Optional[int] = None,
+                 rot_off: int = 0) -> torch.Tensor:
+    """Normalise and rotate the query and key heads of ``x`` -> ``[rows, (n_heads + n_kv_heads) * head_dim]``.
+
+    ``x`` ``[rows, W]`` holds the query heads, then the key heads, in its first columns (the fused QKV
+    projection's output; any row stride; columns behind them are not read). ``table`` is the fp32 (cos,
+    sin) table ``[max_pos, rot_dim / 2, 2]``, ``positions`` one integer per row (None: row ``r`` has
+    position ``r % seq_len``); a position outside the table leaves its row unrotated and sets the device
+    error word. ``rot_dim`` channels from ``rot_off`` are rotated (None: all). On CUDA ``head_dim`` is at
+    most 256, and it, ``rot_dim`` and ``rot_off`` are multiples of 8. Differentiable in ``x`` and the
+    weights.
+    """
+    rot = head_dim if rot_dim is None else rot_dim
+    _check(x, n_heads, n_kv_heads, head_dim, table, q_weight, k_weight, positions, seq_len, layout, norm, rot, rot_off)
+    if not x.is_cuda:
+        return qk_norm_rope_reference(x, n_heads, n_kv_heads, head_dim, table, q_weight, k_weight, positions, seq_len,
+                                      eps, layout, norm, rot, rot_off)
+    if norm == "none":
+        q_weight = k_weight = None
+    pos = _kernel_positions(positions)
+    dims = (n_heads, n_kv_heads, head_dim, int(seq_len or 0), float(eps), layout == "half", NORM_MODES[norm], rot,
+            rot_off)
+    if torch.is_grad_enabled() and (x.requires_grad or (q_weight is not None and (q_weight.requires_grad
+                                                                                 or k_weight.requires_grad))):
+        return _QKNormRopeFn.apply(x, q_weight, k_weight, table, pos, dims)
+    y = torch.empty((x.shape[0], (n_heads + n_kv_heads) * head_dim), device=x.device, dtype=x.dtype)
+    native().qk_norm_fwd(_rows(x), y, n_heads, n_kv_heads, head_dim, table, pos, dims[3], q_weight, k_weight, rot,
+                         rot_off, dims[5], dims[6], False, dims[4])
+    return y
+
+
+def qk_norm_rope_(x: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: int, table: torch.Tensor,
+                  q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None,
+                  positions: Optional[torch.Tensor] = None, seq_len: Optional[int] = None, eps: float = 1e-6,
+                  layout: str = "interleaved", norm: str = "after", rot_dim: Optional[int] = None,
+                  rot_off: int = 0) -> torch.Tensor:
+    """:func:`qk_norm_rope` in place on the query and key columns of ``x`` (no gradient) -> ``x``."""
+    rot = head_dim if rot_dim is None else rot_dim
+    _check(x, n_heads, n_kv_heads, head_dim, table, q_weight, k_weight, positions, seq_len, layout, norm, rot, rot_off)
+    if torch.is_grad_enabled() and x.requires_grad:
+        raise RuntimeError("qk_norm_rope_ has no gradient: use qk_norm_rope")
+    if not x.is_cuda:
+        x[:, : (n_heads + n_kv_heads) * head_dim] = qk_norm_rope_reference(
+            x, n_heads, n_kv_heads, head_dim, table, q_weight, k_weight, positions, seq_len, eps, layout, norm, rot,
+            rot_off)
+        return x
+    if norm == "none":
+        q_weight = k_weight = None
+    native().qk_norm_fwd(x, x, n_heads, n_kv_heads, head_dim, table, _kernel_positions(positions), int(seq_len or 0),
+                         q_weight, k_weight, rot, rot_off, layout == "half", NORM_MODES[norm], False, float(eps))
+    return x

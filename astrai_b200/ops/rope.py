@@ -11,6 +11,7 @@ QKV projection output, so q and k are never copied.
 
 from __future__ import annotations
 
+import math
 from typing import Optional
 
 import torch
@@ -50,3 +51,37 @@ def rope_inplace(buf: torch.Tensor, col0: int, n_heads: int, head_dim: int, tabl
     """
     rd = head_dim if rot_dim is None else rot_dim
     native().rope_(buf, col0, n_heads, head_dim, positions, seq_len, table, inverse, rd, rot_off)
+
+
+ROPE_SCALING_METHODS = ("linear", "yarn")
+
+
+def scaled_rope_table(dim: int, max_len: int, base: float = 10000.0, method: str = "linear", factor: float = 1.0,
+                      original_max_len: Optional[int] = None, beta_fast: float = 32.0, beta_slow: float = 1.0,
+                      attention_factor: Optional[float] = None, device=None) -> torch.Tensor:
+    """fp32 ``[max_len, dim/2, 2]`` (cos, sin) table for contexts ``factor`` times longer than trained.
+
+    * ``linear``: position interpolation, every angle divided by ``factor``.
+    * ``yarn`` (Peng et al., "YaRN: Efficient Context Window Extension of Large Language Models", 2023):
+      a pair that turns r times over ``original_max_len`` positions is interpolated if r <= ``beta_slow``,
+      left alone if r >= ``beta_fast``, and mixed linearly in r between; (cos, sin) are multiplied by
+      ``attention_factor`` (None: ``0.1 ln(factor) + 1``, and 1 for factors up to 1), which scales the
+      scores by its square. The table is then no pure rotation.
+    """
+    if method not in ROPE_SCALING_METHODS:
+        raise ValueError(f"method must be one of {ROPE_SCALING_METHODS}, got {method!r}")
+    if factor <= 0:
+        raise ValueError(f"factor must be positive, got {factor}")
+    inv = base ** (-torch.arange(0, dim, 2, dtype=torch.float64, device=device) / dim)
+    gain = 1.0
+    if method == "linear":
+        inv = inv / factor
+    else:
+        if not original_max_len or beta_fast <= beta_slow:
+            raise ValueError("yarn needs original_max_len and beta_fast > beta_slow")
+        turns = original_max_len * inv / (2 * math.pi)
+        keep = ((turns - beta_slow) / (beta_fast - beta_slow)).clamp(0, 1)
+        inv = inv / factor * (1 - keep) + inv * keep
+        gain = attention_factor if attention_factor is not None else 0.1 * math.log(factor) + 1 if factor > 1 else 1.0
+    ang = torch.outer(torch.arange(max_len, dtype=torch.float64, device=device), inv)
+    return (gain * torch.stack([torch.cos(ang), torch.sin(ang)], dim=-1)).float().contiguous()
