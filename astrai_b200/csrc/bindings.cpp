@@ -493,6 +493,7 @@ int64_t read_error() { return astrai_host::read_and_clear_error(); }
 
 void register_attention(pybind11::module& m);
 void register_inference(pybind11::module& m);
+void register_kv8(pybind11::module& m);
 void register_moe(pybind11::module& m);
 void register_comm(pybind11::module& m);
 void register_qk_norm(pybind11::module& m);
@@ -556,6 +557,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("read_error", &read_error);
   register_attention(m);
   register_inference(m);
+  register_kv8(m);
   register_moe(m);
   register_comm(m);
   register_qk_norm(m);

@@ -1,0 +1,774 @@
+// Paged KV cache in 8-bit integers (sm_100a): append with quantisation, read-back, and causal
+// attention of one or a few new tokens over it. No counterpart in the reference project, whose cache
+// holds the model's type (astrai/inference/core/cache.py:189-276).
+//
+// Layout per layer: values int8 [page][kv_head][slot][D], and one fp32 magnitude for each block of
+// `block` tokens and head, [page][kv_head][page_size / block]. A stored integer q stands for
+// q * absmax / 127. Keeping the magnitude itself instead of the step absmax / 127 makes quantisation
+// exact to describe: q = rint(127 x / absmax), with 127 x exact in fp32 for 16-bit inputs and the
+// division correctly rounded, so ties fall where the real quotient has them.
+//
+// Attention holds the integers as fp16 (exact) on the tensor cores' mma.m16n8k16: the work is one
+// pass over the cache at a few operations per byte, bound by HBM, and fragments straight from
+// converted registers spare the second trip through shared memory that tcgen05 operands would need.
+// S^T = K Q^T and O^T = V^T P^T put the tokens (then the channels) on the 16-row side and the query
+// rows that share a KV head on the 8-column side, so a group of 4 query heads wastes half a tile and
+// not three quarters.
+#include <algorithm>
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace astrai {
+namespace {
+
+// ------------------------------------------------------------------ append
+struct AppendParams {
+  const void* src[2];           // k, v [B, S, Hkv, D]
+  long long sb[2], st[2], sh[2];  // their strides (elements)
+  signed char* cache[2];
+  float* absmax[2];
+  const int* table;
+  const int* starts;
+  const int* lens;
+  int B, S, Hkv, page_size, n_pages, max_pages, windows;
+};
+
+template <typename T>
+__device__ __forceinline__ float bits_to_float(unsigned short u) {
+  if constexpr (std::is_same<T, __half>::value) return __half2float(__ushort_as_half(u));
+  else return __bfloat162float(__ushort_as_bfloat16(u));
+}
+template <typename T>
+__device__ __forceinline__ T from_float(float x) {
+  if constexpr (std::is_same<T, __half>::value) return __float2half_rn(x);
+  else return __float2bfloat16_rn(x);
+}
+
+// One block of tokens of one head of k or v: its live tokens and the new ones end under the larger
+// of their magnitudes. WARPS warps share it, at most 32 tokens each, whose values stay in registers
+// between the maximum and the rounding. A row's append starts at starts[b] and ends at lens[b]; what
+// the cache held from starts[b] on is void. A block with an infinite or NaN input gets the magnitude
+// NaN: reading it gives NaN, as the input would have.
+template <typename T, int D, int BLOCK>
+__global__ void __launch_bounds__(128) kv8_append_kernel(const AppendParams p) {
+  constexpr int WARPS = BLOCK > 32 ? BLOCK / 32 : 1;  // warps per item
+  constexpr int TOK = BLOCK / WARPS;                  // tokens per warp
+  constexpr int LPT = D / 8;                          // lanes per token: 8 values (16 bytes) each
+  constexpr int TPI = 32 / LPT;                       // tokens per warp-wide load
+  constexpr int N = TOK / TPI;
+  __shared__ unsigned most_s[4];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const long long item = blockIdx.x * (4LL / WARPS) + warp / WARPS;
+  const int kv = (int)(item & 1);
+  const int h = (int)((item >> 1) % p.Hkv);
+  const long long bw = (item >> 1) / p.Hkv;
+  const int w = (int)(bw % p.windows), b = (int)(bw / p.windows);
+  bool on = b < p.B;
+  int start = 0, end = 0, base = 0, page = -1, off = 0;
+  if (on) {
+    start = min(max(p.starts[b], 0), p.max_pages * p.page_size);
+    end = min(p.lens[b], start + p.S);
+    base = (start / BLOCK + w) * BLOCK;
+    on = base < end && start < end;
+    const int lp = base / p.page_size;
+    if (on && lp < p.max_pages) page = p.table[(long long)b * p.max_pages + lp];
+    off = base % p.page_size;
+    on = on && page >= 0 && page < p.n_pages;
+  }
+  const int t0 = (warp % WARPS) * TOK + lane / LPT, c = lane % LPT;
+  const T* src = static_cast<const T*>(p.src[kv]) + (long long)b * p.sb[kv] + (long long)h * p.sh[kv] + c * 8;
+  uint4 raw[N];
+  unsigned most = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int t = base + t0 + i * TPI;
+    raw[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (on && t >= start && t < end)
+      raw[i] = *reinterpret_cast<const uint4*>(src + (long long)(t - start) * p.st[kv]);
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i)  // magnitudes compare as integers, infinities and NaN above all others
+    most = __vmaxu2(most, __vmaxu2(__vmaxu2(raw[i].x & 0x7fff7fffu, raw[i].y & 0x7fff7fffu),
+                                   __vmaxu2(raw[i].z & 0x7fff7fffu, raw[i].w & 0x7fff7fffu)));
+  most = max(most & 0xffffu, most >> 16);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffff, most, o));
+  if (WARPS > 1) {
+    if (lane == 0) most_s[warp] = most;
+    __syncthreads();
+    const int w0 = warp / WARPS * WARPS;
+#pragma unroll
+    for (int i = 0; i < WARPS; ++i) most = max(most, most_s[w0 + i]);
+  }
+  const long long row0 = ((long long)page * p.Hkv + h) * p.page_size + off;  // the block's first token
+  float* ap = p.absmax[kv] + row0 / BLOCK;
+  const bool live = on && base < start;
+  const float was = live ? *ap : 0.f;
+  // every warp of the item has read the old magnitude before one replaces it
+  if (WARPS > 1) __syncthreads();
+  if (!on) return;
+  const float fresh = bits_to_float<T>((unsigned short)most);
+  const bool finite = fresh < INFINITY;  // false for NaN, too
+  const float now = finite ? (was >= fresh || was != was ? was : fresh) : __int_as_float(0x7fffffff);
+  if (lane == 0 && warp % WARPS == 0) *ap = now;
+  // products with 127 stay finite; scaling by a power of two changes no quotient
+  const float pre = now > 1e30f ? 0x1p-16f : 1.f;
+  const float by = now * pre, mul = 127.f * pre, old = was * pre;
+  const bool some = now > 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int t = t0 + i * TPI;
+    signed char* dst = p.cache[kv] + (row0 + t) * D + c * 8;
+    uint2 out;
+    signed char* q = reinterpret_cast<signed char*>(&out);
+    if (base + t >= start && base + t < end) {
+      const unsigned short* e = reinterpret_cast<const unsigned short*>(&raw[i]);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float v = some ? rintf(__fdiv_rn(bits_to_float<T>(e[j]) * mul, by)) : 0.f;
+        q[j] = (signed char)(int)fminf(fmaxf(v, -127.f), 127.f);
+      }
+      *reinterpret_cast<uint2*>(dst) = out;
+    } else if (base + t < start && now > was) {  // live under a magnitude that grew
+      out = *reinterpret_cast<const uint2*>(dst);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) q[j] = (signed char)(int)rintf(__fdiv_rn((float)q[j] * old, by));
+      *reinterpret_cast<uint2*>(dst) = out;
+    }
+  }
+}
+
+// ------------------------------------------------------------------ read-back
+struct GatherParams {
+  const signed char* cache[2];
+  const float* absmax[2];
+  const int* table;
+  const int* starts;  // null: from token 0
+  const int* lens;
+  void* out[2];       // [B, total, Hkv, D]
+  int B, total, Hkv, page_size, n_pages, max_pages, block;
+};
+
+constexpr float kStep = 1.f / 127.f;
+
+// One thread per 16 values of k and the same 16 of v.
+template <typename T, int D>
+__global__ void __launch_bounds__(256) kv8_gather_kernel(const GatherParams p) {
+  constexpr int C = D / 16;
+  const long long n = (long long)p.B * p.total * p.Hkv * C;
+  for (long long i = blockIdx.x * 256LL + threadIdx.x; i < n; i += gridDim.x * 256LL) {
+    const int c = (int)(i % C);
+    const long long r = i / C;
+    const int h = (int)(r % p.Hkv);
+    const long long bt = r / p.Hkv;
+    const int t = (int)(bt % p.total), b = (int)(bt / p.total);
+    const int pos = (p.starts ? p.starts[b] : 0) + t;
+    int page = -1;
+    if (pos >= 0 && pos < p.lens[b] && pos / p.page_size < p.max_pages)
+      page = p.table[(long long)b * p.max_pages + pos / p.page_size];
+    const bool ok = page >= 0 && page < p.n_pages;
+    const long long row = ((long long)page * p.Hkv + h) * p.page_size + pos % p.page_size;
+#pragma unroll
+    for (int kv = 0; kv < 2; ++kv) {
+      uint4 o[2] = {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
+      if (ok) {
+        const uint4 raw = *reinterpret_cast<const uint4*>(p.cache[kv] + row * D + c * 16);
+        const float step = p.absmax[kv][row / p.block] * kStep;
+        const signed char* q = reinterpret_cast<const signed char*>(&raw);
+        T* v = reinterpret_cast<T*>(o);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) v[j] = from_float<T>((float)q[j] * step);
+      }
+      uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.out[kv]) + i * 16);
+      dst[0] = o[0];
+      dst[1] = o[1];
+    }
+  }
+}
+
+// ------------------------------------------------------------------ attention
+struct AttendParams {
+  const void* q;  // [B, S, Hq, D]
+  long long qb, qs, qh;
+  const signed char* kc;
+  const signed char* vc;
+  const float* ka;
+  const float* va;
+  const int* table;
+  const int* lens;
+  const int* starts;  // null: lens - S
+  void* out;          // [B, S, Hq, D] contiguous
+  float* part_o;      // [2 * ctas][R][D]
+  float* part_s;      // [2 * ctas][R][3]: running max of scores, of weights, sum
+  int B, S, Hq, Hkv, G, groups, page_size, n_pages, max_pages, block, ctas;
+  float scale;        // softmax scale * log2(e) / 127
+};
+
+constexpr int kWarps = 8;
+constexpr int kTile = 16;                // tokens per warp step
+constexpr int kUnit = kWarps * kTile;    // tokens per unit of work
+constexpr int kMaxBatch = 2048;
+
+__device__ __forceinline__ void cp_async16(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(dst)), "l"(src)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async4(void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((unsigned)__cvta_generic_to_shared(dst)), "l"(src)
+               : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void mma16816(float* d, const unsigned* a, const unsigned* b) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b[0]), "r"(b[1]));
+}
+__device__ __forceinline__ unsigned transpose8x8(unsigned v) {
+  unsigned r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+// Integers to fp16 pairs: a byte u = q + 128 under the high byte 0x64 is the fp16 number 1024 + u, and
+// taking 1152 away is exact. `sel` picks the two bytes of `u` that make the pair.
+__device__ __forceinline__ unsigned ints_to_half2(unsigned u, unsigned sel) {
+  const unsigned m = __byte_perm(u, 0x64646464u, sel);
+  const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&m), __float2half2_rn(1152.f));
+  return *reinterpret_cast<const unsigned*>(&r);
+}
+
+// Tokens that the queries of row b see at most, and the position of its first query.
+__device__ __forceinline__ void row_extent(const AttendParams& p, int b, int& first, int& keys) {
+  const int len = max(p.lens[b], 0);
+  first = p.starts ? min(max(p.starts[b], -(1 << 30)), 1 << 30) : len - p.S;
+  keys = max(0, min(min(len, first + p.S), p.max_pages * p.page_size));
+}
+__device__ __forceinline__ int row_units(const AttendParams& p, int b) {
+  int first, keys;
+  row_extent(p, b, first, keys);
+  return max(1, (keys + kUnit - 1) / kUnit);  // a row without keys still has its zeros to write
+}
+// CTAs that take part: each has a unit at least, so that a segment's CTAs are all those from its first
+// unit's to its last unit's
+__device__ __forceinline__ int live_ctas(const AttendParams& p, long long total) {
+  return (int)min((long long)p.ctas, total);
+}
+// CTA that has unit u when `total` units are dealt out as [c * total / ctas, (c + 1) * total / ctas)
+__device__ __forceinline__ int cta_of(long long u, long long total, int ctas) {
+  return (int)(((u + 1) * ctas - 1) / total);
+}
+
+template <int D>
+__device__ __forceinline__ int swizzle(int row, int chunk) {  // byte offset in a [16][D] tile
+  return D == 128 ? row * 128 + ((chunk ^ (row & 7)) << 4) : row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4);
+}
+
+template <int D>
+struct alignas(16) Stage {
+  unsigned char k[kTile * D];
+  unsigned char v[kTile * D];
+  float ka, va, pad[2];
+};
+
+// Work: every (row b, kv head h, group g of R query rows) is a segment of ceil(keys / 128) units; the
+// units of all segments, in order, are dealt out evenly over the CTAs, whatever the rows' lengths. A
+// CTA's warps take the 16-token tiles of its piece of a segment in turn, each with its own running
+// softmax, and are merged once per piece. A piece that is a whole segment writes the output; others
+// leave partials (at most two per CTA: its first and its last piece) for kv8_combine_kernel.
+//
+// Softmax per query row: m = max of the scores s and l = sum 2^(s - m) as usual. The weights of the
+// integers v are 2^s * absmax_v; they are kept relative to their own running maximum M = max(s +
+// log2 absmax_v), so as fp16 they are at most 1 and lose nothing whatever the magnitudes of the blocks.
+// out = sum w v / l * 2^(M - m) / 127.
+template <typename T, int D, int NT, int STAGES>
+__global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv8_attend_kernel(const AttendParams p) {
+  constexpr int KS = D / 16;     // k-steps of S^T = K Q^T
+  constexpr int MT = D / 16;     // channel tiles of O^T = V^T P^T
+  constexpr int R = 8 * NT;      // query rows of a group
+  constexpr int CH = D / 16;     // 16-byte chunks per token
+  extern __shared__ __align__(128) unsigned char smem[];
+  Stage<D>* ring = reinterpret_cast<Stage<D>*>(smem) + (threadIdx.x >> 5) * STAGES;
+  __shared__ int prefix[kMaxBatch + 1];
+  __shared__ int scan_s[kWarps];
+  __shared__ float stat_s[kWarps][R][3];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the combine waits for this grid itself
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+
+  // units of the rows before each row
+  int before = 0;
+  for (int b0 = 0; b0 < p.B; b0 += kWarps * 32) {
+    const int b = b0 + tid;
+    int v = b < p.B ? row_units(p, b) : 0;
+    const int own = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int u = __shfl_up_sync(0xffffffff, v, o);
+      if (lane >= o) v += u;
+    }
+    if (lane == 31) scan_s[warp] = v;
+    __syncthreads();
+    int sum = 0, all = 0;
+#pragma unroll
+    for (int i = 0; i < kWarps; ++i) {
+      sum += i < warp ? scan_s[i] : 0;
+      all += scan_s[i];
+    }
+    if (b < p.B) prefix[b] = before + sum + v - own;
+    before += all;
+    __syncthreads();
+  }
+  if (tid == 0) prefix[p.B] = before;
+  __syncthreads();
+  const int per = p.Hkv * p.groups;  // segments per row
+  const long long total = (long long)before * per;
+  const int ctas = live_ctas(p, total);
+  if ((int)blockIdx.x >= ctas) return;
+  const long long u_begin = total * blockIdx.x / ctas, u_end = total * (blockIdx.x + 1) / ctas;
+
+  for (long long u = u_begin; u < u_end;) {
+    int lo = 0, hi = p.B - 1;  // the row of unit u: last b with prefix[b] * per <= u
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) / 2;
+      if ((long long)prefix[mid] * per <= u) lo = mid;
+      else hi = mid - 1;
+    }
+    const int b = lo, units = prefix[b + 1] - prefix[b];
+    const int rem = (int)(u - (long long)prefix[b] * per);
+    const int hg = rem / units, unit0 = rem - hg * units;
+    const int n_units = (int)min((long long)(units - unit0), u_end - u);
+    const int h = hg / p.groups, grp = hg - h * p.groups;
+    int first, keys;
+    row_extent(p, b, first, keys);
+
+    // query fragments: lane (g, t) holds channels t * D / 4 .. of query row g of each 8-row tile, as
+    // fp16 scaled by a power of two that brings the row's largest magnitude to [1, 2)
+    unsigned qf[NT][KS][2];
+    float qscale[NT][2];  // of the columns 2t, 2t + 1 of S^T
+    int vis[NT][2];       // keys that those columns see
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int r = grp * R + n * 8 + g, i = r / p.G;
+      const bool ok = r < p.S * p.G;
+      const T* src = static_cast<const T*>(p.q) + (long long)b * p.qb + (long long)i * p.qs +
+                     (long long)(h * p.G + (r - i * p.G)) * p.qh + t * (D / 4);
+      uint4 raw[D / 32];
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j)
+        raw[j] = ok ? reinterpret_cast<const uint4*>(src)[j] : make_uint4(0u, 0u, 0u, 0u);
+      const unsigned short* e = reinterpret_cast<const unsigned short*>(raw);
+      float most = 0.f;
+#pragma unroll
+      for (int j = 0; j < D / 4; ++j) most = fmaxf(most, fabsf(bits_to_float<T>(e[j])));
+      most = fmaxf(most, __shfl_xor_sync(0xffffffff, most, 1));
+      most = fmaxf(most, __shfl_xor_sync(0xffffffff, most, 2));
+      int ex = 0;
+      if (most > 0.f && most < INFINITY) ex = max(ilogbf(most), -120);
+      const float down = ldexpf(1.f, -ex), up = ldexpf(p.scale, ex);
+#pragma unroll
+      for (int s = 0; s < KS; ++s)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const __half2 v = __floats2half2_rn(bits_to_float<T>(e[4 * s + 2 * k]) * down,
+                                              bits_to_float<T>(e[4 * s + 2 * k + 1]) * down);
+          qf[n][s][k] = *reinterpret_cast<const unsigned*>(&v);
+        }
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        qscale[n][k] = __shfl_sync(0xffffffff, up, (2 * t + k) * 4);
+        const int rc = grp * R + n * 8 + 2 * t + k, ic = rc / p.G;
+        vis[n][k] = rc < p.S * p.G && first + ic >= 0 && first + ic < p.lens[b] ? min(first + ic + 1, keys) : 0;
+      }
+    }
+
+    float o[NT][MT][4], m[NT][2], M[NT][2], l[NT][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int k = 0; k < 2; ++k) m[n][k] = M[n][k] = -INFINITY, l[n][k] = 0.f;
+#pragma unroll
+      for (int i = 0; i < MT; ++i)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[n][i][k] = 0.f;
+    }
+
+    // tiles of this warp: first0, first0 + 8, ... below tile_end
+    const int tile_end = min((unit0 + n_units) * kWarps, (keys + kTile - 1) / kTile);
+    const int first0 = unit0 * kWarps + warp;
+    const int count = first0 < tile_end ? (tile_end - first0 + kWarps - 1) / kWarps : 0;
+    const int* trow = p.table + (long long)b * p.max_pages;
+    const int tpp = p.page_size / kTile;  // tiles per page
+    auto page_of = [&](int i) { return i < count ? trow[(first0 + i * kWarps) / tpp] : -1; };
+    auto issue = [&](int i, int page) {
+      if (i < count && page >= 0 && page < p.n_pages) {
+        const int tile = first0 + i * kWarps;
+        const long long row = ((long long)page * p.Hkv + h) * p.page_size + (tile % tpp) * kTile;
+        Stage<D>& st = ring[i % STAGES];
+#pragma unroll
+        for (int j = 0; j < kTile * CH / 32; ++j) {
+          const int c = lane + j * 32, dst = swizzle<D>(c / CH, c % CH);
+          cp_async16(st.k + dst, p.kc + row * D + c * 16);
+          cp_async16(st.v + dst, p.vc + row * D + c * 16);
+        }
+        if (lane == 0) cp_async4(&st.ka, p.ka + row / p.block);
+        if (lane == 1) cp_async4(&st.va, p.va + row / p.block);
+      }
+      cp_async_commit();
+    };
+    int pages[STAGES];  // of the tiles in flight and of the next one to issue
+#pragma unroll
+    for (int i = 0; i < STAGES; ++i) pages[i] = page_of(i);
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) issue(i, pages[i]);
+
+    for (int it = 0; it < count; ++it) {
+      cp_async_wait<STAGES - 2>();
+      __syncwarp();  // this tile has landed for all lanes, and all have left the stage that is refilled now
+      const int page = pages[0];
+#pragma unroll
+      for (int i = 0; i + 1 < STAGES; ++i) pages[i] = pages[i + 1];
+      issue(it + STAGES - 1, pages[STAGES - 2]);
+      pages[STAGES - 1] = page_of(it + STAGES);
+      if (page < 0 || page >= p.n_pages) continue;  // the same for the whole warp
+      const Stage<D>& st = ring[it % STAGES];
+      const int tok = (first0 + it * kWarps) * kTile;
+
+      // S^T: tokens g and g + 8, channels t * D / 4 + 4s .. of k-step s on both sides
+      float sc[NT][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
+#pragma unroll
+      for (int j = 0; j < D / 64; ++j) {
+        const uint4 x = *reinterpret_cast<const uint4*>(st.k + swizzle<D>(g, t * (D / 64) + j));
+        const uint4 y = *reinterpret_cast<const uint4*>(st.k + swizzle<D>(g + 8, t * (D / 64) + j));
+        const unsigned xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const unsigned ux = xs[k] ^ 0x80808080u, uy = ys[k] ^ 0x80808080u;
+          const unsigned a[4] = {ints_to_half2(ux, 0x4140), ints_to_half2(uy, 0x4140), ints_to_half2(ux, 0x4342),
+                                 ints_to_half2(uy, 0x4342)};
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma16816(sc[n], a, qf[n][j * 4 + k]);
+        }
+      }
+
+      const float ka = st.ka, lv = __log2f(st.va);
+      unsigned pf[NT][2];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float w[4], corr[2], corrw[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const float qs = qscale[n][k] * ka;
+          const float s0 = tok + g < vis[n][k] ? sc[n][k] * qs : -INFINITY;
+          const float s1 = tok + g + 8 < vis[n][k] ? sc[n][2 + k] * qs : -INFINITY;
+          float top = fmaxf(s0, s1);
+#pragma unroll
+          for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffff, top, d));
+          const float m1 = fmaxf(m[n][k], top), M1 = fmaxf(M[n][k], top + lv);
+          const float ms = m1 == -INFINITY ? 0.f : m1, Ms = M1 == -INFINITY ? 0.f : M1;
+          corr[k] = exp2f(m[n][k] - ms);
+          corrw[k] = exp2f(M[n][k] - Ms);
+          l[n][k] = l[n][k] * corr[k] + (exp2f(s0 - ms) + exp2f(s1 - ms));
+          w[k] = s0 == -INFINITY ? 0.f : exp2f(s0 + lv - Ms);
+          w[2 + k] = s1 == -INFINITY ? 0.f : exp2f(s1 + lv - Ms);
+          m[n][k] = m1;
+          M[n][k] = M1;
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          o[n][i][0] *= corrw[0], o[n][i][1] *= corrw[1];
+          o[n][i][2] *= corrw[0], o[n][i][3] *= corrw[1];
+        }
+        const __half2 w0 = __floats2half2_rn(w[0], w[1]), w1 = __floats2half2_rn(w[2], w[3]);
+        pf[n][0] = transpose8x8(*reinterpret_cast<const unsigned*>(&w0));
+        pf[n][1] = transpose8x8(*reinterpret_cast<const unsigned*>(&w1));
+      }
+
+      // O^T: lane (g, t) has channels g * D / 8 .. of tokens 2t, 2t + 1, 2t + 8, 2t + 9; channel tile 2j + e
+      // takes channels 4j + 2e (its row g) and 4j + 2e + 1 (row g + 8) of each lane's run
+      unsigned vw[4][D / 32];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int row = 2 * t + (k & 1) + (k >> 1) * 8;
+        if constexpr (D == 128) {
+          const uint4 x = *reinterpret_cast<const uint4*>(st.v + swizzle<D>(row, g));
+          vw[k][0] = x.x ^ 0x80808080u, vw[k][1] = x.y ^ 0x80808080u;
+          vw[k][2] = x.z ^ 0x80808080u, vw[k][3] = x.w ^ 0x80808080u;
+        } else {
+          const uint2 x = *reinterpret_cast<const uint2*>(st.v + swizzle<D>(row, g >> 1) + (g & 1) * 8);
+          vw[k][0] = x.x ^ 0x80808080u, vw[k][1] = x.y ^ 0x80808080u;
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const unsigned x = __byte_perm(vw[0][j], vw[1][j], e ? 0x7362 : 0x5140);
+          const unsigned y = __byte_perm(vw[2][j], vw[3][j], e ? 0x7362 : 0x5140);
+          const unsigned a[4] = {ints_to_half2(x, 0x4140), ints_to_half2(x, 0x4342), ints_to_half2(y, 0x4140),
+                                 ints_to_half2(y, 0x4342)};
+#pragma unroll
+          for (int n = 0; n < NT; ++n) mma16816(o[n][j * 2 + e], a, pf[n]);
+        }
+      }
+    }
+    cp_async_wait<0>();
+    __syncthreads();  // the rings become the merge buffer
+
+    // merge the warps: sums over the tokens of a warp lie on lanes of equal t
+    float* merge = reinterpret_cast<float*>(smem);  // [warp][R][D]
+#pragma unroll
+    for (int n = 0; n < NT; ++n)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        float s = l[n][k];
+#pragma unroll
+        for (int d = 4; d < 32; d <<= 1) s += __shfl_xor_sync(0xffffffff, s, d);
+        if (g == 0) {
+          stat_s[warp][n * 8 + 2 * t + k][0] = m[n][k];
+          stat_s[warp][n * 8 + 2 * t + k][1] = M[n][k];
+          stat_s[warp][n * 8 + 2 * t + k][2] = s;
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i) {
+          const int row = n * 8 + 2 * t + k, ch = g * (D / 8) + 2 * i;
+          *reinterpret_cast<float2*>(merge + (warp * R + row) * D + ch) = make_float2(o[n][i][k], o[n][i][2 + k]);
+        }
+      }
+    __syncthreads();
+    const bool whole = n_units == units;
+    const long long slot = 2LL * blockIdx.x + (u == u_begin ? 0 : 1);
+    for (int idx = tid; idx < R * D / 2; idx += kWarps * 32) {
+      const int row = idx / (D / 2), ch = idx % (D / 2) * 2;
+      const int r = grp * R + row;
+      if (r >= p.S * p.G) continue;
+      float mm = -INFINITY, MM = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < kWarps; ++i) {
+        mm = fmaxf(mm, stat_s[i][row][0]);
+        MM = fmaxf(MM, stat_s[i][row][1]);
+      }
+      const float ms = mm == -INFINITY ? 0.f : mm, Ms = MM == -INFINITY ? 0.f : MM;
+      float2 a = make_float2(0.f, 0.f);
+      float sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < kWarps; ++i) {
+        sum += stat_s[i][row][2] * exp2f(stat_s[i][row][0] - ms);
+        const float f = exp2f(stat_s[i][row][1] - Ms);
+        const float2 v = *reinterpret_cast<const float2*>(merge + (i * R + row) * D + ch);
+        a.x += v.x * f, a.y += v.y * f;
+      }
+      if (whole) {
+        const int i = r / p.G;
+        T* dst = static_cast<T*>(p.out) + (((long long)b * p.S + i) * p.Hq + h * p.G + (r - i * p.G)) * D + ch;
+        // no key seen: zeros. 2^(M - m) is the magnitude of the values, the sum is at least 1
+        const float f = mm == -INFINITY && sum == 0.f ? 0.f : exp2f(Ms - ms) * kStep / sum;
+        dst[0] = from_float<T>(a.x * f);
+        dst[1] = from_float<T>(a.y * f);
+      } else {
+        *reinterpret_cast<float2*>(p.part_o + (slot * R + row) * D + ch) = a;
+        if (ch == 0) {
+          float* st = p.part_s + (slot * R + row) * 3;
+          st[0] = mm, st[1] = MM, st[2] = sum;
+        }
+      }
+    }
+    __syncthreads();
+    u += n_units;
+  }
+}
+
+// Joins the pieces of a segment that several CTAs worked on: one CTA per (segment, query row), one
+// thread per two channels.
+template <typename T, int D, int R>
+__global__ void __launch_bounds__(D / 2) kv8_combine_kernel(const AttendParams p) {
+  __shared__ int sums[2][4];
+  const int tid = threadIdx.x;
+  const int row = blockIdx.x % R, seg = blockIdx.x / R;
+  const int per = p.Hkv * p.groups, b = seg / per, hg = seg - b * per;
+  const int grp = hg % p.groups, h = hg / p.groups, r = grp * R + row;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (r >= p.S * p.G) return;
+  int pre = 0, all = 0;
+  for (int i = tid; i < p.B; i += D / 2) {
+    const int v = row_units(p, i);
+    all += v;
+    pre += i < b ? v : 0;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    all += __shfl_xor_sync(0xffffffff, all, o);
+    pre += __shfl_xor_sync(0xffffffff, pre, o);
+  }
+  if ((tid & 31) == 0) sums[0][tid >> 5] = all, sums[1][tid >> 5] = pre;
+  __syncthreads();
+  all = pre = 0;
+#pragma unroll
+  for (int i = 0; i < D / 64; ++i) all += sums[0][i], pre += sums[1][i];
+  const int units = row_units(p, b);
+  const long long total = (long long)all * per, u0 = (long long)pre * per + (long long)hg * units;
+  const int ctas = live_ctas(p, total);
+  const int c0 = cta_of(u0, total, ctas), c1 = cta_of(u0 + units - 1, total, ctas);
+  if (c0 == c1) return;  // one CTA had it all and wrote the output
+  float mm = -INFINITY, MM = -INFINITY, sum = 0.f;
+  float2 a = make_float2(0.f, 0.f);
+  for (int c = c0; c <= c1; ++c) {
+    // a CTA's piece is its first unless its range began before the segment
+    const long long slot = 2LL * c + (total * c / ctas < u0 ? 1 : 0);
+    const float* st = p.part_s + (slot * R + row) * 3;
+    const float2 v = *reinterpret_cast<const float2*>(p.part_o + (slot * R + row) * D + tid * 2);
+    const float m1 = fmaxf(mm, st[0]), M1 = fmaxf(MM, st[1]);
+    const float ms = m1 == -INFINITY ? 0.f : m1, Ms = M1 == -INFINITY ? 0.f : M1;
+    const float f = exp2f(MM - Ms), e = exp2f(st[1] - Ms);
+    sum = sum * exp2f(mm - ms) + st[2] * exp2f(st[0] - ms);
+    a.x = a.x * f + v.x * e;
+    a.y = a.y * f + v.y * e;
+    mm = m1, MM = M1;
+  }
+  const float ms = mm == -INFINITY ? 0.f : mm, Ms = MM == -INFINITY ? 0.f : MM;
+  const float f = mm == -INFINITY && sum == 0.f ? 0.f : exp2f(Ms - ms) * kStep / sum;
+  const int i = r / p.G;
+  T* dst = static_cast<T*>(p.out) + (((long long)b * p.S + i) * p.Hq + h * p.G + (r - i * p.G)) * D + tid * 2;
+  dst[0] = from_float<T>(a.x * f);
+  dst[1] = from_float<T>(a.y * f);
+}
+
+constexpr int stages_for(int NT) { return NT == 1 ? 3 : 6; }
+template <int D, int NT>
+constexpr int attend_smem() {
+  const int ring = kWarps * stages_for(NT) * (int)sizeof(Stage<D>), merge = kWarps * 8 * NT * D * 4;
+  return ring > merge ? ring : merge;
+}
+
+template <typename T, int D, int NT>
+void launch_attend(const AttendParams& p, bool combine, cudaStream_t s) {
+  constexpr int smem = attend_smem<D, NT>();
+  auto kernel = kv8_attend_kernel<T, D, NT, stages_for(NT)>;
+  static bool set[64] = {};  // the attribute belongs to the device that is current
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev < 0 || dev >= 64 || !set[dev]) {
+    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (dev >= 0 && dev < 64) set[dev] = true;
+  }
+  (note_launch(), kernel<<<p.ctas, kWarps * 32, smem, s>>>(p));
+  if (!combine) return;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(p.B * p.Hkv * p.groups * 8 * NT));
+  cfg.blockDim = dim3(D / 2);
+  cfg.stream = s;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  note_launch();
+  cudaLaunchKernelEx(&cfg, kv8_combine_kernel<T, D, 8 * NT>, p);
+}
+
+}  // namespace
+}  // namespace astrai
+
+namespace astrai_host {
+
+bool kv8_block_supported(int block) { return block == 16 || block == 32 || block == 64 || block == 128; }
+int kv8_max_batch() { return astrai::kMaxBatch; }
+
+void kv8_append(const void* k, const long long* ks, const void* v, const long long* vs, void* kc, void* vc, float* ka,
+                float* va, const int* table, const int* starts, const int* lens, int B, int S, int Hkv, int D,
+                int page_size, int n_pages, int max_pages, int block, int dtype, cudaStream_t s) {
+  using namespace astrai;
+  if (B <= 0 || S <= 0) return;
+  AppendParams p{};
+  p.src[0] = k, p.src[1] = v;
+  p.sb[0] = ks[0], p.st[0] = ks[1], p.sh[0] = ks[2];
+  p.sb[1] = vs[0], p.st[1] = vs[1], p.sh[1] = vs[2];
+  p.cache[0] = static_cast<signed char*>(kc), p.cache[1] = static_cast<signed char*>(vc);
+  p.absmax[0] = ka, p.absmax[1] = va;
+  p.table = table, p.starts = starts, p.lens = lens;
+  p.B = B, p.S = S, p.Hkv = Hkv, p.page_size = page_size, p.n_pages = n_pages, p.max_pages = max_pages;
+  p.windows = (S - 1 + block - 1) / block + 1;  // blocks that S tokens from any offset can touch
+  const long long items = 2LL * B * Hkv * p.windows;
+  const int per_cta = block > 32 ? 4 / (block / 32) : 4;
+  const int blocks = (int)((items + per_cta - 1) / per_cta);
+#define ASTRAI_APPEND(T, D_)                                                                     \
+  switch (block) {                                                                               \
+    case 16: (note_launch(), kv8_append_kernel<T, D_, 16><<<blocks, 128, 0, s>>>(p)); break;     \
+    case 32: (note_launch(), kv8_append_kernel<T, D_, 32><<<blocks, 128, 0, s>>>(p)); break;     \
+    case 64: (note_launch(), kv8_append_kernel<T, D_, 64><<<blocks, 128, 0, s>>>(p)); break;     \
+    default: (note_launch(), kv8_append_kernel<T, D_, 128><<<blocks, 128, 0, s>>>(p)); break;    \
+  }
+  if (dtype == 0 && D == 128) { ASTRAI_APPEND(__nv_bfloat16, 128) }
+  else if (dtype == 0) { ASTRAI_APPEND(__nv_bfloat16, 64) }
+  else if (D == 128) { ASTRAI_APPEND(__half, 128) }
+  else { ASTRAI_APPEND(__half, 64) }
+#undef ASTRAI_APPEND
+}
+
+void kv8_gather(const void* kc, const void* vc, const float* ka, const float* va, const int* table, const int* starts,
+                const int* lens, void* ko, void* vo, int B, int total, int Hkv, int D, int page_size, int n_pages,
+                int max_pages, int block, int dtype, int device, cudaStream_t s) {
+  using namespace astrai;
+  GatherParams p{};
+  p.cache[0] = static_cast<const signed char*>(kc), p.cache[1] = static_cast<const signed char*>(vc);
+  p.absmax[0] = ka, p.absmax[1] = va, p.table = table, p.starts = starts, p.lens = lens;
+  p.out[0] = ko, p.out[1] = vo;
+  p.B = B, p.total = total, p.Hkv = Hkv, p.page_size = page_size, p.n_pages = n_pages, p.max_pages = max_pages;
+  p.block = block;
+  const long long n = (long long)B * total * Hkv * (D / 16);
+  if (n <= 0) return;
+  const int blocks = (int)std::min<long long>((n + 255) / 256, num_sms(device) * 32LL);
+  if (dtype == 0 && D == 128) (note_launch(), kv8_gather_kernel<__nv_bfloat16, 128><<<blocks, 256, 0, s>>>(p));
+  else if (dtype == 0) (note_launch(), kv8_gather_kernel<__nv_bfloat16, 64><<<blocks, 256, 0, s>>>(p));
+  else if (D == 128) (note_launch(), kv8_gather_kernel<__half, 128><<<blocks, 256, 0, s>>>(p));
+  else (note_launch(), kv8_gather_kernel<__half, 64><<<blocks, 256, 0, s>>>(p));
+}
+
+// Launch shape of an attention call, from sizes the host knows (not the lengths, which are on the
+// device): out[0] CTAs, out[1] query rows per group (R), out[2] groups, out[3] 1 if a segment can be
+// split over CTAs, out[4] workspace floats.
+void kv8_attend_plan(int B, int S, int Hq, int Hkv, int D, int page_size, int max_pages, int device, long long* out) {
+  using namespace astrai;
+  const int rows = S * (Hq / Hkv), R = rows <= 8 ? 8 : 16, groups = (rows + R - 1) / R;
+  const long long units = std::max<long long>(1, ((long long)max_pages * page_size + kUnit - 1) / kUnit);
+  const long long most = (long long)B * Hkv * groups * units;
+  const int ctas = (int)std::min<long long>(most, (long long)num_sms(device) * (R == 8 ? 2 : 1));
+  out[0] = ctas, out[1] = R, out[2] = groups, out[3] = units > 1;
+  out[4] = units > 1 ? 2LL * ctas * R * (D + 3) : 0;
+}
+
+void kv8_attend(const void* q, const long long* qs, const void* kc, const void* vc, const float* ka, const float* va,
+                const int* table, const int* lens, const int* starts, void* out, float* workspace, int B, int S,
+                int Hq, int Hkv, int D, int page_size, int n_pages, int max_pages, int block, float scale, int dtype,
+                int device, cudaStream_t s) {
+  using namespace astrai;
+  if (B <= 0 || S <= 0) return;
+  long long plan[5];
+  kv8_attend_plan(B, S, Hq, Hkv, D, page_size, max_pages, device, plan);
+  AttendParams p{};
+  p.q = q, p.qb = qs[0], p.qs = qs[1], p.qh = qs[2];
+  p.kc = static_cast<const signed char*>(kc), p.vc = static_cast<const signed char*>(vc), p.ka = ka, p.va = va;
+  p.table = table, p.lens = lens, p.starts = starts, p.out = out;
+  p.B = B, p.S = S, p.Hq = Hq, p.Hkv = Hkv, p.G = Hq / Hkv, p.groups = (int)plan[2];
+  p.page_size = page_size, p.n_pages = n_pages, p.max_pages = max_pages, p.block = block;
+  p.ctas = (int)plan[0], p.scale = scale * 1.4426950408889634f * kStep;
+  p.part_o = workspace;
+  p.part_s = workspace ? workspace + 2LL * p.ctas * plan[1] * D : nullptr;
+  const bool wide = plan[1] == 16, combine = plan[3] != 0;
+#define ASTRAI_ATTEND(T, D_) \
+  if (wide) launch_attend<T, D_, 2>(p, combine, s); \
+  else launch_attend<T, D_, 1>(p, combine, s);
+  if (dtype == 0 && D == 128) { ASTRAI_ATTEND(__nv_bfloat16, 128) }
+  else if (dtype == 0) { ASTRAI_ATTEND(__nv_bfloat16, 64) }
+  else if (D == 128) { ASTRAI_ATTEND(__half, 128) }
+  else { ASTRAI_ATTEND(__half, 64) }
+#undef ASTRAI_ATTEND
+}
+
+}  // namespace astrai_host
