@@ -201,7 +201,9 @@ struct AttendParams {
   void* out;          // [B, S, Hq, D] contiguous
   float* part_o;      // [2 * ctas][R][D]
   float* part_s;      // [2 * ctas][R][3]: running max of scores, of weights, sum
-  int B, S, Hq, Hkv, G, groups, page_size, n_pages, max_pages, block, ctas;
+  int B, S, Hq, Hkv, G, groups, page_size, n_pages, max_pages, ctas;
+  int tiles_per_page, page_step, tile_step;  // kWarps tiles on: so many pages and tiles further
+  int blocks_per_page, block_shift;          // magnitudes per page and head; log2(block / kTile)
   float scale;        // softmax scale * log2(e) / 127
 };
 
@@ -209,19 +211,46 @@ constexpr int kWarps = 8;
 constexpr int kTile = 16;                // tokens per warp step
 constexpr int kUnit = kWarps * kTile;    // tokens per unit of work
 constexpr int kMaxBatch = 2048;
+// Running maxima start here: below every score, and finite, so that no difference of maxima is NaN.
+constexpr float kNone = -1.7e38f;
+// A running maximum follows the scores only when they pass it by this much (powers of two): weights then
+// reach 2^8, far inside fp16, and most tiles need no reduction over lanes and no rescaling.
+constexpr float kSlack = 8.f;
 
-__device__ __forceinline__ void cp_async16(void* dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((unsigned)__cvta_generic_to_shared(dst)), "l"(src)
-               : "memory");
+__device__ __forceinline__ void cp_async16(unsigned dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
 }
-__device__ __forceinline__ void cp_async4(void* dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((unsigned)__cvta_generic_to_shared(dst)), "l"(src)
-               : "memory");
+__device__ __forceinline__ void cp_async4(unsigned dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void cp_async_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ uint4 lds128(unsigned a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
+}
+__device__ __forceinline__ float2 lds_float2(unsigned a) {
+  float2 v;
+  asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
+  return v;
+}
+// four 8 x 8 matrices of 16-bit elements, each transposed
+__device__ __forceinline__ uint4 ldmatrix4_trans(unsigned a) {
+  uint4 v;
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(a)
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 __device__ __forceinline__ void mma16816(float* d, const unsigned* a, const unsigned* b) {
   asm volatile(
@@ -234,9 +263,14 @@ __device__ __forceinline__ unsigned transpose8x8(unsigned v) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
-// Integers to fp16 pairs: a byte u = q + 128 under the high byte 0x64 is the fp16 number 1024 + u, and
-// taking 1152 away is exact. `sel` picks the two bytes of `u` that make the pair.
-__device__ __forceinline__ unsigned ints_to_half2(unsigned u, unsigned sel) {
+// Integers to fp16 pairs. With u = q + 128 a byte:
+//  * under a zero high byte u is the subnormal fp16 number u 2^-24. Sums over the channels then carry
+//    128 sum(query), no larger than the sums themselves, which is taken off afterwards (keys);
+//  * under the high byte 0x64 it is 1024 + u, and taking 1152 away is exact (values: the weights of a long
+//    context all have one sign, so an offset would grow far past the result).
+// `sel` picks the two bytes of `u` that make the pair.
+__device__ __forceinline__ unsigned bytes_to_subnormal2(unsigned u, unsigned sel) { return __byte_perm(u, 0u, sel); }
+__device__ __forceinline__ unsigned bytes_to_half2(unsigned u, unsigned sel) {
   const unsigned m = __byte_perm(u, 0x64646464u, sel);
   const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&m), __float2half2_rn(1152.f));
   return *reinterpret_cast<const unsigned*>(&r);
@@ -263,17 +297,12 @@ __device__ __forceinline__ int cta_of(long long u, long long total, int ctas) {
   return (int)(((u + 1) * ctas - 1) / total);
 }
 
+// A [16][D] tile of bytes in shared memory: the 16-byte chunks of a token are permuted so that the reads
+// below (8 tokens, one chunk each, or 2 tokens, 4 chunks each) touch all banks once.
 template <int D>
-__device__ __forceinline__ int swizzle(int row, int chunk) {  // byte offset in a [16][D] tile
+__device__ __forceinline__ int swizzle(int row, int chunk) {
   return D == 128 ? row * 128 + ((chunk ^ (row & 7)) << 4) : row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4);
 }
-
-template <int D>
-struct alignas(16) Stage {
-  unsigned char k[kTile * D];
-  unsigned char v[kTile * D];
-  float ka, va, pad[2];
-};
 
 // Work: every (row b, kv head h, group g of R query rows) is a segment of ceil(keys / 128) units; the
 // units of all segments, in order, are dealt out evenly over the CTAs, whatever the rows' lengths. A
@@ -281,24 +310,26 @@ struct alignas(16) Stage {
 // softmax, and are merged once per piece. A piece that is a whole segment writes the output; others
 // leave partials (at most two per CTA: its first and its last piece) for kv8_combine_kernel.
 //
-// Softmax per query row: m = max of the scores s and l = sum 2^(s - m) as usual. The weights of the
-// integers v are 2^s * absmax_v; they are kept relative to their own running maximum M = max(s +
-// log2 absmax_v), so as fp16 they are at most 1 and lose nothing whatever the magnitudes of the blocks.
-// out = sum w v / l * 2^(M - m) / 127.
+// Softmax per query row: a reference m near the maximum of the scores s (within kSlack) and
+// l = sum 2^(s - m). The weights of the integers v are 2^s * absmax_v; they have a reference M of their
+// own near the maximum of s + log2 absmax_v, so as fp16 they keep their precision whatever the
+// magnitudes of the blocks. out = sum w v / l * 2^(M - m) / 127.
 template <typename T, int D, int NT, int STAGES>
 __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv8_attend_kernel(const AttendParams p) {
   constexpr int KS = D / 16;     // k-steps of S^T = K Q^T
   constexpr int MT = D / 16;     // channel tiles of O^T = V^T P^T
   constexpr int R = 8 * NT;      // query rows of a group
-  constexpr int CH = D / 16;     // 16-byte chunks per token
+  constexpr int TB = kTile * D;  // bytes of a tile
   extern __shared__ __align__(128) unsigned char smem[];
-  Stage<D>* ring = reinterpret_cast<Stage<D>*>(smem) + (threadIdx.x >> 5) * STAGES;
   __shared__ int prefix[kMaxBatch + 1];
   __shared__ int scan_s[kWarps];
   __shared__ float stat_s[kWarps][R][3];
+  __shared__ float2 mag_s[kWarps][STAGES];  // magnitudes of k and v of the tiles in the ring
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the combine waits for this grid itself
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+  const unsigned ring = (unsigned)__cvta_generic_to_shared(smem) + warp * STAGES * 2 * TB;
+  const unsigned mags = (unsigned)__cvta_generic_to_shared(&mag_s[warp][0]);
 
   // units of the rows before each row
   int before = 0;
@@ -331,6 +362,12 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv8_attend_kerne
   if ((int)blockIdx.x >= ctas) return;
   const long long u_begin = total * blockIdx.x / ctas, u_end = total * (blockIdx.x + 1) / ctas;
 
+  // this lane's places in a tile: 16 bytes copied per step of 32 chunks; keys: token g, channels
+  // t * D / 4 ..; values: token lane & 15 of the matrices of chunks lane >> 4, ..
+  const unsigned put0 = swizzle<D>(lane / (D / 16), lane % (D / 16));
+  const unsigned put1 = swizzle<D>(lane / (D / 16) + 512 / D, lane % (D / 16));
+  const unsigned key_at = swizzle<D>(g, t * (D / 64)), value_at = TB + swizzle<D>(lane & 15, lane >> 4);
+
   for (long long u = u_begin; u < u_end;) {
     int lo = 0, hi = p.B - 1;  // the row of unit u: last b with prefix[b] * per <= u
     while (lo < hi) {
@@ -346,11 +383,53 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv8_attend_kerne
     int first, keys;
     row_extent(p, b, first, keys);
 
+    // tiles of this warp: first0, first0 + 8, ... below tile_end. The copies run STAGES - 1 tiles ahead,
+    // the page lookups one tile further.
+    const int tile_end = min((unit0 + n_units) * kWarps, (keys + kTile - 1) / kTile);
+    const int first0 = unit0 * kWarps + warp;
+    const int count = first0 < tile_end ? (tile_end - first0 + kWarps - 1) / kWarps : 0;
+    const int* trow = p.table + (long long)b * p.max_pages;
+    int ahead = 0;                                                    // tiles looked up
+    int lp = first0 / p.tiles_per_page, tip = first0 - lp * p.tiles_per_page;  // their next page and tile in it
+    int next_page = -1, next_tip = 0;
+    auto look_up = [&]() {
+      next_page = ahead < count ? trow[lp] : -1;
+      if (next_page >= p.n_pages) next_page = -1;
+      next_tip = tip;
+      lp += p.page_step;
+      tip += p.tile_step;
+      if (tip >= p.tiles_per_page) tip -= p.tiles_per_page, ++lp;
+      ++ahead;
+    };
+    unsigned have = 0;  // bit i: the i-th tile from the current one has a page
+    auto issue = [&](int stage, unsigned bit) {
+      if (next_page >= 0) {
+        have |= bit;
+        const long long head = (long long)next_page * p.Hkv + h;
+        const long long at = (head * p.page_size + next_tip * kTile) * D + lane * 16;
+        const unsigned dst = ring + stage * 2 * TB;
+#pragma unroll
+        for (int j = 0; j < TB / 512; ++j) {
+          const unsigned to = dst + (j & 1 ? put1 : put0) + (j >> 1) * 1024;
+          cp_async16(to, p.kc + at + j * 512);
+          cp_async16(to + TB, p.vc + at + j * 512);
+        }
+        const long long blk = head * p.blocks_per_page + (next_tip >> p.block_shift);
+        if (lane < 2) cp_async4(mags + stage * 8 + lane * 4, (lane ? p.va : p.ka) + blk);
+      }
+      cp_async_commit();
+      look_up();
+    };
+    look_up();
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) issue(i, 1u << i);
+
     // query fragments: lane (g, t) holds channels t * D / 4 .. of query row g of each 8-row tile, as
-    // fp16 scaled by a power of two that brings the row's largest magnitude to [1, 2)
+    // fp16 scaled by a power of two that brings the row's largest magnitude to [2^14, 2^15)
     unsigned qf[NT][KS][2];
-    float qscale[NT][2];  // of the columns 2t, 2t + 1 of S^T
-    int vis[NT][2];       // keys that those columns see
+    float qscale[NT][2], qbias[NT][2];  // of the columns 2t, 2t + 1 of S^T
+    int vis[NT][2];                     // keys that those columns see
+    int seen_by_all = keys;
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const int r = grp * R + n * 8 + g, i = r / p.G;
@@ -368,8 +447,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv8_attend_kerne
       most = fmaxf(most, __shfl_xor_sync(0xffffffff, most, 1));
       most = fmaxf(most, __shfl_xor_sync(0xffffffff, most, 2));
       int ex = 0;
-      if (most > 0.f && most < INFINITY) ex = max(ilogbf(most), -120);
-      const float down = ldexpf(1.f, -ex), up = ldexpf(p.scale, ex);
+      if (most > 0.f && most < INFINITY) ex = max(ilogbf(most), -110);
+      const float down = ldexpf(1.f, 14 - ex), up = ldexpf(p.scale, ex - 14);
+      float sum = 0.f;
 #pragma unroll
       for (int s = 0; s < KS; ++s)
 #pragma unroll
@@ -377,66 +457,48 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv8_attend_kerne
           const __half2 v = __floats2half2_rn(bits_to_float<T>(e[4 * s + 2 * k]) * down,
                                               bits_to_float<T>(e[4 * s + 2 * k + 1]) * down);
           qf[n][s][k] = *reinterpret_cast<const unsigned*>(&v);
+          sum += __low2float(v) + __high2float(v);
         }
+      sum += __shfl_xor_sync(0xffffffff, sum, 1);
+      sum += __shfl_xor_sync(0xffffffff, sum, 2);
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         qscale[n][k] = __shfl_sync(0xffffffff, up, (2 * t + k) * 4);
+        qbias[n][k] = -128.f * qscale[n][k] * __shfl_sync(0xffffffff, sum, (2 * t + k) * 4);
+        qscale[n][k] *= 0x1p24f;
         const int rc = grp * R + n * 8 + 2 * t + k, ic = rc / p.G;
-        vis[n][k] = rc < p.S * p.G && first + ic >= 0 && first + ic < p.lens[b] ? min(first + ic + 1, keys) : 0;
+        // columns behind the last query row are computed like the others and never written
+        vis[n][k] = rc >= p.S * p.G ? keys
+                    : first + ic >= 0 && first + ic < p.lens[b] ? min(first + ic + 1, keys) : 0;
+        seen_by_all = min(seen_by_all, vis[n][k]);
       }
     }
+#pragma unroll
+    for (int d = 1; d < 4; d <<= 1) seen_by_all = min(seen_by_all, __shfl_xor_sync(0xffffffff, seen_by_all, d));
 
     float o[NT][MT][4], m[NT][2], M[NT][2], l[NT][2];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
 #pragma unroll
-      for (int k = 0; k < 2; ++k) m[n][k] = M[n][k] = -INFINITY, l[n][k] = 0.f;
+      for (int k = 0; k < 2; ++k) m[n][k] = M[n][k] = kNone, l[n][k] = 0.f;
 #pragma unroll
       for (int i = 0; i < MT; ++i)
 #pragma unroll
         for (int k = 0; k < 4; ++k) o[n][i][k] = 0.f;
     }
 
-    // tiles of this warp: first0, first0 + 8, ... below tile_end
-    const int tile_end = min((unit0 + n_units) * kWarps, (keys + kTile - 1) / kTile);
-    const int first0 = unit0 * kWarps + warp;
-    const int count = first0 < tile_end ? (tile_end - first0 + kWarps - 1) / kWarps : 0;
-    const int* trow = p.table + (long long)b * p.max_pages;
-    const int tpp = p.page_size / kTile;  // tiles per page
-    auto page_of = [&](int i) { return i < count ? trow[(first0 + i * kWarps) / tpp] : -1; };
-    auto issue = [&](int i, int page) {
-      if (i < count && page >= 0 && page < p.n_pages) {
-        const int tile = first0 + i * kWarps;
-        const long long row = ((long long)page * p.Hkv + h) * p.page_size + (tile % tpp) * kTile;
-        Stage<D>& st = ring[i % STAGES];
-#pragma unroll
-        for (int j = 0; j < kTile * CH / 32; ++j) {
-          const int c = lane + j * 32, dst = swizzle<D>(c / CH, c % CH);
-          cp_async16(st.k + dst, p.kc + row * D + c * 16);
-          cp_async16(st.v + dst, p.vc + row * D + c * 16);
-        }
-        if (lane == 0) cp_async4(&st.ka, p.ka + row / p.block);
-        if (lane == 1) cp_async4(&st.va, p.va + row / p.block);
-      }
-      cp_async_commit();
-    };
-    int pages[STAGES];  // of the tiles in flight and of the next one to issue
-#pragma unroll
-    for (int i = 0; i < STAGES; ++i) pages[i] = page_of(i);
-#pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) issue(i, pages[i]);
-
-    for (int it = 0; it < count; ++it) {
+    int stage = 0, refill = STAGES - 1, tok = first0 * kTile;
+    for (int it = 0; it < count; ++it, tok += kUnit) {
       cp_async_wait<STAGES - 2>();
       __syncwarp();  // this tile has landed for all lanes, and all have left the stage that is refilled now
-      const int page = pages[0];
-#pragma unroll
-      for (int i = 0; i + 1 < STAGES; ++i) pages[i] = pages[i + 1];
-      issue(it + STAGES - 1, pages[STAGES - 2]);
-      pages[STAGES - 1] = page_of(it + STAGES);
-      if (page < 0 || page >= p.n_pages) continue;  // the same for the whole warp
-      const Stage<D>& st = ring[it % STAGES];
-      const int tok = (first0 + it * kWarps) * kTile;
+      const bool held = have & 1u;
+      have >>= 1;
+      issue(refill, 1u << (STAGES - 2));
+      refill = refill + 1 == STAGES ? 0 : refill + 1;
+      const unsigned tile = ring + stage * 2 * TB;
+      const float2 mag = lds_float2(mags + stage * 8);
+      stage = stage + 1 == STAGES ? 0 : stage + 1;
+      if (!held) continue;  // the same for the whole warp
 
       // S^T: tokens g and g + 8, channels t * D / 4 + 4s .. of k-step s on both sides
       float sc[NT][4];
@@ -444,75 +506,91 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv8_attend_kerne
       for (int n = 0; n < NT; ++n) sc[n][0] = sc[n][1] = sc[n][2] = sc[n][3] = 0.f;
 #pragma unroll
       for (int j = 0; j < D / 64; ++j) {
-        const uint4 x = *reinterpret_cast<const uint4*>(st.k + swizzle<D>(g, t * (D / 64) + j));
-        const uint4 y = *reinterpret_cast<const uint4*>(st.k + swizzle<D>(g + 8, t * (D / 64) + j));
+        const uint4 x = lds128(tile + (key_at ^ (j << 4))), y = lds128(tile + (key_at ^ (j << 4)) + 8 * D);
         const unsigned xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const unsigned ux = xs[k] ^ 0x80808080u, uy = ys[k] ^ 0x80808080u;
-          const unsigned a[4] = {ints_to_half2(ux, 0x4140), ints_to_half2(uy, 0x4140), ints_to_half2(ux, 0x4342),
-                                 ints_to_half2(uy, 0x4342)};
+          const unsigned a[4] = {bytes_to_subnormal2(ux, 0x4140), bytes_to_subnormal2(uy, 0x4140),
+                                 bytes_to_subnormal2(ux, 0x4342), bytes_to_subnormal2(uy, 0x4342)};
 #pragma unroll
           for (int n = 0; n < NT; ++n) mma16816(sc[n], a, qf[n][j * 4 + k]);
         }
       }
 
-      const float ka = st.ka, lv = __log2f(st.va);
+      const float lv = __log2f(mag.y);
+      bool rises = false;
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const float a = qscale[n][k] * mag.x, c = qbias[n][k] * mag.x;
+          sc[n][k] = fmaf(sc[n][k], a, c);
+          sc[n][2 + k] = fmaf(sc[n][2 + k], a, c);
+        }
+        if (tok + kTile > seen_by_all) {
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            if (tok + g >= vis[n][k]) sc[n][k] = -INFINITY;
+            if (tok + g + 8 >= vis[n][k]) sc[n][2 + k] = -INFINITY;
+          }
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const float top = fmaxf(sc[n][k], sc[n][2 + k]);
+          rises = rises || top > m[n][k] + kSlack || top + lv > M[n][k] + kSlack;
+        }
+      }
+      if (__any_sync(0xffffffff, rises)) {
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          float fall[2];
+#pragma unroll
+          for (int k = 0; k < 2; ++k) {
+            float top = fmaxf(sc[n][k], sc[n][2 + k]);
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffff, top, d));
+            const float m1 = fmaxf(m[n][k], top), M1 = fmaxf(M[n][k], top + lv);
+            l[n][k] *= ex2(m[n][k] - m1);
+            fall[k] = ex2(M[n][k] - M1);
+            m[n][k] = m1;
+            M[n][k] = M1;
+          }
+#pragma unroll
+          for (int i = 0; i < MT; ++i) {
+            o[n][i][0] *= fall[0], o[n][i][1] *= fall[1];
+            o[n][i][2] *= fall[0], o[n][i][3] *= fall[1];
+          }
+        }
+      }
       unsigned pf[NT][2];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        float w[4], corr[2], corrw[2];
+        float w[4];
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const float qs = qscale[n][k] * ka;
-          const float s0 = tok + g < vis[n][k] ? sc[n][k] * qs : -INFINITY;
-          const float s1 = tok + g + 8 < vis[n][k] ? sc[n][2 + k] * qs : -INFINITY;
-          float top = fmaxf(s0, s1);
-#pragma unroll
-          for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffff, top, d));
-          const float m1 = fmaxf(m[n][k], top), M1 = fmaxf(M[n][k], top + lv);
-          const float ms = m1 == -INFINITY ? 0.f : m1, Ms = M1 == -INFINITY ? 0.f : M1;
-          corr[k] = exp2f(m[n][k] - ms);
-          corrw[k] = exp2f(M[n][k] - Ms);
-          l[n][k] = l[n][k] * corr[k] + (exp2f(s0 - ms) + exp2f(s1 - ms));
-          w[k] = s0 == -INFINITY ? 0.f : exp2f(s0 + lv - Ms);
-          w[2 + k] = s1 == -INFINITY ? 0.f : exp2f(s1 + lv - Ms);
-          m[n][k] = m1;
-          M[n][k] = M1;
-        }
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          o[n][i][0] *= corrw[0], o[n][i][1] *= corrw[1];
-          o[n][i][2] *= corrw[0], o[n][i][3] *= corrw[1];
+          l[n][k] += ex2(sc[n][k] - m[n][k]) + ex2(sc[n][2 + k] - m[n][k]);
+          const float to = lv - M[n][k];
+          // a hidden key has weight 0 whatever its block's magnitude is
+          w[k] = sc[n][k] == -INFINITY ? 0.f : ex2(sc[n][k] + to);
+          w[2 + k] = sc[n][2 + k] == -INFINITY ? 0.f : ex2(sc[n][2 + k] + to);
         }
         const __half2 w0 = __floats2half2_rn(w[0], w[1]), w1 = __floats2half2_rn(w[2], w[3]);
         pf[n][0] = transpose8x8(*reinterpret_cast<const unsigned*>(&w0));
         pf[n][1] = transpose8x8(*reinterpret_cast<const unsigned*>(&w1));
       }
 
-      // O^T: lane (g, t) has channels g * D / 8 .. of tokens 2t, 2t + 1, 2t + 8, 2t + 9; channel tile 2j + e
-      // takes channels 4j + 2e (its row g) and 4j + 2e + 1 (row g + 8) of each lane's run
-      unsigned vw[4][D / 32];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const int row = 2 * t + (k & 1) + (k >> 1) * 8;
-        if constexpr (D == 128) {
-          const uint4 x = *reinterpret_cast<const uint4*>(st.v + swizzle<D>(row, g));
-          vw[k][0] = x.x ^ 0x80808080u, vw[k][1] = x.y ^ 0x80808080u;
-          vw[k][2] = x.z ^ 0x80808080u, vw[k][3] = x.w ^ 0x80808080u;
-        } else {
-          const uint2 x = *reinterpret_cast<const uint2*>(st.v + swizzle<D>(row, g >> 1) + (g & 1) * 8);
-          vw[k][0] = x.x ^ 0x80808080u, vw[k][1] = x.y ^ 0x80808080u;
-        }
-      }
+      // O^T: a transposed matrix of 8 tokens and 16 channels, read as 16-bit pairs of channels, gives lane
+      // (g, t) channels 2g and 2g + 1 of tokens 2t and 2t + 1; channel tile i has channel 16 i + 2g in its row
+      // g and channel 16 i + 2g + 1 in row g + 8
 #pragma unroll
       for (int j = 0; j < D / 32; ++j) {
+        const uint4 x = ldmatrix4_trans(tile + (value_at ^ (j << 5)));
+        const unsigned xs[4] = {x.x ^ 0x80808080u, x.y ^ 0x80808080u, x.z ^ 0x80808080u, x.w ^ 0x80808080u};
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const unsigned x = __byte_perm(vw[0][j], vw[1][j], e ? 0x7362 : 0x5140);
-          const unsigned y = __byte_perm(vw[2][j], vw[3][j], e ? 0x7362 : 0x5140);
-          const unsigned a[4] = {ints_to_half2(x, 0x4140), ints_to_half2(x, 0x4342), ints_to_half2(y, 0x4140),
-                                 ints_to_half2(y, 0x4342)};
+          const unsigned a[4] = {bytes_to_half2(xs[2 * e], 0x4240), bytes_to_half2(xs[2 * e], 0x4341),
+                                 bytes_to_half2(xs[2 * e + 1], 0x4240), bytes_to_half2(xs[2 * e + 1], 0x4341)};
 #pragma unroll
           for (int n = 0; n < NT; ++n) mma16816(o[n][j * 2 + e], a, pf[n]);
         }
@@ -537,7 +615,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv8_attend_kerne
         }
 #pragma unroll
         for (int i = 0; i < MT; ++i) {
-          const int row = n * 8 + 2 * t + k, ch = g * (D / 8) + 2 * i;
+          const int row = n * 8 + 2 * t + k, ch = 16 * i + 2 * g;
           *reinterpret_cast<float2*>(merge + (warp * R + row) * D + ch) = make_float2(o[n][i][k], o[n][i][2 + k]);
         }
       }
@@ -548,27 +626,25 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv8_attend_kerne
       const int row = idx / (D / 2), ch = idx % (D / 2) * 2;
       const int r = grp * R + row;
       if (r >= p.S * p.G) continue;
-      float mm = -INFINITY, MM = -INFINITY;
+      float mm = kNone, MM = kNone;
 #pragma unroll
       for (int i = 0; i < kWarps; ++i) {
         mm = fmaxf(mm, stat_s[i][row][0]);
         MM = fmaxf(MM, stat_s[i][row][1]);
       }
-      const float ms = mm == -INFINITY ? 0.f : mm, Ms = MM == -INFINITY ? 0.f : MM;
       float2 a = make_float2(0.f, 0.f);
       float sum = 0.f;
 #pragma unroll
       for (int i = 0; i < kWarps; ++i) {
-        sum += stat_s[i][row][2] * exp2f(stat_s[i][row][0] - ms);
-        const float f = exp2f(stat_s[i][row][1] - Ms);
+        sum += stat_s[i][row][2] * ex2(stat_s[i][row][0] - mm);
+        const float f = ex2(stat_s[i][row][1] - MM);
         const float2 v = *reinterpret_cast<const float2*>(merge + (i * R + row) * D + ch);
         a.x += v.x * f, a.y += v.y * f;
       }
       if (whole) {
         const int i = r / p.G;
         T* dst = static_cast<T*>(p.out) + (((long long)b * p.S + i) * p.Hq + h * p.G + (r - i * p.G)) * D + ch;
-        // no key seen: zeros. 2^(M - m) is the magnitude of the values, the sum is at least 1
-        const float f = mm == -INFINITY && sum == 0.f ? 0.f : exp2f(Ms - ms) * kStep / sum;
+        const float f = sum == 0.f ? 0.f : exp2f(MM - mm) * kStep / sum;  // no key seen: zeros
         dst[0] = from_float<T>(a.x * f);
         dst[1] = from_float<T>(a.y * f);
       } else {
@@ -584,19 +660,19 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv8_attend_kerne
   }
 }
 
-// Joins the pieces of a segment that several CTAs worked on: one CTA per (segment, query row), one
-// thread per two channels.
+// Joins the pieces of a segment that several CTAs worked on: one CTA per (segment, query row). Four
+// warps take the pieces in turn, a lane D / 32 channels, and are merged at the end.
 template <typename T, int D, int R>
-__global__ void __launch_bounds__(D / 2) kv8_combine_kernel(const AttendParams p) {
+__global__ void __launch_bounds__(128) kv8_combine_kernel(const AttendParams p, int rows) {
+  constexpr int C = D / 32;
   __shared__ int sums[2][4];
-  const int tid = threadIdx.x;
-  const int row = blockIdx.x % R, seg = blockIdx.x / R;
+  __shared__ float stat_s[4][3], o_s[4][D];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int seg = blockIdx.x / rows, row = blockIdx.x - seg * rows;
   const int per = p.Hkv * p.groups, b = seg / per, hg = seg - b * per;
-  const int grp = hg % p.groups, h = hg / p.groups, r = grp * R + row;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  if (r >= p.S * p.G) return;
+  const int h = hg / p.groups, grp = hg - h * p.groups, r = grp * R + row;
   int pre = 0, all = 0;
-  for (int i = tid; i < p.B; i += D / 2) {
+  for (int i = tid; i < p.B; i += 128) {
     const int v = row_units(p, i);
     all += v;
     pre += i < b ? v : 0;
@@ -606,43 +682,57 @@ __global__ void __launch_bounds__(D / 2) kv8_combine_kernel(const AttendParams p
     all += __shfl_xor_sync(0xffffffff, all, o);
     pre += __shfl_xor_sync(0xffffffff, pre, o);
   }
-  if ((tid & 31) == 0) sums[0][tid >> 5] = all, sums[1][tid >> 5] = pre;
+  if (lane == 0) sums[0][warp] = all, sums[1][warp] = pre;
   __syncthreads();
-  all = pre = 0;
-#pragma unroll
-  for (int i = 0; i < D / 64; ++i) all += sums[0][i], pre += sums[1][i];
+  all = sums[0][0] + sums[0][1] + sums[0][2] + sums[0][3];
+  pre = sums[1][0] + sums[1][1] + sums[1][2] + sums[1][3];
   const int units = row_units(p, b);
   const long long total = (long long)all * per, u0 = (long long)pre * per + (long long)hg * units;
   const int ctas = live_ctas(p, total);
   const int c0 = cta_of(u0, total, ctas), c1 = cta_of(u0 + units - 1, total, ctas);
-  if (c0 == c1) return;  // one CTA had it all and wrote the output
-  float mm = -INFINITY, MM = -INFINITY, sum = 0.f;
-  float2 a = make_float2(0.f, 0.f);
-  for (int c = c0; c <= c1; ++c) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // up to here only inputs of the grid before were read
+  if (c0 == c1 || r >= p.S * p.G) return;  // one CTA had it all and wrote the output
+  float m = kNone, M = kNone, sum = 0.f, a[C];
+#pragma unroll
+  for (int i = 0; i < C; ++i) a[i] = 0.f;
+#pragma unroll 4
+  for (int c = c0 + warp; c <= c1; c += 4) {
     // a CTA's piece is its first unless its range began before the segment
-    const long long slot = 2LL * c + (total * c / ctas < u0 ? 1 : 0);
+    const long long slot = 2LL * c + (c == c0 && total * c / ctas < u0 ? 1 : 0);
     const float* st = p.part_s + (slot * R + row) * 3;
-    const float2 v = *reinterpret_cast<const float2*>(p.part_o + (slot * R + row) * D + tid * 2);
-    const float m1 = fmaxf(mm, st[0]), M1 = fmaxf(MM, st[1]);
-    const float ms = m1 == -INFINITY ? 0.f : m1, Ms = M1 == -INFINITY ? 0.f : M1;
-    const float f = exp2f(MM - Ms), e = exp2f(st[1] - Ms);
-    sum = sum * exp2f(mm - ms) + st[2] * exp2f(st[0] - ms);
-    a.x = a.x * f + v.x * e;
-    a.y = a.y * f + v.y * e;
-    mm = m1, MM = M1;
+    const float* src = p.part_o + (slot * R + row) * D + lane * C;
+    float v[C];
+    if constexpr (C == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(src);
+    else *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(src);
+    const float m1 = fmaxf(m, st[0]), M1 = fmaxf(M, st[1]);
+    const float f = ex2(M - M1), e = ex2(st[1] - M1);
+    sum = sum * ex2(m - m1) + st[2] * ex2(st[0] - m1);
+#pragma unroll
+    for (int i = 0; i < C; ++i) a[i] = a[i] * f + v[i] * e;
+    m = m1, M = M1;
   }
-  const float ms = mm == -INFINITY ? 0.f : mm, Ms = MM == -INFINITY ? 0.f : MM;
-  const float f = mm == -INFINITY && sum == 0.f ? 0.f : exp2f(Ms - ms) * kStep / sum;
+  if (lane == 0) stat_s[warp][0] = m, stat_s[warp][1] = M, stat_s[warp][2] = sum;
+#pragma unroll
+  for (int i = 0; i < C; ++i) o_s[warp][lane * C + i] = a[i];
+  __syncthreads();
+  if (tid >= D) return;
+  float mm = kNone, MM = kNone, l = 0.f, o = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) mm = fmaxf(mm, stat_s[i][0]), MM = fmaxf(MM, stat_s[i][1]);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    l += stat_s[i][2] * ex2(stat_s[i][0] - mm);
+    o += o_s[i][tid] * ex2(stat_s[i][1] - MM);
+  }
+  const float f = l == 0.f ? 0.f : exp2f(MM - mm) * kStep / l;
   const int i = r / p.G;
-  T* dst = static_cast<T*>(p.out) + (((long long)b * p.S + i) * p.Hq + h * p.G + (r - i * p.G)) * D + tid * 2;
-  dst[0] = from_float<T>(a.x * f);
-  dst[1] = from_float<T>(a.y * f);
+  static_cast<T*>(p.out)[(((long long)b * p.S + i) * p.Hq + h * p.G + (r - i * p.G)) * D + tid] = from_float<T>(o * f);
 }
 
 constexpr int stages_for(int NT) { return NT == 1 ? 3 : 6; }
 template <int D, int NT>
 constexpr int attend_smem() {
-  const int ring = kWarps * stages_for(NT) * (int)sizeof(Stage<D>), merge = kWarps * 8 * NT * D * 4;
+  const int ring = kWarps * stages_for(NT) * 2 * kTile * D, merge = kWarps * 8 * NT * D * 4;
   return ring > merge ? ring : merge;
 }
 
@@ -660,8 +750,9 @@ void launch_attend(const AttendParams& p, bool combine, cudaStream_t s) {
   (note_launch(), kernel<<<p.ctas, kWarps * 32, smem, s>>>(p));
   if (!combine) return;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(p.B * p.Hkv * p.groups * 8 * NT));
-  cfg.blockDim = dim3(D / 2);
+  const int rows = std::min(8 * NT, p.S * p.G);
+  cfg.gridDim = dim3((unsigned)(p.B * p.Hkv * p.groups * rows));
+  cfg.blockDim = dim3(128);
   cfg.stream = s;
   cudaLaunchAttribute at{};
   at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -669,7 +760,7 @@ void launch_attend(const AttendParams& p, bool combine, cudaStream_t s) {
   cfg.attrs = &at;
   cfg.numAttrs = 1;
   note_launch();
-  cudaLaunchKernelEx(&cfg, kv8_combine_kernel<T, D, 8 * NT>, p);
+  cudaLaunchKernelEx(&cfg, kv8_combine_kernel<T, D, 8 * NT>, p, rows);
 }
 
 }  // namespace
@@ -756,7 +847,11 @@ void kv8_attend(const void* q, const long long* qs, const void* kc, const void* 
   p.kc = static_cast<const signed char*>(kc), p.vc = static_cast<const signed char*>(vc), p.ka = ka, p.va = va;
   p.table = table, p.lens = lens, p.starts = starts, p.out = out;
   p.B = B, p.S = S, p.Hq = Hq, p.Hkv = Hkv, p.G = Hq / Hkv, p.groups = (int)plan[2];
-  p.page_size = page_size, p.n_pages = n_pages, p.max_pages = max_pages, p.block = block;
+  p.page_size = page_size, p.n_pages = n_pages, p.max_pages = max_pages;
+  p.tiles_per_page = page_size / kTile;
+  p.page_step = kWarps / p.tiles_per_page, p.tile_step = kWarps % p.tiles_per_page;
+  p.blocks_per_page = page_size / block;
+  while ((kTile << p.block_shift) < block) ++p.block_shift;
   p.ctas = (int)plan[0], p.scale = scale * 1.4426950408889634f * kStep;
   p.part_o = workspace;
   p.part_s = workspace ? workspace + 2LL * p.ctas * plan[1] * D : nullptr;
