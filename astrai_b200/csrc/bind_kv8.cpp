@@ -147,7 +147,7 @@ int64_t kv8_attend_workspace(int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int6
                   max_pages * page_size < (1LL << 30) && S * (Hq / Hkv) < (1LL << 24),
               "kv8_attend_workspace: sizes");
   if (B == 0 || S == 0) return 0;
-  long long plan[5];
+  long long plan[6];
   astrai_host::kv8_attend_plan((int)B, (int)S, (int)Hq, (int)Hkv, (int)D, (int)page_size, (int)max_pages, (int)device,
                                plan);
   return plan[4];

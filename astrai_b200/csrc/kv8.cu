@@ -202,14 +202,16 @@ struct AttendParams {
   float* part_o;      // [2 * ctas][R][D]
   float* part_s;      // [2 * ctas][R][3]: running max of scores, of weights, sum
   int B, S, Hq, Hkv, G, groups, page_size, n_pages, max_pages, ctas;
-  int tiles_per_page, page_step, tile_step;  // kWarps tiles on: so many pages and tiles further
-  int blocks_per_page, block_shift;          // magnitudes per page and head; log2(block / kTile)
+  int tiles_per_page, blocks_per_page, block_shift;  // magnitudes per page and head; log2(block / kTile)
+  int unit_tiles;     // tiles of a unit of work
   float scale;        // softmax scale * log2(e) / 127
 };
 
 constexpr int kWarps = 8;
 constexpr int kTile = 16;                // tokens per warp step
-constexpr int kUnit = kWarps * kTile;    // tokens per unit of work
+constexpr int kUnit = kWarps * kTile;    // tokens per unit of work: one step of all warps
+constexpr int kPad = 2;                  // units that a segment's start weighs when work is dealt out
+constexpr int kWhole = 4 * kUnit;       // tokens up to which a row is not split
 constexpr int kMaxBatch = 2048;
 // Running maxima start here: below every score, and finite, so that no difference of maxima is NaN.
 constexpr float kNone = -1.7e38f;
@@ -282,13 +284,16 @@ __device__ __forceinline__ void row_extent(const AttendParams& p, int b, int& fi
   first = p.starts ? min(max(p.starts[b], -(1 << 30)), 1 << 30) : len - p.S;
   keys = max(0, min(min(len, first + p.S), p.max_pages * p.page_size));
 }
+// Units of row b in the dealing: those of its keys (a row without keys still has its zeros to write), behind
+// kPad that stand for what starting and merging a piece costs.
 __device__ __forceinline__ int row_units(const AttendParams& p, int b) {
   int first, keys;
   row_extent(p, b, first, keys);
-  return max(1, (keys + kUnit - 1) / kUnit);  // a row without keys still has its zeros to write
+  const int tokens = p.unit_tiles * kTile;
+  return kPad + max(1, (keys + tokens - 1) / tokens);
 }
-// CTAs that take part: each has a unit at least, so that a segment's CTAs are all those from its first
-// unit's to its last unit's
+// CTAs that take part: each has a unit at least, so that the CTAs of a segment's keys are all those from
+// its first unit's to its last unit's
 __device__ __forceinline__ int live_ctas(const AttendParams& p, long long total) {
   return (int)min((long long)p.ctas, total);
 }
@@ -304,31 +309,61 @@ __device__ __forceinline__ int swizzle(int row, int chunk) {
   return D == 128 ? row * 128 + ((chunk ^ (row & 7)) << 4) : row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4);
 }
 
-// Work: every (row b, kv head h, group g of R query rows) is a segment of ceil(keys / 128) units; the
-// units of all segments, in order, are dealt out evenly over the CTAs, whatever the rows' lengths. A
-// CTA's warps take the 16-token tiles of its piece of a segment in turn, each with its own running
-// softmax, and are merged once per piece. A piece that is a whole segment writes the output; others
-// leave partials (at most two per CTA: its first and its last piece) for kv8_combine_kernel.
+// Work: every (row b, kv head h, group g of R query rows) is a segment of ceil(keys / 128) units, and kPad
+// more at its start; the units of all segments, in order, are dealt out evenly over the CTAs, whatever the
+// rows' lengths. A CTA's warps take the 16-token tiles of its piece of a segment in turn, each with its own
+// running softmax, and are merged once per piece. A piece that is a whole segment writes the output; others
+// leave partials (two per CTA at most: one that it begins inside, one that it does not end) for
+// kv8_combine_kernel.
 //
 // Softmax per query row: a reference m near the maximum of the scores s (within kSlack) and
 // l = sum 2^(s - m). The weights of the integers v are 2^s * absmax_v; they have a reference M of their
 // own near the maximum of s + log2 absmax_v, so as fp16 they keep their precision whatever the
 // magnitudes of the blocks. out = sum w v / l * 2^(M - m) / 127.
+template <int C>
+__device__ __forceinline__ void load_floats(const float* src, float* v) {
+  if constexpr (C == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(src);
+  else *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(src);
+}
+// D / 32 channels of query row r of KV head h, scaled
+template <typename T, int D>
+__device__ __forceinline__ void store_out(const AttendParams& p, int b, int h, int r, int ch, const float* a, float by) {
+  const int i = r / p.G;
+  T* dst = static_cast<T*>(p.out) + (((long long)b * p.S + i) * p.Hq + h * p.G + (r - i * p.G)) * D + ch;
+  T v[D / 32];
+#pragma unroll
+  for (int j = 0; j < D / 32; ++j) v[j] = from_float<T>(a[j] * by);
+  if constexpr (D == 128) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(v);
+  else *reinterpret_cast<unsigned*>(dst) = *reinterpret_cast<const unsigned*>(v);
+}
+
+struct Piece {       // of a segment, on one CTA
+  int b, h, grp;     // row, kv head, group
+  int unit0, units;  // its first unit of keys and their number
+  int dealt;         // units taken from the dealing, those that stand for the start among them
+  int first, keys;   // of the row
+  bool whole;
+};
+
 template <typename T, int D, int NT, int STAGES>
 __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv8_attend_kernel(const AttendParams p) {
   constexpr int KS = D / 16;     // k-steps of S^T = K Q^T
   constexpr int MT = D / 16;     // channel tiles of O^T = V^T P^T
   constexpr int R = 8 * NT;      // query rows of a group
   constexpr int TB = kTile * D;  // bytes of a tile
-  extern __shared__ __align__(128) unsigned char smem[];
+  constexpr int SLOT = 2 * TB;   // a ring slot: a tile of keys, then one of values
+  extern __shared__ __align__(128) unsigned char smem[];  // [stage][warp][SLOT]
   __shared__ int prefix[kMaxBatch + 1];
   __shared__ int scan_s[kWarps];
   __shared__ float stat_s[kWarps][R][3];
   __shared__ float2 mag_s[kWarps][STAGES];  // magnitudes of k and v of the tiles in the ring
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the combine waits for this grid itself
+  // This grid may have been scheduled before the one before it ended. The combine may be scheduled from
+  // here on: what it reads before its own wait is then complete.
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const unsigned ring = (unsigned)__cvta_generic_to_shared(smem) + warp * STAGES * 2 * TB;
+  const unsigned ring = (unsigned)__cvta_generic_to_shared(smem) + warp * SLOT;
   const unsigned mags = (unsigned)__cvta_generic_to_shared(&mag_s[warp][0]);
 
   // units of the rows before each row
@@ -368,87 +403,111 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv8_attend_kerne
   const unsigned put1 = swizzle<D>(lane / (D / 16) + 512 / D, lane % (D / 16));
   const unsigned key_at = swizzle<D>(g, t * (D / 64)), value_at = TB + swizzle<D>(lane & 15, lane >> 4);
 
-  for (long long u = u_begin; u < u_end;) {
+  auto find = [&](long long u) {
     int lo = 0, hi = p.B - 1;  // the row of unit u: last b with prefix[b] * per <= u
     while (lo < hi) {
       const int mid = (lo + hi + 1) / 2;
       if ((long long)prefix[mid] * per <= u) lo = mid;
       else hi = mid - 1;
     }
-    const int b = lo, units = prefix[b + 1] - prefix[b];
-    const int rem = (int)(u - (long long)prefix[b] * per);
-    const int hg = rem / units, unit0 = rem - hg * units;
-    const int n_units = (int)min((long long)(units - unit0), u_end - u);
-    const int h = hg / p.groups, grp = hg - h * p.groups;
-    int first, keys;
-    row_extent(p, b, first, keys);
+    Piece c;
+    c.b = lo;
+    const int all = prefix[lo + 1] - prefix[lo];
+    const int rem = (int)(u - (long long)prefix[lo] * per);
+    const int hg = rem / all, at = rem - hg * all;
+    c.dealt = (int)min((long long)(all - at), u_end - u);
+    c.unit0 = max(0, at - kPad);
+    c.units = max(0, at + c.dealt - kPad) - c.unit0;
+    c.whole = c.units == all - kPad;
+    c.h = hg / p.groups, c.grp = hg - c.h * p.groups;
+    row_extent(p, lo, c.first, c.keys);
+    return c;
+  };
 
-    // tiles of this warp: first0, first0 + 8, ... below tile_end. The copies run STAGES - 1 tiles ahead,
-    // the page lookups one tile further.
-    const int tile_end = min((unit0 + n_units) * kWarps, (keys + kTile - 1) / kTile);
-    const int first0 = unit0 * kWarps + warp;
-    const int count = first0 < tile_end ? (tile_end - first0 + kWarps - 1) / kWarps : 0;
-    const int* trow = p.table + (long long)b * p.max_pages;
-    int ahead = 0;                                                    // tiles looked up
-    int lp = first0 / p.tiles_per_page, tip = first0 - lp * p.tiles_per_page;  // their next page and tile in it
-    int next_page = -1, next_tip = 0;
-    auto look_up = [&]() {
-      next_page = ahead < count ? trow[lp] : -1;
-      if (next_page >= p.n_pages) next_page = -1;
-      next_tip = tip;
-      lp += p.page_step;
-      tip += p.tile_step;
-      if (tip >= p.tiles_per_page) tip -= p.tiles_per_page, ++lp;
-      ++ahead;
-    };
-    unsigned have = 0;  // bit i: the i-th tile from the current one has a page
-    auto issue = [&](int stage, unsigned bit) {
-      if (next_page >= 0) {
-        have |= bit;
-        const long long head = (long long)next_page * p.Hkv + h;
-        const long long at = (head * p.page_size + next_tip * kTile) * D + lane * 16;
-        const unsigned dst = ring + stage * 2 * TB;
+  // A warp's tiles of a piece: first0, first0 + 8, ..., `count` of them. Lane i knows the page and the tile
+  // in it of the i-th of every 32.
+  int first0, count, ahead, my_page, my_tip;
+  unsigned have;  // bit i: the i-th tile from the current one has a page
+  const int* trow;
+  auto look_up = [&]() {
+    const int i = ahead + lane, tile = first0 + i * kWarps, lp = tile / p.tiles_per_page;
+    my_tip = tile - lp * p.tiles_per_page;
+    my_page = i < count ? trow[lp] : -1;
+    if (my_page >= p.n_pages) my_page = -1;
+  };
+  auto issue = [&](int stage, unsigned bit, int h) {  // copies of the next tile
+    if ((ahead & 31) == 0 && ahead > 0 && ahead < count) look_up();
+    const int page = __shfl_sync(0xffffffff, my_page, ahead & 31), tip = __shfl_sync(0xffffffff, my_tip, ahead & 31);
+    if (ahead < count && page >= 0) {
+      have |= bit;
+      const long long head = (long long)page * p.Hkv + h;
+      const long long at = (head * p.page_size + tip * kTile) * D + lane * 16;
+      const unsigned dst = ring + stage * kWarps * SLOT;
 #pragma unroll
-        for (int j = 0; j < TB / 512; ++j) {
-          const unsigned to = dst + (j & 1 ? put1 : put0) + (j >> 1) * 1024;
-          cp_async16(to, p.kc + at + j * 512);
-          cp_async16(to + TB, p.vc + at + j * 512);
-        }
-        const long long blk = head * p.blocks_per_page + (next_tip >> p.block_shift);
-        if (lane < 2) cp_async4(mags + stage * 8 + lane * 4, (lane ? p.va : p.ka) + blk);
+      for (int j = 0; j < TB / 512; ++j) {
+        const unsigned to = dst + (j & 1 ? put1 : put0) + (j >> 1) * 1024;
+        cp_async16(to, p.kc + at + j * 512);
+        cp_async16(to + TB, p.vc + at + j * 512);
       }
-      cp_async_commit();
-      look_up();
-    };
+      const long long blk = head * p.blocks_per_page + (tip >> p.block_shift);
+      if (lane < 2) cp_async4(mags + stage * 8 + lane * 4, (lane ? p.va : p.ka) + blk);
+    }
+    cp_async_commit();
+    ++ahead;
+  };
+  // lane (g, t): channels t * D / 4 .. of query row g of each 8-row tile
+  uint4 q_raw[NT][D / 32];
+  auto begin = [&](const Piece& c) {  // loads that the piece starts with
+    const int tile_end = min((c.unit0 + c.units) * p.unit_tiles, (c.keys + kTile - 1) / kTile);
+    first0 = c.unit0 * p.unit_tiles + warp;
+    count = first0 < tile_end ? (tile_end - first0 + kWarps - 1) / kWarps : 0;
+    trow = p.table + (long long)c.b * p.max_pages;
+    ahead = 0, have = 0;
     look_up();
 #pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) issue(i, 1u << i);
+    for (int n = 0; n < NT; ++n) {
+      const int r = c.grp * R + n * 8 + g, i = r / p.G;
+      const T* src = static_cast<const T*>(p.q) + (long long)c.b * p.qb + (long long)i * p.qs +
+                     (long long)(c.h * p.G + (r - i * p.G)) * p.qh + t * (D / 4);
+#pragma unroll
+      for (int j = 0; j < D / 32; ++j)
+        q_raw[n][j] = r < p.S * p.G ? reinterpret_cast<const uint4*>(src)[j] : make_uint4(0u, 0u, 0u, 0u);
+    }
+#pragma unroll
+    for (int i = 0; i < STAGES - 1; ++i) issue(i, 1u << i, c.h);
+  };
 
-    // query fragments: lane (g, t) holds channels t * D / 4 .. of query row g of each 8-row tile, as
-    // fp16 scaled by a power of two that brings the row's largest magnitude to [2^14, 2^15)
+  long long u = u_begin;
+  Piece c = find(u);
+  if (c.units == 0) {  // the range begins with a segment's start alone: the keys after it are another CTA's
+    u += c.dealt;
+    if (u >= u_end) return;
+    c = find(u);
+  }
+  begin(c);
+  for (;;) {
+    // query fragments: fp16 scaled by a power of two that brings the row's largest magnitude to [2^14, 2^15)
     unsigned qf[NT][KS][2];
     float qscale[NT][2], qbias[NT][2];  // of the columns 2t, 2t + 1 of S^T
     int vis[NT][2];                     // keys that those columns see
-    int seen_by_all = keys;
+    int seen_by_all = c.keys;
+    const int len = p.lens[c.b];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const int r = grp * R + n * 8 + g, i = r / p.G;
-      const bool ok = r < p.S * p.G;
-      const T* src = static_cast<const T*>(p.q) + (long long)b * p.qb + (long long)i * p.qs +
-                     (long long)(h * p.G + (r - i * p.G)) * p.qh + t * (D / 4);
-      uint4 raw[D / 32];
+      const unsigned short* e = reinterpret_cast<const unsigned short*>(q_raw[n]);
+      unsigned bits = 0;  // magnitudes compare as integers
 #pragma unroll
       for (int j = 0; j < D / 32; ++j)
-        raw[j] = ok ? reinterpret_cast<const uint4*>(src)[j] : make_uint4(0u, 0u, 0u, 0u);
-      const unsigned short* e = reinterpret_cast<const unsigned short*>(raw);
-      float most = 0.f;
-#pragma unroll
-      for (int j = 0; j < D / 4; ++j) most = fmaxf(most, fabsf(bits_to_float<T>(e[j])));
-      most = fmaxf(most, __shfl_xor_sync(0xffffffff, most, 1));
-      most = fmaxf(most, __shfl_xor_sync(0xffffffff, most, 2));
-      int ex = 0;
-      if (most > 0.f && most < INFINITY) ex = max(ilogbf(most), -110);
-      const float down = ldexpf(1.f, 14 - ex), up = ldexpf(p.scale, ex - 14);
+        bits = __vmaxu2(bits, __vmaxu2(__vmaxu2(q_raw[n][j].x & 0x7fff7fffu, q_raw[n][j].y & 0x7fff7fffu),
+                                       __vmaxu2(q_raw[n][j].z & 0x7fff7fffu, q_raw[n][j].w & 0x7fff7fffu)));
+      bits = max(bits & 0xffffu, bits >> 16);
+      bits = max(bits, __shfl_xor_sync(0xffffffff, bits, 1));
+      bits = max(bits, __shfl_xor_sync(0xffffffff, bits, 2));
+      // the magnitude's exponent, as that of an fp32 number; subnormals and what is not finite scale by 2^14
+      const int fe = (int)(__float_as_uint(bits_to_float<T>((unsigned short)bits)) >> 23);
+      const int ex = fe == 0 || fe == 255 ? 0 : max(fe - 127, -100);
+      const float down = __int_as_float((127 + 14 - ex) << 23);
+      const float up = p.scale * __int_as_float((127 - 14 + max(ex, -100)) << 23);
       float sum = 0.f;
 #pragma unroll
       for (int s = 0; s < KS; ++s)
@@ -466,10 +525,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv8_attend_kerne
         qscale[n][k] = __shfl_sync(0xffffffff, up, (2 * t + k) * 4);
         qbias[n][k] = -128.f * qscale[n][k] * __shfl_sync(0xffffffff, sum, (2 * t + k) * 4);
         qscale[n][k] *= 0x1p24f;
-        const int rc = grp * R + n * 8 + 2 * t + k, ic = rc / p.G;
+        const int rc = c.grp * R + n * 8 + 2 * t + k, pos = c.first + rc / p.G;
         // columns behind the last query row are computed like the others and never written
-        vis[n][k] = rc >= p.S * p.G ? keys
-                    : first + ic >= 0 && first + ic < p.lens[b] ? min(first + ic + 1, keys) : 0;
+        vis[n][k] = rc >= p.S * p.G ? c.keys : pos >= 0 && pos < len ? min(pos + 1, c.keys) : 0;
         seen_by_all = min(seen_by_all, vis[n][k]);
       }
     }
@@ -493,9 +551,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv8_attend_kerne
       __syncwarp();  // this tile has landed for all lanes, and all have left the stage that is refilled now
       const bool held = have & 1u;
       have >>= 1;
-      issue(refill, 1u << (STAGES - 2));
+      issue(refill, 1u << (STAGES - 2), c.h);
       refill = refill + 1 == STAGES ? 0 : refill + 1;
-      const unsigned tile = ring + stage * 2 * TB;
+      const unsigned tile = ring + stage * kWarps * SLOT;
       const float2 mag = lds_float2(mags + stage * 8);
       stage = stage + 1 == STAGES ? 0 : stage + 1;
       if (!held) continue;  // the same for the whole warp
@@ -524,9 +582,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv8_attend_kerne
       for (int n = 0; n < NT; ++n) {
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const float a = qscale[n][k] * mag.x, c = qbias[n][k] * mag.x;
-          sc[n][k] = fmaf(sc[n][k], a, c);
-          sc[n][2 + k] = fmaf(sc[n][2 + k], a, c);
+          const float a = qscale[n][k] * mag.x, c0 = qbias[n][k] * mag.x;
+          sc[n][k] = fmaf(sc[n][k], a, c0);
+          sc[n][2 + k] = fmaf(sc[n][2 + k], a, c0);
         }
         if (tok + kTile > seen_by_all) {
 #pragma unroll
@@ -597,66 +655,82 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv8_attend_kerne
       }
     }
     cp_async_wait<0>();
-    __syncthreads();  // the rings become the merge buffer
+    __syncwarp();
 
-    // merge the warps: sums over the tokens of a warp lie on lanes of equal t
-    float* merge = reinterpret_cast<float*>(smem);  // [warp][R][D]
+    // The next piece's first copies fly while this one is merged: they fill all stages of the ring but the
+    // last NT, which hold what the warps merge.
+    const Piece done = c;
+    const long long slot = 2LL * blockIdx.x + (done.unit0 > 0 ? 0 : 1);
+    u += done.dealt;
+    bool more = u < u_end;
+    if (more) {
+      c = find(u);
+      more = c.units > 0;  // else the range ends with a segment's start alone
+      if (more) begin(c);
+    }
+
+    // [R][D] floats of warp w, 8 rows per ring slot; the channels of a row are permuted by 16 so that the
+    // four rows that a warp writes at a time lie on different banks
+    auto merge_at = [&](int w, int row, int ch) {
+      return reinterpret_cast<float*>(smem + ((STAGES - NT + row / 8) * kWarps + w) * SLOT) + row % 8 * D +
+             (ch ^ ((row >> 1 & 3) << 4));
+    };
+    const int rows = min(R, p.S * p.G - done.grp * R);
 #pragma unroll
     for (int n = 0; n < NT; ++n)
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
-        float s = l[n][k];
+        float s = l[n][k];  // sums over the tokens of a warp lie on lanes of equal t
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) s += __shfl_xor_sync(0xffffffff, s, d);
-        if (g == 0) {
-          stat_s[warp][n * 8 + 2 * t + k][0] = m[n][k];
-          stat_s[warp][n * 8 + 2 * t + k][1] = M[n][k];
-          stat_s[warp][n * 8 + 2 * t + k][2] = s;
-        }
+        const int row = n * 8 + 2 * t + k;
+        if (row < rows) {
+          if (g == 0) stat_s[warp][row][0] = m[n][k], stat_s[warp][row][1] = M[n][k], stat_s[warp][row][2] = s;
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-          const int row = n * 8 + 2 * t + k, ch = 16 * i + 2 * g;
-          *reinterpret_cast<float2*>(merge + (warp * R + row) * D + ch) = make_float2(o[n][i][k], o[n][i][2 + k]);
+          for (int i = 0; i < MT; ++i)
+            *reinterpret_cast<float2*>(merge_at(warp, row, 16 * i + 2 * g)) = make_float2(o[n][i][k], o[n][i][2 + k]);
         }
       }
     __syncthreads();
-    const bool whole = n_units == units;
-    const long long slot = 2LL * blockIdx.x + (u == u_begin ? 0 : 1);
-    for (int idx = tid; idx < R * D / 2; idx += kWarps * 32) {
-      const int row = idx / (D / 2), ch = idx % (D / 2) * 2;
-      const int r = grp * R + row;
-      if (r >= p.S * p.G) continue;
-      float mm = kNone, MM = kNone;
+    for (int row = warp; row < rows; row += kWarps) {  // a warp per row, a lane D / 32 channels
+      constexpr int C = D / 32;
+      const float* st = stat_s[lane & 7][row];
+      float mm = st[0], MM = st[1];
+#pragma unroll
+      for (int d = 1; d < 8; d <<= 1) {
+        mm = fmaxf(mm, __shfl_xor_sync(0xffffffff, mm, d));
+        MM = fmaxf(MM, __shfl_xor_sync(0xffffffff, MM, d));
+      }
+      const float f = ex2(st[1] - MM);
+      float sum = st[2] * ex2(st[0] - mm);
+#pragma unroll
+      for (int d = 1; d < 8; d <<= 1) sum += __shfl_xor_sync(0xffffffff, sum, d);
+      float a[C];
+#pragma unroll
+      for (int j = 0; j < C; ++j) a[j] = 0.f;
 #pragma unroll
       for (int i = 0; i < kWarps; ++i) {
-        mm = fmaxf(mm, stat_s[i][row][0]);
-        MM = fmaxf(MM, stat_s[i][row][1]);
-      }
-      float2 a = make_float2(0.f, 0.f);
-      float sum = 0.f;
+        float v[C];
+        load_floats<C>(merge_at(i, row, lane * C), v);
+        const float fi = __shfl_sync(0xffffffff, f, i);
 #pragma unroll
-      for (int i = 0; i < kWarps; ++i) {
-        sum += stat_s[i][row][2] * ex2(stat_s[i][row][0] - mm);
-        const float f = ex2(stat_s[i][row][1] - MM);
-        const float2 v = *reinterpret_cast<const float2*>(merge + (i * R + row) * D + ch);
-        a.x += v.x * f, a.y += v.y * f;
+        for (int j = 0; j < C; ++j) a[j] += v[j] * fi;
       }
-      if (whole) {
-        const int i = r / p.G;
-        T* dst = static_cast<T*>(p.out) + (((long long)b * p.S + i) * p.Hq + h * p.G + (r - i * p.G)) * D + ch;
-        const float f = sum == 0.f ? 0.f : exp2f(MM - mm) * kStep / sum;  // no key seen: zeros
-        dst[0] = from_float<T>(a.x * f);
-        dst[1] = from_float<T>(a.y * f);
+      if (done.whole) {
+        const float to = sum == 0.f ? 0.f : exp2f(MM - mm) * kStep / sum;  // no key seen: zeros
+        store_out<T, D>(p, done.b, done.h, done.grp * R + row, lane * C, a, to);
       } else {
-        *reinterpret_cast<float2*>(p.part_o + (slot * R + row) * D + ch) = a;
-        if (ch == 0) {
-          float* st = p.part_s + (slot * R + row) * 3;
-          st[0] = mm, st[1] = MM, st[2] = sum;
+        float* to = p.part_o + (slot * R + row) * D + lane * C;
+        if constexpr (C == 4) *reinterpret_cast<float4*>(to) = make_float4(a[0], a[1], a[2], a[3]);
+        else *reinterpret_cast<float2*>(to) = make_float2(a[0], a[1]);
+        if (lane == 0) {
+          float* ps = p.part_s + (slot * R + row) * 3;
+          ps[0] = mm, ps[1] = MM, ps[2] = sum;
         }
       }
     }
-    __syncthreads();
-    u += n_units;
+    if (!more) return;
+    __syncthreads();  // what was merged may be overwritten
   }
 }
 
@@ -667,6 +741,7 @@ __global__ void __launch_bounds__(128) kv8_combine_kernel(const AttendParams p, 
   constexpr int C = D / 32;
   __shared__ int sums[2][4];
   __shared__ float stat_s[4][3], o_s[4][D];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int seg = blockIdx.x / rows, row = blockIdx.x - seg * rows;
   const int per = p.Hkv * p.groups, b = seg / per, hg = seg - b * per;
@@ -687,23 +762,22 @@ __global__ void __launch_bounds__(128) kv8_combine_kernel(const AttendParams p, 
   all = sums[0][0] + sums[0][1] + sums[0][2] + sums[0][3];
   pre = sums[1][0] + sums[1][1] + sums[1][2] + sums[1][3];
   const int units = row_units(p, b);
-  const long long total = (long long)all * per, u0 = (long long)pre * per + (long long)hg * units;
+  const long long total = (long long)all * per;
+  const long long u1 = (long long)pre * per + (long long)(hg + 1) * units, u0 = u1 - units + kPad;  // of the keys
   const int ctas = live_ctas(p, total);
-  const int c0 = cta_of(u0, total, ctas), c1 = cta_of(u0 + units - 1, total, ctas);
-  asm volatile("griddepcontrol.wait;" ::: "memory");  // up to here only inputs of the grid before were read
+  const int c0 = cta_of(u0, total, ctas), c1 = cta_of(u1 - 1, total, ctas);
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // up to here only lengths were read
   if (c0 == c1 || r >= p.S * p.G) return;  // one CTA had it all and wrote the output
   float m = kNone, M = kNone, sum = 0.f, a[C];
 #pragma unroll
   for (int i = 0; i < C; ++i) a[i] = 0.f;
 #pragma unroll 4
   for (int c = c0 + warp; c <= c1; c += 4) {
-    // a CTA's piece is its first unless its range began before the segment
-    const long long slot = 2LL * c + (c == c0 && total * c / ctas < u0 ? 1 : 0);
+    const long long slot = 2LL * c + (total * c / ctas > u0 ? 0 : 1);  // 0: the CTA begins inside the keys
     const float* st = p.part_s + (slot * R + row) * 3;
     const float* src = p.part_o + (slot * R + row) * D + lane * C;
     float v[C];
-    if constexpr (C == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(src);
-    else *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(src);
+    load_floats<C>(src, v);
     const float m1 = fmaxf(m, st[0]), M1 = fmaxf(M, st[1]);
     const float f = ex2(M - M1), e = ex2(st[1] - M1);
     sum = sum * ex2(m - m1) + st[2] * ex2(st[0] - m1);
@@ -730,15 +804,28 @@ __global__ void __launch_bounds__(128) kv8_combine_kernel(const AttendParams p, 
 }
 
 constexpr int stages_for(int NT) { return NT == 1 ? 3 : 6; }
-template <int D, int NT>
-constexpr int attend_smem() {
-  const int ring = kWarps * stages_for(NT) * 2 * kTile * D, merge = kWarps * 8 * NT * D * 4;
-  return ring > merge ? ring : merge;
+
+// With the attribute a kernel may be scheduled while the one before it on the stream still runs; it waits
+// for that one's end itself, so completion stays transitive along the stream.
+template <typename... A>
+void launch_early(void (*kernel)(A...), int grid, int threads, int smem, cudaStream_t s, A... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  note_launch();
+  cudaLaunchKernelEx(&cfg, kernel, args...);
 }
 
 template <typename T, int D, int NT>
 void launch_attend(const AttendParams& p, bool combine, cudaStream_t s) {
-  constexpr int smem = attend_smem<D, NT>();
+  constexpr int smem = kWarps * stages_for(NT) * 2 * kTile * D;
   auto kernel = kv8_attend_kernel<T, D, NT, stages_for(NT)>;
   static bool set[64] = {};  // the attribute belongs to the device that is current
   int dev = 0;
@@ -747,20 +834,10 @@ void launch_attend(const AttendParams& p, bool combine, cudaStream_t s) {
     cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (dev >= 0 && dev < 64) set[dev] = true;
   }
-  (note_launch(), kernel<<<p.ctas, kWarps * 32, smem, s>>>(p));
+  launch_early(kernel, p.ctas, kWarps * 32, smem, s, p);
   if (!combine) return;
-  cudaLaunchConfig_t cfg{};
   const int rows = std::min(8 * NT, p.S * p.G);
-  cfg.gridDim = dim3((unsigned)(p.B * p.Hkv * p.groups * rows));
-  cfg.blockDim = dim3(128);
-  cfg.stream = s;
-  cudaLaunchAttribute at{};
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &at;
-  cfg.numAttrs = 1;
-  note_launch();
-  cudaLaunchKernelEx(&cfg, kv8_combine_kernel<T, D, 8 * NT>, p, rows);
+  launch_early(kv8_combine_kernel<T, D, 8 * NT>, p.B * p.Hkv * p.groups * rows, 128, 0, s, p, rows);
 }
 
 }  // namespace
@@ -823,15 +900,19 @@ void kv8_gather(const void* kc, const void* vc, const float* ka, const float* va
 
 // Launch shape of an attention call, from sizes the host knows (not the lengths, which are on the
 // device): out[0] CTAs, out[1] query rows per group (R), out[2] groups, out[3] 1 if a segment can be
-// split over CTAs, out[4] workspace floats.
+// split over CTAs, out[4] workspace floats, out[5] tokens per unit of work. Rows of at most kWhole tokens
+// are not split: four steps of one CTA take less than joining two CTAs' work.
 void kv8_attend_plan(int B, int S, int Hq, int Hkv, int D, int page_size, int max_pages, int device, long long* out) {
   using namespace astrai;
+  const long long cap = (long long)max_pages * page_size;
   const int rows = S * (Hq / Hkv), R = rows <= 8 ? 8 : 16, groups = (rows + R - 1) / R;
-  const long long units = std::max<long long>(1, ((long long)max_pages * page_size + kUnit - 1) / kUnit);
-  const long long most = (long long)B * Hkv * groups * units;
+  const int unit = cap <= kWhole ? kWhole : kUnit;
+  const long long units = std::max<long long>(1, (cap + unit - 1) / unit);
+  const long long most = (long long)B * Hkv * groups * (units > 1 ? units + kPad : 1);
   const int ctas = (int)std::min<long long>(most, (long long)num_sms(device) * (R == 8 ? 2 : 1));
   out[0] = ctas, out[1] = R, out[2] = groups, out[3] = units > 1;
   out[4] = units > 1 ? 2LL * ctas * R * (D + 3) : 0;
+  out[5] = unit;
 }
 
 void kv8_attend(const void* q, const long long* qs, const void* kc, const void* vc, const float* ka, const float* va,
@@ -840,7 +921,7 @@ void kv8_attend(const void* q, const long long* qs, const void* kc, const void* 
                 int device, cudaStream_t s) {
   using namespace astrai;
   if (B <= 0 || S <= 0) return;
-  long long plan[5];
+  long long plan[6];
   kv8_attend_plan(B, S, Hq, Hkv, D, page_size, max_pages, device, plan);
   AttendParams p{};
   p.q = q, p.qb = qs[0], p.qs = qs[1], p.qh = qs[2];
@@ -849,8 +930,8 @@ void kv8_attend(const void* q, const long long* qs, const void* kc, const void* 
   p.B = B, p.S = S, p.Hq = Hq, p.Hkv = Hkv, p.G = Hq / Hkv, p.groups = (int)plan[2];
   p.page_size = page_size, p.n_pages = n_pages, p.max_pages = max_pages;
   p.tiles_per_page = page_size / kTile;
-  p.page_step = kWarps / p.tiles_per_page, p.tile_step = kWarps % p.tiles_per_page;
   p.blocks_per_page = page_size / block;
+  p.unit_tiles = (int)plan[5] / kTile;
   while ((kTile << p.block_shift) < block) ++p.block_shift;
   p.ctas = (int)plan[0], p.scale = scale * 1.4426950408889634f * kStep;
   p.part_o = workspace;
