@@ -81,7 +81,19 @@ int dtype_code(const at::Tensor& t, const char* name) {
   return t.scalar_type() == at::kHalf;
 }
 
-// [B, S, H, D] with a contiguous last dimension and 16-byte aligned rows; strides of the other three
+// [B, S, H, D] as the kernels read it: a contiguous last dimension and 16-byte aligned rows of any stride;
+// copied if it is not
+at::Tensor heads_of(const at::Tensor& t) {
+  if (t.dim() != 4) return t;  // refused by check_heads
+  bool ok = t.stride(3) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  for (int i = 0; i < 3; ++i) ok = ok && (t.size(i) <= 1 || t.stride(i) % 8 == 0);
+  return ok ? t : t.contiguous();
+}
+at::Tensor int32_of(const at::Tensor& t) {
+  return t.scalar_type() == at::kInt && t.is_contiguous() ? t : t.to(at::kInt).contiguous();
+}
+
+// strides of the batch, token and head dimensions
 void check_heads(const at::Tensor& t, const at::Tensor& like, const char* name, long long* strides) {
   TORCH_CHECK(t.is_cuda() && t.device() == like.device() && t.dim() == 4, "kv8: ", name,
               " must be a CUDA [batch, tokens, heads, head_dim] tensor on the cache's device");
@@ -95,9 +107,11 @@ void check_heads(const at::Tensor& t, const at::Tensor& like, const char* name, 
 
 cudaStream_t stream() { return at::cuda::getCurrentCUDAStream().stream(); }
 
-void kv8_append(const at::Tensor& k, const at::Tensor& v, at::Tensor& kc, at::Tensor& vc, at::Tensor& ka,
-                at::Tensor& va, const at::Tensor& table, const at::Tensor& starts, const at::Tensor& lens) {
+void kv8_append(const at::Tensor& k_in, const at::Tensor& v_in, at::Tensor& kc, at::Tensor& vc, at::Tensor& ka,
+                at::Tensor& va, const at::Tensor& table_in, const at::Tensor& starts_in, const at::Tensor& lens_in) {
   const Cache c = check_cache(kc, vc, ka, va);
+  const at::Tensor k = heads_of(k_in), v = heads_of(v_in);
+  const at::Tensor table = int32_of(table_in), starts = int32_of(starts_in), lens = int32_of(lens_in);
   long long ks[3], vs[3];
   check_heads(k, kc, "k", ks);
   check_heads(v, kc, "v", vs);
@@ -117,27 +131,30 @@ void kv8_append(const at::Tensor& k, const at::Tensor& v, at::Tensor& kc, at::Te
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
-void kv8_gather(const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ka, const at::Tensor& va,
-                const at::Tensor& table, const OptTensor& starts, const at::Tensor& lens, at::Tensor& ko,
-                at::Tensor& vo) {
+std::pair<at::Tensor, at::Tensor> kv8_gather(const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ka,
+                                             const at::Tensor& va, const at::Tensor& table_in,
+                                             const OptTensor& starts_in, const at::Tensor& lens_in, int64_t total,
+                                             at::ScalarType dtype) {
   const Cache c = check_cache(kc, vc, ka, va);
-  for (const auto* t : {&ko, &vo})
-    TORCH_CHECK(t->device() == kc.device() && t->dim() == 4 && t->is_contiguous() && t->sizes() == ko.sizes() &&
-                    t->scalar_type() == ko.scalar_type() && t->size(2) == c.Hkv && t->size(3) == c.D &&
-                    reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0,
-                "kv8_gather: outputs must be contiguous [batch, total, n_kv_heads, head_dim]");
-  const int dt = dtype_code(ko, "output");
-  const int64_t B = ko.size(0);
+  TORCH_CHECK(dtype == at::kBFloat16 || dtype == at::kHalf, "kv8_gather: bfloat16 or float16, got ", dtype);
+  TORCH_CHECK(total >= 0 && total < (1LL << 30), "kv8_gather: total must be in [0, 2^30)");
+  const at::Tensor table = int32_of(table_in), lens = int32_of(lens_in);
+  const int64_t B = table.dim() == 2 ? table.size(0) : -1;
   const int mp = check_table(table, kc, B, c);
-  const bool from = starts.has_value() && starts->defined();
-  const int* st = from ? check_i32(*starts, kc, B, "starts") : nullptr;
+  at::Tensor starts;
+  const int* st = nullptr;
+  if (starts_in.has_value() && starts_in->defined()) {
+    starts = int32_of(*starts_in);
+    st = check_i32(starts, kc, B, "starts");
+  }
   const int* ln = check_i32(lens, kc, B, "lens");
-  TORCH_CHECK(ko.size(1) < (1LL << 30), "kv8_gather: too many tokens");
   const c10::cuda::CUDAGuard g(kc.device());
+  auto ko = at::empty({B, total, c.Hkv, c.D}, kc.options().dtype(dtype)), vo = at::empty_like(ko);
   astrai_host::kv8_gather(kc.data_ptr(), vc.data_ptr(), ka.data_ptr<float>(), va.data_ptr<float>(),
-                          table.data_ptr<int>(), st, ln, ko.data_ptr(), vo.data_ptr(), (int)B, (int)ko.size(1), c.Hkv,
-                          c.D, c.page_size, c.n_pages, mp, c.block, dt, kc.device().index(), stream());
+                          table.data_ptr<int>(), st, ln, ko.data_ptr(), vo.data_ptr(), (int)B, (int)total, c.Hkv, c.D,
+                          c.page_size, c.n_pages, mp, c.block, dtype == at::kHalf, kc.device().index(), stream());
   C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return {ko, vo};
 }
 
 // fp32 elements of workspace that kv8_attend needs for these sizes (0: none)
@@ -153,31 +170,34 @@ int64_t kv8_attend_workspace(int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int6
   return plan[4];
 }
 
-void kv8_attend(const at::Tensor& q, const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ka,
-                const at::Tensor& va, const at::Tensor& table, const at::Tensor& lens, const OptTensor& starts,
-                at::Tensor& out, const OptTensor& workspace, double scale) {
+at::Tensor kv8_attend(const at::Tensor& q_in, const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ka,
+                      const at::Tensor& va, const at::Tensor& table_in, const at::Tensor& lens_in,
+                      const OptTensor& starts_in, const OptTensor& workspace, double scale) {
   const Cache c = check_cache(kc, vc, ka, va);
+  const at::Tensor q = heads_of(q_in), table = int32_of(table_in), lens = int32_of(lens_in);
   long long qs[3];
   check_heads(q, kc, "q", qs);
   const int dt = dtype_code(q, "q");
   const int64_t B = q.size(0), S = q.size(1), Hq = q.size(2);
   TORCH_CHECK(q.size(3) == c.D && Hq % c.Hkv == 0 && Hq >= 1, "kv8_attention: q ", text(q.sizes()),
               " does not fit the cache ", text(kc.sizes()));
-  TORCH_CHECK(out.device() == q.device() && out.scalar_type() == q.scalar_type() && out.is_contiguous() &&
-                  out.sizes() == q.sizes(),
-              "kv8_attention: out must be contiguous, of q's shape and type");
   TORCH_CHECK(B <= astrai_host::kv8_max_batch(), "kv8_attention: at most ",
               text((int64_t)astrai_host::kv8_max_batch()), " rows");
   const int mp = check_table(table, kc, B, c);
   const int* ln = check_i32(lens, kc, B, "lens");
-  const bool from = starts.has_value() && starts->defined();
-  const int* st = from ? check_i32(*starts, kc, B, "starts") : nullptr;
+  at::Tensor starts;
+  const int* st = nullptr;
+  if (starts_in.has_value() && starts_in->defined()) {
+    starts = int32_of(*starts_in);
+    st = check_i32(starts, kc, B, "starts");
+  }
   const int64_t units = ((int64_t)mp * c.page_size + 127) / 128, rows = S * (Hq / c.Hkv);
   TORCH_CHECK(rows < (1LL << 24) && units * B < (1LL << 31) && units * c.Hkv * (rows / 8 + 1) < (1LL << 31) &&
                   B * c.Hkv * (rows + 16) < (1LL << 31),
               "kv8_attention: too many rows or pages");
   const int64_t need = kv8_attend_workspace(B, S, Hq, c.Hkv, c.D, c.page_size, mp, q.device().index());
   const c10::cuda::CUDAGuard g(q.device());
+  auto out = at::empty({B, S, Hq, c.D}, q.options());
   at::Tensor ws;
   float* wp = nullptr;
   if (need > 0) {
@@ -195,6 +215,7 @@ void kv8_attend(const at::Tensor& q, const at::Tensor& kc, const at::Tensor& vc,
                           table.data_ptr<int>(), ln, st, out.data_ptr(), wp, (int)B, (int)S, (int)Hq, c.Hkv, c.D,
                           c.page_size, c.n_pages, mp, c.block, (float)scale, dt, q.device().index(), stream());
   C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return out;
 }
 
 }  // namespace
@@ -204,10 +225,10 @@ void register_kv8(pybind11::module& m) {
   m.def("kv8_append", &kv8_append, py::arg("k"), py::arg("v"), py::arg("k_cache"), py::arg("v_cache"),
         py::arg("k_absmax"), py::arg("v_absmax"), py::arg("page_table"), py::arg("starts"), py::arg("lens"));
   m.def("kv8_gather", &kv8_gather, py::arg("k_cache"), py::arg("v_cache"), py::arg("k_absmax"), py::arg("v_absmax"),
-        py::arg("page_table"), py::arg("starts"), py::arg("lens"), py::arg("k_out"), py::arg("v_out"));
+        py::arg("page_table"), py::arg("starts"), py::arg("lens"), py::arg("total"), py::arg("dtype"));
   m.def("kv8_attend_workspace", &kv8_attend_workspace, py::arg("batch"), py::arg("tokens"), py::arg("n_heads"),
         py::arg("n_kv_heads"), py::arg("head_dim"), py::arg("page_size"), py::arg("max_pages"), py::arg("device"));
   m.def("kv8_attend", &kv8_attend, py::arg("q"), py::arg("k_cache"), py::arg("v_cache"), py::arg("k_absmax"),
-        py::arg("v_absmax"), py::arg("page_table"), py::arg("lens"), py::arg("starts"), py::arg("out"),
+        py::arg("v_absmax"), py::arg("page_table"), py::arg("lens"), py::arg("starts"),
         py::arg("workspace"), py::arg("scale"));
 }

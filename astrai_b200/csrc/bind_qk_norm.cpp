@@ -88,59 +88,149 @@ Shape check(const at::Tensor& x, int64_t hq, int64_t hkv, int64_t D, const at::T
   return s;
 }
 
+struct Options {
+  int64_t hq, hkv, D, seq_len, rot, rot_off, norm;
+  bool half_layout;
+  double eps;
+};
+
+cudaStream_t stream() { return at::cuda::getCurrentCUDAStream().stream(); }
+
 // y may be x itself
-void qk_norm_fwd(const at::Tensor& x, at::Tensor& y, int64_t hq, int64_t hkv, int64_t D, const at::Tensor& table,
-                 const OptTensor& pos, int64_t seq_len, const OptTensor& wq, const OptTensor& wk, int64_t rot,
-                 int64_t rot_off, bool half_layout, int64_t norm, bool inverse, double eps) {
-  const Shape s = check(x, hq, hkv, D, table, pos, seq_len, wq, wk, rot, rot_off, norm);
-  check_rows(y, x, (hq + hkv) * D, "y");
+void forward_into(const at::Tensor& x, const at::Tensor& y, const at::Tensor& table, const OptTensor& pos,
+                  const OptTensor& wq, const OptTensor& wk, const Options& o, bool inverse) {
+  const Shape s = check(x, o.hq, o.hkv, o.D, table, pos, o.seq_len, wq, wk, o.rot, o.rot_off, o.norm);
+  check_rows(y, x, (o.hq + o.hkv) * o.D, "y");
   const c10::cuda::CUDAGuard g(x.device());
   astrai_host::qk_norm_fwd(x.data_ptr(), x.stride(0), y.data_ptr(), y.stride(0), s.rows, s.hq, s.hkv, s.D,
-                           table.data_ptr(), s.max_pos, s.pos, (int)seq_len, norm ? wq->data_ptr() : nullptr,
-                           norm ? wk->data_ptr() : nullptr, s.rot, s.rot_off, half_layout, (int)norm, inverse,
-                           (float)eps, s.dtype, s.device, at::cuda::getCurrentCUDAStream().stream());
+                           table.data_ptr(), s.max_pos, s.pos, (int)o.seq_len, o.norm ? wq->data_ptr() : nullptr,
+                           o.norm ? wk->data_ptr() : nullptr, s.rot, s.rot_off, o.half_layout, (int)o.norm, inverse,
+                           (float)o.eps, s.dtype, s.device, stream());
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
-int64_t qk_norm_bwd_scratch(int64_t rows, int64_t D, int64_t device) {
-  return astrai_host::qk_norm_bwd_blocks((int)rows, (int)device) * 2 * D;
-}
-
-void qk_norm_bwd(const at::Tensor& dy, const at::Tensor& x, at::Tensor& dx, int64_t hq, int64_t hkv, int64_t D,
-                 const at::Tensor& table, const OptTensor& pos, int64_t seq_len, const OptTensor& wq,
-                 const OptTensor& wk, int64_t rot, int64_t rot_off, bool half_layout, int64_t norm, double eps,
-                 at::Tensor& dwq, at::Tensor& dwk, at::Tensor& scratch) {
-  TORCH_CHECK(norm == 1 || norm == 2, "qk_norm_bwd: norm mode");
-  const Shape s = check(x, hq, hkv, D, table, pos, seq_len, wq, wk, rot, rot_off, norm);
-  check_rows(dy, x, (hq + hkv) * D, "dy");
-  check_rows(dx, x, (hq + hkv) * D, "dx");
-  for (const auto* w : {&dwq, &dwk})
-    TORCH_CHECK(w->device() == x.device() && w->scalar_type() == x.scalar_type() && w->is_contiguous() &&
-                    w->numel() == D,
-                "qk_norm_bwd: weight gradients must be contiguous [head_dim] of x's type");
-  TORCH_CHECK(scratch.device() == x.device() && scratch.scalar_type() == at::kFloat && scratch.is_contiguous() &&
-                  scratch.numel() >= qk_norm_bwd_scratch(s.rows, D, s.device),
-              "qk_norm_bwd: scratch too small");
+// Fills the query and key columns of dx; -> gradients of the weights (undefined without a norm).
+std::pair<at::Tensor, at::Tensor> backward_into(const at::Tensor& dy, const at::Tensor& x, const at::Tensor& dx,
+                                                const at::Tensor& table, const OptTensor& pos, const OptTensor& wq,
+                                                const OptTensor& wk, const Options& o) {
+  if (o.norm == 0) {  // the transposed rotation
+    forward_into(dy, dx, table, pos, wq, wk, o, true);
+    return {};
+  }
+  const Shape s = check(x, o.hq, o.hkv, o.D, table, pos, o.seq_len, wq, wk, o.rot, o.rot_off, o.norm);
+  check_rows(dy, x, (o.hq + o.hkv) * o.D, "dy");
+  check_rows(dx, x, (o.hq + o.hkv) * o.D, "dx");
   const c10::cuda::CUDAGuard g(x.device());
+  if (s.rows == 0) return {at::zeros_like(*wq), at::zeros_like(*wk)};
+  auto dwq = at::empty_like(*wq), dwk = at::empty_like(*wk);
+  auto scratch = at::empty({astrai_host::qk_norm_bwd_blocks(s.rows, s.device) * 2 * o.D}, x.options().dtype(at::kFloat));
   astrai_host::qk_norm_bwd(dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0), dx.data_ptr(), dx.stride(0), s.rows,
-                           s.hq, s.hkv, s.D, table.data_ptr(), s.max_pos, s.pos, (int)seq_len, wq->data_ptr(),
-                           wk->data_ptr(), s.rot, s.rot_off, half_layout, (int)norm, (float)eps, dwq.data_ptr(),
-                           dwk.data_ptr(), scratch.data_ptr<float>(), s.dtype, s.device,
-                           at::cuda::getCurrentCUDAStream().stream());
+                           s.hq, s.hkv, s.D, table.data_ptr(), s.max_pos, s.pos, (int)o.seq_len, wq->data_ptr(),
+                           wk->data_ptr(), s.rot, s.rot_off, o.half_layout, (int)o.norm, (float)o.eps, dwq.data_ptr(),
+                           dwk.data_ptr(), scratch.data_ptr<float>(), s.dtype, s.device, stream());
   C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return {dwq, dwk};
+}
+
+// a row view that the kernels can read, copied if t is none
+at::Tensor rows_of(const at::Tensor& t) {
+  const bool ok = t.stride(1) == 1 && (t.stride(0) * t.element_size()) % 16 == 0 &&
+                  reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  return ok ? t : t.contiguous();
+}
+
+// The autograd node, in C++: a training step of short kernels would otherwise wait for Python.
+struct QkNormRope : public torch::autograd::Function<QkNormRope> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const OptTensor& wq,
+                            const OptTensor& wk, const at::Tensor& table, const OptTensor& pos, int64_t hq,
+                            int64_t hkv, int64_t D, int64_t seq_len, int64_t rot, int64_t rot_off, int64_t norm,
+                            bool half_layout, double eps) {
+    const Options o{hq, hkv, D, seq_len, rot, rot_off, norm, half_layout, eps};
+    const at::Tensor rows = rows_of(x);
+    auto y = at::empty({x.size(0), (hq + hkv) * D}, x.options());
+    forward_into(rows, y, table, pos, wq, wk, o, false);
+    const auto or_none = [](const OptTensor& t) { return given(t) ? *t : at::Tensor(); };
+    ctx->save_for_backward({rows, or_none(wq), or_none(wk), table, or_none(pos)});
+    ctx->saved_data["ints"] = std::vector<int64_t>{hq, hkv, D, seq_len, rot, rot_off, norm, half_layout, x.size(1)};
+    ctx->saved_data["eps"] = eps;
+    return y;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    TORCH_CHECK(!at::GradMode::is_enabled(), "qk_norm_rope has no second derivative (create_graph)");
+    const auto saved = ctx->get_saved_variables();
+    const auto n = ctx->saved_data["ints"].toIntVector();
+    const Options o{n[0], n[1], n[2], n[3], n[4], n[5], n[6], n[7] != 0, ctx->saved_data["eps"].toDouble()};
+    const at::Tensor& x = saved[0];
+    torch::autograd::variable_list out(14);
+    if (!grads[0].defined()) return out;
+    const at::Tensor dy = rows_of(grads[0]);
+    const int64_t used = (o.hq + o.hkv) * o.D, width = n[8];
+    auto dx = at::empty({x.size(0), width}, x.options());
+    if (width > used) dx.narrow(1, used, width - used).zero_();  // columns behind the keys are not an input
+    auto dw = backward_into(dy, x, dx, saved[3], saved[4], saved[1], saved[2], o);
+    out[0] = dx, out[1] = dw.first, out[2] = dw.second;
+    return out;
+  }
+};
+
+// The user's call: argument errors are ValueErrors here, wrong tensors RuntimeErrors in check().
+at::Tensor qk_norm_rope(const at::Tensor& x, int64_t hq, int64_t hkv, int64_t D, const at::Tensor& table,
+                        OptTensor wq, OptTensor wk, OptTensor pos, int64_t seq_len, double eps, bool half_layout,
+                        int64_t norm, int64_t rot, int64_t rot_off, bool in_place) {
+  TORCH_CHECK_VALUE(x.dim() == 2 && x.size(1) >= (hq + hkv) * D,
+                    "qk_norm_rope: x must be [rows, >= (n_heads + n_kv_heads) * head_dim]");
+  TORCH_CHECK_VALUE(rot > 0 && rot % 2 == 0 && rot_off >= 0 && rot + rot_off <= D,
+                    "qk_norm_rope: rot_dim at rot_off is no even part of head_dim");
+  TORCH_CHECK_VALUE(table.dim() == 3 && table.size(1) * 2 == rot && table.size(2) == 2,
+                    "qk_norm_rope: table must be [max_pos, rot_dim / 2, 2]");
+  if (norm == 0) wq = wk = OptTensor();
+  TORCH_CHECK_VALUE(norm == 0 || (given(wq) && given(wk) && wq->numel() == D && wk->numel() == D),
+                    "qk_norm_rope: the norm needs q_weight and k_weight of head_dim entries");
+  TORCH_CHECK_VALUE(given(pos) || seq_len > 0, "qk_norm_rope: positions or seq_len must be given");
+  if (given(pos)) {
+    TORCH_CHECK_VALUE(pos->numel() == x.size(0), "qk_norm_rope: positions must have one entry per row");
+    if (pos->scalar_type() != at::kInt || !pos->is_contiguous()) pos = pos->to(at::kInt).contiguous();
+  }
+  const bool grad = at::GradMode::is_enabled() &&
+                    (x.requires_grad() || (norm && (wq->requires_grad() || wk->requires_grad())));
+  const Options o{hq, hkv, D, seq_len, rot, rot_off, norm, half_layout, eps};
+  if (in_place) {
+    TORCH_CHECK(!(at::GradMode::is_enabled() && x.requires_grad()), "qk_norm_rope_ has no gradient: use qk_norm_rope");
+    forward_into(x, x, table, pos, wq, wk, o, false);
+    return x;
+  }
+  if (grad)
+    return QkNormRope::apply(x, wq, wk, table, pos, hq, hkv, D, seq_len, rot, rot_off, norm, half_layout, eps);
+  auto y = at::empty({x.size(0), (hq + hkv) * D}, x.options());
+  forward_into(rows_of(x), y, table, pos, wq, wk, o, false);
+  return y;
 }
 
 }  // namespace
 
 void register_qk_norm(pybind11::module& m) {
   namespace py = pybind11;
-  m.def("qk_norm_fwd", &qk_norm_fwd, py::arg("x"), py::arg("y"), py::arg("n_heads"), py::arg("n_kv_heads"),
-        py::arg("head_dim"), py::arg("table"), py::arg("positions"), py::arg("seq_len"), py::arg("q_weight"),
-        py::arg("k_weight"), py::arg("rot_dim"), py::arg("rot_off"), py::arg("half_layout"), py::arg("norm"),
-        py::arg("inverse"), py::arg("eps"));
-  m.def("qk_norm_bwd_scratch", &qk_norm_bwd_scratch);
-  m.def("qk_norm_bwd", &qk_norm_bwd, py::arg("dy"), py::arg("x"), py::arg("dx"), py::arg("n_heads"),
-        py::arg("n_kv_heads"), py::arg("head_dim"), py::arg("table"), py::arg("positions"), py::arg("seq_len"),
-        py::arg("q_weight"), py::arg("k_weight"), py::arg("rot_dim"), py::arg("rot_off"), py::arg("half_layout"),
-        py::arg("norm"), py::arg("eps"), py::arg("dq_weight"), py::arg("dk_weight"), py::arg("scratch"));
+  m.def("qk_norm_rope", &qk_norm_rope, py::arg("x"), py::arg("n_heads"), py::arg("n_kv_heads"), py::arg("head_dim"),
+        py::arg("table"), py::arg("q_weight"), py::arg("k_weight"), py::arg("positions"), py::arg("seq_len"),
+        py::arg("eps"), py::arg("half_layout"), py::arg("norm"), py::arg("rot_dim"), py::arg("rot_off"),
+        py::arg("in_place"));
+  // on row buffers, for callers with an autograd node of their own
+  m.def("qk_norm_fwd", [](const at::Tensor& x, const at::Tensor& y, int64_t hq, int64_t hkv, int64_t D,
+                          const at::Tensor& table, const OptTensor& pos, int64_t seq_len, const OptTensor& wq,
+                          const OptTensor& wk, int64_t rot, int64_t rot_off, bool half_layout, int64_t norm, double eps) {
+    forward_into(x, y, table, pos, wq, wk, Options{hq, hkv, D, seq_len, rot, rot_off, norm, half_layout, eps}, false);
+  }, py::arg("x"), py::arg("y"), py::arg("n_heads"), py::arg("n_kv_heads"), py::arg("head_dim"), py::arg("table"),
+     py::arg("positions"), py::arg("seq_len"), py::arg("q_weight"), py::arg("k_weight"), py::arg("rot_dim"),
+     py::arg("rot_off"), py::arg("half_layout"), py::arg("norm"), py::arg("eps"));
+  m.def("qk_norm_bwd", [](const at::Tensor& dy, const at::Tensor& x, const at::Tensor& dx, int64_t hq, int64_t hkv,
+                          int64_t D, const at::Tensor& table, const OptTensor& pos, int64_t seq_len, const OptTensor& wq,
+                          const OptTensor& wk, int64_t rot, int64_t rot_off, bool half_layout, int64_t norm, double eps) {
+    auto dw = backward_into(dy, x, dx, table, pos, wq, wk,
+                            Options{hq, hkv, D, seq_len, rot, rot_off, norm, half_layout, eps});
+    auto or_none = [](const at::Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
+    return std::make_pair(or_none(dw.first), or_none(dw.second));
+  }, py::arg("dy"), py::arg("x"), py::arg("dx"), py::arg("n_heads"), py::arg("n_kv_heads"), py::arg("head_dim"),
+     py::arg("table"), py::arg("positions"), py::arg("seq_len"), py::arg("q_weight"), py::arg("k_weight"),
+     py::arg("rot_dim"), py::arg("rot_off"), py::arg("half_layout"), py::arg("norm"), py::arg("eps"));
 }

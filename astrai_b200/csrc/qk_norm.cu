@@ -37,30 +37,45 @@ struct QkNormParams {
   const int* pos;   // null: row % seq_len
   float* dw_part;   // backward: [blocks][2][D]
   int* err;
-  int rows, hq, heads, D, rot, rot_off, seq_len, max_pos, parts;
-  float sign, eps;
+  int rows, hq, hkv, D, rot, rot_off, seq_len, max_pos;
+  int q_parts;      // warps of a row that share its query heads; the others share its key heads
+  float sign, eps, inv_d;
 };
 
-template <typename T>
-__device__ __forceinline__ void load4(const T* p, float* o) {
-  if constexpr (sizeof(T) == 4) {
-    const float4 v = *reinterpret_cast<const float4*>(p);
-    o[0] = v.x, o[1] = v.y, o[2] = v.z, o[3] = v.w;
-  } else {
-    const uint2 v = *reinterpret_cast<const uint2*>(p);
-    const T* e = reinterpret_cast<const T*>(&v);
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if constexpr (std::is_same<T, __half>::value) o[j] = __half2float(e[j]);
-      else o[j] = __bfloat162float(e[j]);
-    }
-  }
-}
 template <typename T>
 __device__ __forceinline__ T round_to(float x) {
   if constexpr (std::is_same<T, __half>::value) return __float2half_rn(x);
   else if constexpr (std::is_same<T, __nv_bfloat16>::value) return __float2bfloat16_rn(x);
   else return x;
+}
+// four values in pairs: two conversions' worth of instructions less per pair than one by one
+template <typename T>
+__device__ __forceinline__ void unpack4(const T* v, float* o) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) o[j] = v[j];
+  } else {
+    const unsigned* u = reinterpret_cast<const unsigned*>(v);
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      float2 f;
+      if constexpr (std::is_same<T, __half>::value) f = __half22float2(*reinterpret_cast<const __half2*>(u + j));
+      else f = make_float2(__uint_as_float(u[j] << 16), __uint_as_float(u[j] & 0xffff0000u));
+      o[2 * j] = f.x, o[2 * j + 1] = f.y;
+    }
+  }
+}
+template <typename T>
+__device__ __forceinline__ void pack4(T* v, float a, float b, float c, float d) {
+  if constexpr (std::is_same<T, __half>::value) {
+    reinterpret_cast<__half2*>(v)[0] = __floats2half2_rn(a, b);
+    reinterpret_cast<__half2*>(v)[1] = __floats2half2_rn(c, d);
+  } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
+    reinterpret_cast<unsigned*>(v)[0] = pack_bf16(a, b);
+    reinterpret_cast<unsigned*>(v)[1] = pack_bf16(c, d);
+  } else {
+    v[0] = a, v[1] = b, v[2] = c, v[3] = d;
+  }
 }
 template <typename T>
 struct alignas(sizeof(T) * 4) Four {
@@ -115,8 +130,8 @@ __device__ __forceinline__ Raw8<T> load_raw(const T* head, const Place<HALF>& at
 template <bool HALF, typename T>
 __device__ __forceinline__ void to_pairs(const Raw8<T>& r, float* a, float* b) {
   float f[8];
-  load4(r.c[0].v, f);
-  load4(r.c[1].v, f + 4);
+  unpack4(r.c[0].v, f);
+  unpack4(r.c[1].v, f + 4);
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     a[i] = HALF ? f[i] : f[2 * i];
@@ -126,15 +141,12 @@ __device__ __forceinline__ void to_pairs(const Raw8<T>& r, float* a, float* b) {
 template <bool HALF, typename T>
 __device__ __forceinline__ void store_pairs(T* head, const Place<HALF>& at, const float* a, const float* b) {
   Raw8<T> r;
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    if constexpr (HALF) {
-      r.c[0].v[i] = round_to<T>(a[i]);
-      r.c[1].v[i] = round_to<T>(b[i]);
-    } else {
-      r.c[i / 2].v[i % 2 * 2] = round_to<T>(a[i]);
-      r.c[i / 2].v[i % 2 * 2 + 1] = round_to<T>(b[i]);
-    }
+  if constexpr (HALF) {
+    pack4(r.c[0].v, a[0], a[1], a[2], a[3]);
+    pack4(r.c[1].v, b[0], b[1], b[2], b[3]);
+  } else {
+    pack4(r.c[0].v, a[0], b[0], a[1], b[1]);
+    pack4(r.c[1].v, a[2], b[2], a[3], b[3]);
   }
   if constexpr (HALF || sizeof(T) == 4) {
     *reinterpret_cast<Four<T>*>(head + at.c0) = r.c[0];
@@ -175,223 +187,251 @@ __device__ __forceinline__ float head_sum(float v) {
   return v;
 }
 
-constexpr int kUnroll = 4;  // heads per lane group and warp item: their loads are in flight together
+// The heads of a row that a warp owns: only query heads or only key heads, so that one weight and one sum of
+// weight gradients stay in its registers. It takes them in steps of 32 / LPH, `stride` steps apart.
+struct Share {
+  int part, stride, col0, heads;
+  bool key;
+  __device__ __forceinline__ Share(const QkNormParams& p, int w, int warps) {
+    key = w >= p.q_parts;
+    part = key ? w - p.q_parts : w;
+    stride = key ? warps - p.q_parts : p.q_parts;
+    col0 = key ? p.hq * p.D : 0;
+    heads = key ? p.hkv : p.hq;
+  }
+};
 
-// One warp per (row, part): the row's heads in steps of 32 / LPH are dealt out to `parts` warps.
-template <typename T, int LPH, bool HALF, int NORM>
-__global__ void __launch_bounds__(256) qk_norm_fwd_kernel(const QkNormParams p) {
-  constexpr int HPW = 32 / LPH;
-  const int lane = threadIdx.x & 31, sub = lane / LPH;
-  const Place<HALF> at(lane % LPH, p);
-  const long long item = blockIdx.x * 8LL + (threadIdx.x >> 5);
-  const int row = (int)(item / p.parts), part = (int)(item % p.parts);
+constexpr int kFwdSteps = 4;  // steps of a warp whose loads are in flight together
+constexpr int kBwdSteps = 2;
+
+// Block (32, warps per row, rows). FULL: every lane of a head has channels (D = 8 LPH).
+template <typename T, int LPH, bool HALF, int NORM, bool FULL>
+__global__ void __launch_bounds__(384, 2) qk_norm_fwd_kernel(const QkNormParams p) {
+  constexpr int HPW = 32 / LPH, U = kFwdSteps;
+  const int lane = threadIdx.x, sub = lane / LPH;
+  Place<HALF> at(lane % LPH, p);
+  if (FULL) at.on = true;
+  const Share sh(p, threadIdx.y, blockDim.y);
+  const int row = blockIdx.x * blockDim.z + threadIdx.z;
   if (row >= p.rows) return;
-  const T* x = static_cast<const T*>(p.x) + (long long)row * p.ldx;
-  T* y = static_cast<T*>(p.out) + (long long)row * p.ldo;
-  Raw8<T> raw[kUnroll];
-#pragma unroll
-  for (int u = 0; u < kUnroll; ++u) {
-    const int h = (part + u * p.parts) * HPW + sub;
-    if (h < p.heads && at.on) raw[u] = load_raw<HALF>(x + h * p.D, at);
-  }
+  const T* x = static_cast<const T*>(p.x) + (long long)row * p.ldx + sh.col0 + sub * p.D;
+  T* y = static_cast<T*>(p.out) + (long long)row * p.ldo + sh.col0 + sub * p.D;
+  const int step = HPW * p.D;
   float2 cs[4];
-  load_cs<HALF>(p, row, at, cs);
-  float w[2][8];
-  if (NORM != kNone && at.on) {
-    to_pairs<HALF>(load_raw<HALF>(static_cast<const T*>(p.wq), at), w[0], w[0] + 4);
-    to_pairs<HALF>(load_raw<HALF>(static_cast<const T*>(p.wk), at), w[1], w[1] + 4);
-  }
+  float wa[4], wb[4];
+  for (int s0 = sh.part; s0 * HPW < sh.heads; s0 += U * sh.stride) {
+    Raw8<T> raw[U];
 #pragma unroll
-  for (int u = 0; u < kUnroll; ++u) {
-    const int h = (part + u * p.parts) * HPW + sub;
-    const bool on = h < p.heads && at.on;
-    if ((part + u * p.parts) * HPW >= p.heads) break;  // the same for the whole warp
-    float a[4], b[4];
-    if (on) to_pairs<HALF>(raw[u], a, b);
-    if (NORM != kBefore && on) rotate(a, b, cs, p.sign);
-    if (NORM != kNone) {
-      float ss = 0.f;
-      if (on) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) ss += a[i] * a[i] + b[i] * b[i];
-      }
-      const float r = rsqrtf(head_sum<LPH>(ss) / (float)p.D + p.eps);
-      if (on) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          a[i] *= r * (h < p.hq ? w[0][i] : w[1][i]);
-          b[i] *= r * (h < p.hq ? w[0][4 + i] : w[1][4 + i]);
-        }
-      }
+    for (int u = 0; u < U; ++u) {
+      const int s = s0 + u * sh.stride;
+      if (s * HPW + sub < sh.heads && at.on) raw[u] = load_raw<HALF>(x + s * step, at);
     }
-    if (NORM == kBefore && on) rotate(a, b, cs, p.sign);
-    if (on) store_pairs<HALF>(y + h * p.D, at, a, b);
+    if (s0 == sh.part) {  // behind the first loads
+      load_cs<HALF>(p, row, at, cs);
+      if (NORM != kNone && at.on)
+        to_pairs<HALF>(load_raw<HALF>(static_cast<const T*>(sh.key ? p.wk : p.wq), at), wa, wb);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int s = s0 + u * sh.stride;
+      if (s * HPW >= sh.heads) break;  // the same for the whole warp
+      const bool on = s * HPW + sub < sh.heads && at.on;
+      float a[4], b[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a[i] = b[i] = 0.f;
+      if (on) to_pairs<HALF>(raw[u], a, b);
+      if (NORM != kBefore) rotate(a, b, cs, p.sign);
+      if (NORM != kNone) {
+        float ss = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) ss = fmaf(a[i], a[i], fmaf(b[i], b[i], ss));
+        const float r = rsqrtf(fmaf(head_sum<LPH>(ss), p.inv_d, p.eps));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) a[i] *= r * wa[i], b[i] *= r * wb[i];
+      }
+      if (NORM == kBefore) rotate(a, b, cs, p.sign);
+      if (on) store_pairs<HALF>(y + s * step, at, a, b);
+    }
   }
 }
 
-// Backward: a warp walks items of the same shape, keeping its lanes' sums of g u in registers; a
-// block's sums go to its own row of dw_part, so the result does not depend on any order in time.
-template <typename T, int LPH, bool HALF, int NORM>
-__global__ void __launch_bounds__(256) qk_norm_bwd_kernel(const QkNormParams p) {
-  constexpr int HPW = 32 / LPH, U = 2;
-  const int lane = threadIdx.x & 31, sub = lane / LPH, warp = threadIdx.x >> 5;
-  const Place<HALF> at(lane % LPH, p);
-  float w[2][8], dw[2][8];
+// Backward: a block's rows are every (blocks * rows per block)-th; the sums of g u stay in registers and go to
+// the block's own row of dw_part, so the result does not depend on any order in time.
+template <typename T, int LPH, bool HALF, int NORM, bool FULL>
+__global__ void __launch_bounds__(384, sizeof(T) == 4 ? 1 : 2) qk_norm_bwd_kernel(const QkNormParams p) {
+  constexpr int HPW = 32 / LPH, U = kBwdSteps;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the sum over blocks waits for this grid
+  const int lane = threadIdx.x, sub = lane / LPH;
+  Place<HALF> at(lane % LPH, p);
+  if (FULL) at.on = true;
+  const Share sh(p, threadIdx.y, blockDim.y);
+  const int step = HPW * p.D;
+  float wa[4], wb[4], da[4], db[4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) w[0][i] = w[1][i] = dw[0][i] = dw[1][i] = 0.f;
-  if (at.on) {
-    to_pairs<HALF>(load_raw<HALF>(static_cast<const T*>(p.wq), at), w[0], w[0] + 4);
-    to_pairs<HALF>(load_raw<HALF>(static_cast<const T*>(p.wk), at), w[1], w[1] + 4);
-  }
-  const long long items = (long long)p.rows * p.parts;
-  for (long long item = blockIdx.x * 8LL + warp; item < items; item += gridDim.x * 8LL) {
-    const int row = (int)(item / p.parts), part = (int)(item % p.parts);
-    const T* x = static_cast<const T*>(p.x) + (long long)row * p.ldx;
-    const T* dy = static_cast<const T*>(p.dy) + (long long)row * p.lddy;
-    T* dx = static_cast<T*>(p.out) + (long long)row * p.ldo;
+  for (int i = 0; i < 4; ++i) wa[i] = wb[i] = da[i] = db[i] = 0.f;
+  if (at.on) to_pairs<HALF>(load_raw<HALF>(static_cast<const T*>(sh.key ? p.wk : p.wq), at), wa, wb);
+  for (int row = blockIdx.x * blockDim.z + threadIdx.z; row < p.rows; row += gridDim.x * blockDim.z) {
+    const T* x = static_cast<const T*>(p.x) + (long long)row * p.ldx + sh.col0 + sub * p.D;
+    const T* dy = static_cast<const T*>(p.dy) + (long long)row * p.lddy + sh.col0 + sub * p.D;
+    T* dx = static_cast<T*>(p.out) + (long long)row * p.ldo + sh.col0 + sub * p.D;
     float2 cs[4];
-    load_cs<HALF>(p, row, at, cs);
-    for (int s0 = part; s0 * HPW < p.heads; s0 += U * p.parts) {
+    for (int s0 = sh.part; s0 * HPW < sh.heads; s0 += U * sh.stride) {
       Raw8<T> rx[U], rg[U];
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int h = (s0 + u * p.parts) * HPW + sub;
-        if (h < p.heads && at.on) {
-          rx[u] = load_raw<HALF>(x + h * p.D, at);
-          rg[u] = load_raw<HALF>(dy + h * p.D, at);
+        const int s = s0 + u * sh.stride;
+        if (s * HPW + sub < sh.heads && at.on) {
+          rx[u] = load_raw<HALF>(x + s * step, at);
+          rg[u] = load_raw<HALF>(dy + s * step, at);
         }
       }
+      if (s0 == sh.part) load_cs<HALF>(p, row, at, cs);
 #pragma unroll
       for (int u = 0; u < U; ++u) {
-        const int h = (s0 + u * p.parts) * HPW + sub;
-        const bool on = h < p.heads && at.on, isq = h < p.hq;
+        const int s = s0 + u * sh.stride;
+        if (s * HPW >= sh.heads) break;  // the same for the whole warp
+        const bool on = s * HPW + sub < sh.heads && at.on;
         float a[4], b[4], ga[4], gb[4], ss = 0.f, gz = 0.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) a[i] = b[i] = ga[i] = gb[i] = 0.f;
         if (on) {
           to_pairs<HALF>(rx[u], a, b);
           to_pairs<HALF>(rg[u], ga, gb);
-          if (NORM == kAfter) rotate(a, b, cs, 1.f);
-          if (NORM == kBefore) rotate(ga, gb, cs, -1.f);
+        }
+        if (NORM == kAfter) rotate(a, b, cs, 1.f);
+        if (NORM == kBefore) rotate(ga, gb, cs, -1.f);
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            ss += a[i] * a[i] + b[i] * b[i];
-            gz += ga[i] * (isq ? w[0][i] : w[1][i]) * a[i] + gb[i] * (isq ? w[0][4 + i] : w[1][4 + i]) * b[i];
-          }
+        for (int i = 0; i < 4; ++i) {
+          ss = fmaf(a[i], a[i], fmaf(b[i], b[i], ss));
+          gz = fmaf(ga[i] * wa[i], a[i], fmaf(gb[i] * wb[i], b[i], gz));
         }
         ss = head_sum<LPH>(ss);
         gz = head_sum<LPH>(gz);
-        const float r = rsqrtf(ss / (float)p.D + p.eps);
-        const float m = gz * r * r / (float)p.D;  // mean(g w u) / rms: times z it is u mean(g w u)
-        if (on) {
+        const float r = rsqrtf(fmaf(ss, p.inv_d, p.eps));
+        const float m = gz * p.inv_d * r * r * r;  // mean(g w u) / rms^2: times z it is u mean(g w u) / rms
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float ta = ga[i] * a[i] * r, tb = gb[i] * b[i] * r;
-            dw[0][i] += isq ? ta : 0.f;
-            dw[1][i] += isq ? 0.f : ta;
-            dw[0][4 + i] += isq ? tb : 0.f;
-            dw[1][4 + i] += isq ? 0.f : tb;
-            a[i] = r * (ga[i] * (isq ? w[0][i] : w[1][i]) - a[i] * m);
-            b[i] = r * (gb[i] * (isq ? w[0][4 + i] : w[1][4 + i]) - b[i] * m);
-          }
-          if (NORM == kAfter) rotate(a, b, cs, -1.f);
-          store_pairs<HALF>(dx + h * p.D, at, a, b);
+        for (int i = 0; i < 4; ++i) {
+          const float ta = ga[i] * r, tb = gb[i] * r;
+          da[i] = fmaf(ta, a[i], da[i]);
+          db[i] = fmaf(tb, b[i], db[i]);
+          a[i] = fmaf(ta, wa[i], -a[i] * m);
+          b[i] = fmaf(tb, wb[i], -b[i] * m);
         }
+        if (NORM == kAfter) rotate(a, b, cs, -1.f);
+        if (on) store_pairs<HALF>(dx + s * step, at, a, b);
       }
     }
   }
-  // lanes of the warp that hold the same channels, then the block's warps in order
-  __shared__ float red[8][2][256];
+  // lanes of the warp that hold the same channels, then the block's warps of each weight in order
+  __shared__ float red[16][256];
+  const int warp = threadIdx.y + threadIdx.z * blockDim.y;
 #pragma unroll
-  for (int k = 0; k < 2; ++k)
+  for (int i = 0; i < 4; ++i)
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
-#pragma unroll
-      for (int o = 16; o >= LPH; o >>= 1) dw[k][i] += __shfl_xor_sync(0xffffffff, dw[k][i], o);
+    for (int o = 16; o >= LPH; o >>= 1) {
+      da[i] += __shfl_xor_sync(0xffffffff, da[i], o);
+      db[i] += __shfl_xor_sync(0xffffffff, db[i], o);
+    }
   if (sub == 0 && at.on) {
 #pragma unroll
-    for (int k = 0; k < 2; ++k)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int ca = HALF ? at.c0 + i : at.c0 + 2 * i, cb = HALF ? at.c1 + i : at.c0 + 2 * i + 1;
-        red[warp][k][ca] = dw[k][i];
-        red[warp][k][cb] = dw[k][4 + i];
-      }
+    for (int i = 0; i < 4; ++i) {
+      red[warp][HALF ? at.c0 + i : at.c0 + 2 * i] = da[i];
+      red[warp][HALF ? at.c1 + i : at.c0 + 2 * i + 1] = db[i];
+    }
   }
   __syncthreads();
-  for (int c = threadIdx.x; c < 2 * p.D; c += 256) {
-    const int k = c >= p.D, ch = c - k * p.D;
+  const int warps = blockDim.y * blockDim.z;
+  for (int c = warp * 32 + lane; c < 2 * p.D; c += warps * 32) {
+    const bool key = c >= p.D;
     float s = 0.f;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) s += red[i][k][ch];
+    for (int z = 0; z < blockDim.z; ++z)
+      for (int w = key ? p.q_parts : 0; w < (key ? (int)blockDim.y : p.q_parts); ++w)
+        s += red[z * blockDim.y + w][c - key * p.D];
     p.dw_part[(long long)blockIdx.x * 2 * p.D + c] = s;
   }
 }
 
 // dw[c] = sum over blocks of part[block][c], c over both weights: 8 columns (one sector of each
-// partial row) per CTA, 32 rows of threads, then a tree through shared memory.
+// partial row) per CTA, 32 rows of threads.
 template <typename T>
 __global__ void __launch_bounds__(256) qk_norm_dw_kernel(const float* __restrict__ part, int blocks, int D,
                                                          T* __restrict__ dwq, T* __restrict__ dwk) {
-  __shared__ float s[32][9];
+  __shared__ float s[8][8];
   const int tx = threadIdx.x & 7, ty = threadIdx.x >> 3;
   const int c = blockIdx.x * 8 + tx;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   float a = 0.f;
-#pragma unroll 4
+#pragma unroll 10
   for (int b = ty; b < blocks; b += 32) a += part[(long long)b * 2 * D + c];
-  s[ty][tx] = a;
+  a += __shfl_xor_sync(0xffffffff, a, 8);
+  a += __shfl_xor_sync(0xffffffff, a, 16);
+  if ((threadIdx.x & 31) < 8) s[threadIdx.x >> 5][tx] = a;
   __syncthreads();
+  if (threadIdx.x < 8) {
+    float t = 0.f;
 #pragma unroll
-  for (int h = 16; h > 0; h >>= 1) {
-    if (ty < h) s[ty][tx] += s[ty + h][tx];
-    __syncthreads();
-  }
-  if (ty == 0) {
+    for (int i = 0; i < 8; ++i) t += s[i][tx];
     T* o = c < D ? dwq + c : dwk + (c - D);
-    *o = round_to<T>(s[0][tx]);
+    *o = round_to<T>(t);
   }
 }
 
-template <typename T, bool HALF, int NORM>
-void launch_fwd(const QkNormParams& p, int lph, int blocks, cudaStream_t s) {
-  switch (lph) {
-    case 8: (note_launch(), qk_norm_fwd_kernel<T, 8, HALF, NORM><<<blocks, 256, 0, s>>>(p)); break;
-    case 16: (note_launch(), qk_norm_fwd_kernel<T, 16, HALF, NORM><<<blocks, 256, 0, s>>>(p)); break;
-    default: (note_launch(), qk_norm_fwd_kernel<T, 32, HALF, NORM><<<blocks, 256, 0, s>>>(p)); break;
-  }
+template <typename T, int LPH, bool HALF, int NORM>
+void launch_fwd(const QkNormParams& p, int blocks, dim3 block, cudaStream_t s) {
+  if (p.D == 8 * LPH) (note_launch(), qk_norm_fwd_kernel<T, LPH, HALF, NORM, true><<<blocks, block, 0, s>>>(p));
+  else (note_launch(), qk_norm_fwd_kernel<T, LPH, HALF, NORM, false><<<blocks, block, 0, s>>>(p));
+}
+template <typename T, int LPH, bool HALF, int NORM>
+void launch_bwd(const QkNormParams& p, int blocks, dim3 block, cudaStream_t s) {
+  if (p.D == 8 * LPH) (note_launch(), qk_norm_bwd_kernel<T, LPH, HALF, NORM, true><<<blocks, block, 0, s>>>(p));
+  else (note_launch(), qk_norm_bwd_kernel<T, LPH, HALF, NORM, false><<<blocks, block, 0, s>>>(p));
 }
 template <typename T, bool HALF, int NORM>
-void launch_bwd(const QkNormParams& p, int lph, int blocks, cudaStream_t s) {
-  switch (lph) {
-    case 8: (note_launch(), qk_norm_bwd_kernel<T, 8, HALF, NORM><<<blocks, 256, 0, s>>>(p)); break;
-    case 16: (note_launch(), qk_norm_bwd_kernel<T, 16, HALF, NORM><<<blocks, 256, 0, s>>>(p)); break;
-    default: (note_launch(), qk_norm_bwd_kernel<T, 32, HALF, NORM><<<blocks, 256, 0, s>>>(p)); break;
+void fwd_heads(const QkNormParams& p, int lph, int blocks, dim3 block, cudaStream_t s) {
+  if (lph == 8) launch_fwd<T, 8, HALF, NORM>(p, blocks, block, s);
+  else if (lph == 16) launch_fwd<T, 16, HALF, NORM>(p, blocks, block, s);
+  else launch_fwd<T, 32, HALF, NORM>(p, blocks, block, s);
+}
+template <typename T, bool HALF, int NORM>
+void bwd_heads(const QkNormParams& p, int lph, int blocks, dim3 block, cudaStream_t s) {
+  if (lph == 8) launch_bwd<T, 8, HALF, NORM>(p, blocks, block, s);
+  else if (lph == 16) launch_bwd<T, 16, HALF, NORM>(p, blocks, block, s);
+  else launch_bwd<T, 32, HALF, NORM>(p, blocks, block, s);
+}
+template <typename T>
+void fwd_typed(const QkNormParams& p, int lph, int blocks, dim3 block, bool half_layout, int norm, cudaStream_t s) {
+  if (half_layout) {
+    if (norm == kNone) fwd_heads<T, true, kNone>(p, lph, blocks, block, s);
+    else if (norm == kAfter) fwd_heads<T, true, kAfter>(p, lph, blocks, block, s);
+    else fwd_heads<T, true, kBefore>(p, lph, blocks, block, s);
+  } else {
+    if (norm == kNone) fwd_heads<T, false, kNone>(p, lph, blocks, block, s);
+    else if (norm == kAfter) fwd_heads<T, false, kAfter>(p, lph, blocks, block, s);
+    else fwd_heads<T, false, kBefore>(p, lph, blocks, block, s);
   }
 }
 template <typename T>
-void fwd_typed(const QkNormParams& p, int lph, int blocks, bool half_layout, int norm, cudaStream_t s) {
+void bwd_typed(const QkNormParams& p, int lph, int blocks, dim3 block, bool half_layout, int norm, void* dwq,
+               void* dwk, cudaStream_t s) {
   if (half_layout) {
-    if (norm == kNone) launch_fwd<T, true, kNone>(p, lph, blocks, s);
-    else if (norm == kAfter) launch_fwd<T, true, kAfter>(p, lph, blocks, s);
-    else launch_fwd<T, true, kBefore>(p, lph, blocks, s);
+    if (norm == kAfter) bwd_heads<T, true, kAfter>(p, lph, blocks, block, s);
+    else bwd_heads<T, true, kBefore>(p, lph, blocks, block, s);
   } else {
-    if (norm == kNone) launch_fwd<T, false, kNone>(p, lph, blocks, s);
-    else if (norm == kAfter) launch_fwd<T, false, kAfter>(p, lph, blocks, s);
-    else launch_fwd<T, false, kBefore>(p, lph, blocks, s);
+    if (norm == kAfter) bwd_heads<T, false, kAfter>(p, lph, blocks, block, s);
+    else bwd_heads<T, false, kBefore>(p, lph, blocks, block, s);
   }
-}
-template <typename T>
-void bwd_typed(const QkNormParams& p, int lph, int blocks, bool half_layout, int norm, void* dwq, void* dwk,
-               cudaStream_t s) {
-  if (half_layout) {
-    if (norm == kAfter) launch_bwd<T, true, kAfter>(p, lph, blocks, s);
-    else launch_bwd<T, true, kBefore>(p, lph, blocks, s);
-  } else {
-    if (norm == kAfter) launch_bwd<T, false, kAfter>(p, lph, blocks, s);
-    else launch_bwd<T, false, kBefore>(p, lph, blocks, s);
-  }
-  (note_launch(), qk_norm_dw_kernel<T><<<2 * p.D / 8, 256, 0, s>>>(p.dw_part, blocks, p.D, static_cast<T*>(dwq),
-                                                                   static_cast<T*>(dwk)));
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(2 * p.D / 8);
+  cfg.blockDim = dim3(256);
+  cfg.stream = s;
+  cudaLaunchAttribute attr{};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  note_launch();
+  cudaLaunchKernelEx(&cfg, qk_norm_dw_kernel<T>, (const float*)p.dw_part, blocks, p.D, static_cast<T*>(dwq),
+                     static_cast<T*>(dwk));
 }
 
 int lanes_per_head(int D) { return D <= 64 ? 8 : D <= 128 ? 16 : 32; }
@@ -401,6 +441,16 @@ int lanes_per_head(int D) { return D <= 64 ? 8 : D <= 128 ? 16 : 32; }
 
 namespace astrai_host {
 
+// Warps per row and rows per block: a warp gets `steps` steps of heads of its kind, at most 12 warps a row.
+// A row's warps sit in one block, so its (cos, sin) pairs come from L2 once.
+static dim3 qk_norm_block(astrai::QkNormParams& p, int lph, int steps, int block_warps) {
+  const int hpw = 32 / lph;
+  const int sq = (p.hq + hpw - 1) / hpw, sk = (p.hkv + hpw - 1) / hpw;
+  p.q_parts = std::min(8, (sq + steps - 1) / steps);
+  const int k_parts = std::min(4, (sk + steps - 1) / steps), warps = p.q_parts + k_parts;
+  return dim3(32, warps, std::max(1, block_warps / warps));
+}
+
 // dtype: 0 bf16, 1 fp16, 2 fp32. norm: 0 none, 1 after the rotation, 2 before it.
 void qk_norm_fwd(const void* x, long long ldx, void* y, long long ldy, int rows, int hq, int hkv, int D,
                  const void* table, int max_pos, const int* pos, int seq_len, const void* wq, const void* wk, int rot,
@@ -408,38 +458,40 @@ void qk_norm_fwd(const void* x, long long ldx, void* y, long long ldy, int rows,
                  cudaStream_t s) {
   using namespace astrai;
   if (rows <= 0) return;
-  const int lph = lanes_per_head(D), steps = (hq + hkv + 32 / lph - 1) / (32 / lph);
   QkNormParams p{};
   p.x = x, p.out = y, p.ldx = ldx, p.ldo = ldy, p.wq = wq, p.wk = wk;
   p.table = static_cast<const float2*>(table), p.pos = pos, p.err = error_word(device);
-  p.rows = rows, p.hq = hq, p.heads = hq + hkv, p.D = D, p.rot = rot, p.rot_off = rot_off;
-  p.seq_len = seq_len, p.max_pos = max_pos, p.sign = inverse ? -1.f : 1.f, p.eps = eps;
-  p.parts = (steps + kUnroll - 1) / kUnroll;
-  const int blocks = (int)(((long long)rows * p.parts + 7) / 8);
-  if (dtype == 0) fwd_typed<__nv_bfloat16>(p, lph, blocks, half_layout, norm, s);
-  else if (dtype == 1) fwd_typed<__half>(p, lph, blocks, half_layout, norm, s);
-  else fwd_typed<float>(p, lph, blocks, half_layout, norm, s);
+  p.rows = rows, p.hq = hq, p.hkv = hkv, p.D = D, p.rot = rot, p.rot_off = rot_off;
+  p.seq_len = seq_len, p.max_pos = max_pos, p.sign = inverse ? -1.f : 1.f, p.eps = eps, p.inv_d = 1.f / D;
+  const int lph = lanes_per_head(D);
+  // few rows: one step per warp, for the shortest time; many: kFwdSteps, for the most loads in flight
+  const dim3 block = qk_norm_block(p, lph, rows <= num_sms(device) ? 1 : kFwdSteps, 8);
+  const int blocks = (rows + (int)block.z - 1) / (int)block.z;
+  if (dtype == 0) fwd_typed<__nv_bfloat16>(p, lph, blocks, block, half_layout, norm, s);
+  else if (dtype == 1) fwd_typed<__half>(p, lph, blocks, block, half_layout, norm, s);
+  else fwd_typed<float>(p, lph, blocks, block, half_layout, norm, s);
 }
 
 // Blocks of the backward launch, each with 2 * D floats of scratch.
-int qk_norm_bwd_blocks(int rows, int device) {
-  return std::max(1, std::min((rows + 7) / 8, num_sms(device) * 3));
-}
+int qk_norm_bwd_blocks(int rows, int device) { return std::max(1, std::min(rows, num_sms(device) * 2)); }
 
 void qk_norm_bwd(const void* dy, long long lddy, const void* x, long long ldx, void* dx, long long lddx, int rows,
                  int hq, int hkv, int D, const void* table, int max_pos, const int* pos, int seq_len, const void* wq,
                  const void* wk, int rot, int rot_off, bool half_layout, int norm, float eps, void* dwq, void* dwk,
                  float* scratch, int dtype, int device, cudaStream_t s) {
   using namespace astrai;
+  if (rows <= 0) return;
   QkNormParams p{};
   p.x = x, p.dy = dy, p.out = dx, p.ldx = ldx, p.lddy = lddy, p.ldo = lddx, p.wq = wq, p.wk = wk;
   p.table = static_cast<const float2*>(table), p.pos = pos, p.dw_part = scratch, p.err = error_word(device);
-  p.rows = rows, p.hq = hq, p.heads = hq + hkv, p.D = D, p.rot = rot, p.rot_off = rot_off;
-  p.seq_len = seq_len, p.max_pos = max_pos, p.sign = 1.f, p.eps = eps, p.parts = 1;
-  const int lph = lanes_per_head(D), blocks = qk_norm_bwd_blocks(rows, device);
-  if (dtype == 0) bwd_typed<__nv_bfloat16>(p, lph, blocks, half_layout, norm, dwq, dwk, s);
-  else if (dtype == 1) bwd_typed<__half>(p, lph, blocks, half_layout, norm, dwq, dwk, s);
-  else bwd_typed<float>(p, lph, blocks, half_layout, norm, dwq, dwk, s);
+  p.rows = rows, p.hq = hq, p.hkv = hkv, p.D = D, p.rot = rot, p.rot_off = rot_off;
+  p.seq_len = seq_len, p.max_pos = max_pos, p.sign = 1.f, p.eps = eps, p.inv_d = 1.f / D;
+  const int lph = lanes_per_head(D);
+  const dim3 block = qk_norm_block(p, lph, kBwdSteps, 12);
+  const int blocks = std::min(qk_norm_bwd_blocks(rows, device), (rows + (int)block.z - 1) / (int)block.z);
+  if (dtype == 0) bwd_typed<__nv_bfloat16>(p, lph, blocks, block, half_layout, norm, dwq, dwk, s);
+  else if (dtype == 1) bwd_typed<__half>(p, lph, blocks, block, half_layout, norm, dwq, dwk, s);
+  else bwd_typed<float>(p, lph, blocks, block, half_layout, norm, dwq, dwk, s);
 }
 
 }  // namespace astrai_host

@@ -57,18 +57,6 @@ class KV8(NamedTuple):
         return self.k.shape[2] // self.k_absmax.shape[2]
 
 
-def _i32(t: torch.Tensor) -> torch.Tensor:
-    return t if t.dtype == torch.int32 and t.is_contiguous() else t.to(torch.int32).contiguous()
-
-
-def _heads(t: torch.Tensor) -> torch.Tensor:
-    """[B, S, H, D] as the kernels read it (16-byte aligned rows of any stride), copied if it is not."""
-    if t.dim() == 4 and (t.stride(3) != 1 or t.data_ptr() % 16
-                         or any(t.shape[i] > 1 and t.stride(i) % 8 for i in range(3))):
-        return t.contiguous()
-    return t
-
-
 # ----------------------------------------------------------------------------- append
 def _append_reference(cache: KV8, k, v, page_table, starts, lens) -> None:
     block, page = cache.block, cache.page_size
@@ -108,11 +96,10 @@ def kv8_append(cache: KV8, k: torch.Tensor, v: torch.Tensor, page_table: torch.T
     that grew. Tokens whose page is missing are dropped. A block with an infinity or NaN among its new
     values reads as NaN.
     """
-    if not cache.k.is_cuda:
+    if cache.k.is_cuda:
+        native().kv8_append(k, v, *cache, page_table, starts, lens)
+    else:
         _append_reference(cache, k, v, page_table, starts, lens)
-        return
-    native().kv8_append(_heads(k), _heads(v), cache.k, cache.v, cache.k_absmax, cache.v_absmax, _i32(page_table),
-                        _i32(starts), _i32(lens))
 
 
 # ----------------------------------------------------------------------------- read-back
@@ -121,13 +108,9 @@ def kv8_gather(cache: KV8, page_table: torch.Tensor, lens: torch.Tensor, total: 
                ) -> Tuple[torch.Tensor, torch.Tensor]:
     """Values of tokens ``starts[b] .. starts[b] + total - 1`` (None: from 0) -> k, v
     ``[B, total, n_kv_heads, head_dim]``; zeros from ``lens[b]`` on and where a page is missing."""
-    B = page_table.shape[0]
-    shape = (B, int(total), cache.k.shape[1], cache.k.shape[3])
     if cache.k.is_cuda:
-        ko, vo = (torch.empty(shape, dtype=dtype, device=cache.k.device) for _ in range(2))
-        native().kv8_gather(cache.k, cache.v, cache.k_absmax, cache.v_absmax, _i32(page_table),
-                            None if starts is None else _i32(starts), _i32(lens), ko, vo)
-        return ko, vo
+        return native().kv8_gather(*cache, page_table, starts, lens, total, dtype)
+    B = page_table.shape[0]
     page, block = cache.page_size, cache.block
     pos = torch.arange(int(total)) + (0 if starts is None else starts.long()[:, None]) + torch.zeros(B, 1, dtype=torch.long)
     where = pos.clamp(min=0) // page
@@ -176,11 +159,7 @@ def kv8_attention(q: torch.Tensor, cache: KV8, page_table: torch.Tensor, lens: t
     sc = float(scale) if scale is not None else 1.0 / math.sqrt(q.shape[-1])
     if not cache.k.is_cuda:
         return _attention_reference(q, cache, page_table, lens, starts, sc)
-    q = _heads(q)
-    out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    native().kv8_attend(q, cache.k, cache.v, cache.k_absmax, cache.v_absmax, _i32(page_table), _i32(lens),
-                        None if starts is None else _i32(starts), out, workspace, sc)
-    return out
+    return native().kv8_attend(q, *cache, page_table, lens, starts, workspace, sc)
 
 
 def kv8_attention_workspace(batch: int, tokens: int, n_heads: int, cache: KV8, max_pages: int) -> int:

@@ -66,56 +66,6 @@ def qk_norm_rope_reference(x, n_heads, n_kv_heads, head_dim, table, q_weight=Non
     return z.reshape(-1, H * head_dim).to(x.dtype)
 
 
-def _rows(t: torch.Tensor) -> torch.Tensor:
-    """A row view that the kernels can read (unit inner stride, 16-byte aligned rows), copied if it is none."""
-    if t.stride(1) != 1 or (t.stride(0) * t.element_size()) % 16 or t.data_ptr() % 16:
-        return t.contiguous()
-    return t
-
-
-def qk_norm_backward(dy, x, dx, n_heads, n_kv_heads, head_dim, table, q_weight, k_weight, positions, seq_len, eps,
-                     half, mode, rot_dim, rot_off):
-    """Backward kernels on row buffers: fills the q and k columns of ``dx``; -> (dq_weight, dk_weight)."""
-    C = native()
-    if mode == 0:  # the transposed rotation
-        C.qk_norm_fwd(dy, dx, n_heads, n_kv_heads, head_dim, table, positions, seq_len, None, None, rot_dim, rot_off,
-                      half, 0, True, eps)
-        return None, None
-    dwq, dwk = torch.empty_like(q_weight), torch.empty_like(k_weight)
-    scratch = torch.empty(C.qk_norm_bwd_scratch(x.shape[0], head_dim, x.device.index), device=x.device,
-                          dtype=torch.float32)
-    if x.shape[0] == 0:
-        return dwq.zero_(), dwk.zero_()
-    C.qk_norm_bwd(dy, x, dx, n_heads, n_kv_heads, head_dim, table, positions, seq_len, q_weight, k_weight, rot_dim,
-                  rot_off, half, mode, eps, dwq, dwk, scratch)
-    return dwq, dwk
-
-
-class _QKNormRopeFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, q_weight, k_weight, table, positions, dims):
-        hq, hkv, D, seq_len, eps, half, mode, rot, off = dims
-        y = torch.empty((x.shape[0], (hq + hkv) * D), device=x.device, dtype=x.dtype)
-        xr = _rows(x)
-        native().qk_norm_fwd(xr, y, hq, hkv, D, table, positions, seq_len, q_weight, k_weight, rot, off, half, mode,
-                             False, eps)
-        ctx.save_for_backward(xr, q_weight, k_weight, table, positions)
-        ctx.dims, ctx.width = dims, x.shape[1]
-        return y
-
-    @staticmethod
-    def backward(ctx, dy):
-        x, q_weight, k_weight, table, positions = ctx.saved_tensors
-        hq, hkv, D, seq_len, eps, half, mode, rot, off = ctx.dims
-        used = (hq + hkv) * D
-        dx = torch.empty((x.shape[0], ctx.width), device=x.device, dtype=x.dtype)
-        if ctx.width > used:  # columns behind the keys are not an input
-            dx[:, used:].zero_()
-        dwq, dwk = qk_norm_backward(_rows(dy), x, dx, hq, hkv, D, table, q_weight, k_weight, positions, seq_len, eps,
-                                    half, mode, rot, off)
-        return dx, dwq, dwk, None, None, None
-
-
 def _check(x, n_heads, n_kv_heads, head_dim, table, q_weight, k_weight, positions, seq_len, layout, norm, rot, off):
     if layout not in LAYOUTS:
         raise ValueError(f"layout must be one of {LAYOUTS}, got {layout!r}")
@@ -136,12 +86,16 @@ def _check(x, n_heads, n_kv_heads, head_dim, table, q_weight, k_weight, position
         raise ValueError(f"positions must have one entry per row ({x.shape[0]}), got {positions.numel()}")
 
 
-def _kernel_positions(positions: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
-    if positions is None:
-        return None
-    if positions.dtype == torch.int32 and positions.dim() == 1 and positions.is_contiguous():
-        return positions
-    return positions.reshape(-1).to(torch.int32).contiguous()
+def _native(x, n_heads, n_kv_heads, head_dim, table, q_weight, k_weight, positions, seq_len, eps, layout, norm, rot, off,
+            in_place):
+    """The kernels' call; it checks its arguments itself (csrc/bind_qk_norm.cpp)."""
+    mode = NORM_MODES.get(norm)
+    if mode is None:
+        raise ValueError(f"norm must be one of {tuple(NORM_MODES)}, got {norm!r}")
+    if layout not in LAYOUTS:
+        raise ValueError(f"layout must be one of {LAYOUTS}, got {layout!r}")
+    return native().qk_norm_rope(x, n_heads, n_kv_heads, head_dim, table, q_weight, k_weight, positions, seq_len or 0,
+                                 eps, layout == "half", mode, rot, off, in_place)
 
 
 def qk_norm_rope(x: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: int, table: torch.Tensor,
@@ -160,22 +114,12 @@ def qk_norm_rope(x: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: int, 
     weights.
     """
     rot = head_dim if rot_dim is None else rot_dim
+    if x.is_cuda:
+        return _native(x, n_heads, n_kv_heads, head_dim, table, q_weight, k_weight, positions, seq_len, eps, layout, norm,
+                       rot, rot_off, False)
     _check(x, n_heads, n_kv_heads, head_dim, table, q_weight, k_weight, positions, seq_len, layout, norm, rot, rot_off)
-    if not x.is_cuda:
-        return qk_norm_rope_reference(x, n_heads, n_kv_heads, head_dim, table, q_weight, k_weight, positions, seq_len,
-                                      eps, layout, norm, rot, rot_off)
-    if norm == "none":
-        q_weight = k_weight = None
-    pos = _kernel_positions(positions)
-    dims = (n_heads, n_kv_heads, head_dim, int(seq_len or 0), float(eps), layout == "half", NORM_MODES[norm], rot,
-            rot_off)
-    if torch.is_grad_enabled() and (x.requires_grad or (q_weight is not None and (q_weight.requires_grad
-                                                                                 or k_weight.requires_grad))):
-        return _QKNormRopeFn.apply(x, q_weight, k_weight, table, pos, dims)
-    y = torch.empty((x.shape[0], (n_heads + n_kv_heads) * head_dim), device=x.device, dtype=x.dtype)
-    native().qk_norm_fwd(_rows(x), y, n_heads, n_kv_heads, head_dim, table, pos, dims[3], q_weight, k_weight, rot,
-                         rot_off, dims[5], dims[6], False, dims[4])
-    return y
+    return qk_norm_rope_reference(x, n_heads, n_kv_heads, head_dim, table, q_weight, k_weight, positions, seq_len, eps,
+                                  layout, norm, rot, rot_off)
 
 
 def qk_norm_rope_(x: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: int, table: torch.Tensor,
@@ -185,16 +129,12 @@ def qk_norm_rope_(x: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: int,
                   rot_off: int = 0) -> torch.Tensor:
     """:func:`qk_norm_rope` in place on the query and key columns of ``x`` (no gradient) -> ``x``."""
     rot = head_dim if rot_dim is None else rot_dim
+    if x.is_cuda:
+        return _native(x, n_heads, n_kv_heads, head_dim, table, q_weight, k_weight, positions, seq_len, eps, layout, norm,
+                       rot, rot_off, True)
     _check(x, n_heads, n_kv_heads, head_dim, table, q_weight, k_weight, positions, seq_len, layout, norm, rot, rot_off)
     if torch.is_grad_enabled() and x.requires_grad:
         raise RuntimeError("qk_norm_rope_ has no gradient: use qk_norm_rope")
-    if not x.is_cuda:
-        x[:, : (n_heads + n_kv_heads) * head_dim] = qk_norm_rope_reference(
-            x, n_heads, n_kv_heads, head_dim, table, q_weight, k_weight, positions, seq_len, eps, layout, norm, rot,
-            rot_off)
-        return x
-    if norm == "none":
-        q_weight = k_weight = None
-    native().qk_norm_fwd(x, x, n_heads, n_kv_heads, head_dim, table, _kernel_positions(positions), int(seq_len or 0),
-                         q_weight, k_weight, rot, rot_off, layout == "half", NORM_MODES[norm], False, float(eps))
+    x[:, : (n_heads + n_kv_heads) * head_dim] = qk_norm_rope_reference(
+        x, n_heads, n_kv_heads, head_dim, table, q_weight, k_weight, positions, seq_len, eps, layout, norm, rot, rot_off)
     return x
