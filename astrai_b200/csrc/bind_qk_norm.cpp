@@ -11,7 +11,7 @@ void qk_norm_fwd(const void* x, long long ldx, void* y, long long ldy, int rows,
                  const void* table, int max_pos, const int* pos, int seq_len, const void* wq, const void* wk, int rot,
                  int rot_off, bool half_layout, int norm, int inverse, float eps, int dtype, int device,
                  cudaStream_t s);
-int qk_norm_bwd_blocks(int rows, int device);
+long long qk_norm_bwd_scratch(int rows, int heads, int D, int rot, int elem, int device);
 void qk_norm_bwd(const void* dy, long long lddy, const void* x, long long ldx, void* dx, long long lddx, int rows,
                  int hq, int hkv, int D, const void* table, int max_pos, const int* pos, int seq_len, const void* wq,
                  const void* wk, int rot, int rot_off, bool half_layout, int norm, float eps, void* dwq, void* dwk,
@@ -123,7 +123,8 @@ std::pair<at::Tensor, at::Tensor> backward_into(const at::Tensor& dy, const at::
   const c10::cuda::CUDAGuard g(x.device());
   if (s.rows == 0) return {at::zeros_like(*wq), at::zeros_like(*wk)};
   auto dwq = at::empty_like(*wq), dwk = at::empty_like(*wk);
-  auto scratch = at::empty({astrai_host::qk_norm_bwd_blocks(s.rows, s.device) * 2 * o.D}, x.options().dtype(at::kFloat));
+  auto scratch = at::empty({(int64_t)astrai_host::qk_norm_bwd_scratch(s.rows, s.hq + s.hkv, s.D, s.rot, (int)x.element_size(), s.device)},
+                           x.options().dtype(at::kFloat));
   astrai_host::qk_norm_bwd(dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0), dx.data_ptr(), dx.stride(0), s.rows,
                            s.hq, s.hkv, s.D, table.data_ptr(), s.max_pos, s.pos, (int)o.seq_len, wq->data_ptr(),
                            wk->data_ptr(), s.rot, s.rot_off, o.half_layout, (int)o.norm, (float)o.eps, dwq.data_ptr(),

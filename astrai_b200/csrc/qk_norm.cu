@@ -201,13 +201,55 @@ struct Share {
   }
 };
 
-constexpr int kFwdSteps = 4;  // steps of a warp whose loads are in flight together
-constexpr int kBwdSteps = 2;
+// One head in a lane group's registers, forward: z = the pairs (a, b), returned normalised and rotated.
+template <int LPH, int NORM>
+__device__ __forceinline__ void head_forward(float* a, float* b, const float2* cs, const float* wa, const float* wb,
+                                             const QkNormParams& p) {
+  if (NORM != kBefore) rotate(a, b, cs, p.sign);
+  if (NORM != kNone) {
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) ss = fmaf(a[i], a[i], fmaf(b[i], b[i], ss));
+    const float r = rsqrtf(fmaf(head_sum<LPH>(ss), p.inv_d, p.eps));
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] *= r * wa[i], b[i] *= r * wb[i];
+  }
+  if (NORM == kBefore) rotate(a, b, cs, p.sign);
+}
+// and backward: (a, b) of x and (ga, gb) of dy; (a, b) becomes dx, (da, db) gains g u
+template <int LPH, int NORM>
+__device__ __forceinline__ void head_backward(float* a, float* b, float* ga, float* gb, const float2* cs, const float* wa,
+                                              const float* wb, float* da, float* db, const QkNormParams& p) {
+  if (NORM == kAfter) rotate(a, b, cs, 1.f);
+  if (NORM == kBefore) rotate(ga, gb, cs, -1.f);
+  float ss = 0.f, gz = 0.f;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    ss = fmaf(a[i], a[i], fmaf(b[i], b[i], ss));
+    gz = fmaf(ga[i] * wa[i], a[i], fmaf(gb[i] * wb[i], b[i], gz));
+  }
+  ss = head_sum<LPH>(ss);
+  gz = head_sum<LPH>(gz);
+  const float r = rsqrtf(fmaf(ss, p.inv_d, p.eps));
+  const float m = gz * p.inv_d * r * r * r;  // mean(g w u) / rms^2: times z it is u mean(g w u) / rms
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float ta = ga[i] * r, tb = gb[i] * r;
+    da[i] = fmaf(ta, a[i], da[i]);
+    db[i] = fmaf(tb, b[i], db[i]);
+    a[i] = fmaf(ta, wa[i], -a[i] * m);
+    b[i] = fmaf(tb, wb[i], -b[i] * m);
+  }
+  if (NORM == kAfter) rotate(a, b, cs, -1.f);
+}
 
-// Block (32, warps per row, rows). FULL: every lane of a head has channels (D = 8 LPH).
+constexpr int kSteps = 4;  // steps of a warp whose loads are in flight together
+
+// Few rows: block (32, warps per row, rows), straight from global memory. FULL: every lane of a head has channels
+// (D = 8 LPH).
 template <typename T, int LPH, bool HALF, int NORM, bool FULL>
 __global__ void __launch_bounds__(384, 2) qk_norm_fwd_kernel(const QkNormParams p) {
-  constexpr int HPW = 32 / LPH, U = kFwdSteps;
+  constexpr int HPW = 32 / LPH, U = kSteps;
   const int lane = threadIdx.x, sub = lane / LPH;
   Place<HALF> at(lane % LPH, p);
   if (FULL) at.on = true;
@@ -240,91 +282,121 @@ __global__ void __launch_bounds__(384, 2) qk_norm_fwd_kernel(const QkNormParams 
 #pragma unroll
       for (int i = 0; i < 4; ++i) a[i] = b[i] = 0.f;
       if (on) to_pairs<HALF>(raw[u], a, b);
-      if (NORM != kBefore) rotate(a, b, cs, p.sign);
-      if (NORM != kNone) {
-        float ss = 0.f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) ss = fmaf(a[i], a[i], fmaf(b[i], b[i], ss));
-        const float r = rsqrtf(fmaf(head_sum<LPH>(ss), p.inv_d, p.eps));
-#pragma unroll
-        for (int i = 0; i < 4; ++i) a[i] *= r * wa[i], b[i] *= r * wb[i];
-      }
-      if (NORM == kBefore) rotate(a, b, cs, p.sign);
+      head_forward<LPH, NORM>(a, b, cs, wa, wb, p);
       if (on) store_pairs<HALF>(y + s * step, at, a, b);
     }
   }
 }
 
-// Backward: a block's rows are every (blocks * rows per block)-th; the sums of g u stay in registers and go to
-// the block's own row of dw_part, so the result does not depend on any order in time.
-template <typename T, int LPH, bool HALF, int NORM, bool FULL>
-__global__ void __launch_bounds__(384, sizeof(T) == 4 ? 1 : 2) qk_norm_bwd_kernel(const QkNormParams p) {
-  constexpr int HPW = 32 / LPH, U = kBwdSteps;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the sum over blocks waits for this grid
-  const int lane = threadIdx.x, sub = lane / LPH;
+// Many rows, both directions: a producer warp keeps STAGES chunks of `chunk` rows (x, dy in the backward, and
+// their (cos, sin) rows) on their way into shared memory with bulk copies, so that the loads in flight do not
+// depend on registers or occupancy; the other warps take their heads of each row out of it. CTA c has the
+// chunks c, c + grid, ... In the backward the sums of g u stay in registers and go to the CTA's own row of dw_part,
+// so the result does not depend on any order in time.
+constexpr int kStages = 4;
+constexpr int kMaxWarps = 12;  // consumers
+constexpr int kRowsSmem = 100 * 1024;  // of which an SM holds two
+
+template <typename T, int LPH, bool HALF, int NORM, bool FULL, bool BWD>
+__global__ void __launch_bounds__(32 * (kMaxWarps + 1), 2) qk_norm_rows_kernel(const QkNormParams p, int chunk) {
+  constexpr int HPW = 32 / LPH;
+  extern __shared__ __align__(128) unsigned char smem[];
+  __shared__ uint64_t full[kStages], empty[kStages];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = (blockDim.x >> 5) - 1;
+  const int row_bytes = (p.hq + p.hkv) * p.D * (int)sizeof(T), cs_bytes = p.rot * 4;
+  const int per_row = row_bytes * (BWD ? 2 : 1) + cs_bytes, stage_bytes = per_row * chunk;
+  const int chunks = (p.rows + chunk - 1) / chunk;
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kStages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], warps);
+    }
+    fence_mbar_init();
+  }
+  if (BWD) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the sum over CTAs waits for this grid
+  __syncthreads();
+  float da[4], db[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) da[i] = db[i] = 0.f;
   Place<HALF> at(lane % LPH, p);
   if (FULL) at.on = true;
-  const Share sh(p, threadIdx.y, blockDim.y);
-  const int step = HPW * p.D;
-  float wa[4], wb[4], da[4], db[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) wa[i] = wb[i] = da[i] = db[i] = 0.f;
-  if (at.on) to_pairs<HALF>(load_raw<HALF>(static_cast<const T*>(sh.key ? p.wk : p.wq), at), wa, wb);
-  for (int row = blockIdx.x * blockDim.z + threadIdx.z; row < p.rows; row += gridDim.x * blockDim.z) {
-    const T* x = static_cast<const T*>(p.x) + (long long)row * p.ldx + sh.col0 + sub * p.D;
-    const T* dy = static_cast<const T*>(p.dy) + (long long)row * p.lddy + sh.col0 + sub * p.D;
-    T* dx = static_cast<T*>(p.out) + (long long)row * p.ldo + sh.col0 + sub * p.D;
-    float2 cs[4];
-    for (int s0 = sh.part; s0 * HPW < sh.heads; s0 += U * sh.stride) {
-      Raw8<T> rx[U], rg[U];
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int s = s0 + u * sh.stride;
-        if (s * HPW + sub < sh.heads && at.on) {
-          rx[u] = load_raw<HALF>(x + s * step, at);
-          rg[u] = load_raw<HALF>(dy + s * step, at);
-        }
+  const int sub = lane / LPH;
+
+  if (warp == warps) {  // producer: lane r copies row r of the chunk
+    int n = 0;
+    for (int c = blockIdx.x; c < chunks; c += gridDim.x, ++n) {
+      const int st = n % kStages, row = c * chunk + lane, live = min(chunk, p.rows - c * chunk);
+      int pos = 0;
+      if (lane < live) pos = p.pos ? p.pos[row] : row % p.seq_len;
+      const bool in_table = pos >= 0 && pos < p.max_pos;
+      if (n >= kStages && !mbar_wait(&empty[st], (n / kStages - 1) & 1, p.err, kErrWaitEmpty)) break;
+      unsigned char* at_row = smem + st * stage_bytes + lane * per_row;
+      if (lane < live && !in_table) {  // left unrotated
+        set_error(p.err, kErrBadArg);
+        for (int i = 0; i < p.rot / 2; ++i)
+          reinterpret_cast<float2*>(at_row + per_row - cs_bytes)[i] = make_float2(1.f, 0.f);
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before a later copy into the same place
       }
-      if (s0 == sh.part) load_cs<HALF>(p, row, at, cs);
-#pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int s = s0 + u * sh.stride;
-        if (s * HPW >= sh.heads) break;  // the same for the whole warp
-        const bool on = s * HPW + sub < sh.heads && at.on;
-        float a[4], b[4], ga[4], gb[4], ss = 0.f, gz = 0.f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) a[i] = b[i] = ga[i] = gb[i] = 0.f;
-        if (on) {
-          to_pairs<HALF>(rx[u], a, b);
-          to_pairs<HALF>(rg[u], ga, gb);
-        }
-        if (NORM == kAfter) rotate(a, b, cs, 1.f);
-        if (NORM == kBefore) rotate(ga, gb, cs, -1.f);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          ss = fmaf(a[i], a[i], fmaf(b[i], b[i], ss));
-          gz = fmaf(ga[i] * wa[i], a[i], fmaf(gb[i] * wb[i], b[i], gz));
-        }
-        ss = head_sum<LPH>(ss);
-        gz = head_sum<LPH>(gz);
-        const float r = rsqrtf(fmaf(ss, p.inv_d, p.eps));
-        const float m = gz * p.inv_d * r * r * r;  // mean(g w u) / rms^2: times z it is u mean(g w u) / rms
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float ta = ga[i] * r, tb = gb[i] * r;
-          da[i] = fmaf(ta, a[i], da[i]);
-          db[i] = fmaf(tb, b[i], db[i]);
-          a[i] = fmaf(ta, wa[i], -a[i] * m);
-          b[i] = fmaf(tb, wb[i], -b[i] * m);
-        }
-        if (NORM == kAfter) rotate(a, b, cs, -1.f);
-        if (on) store_pairs<HALF>(dx + s * step, at, a, b);
+      const int tables = __popc(__ballot_sync(0xffffffff, lane < live && in_table));
+      if (lane == 0) mbar_expect_tx(&full[st], live * (per_row - cs_bytes) + tables * cs_bytes);
+      __syncwarp();
+      if (lane < live) {
+        bulk_load(at_row, static_cast<const T*>(p.x) + (long long)row * p.ldx, row_bytes, &full[st]);
+        if (BWD)
+          bulk_load(at_row + row_bytes, static_cast<const T*>(p.dy) + (long long)row * p.lddy, row_bytes, &full[st]);
+        if (in_table)
+          bulk_load(at_row + per_row - cs_bytes, p.table + (long long)pos * (p.rot / 2), cs_bytes, &full[st]);
       }
     }
+  } else {
+    const Share sh(p, warp, warps);
+    float wa[4], wb[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) wa[i] = wb[i] = 0.f;
+    if (NORM != kNone && at.on)
+      to_pairs<HALF>(load_raw<HALF>(static_cast<const T*>(sh.key ? p.wk : p.wq), at), wa, wb);
+    const int step = HPW * p.D, col = sh.col0 + sub * p.D;
+    int n = 0;
+    for (int c = blockIdx.x; c < chunks; c += gridDim.x, ++n) {
+      const int st = n % kStages, live = min(chunk, p.rows - c * chunk);
+      if (!mbar_wait(&full[st], (n / kStages) & 1, p.err, kErrWaitFull)) break;
+      const unsigned char* src = smem + st * stage_bytes;
+      T* out = static_cast<T*>(p.out) + (long long)c * chunk * p.ldo + col;
+      for (int r = 0; r < live; ++r, src += per_row, out += p.ldo) {
+        float2 cs[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) cs[i] = make_float2(1.f, 0.f);
+        if (at.on && at.cs >= 0) {
+          const float4* q = reinterpret_cast<const float4*>(src + per_row - cs_bytes + at.cs * 8);
+          const float4 u = q[0], v = q[1];
+          cs[0] = make_float2(u.x, u.y), cs[1] = make_float2(u.z, u.w);
+          cs[2] = make_float2(v.x, v.y), cs[3] = make_float2(v.z, v.w);
+        }
+        const T* x = reinterpret_cast<const T*>(src) + col;
+        const T* dy = reinterpret_cast<const T*>(src + row_bytes) + col;
+        for (int s = sh.part; s * HPW < sh.heads; s += sh.stride) {
+          const bool on = s * HPW + sub < sh.heads && at.on;
+          float a[4], b[4], ga[4], gb[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) a[i] = b[i] = ga[i] = gb[i] = 0.f;
+          if (on) to_pairs<HALF>(load_raw<HALF>(x + s * step, at), a, b);
+          if (BWD) {
+            if (on) to_pairs<HALF>(load_raw<HALF>(dy + s * step, at), ga, gb);
+            head_backward<LPH, NORM>(a, b, ga, gb, cs, wa, wb, da, db, p);
+          } else {
+            head_forward<LPH, NORM>(a, b, cs, wa, wb, p);
+          }
+          if (on) store_pairs<HALF>(out + s * step, at, a, b);
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&empty[st]);
+    }
   }
-  // lanes of the warp that hold the same channels, then the block's warps of each weight in order
-  __shared__ float red[16][256];
-  const int warp = threadIdx.y + threadIdx.z * blockDim.y;
+  if (!BWD) return;
+  // lanes of a warp that hold the same channels, then the CTA's warps of each weight in order
+  __syncthreads();
+  float* red = reinterpret_cast<float*>(smem);  // [warp][D]; every copy has been waited for
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
@@ -332,21 +404,18 @@ __global__ void __launch_bounds__(384, sizeof(T) == 4 ? 1 : 2) qk_norm_bwd_kerne
       da[i] += __shfl_xor_sync(0xffffffff, da[i], o);
       db[i] += __shfl_xor_sync(0xffffffff, db[i], o);
     }
-  if (sub == 0 && at.on) {
+  if (warp < warps && sub == 0 && at.on) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      red[warp][HALF ? at.c0 + i : at.c0 + 2 * i] = da[i];
-      red[warp][HALF ? at.c1 + i : at.c0 + 2 * i + 1] = db[i];
+      red[warp * p.D + (HALF ? at.c0 + i : at.c0 + 2 * i)] = da[i];
+      red[warp * p.D + (HALF ? at.c1 + i : at.c0 + 2 * i + 1)] = db[i];
     }
   }
   __syncthreads();
-  const int warps = blockDim.y * blockDim.z;
-  for (int c = warp * 32 + lane; c < 2 * p.D; c += warps * 32) {
+  for (int c = threadIdx.x; c < 2 * p.D; c += blockDim.x) {
     const bool key = c >= p.D;
     float s = 0.f;
-    for (int z = 0; z < blockDim.z; ++z)
-      for (int w = key ? p.q_parts : 0; w < (key ? (int)blockDim.y : p.q_parts); ++w)
-        s += red[z * blockDim.y + w][c - key * p.D];
+    for (int w = key ? p.q_parts : 0; w < (key ? warps : p.q_parts); ++w) s += red[w * p.D + c - key * p.D];
     p.dw_part[(long long)blockIdx.x * 2 * p.D + c] = s;
   }
 }
@@ -376,50 +445,69 @@ __global__ void __launch_bounds__(256) qk_norm_dw_kernel(const float* __restrict
   }
 }
 
-template <typename T, int LPH, bool HALF, int NORM>
-void launch_fwd(const QkNormParams& p, int blocks, dim3 block, cudaStream_t s) {
-  if (p.D == 8 * LPH) (note_launch(), qk_norm_fwd_kernel<T, LPH, HALF, NORM, true><<<blocks, block, 0, s>>>(p));
-  else (note_launch(), qk_norm_fwd_kernel<T, LPH, HALF, NORM, false><<<blocks, block, 0, s>>>(p));
+// How a call runs. chunk 0: qk_norm_fwd_kernel with `block`; else qk_norm_rows_kernel.
+struct Launch {
+  int lph, blocks, chunk, smem;
+  dim3 block;
+};
+
+template <typename K>
+void allow_smem(K kernel, int smem, bool* set) {  // the attribute belongs to the device that is current
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (dev >= 0 && dev < 64 && set[dev]) return;
+  cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  if (dev >= 0 && dev < 64) set[dev] = true;
 }
-template <typename T, int LPH, bool HALF, int NORM>
-void launch_bwd(const QkNormParams& p, int blocks, dim3 block, cudaStream_t s) {
-  if (p.D == 8 * LPH) (note_launch(), qk_norm_bwd_kernel<T, LPH, HALF, NORM, true><<<blocks, block, 0, s>>>(p));
-  else (note_launch(), qk_norm_bwd_kernel<T, LPH, HALF, NORM, false><<<blocks, block, 0, s>>>(p));
+template <typename T, int LPH, bool HALF, int NORM, bool FULL>
+void launch_fwd(const QkNormParams& p, const Launch& l, cudaStream_t s) {
+  if (l.chunk == 0) {
+    (note_launch(), qk_norm_fwd_kernel<T, LPH, HALF, NORM, FULL><<<l.blocks, l.block, 0, s>>>(p));
+    return;
+  }
+  auto kernel = qk_norm_rows_kernel<T, LPH, HALF, NORM, FULL, false>;
+  static bool set[64] = {};
+  allow_smem(kernel, kRowsSmem, set);
+  (note_launch(), kernel<<<l.blocks, l.block, l.smem, s>>>(p, l.chunk));
 }
-template <typename T, bool HALF, int NORM>
-void fwd_heads(const QkNormParams& p, int lph, int blocks, dim3 block, cudaStream_t s) {
-  if (lph == 8) launch_fwd<T, 8, HALF, NORM>(p, blocks, block, s);
-  else if (lph == 16) launch_fwd<T, 16, HALF, NORM>(p, blocks, block, s);
-  else launch_fwd<T, 32, HALF, NORM>(p, blocks, block, s);
+template <typename T, int LPH, bool HALF, int NORM, bool FULL>
+void launch_bwd(const QkNormParams& p, const Launch& l, cudaStream_t s) {
+  auto kernel = qk_norm_rows_kernel<T, LPH, HALF, NORM, FULL, true>;
+  static bool set[64] = {};
+  allow_smem(kernel, kRowsSmem, set);
+  (note_launch(), kernel<<<l.blocks, l.block, l.smem, s>>>(p, l.chunk));
 }
-template <typename T, bool HALF, int NORM>
-void bwd_heads(const QkNormParams& p, int lph, int blocks, dim3 block, cudaStream_t s) {
-  if (lph == 8) launch_bwd<T, 8, HALF, NORM>(p, blocks, block, s);
-  else if (lph == 16) launch_bwd<T, 16, HALF, NORM>(p, blocks, block, s);
-  else launch_bwd<T, 32, HALF, NORM>(p, blocks, block, s);
+template <typename T, bool HALF, int NORM, bool BWD>
+void by_heads(const QkNormParams& p, const Launch& l, cudaStream_t s) {
+#define ASTRAI_QK_HEADS(LPH)                                                                  \
+  if (BWD) {                                                                                  \
+    if constexpr (NORM != kNone) {                                                            \
+      if (p.D == 8 * LPH) launch_bwd<T, LPH, HALF, NORM, true>(p, l, s);                      \
+      else launch_bwd<T, LPH, HALF, NORM, false>(p, l, s);                                    \
+    }                                                                                         \
+  } else {                                                                                    \
+    if (p.D == 8 * LPH) launch_fwd<T, LPH, HALF, NORM, true>(p, l, s);                        \
+    else launch_fwd<T, LPH, HALF, NORM, false>(p, l, s);                                      \
+  }
+  if (l.lph == 8) { ASTRAI_QK_HEADS(8) }
+  else if (l.lph == 16) { ASTRAI_QK_HEADS(16) }
+  else { ASTRAI_QK_HEADS(32) }
+#undef ASTRAI_QK_HEADS
 }
-template <typename T>
-void fwd_typed(const QkNormParams& p, int lph, int blocks, dim3 block, bool half_layout, int norm, cudaStream_t s) {
+template <typename T, bool BWD>
+void by_mode(const QkNormParams& p, const Launch& l, bool half_layout, int norm, cudaStream_t s) {
   if (half_layout) {
-    if (norm == kNone) fwd_heads<T, true, kNone>(p, lph, blocks, block, s);
-    else if (norm == kAfter) fwd_heads<T, true, kAfter>(p, lph, blocks, block, s);
-    else fwd_heads<T, true, kBefore>(p, lph, blocks, block, s);
+    if (norm == kNone) by_heads<T, true, kNone, BWD>(p, l, s);
+    else if (norm == kAfter) by_heads<T, true, kAfter, BWD>(p, l, s);
+    else by_heads<T, true, kBefore, BWD>(p, l, s);
   } else {
-    if (norm == kNone) fwd_heads<T, false, kNone>(p, lph, blocks, block, s);
-    else if (norm == kAfter) fwd_heads<T, false, kAfter>(p, lph, blocks, block, s);
-    else fwd_heads<T, false, kBefore>(p, lph, blocks, block, s);
+    if (norm == kNone) by_heads<T, false, kNone, BWD>(p, l, s);
+    else if (norm == kAfter) by_heads<T, false, kAfter, BWD>(p, l, s);
+    else by_heads<T, false, kBefore, BWD>(p, l, s);
   }
 }
 template <typename T>
-void bwd_typed(const QkNormParams& p, int lph, int blocks, dim3 block, bool half_layout, int norm, void* dwq,
-               void* dwk, cudaStream_t s) {
-  if (half_layout) {
-    if (norm == kAfter) bwd_heads<T, true, kAfter>(p, lph, blocks, block, s);
-    else bwd_heads<T, true, kBefore>(p, lph, blocks, block, s);
-  } else {
-    if (norm == kAfter) bwd_heads<T, false, kAfter>(p, lph, blocks, block, s);
-    else bwd_heads<T, false, kBefore>(p, lph, blocks, block, s);
-  }
+void sum_dw(const QkNormParams& p, int blocks, void* dwq, void* dwk, cudaStream_t s) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(2 * p.D / 8);
   cfg.blockDim = dim3(256);
@@ -434,22 +522,68 @@ void bwd_typed(const QkNormParams& p, int lph, int blocks, dim3 block, bool half
                      static_cast<T*>(dwk));
 }
 
-int lanes_per_head(int D) { return D <= 64 ? 8 : D <= 128 ? 16 : 32; }
-
 }  // namespace
 }  // namespace astrai
 
 namespace astrai_host {
 
-// Warps per row and rows per block: a warp gets `steps` steps of heads of its kind, at most 12 warps a row.
-// A row's warps sit in one block, so its (cos, sin) pairs come from L2 once.
-static dim3 qk_norm_block(astrai::QkNormParams& p, int lph, int steps, int block_warps) {
-  const int hpw = 32 / lph;
-  const int sq = (p.hq + hpw - 1) / hpw, sk = (p.hkv + hpw - 1) / hpw;
-  p.q_parts = std::min(8, (sq + steps - 1) / steps);
-  const int k_parts = std::min(4, (sk + steps - 1) / steps), warps = p.q_parts + k_parts;
-  return dim3(32, warps, std::max(1, block_warps / warps));
+namespace {
+
+int lanes_per_head(int D) { return D <= 64 ? 8 : D <= 128 ? 16 : 32; }
+
+// Few rows: one step per warp at most 12 warps a row. A row's warps sit in one block, so its (cos, sin) pairs
+// come from L2 once.
+astrai::Launch few_rows(astrai::QkNormParams& p) {
+  astrai::Launch l{};
+  l.lph = lanes_per_head(p.D);
+  const int hpw = 32 / l.lph, sq = (p.hq + hpw - 1) / hpw, sk = (p.hkv + hpw - 1) / hpw;
+  p.q_parts = std::min(8, sq);
+  const int warps = p.q_parts + std::min(4, sk);
+  l.block = dim3(32, warps, std::max(1, 8 / warps));
+  l.blocks = (p.rows + (int)l.block.z - 1) / (int)l.block.z;
+  return l;
 }
+
+// Heads of a row that qk_norm_rows_kernel can take at a time: kStages of them fit half an SM's shared memory.
+int heads_that_fit(int D, int rot, int elem, bool bwd) {
+  return (astrai::kRowsSmem / astrai::kStages - rot * 4) / (D * elem * (bwd ? 2 : 1));
+}
+int launches_of_rows(int heads, int D, int rot, int elem, bool bwd) {
+  const int n = heads_that_fit(D, rot, elem, bwd);
+  return (heads + n - 1) / n;
+}
+
+// Many rows: consumer warps in the ratio of query to key heads, chunks of at most 4 rows (more even shares).
+astrai::Launch many_rows(astrai::QkNormParams& p, int elem, bool bwd, int sms) {
+  using namespace astrai;
+  Launch l{};
+  l.lph = lanes_per_head(p.D);
+  const int hpw = 32 / l.lph, sq = (p.hq + hpw - 1) / hpw, sk = (p.hkv + hpw - 1) / hpw;
+  int turns = 1;  // steps of a warp per row
+  while ((sq + turns - 1) / turns + (sk + turns - 1) / turns > kMaxWarps) ++turns;
+  p.q_parts = (sq + turns - 1) / turns;
+  const int warps = p.q_parts + (sk + turns - 1) / turns;
+  const int per_row = (p.hq + p.hkv) * p.D * elem * (bwd ? 2 : 1) + p.rot * 4;
+  l.chunk = std::min(std::min(4, (p.rows + 2 * sms - 1) / (2 * sms)), kRowsSmem / (kStages * per_row));
+  l.smem = std::max(per_row * l.chunk * kStages, bwd ? warps * p.D * 4 : 0);
+  l.block = dim3(32 * (warps + 1));
+  l.blocks = std::min(2 * sms, (p.rows + l.chunk - 1) / l.chunk);
+  return l;
+}
+
+// The heads [h0, h0 + n) of a call as a call of its own.
+astrai::QkNormParams some_heads(const astrai::QkNormParams& p, int h0, int n, int elem) {
+  astrai::QkNormParams r = p;
+  const long long off = (long long)h0 * p.D * elem;
+  r.x = static_cast<const char*>(p.x) + off;
+  if (p.dy) r.dy = static_cast<const char*>(p.dy) + off;
+  r.out = static_cast<char*>(p.out) + off;
+  r.hq = std::max(0, std::min(p.hq - h0, n));
+  r.hkv = n - r.hq;
+  return r;
+}
+
+}  // namespace
 
 // dtype: 0 bf16, 1 fp16, 2 fp32. norm: 0 none, 1 after the rotation, 2 before it.
 void qk_norm_fwd(const void* x, long long ldx, void* y, long long ldy, int rows, int hq, int hkv, int D,
@@ -463,17 +597,29 @@ void qk_norm_fwd(const void* x, long long ldx, void* y, long long ldy, int rows,
   p.table = static_cast<const float2*>(table), p.pos = pos, p.err = error_word(device);
   p.rows = rows, p.hq = hq, p.hkv = hkv, p.D = D, p.rot = rot, p.rot_off = rot_off;
   p.seq_len = seq_len, p.max_pos = max_pos, p.sign = inverse ? -1.f : 1.f, p.eps = eps, p.inv_d = 1.f / D;
-  const int lph = lanes_per_head(D);
-  // few rows: one step per warp, for the shortest time; many: kFwdSteps, for the most loads in flight
-  const dim3 block = qk_norm_block(p, lph, rows <= num_sms(device) ? 1 : kFwdSteps, 8);
-  const int blocks = (rows + (int)block.z - 1) / (int)block.z;
-  if (dtype == 0) fwd_typed<__nv_bfloat16>(p, lph, blocks, block, half_layout, norm, s);
-  else if (dtype == 1) fwd_typed<__half>(p, lph, blocks, block, half_layout, norm, s);
-  else fwd_typed<float>(p, lph, blocks, block, half_layout, norm, s);
+  const int sms = num_sms(device), elem = dtype == 2 ? 4 : 2, heads = hq + hkv;
+  const auto run = [&](const QkNormParams& part, const Launch& l) {
+    if (dtype == 0) by_mode<__nv_bfloat16, false>(part, l, half_layout, norm, s);
+    else if (dtype == 1) by_mode<__half, false>(part, l, half_layout, norm, s);
+    else by_mode<float, false>(part, l, half_layout, norm, s);
+  };
+  if (rows <= 4 * sms) {
+    const Launch l = few_rows(p);
+    run(p, l);
+    return;
+  }
+  const int n = launches_of_rows(heads, D, rot, elem, false), per = (heads + n - 1) / n;
+  for (int h0 = 0; h0 < heads; h0 += per) {
+    QkNormParams part = some_heads(p, h0, std::min(per, heads - h0), elem);
+    const Launch l = many_rows(part, elem, false, sms);
+    run(part, l);
+  }
 }
 
-// Blocks of the backward launch, each with 2 * D floats of scratch.
-int qk_norm_bwd_blocks(int rows, int device) { return std::max(1, std::min(rows, num_sms(device) * 2)); }
+// fp32 elements of scratch that the backward needs: 2 * D for each CTA of each of its launches.
+long long qk_norm_bwd_scratch(int rows, int heads, int D, int rot, int elem, int device) {
+  return 2LL * D * std::min(rows, num_sms(device) * 2) * launches_of_rows(heads, D, rot, elem, true);
+}
 
 void qk_norm_bwd(const void* dy, long long lddy, const void* x, long long ldx, void* dx, long long lddx, int rows,
                  int hq, int hkv, int D, const void* table, int max_pos, const int* pos, int seq_len, const void* wq,
@@ -486,12 +632,21 @@ void qk_norm_bwd(const void* dy, long long lddy, const void* x, long long ldx, v
   p.table = static_cast<const float2*>(table), p.pos = pos, p.dw_part = scratch, p.err = error_word(device);
   p.rows = rows, p.hq = hq, p.hkv = hkv, p.D = D, p.rot = rot, p.rot_off = rot_off;
   p.seq_len = seq_len, p.max_pos = max_pos, p.sign = 1.f, p.eps = eps, p.inv_d = 1.f / D;
-  const int lph = lanes_per_head(D);
-  const dim3 block = qk_norm_block(p, lph, kBwdSteps, 12);
-  const int blocks = std::min(qk_norm_bwd_blocks(rows, device), (rows + (int)block.z - 1) / (int)block.z);
-  if (dtype == 0) bwd_typed<__nv_bfloat16>(p, lph, blocks, block, half_layout, norm, dwq, dwk, s);
-  else if (dtype == 1) bwd_typed<__half>(p, lph, blocks, block, half_layout, norm, dwq, dwk, s);
-  else bwd_typed<float>(p, lph, blocks, block, half_layout, norm, dwq, dwk, s);
+  const int sms = num_sms(device), elem = dtype == 2 ? 4 : 2, heads = hq + hkv;
+  const int n = launches_of_rows(heads, D, rot, elem, true), per = (heads + n - 1) / n;
+  int parts = 0;
+  for (int h0 = 0; h0 < heads; h0 += per) {
+    QkNormParams part = some_heads(p, h0, std::min(per, heads - h0), elem);
+    const Launch l = many_rows(part, elem, true, sms);
+    part.dw_part = scratch + 2LL * D * parts;
+    parts += l.blocks;
+    if (dtype == 0) by_mode<__nv_bfloat16, true>(part, l, half_layout, norm, s);
+    else if (dtype == 1) by_mode<__half, true>(part, l, half_layout, norm, s);
+    else by_mode<float, true>(part, l, half_layout, norm, s);
+  }
+  if (dtype == 0) sum_dw<__nv_bfloat16>(p, parts, dwq, dwk, s);
+  else if (dtype == 1) sum_dw<__half>(p, parts, dwq, dwk, s);
+  else sum_dw<float>(p, parts, dwq, dwk, s);
 }
 
 }  // namespace astrai_host

@@ -88,6 +88,8 @@ CASES = [
     (61, 61, 9, 2, 72, 8, 0, "interleaved", "none", torch.bfloat16),
     (61, 61, 9, 2, 40, 24, 8, "half", "none", torch.float32),
     (2500, 1250, 12, 4, 128, 128, 0, "interleaved", "after", torch.bfloat16),
+    (700, 350, 40, 8, 256, 128, 64, "half", "before", torch.float32),  # rows that take several launches
+    (1301, 77, 31, 9, 96, 96, 0, "interleaved", "before", torch.float16),
 ]
 
 
