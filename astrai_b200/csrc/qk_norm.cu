@@ -39,6 +39,7 @@ struct QkNormParams {
   int* err;
   int rows, hq, hkv, D, rot, rot_off, seq_len, max_pos;
   int q_parts;      // warps of a row that share its query heads; the others share its key heads
+  int warps_per_row, rows_at_once;  // of a CTA's consumers in qk_norm_rows_kernel
   float sign, eps, inv_d;
 };
 
@@ -48,34 +49,51 @@ __device__ __forceinline__ T round_to(float x) {
   else if constexpr (std::is_same<T, __nv_bfloat16>::value) return __float2bfloat16_rn(x);
   else return x;
 }
-// four values in pairs: two conversions' worth of instructions less per pair than one by one
+// Two fp32 numbers in one 64-bit register: sm_100's packed instructions work on both at once.
+struct F2 {
+  unsigned long long v;
+};
+__device__ __forceinline__ F2 f2(float lo, float hi) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ float2 split(F2 a) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(a.v));
+  return r;
+}
+__device__ __forceinline__ F2 mul(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ float sum(F2 a) {
+  const float2 f = split(a);
+  return f.x + f.y;
+}
+// two neighbours of T, as loaded
 template <typename T>
-__device__ __forceinline__ void unpack4(const T* v, float* o) {
+__device__ __forceinline__ float2 unpack2(const T* v) {
   if constexpr (sizeof(T) == 4) {
-#pragma unroll
-    for (int j = 0; j < 4; ++j) o[j] = v[j];
+    return make_float2(v[0], v[1]);
+  } else if constexpr (std::is_same<T, __half>::value) {
+    return __half22float2(*reinterpret_cast<const __half2*>(v));
   } else {
-    const unsigned* u = reinterpret_cast<const unsigned*>(v);
-#pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      float2 f;
-      if constexpr (std::is_same<T, __half>::value) f = __half22float2(*reinterpret_cast<const __half2*>(u + j));
-      else f = make_float2(__uint_as_float(u[j] << 16), __uint_as_float(u[j] & 0xffff0000u));
-      o[2 * j] = f.x, o[2 * j + 1] = f.y;
-    }
+    const unsigned u = *reinterpret_cast<const unsigned*>(v);
+    return make_float2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
   }
 }
 template <typename T>
-__device__ __forceinline__ void pack4(T* v, float a, float b, float c, float d) {
-  if constexpr (std::is_same<T, __half>::value) {
-    reinterpret_cast<__half2*>(v)[0] = __floats2half2_rn(a, b);
-    reinterpret_cast<__half2*>(v)[1] = __floats2half2_rn(c, d);
-  } else if constexpr (std::is_same<T, __nv_bfloat16>::value) {
-    reinterpret_cast<unsigned*>(v)[0] = pack_bf16(a, b);
-    reinterpret_cast<unsigned*>(v)[1] = pack_bf16(c, d);
-  } else {
-    v[0] = a, v[1] = b, v[2] = c, v[3] = d;
-  }
+__device__ __forceinline__ void pack2(T* v, float a, float b) {
+  if constexpr (sizeof(T) == 4) v[0] = a, v[1] = b;
+  else if constexpr (std::is_same<T, __half>::value) *reinterpret_cast<__half2*>(v) = __floats2half2_rn(a, b);
+  else *reinterpret_cast<unsigned*>(v) = pack_bf16(a, b);
 }
 template <typename T>
 struct alignas(sizeof(T) * 4) Four {
@@ -126,27 +144,38 @@ __device__ __forceinline__ Raw8<T> load_raw(const T* head, const Place<HALF>& at
   }
   return r;
 }
-// raw channels -> the pairs' first and second members
+// A lane's channels in registers: the first members of its four pairs and the second ones, two to a register.
+struct Head {
+  F2 a[2], b[2];
+};
 template <bool HALF, typename T>
-__device__ __forceinline__ void to_pairs(const Raw8<T>& r, float* a, float* b) {
-  float f[8];
-  unpack4(r.c[0].v, f);
-  unpack4(r.c[1].v, f + 4);
+__device__ __forceinline__ Head to_head(const Raw8<T>& r) {
+  Head z;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    a[i] = HALF ? f[i] : f[2 * i];
-    b[i] = HALF ? f[4 + i] : f[2 * i + 1];
+  for (int i = 0; i < 2; ++i) {
+    if constexpr (HALF) {
+      const float2 u = unpack2(r.c[0].v + 2 * i), v = unpack2(r.c[1].v + 2 * i);
+      z.a[i] = f2(u.x, u.y), z.b[i] = f2(v.x, v.y);
+    } else {
+      const float2 u = unpack2(r.c[i].v), v = unpack2(r.c[i].v + 2);
+      z.a[i] = f2(u.x, v.x), z.b[i] = f2(u.y, v.y);
+    }
   }
+  return z;
 }
 template <bool HALF, typename T>
-__device__ __forceinline__ void store_pairs(T* head, const Place<HALF>& at, const float* a, const float* b) {
+__device__ __forceinline__ void store_head(T* head, const Place<HALF>& at, const Head& z) {
   Raw8<T> r;
-  if constexpr (HALF) {
-    pack4(r.c[0].v, a[0], a[1], a[2], a[3]);
-    pack4(r.c[1].v, b[0], b[1], b[2], b[3]);
-  } else {
-    pack4(r.c[0].v, a[0], b[0], a[1], b[1]);
-    pack4(r.c[1].v, a[2], b[2], a[3], b[3]);
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float2 a = split(z.a[i]), b = split(z.b[i]);
+    if constexpr (HALF) {
+      pack2(r.c[0].v + 2 * i, a.x, a.y);
+      pack2(r.c[1].v + 2 * i, b.x, b.y);
+    } else {
+      pack2(r.c[i].v, a.x, b.x);
+      pack2(r.c[i].v + 2, a.y, b.y);
+    }
   }
   if constexpr (HALF || sizeof(T) == 4) {
     *reinterpret_cast<Four<T>*>(head + at.c0) = r.c[0];
@@ -155,30 +184,59 @@ __device__ __forceinline__ void store_pairs(T* head, const Place<HALF>& at, cons
     *reinterpret_cast<uint4*>(head + at.c0) = *reinterpret_cast<const uint4*>(&r);
   }
 }
-__device__ __forceinline__ void rotate(float* a, float* b, const float2* cs, float sign) {
+__device__ __forceinline__ Head zero_head() {
+  Head z;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float s = sign * cs[i].y, x = a[i];
-    a[i] = x * cs[i].x - b[i] * s;
-    b[i] = x * s + b[i] * cs[i].x;
+  for (int i = 0; i < 2; ++i) z.a[i] = z.b[i] = f2(0.f, 0.f);
+  return z;
+}
+struct Turn {  // cos, sin and -sin of a lane's four pairs
+  F2 c[2], s[2], n[2];
+};
+__device__ __forceinline__ Turn no_turn() {
+  Turn t;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) t.c[i] = f2(1.f, 1.f), t.s[i] = t.n[i] = f2(0.f, 0.f);
+  return t;
+}
+__device__ __forceinline__ Turn to_turn(const float4* q, float sign) {
+  Turn t;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const float4 u = q[i];
+    t.c[i] = f2(u.x, u.z);
+    t.s[i] = f2(sign * u.y, sign * u.w);
+    t.n[i] = f2(-sign * u.y, -sign * u.w);
+  }
+  return t;
+}
+__device__ __forceinline__ void rotate(Head& z, const Turn& t) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const F2 a = z.a[i];
+    z.a[i] = fma2(a, t.c[i], mul(z.b[i], t.n[i]));
+    z.b[i] = fma2(a, t.s[i], mul(z.b[i], t.c[i]));
+  }
+}
+__device__ __forceinline__ void rotate_back(Head& z, const Turn& t) {  // by the transpose
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const F2 a = z.a[i];
+    z.a[i] = fma2(a, t.c[i], mul(z.b[i], t.s[i]));
+    z.b[i] = fma2(a, t.n[i], mul(z.b[i], t.c[i]));
   }
 }
 // A lane's four (cos, sin) pairs of a row. A position outside the table records kErrBadArg and leaves
 // the row unrotated.
 template <bool HALF>
-__device__ __forceinline__ void load_cs(const QkNormParams& p, int row, const Place<HALF>& at, float2* cs) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) cs[i] = make_float2(1.f, 0.f);
-  if (!at.on || at.cs < 0) return;
+__device__ __forceinline__ Turn load_turn(const QkNormParams& p, int row, const Place<HALF>& at) {
+  if (!at.on || at.cs < 0) return no_turn();
   const int t = p.pos ? p.pos[row] : row % p.seq_len;
   if (t < 0 || t >= p.max_pos) {
     set_error(p.err, kErrBadArg);
-    return;
+    return no_turn();
   }
-  const float4* c = reinterpret_cast<const float4*>(p.table + (long long)t * (p.rot / 2) + at.cs);
-  const float4 u = c[0], v = c[1];
-  cs[0] = make_float2(u.x, u.y), cs[1] = make_float2(u.z, u.w);
-  cs[2] = make_float2(v.x, v.y), cs[3] = make_float2(v.z, v.w);
+  return to_turn(reinterpret_cast<const float4*>(p.table + (long long)t * (p.rot / 2) + at.cs), p.sign);
 }
 template <int LPH>
 __device__ __forceinline__ float head_sum(float v) {
@@ -201,46 +259,47 @@ struct Share {
   }
 };
 
-// One head in a lane group's registers, forward: z = the pairs (a, b), returned normalised and rotated.
+// One head in a lane group's registers, forward.
 template <int LPH, int NORM>
-__device__ __forceinline__ void head_forward(float* a, float* b, const float2* cs, const float* wa, const float* wb,
-                                             const QkNormParams& p) {
-  if (NORM != kBefore) rotate(a, b, cs, p.sign);
+__device__ __forceinline__ void head_forward(Head& z, const Turn& t, const Head& w, const QkNormParams& p) {
+  if (NORM != kBefore) rotate(z, t);
   if (NORM != kNone) {
-    float ss = 0.f;
+    F2 ss = mul(z.a[0], z.a[0]);
+    ss = fma2(z.b[0], z.b[0], ss);
+    ss = fma2(z.a[1], z.a[1], ss);
+    ss = fma2(z.b[1], z.b[1], ss);
+    const float r = rsqrtf(fmaf(head_sum<LPH>(sum(ss)), p.inv_d, p.eps));
+    const F2 rr = f2(r, r);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) ss = fmaf(a[i], a[i], fmaf(b[i], b[i], ss));
-    const float r = rsqrtf(fmaf(head_sum<LPH>(ss), p.inv_d, p.eps));
-#pragma unroll
-    for (int i = 0; i < 4; ++i) a[i] *= r * wa[i], b[i] *= r * wb[i];
+    for (int i = 0; i < 2; ++i) {
+      z.a[i] = mul(z.a[i], mul(rr, w.a[i]));
+      z.b[i] = mul(z.b[i], mul(rr, w.b[i]));
+    }
   }
-  if (NORM == kBefore) rotate(a, b, cs, p.sign);
+  if (NORM == kBefore) rotate(z, t);
 }
-// and backward: (a, b) of x and (ga, gb) of dy; (a, b) becomes dx, (da, db) gains g u
+// and backward: z of x becomes dx, dw gains g u
 template <int LPH, int NORM>
-__device__ __forceinline__ void head_backward(float* a, float* b, float* ga, float* gb, const float2* cs, const float* wa,
-                                              const float* wb, float* da, float* db, const QkNormParams& p) {
-  if (NORM == kAfter) rotate(a, b, cs, 1.f);
-  if (NORM == kBefore) rotate(ga, gb, cs, -1.f);
-  float ss = 0.f, gz = 0.f;
+__device__ __forceinline__ void head_backward(Head& z, Head& g, const Turn& t, const Head& w, Head& dw,
+                                              const QkNormParams& p) {
+  if (NORM == kAfter) rotate(z, t);
+  if (NORM == kBefore) rotate_back(g, t);
+  F2 ss = mul(z.a[0], z.a[0]), gz = mul(mul(g.a[0], w.a[0]), z.a[0]);
+  ss = fma2(z.b[0], z.b[0], ss), gz = fma2(mul(g.b[0], w.b[0]), z.b[0], gz);
+  ss = fma2(z.a[1], z.a[1], ss), gz = fma2(mul(g.a[1], w.a[1]), z.a[1], gz);
+  ss = fma2(z.b[1], z.b[1], ss), gz = fma2(mul(g.b[1], w.b[1]), z.b[1], gz);
+  const float r = rsqrtf(fmaf(head_sum<LPH>(sum(ss)), p.inv_d, p.eps));
+  const float m = -head_sum<LPH>(sum(gz)) * p.inv_d * r * r * r;  // -mean(g w u) / rms^2: times z, -u mean(g w u) / rms
+  const F2 rr = f2(r, r), mm = f2(m, m);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    ss = fmaf(a[i], a[i], fmaf(b[i], b[i], ss));
-    gz = fmaf(ga[i] * wa[i], a[i], fmaf(gb[i] * wb[i], b[i], gz));
+  for (int i = 0; i < 2; ++i) {
+    const F2 ta = mul(g.a[i], rr), tb = mul(g.b[i], rr);
+    dw.a[i] = fma2(ta, z.a[i], dw.a[i]);
+    dw.b[i] = fma2(tb, z.b[i], dw.b[i]);
+    z.a[i] = fma2(ta, w.a[i], mul(z.a[i], mm));
+    z.b[i] = fma2(tb, w.b[i], mul(z.b[i], mm));
   }
-  ss = head_sum<LPH>(ss);
-  gz = head_sum<LPH>(gz);
-  const float r = rsqrtf(fmaf(ss, p.inv_d, p.eps));
-  const float m = gz * p.inv_d * r * r * r;  // mean(g w u) / rms^2: times z it is u mean(g w u) / rms
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float ta = ga[i] * r, tb = gb[i] * r;
-    da[i] = fmaf(ta, a[i], da[i]);
-    db[i] = fmaf(tb, b[i], db[i]);
-    a[i] = fmaf(ta, wa[i], -a[i] * m);
-    b[i] = fmaf(tb, wb[i], -b[i] * m);
-  }
-  if (NORM == kAfter) rotate(a, b, cs, -1.f);
+  if (NORM == kAfter) rotate_back(z, t);
 }
 
 constexpr int kSteps = 4;  // steps of a warp whose loads are in flight together
@@ -249,7 +308,7 @@ constexpr int kSteps = 4;  // steps of a warp whose loads are in flight together
 // (D = 8 LPH).
 template <typename T, int LPH, bool HALF, int NORM, bool FULL>
 __global__ void __launch_bounds__(384, 2) qk_norm_fwd_kernel(const QkNormParams p) {
-  constexpr int HPW = 32 / LPH, U = kSteps;
+  constexpr int HPW = 32 / LPH, U = sizeof(T) == 4 ? kSteps / 2 : kSteps;
   const int lane = threadIdx.x, sub = lane / LPH;
   Place<HALF> at(lane % LPH, p);
   if (FULL) at.on = true;
@@ -259,8 +318,8 @@ __global__ void __launch_bounds__(384, 2) qk_norm_fwd_kernel(const QkNormParams 
   const T* x = static_cast<const T*>(p.x) + (long long)row * p.ldx + sh.col0 + sub * p.D;
   T* y = static_cast<T*>(p.out) + (long long)row * p.ldo + sh.col0 + sub * p.D;
   const int step = HPW * p.D;
-  float2 cs[4];
-  float wa[4], wb[4];
+  Turn turn;
+  Head w = zero_head();
   for (int s0 = sh.part; s0 * HPW < sh.heads; s0 += U * sh.stride) {
     Raw8<T> raw[U];
 #pragma unroll
@@ -269,21 +328,17 @@ __global__ void __launch_bounds__(384, 2) qk_norm_fwd_kernel(const QkNormParams 
       if (s * HPW + sub < sh.heads && at.on) raw[u] = load_raw<HALF>(x + s * step, at);
     }
     if (s0 == sh.part) {  // behind the first loads
-      load_cs<HALF>(p, row, at, cs);
-      if (NORM != kNone && at.on)
-        to_pairs<HALF>(load_raw<HALF>(static_cast<const T*>(sh.key ? p.wk : p.wq), at), wa, wb);
+      turn = load_turn<HALF>(p, row, at);
+      if (NORM != kNone && at.on) w = to_head<HALF>(load_raw<HALF>(static_cast<const T*>(sh.key ? p.wk : p.wq), at));
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int s = s0 + u * sh.stride;
       if (s * HPW >= sh.heads) break;  // the same for the whole warp
       const bool on = s * HPW + sub < sh.heads && at.on;
-      float a[4], b[4];
-#pragma unroll
-      for (int i = 0; i < 4; ++i) a[i] = b[i] = 0.f;
-      if (on) to_pairs<HALF>(raw[u], a, b);
-      head_forward<LPH, NORM>(a, b, cs, wa, wb, p);
-      if (on) store_pairs<HALF>(y + s * step, at, a, b);
+      Head z = on ? to_head<HALF>(raw[u]) : zero_head();
+      head_forward<LPH, NORM>(z, turn, w, p);
+      if (on) store_head<HALF>(y + s * step, at, z);
     }
   }
 }
@@ -315,9 +370,7 @@ __global__ void __launch_bounds__(32 * (kMaxWarps + 1), 2) qk_norm_rows_kernel(c
   }
   if (BWD) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the sum over CTAs waits for this grid
   __syncthreads();
-  float da[4], db[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) da[i] = db[i] = 0.f;
+  Head dw = zero_head();
   Place<HALF> at(lane % LPH, p);
   if (FULL) at.on = true;
   const int sub = lane / LPH;
@@ -349,44 +402,36 @@ __global__ void __launch_bounds__(32 * (kMaxWarps + 1), 2) qk_norm_rows_kernel(c
       }
     }
   } else {
-    const Share sh(p, warp, warps);
-    float wa[4], wb[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) wa[i] = wb[i] = 0.f;
-    if (NORM != kNone && at.on)
-      to_pairs<HALF>(load_raw<HALF>(static_cast<const T*>(sh.key ? p.wk : p.wq), at), wa, wb);
+    const int z = warp / p.warps_per_row;  // of every p.rows_at_once rows, this warp has the z-th
+    const Share sh(p, warp - z * p.warps_per_row, p.warps_per_row);
+    const Head w = NORM != kNone && at.on
+                       ? to_head<HALF>(load_raw<HALF>(static_cast<const T*>(sh.key ? p.wk : p.wq), at)) : zero_head();
     const int step = HPW * p.D, col = sh.col0 + sub * p.D;
     int n = 0;
     for (int c = blockIdx.x; c < chunks; c += gridDim.x, ++n) {
       const int st = n % kStages, live = min(chunk, p.rows - c * chunk);
       if (!mbar_wait(&full[st], (n / kStages) & 1, p.err, kErrWaitFull)) break;
-      const unsigned char* src = smem + st * stage_bytes;
-      T* out = static_cast<T*>(p.out) + (long long)c * chunk * p.ldo + col;
-      for (int r = 0; r < live; ++r, src += per_row, out += p.ldo) {
-        float2 cs[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) cs[i] = make_float2(1.f, 0.f);
-        if (at.on && at.cs >= 0) {
-          const float4* q = reinterpret_cast<const float4*>(src + per_row - cs_bytes + at.cs * 8);
-          const float4 u = q[0], v = q[1];
-          cs[0] = make_float2(u.x, u.y), cs[1] = make_float2(u.z, u.w);
-          cs[2] = make_float2(v.x, v.y), cs[3] = make_float2(v.z, v.w);
-        }
+      const unsigned char* src = smem + st * stage_bytes + z * per_row;
+      T* out = static_cast<T*>(p.out) + ((long long)c * chunk + z) * p.ldo + col;
+      for (int r = z; r < live; r += p.rows_at_once, src += p.rows_at_once * per_row, out += p.rows_at_once * p.ldo) {
+        const Turn turn = at.on && at.cs >= 0
+                              ? to_turn(reinterpret_cast<const float4*>(src + per_row - cs_bytes + at.cs * 8), p.sign)
+                              : no_turn();
         const T* x = reinterpret_cast<const T*>(src) + col;
         const T* dy = reinterpret_cast<const T*>(src + row_bytes) + col;
+#pragma unroll (BWD || sizeof(T) == 4 ? 1 : 2)
         for (int s = sh.part; s * HPW < sh.heads; s += sh.stride) {
-          const bool on = s * HPW + sub < sh.heads && at.on;
-          float a[4], b[4], ga[4], gb[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) a[i] = b[i] = ga[i] = gb[i] = 0.f;
-          if (on) to_pairs<HALF>(load_raw<HALF>(x + s * step, at), a, b);
+          // lanes behind the last head repeat it and store nothing; lanes without channels hold zeros
+          const bool on = s * HPW + sub < sh.heads;
+          const int at_step = on ? s * step : (sh.heads - 1 - sub) * p.D;
+          Head v = FULL || at.on ? to_head<HALF>(load_raw<HALF>(x + at_step, at)) : zero_head();
           if (BWD) {
-            if (on) to_pairs<HALF>(load_raw<HALF>(dy + s * step, at), ga, gb);
-            head_backward<LPH, NORM>(a, b, ga, gb, cs, wa, wb, da, db, p);
+            Head g = (FULL || at.on) && on ? to_head<HALF>(load_raw<HALF>(dy + at_step, at)) : zero_head();
+            head_backward<LPH, NORM>(v, g, turn, w, dw, p);
           } else {
-            head_forward<LPH, NORM>(a, b, cs, wa, wb, p);
+            head_forward<LPH, NORM>(v, turn, w, p);
           }
-          if (on) store_pairs<HALF>(out + s * step, at, a, b);
+          if (on && (FULL || at.on)) store_head<HALF>(out + s * step, at, v);
         }
       }
       __syncwarp();
@@ -398,24 +443,25 @@ __global__ void __launch_bounds__(32 * (kMaxWarps + 1), 2) qk_norm_rows_kernel(c
   __syncthreads();
   float* red = reinterpret_cast<float*>(smem);  // [warp][D]; every copy has been waited for
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
+  for (int i = 0; i < 2; ++i) {
+    float2 a = split(dw.a[i]), b = split(dw.b[i]);
 #pragma unroll
     for (int o = 16; o >= LPH; o >>= 1) {
-      da[i] += __shfl_xor_sync(0xffffffff, da[i], o);
-      db[i] += __shfl_xor_sync(0xffffffff, db[i], o);
+      a.x += __shfl_xor_sync(0xffffffff, a.x, o), a.y += __shfl_xor_sync(0xffffffff, a.y, o);
+      b.x += __shfl_xor_sync(0xffffffff, b.x, o), b.y += __shfl_xor_sync(0xffffffff, b.y, o);
     }
-  if (warp < warps && sub == 0 && at.on) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      red[warp * p.D + (HALF ? at.c0 + i : at.c0 + 2 * i)] = da[i];
-      red[warp * p.D + (HALF ? at.c1 + i : at.c0 + 2 * i + 1)] = db[i];
+    if (warp < warps && sub == 0 && at.on) {
+      float* to = red + warp * p.D;
+      if (HALF) to[at.c0 + 2 * i] = a.x, to[at.c0 + 2 * i + 1] = a.y, to[at.c1 + 2 * i] = b.x, to[at.c1 + 2 * i + 1] = b.y;
+      else to[at.c0 + 4 * i] = a.x, to[at.c0 + 4 * i + 1] = b.x, to[at.c0 + 4 * i + 2] = a.y, to[at.c0 + 4 * i + 3] = b.y;
     }
   }
   __syncthreads();
   for (int c = threadIdx.x; c < 2 * p.D; c += blockDim.x) {
     const bool key = c >= p.D;
     float s = 0.f;
-    for (int w = key ? p.q_parts : 0; w < (key ? warps : p.q_parts); ++w) s += red[w * p.D + c - key * p.D];
+    for (int w = 0; w < warps; ++w)
+      if ((w % p.warps_per_row >= p.q_parts) == key) s += red[w * p.D + c - key * p.D];
     p.dw_part[(long long)blockIdx.x * 2 * p.D + c] = s;
   }
 }
@@ -559,12 +605,14 @@ astrai::Launch many_rows(astrai::QkNormParams& p, int elem, bool bwd, int sms) {
   Launch l{};
   l.lph = lanes_per_head(p.D);
   const int hpw = 32 / l.lph, sq = (p.hq + hpw - 1) / hpw, sk = (p.hkv + hpw - 1) / hpw;
-  int turns = 1;  // steps of a warp per row
+  int turns = std::min(2, std::max(sq, sk));  // steps of a warp per row, which then share its (cos, sin) pairs
   while ((sq + turns - 1) / turns + (sk + turns - 1) / turns > kMaxWarps) ++turns;
   p.q_parts = (sq + turns - 1) / turns;
-  const int warps = p.q_parts + (sk + turns - 1) / turns;
+  p.warps_per_row = p.q_parts + (sk + turns - 1) / turns;
   const int per_row = (p.hq + p.hkv) * p.D * elem * (bwd ? 2 : 1) + p.rot * 4;
   l.chunk = std::min(std::min(4, (p.rows + 2 * sms - 1) / (2 * sms)), kRowsSmem / (kStages * per_row));
+  p.rows_at_once = std::max(1, std::min(kMaxWarps / p.warps_per_row, l.chunk));
+  const int warps = p.warps_per_row * p.rows_at_once;
   l.smem = std::max(per_row * l.chunk * kStages, bwd ? warps * p.D * 4 : 0);
   l.block = dim3(32 * (warps + 1));
   l.blocks = std::min(2 * sms, (p.rows + l.chunk - 1) / l.chunk);
