@@ -40,7 +40,8 @@ struct QkNormParams {
   int rows, hq, hkv, D, rot, rot_off, seq_len, max_pos;
   int q_parts;      // warps of a row that share its query heads; the others share its key heads
   int warps_per_row, rows_at_once;  // of a CTA's consumers in qk_norm_rows_kernel
-  float sign, eps, inv_d;
+  float eps, inv_d;
+  bool inverse;     // without a norm: the transposed rotation
 };
 
 template <typename T>
@@ -199,14 +200,14 @@ __device__ __forceinline__ Turn no_turn() {
   for (int i = 0; i < 2; ++i) t.c[i] = f2(1.f, 1.f), t.s[i] = t.n[i] = f2(0.f, 0.f);
   return t;
 }
-__device__ __forceinline__ Turn to_turn(const float4* q, float sign) {
+__device__ __forceinline__ Turn to_turn(const float4* q) {
   Turn t;
 #pragma unroll
   for (int i = 0; i < 2; ++i) {
     const float4 u = q[i];
     t.c[i] = f2(u.x, u.z);
-    t.s[i] = f2(sign * u.y, sign * u.w);
-    t.n[i] = f2(-sign * u.y, -sign * u.w);
+    t.s[i] = f2(u.y, u.w);
+    t.n[i] = f2(-u.y, -u.w);
   }
   return t;
 }
@@ -236,7 +237,7 @@ __device__ __forceinline__ Turn load_turn(const QkNormParams& p, int row, const 
     set_error(p.err, kErrBadArg);
     return no_turn();
   }
-  return to_turn(reinterpret_cast<const float4*>(p.table + (long long)t * (p.rot / 2) + at.cs), p.sign);
+  return to_turn(reinterpret_cast<const float4*>(p.table + (long long)t * (p.rot / 2) + at.cs));
 }
 template <int LPH>
 __device__ __forceinline__ float head_sum(float v) {
@@ -262,6 +263,10 @@ struct Share {
 // One head in a lane group's registers, forward.
 template <int LPH, int NORM>
 __device__ __forceinline__ void head_forward(Head& z, const Turn& t, const Head& w, const QkNormParams& p) {
+  if (NORM == kNone && p.inverse) {
+    rotate_back(z, t);
+    return;
+  }
   if (NORM != kBefore) rotate(z, t);
   if (NORM != kNone) {
     F2 ss = mul(z.a[0], z.a[0]);
@@ -304,14 +309,12 @@ __device__ __forceinline__ void head_backward(Head& z, Head& g, const Turn& t, c
 
 constexpr int kSteps = 4;  // steps of a warp whose loads are in flight together
 
-// Few rows: block (32, warps per row, rows), straight from global memory. FULL: every lane of a head has channels
-// (D = 8 LPH).
-template <typename T, int LPH, bool HALF, int NORM, bool FULL>
+// Few rows: block (32, warps per row, rows), straight from global memory.
+template <typename T, int LPH, bool HALF, int NORM>
 __global__ void __launch_bounds__(384, 2) qk_norm_fwd_kernel(const QkNormParams p) {
   constexpr int HPW = 32 / LPH, U = sizeof(T) == 4 ? kSteps / 2 : kSteps;
   const int lane = threadIdx.x, sub = lane / LPH;
-  Place<HALF> at(lane % LPH, p);
-  if (FULL) at.on = true;
+  const Place<HALF> at(lane % LPH, p);
   const Share sh(p, threadIdx.y, blockDim.y);
   const int row = blockIdx.x * blockDim.z + threadIdx.z;
   if (row >= p.rows) return;
@@ -349,10 +352,11 @@ __global__ void __launch_bounds__(384, 2) qk_norm_fwd_kernel(const QkNormParams 
 // chunks c, c + grid, ... In the backward the sums of g u stay in registers and go to the CTA's own row of dw_part,
 // so the result does not depend on any order in time.
 constexpr int kStages = 4;
-constexpr int kMaxWarps = 12;  // consumers
+constexpr int kMaxWarps = 10;  // consumers
 constexpr int kRowsSmem = 100 * 1024;  // of which an SM holds two
 
-template <typename T, int LPH, bool HALF, int NORM, bool FULL, bool BWD>
+// EVEN: every lane group of every step has a whole head (D = 8 LPH, head counts multiples of 32 / LPH).
+template <typename T, int LPH, bool HALF, int NORM, bool EVEN, bool BWD>
 __global__ void __launch_bounds__(32 * (kMaxWarps + 1), 2) qk_norm_rows_kernel(const QkNormParams p, int chunk) {
   constexpr int HPW = 32 / LPH;
   extern __shared__ __align__(128) unsigned char smem[];
@@ -372,7 +376,7 @@ __global__ void __launch_bounds__(32 * (kMaxWarps + 1), 2) qk_norm_rows_kernel(c
   __syncthreads();
   Head dw = zero_head();
   Place<HALF> at(lane % LPH, p);
-  if (FULL) at.on = true;
+  if (EVEN) at.on = true;
   const int sub = lane / LPH;
 
   if (warp == warps) {  // producer: lane r copies row r of the chunk
@@ -406,7 +410,11 @@ __global__ void __launch_bounds__(32 * (kMaxWarps + 1), 2) qk_norm_rows_kernel(c
     const Share sh(p, warp - z * p.warps_per_row, p.warps_per_row);
     const Head w = NORM != kNone && at.on
                        ? to_head<HALF>(load_raw<HALF>(static_cast<const T*>(sh.key ? p.wk : p.wq), at)) : zero_head();
-    const int step = HPW * p.D, col = sh.col0 + sub * p.D;
+    const int stride = sh.stride * HPW * p.D, col = sh.col0 + (sh.part * HPW + sub) * p.D;
+    const int left = sh.heads - sh.part * HPW;  // heads from the warp's first on
+    const int steps = left > 0 ? (left + sh.stride * HPW - 1) / (sh.stride * HPW) : 0;
+    // a lane group behind the last head has a step less, lanes without channels have none
+    const int mine = EVEN ? steps : at.on ? max(0, (left - sub + sh.stride * HPW - 1) / (sh.stride * HPW)) : 0;
     int n = 0;
     for (int c = blockIdx.x; c < chunks; c += gridDim.x, ++n) {
       const int st = n % kStages, live = min(chunk, p.rows - c * chunk);
@@ -415,23 +423,21 @@ __global__ void __launch_bounds__(32 * (kMaxWarps + 1), 2) qk_norm_rows_kernel(c
       T* out = static_cast<T*>(p.out) + ((long long)c * chunk + z) * p.ldo + col;
       for (int r = z; r < live; r += p.rows_at_once, src += p.rows_at_once * per_row, out += p.rows_at_once * p.ldo) {
         const Turn turn = at.on && at.cs >= 0
-                              ? to_turn(reinterpret_cast<const float4*>(src + per_row - cs_bytes + at.cs * 8), p.sign)
-                              : no_turn();
+                              ? to_turn(reinterpret_cast<const float4*>(src + per_row - cs_bytes + at.cs * 8)) : no_turn();
         const T* x = reinterpret_cast<const T*>(src) + col;
-        const T* dy = reinterpret_cast<const T*>(src + row_bytes) + col;
-#pragma unroll (BWD || sizeof(T) == 4 ? 1 : 2)
-        for (int s = sh.part; s * HPW < sh.heads; s += sh.stride) {
-          // lanes behind the last head repeat it and store nothing; lanes without channels hold zeros
-          const bool on = s * HPW + sub < sh.heads;
-          const int at_step = on ? s * step : (sh.heads - 1 - sub) * p.D;
-          Head v = FULL || at.on ? to_head<HALF>(load_raw<HALF>(x + at_step, at)) : zero_head();
+        T* y = out;
+#pragma unroll(BWD || sizeof(T) == 4 ? 1 : 2)
+        for (int s = 0; s < steps; ++s, x += stride, y += stride) {
+          const bool on = EVEN || s < mine;
+          Head v = on ? to_head<HALF>(load_raw<HALF>(x, at)) : zero_head();
           if (BWD) {
-            Head g = (FULL || at.on) && on ? to_head<HALF>(load_raw<HALF>(dy + at_step, at)) : zero_head();
+            const T* dy = reinterpret_cast<const T*>(reinterpret_cast<const unsigned char*>(x) + row_bytes);
+            Head g = on ? to_head<HALF>(load_raw<HALF>(dy, at)) : zero_head();
             head_backward<LPH, NORM>(v, g, turn, w, dw, p);
           } else {
             head_forward<LPH, NORM>(v, turn, w, p);
           }
-          if (on && (FULL || at.on)) store_head<HALF>(out + s * step, at, v);
+          if (on) store_head<HALF>(y, at, v);
         }
       }
       __syncwarp();
@@ -505,40 +511,27 @@ void allow_smem(K kernel, int smem, bool* set) {  // the attribute belongs to th
   cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (dev >= 0 && dev < 64) set[dev] = true;
 }
-template <typename T, int LPH, bool HALF, int NORM, bool FULL>
-void launch_fwd(const QkNormParams& p, const Launch& l, cudaStream_t s) {
-  if (l.chunk == 0) {
-    (note_launch(), qk_norm_fwd_kernel<T, LPH, HALF, NORM, FULL><<<l.blocks, l.block, 0, s>>>(p));
-    return;
-  }
-  auto kernel = qk_norm_rows_kernel<T, LPH, HALF, NORM, FULL, false>;
+template <typename T, int LPH, bool HALF, int NORM, bool EVEN, bool BWD>
+void launch_rows(const QkNormParams& p, const Launch& l, cudaStream_t s) {
+  auto kernel = qk_norm_rows_kernel<T, LPH, HALF, NORM, EVEN, BWD>;
   static bool set[64] = {};
   allow_smem(kernel, kRowsSmem, set);
   (note_launch(), kernel<<<l.blocks, l.block, l.smem, s>>>(p, l.chunk));
 }
-template <typename T, int LPH, bool HALF, int NORM, bool FULL>
-void launch_bwd(const QkNormParams& p, const Launch& l, cudaStream_t s) {
-  auto kernel = qk_norm_rows_kernel<T, LPH, HALF, NORM, FULL, true>;
-  static bool set[64] = {};
-  allow_smem(kernel, kRowsSmem, set);
-  (note_launch(), kernel<<<l.blocks, l.block, l.smem, s>>>(p, l.chunk));
+template <typename T, int LPH, bool HALF, int NORM, bool BWD>
+void launch(const QkNormParams& p, const Launch& l, cudaStream_t s) {
+  constexpr int HPW = 32 / LPH;
+  if constexpr (BWD && NORM == kNone) return;  // the transposed rotation is a forward call
+  if (!BWD && l.chunk == 0)
+    (note_launch(), qk_norm_fwd_kernel<T, LPH, HALF, NORM><<<l.blocks, l.block, 0, s>>>(p));
+  else if (p.D == 8 * LPH && p.hq % HPW == 0 && p.hkv % HPW == 0) launch_rows<T, LPH, HALF, NORM, true, BWD>(p, l, s);
+  else launch_rows<T, LPH, HALF, NORM, false, BWD>(p, l, s);
 }
 template <typename T, bool HALF, int NORM, bool BWD>
 void by_heads(const QkNormParams& p, const Launch& l, cudaStream_t s) {
-#define ASTRAI_QK_HEADS(LPH)                                                                  \
-  if (BWD) {                                                                                  \
-    if constexpr (NORM != kNone) {                                                            \
-      if (p.D == 8 * LPH) launch_bwd<T, LPH, HALF, NORM, true>(p, l, s);                      \
-      else launch_bwd<T, LPH, HALF, NORM, false>(p, l, s);                                    \
-    }                                                                                         \
-  } else {                                                                                    \
-    if (p.D == 8 * LPH) launch_fwd<T, LPH, HALF, NORM, true>(p, l, s);                        \
-    else launch_fwd<T, LPH, HALF, NORM, false>(p, l, s);                                      \
-  }
-  if (l.lph == 8) { ASTRAI_QK_HEADS(8) }
-  else if (l.lph == 16) { ASTRAI_QK_HEADS(16) }
-  else { ASTRAI_QK_HEADS(32) }
-#undef ASTRAI_QK_HEADS
+  if (l.lph == 8) launch<T, 8, HALF, NORM, BWD>(p, l, s);
+  else if (l.lph == 16) launch<T, 16, HALF, NORM, BWD>(p, l, s);
+  else launch<T, 32, HALF, NORM, BWD>(p, l, s);
 }
 template <typename T, bool BWD>
 void by_mode(const QkNormParams& p, const Launch& l, bool half_layout, int norm, cudaStream_t s) {
@@ -644,7 +637,7 @@ void qk_norm_fwd(const void* x, long long ldx, void* y, long long ldy, int rows,
   p.x = x, p.out = y, p.ldx = ldx, p.ldo = ldy, p.wq = wq, p.wk = wk;
   p.table = static_cast<const float2*>(table), p.pos = pos, p.err = error_word(device);
   p.rows = rows, p.hq = hq, p.hkv = hkv, p.D = D, p.rot = rot, p.rot_off = rot_off;
-  p.seq_len = seq_len, p.max_pos = max_pos, p.sign = inverse ? -1.f : 1.f, p.eps = eps, p.inv_d = 1.f / D;
+  p.seq_len = seq_len, p.max_pos = max_pos, p.inverse = inverse != 0, p.eps = eps, p.inv_d = 1.f / D;
   const int sms = num_sms(device), elem = dtype == 2 ? 4 : 2, heads = hq + hkv;
   const auto run = [&](const QkNormParams& part, const Launch& l) {
     if (dtype == 0) by_mode<__nv_bfloat16, false>(part, l, half_layout, norm, s);
@@ -679,7 +672,7 @@ void qk_norm_bwd(const void* dy, long long lddy, const void* x, long long ldx, v
   p.x = x, p.dy = dy, p.out = dx, p.ldx = ldx, p.lddy = lddy, p.ldo = lddx, p.wq = wq, p.wk = wk;
   p.table = static_cast<const float2*>(table), p.pos = pos, p.dw_part = scratch, p.err = error_word(device);
   p.rows = rows, p.hq = hq, p.hkv = hkv, p.D = D, p.rot = rot, p.rot_off = rot_off;
-  p.seq_len = seq_len, p.max_pos = max_pos, p.sign = 1.f, p.eps = eps, p.inv_d = 1.f / D;
+  p.seq_len = seq_len, p.max_pos = max_pos, p.eps = eps, p.inv_d = 1.f / D;
   const int sms = num_sms(device), elem = dtype == 2 ? 4 : 2, heads = hq + hkv;
   const int n = launches_of_rows(heads, D, rot, elem, true), per = (heads + n - 1) / n;
   int parts = 0;
