@@ -14,7 +14,7 @@ void kv8_append(const void* k, const long long* ks, const void* v, const long lo
                 int page_size, int n_pages, int max_pages, int block, int dtype, cudaStream_t s);
 void kv8_gather(const void* kc, const void* vc, const float* ka, const float* va, const int* table, const int* starts,
                 const int* lens, void* ko, void* vo, int B, int total, int Hkv, int D, int page_size, int n_pages,
-                int max_pages, int block, int dtype, int device, cudaStream_t s);
+                int max_pages, int block, int dtype, cudaStream_t s);
 void kv8_attend_plan(int B, int S, int Hq, int Hkv, int D, int page_size, int max_pages, int device, long long* out);
 void kv8_attend(const void* q, const long long* qs, const void* kc, const void* vc, const float* ka, const float* va,
                 const int* table, const int* lens, const int* starts, void* out, float* workspace, int B, int S,
@@ -138,6 +138,7 @@ std::pair<at::Tensor, at::Tensor> kv8_gather(const at::Tensor& kc, const at::Ten
   const Cache c = check_cache(kc, vc, ka, va);
   TORCH_CHECK(dtype == at::kBFloat16 || dtype == at::kHalf, "kv8_gather: bfloat16 or float16, got ", dtype);
   TORCH_CHECK(total >= 0 && total < (1LL << 30), "kv8_gather: total must be in [0, 2^30)");
+  TORCH_CHECK(table_in.size(0) < 65536, "kv8_gather: at most 65535 rows");
   const at::Tensor table = int32_of(table_in), lens = int32_of(lens_in);
   const int64_t B = table.dim() == 2 ? table.size(0) : -1;
   const int mp = check_table(table, kc, B, c);
@@ -152,7 +153,7 @@ std::pair<at::Tensor, at::Tensor> kv8_gather(const at::Tensor& kc, const at::Ten
   auto ko = at::empty({B, total, c.Hkv, c.D}, kc.options().dtype(dtype)), vo = at::empty_like(ko);
   astrai_host::kv8_gather(kc.data_ptr(), vc.data_ptr(), ka.data_ptr<float>(), va.data_ptr<float>(),
                           table.data_ptr<int>(), st, ln, ko.data_ptr(), vo.data_ptr(), (int)B, (int)total, c.Hkv, c.D,
-                          c.page_size, c.n_pages, mp, c.block, dtype == at::kHalf, kc.device().index(), stream());
+                          c.page_size, c.n_pages, mp, c.block, dtype == at::kHalf, stream());
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   return {ko, vo};
 }

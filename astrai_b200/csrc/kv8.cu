@@ -18,6 +18,7 @@
 #include <cuda_fp16.h>
 
 #include "common.cuh"
+#include "launch.cuh"
 
 namespace astrai {
 namespace {
@@ -40,13 +41,52 @@ __device__ __forceinline__ float bits_to_float(unsigned short u) {
   else return __bfloat162float(__ushort_as_bfloat16(u));
 }
 template <typename T>
+__device__ __forceinline__ unsigned pack_pair(float a, float b) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const unsigned*>(&v);
+  } else {
+    return pack_bf16(a, b);
+  }
+}
+template <typename T>
 __device__ __forceinline__ T from_float(float x) {
   if constexpr (std::is_same<T, __half>::value) return __float2half_rn(x);
   else return __float2bfloat16_rn(x);
 }
 
+__device__ __forceinline__ void cp_async16(unsigned dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async4(unsigned dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ uint4 lds128(unsigned a) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
+  return v;
+}
+
+// rint(x / by) in the low byte, for |x / by| up to 127 and r = 1 / by rounded. The product x r is off by
+// some units in its last place; one step of residual correction (Markstein, IBM J. Res. Dev. 34, 1990) gives
+// the quotient rounded, exact where it is half an integer, and so the integer that the division would: x has
+// at most 18 and by 11 significant bits, so other quotients are 2^-12 and more away from such ties. Adding
+// 1.5 * 2^23 rounds to an integer, ties to even, and leaves it in the low bits.
+__device__ __forceinline__ unsigned round_quotient(float x, float by, float r) {
+  const float t = x * r;
+  return __float_as_uint(fmaf(fmaf(-t, by, x), r, t) + 12582912.f);
+}
+__device__ __forceinline__ unsigned low_bytes(unsigned a, unsigned b, unsigned c, unsigned d) {
+  return __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+}
+
 // One block of tokens of one head of k or v: its live tokens and the new ones end under the larger
-// of their magnitudes. WARPS warps share it, at most 32 tokens each, whose values stay in registers
+// of their magnitudes. WARPS warps share it, at most 32 tokens each, whose values wait in shared memory
 // between the maximum and the rounding. A row's append starts at starts[b] and ends at lens[b]; what
 // the cache held from starts[b] on is void. A block with an infinite or NaN input gets the magnitude
 // NaN: reading it gives NaN, as the input would have.
@@ -54,16 +94,15 @@ template <typename T, int D, int BLOCK>
 __global__ void __launch_bounds__(128) kv8_append_kernel(const AppendParams p) {
   constexpr int WARPS = BLOCK > 32 ? BLOCK / 32 : 1;  // warps per item
   constexpr int TOK = BLOCK / WARPS;                  // tokens per warp
-  constexpr int LPT = D / 8;                          // lanes per token: 8 values (16 bytes) each
-  constexpr int TPI = 32 / LPT;                       // tokens per warp-wide load
-  constexpr int N = TOK / TPI;
+  constexpr int LPT = D / 8;                          // 16-byte pieces (8 values) per token
+  __shared__ __align__(16) unsigned char hold[4][TOK * D * 2];
   __shared__ unsigned most_s[4];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const long long item = blockIdx.x * (4LL / WARPS) + warp / WARPS;
-  const int kv = (int)(item & 1);
-  const int h = (int)((item >> 1) % p.Hkv);
-  const long long bw = (item >> 1) / p.Hkv;
-  const int w = (int)(bw % p.windows), b = (int)(bw / p.windows);
+  const int item = blockIdx.x * (4 / WARPS) + warp / WARPS;
+  const int kv = item & 1;
+  const unsigned bwh = (unsigned)item >> 1, bw = bwh / (unsigned)p.Hkv;
+  const int h = (int)(bwh - bw * p.Hkv), b = (int)(bw / (unsigned)p.windows), w = (int)(bw - (unsigned)b * p.windows);
+  begin_early();
   bool on = b < p.B;
   int start = 0, end = 0, base = 0, page = -1, off = 0;
   if (on) {
@@ -71,70 +110,74 @@ __global__ void __launch_bounds__(128) kv8_append_kernel(const AppendParams p) {
     end = min(p.lens[b], start + p.S);
     base = (start / BLOCK + w) * BLOCK;
     on = base < end && start < end;
+  }
+  // this warp's tokens first .. first + n - 1 of the block are new
+  const int mine = warp % WARPS * TOK;
+  const int first = max(start - base, mine), n = on ? max(0, min(end - base, mine + TOK) - first) : 0;
+  const T* src = static_cast<const T*>(p.src[kv]) + (long long)b * p.sb[kv] + (long long)h * p.sh[kv] +
+                 (long long)(base + first - start) * p.st[kv];
+  const unsigned held = (unsigned)__cvta_generic_to_shared(hold[warp]) + lane * 16;
+#pragma unroll 4
+  for (int i = lane; i < n * LPT; i += 32)
+    cp_async16(held + (i - lane) * 16, src + (i / LPT) * p.st[kv] + i % LPT * 8);
+  cp_async_commit();
+  if (on) {
     const int lp = base / p.page_size;
-    if (on && lp < p.max_pages) page = p.table[(long long)b * p.max_pages + lp];
-    off = base % p.page_size;
-    on = on && page >= 0 && page < p.n_pages;
+    if (lp < p.max_pages) page = p.table[(long long)b * p.max_pages + lp];
+    off = base - lp * p.page_size;
+    on = page >= 0 && page < p.n_pages;
   }
-  const int t0 = (warp % WARPS) * TOK + lane / LPT, c = lane % LPT;
-  const T* src = static_cast<const T*>(p.src[kv]) + (long long)b * p.sb[kv] + (long long)h * p.sh[kv] + c * 8;
-  uint4 raw[N];
+  const long long row0 = ((long long)page * p.Hkv + h) * p.page_size + off;  // the block's first token
+  float* ap = p.absmax[kv] + row0 / BLOCK;
+  const float was = on && base < start ? *ap : 0.f;  // live tokens only
+  cp_async_wait<0>();
   unsigned most = 0;
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int t = base + t0 + i * TPI;
-    raw[i] = make_uint4(0u, 0u, 0u, 0u);
-    if (on && t >= start && t < end)
-      raw[i] = *reinterpret_cast<const uint4*>(src + (long long)(t - start) * p.st[kv]);
+#pragma unroll 4
+  for (int i = lane; i < n * LPT; i += 32) {  // magnitudes compare as integers, infinities and NaN above all others
+    const uint4 v = lds128(held + (i - lane) * 16);
+    most = __vmaxu2(most, __vmaxu2(__vmaxu2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu),
+                                   __vmaxu2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu)));
   }
-#pragma unroll
-  for (int i = 0; i < N; ++i)  // magnitudes compare as integers, infinities and NaN above all others
-    most = __vmaxu2(most, __vmaxu2(__vmaxu2(raw[i].x & 0x7fff7fffu, raw[i].y & 0x7fff7fffu),
-                                   __vmaxu2(raw[i].z & 0x7fff7fffu, raw[i].w & 0x7fff7fffu)));
   most = max(most & 0xffffu, most >> 16);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) most = max(most, __shfl_xor_sync(0xffffffff, most, o));
+  most = __reduce_max_sync(0xffffffff, most);
   if (WARPS > 1) {
     if (lane == 0) most_s[warp] = most;
-    __syncthreads();
+    __syncthreads();  // and every warp has read the old magnitude before one replaces it
     const int w0 = warp / WARPS * WARPS;
 #pragma unroll
     for (int i = 0; i < WARPS; ++i) most = max(most, most_s[w0 + i]);
   }
-  const long long row0 = ((long long)page * p.Hkv + h) * p.page_size + off;  // the block's first token
-  float* ap = p.absmax[kv] + row0 / BLOCK;
-  const bool live = on && base < start;
-  const float was = live ? *ap : 0.f;
-  // every warp of the item has read the old magnitude before one replaces it
-  if (WARPS > 1) __syncthreads();
   if (!on) return;
   const float fresh = bits_to_float<T>((unsigned short)most);
   const bool finite = fresh < INFINITY;  // false for NaN, too
   const float now = finite ? (was >= fresh || was != was ? was : fresh) : __int_as_float(0x7fffffff);
   if (lane == 0 && warp % WARPS == 0) *ap = now;
-  // products with 127 stay finite; scaling by a power of two changes no quotient
-  const float pre = now > 1e30f ? 0x1p-16f : 1.f;
-  const float by = now * pre, mul = 127.f * pre, old = was * pre;
+  // scaled by a power of two, which changes no quotient, magnitude and products stay normal numbers
+  const float pre = now > 1e30f ? 0x1p-16f : now < 1e-30f ? 0x1p40f : 1.f;
   const bool some = now > 0.f;
+  const float by = some ? now * pre : 1.f, r = 1.f / by, mul = some ? 127.f * pre : 0.f;
+  signed char* dst = p.cache[kv] + (row0 + first) * D;
+#pragma unroll 2
+  for (int i = lane; i < n * LPT; i += 32) {
+    const uint4 v = lds128(held + (i - lane) * 16);
+    const unsigned short* e = reinterpret_cast<const unsigned short*>(&v);
+    unsigned q[8];
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const int t = t0 + i * TPI;
-    signed char* dst = p.cache[kv] + (row0 + t) * D + c * 8;
-    uint2 out;
-    signed char* q = reinterpret_cast<signed char*>(&out);
-    if (base + t >= start && base + t < end) {
-      const unsigned short* e = reinterpret_cast<const unsigned short*>(&raw[i]);
+    for (int j = 0; j < 8; ++j) q[j] = round_quotient(some ? bits_to_float<T>(e[j]) * mul : 0.f, by, r);
+    *reinterpret_cast<uint2*>(dst + i * 8) =
+        make_uint2(low_bytes(q[0], q[1], q[2], q[3]), low_bytes(q[4], q[5], q[6], q[7]));
+  }
+  if (now > was && base < start) {  // live tokens under a magnitude that grew
+    const float old = was * pre;
+    uint2* live = reinterpret_cast<uint2*>(p.cache[kv] + (row0 + mine) * D);
+#pragma unroll 1
+    for (int i = lane; i < min(start - base - mine, TOK) * LPT; i += 32) {
+      const uint2 v = live[i];
+      const signed char* e = reinterpret_cast<const signed char*>(&v);
+      unsigned q[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        const float v = some ? rintf(__fdiv_rn(bits_to_float<T>(e[j]) * mul, by)) : 0.f;
-        q[j] = (signed char)(int)fminf(fmaxf(v, -127.f), 127.f);
-      }
-      *reinterpret_cast<uint2*>(dst) = out;
-    } else if (base + t < start && now > was) {  // live under a magnitude that grew
-      out = *reinterpret_cast<const uint2*>(dst);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) q[j] = (signed char)(int)rintf(__fdiv_rn((float)q[j] * old, by));
-      *reinterpret_cast<uint2*>(dst) = out;
+      for (int j = 0; j < 8; ++j) q[j] = round_quotient((float)e[j] * old, by, r);
+      live[i] = make_uint2(low_bytes(q[0], q[1], q[2], q[3]), low_bytes(q[4], q[5], q[6], q[7]));
     }
   }
 }
@@ -147,42 +190,67 @@ struct GatherParams {
   const int* starts;  // null: from token 0
   const int* lens;
   void* out[2];       // [B, total, Hkv, D]
-  int B, total, Hkv, page_size, n_pages, max_pages, block;
+  int B, total, Hkv, page_size, n_pages, max_pages;
+  int blocks_per_page, block_bits;  // magnitudes per page and head; log2(block)
 };
 
 constexpr float kStep = 1.f / 127.f;
 
-// One thread per 16 values of k and the same 16 of v.
+// integers of a word (as q + 128) to four fp32 numbers: under the high bytes of 2^23 a byte is 2^23 + u
+__device__ __forceinline__ void word_to_floats(unsigned u, float* v) {
+#pragma unroll
+  for (int j = 0; j < 4; ++j) v[j] = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7440 | j)) - 8388736.f;
+}
+
+constexpr int kGatherTokens = 64;  // of a CTA
+
+// Grid (tokens, heads, rows); a lane 16 values of k and the same 16 of v.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) kv8_gather_kernel(const GatherParams p) {
-  constexpr int C = D / 16;
-  const long long n = (long long)p.B * p.total * p.Hkv * C;
-  for (long long i = blockIdx.x * 256LL + threadIdx.x; i < n; i += gridDim.x * 256LL) {
-    const int c = (int)(i % C);
-    const long long r = i / C;
-    const int h = (int)(r % p.Hkv);
-    const long long bt = r / p.Hkv;
-    const int t = (int)(bt % p.total), b = (int)(bt / p.total);
-    const int pos = (p.starts ? p.starts[b] : 0) + t;
+  constexpr int C = D / 16, PER = 256 / C, N = kGatherTokens / PER;
+  const int b = blockIdx.z, h = blockIdx.y, c = threadIdx.x % C;
+  begin_early();
+  const int start = p.starts ? min(max(p.starts[b], -(1 << 30)), 1 << 30) : 0, len = p.lens[b];
+  const int t0 = blockIdx.x * kGatherTokens + threadIdx.x / C;
+  uint4 raw[N][2];
+  float step[N][2];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int t = t0 + i * PER, pos = start + t, lp = pos / p.page_size;
     int page = -1;
-    if (pos >= 0 && pos < p.lens[b] && pos / p.page_size < p.max_pages)
-      page = p.table[(long long)b * p.max_pages + pos / p.page_size];
-    const bool ok = page >= 0 && page < p.n_pages;
-    const long long row = ((long long)page * p.Hkv + h) * p.page_size + pos % p.page_size;
+    if (t < p.total && pos >= 0 && pos < len && lp < p.max_pages) page = p.table[(long long)b * p.max_pages + lp];
+    raw[i][0] = raw[i][1] = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);  // zeros, below
+    step[i][0] = step[i][1] = 0.f;
+    if (page >= 0 && page < p.n_pages) {
+      const long long head = (long long)page * p.Hkv + h;
+      const int in = pos - lp * p.page_size;
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) {
+        const uint4 v = *reinterpret_cast<const uint4*>(p.cache[kv] + (head * p.page_size + in) * D + c * 16);
+        raw[i][kv] = make_uint4(v.x ^ 0x80808080u, v.y ^ 0x80808080u, v.z ^ 0x80808080u, v.w ^ 0x80808080u);
+        step[i][kv] = p.absmax[kv][head * p.blocks_per_page + (in >> p.block_bits)] * kStep;
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int t = t0 + i * PER;
+    if (t >= p.total) break;
 #pragma unroll
     for (int kv = 0; kv < 2; ++kv) {
-      uint4 o[2] = {make_uint4(0u, 0u, 0u, 0u), make_uint4(0u, 0u, 0u, 0u)};
-      if (ok) {
-        const uint4 raw = *reinterpret_cast<const uint4*>(p.cache[kv] + row * D + c * 16);
-        const float step = p.absmax[kv][row / p.block] * kStep;
-        const signed char* q = reinterpret_cast<const signed char*>(&raw);
-        T* v = reinterpret_cast<T*>(o);
+      const unsigned u[4] = {raw[i][kv].x, raw[i][kv].y, raw[i][kv].z, raw[i][kv].w};
+      unsigned o[8];
 #pragma unroll
-        for (int j = 0; j < 16; ++j) v[j] = from_float<T>((float)q[j] * step);
+      for (int j = 0; j < 4; ++j) {
+        float v[4];
+        word_to_floats(u[j], v);
+        o[2 * j] = pack_pair<T>(v[0] * step[i][kv], v[1] * step[i][kv]);
+        o[2 * j + 1] = pack_pair<T>(v[2] * step[i][kv], v[3] * step[i][kv]);
       }
-      uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.out[kv]) + i * 16);
-      dst[0] = o[0];
-      dst[1] = o[1];
+      uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(p.out[kv]) +
+                                            (((long long)b * p.total + t) * p.Hkv + h) * D + c * 16);
+      dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
+      dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
     }
   }
 }
@@ -219,22 +287,6 @@ constexpr float kNone = -1.7e38f;
 // reach 2^8, far inside fp16, and most tiles need no reduction over lanes and no rescaling.
 constexpr float kSlack = 8.f;
 
-__device__ __forceinline__ void cp_async16(unsigned dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async4(unsigned dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
-}
-__device__ __forceinline__ uint4 lds128(unsigned a) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(a) : "memory");
-  return v;
-}
 __device__ __forceinline__ float2 lds_float2(unsigned a) {
   float2 v;
   asm volatile("ld.shared.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(a) : "memory");
@@ -359,8 +411,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv8_attend_kerne
   __shared__ float2 mag_s[kWarps][STAGES];  // magnitudes of k and v of the tiles in the ring
   // This grid may have been scheduled before the one before it ended. The combine may be scheduled from
   // here on: what it reads before its own wait is then complete.
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  begin_early();
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const unsigned ring = (unsigned)__cvta_generic_to_shared(smem) + warp * SLOT;
@@ -805,24 +856,6 @@ __global__ void __launch_bounds__(128) kv8_combine_kernel(const AttendParams p, 
 
 constexpr int stages_for(int NT) { return NT == 1 ? 3 : 6; }
 
-// With the attribute a kernel may be scheduled while the one before it on the stream still runs; it waits
-// for that one's end itself, so completion stays transitive along the stream.
-template <typename... A>
-void launch_early(void (*kernel)(A...), int grid, int threads, int smem, cudaStream_t s, A... args) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)grid);
-  cfg.blockDim = dim3((unsigned)threads);
-  cfg.dynamicSmemBytes = (size_t)smem;
-  cfg.stream = s;
-  cudaLaunchAttribute at{};
-  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &at;
-  cfg.numAttrs = 1;
-  note_launch();
-  cudaLaunchKernelEx(&cfg, kernel, args...);
-}
-
 template <typename T, int D, int NT>
 void launch_attend(const AttendParams& p, bool combine, cudaStream_t s) {
   constexpr int smem = kWarps * stages_for(NT) * 2 * kTile * D;
@@ -834,10 +867,11 @@ void launch_attend(const AttendParams& p, bool combine, cudaStream_t s) {
     cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (dev >= 0 && dev < 64) set[dev] = true;
   }
-  launch_early(kernel, p.ctas, kWarps * 32, smem, s, p);
+  launch_early(kernel, dim3(p.ctas), dim3(kWarps * 32), smem, s, p);
   if (!combine) return;
   const int rows = std::min(8 * NT, p.S * p.G);
-  launch_early(kv8_combine_kernel<T, D, 8 * NT>, p.B * p.Hkv * p.groups * rows, 128, 0, s, p, rows);
+  launch_early(kv8_combine_kernel<T, D, 8 * NT>, dim3((unsigned)(p.B * p.Hkv * p.groups * rows)), dim3(128), 0, s, p,
+               rows);
 }
 
 }  // namespace
@@ -867,10 +901,10 @@ void kv8_append(const void* k, const long long* ks, const void* v, const long lo
   const int blocks = (int)((items + per_cta - 1) / per_cta);
 #define ASTRAI_APPEND(T, D_)                                                                     \
   switch (block) {                                                                               \
-    case 16: (note_launch(), kv8_append_kernel<T, D_, 16><<<blocks, 128, 0, s>>>(p)); break;     \
-    case 32: (note_launch(), kv8_append_kernel<T, D_, 32><<<blocks, 128, 0, s>>>(p)); break;     \
-    case 64: (note_launch(), kv8_append_kernel<T, D_, 64><<<blocks, 128, 0, s>>>(p)); break;     \
-    default: (note_launch(), kv8_append_kernel<T, D_, 128><<<blocks, 128, 0, s>>>(p)); break;    \
+    case 16: launch_early(kv8_append_kernel<T, D_, 16>, dim3(blocks), dim3(128), 0, s, p); break; \
+    case 32: launch_early(kv8_append_kernel<T, D_, 32>, dim3(blocks), dim3(128), 0, s, p); break; \
+    case 64: launch_early(kv8_append_kernel<T, D_, 64>, dim3(blocks), dim3(128), 0, s, p); break; \
+    default: launch_early(kv8_append_kernel<T, D_, 128>, dim3(blocks), dim3(128), 0, s, p); break; \
   }
   if (dtype == 0 && D == 128) { ASTRAI_APPEND(__nv_bfloat16, 128) }
   else if (dtype == 0) { ASTRAI_APPEND(__nv_bfloat16, 64) }
@@ -881,21 +915,21 @@ void kv8_append(const void* k, const long long* ks, const void* v, const long lo
 
 void kv8_gather(const void* kc, const void* vc, const float* ka, const float* va, const int* table, const int* starts,
                 const int* lens, void* ko, void* vo, int B, int total, int Hkv, int D, int page_size, int n_pages,
-                int max_pages, int block, int dtype, int device, cudaStream_t s) {
+                int max_pages, int block, int dtype, cudaStream_t s) {
   using namespace astrai;
   GatherParams p{};
   p.cache[0] = static_cast<const signed char*>(kc), p.cache[1] = static_cast<const signed char*>(vc);
   p.absmax[0] = ka, p.absmax[1] = va, p.table = table, p.starts = starts, p.lens = lens;
   p.out[0] = ko, p.out[1] = vo;
   p.B = B, p.total = total, p.Hkv = Hkv, p.page_size = page_size, p.n_pages = n_pages, p.max_pages = max_pages;
-  p.block = block;
-  const long long n = (long long)B * total * Hkv * (D / 16);
-  if (n <= 0) return;
-  const int blocks = (int)std::min<long long>((n + 255) / 256, num_sms(device) * 32LL);
-  if (dtype == 0 && D == 128) (note_launch(), kv8_gather_kernel<__nv_bfloat16, 128><<<blocks, 256, 0, s>>>(p));
-  else if (dtype == 0) (note_launch(), kv8_gather_kernel<__nv_bfloat16, 64><<<blocks, 256, 0, s>>>(p));
-  else if (D == 128) (note_launch(), kv8_gather_kernel<__half, 128><<<blocks, 256, 0, s>>>(p));
-  else (note_launch(), kv8_gather_kernel<__half, 64><<<blocks, 256, 0, s>>>(p));
+  p.blocks_per_page = page_size / block;
+  while ((1 << p.block_bits) < block) ++p.block_bits;
+  if (B <= 0 || total <= 0) return;
+  const dim3 grid((total + kGatherTokens - 1) / kGatherTokens, Hkv, B);
+  if (dtype == 0 && D == 128) launch_early(kv8_gather_kernel<__nv_bfloat16, 128>, grid, dim3(256), 0, s, p);
+  else if (dtype == 0) launch_early(kv8_gather_kernel<__nv_bfloat16, 64>, grid, dim3(256), 0, s, p);
+  else if (D == 128) launch_early(kv8_gather_kernel<__half, 128>, grid, dim3(256), 0, s, p);
+  else launch_early(kv8_gather_kernel<__half, 64>, grid, dim3(256), 0, s, p);
 }
 
 // Launch shape of an attention call, from sizes the host knows (not the lengths, which are on the

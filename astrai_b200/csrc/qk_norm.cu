@@ -20,6 +20,7 @@
 #include <cuda_fp16.h>
 
 #include "common.cuh"
+#include "launch.cuh"
 
 namespace astrai {
 namespace {
@@ -316,6 +317,7 @@ __global__ void __launch_bounds__(384, 2) qk_norm_fwd_kernel(const QkNormParams 
   const int lane = threadIdx.x, sub = lane / LPH;
   const Place<HALF> at(lane % LPH, p);
   const Share sh(p, threadIdx.y, blockDim.y);
+  begin_early();
   const int row = blockIdx.x * blockDim.z + threadIdx.z;
   if (row >= p.rows) return;
   const T* x = static_cast<const T*>(p.x) + (long long)row * p.ldx + sh.col0 + sub * p.D;
@@ -372,7 +374,7 @@ __global__ void __launch_bounds__(32 * (kMaxWarps + 1), 2) qk_norm_rows_kernel(c
     }
     fence_mbar_init();
   }
-  if (BWD) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");  // the sum over CTAs waits for this grid
+  begin_early();
   __syncthreads();
   Head dw = zero_head();
   Place<HALF> at(lane % LPH, p);
@@ -475,12 +477,11 @@ __global__ void __launch_bounds__(32 * (kMaxWarps + 1), 2) qk_norm_rows_kernel(c
 // dw[c] = sum over blocks of part[block][c], c over both weights: 8 columns (one sector of each
 // partial row) per CTA, 32 rows of threads.
 template <typename T>
-__global__ void __launch_bounds__(256) qk_norm_dw_kernel(const float* __restrict__ part, int blocks, int D,
-                                                         T* __restrict__ dwq, T* __restrict__ dwk) {
+__global__ void __launch_bounds__(256) qk_norm_dw_kernel(const float* part, int blocks, int D, T* dwq, T* dwk) {
+  begin_early();
   __shared__ float s[8][8];
   const int tx = threadIdx.x & 7, ty = threadIdx.x >> 3;
   const int c = blockIdx.x * 8 + tx;
-  asm volatile("griddepcontrol.wait;" ::: "memory");
   float a = 0.f;
 #pragma unroll 10
   for (int b = ty; b < blocks; b += 32) a += part[(long long)b * 2 * D + c];
@@ -516,14 +517,14 @@ void launch_rows(const QkNormParams& p, const Launch& l, cudaStream_t s) {
   auto kernel = qk_norm_rows_kernel<T, LPH, HALF, NORM, EVEN, BWD>;
   static bool set[64] = {};
   allow_smem(kernel, kRowsSmem, set);
-  (note_launch(), kernel<<<l.blocks, l.block, l.smem, s>>>(p, l.chunk));
+  launch_early(kernel, dim3(l.blocks), l.block, l.smem, s, p, l.chunk);
 }
 template <typename T, int LPH, bool HALF, int NORM, bool BWD>
 void launch(const QkNormParams& p, const Launch& l, cudaStream_t s) {
   constexpr int HPW = 32 / LPH;
   if constexpr (BWD && NORM == kNone) return;  // the transposed rotation is a forward call
   if (!BWD && l.chunk == 0)
-    (note_launch(), qk_norm_fwd_kernel<T, LPH, HALF, NORM><<<l.blocks, l.block, 0, s>>>(p));
+    launch_early(qk_norm_fwd_kernel<T, LPH, HALF, NORM>, dim3(l.blocks), l.block, 0, s, p);
   else if (p.D == 8 * LPH && p.hq % HPW == 0 && p.hkv % HPW == 0) launch_rows<T, LPH, HALF, NORM, true, BWD>(p, l, s);
   else launch_rows<T, LPH, HALF, NORM, false, BWD>(p, l, s);
 }
@@ -547,18 +548,8 @@ void by_mode(const QkNormParams& p, const Launch& l, bool half_layout, int norm,
 }
 template <typename T>
 void sum_dw(const QkNormParams& p, int blocks, void* dwq, void* dwk, cudaStream_t s) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(2 * p.D / 8);
-  cfg.blockDim = dim3(256);
-  cfg.stream = s;
-  cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = &attr;
-  cfg.numAttrs = 1;
-  note_launch();
-  cudaLaunchKernelEx(&cfg, qk_norm_dw_kernel<T>, (const float*)p.dw_part, blocks, p.D, static_cast<T*>(dwq),
-                     static_cast<T*>(dwk));
+  launch_early(qk_norm_dw_kernel<T>, dim3(2 * p.D / 8), dim3(256), 0, s, (const float*)p.dw_part, blocks, p.D,
+               static_cast<T*>(dwq), static_cast<T*>(dwk));
 }
 
 }  // namespace
