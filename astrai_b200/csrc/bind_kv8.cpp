@@ -8,14 +8,13 @@
 
 namespace astrai_host {
 bool kv8_block_supported(int block);
-int kv8_max_batch();
 void kv8_append(const void* k, const long long* ks, const void* v, const long long* vs, void* kc, void* vc, float* ka,
                 float* va, const int* table, const int* starts, const int* lens, int B, int S, int Hkv, int D,
                 int page_size, int n_pages, int max_pages, int block, int dtype, cudaStream_t s);
 void kv8_gather(const void* kc, const void* vc, const float* ka, const float* va, const int* table, const int* starts,
                 const int* lens, void* ko, void* vo, int B, int total, int Hkv, int D, int page_size, int n_pages,
                 int max_pages, int block, int dtype, cudaStream_t s);
-void kv8_attend_plan(int B, int S, int Hq, int Hkv, int D, int page_size, int max_pages, int device, long long* out);
+long long kv8_attend_workspace(int B, int S, int Hq, int Hkv, int D, int page_size, int max_pages, int device);
 void kv8_attend(const void* q, const long long* qs, const void* kc, const void* vc, const float* ka, const float* va,
                 const int* table, const int* lens, const int* starts, void* out, float* workspace, int B, int S,
                 int Hq, int Hkv, int D, int page_size, int n_pages, int max_pages, int block, float scale, int dtype,
@@ -165,10 +164,8 @@ int64_t kv8_attend_workspace(int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int6
                   max_pages * page_size < (1LL << 30) && S * (Hq / Hkv) < (1LL << 24),
               "kv8_attend_workspace: sizes");
   if (B == 0 || S == 0) return 0;
-  long long plan[6];
-  astrai_host::kv8_attend_plan((int)B, (int)S, (int)Hq, (int)Hkv, (int)D, (int)page_size, (int)max_pages, (int)device,
-                               plan);
-  return plan[4];
+  return astrai_host::kv8_attend_workspace((int)B, (int)S, (int)Hq, (int)Hkv, (int)D, (int)page_size, (int)max_pages,
+                                           (int)device);
 }
 
 at::Tensor kv8_attend(const at::Tensor& q_in, const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ka,
@@ -182,8 +179,6 @@ at::Tensor kv8_attend(const at::Tensor& q_in, const at::Tensor& kc, const at::Te
   const int64_t B = q.size(0), S = q.size(1), Hq = q.size(2);
   TORCH_CHECK(q.size(3) == c.D && Hq % c.Hkv == 0 && Hq >= 1, "kv8_attention: q ", text(q.sizes()),
               " does not fit the cache ", text(kc.sizes()));
-  TORCH_CHECK(B <= astrai_host::kv8_max_batch(), "kv8_attention: at most ",
-              text((int64_t)astrai_host::kv8_max_batch()), " rows");
   const int mp = check_table(table, kc, B, c);
   const int* ln = check_i32(lens, kc, B, "lens");
   at::Tensor starts;
@@ -193,7 +188,7 @@ at::Tensor kv8_attend(const at::Tensor& q_in, const at::Tensor& kc, const at::Te
     st = check_i32(starts, kc, B, "starts");
   }
   const int64_t units = ((int64_t)mp * c.page_size + 127) / 128, rows = S * (Hq / c.Hkv);
-  TORCH_CHECK(rows < (1LL << 24) && units * B < (1LL << 31) && units * c.Hkv * (rows / 8 + 1) < (1LL << 31) &&
+  TORCH_CHECK(rows < (1LL << 24) && (units + 8) * 1024 < (1LL << 31) && (units + 8) * c.Hkv * (rows / 8 + 1) < (1LL << 31) &&
                   B * c.Hkv * (rows + 16) < (1LL << 31),
               "kv8_attention: too many rows or pages");
   const int64_t need = kv8_attend_workspace(B, S, Hq, c.Hkv, c.D, c.page_size, mp, q.device().index());

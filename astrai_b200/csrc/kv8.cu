@@ -278,9 +278,8 @@ struct AttendParams {
 constexpr int kWarps = 8;
 constexpr int kTile = 16;                // tokens per warp step
 constexpr int kUnit = kWarps * kTile;    // tokens per unit of work: one step of all warps
-constexpr int kPad = 2;                  // units that a segment's start weighs when work is dealt out
-constexpr int kWhole = 4 * kUnit;       // tokens up to which a row is not split
-constexpr int kMaxBatch = 2048;
+constexpr int kPad = 4;                  // units that a segment's start weighs when work is dealt out
+constexpr int kMaxBatch = 1024;        // rows of a launch
 // Running maxima start here: below every score, and finite, so that no difference of maxima is NaN.
 constexpr float kNone = -1.7e38f;
 // A running maximum follows the scores only when they pass it by this much (powers of two): weights then
@@ -330,17 +329,16 @@ __device__ __forceinline__ unsigned bytes_to_half2(unsigned u, unsigned sel) {
   return *reinterpret_cast<const unsigned*>(&r);
 }
 
-// Tokens that the queries of row b see at most, and the position of its first query.
-__device__ __forceinline__ void row_extent(const AttendParams& p, int b, int& first, int& keys) {
-  const int len = max(p.lens[b], 0);
+// Tokens that the queries of row b, of length len, see at most, and the position of its first query.
+__device__ __forceinline__ void row_extent(const AttendParams& p, int b, int len, int& first, int& keys) {
   first = p.starts ? min(max(p.starts[b], -(1 << 30)), 1 << 30) : len - p.S;
   keys = max(0, min(min(len, first + p.S), p.max_pages * p.page_size));
 }
 // Units of row b in the dealing: those of its keys (a row without keys still has its zeros to write), behind
 // kPad that stand for what starting and merging a piece costs.
-__device__ __forceinline__ int row_units(const AttendParams& p, int b) {
+__device__ __forceinline__ int row_units(const AttendParams& p, int b, int len) {
   int first, keys;
-  row_extent(p, b, first, keys);
+  row_extent(p, b, len, first, keys);
   const int tokens = p.unit_tiles * kTile;
   return kPad + max(1, (keys + tokens - 1) / tokens);
 }
@@ -393,7 +391,7 @@ struct Piece {       // of a segment, on one CTA
   int b, h, grp;     // row, kv head, group
   int unit0, units;  // its first unit of keys and their number
   int dealt;         // units taken from the dealing, those that stand for the start among them
-  int first, keys;   // of the row
+  int len, first, keys;  // of the row
   bool whole;
 };
 
@@ -406,6 +404,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv8_attend_kerne
   constexpr int SLOT = 2 * TB;   // a ring slot: a tile of keys, then one of values
   extern __shared__ __align__(128) unsigned char smem[];  // [stage][warp][SLOT]
   __shared__ int prefix[kMaxBatch + 1];
+  __shared__ int len_s[kMaxBatch];
   __shared__ int scan_s[kWarps];
   __shared__ float stat_s[kWarps][R][3];
   __shared__ float2 mag_s[kWarps][STAGES];  // magnitudes of k and v of the tiles in the ring
@@ -421,7 +420,11 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv8_attend_kerne
   int before = 0;
   for (int b0 = 0; b0 < p.B; b0 += kWarps * 32) {
     const int b = b0 + tid;
-    int v = b < p.B ? row_units(p, b) : 0;
+    int v = 0;
+    if (b < p.B) {
+      len_s[b] = max(p.lens[b], 0);
+      v = row_units(p, b, len_s[b]);
+    }
     const int own = v;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -471,7 +474,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv8_attend_kerne
     c.units = max(0, at + c.dealt - kPad) - c.unit0;
     c.whole = c.units == all - kPad;
     c.h = hg / p.groups, c.grp = hg - c.h * p.groups;
-    row_extent(p, lo, c.first, c.keys);
+    c.len = len_s[lo];
+    row_extent(p, lo, c.len, c.first, c.keys);
     return c;
   };
 
@@ -542,7 +546,6 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv8_attend_kerne
     float qscale[NT][2], qbias[NT][2];  // of the columns 2t, 2t + 1 of S^T
     int vis[NT][2];                     // keys that those columns see
     int seen_by_all = c.keys;
-    const int len = p.lens[c.b];
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
       const unsigned short* e = reinterpret_cast<const unsigned short*>(q_raw[n]);
@@ -578,7 +581,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv8_attend_kerne
         qscale[n][k] *= 0x1p24f;
         const int rc = c.grp * R + n * 8 + 2 * t + k, pos = c.first + rc / p.G;
         // columns behind the last query row are computed like the others and never written
-        vis[n][k] = rc >= p.S * p.G ? c.keys : pos >= 0 && pos < len ? min(pos + 1, c.keys) : 0;
+        vis[n][k] = rc >= p.S * p.G ? c.keys : pos >= 0 && pos < c.len ? min(pos + 1, c.keys) : 0;
         seen_by_all = min(seen_by_all, vis[n][k]);
       }
     }
@@ -785,34 +788,32 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv8_attend_kerne
   }
 }
 
-// Joins the pieces of a segment that several CTAs worked on: one CTA per (segment, query row). Four
-// warps take the pieces in turn, a lane D / 32 channels, and are merged at the end.
-template <typename T, int D, int R>
-__global__ void __launch_bounds__(128) kv8_combine_kernel(const AttendParams p, int rows) {
-  constexpr int C = D / 32;
-  __shared__ int sums[2][4];
-  __shared__ float stat_s[4][3], o_s[4][D];
+// Joins the pieces of a segment that several CTAs worked on: one CTA per (segment, query row). Its warps
+// take the pieces in turn, a lane D / 32 channels, and are merged at the end.
+template <typename T, int D, int R, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS) kv8_combine_kernel(const AttendParams p, int rows) {
+  constexpr int C = D / 32, N = 8;  // pieces of a warp whose loads are in flight together
+  __shared__ int sums[2][WARPS];
+  __shared__ float stat_s[WARPS][3], o_s[WARPS][D];
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int seg = blockIdx.x / rows, row = blockIdx.x - seg * rows;
   const int per = p.Hkv * p.groups, b = seg / per, hg = seg - b * per;
   const int h = hg / p.groups, grp = hg - h * p.groups, r = grp * R + row;
   int pre = 0, all = 0;
-  for (int i = tid; i < p.B; i += 128) {
-    const int v = row_units(p, i);
+  for (int i = tid; i < p.B; i += 32 * WARPS) {
+    const int v = row_units(p, i, max(p.lens[i], 0));
     all += v;
     pre += i < b ? v : 0;
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    all += __shfl_xor_sync(0xffffffff, all, o);
-    pre += __shfl_xor_sync(0xffffffff, pre, o);
-  }
+  all = __reduce_add_sync(0xffffffff, all);
+  pre = __reduce_add_sync(0xffffffff, pre);
   if (lane == 0) sums[0][warp] = all, sums[1][warp] = pre;
+  const int units = row_units(p, b, max(p.lens[b], 0));
   __syncthreads();
-  all = sums[0][0] + sums[0][1] + sums[0][2] + sums[0][3];
-  pre = sums[1][0] + sums[1][1] + sums[1][2] + sums[1][3];
-  const int units = row_units(p, b);
+  all = pre = 0;
+#pragma unroll
+  for (int i = 0; i < WARPS; ++i) all += sums[0][i], pre += sums[1][i];
   const long long total = (long long)all * per;
   const long long u1 = (long long)pre * per + (long long)(hg + 1) * units, u0 = u1 - units + kPad;  // of the keys
   const int ctas = live_ctas(p, total);
@@ -822,18 +823,34 @@ __global__ void __launch_bounds__(128) kv8_combine_kernel(const AttendParams p, 
   float m = kNone, M = kNone, sum = 0.f, a[C];
 #pragma unroll
   for (int i = 0; i < C; ++i) a[i] = 0.f;
-#pragma unroll 4
-  for (int c = c0 + warp; c <= c1; c += 4) {
-    const long long slot = 2LL * c + (total * c / ctas > u0 ? 0 : 1);  // 0: the CTA begins inside the keys
-    const float* st = p.part_s + (slot * R + row) * 3;
-    const float* src = p.part_o + (slot * R + row) * D + lane * C;
-    float v[C];
-    load_floats<C>(src, v);
-    const float m1 = fmaxf(m, st[0]), M1 = fmaxf(M, st[1]);
-    const float f = ex2(M - M1), e = ex2(st[1] - M1);
-    sum = sum * ex2(m - m1) + st[2] * ex2(st[0] - m1);
+  for (int c = c0 + warp; c <= c1; c += N * WARPS) {
+    float st[N][3], v[N][C];
 #pragma unroll
-    for (int i = 0; i < C; ++i) a[i] = a[i] * f + v[i] * e;
+    for (int k = 0; k < N; ++k) {
+      const int ck = c + k * WARPS;
+      st[k][0] = st[k][1] = kNone, st[k][2] = 0.f;
+#pragma unroll
+      for (int i = 0; i < C; ++i) v[k][i] = 0.f;
+      if (ck > c1) continue;
+      const long long slot = 2LL * ck + (total * ck / ctas > u0 ? 0 : 1);  // 0: the CTA begins inside the keys
+      const float* s = p.part_s + (slot * R + row) * 3;
+      st[k][0] = s[0], st[k][1] = s[1], st[k][2] = s[2];
+      load_floats<C>(p.part_o + (slot * R + row) * D + lane * C, v[k]);
+    }
+    float m1 = m, M1 = M;
+#pragma unroll
+    for (int k = 0; k < N; ++k) m1 = fmaxf(m1, st[k][0]), M1 = fmaxf(M1, st[k][1]);
+    const float f = ex2(M - M1);
+    sum *= ex2(m - m1);
+#pragma unroll
+    for (int i = 0; i < C; ++i) a[i] *= f;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const float e = ex2(st[k][1] - M1);
+      sum += st[k][2] * ex2(st[k][0] - m1);
+#pragma unroll
+      for (int i = 0; i < C; ++i) a[i] += v[k][i] * e;
+    }
     m = m1, M = M1;
   }
   if (lane == 0) stat_s[warp][0] = m, stat_s[warp][1] = M, stat_s[warp][2] = sum;
@@ -843,9 +860,9 @@ __global__ void __launch_bounds__(128) kv8_combine_kernel(const AttendParams p, 
   if (tid >= D) return;
   float mm = kNone, MM = kNone, l = 0.f, o = 0.f;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) mm = fmaxf(mm, stat_s[i][0]), MM = fmaxf(MM, stat_s[i][1]);
+  for (int i = 0; i < WARPS; ++i) mm = fmaxf(mm, stat_s[i][0]), MM = fmaxf(MM, stat_s[i][1]);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < WARPS; ++i) {
     l += stat_s[i][2] * ex2(stat_s[i][0] - mm);
     o += o_s[i][tid] * ex2(stat_s[i][1] - MM);
   }
@@ -869,9 +886,11 @@ void launch_attend(const AttendParams& p, bool combine, cudaStream_t s) {
   }
   launch_early(kernel, dim3(p.ctas), dim3(kWarps * 32), smem, s, p);
   if (!combine) return;
-  const int rows = std::min(8 * NT, p.S * p.G);
-  launch_early(kv8_combine_kernel<T, D, 8 * NT>, dim3((unsigned)(p.B * p.Hkv * p.groups * rows)), dim3(128), 0, s, p,
-               rows);
+  const int rows = std::min(8 * NT, p.S * p.G), segs = p.B * p.Hkv * p.groups;
+  // warps for the pieces that a segment has on average: with 3 pieces 4 warps take 2 us less than 8, with 64
+  // pieces 1 us more
+  if (p.ctas < 12 * segs) launch_early(kv8_combine_kernel<T, D, 8 * NT, 4>, dim3(segs * rows), dim3(128), 0, s, p, rows);
+  else launch_early(kv8_combine_kernel<T, D, 8 * NT, 8>, dim3(segs * rows), dim3(256), 0, s, p, rows);
 }
 
 }  // namespace
@@ -880,7 +899,6 @@ void launch_attend(const AttendParams& p, bool combine, cudaStream_t s) {
 namespace astrai_host {
 
 bool kv8_block_supported(int block) { return block == 16 || block == 32 || block == 64 || block == 128; }
-int kv8_max_batch() { return astrai::kMaxBatch; }
 
 void kv8_append(const void* k, const long long* ks, const void* v, const long long* vs, void* kc, void* vc, float* ka,
                 float* va, const int* table, const int* starts, const int* lens, int B, int S, int Hkv, int D,
@@ -932,21 +950,52 @@ void kv8_gather(const void* kc, const void* vc, const float* ka, const float* va
   else launch_early(kv8_gather_kernel<__half, 64>, grid, dim3(256), 0, s, p);
 }
 
-// Launch shape of an attention call, from sizes the host knows (not the lengths, which are on the
-// device): out[0] CTAs, out[1] query rows per group (R), out[2] groups, out[3] 1 if a segment can be
-// split over CTAs, out[4] workspace floats, out[5] tokens per unit of work. Rows of at most kWhole tokens
-// are not split: four steps of one CTA take less than joining two CTAs' work.
-void kv8_attend_plan(int B, int S, int Hq, int Hkv, int D, int page_size, int max_pages, int device, long long* out) {
+namespace {
+
+// Launch shape of an attention call, from sizes the host knows: the lengths are on the device, so a row counts
+// as the tokens that its pages hold.
+struct AttendPlan {
+  int R, groups;       // query rows per group, groups
+  int ctas, unit;      // CTAs, tokens per unit of work
+  bool split;          // whether a segment can be split over CTAs
+  long long floats;    // workspace
+};
+
+// Splitting rows over CTAs evens the work out but costs the join, a second piece for many CTAs and, with
+// that, about kJoinUs; whole rows cost the idle slots of the last wave and, if they are few, the rate that one
+// CTA reaches alone. Both sides are estimated from rates measured on B200 (cache bytes: 6 TB/s in all, 36 GB/s
+// for one CTA): at 64 rows of 1024 tokens of 4 heads of 128 whole rows take 18.5 us and split ones 24.0, at 4
+// rows 11.4 and 8.9.
+constexpr double kAllRate = 6e6, kOneRate = 3.6e4, kJoinUs = 3.3;  // bytes per us
+
+AttendPlan attend_plan(int B, int S, int Hq, int Hkv, int D, int page_size, int max_pages, int sms) {
   using namespace astrai;
+  AttendPlan a{};
   const long long cap = (long long)max_pages * page_size;
-  const int rows = S * (Hq / Hkv), R = rows <= 8 ? 8 : 16, groups = (rows + R - 1) / R;
-  const int unit = cap <= kWhole ? kWhole : kUnit;
-  const long long units = std::max<long long>(1, (cap + unit - 1) / unit);
-  const long long most = (long long)B * Hkv * groups * (units > 1 ? units + kPad : 1);
-  const int ctas = (int)std::min<long long>(most, (long long)num_sms(device) * (R == 8 ? 2 : 1));
-  out[0] = ctas, out[1] = R, out[2] = groups, out[3] = units > 1;
-  out[4] = units > 1 ? 2LL * ctas * R * (D + 3) : 0;
-  out[5] = unit;
+  const int rows = S * (Hq / Hkv);
+  a.R = rows <= 8 ? 8 : 16;
+  a.groups = (rows + a.R - 1) / a.R;
+  const long long segs = (long long)B * Hkv * a.groups, slots = (long long)sms * (a.R == 8 ? 2 : 1);
+  const long long units = (cap + kUnit - 1) / kUnit;
+  const double bytes = 2.0 * D * (double)cap;
+  const auto rate = [&](double busy) { return std::min(kOneRate, kAllRate / busy); };
+  const double at_once = (double)std::min(segs, slots), waves = (double)((segs + slots - 1) / slots);
+  const double whole = waves * bytes / rate(at_once);
+  const double spread = (double)std::min(segs * units, slots);
+  const double parts = (double)segs * bytes / (spread * rate(spread)) + kJoinUs;
+  a.split = units > 1 && parts < whole;
+  a.unit = (int)(a.split ? kUnit : std::max<long long>(1, units) * kUnit);
+  a.ctas = (int)std::min(a.split ? segs * (units + kPad) : segs, slots);
+  a.floats = a.split ? 2LL * a.ctas * a.R * (D + 3) : 0;
+  return a;
+}
+
+}  // namespace
+
+// fp32 elements of workspace that kv8_attend needs (0: none)
+long long kv8_attend_workspace(int B, int S, int Hq, int Hkv, int D, int page_size, int max_pages, int device) {
+  // rows beyond the batch of one launch come in launches of their own, one after the other
+  return attend_plan(std::min(B, astrai::kMaxBatch), S, Hq, Hkv, D, page_size, max_pages, num_sms(device)).floats;
 }
 
 void kv8_attend(const void* q, const long long* qs, const void* kc, const void* vc, const float* ka, const float* va,
@@ -955,30 +1004,34 @@ void kv8_attend(const void* q, const long long* qs, const void* kc, const void* 
                 int device, cudaStream_t s) {
   using namespace astrai;
   if (B <= 0 || S <= 0) return;
-  long long plan[6];
-  kv8_attend_plan(B, S, Hq, Hkv, D, page_size, max_pages, device, plan);
-  AttendParams p{};
-  p.q = q, p.qb = qs[0], p.qs = qs[1], p.qh = qs[2];
-  p.kc = static_cast<const signed char*>(kc), p.vc = static_cast<const signed char*>(vc), p.ka = ka, p.va = va;
-  p.table = table, p.lens = lens, p.starts = starts, p.out = out;
-  p.B = B, p.S = S, p.Hq = Hq, p.Hkv = Hkv, p.G = Hq / Hkv, p.groups = (int)plan[2];
-  p.page_size = page_size, p.n_pages = n_pages, p.max_pages = max_pages;
-  p.tiles_per_page = page_size / kTile;
-  p.blocks_per_page = page_size / block;
-  p.unit_tiles = (int)plan[5] / kTile;
-  while ((kTile << p.block_shift) < block) ++p.block_shift;
-  p.ctas = (int)plan[0], p.scale = scale * 1.4426950408889634f * kStep;
-  p.part_o = workspace;
-  p.part_s = workspace ? workspace + 2LL * p.ctas * plan[1] * D : nullptr;
-  const bool wide = plan[1] == 16, combine = plan[3] != 0;
+  for (int b0 = 0; b0 < B; b0 += kMaxBatch) {
+    const int n = std::min(B - b0, kMaxBatch);
+    // the workspace was sized for the first launch; a later, smaller one keeps its shape
+    const AttendPlan a = attend_plan(std::min(B, kMaxBatch), S, Hq, Hkv, D, page_size, max_pages, num_sms(device));
+    AttendParams p{};
+    p.q = static_cast<const char*>(q) + 2LL * b0 * qs[0];
+    p.qb = qs[0], p.qs = qs[1], p.qh = qs[2];
+    p.kc = static_cast<const signed char*>(kc), p.vc = static_cast<const signed char*>(vc), p.ka = ka, p.va = va;
+    p.table = table + (long long)b0 * max_pages, p.lens = lens + b0, p.starts = starts ? starts + b0 : nullptr;
+    p.out = static_cast<char*>(out) + 2LL * b0 * S * Hq * D;
+    p.B = n, p.S = S, p.Hq = Hq, p.Hkv = Hkv, p.G = Hq / Hkv, p.groups = a.groups;
+    p.page_size = page_size, p.n_pages = n_pages, p.max_pages = max_pages;
+    p.tiles_per_page = page_size / kTile;
+    p.blocks_per_page = page_size / block;
+    p.unit_tiles = a.unit / kTile;
+    while ((kTile << p.block_shift) < block) ++p.block_shift;
+    p.ctas = a.ctas, p.scale = scale * 1.4426950408889634f * kStep;
+    p.part_o = workspace;
+    p.part_s = workspace ? workspace + 2LL * p.ctas * a.R * D : nullptr;
 #define ASTRAI_ATTEND(T, D_) \
-  if (wide) launch_attend<T, D_, 2>(p, combine, s); \
-  else launch_attend<T, D_, 1>(p, combine, s);
-  if (dtype == 0 && D == 128) { ASTRAI_ATTEND(__nv_bfloat16, 128) }
-  else if (dtype == 0) { ASTRAI_ATTEND(__nv_bfloat16, 64) }
-  else if (D == 128) { ASTRAI_ATTEND(__half, 128) }
-  else { ASTRAI_ATTEND(__half, 64) }
+  if (a.R == 16) launch_attend<T, D_, 2>(p, a.split, s); \
+  else launch_attend<T, D_, 1>(p, a.split, s);
+    if (dtype == 0 && D == 128) { ASTRAI_ATTEND(__nv_bfloat16, 128) }
+    else if (dtype == 0) { ASTRAI_ATTEND(__nv_bfloat16, 64) }
+    else if (D == 128) { ASTRAI_ATTEND(__half, 128) }
+    else { ASTRAI_ATTEND(__half, 64) }
 #undef ASTRAI_ATTEND
+  }
 }
 
 }  // namespace astrai_host
