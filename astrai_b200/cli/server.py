@@ -4,7 +4,8 @@
 
 Parity: scripts/tools/server.py:9-68 of the reference (same flags). Added:
 ``--n_pages`` / ``--page_size`` serve from a paged KV cache with prefix
-sharing instead of the per-slot cache.
+sharing instead of the per-slot cache; ``--kv_cache_dtype int8`` holds the
+cache as 8-bit integers (``--kv_block`` tokens share a magnitude).
 """
 
 from __future__ import annotations
@@ -29,11 +30,15 @@ def main(argv: Optional[List[str]] = None) -> None:
     p.add_argument("--max_batch_size", type=int, default=16)
     p.add_argument("--n_pages", type=int, default=None, help="Paged KV cache with this many pages.")
     p.add_argument("--page_size", type=int, default=128)
+    p.add_argument("--kv_cache_dtype", default="auto", choices=["auto", "int8"])
+    p.add_argument("--kv_block", type=int, default=32, choices=[16, 32, 64, 128])
     a = p.parse_args(argv)
     if a.param_path is None:
         raise SystemExit("--param_path is required")
     dtype = {"bfloat16": torch.bfloat16, "float16": torch.float16, "float32": torch.float32}[a.dtype]
     extra = {"n_pages": a.n_pages, "page_size": a.page_size} if a.n_pages else {}
+    if a.kv_cache_dtype != "auto":
+        extra.update(kv_cache_dtype=a.kv_cache_dtype, kv_block=a.kv_block)
     run_server(Path(a.param_path), host=a.host, port=a.port, reload=a.reload, device=a.device, dtype=dtype,
                max_batch_size=a.max_batch_size, **extra)
 

@@ -11,7 +11,22 @@ the reference behaviour:
                             ``intermediate_size``);
 * ``moe_aux_loss_coef``  - coefficient of the switch-style balance loss;
 * ``shared_expert_mode`` - ``"mean"`` (reference: shared experts averaged)
-                            or ``"sum"``.
+                            or ``"sum"``;
+* ``rope_layout``        - ``"interleaved"`` (reference) or ``"half"``: channel i
+                            rotates with i + rotated channels / 2;
+* ``rope_fraction``      - share of each head's channels that is rotated, the
+                            first ones (1.0);
+* ``rope_scaling_method`` - ``"linear"`` or ``"yarn"``: long-context scaling of
+                            the angle table with ``rope_scaling``'s ``factor``,
+                            ``original_max_position_embeddings``,
+                            ``beta_fast``, ``beta_slow``, ``attention_factor``
+                            (absent: ``rope_scaling`` means NTK, as in the
+                            reference);
+* ``qk_norm_first``      - QK-norm before the rotation instead of after it;
+* ``fused_qk_norm``      - QK-norm and rotation in one pass over the projection
+                            output, rounded once. Any of ``rope_layout="half"``,
+                            ``rope_fraction < 1`` and ``qk_norm_first`` implies
+                            it. These five apply to ``attn_type="gqa"``.
 """
 
 from __future__ import annotations
@@ -68,6 +83,11 @@ class AutoRegressiveLMConfig(BaseModelConfig):
     moe_intermediate_size: Optional[int] = None
     moe_aux_loss_coef: Optional[float] = None
     shared_expert_mode: Optional[str] = None
+    rope_layout: Optional[str] = None
+    rope_fraction: Optional[float] = None
+    rope_scaling_method: Optional[str] = None
+    qk_norm_first: Optional[bool] = None
+    fused_qk_norm: Optional[bool] = None
 
 
 @ConfigFactory.register("embedding")

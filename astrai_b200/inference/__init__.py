@@ -6,7 +6,8 @@ from astrai_b200.inference.api import (AnthropicMessage, AnthropicResponseBuilde
                                        OpenAIResponseBuilder, ProtocolHandler, SimpleJsonToolParser, StopChecker,
                                        ToolDef, ToolParserFactory, get_app, run_server)
 from astrai_b200.inference.core import (STOP, Allocator, CacheView, ContiguousCache, ContiguousCacheView, Executor,
-                                        InferenceScheduler, KVCache, PageCache, PageCacheView, PagePool, PrefixCache,
+                                        InferenceScheduler, Int8Storage, KVCache, PageCache, PageCacheView, PagePool,
+                                        PrefixCache,
                                         Storage, StreamDecoder, Task, TaskManager, TaskStatus, TaskTable, page_hash)
 from astrai_b200.inference.engine import GenerateResult, GenerationRequest, InferenceEngine
 from astrai_b200.inference.sample import (BaseSamplingStrategy, DeviceRNG, FrequencyPenaltyStrategy, SamplingPipeline,
@@ -15,7 +16,7 @@ from astrai_b200.inference.sample import (BaseSamplingStrategy, DeviceRNG, Frequ
 __all__ = [
     "InferenceEngine", "GenerationRequest", "GenerateResult", "InferenceScheduler", "Executor", "STOP", "Task",
     "TaskManager", "TaskStatus", "StreamDecoder", "Allocator", "CacheView", "KVCache", "ContiguousCache",
-    "ContiguousCacheView", "PageCache", "PageCacheView", "PagePool", "PrefixCache", "Storage", "TaskTable",
+    "ContiguousCacheView", "PageCache", "PageCacheView", "PagePool", "PrefixCache", "Storage", "Int8Storage", "TaskTable",
     "page_hash", "sample", "fused_sample", "DeviceRNG", "BaseSamplingStrategy", "TemperatureStrategy",
     "TopKStrategy", "TopPStrategy", "FrequencyPenaltyStrategy", "SamplingPipeline", "ProtocolHandler",
     "StopChecker", "GenContext", "BaseToolParser", "SimpleJsonToolParser", "ToolParserFactory",

@@ -5,6 +5,7 @@ from astrai_b200.inference.core.cache import (
     CacheView,
     ContiguousCache,
     ContiguousCacheView,
+    Int8Storage,
     KVCache,
     PageCache,
     PageCacheView,
@@ -19,5 +20,6 @@ from astrai_b200.inference.core.scheduler import InferenceScheduler
 from astrai_b200.inference.core.task import STOP, StreamDecoder, Task, TaskManager, TaskStatus
 
 __all__ = ["Allocator", "CacheView", "ContiguousCache", "ContiguousCacheView", "Executor", "InferenceScheduler",
+           "Int8Storage",
            "KVCache", "PageCache", "PageCacheView", "PagePool", "PrefixCache", "STOP", "Storage", "StreamDecoder",
            "Task", "TaskManager", "TaskStatus", "TaskTable", "page_hash"]

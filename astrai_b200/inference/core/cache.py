@@ -23,6 +23,10 @@ Layout and execution differ:
   equal page contents after different prefixes share KV that differs.
 * A prompt never hits all of its pages: at least its last token is
   recomputed, so prefill always produces the logits of the last prompt token.
+* ``kv_dtype="int8"`` holds K/V as 8-bit integers with one magnitude per block
+  of ``kv_block`` tokens and head (:class:`Int8Storage`, :mod:`astrai_b200.ops.kv8`):
+  half the memory of bfloat16 and half the bytes of a decode step. A prompt's
+  own prefill attends to its unrounded k/v; every later step reads the cache.
 """
 
 from __future__ import annotations
@@ -40,6 +44,7 @@ from torch import Tensor
 _MASK64 = 0xFFFFFFFFFFFFFFFF
 HEAD_DIM = 128
 KERNEL_HEAD_DIMS = (64, 128)  # head sizes the cache kernels (write, gather, decode) support
+INT8_ROWS = 64  # query rows of a KV head up to which new tokens attend over an int8 cache in place
 
 
 def _page_hash_step(prev: int, token_ids: Sequence[int], start: int, end: int) -> int:
@@ -312,6 +317,62 @@ class Storage:
         return self.gather_rows(layer_id, page_table, lens, total_len)
 
 
+class Int8Storage(Storage):
+    """K/V pages as 8-bit integers with block magnitudes; ``dtype`` is that of the values written and read."""
+
+    def __init__(self, n_layers: int, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, device,
+                 dtype: torch.dtype, block: int = 32):
+        from astrai_b200.ops.kv8 import KV8
+
+        if torch.device(device).type == "cuda" and (dtype not in (torch.bfloat16, torch.float16)
+                                                    or head_dim not in KERNEL_HEAD_DIMS):
+            raise ValueError(f"an int8 KV cache on CUDA needs bfloat16 or float16 and a head_dim of {KERNEL_HEAD_DIMS}, "
+                             f"got {dtype} and {head_dim}")
+        self.n_layers, self.n_pages, self.page_size = n_layers, n_pages, page_size
+        self.n_kv_heads, self.head_dim, self.dtype, self.block = n_kv_heads, head_dim, dtype, block
+        self.layers = [KV8.allocate(n_pages, n_kv_heads, page_size, head_dim, block, device) for _ in range(n_layers)]
+
+    @property
+    def native_ok(self) -> bool:
+        return self.layers[0].k.is_cuda and self.dtype == torch.bfloat16
+
+    def append_rows(self, layer_id: int, table: Tensor, starts: Tensor, lens: Tensor, k: Tensor, v: Tensor) -> None:
+        """k/v ``[B, S, Hkv, D]`` become tokens ``starts[b] .. lens[b] - 1`` of each row."""
+        from astrai_b200.ops.kv8 import kv8_append
+
+        kv8_append(self.layers[layer_id], k, v, table, starts, lens)
+
+    def attend_rows(self, layer_id: int, q: Tensor, table: Tensor, lens: Tensor) -> Tensor:
+        """Causal attention of the rows' last tokens, q ``[B, S, Hq, D]``, over the cached ones."""
+        from astrai_b200.ops.kv8 import kv8_attention
+
+        return kv8_attention(q, self.layers[layer_id], table, lens)
+
+    def write_slots(self, layer_id: int, slots: Tensor, k: Tensor, v: Tensor) -> None:
+        raise RuntimeError("an int8 KV cache takes consecutive tokens of rows (append_rows), not single slots: "
+                           "the tokens of a block share a magnitude")
+
+    def gather_rows(self, layer_id: int, table: Tensor, lens: Tensor, total: int) -> Tuple[Tensor, Tensor]:
+        from astrai_b200.ops.kv8 import kv8_gather
+
+        return kv8_gather(self.layers[layer_id], table, lens, int(total), dtype=self.dtype)
+
+    def write(self, layer_id: int, page_table: Tensor, start_pos: int, k: Tensor, v: Tensor) -> None:
+        B, S = k.shape[:2]
+        starts = torch.full((B,), start_pos, dtype=torch.int32, device=page_table.device)
+        self.append_rows(layer_id, page_table, starts, starts + S, k, v)
+
+
+def make_storage(n_layers: int, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, device,
+                 dtype: torch.dtype, kv_dtype: Optional[str] = None, kv_block: int = 32) -> Storage:
+    """``kv_dtype`` None: pages of ``dtype``; ``"int8"``: :class:`Int8Storage`."""
+    if kv_dtype is None:
+        return Storage(n_layers, n_pages, page_size, n_kv_heads, head_dim, device, dtype)
+    if kv_dtype == "int8":
+        return Int8Storage(n_layers, n_pages, page_size, n_kv_heads, head_dim, device, dtype, kv_block)
+    raise ValueError(f"kv_dtype must be None or 'int8', got {kv_dtype!r}")
+
+
 def _slots_uniform(table: Tensor, start: int, S: int, page_size: int) -> Tensor:
     pos = torch.arange(start, start + S, device=table.device)
     pages = table.long()[:, pos // page_size]
@@ -380,6 +441,8 @@ class PageCacheView(CacheView):
         self.n_new = n_new
         self._positions = positions
         self._slots: Dict[int, Tensor] = {}
+        self._starts: Dict[int, Tensor] = {}
+        self._int8 = isinstance(storage, Int8Storage)
         self._workspace = workspace
         self._splits = splits
 
@@ -407,6 +470,12 @@ class PageCacheView(CacheView):
             self._slots[S] = torch.where(ok, pages * ps + pos % ps, -1).reshape(-1).to(torch.int32).contiguous()
         return self._slots[S]
 
+    def starts(self, S: int) -> Tensor:
+        """int32 ``[B]`` position of each row's first new token."""
+        if S not in self._starts:
+            self._starts[S] = self.lens - S
+        return self._starts[S]
+
     def _start(self, S: int) -> Optional[int]:
         if self.uniform_start is not None:
             return self.uniform_start
@@ -417,6 +486,9 @@ class PageCacheView(CacheView):
     # ------------------------------------------------------------ reference-shaped API
     def write(self, layer_id: int, k: Tensor, v: Tensor) -> None:
         B, S = k.shape[:2]
+        if self._int8:
+            self._storage.append_rows(layer_id, self.table, self.starts(S), self.lens, k, v)
+            return
         self._storage.write_slots(layer_id, self.slots(S), k.reshape(B * S, -1).contiguous(),
                                   v.reshape(B * S, -1).contiguous())
 
@@ -442,12 +514,30 @@ class PageCacheView(CacheView):
                        1.0 / math.sqrt(D), self._splits, self._workspace)
         return out
 
+    def _attend_int8(self, layer_id: int, q: Tensor, k: Tensor, v: Tensor) -> Tensor:
+        """Attention after the append. A prompt from its start attends to its own k/v. New tokens behind cached
+        ones read the cache in the kernel while a KV head's query rows are few, or when the rows differ in length;
+        past that the cache's values are gathered once for the prefill kernel."""
+        from astrai_b200.ops.attention import attention
+
+        S, Hq = q.shape[1], q.shape[2]
+        start = self._start(S)
+        if start == 0 and S > 1:
+            return attention(q, k, v, causal=True)
+        st = self._storage
+        if start is None or not q.is_cuda or S * Hq // st.n_kv_heads <= INT8_ROWS:
+            return st.attend_rows(layer_id, q, self.table, self.lens)
+        kk, vv = st.gather_rows(layer_id, self.table, self.lens, start + S)
+        return attention(q, kk, vv, causal=True)
+
     def attend(self, layer_id: int, q: Tensor, k: Tensor, v: Tensor) -> Tensor:
         """q ``[B,S,Hq,D]``, k/v ``[B,S,Hkv,D]`` (RoPE applied) -> ``[B,S,Hq,D]``."""
         from astrai_b200.ops.attention import attention, attention_reference
 
         B, S, Hq, D = q.shape
         self.write(layer_id, k, v)
+        if self._int8:
+            return self._attend_int8(layer_id, q, k, v)
         native = self._storage.native_ok and D == self._storage.head_dim and q.dtype == torch.bfloat16
         if native and S == 1:
             o = self._decode_native(layer_id, q.reshape(B, Hq * D).contiguous(), Hq)
@@ -460,15 +550,25 @@ class PageCacheView(CacheView):
             return attention(q, kk, vv, causal=True)
         return self._ragged(layer_id, q, B, S, Hq)  # rows of different lengths
 
-    def attend_qkv(self, layer_id: int, qkv: Tensor, B: int, S: int, Hq: int, Hkv: int, table: Tensor) -> Tensor:
-        """Fused path on a ``[B*S, (Hq+2Hkv)*D]`` bf16 buffer (D = 64 or 128): RoPE in place,
-        K/V written straight from the buffer, attention -> ``[B*S, Hq*D]``."""
+    def attend_qkv(self, layer_id: int, qkv: Tensor, B: int, S: int, Hq: int, Hkv: int, table: Tensor,
+                   rotary=None) -> Tensor:
+        """Fused path on a ``[B*S, (Hq+2Hkv)*D]`` bf16 buffer (D = 64 or 128): RoPE in place (``rotary``, a
+        :class:`astrai_b200.ops.qk_norm.QKRotary`: that instead, QK-norm included), K/V written straight from the
+        buffer, attention -> ``[B*S, Hq*D]``."""
         from astrai_b200.ops.attention import flash_forward
         from astrai_b200.ops.rope import rope_inplace
 
         D = self._storage.head_dim
         pos = self.positions(S)
-        rope_inplace(qkv, 0, Hq + Hkv, D, table, pos, S)
+        if rotary is not None:
+            rotary.apply_(qkv, Hq, Hkv, D, positions=pos)
+        else:
+            rope_inplace(qkv, 0, Hq + Hkv, D, table, pos, S)
+        if self._int8:
+            heads = qkv.view(B, S, Hq + 2 * Hkv, D)
+            q, k, v = heads[:, :, :Hq], heads[:, :, Hq:Hq + Hkv], heads[:, :, Hq + Hkv:]
+            self.write(layer_id, k, v)
+            return self._attend_int8(layer_id, q, k, v).reshape(B * S, Hq * D)
         self._storage.write_slots(layer_id, self.slots(S), qkv[:, Hq * D:(Hq + Hkv) * D],
                                   qkv[:, (Hq + Hkv) * D:])
         if S == 1:
@@ -530,11 +630,12 @@ class PageCache(_TableCache):
     """Paged KV cache with prefix sharing across tasks."""
 
     def __init__(self, n_layers: int, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, device,
-                 dtype: torch.dtype):
+                 dtype: torch.dtype, kv_dtype: Optional[str] = None, kv_block: int = 32):
         self.page_size = page_size
         self._pool = PagePool(Allocator(n_pages), PrefixCache(page_size))
         self._table = TaskTable(page_size)
-        self._storage = Storage(n_layers, n_pages, page_size, n_kv_heads, head_dim, device, dtype)
+        self._storage = make_storage(n_layers, n_pages, page_size, n_kv_heads, head_dim, device, dtype, kv_dtype,
+                                     kv_block)
 
     @property
     def pool(self) -> PagePool:
@@ -592,12 +693,13 @@ class ContiguousCache(_TableCache):
     """One slot of ``max_seq_len`` keys per running task (no sharing)."""
 
     def __init__(self, n_layers: int, max_batch_size: int, max_seq_len: int, n_kv_heads: int, head_dim: int, device,
-                 dtype: torch.dtype):
+                 dtype: torch.dtype, kv_dtype: Optional[str] = None, kv_block: int = 32):
         self.max_seq_len = max_seq_len
         # a slot holds max_seq_len keys, rounded up to the 128-key tile of the tensor-core decode kernel
         # (its TMA boxes never straddle two slots); the capacity checks still use max_seq_len
         self.page_size = (max_seq_len + 127) // 128 * 128
-        self._storage = Storage(n_layers, max_batch_size, self.page_size, n_kv_heads, head_dim, device, dtype)
+        self._storage = make_storage(n_layers, max_batch_size, self.page_size, n_kv_heads, head_dim, device, dtype,
+                                     kv_dtype, kv_block)
         self._table = TaskTable(self.page_size)
         self._free_slots = list(range(max_batch_size))
         self._lock = threading.Lock()

@@ -38,7 +38,8 @@ def model_head_dim(model) -> int:
 class InferenceScheduler:
     def __init__(self, model, tokenizer, max_batch_size: int = 16, max_seq_len: Optional[int] = None,
                  max_prompt_len: int = 2048, device=None, dtype: Optional[torch.dtype] = None,
-                 cache: Optional[KVCache] = None, use_cuda_graph: Optional[bool] = None, seed: Optional[int] = None):
+                 cache: Optional[KVCache] = None, use_cuda_graph: Optional[bool] = None, seed: Optional[int] = None,
+                 kv_cache_dtype: Optional[str] = None, kv_block: int = 32):
         cfg = model.config
         if max_seq_len is None:
             max_seq_len = getattr(cfg, "max_position_embeddings", None)
@@ -52,7 +53,7 @@ class InferenceScheduler:
         self.dtype = dtype or p.dtype
         self._cache = cache if cache is not None else ContiguousCache(
             cfg.num_hidden_layers, max_batch_size, self.max_seq_len, cfg.num_key_value_heads, model_head_dim(model),
-            self.device, self.dtype)
+            self.device, self.dtype, kv_cache_dtype, kv_block)
         self._task_mgr = TaskManager(tokenizer, max_batch_size, self.max_seq_len, max_prompt_len)
         if use_cuda_graph is None:
             use_cuda_graph = self.device.type == "cuda" and self.dtype == torch.bfloat16

@@ -12,7 +12,8 @@ generation are the same drain loop (:meth:`GenerateResult.events`); the blocking
 the pieces. The end of a prompt's stream is the ``STOP`` sentinel. Leaving a drain loop early
 (a consumer that stops iterating, a timeout) removes the call's tasks from the scheduler, so
 their KV pages come back. With ``n_pages`` set, the engine builds a :class:`PageCache` (prefix
-sharing across requests) instead of the per-slot contiguous cache.
+sharing across requests) instead of the per-slot contiguous cache. ``kv_cache_dtype="int8"`` holds
+the cache as 8-bit integers with one magnitude per ``kv_block`` tokens and head.
 """
 
 from __future__ import annotations
@@ -133,22 +134,27 @@ class InferenceEngine:
 
     def __init__(self, model: nn.Module, tokenizer, max_batch_size: int = 1, max_seq_len: Optional[int] = None,
                  max_prompt_len: int = 2048, page_size: int = 128, cache: Optional[KVCache] = None,
-                 n_pages: Optional[int] = None, use_cuda_graph: Optional[bool] = None, seed: Optional[int] = None):
+                 n_pages: Optional[int] = None, use_cuda_graph: Optional[bool] = None, seed: Optional[int] = None,
+                 kv_cache_dtype: Optional[str] = None, kv_block: int = 32):
         self.model = model
         self.tokenizer = tokenizer
+        if cache is not None and kv_cache_dtype is not None:
+            raise ValueError("kv_cache_dtype is for the cache that the engine builds; a given cache has its own")
         if cache is None and n_pages:
-            cache = self._paged_cache(model, n_pages, page_size)
+            cache = self._paged_cache(model, n_pages, page_size, kv_cache_dtype, kv_block)
         self.scheduler = InferenceScheduler(model, tokenizer, max_batch_size=max_batch_size, max_seq_len=max_seq_len,
                                             max_prompt_len=max_prompt_len, cache=cache,
-                                            use_cuda_graph=use_cuda_graph, seed=seed)
+                                            use_cuda_graph=use_cuda_graph, seed=seed,
+                                            kv_cache_dtype=kv_cache_dtype, kv_block=kv_block)
         self.scheduler.start()
 
     @staticmethod
-    def _paged_cache(model: nn.Module, n_pages: int, page_size: int) -> PageCache:
+    def _paged_cache(model: nn.Module, n_pages: int, page_size: int, kv_dtype: Optional[str] = None,
+                     kv_block: int = 32) -> PageCache:
         ref = next(model.parameters())
         c = model.config
         return PageCache(c.num_hidden_layers, n_pages, page_size, c.num_key_value_heads, model_head_dim(model),
-                         ref.device, ref.dtype)
+                         ref.device, ref.dtype, kv_dtype, kv_block)
 
     def __enter__(self) -> "InferenceEngine":
         return self

@@ -5,6 +5,9 @@ GQA has ``q_proj, k_proj, v_proj, o_proj`` (+ ``q_norm, k_norm`` for QK-norm,
 ``gate`` for gated attention); MLA has ``q_proj, kv_a_proj, kv_norm,
 kv_b_proj, o_proj`` (+ ``gate``). Semantics kept: RoPE on q/k, QK-norm
 applied after RoPE, sigmoid output gate, o_proj init std 0.02/sqrt(2L).
+Config additions for GQA (see model_config.py): the half layout, a rotated part
+of each head, QK-norm before the rotation, and ``fused_qk_norm``; with any of
+them norm and rotation run in one pass (:mod:`astrai_b200.ops.qk_norm`).
 
 Execution differs: on the GPU the three projections run as ONE GEMM over the
 concatenated weight (autograd splits the weight gradient back), RoPE is
@@ -22,7 +25,8 @@ import torch.nn as nn
 
 from astrai_b200.factory import Registry
 from astrai_b200.models.components.basic import Linear, RMSNorm
-from astrai_b200.ops.attention import attention, attention_qkv, attention_reference
+from astrai_b200.ops.attention import attention, attention_qk_norm, attention_qkv, attention_reference
+from astrai_b200.ops.qk_norm import QKRotary
 from astrai_b200.ops.rope import apply_rope_reference
 
 
@@ -68,14 +72,27 @@ class AttnFactory(Registry[nn.Module]):
 @AttnFactory.register("gqa")
 class GQA(nn.Module):
     def __init__(self, dim: int, n_heads: int, n_kv_heads: int, use_qk_norm: bool = False, norm_eps: float = 1e-6,
-                 use_gated_attention: bool = False, layer_id: int = 0, n_layers: int = 1):
+                 use_gated_attention: bool = False, layer_id: int = 0, n_layers: int = 1,
+                 rope_layout: Optional[str] = None, rope_fraction: Optional[float] = None,
+                 qk_norm_first: Optional[bool] = None, fused_qk_norm: Optional[bool] = None):
         super().__init__()
         assert dim % n_heads == 0 and n_heads % n_kv_heads == 0
+        if rope_layout not in (None, "interleaved", "half"):
+            raise ValueError(f"rope_layout must be 'interleaved' or 'half', got {rope_layout!r}")
+        if rope_fraction is not None:
+            turned = dim // n_heads * rope_fraction
+            if not 0 < rope_fraction <= 1 or abs(turned - round(turned)) > 1e-6 or round(turned) % 2:
+                raise ValueError(f"rope_fraction must be an even number of a head's {dim // n_heads} channels, "
+                                 f"got {rope_fraction}")
         self.dim, self.n_heads, self.n_kv_heads = dim, n_heads, n_kv_heads
         self.head_dim = dim // n_heads
         self.layer_id = layer_id
         self.use_qk_norm = bool(use_qk_norm)
         self.use_gated_attention = bool(use_gated_attention)
+        self.rope_layout = rope_layout or "interleaved"
+        self.qk_norm_first = bool(qk_norm_first)
+        self.one_pass = (self.rope_layout == "half" or (rope_fraction or 1.0) < 1 or self.qk_norm_first
+                         or bool(fused_qk_norm))
         self.q_proj = Linear(dim, n_heads * self.head_dim)
         self.k_proj = Linear(dim, n_kv_heads * self.head_dim)
         self.v_proj = Linear(dim, n_kv_heads * self.head_dim)
@@ -92,6 +109,11 @@ class GQA(nn.Module):
     def forward(self, x: torch.Tensor, ctx: AttnContext, residual: Optional[torch.Tensor] = None) -> torch.Tensor:
         B, S, _ = x.shape
         Hq, Hkv, D = self.n_heads, self.n_kv_heads, self.head_dim
+        if self.one_pass:
+            o = self._one_pass(x, ctx)
+            if self.use_gated_attention:
+                o = o * torch.sigmoid(self.gate(x))
+            return self.o_proj(o, residual=residual)
         fused = not self.use_qk_norm and ctx.dense_mask is None
         if fused and ctx.cache is not None:  # inference: the cache view runs RoPE + KV write + attention
             fused = getattr(ctx.cache, "supports_qkv", False) and x.is_cuda and x.dtype == torch.bfloat16
@@ -126,6 +148,32 @@ class GQA(nn.Module):
         if self.use_gated_attention:
             o = o * torch.sigmoid(self.gate(x))
         return self.o_proj(o, residual=residual)
+
+    def rotary(self, ctx: AttnContext) -> QKRotary:
+        if not self.use_qk_norm:
+            return QKRotary(ctx.table, layout=self.rope_layout, norm="none")
+        return QKRotary(ctx.table, self.q_norm.weight, self.k_norm.weight, self.q_norm.norm_eps, self.rope_layout,
+                        "before" if self.qk_norm_first else "after")
+
+    def _one_pass(self, x: torch.Tensor, ctx: AttnContext) -> torch.Tensor:
+        """QK-norm and rotation in one pass, then attention -> [B, S, Hq*D]."""
+        B, S, _ = x.shape
+        Hq, Hkv, D = self.n_heads, self.n_kv_heads, self.head_dim
+        rotary = self.rotary(ctx)
+        qkv = self.qkv_proj(x).reshape(B * S, (Hq + 2 * Hkv) * D)
+        if ctx.cache is None and ctx.dense_mask is None:
+            o = attention_qk_norm(qkv, rotary, B, S, Hq, Hkv, ctx.positions, ctx.causal, ctx.seg)
+        elif ctx.cache is not None and getattr(ctx.cache, "supports_qkv", False) and x.is_cuda \
+                and x.dtype == torch.bfloat16:
+            o = ctx.cache.attend_qkv(self.layer_id, qkv, B, S, Hq, Hkv, ctx.table, rotary=rotary)
+        else:
+            qk = rotary.apply(qkv, Hq, Hkv, D, positions=ctx.positions, seq_len=S).view(B, S, Hq + Hkv, D)
+            q, k, v = qk[:, :, :Hq], qk[:, :, Hq:], qkv.view(B, S, Hq + 2 * Hkv, D)[:, :, Hq + Hkv:]
+            if ctx.cache is not None:
+                o = ctx.cache.attend(self.layer_id, q, k, v)
+            else:
+                o = _dense_attention(q, k, v, ctx.dense_mask)
+        return o.reshape(B, S, Hq * D)
 
     def qkv_proj_rope(self, x: torch.Tensor, ctx) -> Optional[torch.Tensor]:
         """q|k|v projection with RoPE already applied to q and k (GEMM epilogue), or None."""

@@ -20,7 +20,7 @@ from astrai_b200.ops.embedding import embedding as _embedding
 from astrai_b200.ops.gemm import linear as _linear
 from astrai_b200.ops.gemm import packed_linear as _packed_linear
 from astrai_b200.ops.norm import rms_norm as _rms_norm
-from astrai_b200.ops.rope import ntk_base, rope_table
+from astrai_b200.ops.rope import ntk_base, rope_table, scaled_rope_table
 
 
 class Linear(nn.Module):
@@ -92,28 +92,39 @@ class Embedding(nn.Module):
 
 
 class RotaryEmbedding(nn.Module):
-    """Interleaved RoPE angle table; stays fp32 when the model is cast."""
+    """RoPE angle table; stays fp32 when the model is cast. ``scaling_method`` None: ``rope_scaling`` is NTK
+    scaling (as in the reference); "linear" / "yarn": :func:`astrai_b200.ops.rope.scaled_rope_table`."""
 
-    def __init__(self, dim: int, max_len: int, base: float = 10000.0, rope_scaling: Optional[Dict] = None):
+    def __init__(self, dim: int, max_len: int, base: float = 10000.0, rope_scaling: Optional[Dict] = None,
+                 scaling_method: Optional[str] = None):
         super().__init__()
         self.dim = dim
         self.max_len = max_len or 4096
         self.base = base if base is not None else 10000.0
         self.rope_scaling = rope_scaling
-        if rope_scaling is not None and rope_scaling.get("type", "ntk") == "ntk":
+        self.scaling_method = scaling_method
+        if scaling_method is None and rope_scaling is not None and rope_scaling.get("type", "ntk") == "ntk":
             self.base = ntk_base(self.base, dim, rope_scaling.get("factor", 1.0))
-        self.register_buffer("freqs_cis", rope_table(dim, self.max_len, self.base), persistent=False)
+        self.register_buffer("freqs_cis", self._build(), persistent=False)
+
+    def _build(self, device=None) -> torch.Tensor:
+        if self.scaling_method is None:
+            return rope_table(self.dim, self.max_len, self.base, device=device)
+        sc = self.rope_scaling or {}
+        return scaled_rope_table(self.dim, self.max_len, self.base, self.scaling_method, sc.get("factor", 1.0),
+                                 sc.get("original_max_position_embeddings"), sc.get("beta_fast", 32.0),
+                                 sc.get("beta_slow", 1.0), sc.get("attention_factor"), device=device)
 
     def _apply(self, fn, recurse=True):
         # keep the angle table in fp32 whatever dtype the model is cast to
         super()._apply(fn, recurse)
         if self.freqs_cis.dtype != torch.float32:
-            self.freqs_cis = rope_table(self.dim, self.max_len, self.base, device=self.freqs_cis.device)
+            self.freqs_cis = self._build(self.freqs_cis.device)
         return self
 
     def reset_buffers(self) -> None:
         """Recompute the angle table in place (after ``to_empty`` left it uninitialised)."""
-        self.freqs_cis = rope_table(self.dim, self.max_len, self.base, device=self.freqs_cis.device)
+        self.freqs_cis = self._build(self.freqs_cis.device)
 
     def table(self) -> torch.Tensor:
         return self.freqs_cis

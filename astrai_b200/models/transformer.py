@@ -39,7 +39,9 @@ def process_attention_mask(input_mask: Optional[torch.Tensor]) -> Optional[torch
 def _rope_dim(config) -> int:
     if getattr(config, "attn_type", "gqa") == "mla":
         return config.qk_rope_head_dim
-    return config.hidden_size // config.num_attention_heads
+    head_dim = config.hidden_size // config.num_attention_heads
+    fraction = getattr(config, "rope_fraction", None)
+    return head_dim if fraction is None else round(head_dim * fraction)
 
 
 def build_trunk(model: nn.Module, config) -> None:
@@ -48,7 +50,8 @@ def build_trunk(model: nn.Module, config) -> None:
     none), ``embed_tokens``, ``layers`` and the final ``norm``."""
     base = config.rope_theta if config.rope_theta is not None else 10000
     model.rotary_embedding = RotaryEmbedding(_rope_dim(config), config.max_position_embeddings, base,
-                                             rope_scaling=config.rope_scaling)
+                                             rope_scaling=config.rope_scaling,
+                                             scaling_method=getattr(config, "rope_scaling_method", None))
     model.embed_tokens = Embedding(config.vocab_size, config.hidden_size, neftune_alpha=config.neftune_alpha)
     model.layers = nn.ModuleList([DecoderBlock(config, i) for i in range(config.num_hidden_layers)])
     model.norm = RMSNorm(config.hidden_size, config.rms_norm_eps)

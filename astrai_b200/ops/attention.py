@@ -160,6 +160,60 @@ def attention_qkv(qkv: torch.Tensor, B: int, S: int, Hq: int, Hkv: int, table: t
     return _sdpa(q, k, v, causal, seg).reshape(B * S, Hq * D)
 
 
+class _AttnQKNormFn(torch.autograd.Function):
+    """QK-norm + rotation (one kernel) and flash attention on a fused QKV buffer. The normalised q and k go
+    to a buffer of their own (the norm's backward needs its input); v is read from the projection output. The
+    attention gradients land in one buffer, on whose q and k columns the norm's backward runs in place."""
+
+    @staticmethod
+    def forward(ctx, qkv, q_weight, k_weight, rotary, positions, seg, B, S, Hq, Hkv, causal):
+        D = HEAD_DIM
+        C = native()
+        wq, wk, rot, off, half, mode, eps = rotary.kernel_args()
+        qk = torch.empty((B * S, (Hq + Hkv) * D), device=qkv.device, dtype=qkv.dtype)
+        C.qk_norm_fwd(qkv, qk, Hq, Hkv, D, rotary.table, positions, S, wq, wk, rot, off, half, mode, eps)
+        o = torch.empty((B * S, Hq * D), device=qkv.device, dtype=torch.bfloat16)
+        lse = torch.empty((B, Hq, S), device=qkv.device, dtype=torch.float32)
+        flash_forward(qk, 0, qk, Hq * D, qkv, (Hq + Hkv) * D, o, lse, B, S, S, Hq, Hkv, D, 1.0 / math.sqrt(D), causal,
+                      seg)
+        ctx.save_for_backward(qkv, qk, o, lse, q_weight, k_weight, rotary.table, positions, seg)
+        ctx.dims = (B, S, Hq, Hkv, causal, rot, off, half, mode, eps)
+        return o
+
+    @staticmethod
+    def backward(ctx, do):
+        qkv, qk, o, lse, q_weight, k_weight, table, positions, seg = ctx.saved_tensors
+        B, S, Hq, Hkv, causal, rot, off, half, mode, eps = ctx.dims
+        D = HEAD_DIM
+        C = native()
+        do = do.contiguous()
+        dqkv = torch.empty_like(qkv)
+        dq_acc = torch.empty((B * S, Hq * D), device=qkv.device, dtype=torch.float32)  # zeroed by the kernel
+        delta = torch.empty(2 * B * Hq * ((S + 63) // 64 * 64), device=qkv.device, dtype=torch.float32)
+        C.flash_bwd(qk, 0, qk, Hq * D, qkv, (Hq + Hkv) * D, o, do, lse, delta, dq_acc, dqkv, 0, dqkv, Hq * D, dqkv,
+                    (Hq + Hkv) * D, B, S, S, Hq, Hkv, 1.0 / math.sqrt(D), causal, seg)
+        dwq, dwk = C.qk_norm_bwd(dqkv, qkv, dqkv, Hq, Hkv, D, table, positions, S, q_weight, k_weight, rot, off, half,
+                                 mode, eps)
+        return dqkv, dwq, dwk, None, None, None, None, None, None, None, None
+
+
+def attention_qk_norm(qkv: torch.Tensor, rotary, B: int, S: int, Hq: int, Hkv: int,
+                      positions: Optional[torch.Tensor] = None, causal: bool = True,
+                      seg: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Attention on a fused QKV buffer ``[B*S, (Hq+2Hkv)*D]`` with ``rotary``
+    (:class:`astrai_b200.ops.qk_norm.QKRotary`) on its query and key heads -> ``[B*S, Hq*D]``. ``positions`` int
+    [B, S] (None -> 0..S-1 per sequence). The buffer is not changed."""
+    D = qkv.shape[-1] // (Hq + 2 * Hkv)
+    pos = positions.reshape(-1).to(torch.int32).contiguous() if positions is not None else None
+    if qkv.is_cuda and qkv.dtype == torch.bfloat16 and D == HEAD_DIM and qkv.is_contiguous():
+        sg = seg.to(torch.int32).contiguous() if seg is not None else None
+        w = rotary.kernel_args()[:2]
+        return _AttnQKNormFn.apply(qkv, *w, rotary, pos, sg, B, S, Hq, Hkv, causal)
+    qk = rotary.apply(qkv, Hq, Hkv, D, positions=pos, seq_len=S).view(B, S, Hq + Hkv, D)
+    v = qkv.view(B, S, Hq + 2 * Hkv, D)[:, :, Hq + Hkv:]
+    return attention(qk[:, :, :Hq], qk[:, :, Hq:], v, causal=causal, seg=seg).reshape(B * S, Hq * D)
+
+
 # ----------------------------------------------------------------------------- generic path
 class _AttnFn(torch.autograd.Function):
     @staticmethod

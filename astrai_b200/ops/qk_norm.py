@@ -19,6 +19,7 @@ rounding at the end); CPU tensors take the plain PyTorch math of :func:`qk_norm_
 
 from __future__ import annotations
 
+from dataclasses import dataclass
 from typing import Optional
 
 import torch
@@ -51,7 +52,7 @@ def qk_norm_rope_reference(x, n_heads, n_kv_heads, head_dim, table, q_weight=Non
     z = x[:, : H * head_dim].to(wide).reshape(-1, H, head_dim)
     if positions is None:
         positions = torch.arange(z.shape[0], device=x.device) % seq_len
-    cs = table.to(wide)[positions.long()]
+    cs = table.to(wide)[positions.reshape(-1).long()]
     if norm != "none":
         w = torch.cat([q_weight.to(wide).expand(n_heads, head_dim), k_weight.to(wide).expand(n_kv_heads, head_dim)])
 
@@ -138,3 +139,35 @@ def qk_norm_rope_(x: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: int,
     x[:, : (n_heads + n_kv_heads) * head_dim] = qk_norm_rope_reference(
         x, n_heads, n_kv_heads, head_dim, table, q_weight, k_weight, positions, seq_len, eps, layout, norm, rot, rot_off)
     return x
+
+
+@dataclass
+class QKRotary:
+    """What a layer does to its query and key heads: the arguments of :func:`qk_norm_rope` that do not
+    depend on the batch."""
+
+    table: torch.Tensor
+    q_weight: Optional[torch.Tensor] = None
+    k_weight: Optional[torch.Tensor] = None
+    eps: float = 1e-6
+    layout: str = "interleaved"
+    norm: str = "after"
+
+    @property
+    def rot_dim(self) -> int:
+        return 2 * self.table.shape[1]
+
+    def _args(self, positions, seq_len) -> dict:
+        return dict(table=self.table, q_weight=self.q_weight, k_weight=self.k_weight, positions=positions,
+                    seq_len=seq_len, eps=self.eps, layout=self.layout, norm=self.norm, rot_dim=self.rot_dim)
+
+    def apply(self, x, n_heads, n_kv_heads, head_dim, positions=None, seq_len=None) -> torch.Tensor:
+        return qk_norm_rope(x, n_heads, n_kv_heads, head_dim, **self._args(positions, seq_len))
+
+    def apply_(self, x, n_heads, n_kv_heads, head_dim, positions=None, seq_len=None) -> torch.Tensor:
+        return qk_norm_rope_(x, n_heads, n_kv_heads, head_dim, **self._args(positions, seq_len))
+
+    def kernel_args(self):
+        """(weights, rot_dim, rot_off, half layout, norm mode, eps) as the row-buffer kernels take them."""
+        w = (None, None) if self.norm == "none" else (self.q_weight, self.k_weight)
+        return (*w, self.rot_dim, 0, self.layout == "half", NORM_MODES[self.norm], float(self.eps))
