@@ -402,6 +402,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv8_attend_kerne
   constexpr int R = 8 * NT;      // query rows of a group
   constexpr int TB = kTile * D;  // bytes of a tile
   constexpr int SLOT = 2 * TB;   // a ring slot: a tile of keys, then one of values
+  constexpr int AHEAD = STAGES - NT;  // tiles that the copies run ahead: the other NT slots are for merges
   extern __shared__ __align__(128) unsigned char smem[];  // [stage][warp][SLOT]
   __shared__ int prefix[kMaxBatch + 1];
   __shared__ int len_s[kMaxBatch];
@@ -529,7 +530,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv8_attend_kerne
         q_raw[n][j] = r < p.S * p.G ? reinterpret_cast<const uint4*>(src)[j] : make_uint4(0u, 0u, 0u, 0u);
     }
 #pragma unroll
-    for (int i = 0; i < STAGES - 1; ++i) issue(i, 1u << i, c.h);
+    for (int i = 0; i < AHEAD; ++i) issue(i, 1u << i, c.h);
   };
 
   long long u = u_begin;
@@ -599,13 +600,13 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv8_attend_kerne
         for (int k = 0; k < 4; ++k) o[n][i][k] = 0.f;
     }
 
-    int stage = 0, refill = STAGES - 1, tok = first0 * kTile;
+    int stage = 0, refill = AHEAD, tok = first0 * kTile;
     for (int it = 0; it < count; ++it, tok += kUnit) {
-      cp_async_wait<STAGES - 2>();
+      cp_async_wait<AHEAD - 1>();
       __syncwarp();  // this tile has landed for all lanes, and all have left the stage that is refilled now
       const bool held = have & 1u;
       have >>= 1;
-      issue(refill, 1u << (STAGES - 2), c.h);
+      issue(refill, 1u << (AHEAD - 1), c.h);
       refill = refill + 1 == STAGES ? 0 : refill + 1;
       const unsigned tile = ring + stage * kWarps * SLOT;
       const float2 mag = lds_float2(mags + stage * 8);
@@ -711,8 +712,8 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv8_attend_kerne
     cp_async_wait<0>();
     __syncwarp();
 
-    // The next piece's first copies fly while this one is merged: they fill all stages of the ring but the
-    // last NT, which hold what the warps merge.
+    // The next piece's first copies fly while this one is merged: they fill the first AHEAD slots, and the
+    // last NT hold what the warps merge.
     const Piece done = c;
     const long long slot = 2LL * blockIdx.x + (done.unit0 > 0 ? 0 : 1);
     u += done.dealt;

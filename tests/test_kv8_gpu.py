@@ -287,6 +287,21 @@ def test_rows_split_over_many_ctas_and_ragged_batches():
         assert torch.equal(kv8_attention(q, cache, table, _i32(*lens)), first)
 
 
+@pytest.mark.parametrize("S,Hq,Hkv,D,lens", [(4, 32, 8, 64, [4000, 3000, 2500, 1200]), (4, 16, 4, 128, [3500, 2100, 3333]),
+                                             (1, 16, 1, 128, [4100, 2000, 3000, 700, 3900]), (11, 6, 2, 64, [3000, 4000])])
+def test_wide_groups_in_several_pieces(S, Hq, Hkv, D, lens):
+    """16 query rows at a time, rows long enough that a CTA's second piece fills the copy ring while its first is
+    merged."""
+    B, page, block = len(lens), 128, 32
+    width = -(-max(lens) // page)
+    cache = _cache(B * width, Hkv, page, D, block, spread=0.1)
+    table = _table(B, width, B * width)
+    q = torch.randn(B, S, Hq, D, device="cuda", generator=_gen(9)).to(torch.bfloat16) * 0.3
+    first = _check_attention(q, cache, table, _i32(*lens))
+    for _ in range(3):
+        assert torch.equal(_check_attention(q, cache, table, _i32(*lens)), first)
+
+
 @pytest.mark.parametrize("D", [64, 128])
 def test_magnitudes_of_any_size(D):
     """Blocks whose values are 2^60 apart, a block of zeros, and queries far from 1."""
