@@ -402,6 +402,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv8_attend_kerne
   constexpr int R = 8 * NT;      // query rows of a group
   constexpr int TB = kTile * D;  // bytes of a tile
   constexpr int SLOT = 2 * TB;   // a ring slot: a tile of keys, then one of values
+  constexpr bool kRest = std::is_same<T, __half>::value;
   constexpr int AHEAD = STAGES - NT;  // tiles that the copies run ahead: the other NT slots are for merges
   extern __shared__ __align__(128) unsigned char smem[];  // [stage][warp][SLOT]
   __shared__ int prefix[kMaxBatch + 1];
@@ -676,7 +677,9 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv8_attend_kerne
           }
         }
       }
-      unsigned pf[NT][2];
+      // weights as fp16; for fp16 outputs their rest as well, or its share of the error would be as large as the
+      // output's own rounding (measured: 3.3e-4 against 2.1e-4 of the result in norm)
+      unsigned pf[NT][2], pr[NT][2];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         float w[4];
@@ -691,6 +694,12 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv8_attend_kerne
         const __half2 w0 = __floats2half2_rn(w[0], w[1]), w1 = __floats2half2_rn(w[2], w[3]);
         pf[n][0] = transpose8x8(*reinterpret_cast<const unsigned*>(&w0));
         pf[n][1] = transpose8x8(*reinterpret_cast<const unsigned*>(&w1));
+        if (kRest) {
+          const float2 f0 = __half22float2(w0), f1 = __half22float2(w1);
+          const __half2 r0 = __floats2half2_rn(w[0] - f0.x, w[1] - f0.y), r1 = __floats2half2_rn(w[2] - f1.x, w[3] - f1.y);
+          pr[n][0] = transpose8x8(*reinterpret_cast<const unsigned*>(&r0));
+          pr[n][1] = transpose8x8(*reinterpret_cast<const unsigned*>(&r1));
+        }
       }
 
       // O^T: a transposed matrix of 8 tokens and 16 channels, read as 16-bit pairs of channels, gives lane
@@ -705,7 +714,10 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv8_attend_kerne
           const unsigned a[4] = {bytes_to_half2(xs[2 * e], 0x4240), bytes_to_half2(xs[2 * e], 0x4341),
                                  bytes_to_half2(xs[2 * e + 1], 0x4240), bytes_to_half2(xs[2 * e + 1], 0x4341)};
 #pragma unroll
-          for (int n = 0; n < NT; ++n) mma16816(o[n][j * 2 + e], a, pf[n]);
+          for (int n = 0; n < NT; ++n) {
+            mma16816(o[n][j * 2 + e], a, pf[n]);
+            if (kRest) mma16816(o[n][j * 2 + e], a, pr[n]);
+          }
         }
       }
     }

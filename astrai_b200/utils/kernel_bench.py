@@ -787,6 +787,58 @@ def bench_norm(rows: int = 8192, D: int = 2048):
                           "frac_of_hbm": round(gbs / hbm, 3), "peak_src": src}))
 
 
+def bench_qk_norm():
+    """QK-norm + rotation in one pass, forward and backward, on the 1.1B step's 8192 rows of 16 + 4 heads of 128, a
+    2048-token prefill at head size 64 and a 4-row decode step; bytes: input and output once (backward: dy, x, dx)."""
+    from astrai_b200.ops.rope import rope_table
+
+    C = native()
+    hbm, _, src = peaks()
+    for rows, hq, hkv, D, half in ((8192, 16, 4, 128, False), (2048, 24, 4, 64, True), (4, 16, 4, 128, False)):
+        H = hq + hkv
+        x, dy = (torch.randn(rows, H * D, device="cuda").to(torch.bfloat16) for _ in range(2))
+        w = torch.ones(D, device="cuda", dtype=torch.bfloat16)
+        tab, y, dx = rope_table(D, max(rows, 16), 1e6, device="cuda"), torch.empty_like(x), torch.empty_like(x)
+        args = (hq, hkv, D, tab, None, rows, w, w, D, 0, half, 1, 1e-6)
+        for name, fn, n in (("fwd", lambda: C.qk_norm_fwd(x, y, *args), 2), ("bwd", lambda: C.qk_norm_bwd(dy, x, dx, *args), 3)):
+            ms = time_flushed(fn)
+            by = n * x.numel() * 2
+            print(json.dumps({"kernel": f"qk_norm_{name}", "rows": rows, "heads": [hq, hkv, D], "ms": round(ms, 4),
+                              "gbs": round(by / ms / 1e6, 1), "frac_of_copy": round(by / ms / 1e6 / hbm, 3), "peak_src": src}))
+
+
+def bench_kv8():
+    """8-bit paged KV cache: attention of one new token per row, an append of 512 tokens per row, read-back."""
+    from astrai_b200.ops.kv8 import KV8, kv8_append, kv8_attention, kv8_gather
+
+    hbm, _, src = peaks()
+    for B, L, Hq, Hkv, D in ((4, 131072, 16, 4, 128), (32, 4096, 16, 4, 128), (64, 1024, 16, 4, 128), (1, 8192, 16, 4, 128)):
+        P = -(-L // 128)
+        c = KV8.allocate(B * P, Hkv, 128, D, 32, "cuda")
+        for q in (c.k, c.v):
+            q.random_(-127, 128)
+        for a in (c.k_absmax, c.v_absmax):
+            a.fill_(1.0)
+        table = torch.randperm(B * P, device="cuda").view(B, P).int()
+        lens = torch.full((B,), L, device="cuda", dtype=torch.int32)
+        q = torch.randn(B, 1, Hq, D, device="cuda").to(torch.bfloat16)
+        ms = time_flushed(lambda: kv8_attention(q, c, table, lens))
+        by = B * L * Hkv * 2 * (D + 4 / 32)
+        print(json.dumps({"kernel": "kv8_attention", "B": B, "tokens": L, "heads": [Hq, Hkv, D], "ms": round(ms, 4),
+                          "gbs": round(by / ms / 1e6, 1), "frac_of_copy": round(by / ms / 1e6 / hbm, 3), "peak_src": src}))
+        if L == 4096:
+            k, v = (torch.randn(B, 512, Hkv, D, device="cuda").to(torch.bfloat16) for _ in range(2))
+            starts = lens - 512
+            ms = time_flushed(lambda: kv8_append(c, k, v, table, starts, lens))
+            by = B * 512 * Hkv * D * 2 * 3
+            print(json.dumps({"kernel": "kv8_append", "B": B, "new": 512, "ms": round(ms, 4), "gbs": round(by / ms / 1e6, 1),
+                              "frac_of_copy": round(by / ms / 1e6 / hbm, 3)}))
+            ms = time_flushed(lambda: kv8_gather(c, table, lens, L))
+            by = B * L * Hkv * D * 2 * 3
+            print(json.dumps({"kernel": "kv8_gather", "B": B, "tokens": L, "ms": round(ms, 4), "gbs": round(by / ms / 1e6, 1),
+                              "frac_of_copy": round(by / ms / 1e6 / hbm, 3)}))
+
+
 def main(argv=None):
     args = argv or sys.argv[1:] or ["all"]
     which = args[0]
@@ -828,6 +880,10 @@ def main(argv=None):
         bench_gemm(args[1] if which == "gemm" and len(args) > 1 else None)
     if which in ("norm", "all"):
         bench_norm()
+    if which in ("qk_norm", "all"):
+        bench_qk_norm()
+    if which in ("kv8", "all"):
+        bench_kv8()
     if which in ("attn", "all"):
         try:
             from astrai_b200.ops.attention import bench_attention
