@@ -790,6 +790,7 @@ def bench_norm(rows: int = 8192, D: int = 2048):
 def bench_qk_norm():
     """QK-norm + rotation in one pass, forward and backward, on the 1.1B step's 8192 rows of 16 + 4 heads of 128, a
     2048-token prefill at head size 64 and a 4-row decode step; bytes: input and output once (backward: dy, x, dx)."""
+    from astrai_b200.ops._ext import native
     from astrai_b200.ops.rope import rope_table
 
     C = native()
