@@ -354,7 +354,9 @@ __global__ void __launch_bounds__(384, 2) qk_norm_fwd_kernel(const QkNormParams 
 // chunks c, c + grid, ... In the backward the sums of g u stay in registers and go to the CTA's own row of dw_part,
 // so the result does not depend on any order in time.
 constexpr int kStages = 4;
-constexpr int kMaxWarps = 10;  // consumers
+// consumer warps of a CTA at most: 10 leave the backward of 16-bit types enough registers not to spill (33.7 -> 30 us at
+// 8192 rows of 20 heads of 128), 4-byte rows are so wide that often only one is in a chunk and all warps share it
+__host__ __device__ constexpr int max_warps(int elem) { return elem == 4 ? 12 : 10; }
 constexpr int kRowsSmem = 100 * 1024;  // of which an SM holds two
 // Input bytes from which the forward takes qk_norm_rows_kernel. Measured on B200, 20 heads of 128 in bfloat16: 148
 // rows (0.8 MB) 2.08 us straight from global memory and 2.13 through shared memory, 300 rows 3.19 and 2.67, 8192 rows
@@ -363,7 +365,7 @@ constexpr long long kFewBytes = 1400000;
 
 // EVEN: every lane group of every step has a whole head (D = 8 LPH, head counts multiples of 32 / LPH).
 template <typename T, int LPH, bool HALF, int NORM, bool EVEN, bool BWD>
-__global__ void __launch_bounds__(32 * (kMaxWarps + 1), 2) qk_norm_rows_kernel(const QkNormParams p, int chunk) {
+__global__ void __launch_bounds__(32 * (max_warps(sizeof(T)) + 1), 2) qk_norm_rows_kernel(const QkNormParams p, int chunk) {
   constexpr int HPW = 32 / LPH;
   extern __shared__ __align__(128) unsigned char smem[];
   __shared__ uint64_t full[kStages], empty[kStages];
@@ -593,13 +595,19 @@ astrai::Launch many_rows(astrai::QkNormParams& p, int elem, bool bwd, int sms) {
   Launch l{};
   l.lph = lanes_per_head(p.D);
   const int hpw = 32 / l.lph, sq = (p.hq + hpw - 1) / hpw, sk = (p.hkv + hpw - 1) / hpw;
-  int turns = std::min(2, std::max(sq, sk));  // steps of a warp per row, which then share its (cos, sin) pairs
-  while ((sq + turns - 1) / turns + (sk + turns - 1) / turns > kMaxWarps) ++turns;
-  p.q_parts = (sq + turns - 1) / turns;
-  p.warps_per_row = p.q_parts + (sk + turns - 1) / turns;
   const int per_row = (p.hq + p.hkv) * p.D * elem * (bwd ? 2 : 1) + p.rot * 4;
   l.chunk = std::min(std::min(4, (p.rows + 2 * sms - 1) / (2 * sms)), kRowsSmem / (kStages * per_row));
-  p.rows_at_once = std::max(1, std::min(kMaxWarps / p.warps_per_row, l.chunk));
+  // `turns` steps of a warp per row and as many rows at once as there are warps for: the most rows per step, and of
+  // equals two turns, which share a row's (cos, sin) pairs (24 + 4 heads of 64, 2048 rows: 2 turns 4.8 us, 3 turns 5.3)
+  double best = 0;
+  for (int turns = 1; turns <= std::max(sq, sk); ++turns) {
+    const int q = (sq + turns - 1) / turns, w = q + (sk + turns - 1) / turns;
+    if (w > max_warps(elem)) continue;
+    const int rows = std::min(max_warps(elem) / w, l.chunk);
+    if ((double)rows / turns < best || ((double)rows / turns == best && turns > 2)) continue;
+    best = (double)rows / turns;
+    p.q_parts = q, p.warps_per_row = w, p.rows_at_once = rows;
+  }
   const int warps = p.warps_per_row * p.rows_at_once;
   l.smem = std::max(per_row * l.chunk * kStages, bwd ? warps * p.D * 4 : 0);
   l.block = dim3(32 * (warps + 1));
