@@ -90,6 +90,9 @@ __device__ __forceinline__ unsigned low_bytes(unsigned a, unsigned b, unsigned c
 // between the maximum and the rounding. A row's append starts at starts[b] and ends at lens[b]; what
 // the cache held from starts[b] on is void. A block with an infinite or NaN input gets the magnitude
 // NaN: reading it gives NaN, as the input would have.
+// Bound by its chain of loads (lengths, tokens, magnitude) at decode sizes, 2 us for 32 single tokens; 32 x 512
+// tokens of 4 heads of 128 take 19 us, 0.4 of the copy rate. A block to a warp needs one pass over the input and no
+// atomics; holding the values in registers instead unrolled into code that ran at the rate of instruction fetches.
 template <typename T, int D, int BLOCK>
 __global__ void __launch_bounds__(128) kv8_append_kernel(const AppendParams p) {
   constexpr int WARPS = BLOCK > 32 ? BLOCK / 32 : 1;  // warps per item
@@ -204,7 +207,8 @@ __device__ __forceinline__ void word_to_floats(unsigned u, float* v) {
 
 constexpr int kGatherTokens = 64;  // of a CTA
 
-// Grid (tokens, heads, rows); a lane 16 values of k and the same 16 of v.
+// Grid (tokens, heads, rows); a lane 16 values of k and the same 16 of v. Bound by HBM, two thirds of it writes: 32 x
+// 4096 tokens of 4 heads of 128 take 81 us, 0.76 of the copy rate.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) kv8_gather_kernel(const GatherParams p) {
   constexpr int C = D / 16, PER = 256 / C, N = kGatherTokens / PER;
@@ -370,6 +374,10 @@ __device__ __forceinline__ int swizzle(int row, int chunk) {
 // l = sum 2^(s - m). The weights of the integers v are 2^s * absmax_v; they have a reference M of their
 // own near the maximum of s + log2 absmax_v, so as fp16 they keep their precision whatever the
 // magnitudes of the blocks. out = sum w v / l * 2^(M - m) / 127.
+//
+// Bound by HBM on long rows (4 x 131072 tokens of 4 heads of 128: 95 us, 0.86 of the copy rate), by its start (1.7 us
+// to the first copy), merge (2 us) and join (3 us) on short ones (32 x 4096: 31.6 us, 0.65). Two CTAs of 8 warps per
+// SM: with 4 or 16 warps per CTA the long case takes 114 or 96 us.
 template <int C>
 __device__ __forceinline__ void load_floats(const float* src, float* v) {
   if constexpr (C == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(src);

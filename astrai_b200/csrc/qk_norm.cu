@@ -353,6 +353,8 @@ __global__ void __launch_bounds__(384, 2) qk_norm_fwd_kernel(const QkNormParams 
 // depend on registers or occupancy; the other warps take their heads of each row out of it. CTA c has the
 // chunks c, c + grid, ... In the backward the sums of g u stay in registers and go to the CTA's own row of dw_part,
 // so the result does not depend on any order in time.
+// Bound by instructions (105 per two heads forward, 190 backward) and, forward, nearly by HBM: 8192 rows of 20 heads
+// of 128 in bfloat16 take 15.5 us forward (84 MB, 0.83 of the copy rate) and 29 us backward (126 MB, 0.66).
 constexpr int kStages = 4;
 // consumer warps of a CTA at most: 10 leave the backward of 16-bit types enough registers not to spill (33.7 -> 30 us at
 // 8192 rows of 20 heads of 128), 4-byte rows are so wide that often only one is in a chunk and all warps share it
@@ -413,6 +415,8 @@ __global__ void __launch_bounds__(32 * (max_warps(sizeof(T)) + 1), 2) qk_norm_ro
           bulk_load(at_row + per_row - cs_bytes, p.table + (long long)pos * (p.rot / 2), cs_bytes, &full[st]);
       }
     }
+    // no copy outlives the CTA, should its consumers have given up
+    for (int i = max(0, n - kStages); i < n; ++i) mbar_wait(&full[i % kStages], (i / kStages) & 1, p.err, kErrWaitFull);
   } else {
     const int z = warp / p.warps_per_row;  // of every p.rows_at_once rows, this warp has the z-th
     const Share sh(p, warp - z * p.warps_per_row, p.warps_per_row);

@@ -141,3 +141,17 @@ def test_config_options():
             _model(**bad)
     with pytest.raises(ValueError):
         _model(rope_scaling_method="other", rope_scaling=dict(factor=2.0))
+
+
+def test_command_line_flags(monkeypatch, tmp_path):
+    from astrai_b200.cli import server
+    from astrai_b200.inference.api import server as api
+
+    seen = {}
+    monkeypatch.setattr(api, "run_server", lambda path, **kw: seen.update(kw))
+    server.main(["--param_path", str(tmp_path)])
+    assert "kv_cache_dtype" not in seen
+    server.main(["--param_path", str(tmp_path), "--n_pages", "8", "--kv_cache_dtype", "int8", "--kv_block", "64"])
+    assert seen["kv_cache_dtype"] == "int8" and seen["kv_block"] == 64 and seen["n_pages"] == 8
+    with pytest.raises(SystemExit):
+        server.main(["--param_path", str(tmp_path), "--kv_cache_dtype", "int4"])

@@ -473,3 +473,20 @@ def test_refusals():
               cache._replace(k=cache.k.transpose(1, 2), v=cache.v.transpose(1, 2))):
         with pytest.raises((RuntimeError, ZeroDivisionError)):
             kv8_gather(c, table, lens, 8)
+
+
+def test_more_rows_than_one_launch_takes():
+    """1024 rows go in one launch: 1100 rows, split and whole ones, with and without a caller's workspace."""
+    from astrai_b200.ops.kv8 import kv8_attention, kv8_attention_workspace
+
+    for width in (1, 12):
+        B, page, Hq, Hkv, D = 1100, 64, 4, 1, 64
+        cache = _cache(40, Hkv, page, D, 32)
+        table = (torch.arange(B * width, device="cuda") % 40).view(B, width).int()  # pages shared between rows
+        lens = (torch.arange(B, device="cuda") * 7 % (width * page + 1)).int()
+        q = torch.randn(B, 1, Hq, D, device="cuda", generator=_gen(4)).to(torch.bfloat16)
+        got = kv8_attention(q, cache, table, lens)
+        ws = torch.empty(max(1, kv8_attention_workspace(B, 1, Hq, cache, width)), device="cuda")
+        assert torch.equal(kv8_attention(q, cache, table, lens, workspace=ws), got)
+        pick = torch.tensor([0, 1, 5, 1023, 1024, 1025, 1099], device="cuda")
+        _check_attention(q[pick], cache, table[pick], lens[pick], got=got[pick])
