@@ -1,5 +1,6 @@
 // Python bindings of the 8-bit paged KV cache kernels (kv8.cu): every tensor check is here.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
@@ -24,6 +25,12 @@ void kv8_attend(const void* q, const long long* qs, const void* kc, const void* 
 namespace {
 
 using OptTensor = c10::optional<at::Tensor>;
+
+// Uninitialised memory straight from the caching allocator: a call of a few microseconds feels the dispatcher's share
+// of at::empty.
+at::Tensor new_like(const at::Tensor& t, at::IntArrayRef sizes, at::ScalarType dtype) {
+  return at::Tensor(at::detail::empty_cuda(sizes, dtype, t.device(), c10::nullopt));
+}
 
 // Numbers enter messages as text made here: a build whose compiler links its own static libstdc++ must not
 // stream them through the locale of the one that torch loaded.
@@ -149,7 +156,8 @@ std::pair<at::Tensor, at::Tensor> kv8_gather(const at::Tensor& kc, const at::Ten
   }
   const int* ln = check_i32(lens, kc, B, "lens");
   const c10::cuda::CUDAGuard g(kc.device());
-  auto ko = at::empty({B, total, c.Hkv, c.D}, kc.options().dtype(dtype)), vo = at::empty_like(ko);
+  const int64_t sizes[4] = {B, total, c.Hkv, c.D};
+  auto ko = new_like(kc, sizes, dtype), vo = new_like(kc, sizes, dtype);
   astrai_host::kv8_gather(kc.data_ptr(), vc.data_ptr(), ka.data_ptr<float>(), va.data_ptr<float>(),
                           table.data_ptr<int>(), st, ln, ko.data_ptr(), vo.data_ptr(), (int)B, (int)total, c.Hkv, c.D,
                           c.page_size, c.n_pages, mp, c.block, dtype == at::kHalf, stream());
@@ -193,7 +201,7 @@ at::Tensor kv8_attend(const at::Tensor& q_in, const at::Tensor& kc, const at::Te
               "kv8_attention: too many rows or pages");
   const int64_t need = kv8_attend_workspace(B, S, Hq, c.Hkv, c.D, c.page_size, mp, q.device().index());
   const c10::cuda::CUDAGuard g(q.device());
-  auto out = at::empty({B, S, Hq, c.D}, q.options());
+  auto out = new_like(q, {B, S, Hq, c.D}, q.scalar_type());
   at::Tensor ws;
   float* wp = nullptr;
   if (need > 0) {
@@ -203,7 +211,7 @@ at::Tensor kv8_attend(const at::Tensor& q_in, const at::Tensor& kc, const at::Te
                       reinterpret_cast<uintptr_t>(ws.data_ptr()) % 16 == 0,
                   "kv8_attention: workspace must be contiguous fp32 of at least ", text(need), " elements");
     } else {
-      ws = at::empty({need}, q.options().dtype(at::kFloat));
+      ws = new_like(q, {need}, at::kFloat);
     }
     wp = ws.data_ptr<float>();
   }

@@ -1,5 +1,6 @@
 // Python bindings of the per-head norm + rotation kernels (qk_norm.cu): every tensor check is here.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
@@ -23,6 +24,12 @@ namespace {
 using OptTensor = c10::optional<at::Tensor>;
 
 bool given(const OptTensor& t) { return t.has_value() && t->defined(); }
+
+// Uninitialised memory straight from the caching allocator: a call of a few microseconds feels the dispatcher's share
+// of at::empty.
+at::Tensor new_like(const at::Tensor& t, at::IntArrayRef sizes, at::ScalarType dtype) {
+  return at::Tensor(at::detail::empty_cuda(sizes, dtype, t.device(), c10::nullopt));
+}
 
 int dtype_code(const at::Tensor& t) {
   switch (t.scalar_type()) {
@@ -122,9 +129,9 @@ std::pair<at::Tensor, at::Tensor> backward_into(const at::Tensor& dy, const at::
   check_rows(dx, x, (o.hq + o.hkv) * o.D, "dx");
   const c10::cuda::CUDAGuard g(x.device());
   if (s.rows == 0) return {at::zeros_like(*wq), at::zeros_like(*wk)};
-  auto dwq = at::empty_like(*wq), dwk = at::empty_like(*wk);
-  auto scratch = at::empty({(int64_t)astrai_host::qk_norm_bwd_scratch(s.rows, s.hq + s.hkv, s.D, s.rot, (int)x.element_size(), s.device)},
-                           x.options().dtype(at::kFloat));
+  auto dwq = new_like(x, wq->sizes(), x.scalar_type()), dwk = new_like(x, wk->sizes(), x.scalar_type());
+  const int64_t need = astrai_host::qk_norm_bwd_scratch(s.rows, s.hq + s.hkv, s.D, s.rot, (int)x.element_size(), s.device);
+  auto scratch = new_like(x, {need}, at::kFloat);
   astrai_host::qk_norm_bwd(dy.data_ptr(), dy.stride(0), x.data_ptr(), x.stride(0), dx.data_ptr(), dx.stride(0), s.rows,
                            s.hq, s.hkv, s.D, table.data_ptr(), s.max_pos, s.pos, (int)o.seq_len, wq->data_ptr(),
                            wk->data_ptr(), s.rot, s.rot_off, o.half_layout, (int)o.norm, (float)o.eps, dwq.data_ptr(),
@@ -148,7 +155,7 @@ struct QkNormRope : public torch::autograd::Function<QkNormRope> {
                             bool half_layout, double eps) {
     const Options o{hq, hkv, D, seq_len, rot, rot_off, norm, half_layout, eps};
     const at::Tensor rows = rows_of(x);
-    auto y = at::empty({x.size(0), (hq + hkv) * D}, x.options());
+    auto y = new_like(x, {x.size(0), (hq + hkv) * D}, x.scalar_type());
     forward_into(rows, y, table, pos, wq, wk, o, false);
     const auto or_none = [](const OptTensor& t) { return given(t) ? *t : at::Tensor(); };
     ctx->save_for_backward({rows, or_none(wq), or_none(wk), table, or_none(pos)});
@@ -167,7 +174,7 @@ struct QkNormRope : public torch::autograd::Function<QkNormRope> {
     if (!grads[0].defined()) return out;
     const at::Tensor dy = rows_of(grads[0]);
     const int64_t used = (o.hq + o.hkv) * o.D, width = n[8];
-    auto dx = at::empty({x.size(0), width}, x.options());
+    auto dx = new_like(x, {x.size(0), width}, x.scalar_type());
     if (width > used) dx.narrow(1, used, width - used).zero_();  // columns behind the keys are not an input
     auto dw = backward_into(dy, x, dx, saved[3], saved[4], saved[1], saved[2], o);
     out[0] = dx, out[1] = dw.first, out[2] = dw.second;
@@ -203,7 +210,7 @@ at::Tensor qk_norm_rope(const at::Tensor& x, int64_t hq, int64_t hkv, int64_t D,
   }
   if (grad)
     return QkNormRope::apply(x, wq, wk, table, pos, hq, hkv, D, seq_len, rot, rot_off, norm, half_layout, eps);
-  auto y = at::empty({x.size(0), (hq + hkv) * D}, x.options());
+  auto y = new_like(x, {x.size(0), (hq + hkv) * D}, x.scalar_type());
   forward_into(rows_of(x), y, table, pos, wq, wk, o, false);
   return y;
 }
