@@ -55,7 +55,7 @@ Cache check_cache(const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& 
                     t->is_contiguous() && t->sizes() == ka.sizes(),
                 "kv8: the magnitudes must be contiguous CUDA fp32 [n_pages, n_kv_heads, page_size / block]");
   TORCH_CHECK(kc.size(3) == 64 || kc.size(3) == 128, "kv8: head_dim must be 64 or 128, got ", text(kc.size(3)));
-  TORCH_CHECK(ka.size(0) == kc.size(0) && ka.size(1) == kc.size(1) && ka.size(2) >= 1 &&
+  TORCH_CHECK(kc.size(1) >= 1 && ka.size(0) == kc.size(0) && ka.size(1) == kc.size(1) && ka.size(2) >= 1 &&
                   kc.size(2) % ka.size(2) == 0,
               "kv8: cache ", text(kc.sizes()), " and magnitudes ", text(ka.sizes()), " do not belong together");
   const int64_t block = kc.size(2) / ka.size(2);

@@ -87,8 +87,8 @@ __device__ __forceinline__ unsigned low_bytes(unsigned a, unsigned b, unsigned c
 
 // One block of tokens of one head of k or v: its live tokens and the new ones end under the larger
 // of their magnitudes. WARPS warps share it, at most 32 tokens each, whose values wait in shared memory
-// between the maximum and the rounding. A row's append starts at starts[b] and ends at lens[b]; what
-// the cache held from starts[b] on is void. A block with an infinite or NaN input gets the magnitude
+// between the maximum and the rounding. A row's append starts at starts[b] and ends at lens[b]; tokens
+// before position 0 are dropped, and what the cache held from starts[b] on is void. A block with an infinite or NaN input gets the magnitude
 // NaN: reading it gives NaN, as the input would have.
 // Bound by its chain of loads (lengths, tokens, magnitude) at decode sizes, 2 us for 32 single tokens; 32 x 512
 // tokens of 4 heads of 128 take 19 us, 0.4 of the copy rate. A block to a warp needs one pass over the input and no
@@ -107,10 +107,11 @@ __global__ void __launch_bounds__(128) kv8_append_kernel(const AppendParams p) {
   const int h = (int)(bwh - bw * p.Hkv), b = (int)(bw / (unsigned)p.windows), w = (int)(bw - (unsigned)b * p.windows);
   begin_early();
   bool on = b < p.B;
-  int start = 0, end = 0, base = 0, page = -1, off = 0;
+  int first_pos = 0, start = 0, end = 0, base = 0, page = -1, off = 0;  // first_pos: of the row's first token in src
   if (on) {
-    start = min(max(p.starts[b], 0), p.max_pages * p.page_size);
-    end = min(p.lens[b], start + p.S);
+    first_pos = min(max(p.starts[b], -(1 << 30)), p.max_pages * p.page_size);
+    start = max(first_pos, 0);
+    end = min(p.lens[b], first_pos + p.S);
     base = (start / BLOCK + w) * BLOCK;
     on = base < end && start < end;
   }
@@ -118,7 +119,7 @@ __global__ void __launch_bounds__(128) kv8_append_kernel(const AppendParams p) {
   const int mine = warp % WARPS * TOK;
   const int first = max(start - base, mine), n = on ? max(0, min(end - base, mine + TOK) - first) : 0;
   const T* src = static_cast<const T*>(p.src[kv]) + (long long)b * p.sb[kv] + (long long)h * p.sh[kv] +
-                 (long long)(base + first - start) * p.st[kv];
+                 (long long)(base + first - first_pos) * p.st[kv];
   const unsigned held = (unsigned)__cvta_generic_to_shared(hold[warp]) + lane * 16;
 #pragma unroll 4
   for (int i = lane; i < n * LPT; i += 32)
@@ -149,6 +150,8 @@ __global__ void __launch_bounds__(128) kv8_append_kernel(const AppendParams p) {
     const int w0 = warp / WARPS * WARPS;
 #pragma unroll
     for (int i = 0; i < WARPS; ++i) most = max(most, most_s[w0 + i]);
+  } else {
+    __syncwarp();  // every lane has read the old magnitude before one replaces it
   }
   if (!on) return;
   const float fresh = bits_to_float<T>((unsigned short)most);
@@ -363,21 +366,6 @@ __device__ __forceinline__ int swizzle(int row, int chunk) {
   return D == 128 ? row * 128 + ((chunk ^ (row & 7)) << 4) : row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4);
 }
 
-// Work: every (row b, kv head h, group g of R query rows) is a segment of ceil(keys / 128) units, and kPad
-// more at its start; the units of all segments, in order, are dealt out evenly over the CTAs, whatever the
-// rows' lengths. A CTA's warps take the 16-token tiles of its piece of a segment in turn, each with its own
-// running softmax, and are merged once per piece. A piece that is a whole segment writes the output; others
-// leave partials (two per CTA at most: one that it begins inside, one that it does not end) for
-// kv8_combine_kernel.
-//
-// Softmax per query row: a reference m near the maximum of the scores s (within kSlack) and
-// l = sum 2^(s - m). The weights of the integers v are 2^s * absmax_v; they have a reference M of their
-// own near the maximum of s + log2 absmax_v, so as fp16 they keep their precision whatever the
-// magnitudes of the blocks. out = sum w v / l * 2^(M - m) / 127.
-//
-// Bound by HBM on long rows (4 x 131072 tokens of 4 heads of 128: 95 us, 0.86 of the copy rate), by its start (1.7 us
-// to the first copy), merge (2 us) and join (3 us) on short ones (32 x 4096: 31.6 us, 0.65). Two CTAs of 8 warps per
-// SM: with 4 or 16 warps per CTA the long case takes 114 or 96 us.
 template <int C>
 __device__ __forceinline__ void load_floats(const float* src, float* v) {
   if constexpr (C == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(src);
@@ -403,6 +391,21 @@ struct Piece {       // of a segment, on one CTA
   bool whole;
 };
 
+// Work: every (row b, kv head h, group g of R query rows) is a segment of ceil(keys / 128) units, and kPad
+// more at its start; the units of all segments, in order, are dealt out evenly over the CTAs, whatever the
+// rows' lengths. A CTA's warps take the 16-token tiles of its piece of a segment in turn, each with its own
+// running softmax, and are merged once per piece. A piece that is a whole segment writes the output; others
+// leave partials (two per CTA at most: one that it begins inside, one that it does not end) for
+// kv8_combine_kernel.
+//
+// Softmax per query row: a reference m near the maximum of the scores s (within kSlack) and
+// l = sum 2^(s - m). The weights of the integers v are 2^s * absmax_v; they have a reference M of their
+// own near the maximum of s + log2 absmax_v, so as fp16 they keep their precision whatever the
+// magnitudes of the blocks. out = sum w v / l * 2^(M - m) / 127.
+//
+// Bound by HBM on long rows (4 x 131072 tokens of 4 heads of 128: 95 us, 0.86 of the copy rate), by its start (1.7 us
+// to the first copy), merge (2 us) and join (3 us) on short ones (32 x 4096: 31.6 us, 0.65). Two CTAs of 8 warps per
+// SM: with 4 or 16 warps per CTA the long case takes 114 or 96 us.
 template <typename T, int D, int NT, int STAGES>
 __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv8_attend_kernel(const AttendParams p) {
   constexpr int KS = D / 16;     // k-steps of S^T = K Q^T

@@ -61,9 +61,8 @@ class KV8(NamedTuple):
 def _append_reference(cache: KV8, k, v, page_table, starts, lens) -> None:
     block, page = cache.block, cache.page_size
     S = k.shape[1]
-    for b, (start, end) in enumerate(zip(starts.tolist(), lens.tolist())):
-        start = max(start, 0)
-        end = min(end, start + S)
+    for b, (first, end) in enumerate(zip(starts.tolist(), lens.tolist())):
+        start, end = max(first, 0), min(end, first + S)
         for base in range(start // block * block, end if end > start else 0, block):
             lp = base // page
             p = int(page_table[b, lp]) if lp < page_table.shape[1] else -1
@@ -71,7 +70,7 @@ def _append_reference(cache: KV8, k, v, page_table, starts, lens) -> None:
                 continue
             off, kept, stop = base % page, max(0, start - base), min(end - base, block)
             for q, absmax, new in ((cache.k, cache.k_absmax, k), (cache.v, cache.v_absmax, v)):
-                x = new[b, base + kept - start: base + stop - start].float().transpose(0, 1)  # [Hkv, n, D]
+                x = new[b, base + kept - first: base + stop - first].float().transpose(0, 1)  # [Hkv, n, D]
                 fresh = x.abs().amax((1, 2))
                 was = absmax[p, :, off // block].clone() if kept else torch.zeros_like(fresh)
                 now = torch.where(torch.isfinite(fresh), torch.maximum(was, fresh), math.nan)
@@ -91,10 +90,11 @@ def kv8_append(cache: KV8, k: torch.Tensor, v: torch.Tensor, page_table: torch.T
 
     k, v ``[B, S, n_kv_heads, head_dim]`` (any strides with 16-byte aligned rows, e.g. slices of the QKV
     projection). Row ``b`` keeps its tokens before ``starts[b]`` and gets ``lens[b] - starts[b]`` (at most
-    S) new ones, ``k[b, 0]`` first; what the cache held from ``starts[b]`` on is void. A block that held
-    earlier tokens ends under the larger of the two magnitudes, and its integers are rounded again when
-    that grew. Tokens whose page is missing are dropped. A block with an infinity or NaN among its new
-    values reads as NaN.
+    S) new ones, ``k[b, i]`` at position ``starts[b] + i``; what the cache held from ``starts[b]`` on is
+    void. A block that held earlier tokens ends under the larger of the two magnitudes, and its integers
+    are rounded again when that grew. Tokens before position 0 and tokens whose page is missing are
+    dropped. A block with an infinity or NaN among its new values reads as NaN. No page may be in the
+    table twice.
     """
     if cache.k.is_cuda:
         native().kv8_append(k, v, *cache, page_table, starts, lens)

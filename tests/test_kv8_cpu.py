@@ -52,6 +52,18 @@ def test_append_behind_live_tokens_and_growth():
     assert (got[0, 64] == 0.25).all() and (got[1, 0] == 0.25).all() and (got[2, 32] == 0.25).all()
 
 
+def test_tokens_before_position_zero_are_dropped():
+    torch.manual_seed(1)
+    k, v = torch.randn(3, 40, 2, 64), torch.randn(3, 40, 2, 64)
+    table = torch.tensor([[0, 1], [2, 3], [4, 5]], dtype=torch.int32)
+    starts, lens = torch.tensor([-3, -40, -39]), torch.tensor([37, 0, 5])  # row 2 ends with the tokens that it has
+    c, want = (KV8.allocate(6, 2, 32, 64, 16) for _ in range(2))
+    kv8_append(c, k, v, table, starts, lens)
+    for b, n in ((0, 37), (2, 1)):
+        kv8_append(want, k[b: b + 1, 40 - n:], v[b: b + 1, 40 - n:], table[b: b + 1], torch.tensor([0]), torch.tensor([n]))
+    assert all(torch.equal(x, y) for x, y in zip(c, want)) and c.k[0].any()
+
+
 def test_non_finite_blocks_and_missing_pages():
     c = KV8.allocate(4, 1, 32, 64, 16)
     table = torch.tensor([[0, 1], [-1, 9]], dtype=torch.int32)

@@ -134,6 +134,24 @@ def test_append_token_by_token_keeps_what_it_should():
     assert torch.equal(cache.k[spare], _cache(B + 1, H, page, D, block).k[spare])
 
 
+@pytest.mark.parametrize("block", [16, 32, 64, 128])
+def test_append_drops_tokens_before_position_zero(block):
+    """k[b, i] has position starts[b] + i, also where that is negative for the first of them."""
+    from astrai_b200.ops.kv8 import kv8_append
+
+    H, D, page, S = 2, 64, 128, 150
+    starts, lens = [-3, -150, -149, -1000, -70], [147, 0, 5, 20, 40]
+    live = [(3, 147), (150, 0), (149, 1), (150, 0), (70, 40)]  # first token kept and their number
+    c, want = _cache(12, H, page, D, block), _cache(12, H, page, D, block)
+    table = _table(5, 2, 12)
+    k, v = _new(5, S, H, D, torch.bfloat16)
+    kv8_append(c, k, v, table, _i32(*starts), _i32(*lens))
+    for b, (i, n) in enumerate(live):
+        if n:
+            kv8_append(want, k[b: b + 1, i: i + n], v[b: b + 1, i: i + n], table[b: b + 1], _i32(0), _i32(n))
+    assert all(torch.equal(x, y) for x, y in zip(c, want))
+
+
 def test_append_edges_missing_pages_zeros_and_non_finite():
     from astrai_b200.ops.kv8 import kv8_append, kv8_gather
 
@@ -473,6 +491,21 @@ def test_refusals():
               cache._replace(k=cache.k.transpose(1, 2), v=cache.v.transpose(1, 2))):
         with pytest.raises((RuntimeError, ZeroDivisionError)):
             kv8_gather(c, table, lens, 8)
+
+
+def test_caches_without_heads_or_pages():
+    from astrai_b200.ops.kv8 import KV8, kv8_append, kv8_attention, kv8_gather
+
+    table, lens, starts = _i32(0, 1).view(1, 2), _i32(20), _i32(0)
+    q, k = torch.randn(1, 4, 4, 128, device="cuda").bfloat16(), torch.randn(1, 20, 2, 128, device="cuda").bfloat16()
+    none = KV8.allocate(4, 0, 64, 128, 32, "cuda")
+    for call in (lambda: kv8_attention(q, none, table, lens), lambda: kv8_gather(none, table, lens, 8),
+                 lambda: kv8_append(none, k[:, :, :0], k[:, :, :0], table, starts, lens)):
+        with pytest.raises(RuntimeError):
+            call()
+    empty = KV8.allocate(0, 2, 64, 128, 32, "cuda")  # no page to read
+    kv8_append(empty, k, k, table, starts, lens)
+    assert (kv8_attention(q, empty, table, lens) == 0).all() and (kv8_gather(empty, table, lens, 8)[0] == 0).all()
 
 
 def test_more_rows_than_one_launch_takes():
