@@ -51,6 +51,10 @@ void check_rows(const at::Tensor& t, const at::Tensor& like, int64_t width, cons
                   reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0,
               "qk_norm_rope: ", name, " needs a contiguous inner dimension and 16-byte aligned rows");
 }
+void check_output(const at::Tensor& t, const at::Tensor& like, int64_t width, const char* name) {
+  check_rows(t, like, width, name);
+  TORCH_CHECK(t.size(0) <= 1 || t.stride(0) >= width, "qk_norm_rope: rows of ", name, " overlap");
+}
 
 struct Shape {
   int rows, hq, hkv, D, max_pos, rot, rot_off, dtype, device;
@@ -67,7 +71,7 @@ Shape check(const at::Tensor& x, int64_t hq, int64_t hkv, int64_t D, const at::T
   TORCH_CHECK(rot >= 8 && rot % 8 == 0 && rot_off >= 0 && rot_off % 8 == 0 && rot + rot_off <= D,
               "qk_norm_rope: rot_dim and rot_off must be multiples of 8 inside head_dim");
   TORCH_CHECK(norm >= 0 && norm <= 2, "qk_norm_rope: norm mode");
-  TORCH_CHECK(x.size(0) < (1LL << 31), "qk_norm_rope: too many rows");
+  TORCH_CHECK(x.size(0) <= (1LL << 30), "qk_norm_rope: too many rows");
   check_rows(x, x, (hq + hkv) * D, "x");
   TORCH_CHECK(table.is_cuda() && table.device() == x.device() && table.scalar_type() == at::kFloat &&
                   table.is_contiguous() && table.dim() == 3 && table.size(1) == rot / 2 && table.size(2) == 2 &&
@@ -107,7 +111,7 @@ cudaStream_t stream() { return at::cuda::getCurrentCUDAStream().stream(); }
 void forward_into(const at::Tensor& x, const at::Tensor& y, const at::Tensor& table, const OptTensor& pos,
                   const OptTensor& wq, const OptTensor& wk, const Options& o, bool inverse) {
   const Shape s = check(x, o.hq, o.hkv, o.D, table, pos, o.seq_len, wq, wk, o.rot, o.rot_off, o.norm);
-  check_rows(y, x, (o.hq + o.hkv) * o.D, "y");
+  check_output(y, x, (o.hq + o.hkv) * o.D, "y");
   const c10::cuda::CUDAGuard g(x.device());
   astrai_host::qk_norm_fwd(x.data_ptr(), x.stride(0), y.data_ptr(), y.stride(0), s.rows, s.hq, s.hkv, s.D,
                            table.data_ptr(), s.max_pos, s.pos, (int)o.seq_len, o.norm ? wq->data_ptr() : nullptr,
@@ -126,7 +130,7 @@ std::pair<at::Tensor, at::Tensor> backward_into(const at::Tensor& dy, const at::
   }
   const Shape s = check(x, o.hq, o.hkv, o.D, table, pos, o.seq_len, wq, wk, o.rot, o.rot_off, o.norm);
   check_rows(dy, x, (o.hq + o.hkv) * o.D, "dy");
-  check_rows(dx, x, (o.hq + o.hkv) * o.D, "dx");
+  check_output(dx, x, (o.hq + o.hkv) * o.D, "dx");
   const c10::cuda::CUDAGuard g(x.device());
   if (s.rows == 0) return {at::zeros_like(*wq), at::zeros_like(*wk)};
   auto dwq = new_like(x, wq->sizes(), x.scalar_type()), dwk = new_like(x, wk->sizes(), x.scalar_type());
@@ -206,6 +210,7 @@ at::Tensor qk_norm_rope(const at::Tensor& x, int64_t hq, int64_t hkv, int64_t D,
   if (in_place) {
     TORCH_CHECK(!(at::GradMode::is_enabled() && x.requires_grad()), "qk_norm_rope_ has no gradient: use qk_norm_rope");
     forward_into(x, x, table, pos, wq, wk, o, false);
+    if (!x.is_inference()) x.unsafeGetTensorImpl()->bump_version();  // a backward that saved x has to notice
     return x;
   }
   if (grad)

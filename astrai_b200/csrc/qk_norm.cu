@@ -405,6 +405,7 @@ __global__ void __launch_bounds__(32 * (max_warps(sizeof(T)) + 1), 2) qk_norm_ro
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // before a later copy into the same place
       }
       const int tables = __popc(__ballot_sync(0xffffffff, lane < live && in_table));
+      __syncwarp();  // rows written here are visible to the lane that arrives
       if (lane == 0) mbar_expect_tx(&full[st], live * (per_row - cs_bytes) + tables * cs_bytes);
       __syncwarp();
       if (lane < live) {

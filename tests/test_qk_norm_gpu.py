@@ -279,6 +279,39 @@ def test_refusals():
         call(x=buf.clone().requires_grad_(), fn=qk_norm_rope_)
 
 
+def test_in_place_is_noticed_and_refuses_rows_that_overlap():
+    from astrai_b200.ops.qk_norm import qk_norm_rope, qk_norm_rope_
+
+    hq, hkv, d, rows = 2, 1, 64, 4
+    buf, wq, wk, _ = _inputs(rows, hq, hkv, d, torch.bfloat16)
+    t = _table(d, rows)
+    w = torch.ones_like(buf).requires_grad_()
+    out = buf * w  # saves buf
+    qk_norm_rope_(buf, hq, hkv, d, t, wq, wk, seq_len=rows)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        out.sum().backward()
+    same = buf[:1].expand(rows, -1)  # read, but not written
+    y = qk_norm_rope(same, hq, hkv, d, t, wq, wk, seq_len=rows)
+    assert torch.equal(y, qk_norm_rope(same.contiguous(), hq, hkv, d, t, wq, wk, seq_len=rows))
+    with pytest.raises(RuntimeError):
+        qk_norm_rope_(same, hq, hkv, d, t, wq, wk, seq_len=rows)
+    with torch.inference_mode():
+        x = buf.clone()
+        assert torch.equal(qk_norm_rope_(x, hq, hkv, d, t, wq, wk, seq_len=rows),
+                           qk_norm_rope(buf, hq, hkv, d, t, wq, wk, seq_len=rows))
+
+
+def test_a_weight_of_any_shape_gets_a_gradient_of_it():
+    from astrai_b200.ops.qk_norm import qk_norm_rope
+
+    buf, wq, wk, dy = _inputs(6, 2, 1, 64, torch.bfloat16)
+    t = _table(64, 6)
+    flat = [w.clone().requires_grad_() for w in (wq, wk)]
+    row = [w.view(1, 64).clone().requires_grad_() for w in (wq, wk)]
+    a, b = (torch.autograd.grad(qk_norm_rope(buf, 2, 1, 64, t, *w, seq_len=6), w, dy) for w in (flat, row))
+    assert all(y.shape == (1, 64) and torch.equal(x, y[0]) for x, y in zip(a, b))
+
+
 def test_weight_gradients_are_the_same_every_time():
     from astrai_b200.ops.qk_norm import qk_norm_rope
 
