@@ -564,6 +564,7 @@ class PageCacheView(CacheView):
 
         D = self._storage.head_dim
         pos = self.positions(S)
+        qkv = qkv.detach()  # changed in place, and attention over a cache has no gradient
         if rotary is not None:
             rotary.apply_(qkv, Hq, Hkv, D, positions=pos)
         else:

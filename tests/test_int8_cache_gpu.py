@@ -156,6 +156,44 @@ def test_prefill_behind_shared_pages_and_rows_of_several_tokens():
     assert _rel(both[0], full[0, 256:260]) < 0.03 and _rel(both[1], full[0, 96:100]) < 0.03
 
 
+@pytest.mark.parametrize("kv_dtype", [None, "int8"])
+def test_one_pass_over_a_cache_outside_no_grad(kv_dtype):
+    """A forward over a cache has no gradient and needs no no_grad() around it."""
+    from astrai_b200.inference import PageCache
+
+    _, model = _models(**OPTIONS["fused"])
+    model = model.eval()
+    ids, outs = list(range(7, 60)), []
+    for grad in (True, False):
+        cache = PageCache(2, 8, 64, 2, 128, "cuda", torch.bfloat16, kv_dtype)
+        assert cache.task_alloc("a", ids)
+        with torch.set_grad_enabled(grad):
+            outs.append(model(torch.tensor([ids], device="cuda"), position_ids=torch.arange(53, device="cuda")[None],
+                              paged_cache=cache.bind(["a"], [53], 53, "cuda", uniform_start=0))["logits"].detach())
+    assert torch.equal(*outs)
+
+
+def test_rows_shorter_than_the_step():
+    """Four tokens a row of which one row has two: its first two have no position and are not kept."""
+    from astrai_b200.inference import PageCache
+    from astrai_b200.ops._ext import native
+
+    _, model = _models()
+    model = model.eval()
+    ids = torch.randint(0, 512, (2, 4), generator=torch.Generator().manual_seed(3))
+    cache = PageCache(2, 8, 64, 2, 128, "cuda", torch.bfloat16, "int8")
+    with torch.inference_mode():
+        for name, n in (("a", 4), ("b", 2), ("c", 2)):
+            assert cache.task_alloc(name, [1] * n)
+        pos = torch.tensor([[0, 1, 2, 3], [0, 0, 0, 1]], device="cuda")
+        both = model(ids.cuda(), paged_cache=cache.bind(["a", "b"], [4, 2], 4, "cuda"), position_ids=pos)["logits"]
+        alone = model(ids[1:, 2:].cuda(), paged_cache=cache.bind(["c"], [2], 2, "cuda"),
+                      position_ids=torch.arange(2, device="cuda")[None])["logits"]
+    torch.cuda.synchronize()
+    native().read_error()  # the rotation records positions before 0
+    assert _rel(both[1, 2:], alone[0]) < 0.03
+
+
 @pytest.mark.parametrize("paged", [False, True])
 def test_graph_decode_equals_eager_decode(paged):
     from astrai_b200.inference import ContiguousCache, PageCache
