@@ -856,7 +856,7 @@ __global__ void __launch_bounds__(32 * WARPS) kv8_combine_kernel(const AttendPar
 #pragma unroll
       for (int i = 0; i < C; ++i) v[k][i] = 0.f;
       if (ck > c1) continue;
-      const long long slot = 2LL * ck + (total * ck / ctas > u0 ? 0 : 1);  // 0: the CTA begins inside the keys
+      const long long slot = 2LL * ck + (ck == c0);  // the first of the CTAs does not begin inside the keys
       const float* s = p.part_s + (slot * R + row) * 3;
       st[k][0] = s[0], st[k][1] = s[1], st[k][2] = s[2];
       load_floats<C>(p.part_o + (slot * R + row) * D + lane * C, v[k]);
