@@ -403,7 +403,7 @@ struct Piece {       // of a segment, on one CTA
 // own near the maximum of s + log2 absmax_v, so as fp16 they keep their precision whatever the
 // magnitudes of the blocks. out = sum w v / l * 2^(M - m) / 127.
 //
-// Bound by HBM on long rows (4 x 131072 tokens of 4 heads of 128: 95 us, 0.86 of the copy rate), by its start (1.7 us
+// Bound by HBM on long rows (4 x 131072 tokens of 4 heads of 128: 94 us, 0.87 of the copy rate), by its start (1.7 us
 // to the first copy), merge (2 us) and join (3 us) on short ones (32 x 4096: 31.6 us, 0.65). Two CTAs of 8 warps per
 // SM: with 4 or 16 warps per CTA the long case takes 114 or 96 us.
 template <typename T, int D, int NT, int STAGES>
