@@ -3,6 +3,9 @@
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/utils.h>
+#include <torch/csrc/autograd/saved_variable.h>
 #include <torch/extension.h>
 
 #include <cuda_runtime.h>
@@ -151,40 +154,54 @@ at::Tensor rows_of(const at::Tensor& t) {
   return ok ? t : t.contiguous();
 }
 
-// The autograd node, in C++: a training step of short kernels would otherwise wait for Python.
-struct QkNormRope : public torch::autograd::Function<QkNormRope> {
-  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const OptTensor& wq,
-                            const OptTensor& wk, const at::Tensor& table, const OptTensor& pos, int64_t hq,
-                            int64_t hkv, int64_t D, int64_t seq_len, int64_t rot, int64_t rot_off, int64_t norm,
-                            bool half_layout, double eps) {
-    const Options o{hq, hkv, D, seq_len, rot, rot_off, norm, half_layout, eps};
-    const at::Tensor rows = rows_of(x);
-    auto y = new_like(x, {x.size(0), (hq + hkv) * D}, x.scalar_type());
-    forward_into(rows, y, table, pos, wq, wk, o, false);
-    const auto or_none = [](const OptTensor& t) { return given(t) ? *t : at::Tensor(); };
-    ctx->save_for_backward({rows, or_none(wq), or_none(wk), table, or_none(pos)});
-    ctx->saved_data["ints"] = std::vector<int64_t>{hq, hkv, D, seq_len, rot, rot_off, norm, half_layout, x.size(1)};
-    ctx->saved_data["eps"] = eps;
-    return y;
+// The autograd node, in C++ and a Node of its own: a training step of short kernels would otherwise wait for Python,
+// and for the list and dictionary in which torch::autograd::Function keeps what it was given.
+struct QkNormRopeBackward : public torch::autograd::Node {
+  torch::autograd::SavedVariable x, wq, wk, table, pos;
+  Options o;
+  int64_t width = 0;  // columns of x
+  std::string name() const override { return "QkNormRopeBackward"; }
+  void release_variables() override {
+    std::lock_guard<std::mutex> lock(mutex_);
+    for (auto* v : {&x, &wq, &wk, &table, &pos}) v->reset_data();
   }
-  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
-                                                 torch::autograd::variable_list grads) {
+  torch::autograd::variable_list apply(torch::autograd::variable_list&& grads) override {
     TORCH_CHECK(!at::GradMode::is_enabled(), "qk_norm_rope has no second derivative (create_graph)");
-    const auto saved = ctx->get_saved_variables();
-    const auto n = ctx->saved_data["ints"].toIntVector();
-    const Options o{n[0], n[1], n[2], n[3], n[4], n[5], n[6], n[7] != 0, ctx->saved_data["eps"].toDouble()};
-    const at::Tensor& x = saved[0];
-    torch::autograd::variable_list out(14);
+    std::lock_guard<std::mutex> lock(mutex_);
+    torch::autograd::variable_list out(3);
     if (!grads[0].defined()) return out;
-    const at::Tensor dy = rows_of(grads[0]);
-    const int64_t used = (o.hq + o.hkv) * o.D, width = n[8];
-    auto dx = new_like(x, {x.size(0), width}, x.scalar_type());
+    const at::Tensor x_ = x.unpack(), table_ = table.unpack(), dy = rows_of(grads[0]);
+    const auto given_or_none = [](const at::Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
+    const int64_t used = (o.hq + o.hkv) * o.D;
+    auto dx = new_like(x_, {x_.size(0), width}, x_.scalar_type());
     if (width > used) dx.narrow(1, used, width - used).zero_();  // columns behind the keys are not an input
-    auto dw = backward_into(dy, x, dx, saved[3], saved[4], saved[1], saved[2], o);
-    out[0] = dx, out[1] = dw.first, out[2] = dw.second;
+    auto dw = backward_into(dy, x_, dx, table_, given_or_none(pos.unpack()), given_or_none(wq.unpack()),
+                            given_or_none(wk.unpack()), o);
+    out[0] = std::move(dx), out[1] = std::move(dw.first), out[2] = std::move(dw.second);
     return out;
   }
 };
+
+at::Tensor with_gradient(const at::Tensor& x, const OptTensor& wq, const OptTensor& wk, const at::Tensor& table,
+                         const OptTensor& pos, const Options& o) {
+  const auto or_none = [](const OptTensor& t) { return given(t) ? *t : at::Tensor(); };
+  for (const auto& t : {x, or_none(wq), or_none(wk)})
+    TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), "qk_norm_rope has no forward-mode derivative");
+  at::Tensor rows, y;
+  {
+    const at::NoGradGuard off;
+    rows = rows_of(x);
+    y = new_like(x, {x.size(0), (o.hq + o.hkv) * o.D}, x.scalar_type());
+    forward_into(rows, y, table, pos, wq, wk, o, false);
+  }
+  std::shared_ptr<QkNormRopeBackward> node(new QkNormRopeBackward(), torch::autograd::deleteNode);
+  node->set_next_edges(torch::autograd::collect_next_edges(x, or_none(wq), or_none(wk)));
+  node->x = {rows, false}, node->wq = {or_none(wq), false}, node->wk = {or_none(wk), false};
+  node->table = {table, false}, node->pos = {or_none(pos), false};
+  node->o = o, node->width = x.size(1);
+  torch::autograd::set_history(y, node);
+  return y;
+}
 
 // The user's call: argument errors are ValueErrors here, wrong tensors RuntimeErrors in check().
 at::Tensor qk_norm_rope(const at::Tensor& x, int64_t hq, int64_t hkv, int64_t D, const at::Tensor& table,
@@ -214,7 +231,7 @@ at::Tensor qk_norm_rope(const at::Tensor& x, int64_t hq, int64_t hkv, int64_t D,
     return x;
   }
   if (grad)
-    return QkNormRope::apply(x, wq, wk, table, pos, hq, hkv, D, seq_len, rot, rot_off, norm, half_layout, eps);
+    return with_gradient(x, wq, wk, table, pos, o);
   auto y = new_like(x, {x.size(0), (hq + hkv) * D}, x.scalar_type());
   forward_into(rows_of(x), y, table, pos, wq, wk, o, false);
   return y;

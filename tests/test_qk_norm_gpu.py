@@ -322,3 +322,47 @@ def test_weight_gradients_are_the_same_every_time():
             for _ in range(3)]
     for r in runs[1:]:
         assert all(torch.equal(a, b) for a, b in zip(r, runs[0]))
+
+
+def test_autograd_node():
+    """What autograd asks of a node: saved-tensor hooks, one backward unless kept, no second derivative, no tangents,
+    gradients for some of the inputs, a checkpointed region."""
+    from torch.utils.checkpoint import checkpoint
+
+    from astrai_b200.ops.qk_norm import qk_norm_rope
+
+    buf, wq, wk, dy = _inputs(6, 2, 1, 64, torch.bfloat16)
+    t, pos = _table(64, 6), torch.arange(6, device="cuda").int()
+    x, wq, wk = buf.clone().requires_grad_(), wq.clone().requires_grad_(), wk.clone().requires_grad_()
+
+    def run(a=x, b=wq, c=wk, **kw):
+        return qk_norm_rope(a, 2, 1, 64, t, b, c, **(kw or dict(positions=pos)))
+
+    y = run()
+    assert y.grad_fn.name() == "QkNormRopeBackward" and not run(x.detach(), wq.detach(), wk.detach()).requires_grad
+    want = torch.autograd.grad(y, (x, wq, wk), dy, retain_graph=True)
+    again = torch.autograd.grad(y, (x, wq, wk), dy)
+    with pytest.raises(RuntimeError, match="second time"):
+        torch.autograd.grad(y, x, dy)
+    kept = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda v: kept.append(v.shape) or v.cpu(), lambda v: v.cuda()):
+        hooked = torch.autograd.grad(run(), (x, wq, wk), dy)
+    remade = torch.autograd.grad(checkpoint(run, x, wq, wk, use_reentrant=False), (x, wq, wk), dy)
+    assert len(kept) == 5
+    for got in (again, hooked, remade):
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert torch.equal(torch.autograd.grad(run(x, wq.detach(), wk.detach()), x, dy)[0], want[0])
+    assert torch.equal(torch.autograd.grad(run(x.detach()), wk, dy)[0], want[2])
+    with pytest.raises(RuntimeError, match="second derivative"):
+        torch.autograd.grad(run(), x, dy, create_graph=True)
+    with torch.autograd.forward_ad.dual_level():
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            run(torch.autograd.forward_ad.make_dual(x, dy))
+    y = run()
+    with torch.no_grad():
+        x.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward(dy)
+    turned = qk_norm_rope(x, 2, 1, 64, t, norm="none", seq_len=6)
+    turned.backward(dy)
+    assert x.grad is not None and wq.grad is None
