@@ -292,6 +292,9 @@ constexpr float kNone = -1.7e38f;
 // A running maximum follows the scores only when they pass it by this much (powers of two): weights then
 // reach 2^8, far inside fp16, and most tiles need no reduction over lanes and no rescaling.
 constexpr float kSlack = 8.f;
+// The weights' reference stays this far below their largest, which is then 2^kLift to 2^(kLift + kSlack) as fp16, half
+// its range: a weight of 2^-32 of the largest still reaches its last place.
+constexpr float kLift = 7.f;
 
 __device__ __forceinline__ float2 lds_float2(unsigned a) {
   float2 v;
@@ -406,14 +409,18 @@ struct Piece {       // of a segment, on one CTA
 // Bound by HBM on long rows (4 x 131072 tokens of 4 heads of 128: 94 us, 0.87 of the copy rate), by its start (1.7 us
 // to the first copy), merge (2 us) and join (3 us) on short ones (32 x 4096: 31.6 us, 0.65). Two CTAs of 8 warps per
 // SM: with 4 or 16 warps per CTA the long case takes 114 or 96 us.
-template <typename T, int D, int NT, int STAGES>
+//
+// A weight is held as two fp16 numbers, itself and what that leaves, 22 bits in all: rounded once, the weights put
+// errors of up to 3.3e-4 in norm into outputs whose own rounding is 2.1e-4 (fp16) and moved 7e-4 of bfloat16 ones to
+// the next value; now both are below 2e-4. TWIN: at most four query rows, each in two columns, one of which takes
+// what the other's weights leave (32 x 4096: 32.3 us); otherwise a second product does (34.5 us for the same).
+template <typename T, int D, int NT, int STAGES, bool TWIN>
 __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv8_attend_kernel(const AttendParams p) {
   constexpr int KS = D / 16;     // k-steps of S^T = K Q^T
   constexpr int MT = D / 16;     // channel tiles of O^T = V^T P^T
   constexpr int R = 8 * NT;      // query rows of a group
   constexpr int TB = kTile * D;  // bytes of a tile
   constexpr int SLOT = 2 * TB;   // a ring slot: a tile of keys, then one of values
-  constexpr bool kRest = std::is_same<T, __half>::value;
   constexpr int AHEAD = STAGES - NT;  // tiles that the copies run ahead: the other NT slots are for merges
   extern __shared__ __align__(128) unsigned char smem[];  // [stage][warp][SLOT]
   __shared__ int prefix[kMaxBatch + 1];
@@ -534,7 +541,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv8_attend_kerne
     look_up();
 #pragma unroll
     for (int n = 0; n < NT; ++n) {
-      const int r = c.grp * R + n * 8 + g, i = r / p.G;
+      const int r = TWIN ? g & 3 : c.grp * R + n * 8 + g, i = r / p.G;
       const T* src = static_cast<const T*>(p.q) + (long long)c.b * p.qb + (long long)i * p.qs +
                      (long long)(c.h * p.G + (r - i * p.G)) * p.qh + t * (D / 4);
 #pragma unroll
@@ -592,7 +599,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv8_attend_kerne
         qscale[n][k] = __shfl_sync(0xffffffff, up, (2 * t + k) * 4);
         qbias[n][k] = -128.f * qscale[n][k] * __shfl_sync(0xffffffff, sum, (2 * t + k) * 4);
         qscale[n][k] *= 0x1p24f;
-        const int rc = c.grp * R + n * 8 + 2 * t + k, pos = c.first + rc / p.G;
+        const int rc = TWIN ? (2 * t + k) & 3 : c.grp * R + n * 8 + 2 * t + k, pos = c.first + rc / p.G;
         // columns behind the last query row are computed like the others and never written
         vis[n][k] = rc >= p.S * p.G ? c.keys : pos >= 0 && pos < c.len ? min(pos + 1, c.keys) : 0;
         seen_by_all = min(seen_by_all, vis[n][k]);
@@ -663,7 +670,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv8_attend_kerne
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           const float top = fmaxf(sc[n][k], sc[n][2 + k]);
-          rises = rises || top > m[n][k] + kSlack || top + lv > M[n][k] + kSlack;
+          rises = rises || top > m[n][k] + kSlack || top + lv > M[n][k] + (kSlack + kLift);
         }
       }
       if (__any_sync(0xffffffff, rises)) {
@@ -675,7 +682,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv8_attend_kerne
             float top = fmaxf(sc[n][k], sc[n][2 + k]);
 #pragma unroll
             for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffff, top, d));
-            const float m1 = fmaxf(m[n][k], top), M1 = fmaxf(M[n][k], top + lv);
+            const float m1 = fmaxf(m[n][k], top), M1 = fmaxf(M[n][k], top + lv - kLift);
             l[n][k] *= ex2(m[n][k] - m1);
             fall[k] = ex2(M[n][k] - M1);
             m[n][k] = m1;
@@ -688,8 +695,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv8_attend_kerne
           }
         }
       }
-      // weights as fp16; for fp16 outputs their rest as well, or its share of the error would be as large as the
-      // output's own rounding (measured: 3.3e-4 against 2.1e-4 of the result in norm)
+      // weights as fp16, and what that leaves of them
       unsigned pf[NT][2], pr[NT][2];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
@@ -702,15 +708,17 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv8_attend_kerne
           w[k] = sc[n][k] == -INFINITY ? 0.f : ex2(sc[n][k] + to);
           w[2 + k] = sc[n][2 + k] == -INFINITY ? 0.f : ex2(sc[n][2 + k] + to);
         }
-        const __half2 w0 = __floats2half2_rn(w[0], w[1]), w1 = __floats2half2_rn(w[2], w[3]);
-        pf[n][0] = transpose8x8(*reinterpret_cast<const unsigned*>(&w0));
-        pf[n][1] = transpose8x8(*reinterpret_cast<const unsigned*>(&w1));
-        if (kRest) {
-          const float2 f0 = __half22float2(w0), f1 = __half22float2(w1);
-          const __half2 r0 = __floats2half2_rn(w[0] - f0.x, w[1] - f0.y), r1 = __floats2half2_rn(w[2] - f1.x, w[3] - f1.y);
+        __half2 w0 = __floats2half2_rn(w[0], w[1]), w1 = __floats2half2_rn(w[2], w[3]);
+        const float2 f0 = __half22float2(w0), f1 = __half22float2(w1);
+        const __half2 r0 = __floats2half2_rn(w[0] - f0.x, w[1] - f0.y), r1 = __floats2half2_rn(w[2] - f1.x, w[3] - f1.y);
+        if (TWIN) {
+          w0 = t < 2 ? w0 : r0, w1 = t < 2 ? w1 : r1;
+        } else {
           pr[n][0] = transpose8x8(*reinterpret_cast<const unsigned*>(&r0));
           pr[n][1] = transpose8x8(*reinterpret_cast<const unsigned*>(&r1));
         }
+        pf[n][0] = transpose8x8(*reinterpret_cast<const unsigned*>(&w0));
+        pf[n][1] = transpose8x8(*reinterpret_cast<const unsigned*>(&w1));
       }
 
       // O^T: a transposed matrix of 8 tokens and 16 channels, read as 16-bit pairs of channels, gives lane
@@ -727,7 +735,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv8_attend_kerne
 #pragma unroll
           for (int n = 0; n < NT; ++n) {
             mma16816(o[n][j * 2 + e], a, pf[n]);
-            if (kRest) mma16816(o[n][j * 2 + e], a, pr[n]);
+            if (!TWIN) mma16816(o[n][j * 2 + e], a, pr[n]);
           }
         }
       }
@@ -762,7 +770,7 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv8_attend_kerne
 #pragma unroll
         for (int d = 4; d < 32; d <<= 1) s += __shfl_xor_sync(0xffffffff, s, d);
         const int row = n * 8 + 2 * t + k;
-        if (row < rows) {
+        if ((TWIN ? row & 3 : row) < rows) {
           if (g == 0) stat_s[warp][row][0] = m[n][k], stat_s[warp][row][1] = M[n][k], stat_s[warp][row][2] = s;
 #pragma unroll
           for (int i = 0; i < MT; ++i)
@@ -790,6 +798,12 @@ __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv8_attend_kerne
       for (int i = 0; i < kWarps; ++i) {
         float v[C];
         load_floats<C>(merge_at(i, row, lane * C), v);
+        if (TWIN) {
+          float rest[C];
+          load_floats<C>(merge_at(i, row + 4, lane * C), rest);
+#pragma unroll
+          for (int j = 0; j < C; ++j) v[j] += rest[j];
+        }
         const float fi = __shfl_sync(0xffffffff, f, i);
 #pragma unroll
         for (int j = 0; j < C; ++j) a[j] += v[j] * fi;
@@ -897,10 +911,10 @@ __global__ void __launch_bounds__(32 * WARPS) kv8_combine_kernel(const AttendPar
 
 constexpr int stages_for(int NT) { return NT == 1 ? 3 : 6; }
 
-template <typename T, int D, int NT>
+template <typename T, int D, int NT, bool TWIN>
 void launch_attend(const AttendParams& p, bool combine, cudaStream_t s) {
   constexpr int smem = kWarps * stages_for(NT) * 2 * kTile * D;
-  auto kernel = kv8_attend_kernel<T, D, NT, stages_for(NT)>;
+  auto kernel = kv8_attend_kernel<T, D, NT, stages_for(NT), TWIN>;
   static bool set[64] = {};  // the attribute belongs to the device that is current
   int dev = 0;
   cudaGetDevice(&dev);
@@ -1048,8 +1062,9 @@ void kv8_attend(const void* q, const long long* qs, const void* kc, const void* 
     p.part_o = workspace;
     p.part_s = workspace ? workspace + 2LL * p.ctas * a.R * D : nullptr;
 #define ASTRAI_ATTEND(T, D_) \
-  if (a.R == 16) launch_attend<T, D_, 2>(p, a.split, s); \
-  else launch_attend<T, D_, 1>(p, a.split, s);
+  if (a.R == 16) launch_attend<T, D_, 2, false>(p, a.split, s); \
+  else if (S * p.G > 4) launch_attend<T, D_, 1, false>(p, a.split, s); \
+  else launch_attend<T, D_, 1, true>(p, a.split, s);
     if (dtype == 0 && D == 128) { ASTRAI_ATTEND(__nv_bfloat16, 128) }
     else if (dtype == 0) { ASTRAI_ATTEND(__nv_bfloat16, 64) }
     else if (D == 128) { ASTRAI_ATTEND(__half, 128) }
