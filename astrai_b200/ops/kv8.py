@@ -140,7 +140,12 @@ def _attention_reference(q, cache: KV8, page_table, lens, starts, scale) -> torc
     s = torch.einsum("bshd,bkhd->bhsk", q.float(), k.repeat_interleave(G, 2)) * scale
     p = torch.softmax(s.masked_fill(~seen[:, None], -math.inf), -1)
     p = torch.where(seen.any(-1)[:, None, :, None], p, 0.0)
-    return torch.einsum("bhsk,bkhd->bshd", p, v.repeat_interleave(G, 2)).to(q.dtype)
+    v = v.repeat_interleave(G, 2)
+    bad = ~torch.isfinite(v)
+    o = torch.einsum("bhsk,bkhd->bshd", p, v.masked_fill(bad, 0.0))
+    if bad.any():  # a weight of 0 would not keep what is not finite out of a sum
+        o = o.masked_fill(torch.einsum("bsk,bkhd->bshd", seen.float(), bad.float()) > 0, math.nan)
+    return o.to(q.dtype)
 
 
 def kv8_attention(q: torch.Tensor, cache: KV8, page_table: torch.Tensor, lens: torch.Tensor,
