@@ -58,6 +58,7 @@ class KV8(NamedTuple):
 
 
 # ----------------------------------------------------------------------------- append
+@torch.no_grad()
 def _append_reference(cache: KV8, k, v, page_table, starts, lens) -> None:
     block, page = cache.block, cache.page_size
     S = k.shape[1]
@@ -94,7 +95,7 @@ def kv8_append(cache: KV8, k: torch.Tensor, v: torch.Tensor, page_table: torch.T
     void. A block that held earlier tokens ends under the larger of the two magnitudes, and its integers
     are rounded again when that grew. Tokens before position 0 and tokens whose page is missing are
     dropped. A block with an infinity or NaN among its new values reads as NaN. No page may be in the
-    table twice.
+    table twice. No gradient reaches k and v through the cache.
     """
     if cache.k.is_cuda:
         native().kv8_append(k, v, *cache, page_table, starts, lens)
