@@ -170,6 +170,7 @@ struct QkNormRopeBackward : public torch::autograd::Node {
     std::lock_guard<std::mutex> lock(mutex_);
     torch::autograd::variable_list out(3);
     if (!grads[0].defined()) return out;
+    TORCH_CHECK(!grads[0]._fw_grad(0).defined(), "qk_norm_rope has no second derivative (a tangent in its backward)");
     const at::Tensor x_ = x.unpack(), table_ = table.unpack(), dy = rows_of(grads[0]);
     const auto given_or_none = [](const at::Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
     const int64_t used = (o.hq + o.hkv) * o.D;
@@ -185,8 +186,6 @@ struct QkNormRopeBackward : public torch::autograd::Node {
 at::Tensor with_gradient(const at::Tensor& x, const OptTensor& wq, const OptTensor& wk, const at::Tensor& table,
                          const OptTensor& pos, const Options& o) {
   const auto or_none = [](const OptTensor& t) { return given(t) ? *t : at::Tensor(); };
-  for (const auto& t : {x, or_none(wq), or_none(wk)})
-    TORCH_CHECK(!t.defined() || !t._fw_grad(0).defined(), "qk_norm_rope has no forward-mode derivative");
   at::Tensor rows, y;
   {
     const at::NoGradGuard off;
@@ -221,6 +220,11 @@ at::Tensor qk_norm_rope(const at::Tensor& x, int64_t hq, int64_t hkv, int64_t D,
     TORCH_CHECK_VALUE(pos->numel() == x.size(0), "qk_norm_rope: positions must have one entry per row");
     if (pos->scalar_type() != at::kInt || !pos->is_contiguous()) pos = pos->to(at::kInt).contiguous();
   }
+  // a dual number need not require a gradient, and GradMode does not stop tangents
+  const at::Tensor* const inputs[] = {&x, &table, given(wq) ? &*wq : nullptr, given(wk) ? &*wk : nullptr};
+  for (const at::Tensor* t : inputs)
+    TORCH_CHECK(!t || !t->_fw_grad(0).defined(), "qk_norm_rope has no forward-mode derivative");
+  TORCH_CHECK(!(at::GradMode::is_enabled() && table.requires_grad()), "qk_norm_rope has no gradient of the table");
   const bool grad = at::GradMode::is_enabled() &&
                     (x.requires_grad() || (norm && (wq->requires_grad() || wk->requires_grad())));
   const Options o{hq, hkv, D, seq_len, rot, rot_off, norm, half_layout, eps};

@@ -112,7 +112,7 @@ def qk_norm_rope(x: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: int, 
     position ``r % seq_len``); a position outside the table leaves its row unrotated and sets the device
     error word. ``rot_dim`` channels from ``rot_off`` are rotated (None: all). On CUDA ``head_dim`` is at
     most 256, and it, ``rot_dim`` and ``rot_off`` are multiples of 8. Differentiable in ``x`` and the
-    weights.
+    weights, in reverse mode and once; on CUDA tangents and a table that requires a gradient are refused.
     """
     rot = head_dim if rot_dim is None else rot_dim
     if x.is_cuda:
