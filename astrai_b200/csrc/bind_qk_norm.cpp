@@ -229,7 +229,7 @@ at::Tensor qk_norm_rope(const at::Tensor& x, int64_t hq, int64_t hkv, int64_t D,
                     (x.requires_grad() || (norm && (wq->requires_grad() || wk->requires_grad())));
   const Options o{hq, hkv, D, seq_len, rot, rot_off, norm, half_layout, eps};
   if (in_place) {
-    TORCH_CHECK(!(at::GradMode::is_enabled() && x.requires_grad()), "qk_norm_rope_ has no gradient: use qk_norm_rope");
+    TORCH_CHECK(!grad, "qk_norm_rope_ has no gradient (of x or the weights): use qk_norm_rope");
     forward_into(x, x, table, pos, wq, wk, o, false);
     if (!x.is_inference()) x.unsafeGetTensorImpl()->bump_version();  // a backward that saved x has to notice
     return x;

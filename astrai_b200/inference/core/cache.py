@@ -566,7 +566,8 @@ class PageCacheView(CacheView):
         pos = self.positions(S)
         qkv = qkv.detach()  # changed in place, and attention over a cache has no gradient
         if rotary is not None:
-            rotary.apply_(qkv, Hq, Hkv, D, positions=pos)
+            with torch.no_grad():
+                rotary.apply_(qkv, Hq, Hkv, D, positions=pos)
         else:
             rope_inplace(qkv, 0, Hq + Hkv, D, table, pos, S)
         if self._int8:

@@ -128,14 +128,16 @@ def qk_norm_rope_(x: torch.Tensor, n_heads: int, n_kv_heads: int, head_dim: int,
                   positions: Optional[torch.Tensor] = None, seq_len: Optional[int] = None, eps: float = 1e-6,
                   layout: str = "interleaved", norm: str = "after", rot_dim: Optional[int] = None,
                   rot_off: int = 0) -> torch.Tensor:
-    """:func:`qk_norm_rope` in place on the query and key columns of ``x`` (no gradient) -> ``x``."""
+    """:func:`qk_norm_rope` in place on the query and key columns of ``x`` -> ``x``. It has no gradient: under grad
+    mode no input may require one."""
     rot = head_dim if rot_dim is None else rot_dim
     if x.is_cuda:
         return _native(x, n_heads, n_kv_heads, head_dim, table, q_weight, k_weight, positions, seq_len, eps, layout, norm,
                        rot, rot_off, True)
     _check(x, n_heads, n_kv_heads, head_dim, table, q_weight, k_weight, positions, seq_len, layout, norm, rot, rot_off)
-    if torch.is_grad_enabled() and x.requires_grad:
-        raise RuntimeError("qk_norm_rope_ has no gradient: use qk_norm_rope")
+    inputs = (x, table) if norm == "none" else (x, table, q_weight, k_weight)
+    if torch.is_grad_enabled() and any(t.requires_grad for t in inputs):
+        raise RuntimeError("qk_norm_rope_ has no gradient (of x, the weights or the table): use qk_norm_rope")
     x[:, : (n_heads + n_kv_heads) * head_dim] = qk_norm_rope_reference(
         x, n_heads, n_kv_heads, head_dim, table, q_weight, k_weight, positions, seq_len, eps, layout, norm, rot, rot_off)
     return x

@@ -55,3 +55,19 @@ def test_a_tangent_in_the_backward_is_refused():
     with forward_ad.dual_level():
         with pytest.raises(RuntimeError, match="second derivative"):
             torch.autograd.grad(y, leaf, forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y)))
+
+
+@pytest.mark.parametrize("which", ["q_weight", "k_weight"])
+def test_in_place_refuses_weights_that_require_a_gradient(which):
+    from astrai_b200.ops.qk_norm import qk_norm_rope_
+
+    x, wq, wk, t = _inputs()
+    kw = dict(table=t, q_weight=wq, k_weight=wk)
+    kw[which] = kw[which].clone().requires_grad_()
+    before = x.clone()
+    with pytest.raises(RuntimeError, match="no gradient"):
+        qk_norm_rope_(x, 2, 1, 64, seq_len=6, **kw)
+    assert torch.equal(x, before)
+    qk_norm_rope_(x.clone(), 2, 1, 64, seq_len=6, norm="none", **kw)  # the weight has no part in it
+    with torch.no_grad():
+        assert qk_norm_rope_(x, 2, 1, 64, seq_len=6, **kw) is x
