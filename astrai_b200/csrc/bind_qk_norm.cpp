@@ -157,7 +157,7 @@ at::Tensor rows_of(const at::Tensor& t) {
 // The autograd node, in C++ and a Node of its own: a training step of short kernels would otherwise wait for Python,
 // and for the list and dictionary in which torch::autograd::Function keeps what it was given.
 struct QkNormRopeBackward : public torch::autograd::Node {
-  torch::autograd::SavedVariable x, wq, wk, table, pos;
+  torch::autograd::SavedVariable x, wq, wk, table, pos;  // x and the weights: undefined without a norm
   Options o;
   int64_t width = 0;  // columns of x
   std::string name() const override { return "QkNormRopeBackward"; }
@@ -171,10 +171,10 @@ struct QkNormRopeBackward : public torch::autograd::Node {
     torch::autograd::variable_list out(3);
     if (!grads[0].defined()) return out;
     TORCH_CHECK(!grads[0]._fw_grad(0).defined(), "qk_norm_rope has no second derivative (a tangent in its backward)");
-    const at::Tensor x_ = x.unpack(), table_ = table.unpack(), dy = rows_of(grads[0]);
+    const at::Tensor table_ = table.unpack(), dy = rows_of(grads[0]), x_ = o.norm ? x.unpack() : dy;
     const auto given_or_none = [](const at::Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
     const int64_t used = (o.hq + o.hkv) * o.D;
-    auto dx = new_like(x_, {x_.size(0), width}, x_.scalar_type());
+    auto dx = new_like(dy, {dy.size(0), width}, dy.scalar_type());
     if (width > used) dx.narrow(1, used, width - used).zero_();  // columns behind the keys are not an input
     auto dw = backward_into(dy, x_, dx, table_, given_or_none(pos.unpack()), given_or_none(wq.unpack()),
                             given_or_none(wk.unpack()), o);
@@ -195,7 +195,8 @@ at::Tensor with_gradient(const at::Tensor& x, const OptTensor& wq, const OptTens
   }
   std::shared_ptr<QkNormRopeBackward> node(new QkNormRopeBackward(), torch::autograd::deleteNode);
   node->set_next_edges(torch::autograd::collect_next_edges(x, or_none(wq), or_none(wk)));
-  node->x = {rows, false}, node->wq = {or_none(wq), false}, node->wk = {or_none(wk), false};
+  if (o.norm) node->x = {rows, false};  // a rotation's gradient does not depend on its input
+  node->wq = {or_none(wq), false}, node->wk = {or_none(wk), false};
   node->table = {table, false}, node->pos = {or_none(pos), false};
   node->o = o, node->width = x.size(1);
   torch::autograd::set_history(y, node);

@@ -71,3 +71,20 @@ def test_in_place_refuses_weights_that_require_a_gradient(which):
     qk_norm_rope_(x.clone(), 2, 1, 64, seq_len=6, norm="none", **kw)  # the weight has no part in it
     with torch.no_grad():
         assert qk_norm_rope_(x, 2, 1, 64, seq_len=6, **kw) is x
+
+
+def test_a_rotation_alone_keeps_no_input():
+    """Its backward is the transposed rotation of the gradient: x may change before it, and is not kept alive."""
+    from astrai_b200.ops.qk_norm import qk_norm_rope
+
+    x, _, _, t = _inputs()
+    dy = torch.randn(6, 192, device="cuda", generator=torch.Generator(device="cuda").manual_seed(1)).to(torch.bfloat16)
+    leaf = x.clone().requires_grad_()
+    want = torch.autograd.grad(qk_norm_rope(leaf, 2, 1, 64, t, norm="none", seq_len=6), leaf, dy)[0]
+    kept = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda v: kept.append(v.shape) or v, lambda v: v):
+        y = qk_norm_rope(leaf, 2, 1, 64, t, norm="none", seq_len=6)
+    assert leaf.shape not in kept
+    with torch.no_grad():
+        leaf.mul_(2)
+    assert torch.equal(torch.autograd.grad(y, leaf, dy)[0], want)
