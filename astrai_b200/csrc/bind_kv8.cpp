@@ -179,6 +179,8 @@ int64_t kv8_attend_workspace(int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int6
 at::Tensor kv8_attend(const at::Tensor& q_in, const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& ka,
                       const at::Tensor& va, const at::Tensor& table_in, const at::Tensor& lens_in,
                       const OptTensor& starts_in, const OptTensor& workspace, double scale) {
+  TORCH_CHECK(!(at::GradMode::is_enabled() && q_in.requires_grad()), "kv8_attention has no gradient: detach the query");
+  TORCH_CHECK(!q_in._fw_grad(0).defined(), "kv8_attention has no forward-mode derivative");
   const Cache c = check_cache(kc, vc, ka, va);
   const at::Tensor q = heads_of(q_in), table = int32_of(table_in), lens = int32_of(lens_in);
   long long qs[3];

@@ -347,10 +347,10 @@ class Int8Storage(Storage):
         kv8_append(self.layers[layer_id], k, v, table, starts, lens)
 
     def attend_rows(self, layer_id: int, q: Tensor, table: Tensor, lens: Tensor) -> Tensor:
-        """Causal attention of the rows' last tokens, q ``[B, S, Hq, D]``, over the cached ones."""
+        """Causal attention of the rows' last tokens, q ``[B, S, Hq, D]``, over the cached ones (no gradient)."""
         from astrai_b200.ops.kv8 import kv8_attention
 
-        return kv8_attention(q, self.layers[layer_id], table, lens)
+        return kv8_attention(q.detach(), self.layers[layer_id], table, lens)
 
     def write_slots(self, layer_id: int, slots: Tensor, k: Tensor, v: Tensor) -> None:
         raise RuntimeError("an int8 KV cache takes consecutive tokens of rows (append_rows), not single slots: "

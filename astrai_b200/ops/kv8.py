@@ -160,7 +160,8 @@ def kv8_attention(q: torch.Tensor, cache: KV8, page_table: torch.Tensor, lens: t
     with no page to read gives zeros. Query head ``h`` reads KV head ``h // (n_heads // n_kv_heads)``.
     ``scale`` defaults to ``1 / sqrt(head_dim)``. ``workspace`` fp32 of :func:`kv8_attention_workspace`
     elements is used if given (a caller that captures graphs keeps one per stream); otherwise one is
-    allocated.
+    allocated. On CUDA it has no gradient: under grad mode a query that requires one is refused, and so is a
+    tangent.
     """
     sc = float(scale) if scale is not None else 1.0 / math.sqrt(q.shape[-1])
     if not cache.k.is_cuda:
