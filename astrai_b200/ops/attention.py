@@ -28,6 +28,7 @@ from typing import Optional
 
 import torch
 import torch.nn.functional as F
+from torch.autograd.function import once_differentiable
 
 from astrai_b200.ops._ext import native
 from astrai_b200.ops.rope import apply_rope_reference, rope_inplace
@@ -181,6 +182,7 @@ class _AttnQKNormFn(torch.autograd.Function):
         return o
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, do):
         qkv, qk, o, lse, q_weight, k_weight, table, positions, seg = ctx.saved_tensors
         B, S, Hq, Hkv, causal, rot, off, half, mode, eps = ctx.dims
