@@ -44,15 +44,26 @@ int dtype_code(const at::Tensor& t) {
   return -1;
 }
 
+bool on_grid(const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
+bool rows_on_grid(const at::Tensor& t) {
+  return t.stride(1) == 1 && (t.size(0) <= 1 || (t.stride(0) * t.element_size()) % 16 == 0) && on_grid(t);
+}
+// The first `used` columns as the kernels can read them: t itself, or a copy (contiguous() would return a contiguous
+// tensor as it is, wherever its rows start).
+at::Tensor rows_of(const at::Tensor& t, int64_t used) {
+  return rows_on_grid(t) ? t : t.narrow(1, 0, used).clone(at::MemoryFormat::Contiguous);
+}
+OptTensor weight_of(const OptTensor& w) {
+  return given(w) && !(w->is_contiguous() && on_grid(*w)) ? OptTensor(w->clone(at::MemoryFormat::Contiguous)) : w;
+}
+
 // rows of at least `width` columns, of like's type and device, each on a 16-byte boundary
 void check_rows(const at::Tensor& t, const at::Tensor& like, int64_t width, const char* name) {
   TORCH_CHECK(t.is_cuda() && t.device() == like.device() && t.scalar_type() == like.scalar_type(), "qk_norm_rope: ",
               name, " must be a CUDA tensor of the input's type and device");
   TORCH_CHECK(t.dim() == 2 && t.size(0) == like.size(0) && t.size(1) >= width, "qk_norm_rope: ", name,
               " must be [rows, >= (n_heads + n_kv_heads) * head_dim]");
-  TORCH_CHECK(t.stride(1) == 1 && (t.stride(0) * t.element_size()) % 16 == 0 &&
-                  reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0,
-              "qk_norm_rope: ", name, " needs a contiguous inner dimension and 16-byte aligned rows");
+  TORCH_CHECK(rows_on_grid(t), "qk_norm_rope: ", name, " needs a contiguous inner dimension and 16-byte aligned rows");
 }
 void check_output(const at::Tensor& t, const at::Tensor& like, int64_t width, const char* name) {
   check_rows(t, like, width, name);
@@ -78,7 +89,7 @@ Shape check(const at::Tensor& x, int64_t hq, int64_t hkv, int64_t D, const at::T
   check_rows(x, x, (hq + hkv) * D, "x");
   TORCH_CHECK(table.is_cuda() && table.device() == x.device() && table.scalar_type() == at::kFloat &&
                   table.is_contiguous() && table.dim() == 3 && table.size(1) == rot / 2 && table.size(2) == 2 &&
-                  reinterpret_cast<uintptr_t>(table.data_ptr()) % 16 == 0,
+                  on_grid(table),
               "qk_norm_rope: table must be contiguous fp32 [max_pos, rot_dim / 2, 2] on x's device, 16-byte aligned");
   s.pos = nullptr;
   if (given(pos)) {
@@ -92,8 +103,7 @@ Shape check(const at::Tensor& x, int64_t hq, int64_t hkv, int64_t D, const at::T
   if (norm != 0) {
     for (const auto* w : {&wq, &wk}) {
       TORCH_CHECK(given(*w) && (*w)->device() == x.device() && (*w)->scalar_type() == x.scalar_type() &&
-                      (*w)->is_contiguous() && (*w)->numel() == D &&
-                      reinterpret_cast<uintptr_t>((*w)->data_ptr()) % 16 == 0,
+                      (*w)->is_contiguous() && (*w)->numel() == D && on_grid(**w),
                   "qk_norm_rope: weights must be contiguous [head_dim], of x's type and device, 16-byte aligned");
     }
   }
@@ -112,7 +122,8 @@ cudaStream_t stream() { return at::cuda::getCurrentCUDAStream().stream(); }
 
 // y may be x itself
 void forward_into(const at::Tensor& x, const at::Tensor& y, const at::Tensor& table, const OptTensor& pos,
-                  const OptTensor& wq, const OptTensor& wk, const Options& o, bool inverse) {
+                  const OptTensor& wq_in, const OptTensor& wk_in, const Options& o, bool inverse) {
+  const OptTensor wq = weight_of(wq_in), wk = weight_of(wk_in);
   const Shape s = check(x, o.hq, o.hkv, o.D, table, pos, o.seq_len, wq, wk, o.rot, o.rot_off, o.norm);
   check_output(y, x, (o.hq + o.hkv) * o.D, "y");
   const c10::cuda::CUDAGuard g(x.device());
@@ -125,8 +136,9 @@ void forward_into(const at::Tensor& x, const at::Tensor& y, const at::Tensor& ta
 
 // Fills the query and key columns of dx; -> gradients of the weights (undefined without a norm).
 std::pair<at::Tensor, at::Tensor> backward_into(const at::Tensor& dy, const at::Tensor& x, const at::Tensor& dx,
-                                                const at::Tensor& table, const OptTensor& pos, const OptTensor& wq,
-                                                const OptTensor& wk, const Options& o) {
+                                                const at::Tensor& table, const OptTensor& pos,
+                                                const OptTensor& wq_in, const OptTensor& wk_in, const Options& o) {
+  const OptTensor wq = weight_of(wq_in), wk = weight_of(wk_in);
   if (o.norm == 0) {  // the transposed rotation
     forward_into(dy, dx, table, pos, wq, wk, o, true);
     return {};
@@ -147,13 +159,6 @@ std::pair<at::Tensor, at::Tensor> backward_into(const at::Tensor& dy, const at::
   return {dwq, dwk};
 }
 
-// a row view that the kernels can read, copied if t is none
-at::Tensor rows_of(const at::Tensor& t) {
-  const bool ok = t.stride(1) == 1 && (t.stride(0) * t.element_size()) % 16 == 0 &&
-                  reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
-  return ok ? t : t.contiguous();
-}
-
 // The autograd node, in C++ and a Node of its own: a training step of short kernels would otherwise wait for Python,
 // and for the list and dictionary in which torch::autograd::Function keeps what it was given.
 struct QkNormRopeBackward : public torch::autograd::Node {
@@ -171,10 +176,12 @@ struct QkNormRopeBackward : public torch::autograd::Node {
     torch::autograd::variable_list out(3);
     if (!grads[0].defined()) return out;
     TORCH_CHECK(!grads[0]._fw_grad(0).defined(), "qk_norm_rope has no second derivative (a tangent in its backward)");
-    const at::Tensor table_ = table.unpack(), dy = rows_of(grads[0]), x_ = o.norm ? x.unpack() : dy;
+    const at::Tensor table_ = table.unpack(), dy = rows_of(grads[0], grads[0].size(1)),
+                     x_ = o.norm ? x.unpack() : dy;
     const auto given_or_none = [](const at::Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
     const int64_t used = (o.hq + o.hkv) * o.D;
-    auto dx = new_like(dy, {dy.size(0), width}, dy.scalar_type());
+    const int64_t grid = 16 / dy.element_size();  // rows of dx start on the 16-byte grid, whatever x's width is
+    auto dx = new_like(dy, {dy.size(0), (width + grid - 1) / grid * grid}, dy.scalar_type()).narrow(1, 0, width);
     if (width > used) dx.narrow(1, used, width - used).zero_();  // columns behind the keys are not an input
     auto dw = backward_into(dy, x_, dx, table_, given_or_none(pos.unpack()), given_or_none(wq.unpack()),
                             given_or_none(wk.unpack()), o);
@@ -189,7 +196,7 @@ at::Tensor with_gradient(const at::Tensor& x, const OptTensor& wq, const OptTens
   at::Tensor rows, y;
   {
     const at::NoGradGuard off;
-    rows = rows_of(x);
+    rows = rows_of(x, (o.hq + o.hkv) * o.D);
     y = new_like(x, {x.size(0), (o.hq + o.hkv) * o.D}, x.scalar_type());
     forward_into(rows, y, table, pos, wq, wk, o, false);
   }
@@ -238,7 +245,7 @@ at::Tensor qk_norm_rope(const at::Tensor& x, int64_t hq, int64_t hkv, int64_t D,
   if (grad)
     return with_gradient(x, wq, wk, table, pos, o);
   auto y = new_like(x, {x.size(0), (hq + hkv) * D}, x.scalar_type());
-  forward_into(rows_of(x), y, table, pos, wq, wk, o, false);
+  forward_into(rows_of(x, (hq + hkv) * D), y, table, pos, wq, wk, o, false);
   return y;
 }
 
