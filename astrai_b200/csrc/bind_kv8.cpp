@@ -88,12 +88,12 @@ int dtype_code(const at::Tensor& t, const char* name) {
 }
 
 // [B, S, H, D] as the kernels read it: a contiguous last dimension and 16-byte aligned rows of any stride;
-// copied if it is not
+// copied if it is not (contiguous() would return a contiguous tensor as it is, wherever it starts)
 at::Tensor heads_of(const at::Tensor& t) {
   if (t.dim() != 4) return t;  // refused by check_heads
   bool ok = t.stride(3) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
   for (int i = 0; i < 3; ++i) ok = ok && (t.size(i) <= 1 || t.stride(i) % 8 == 0);
-  return ok ? t : t.contiguous();
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);
 }
 at::Tensor int32_of(const at::Tensor& t) {
   return t.scalar_type() == at::kInt && t.is_contiguous() ? t : t.to(at::kInt).contiguous();

@@ -69,3 +69,24 @@ def test_qk_norm_rope_gradient_through_a_concatenation():
     y = qk_norm_rope(leaf, 4, 2, 64, t, wq, wk, seq_len=5)
     flat = torch.cat([torch.zeros(3, device="cuda", dtype=x.dtype), y.flatten()])
     assert torch.equal(torch.autograd.grad(flat, leaf, torch.cat([flat.detach()[:3], dy.flatten()]))[0], want)
+
+
+@pytest.mark.parametrize("dtype", DTYPES[:2])
+def test_kv8_operands_off_the_grid(dtype):
+    from astrai_b200.ops.kv8 import KV8, kv8_append, kv8_attention
+
+    g = torch.Generator(device="cuda").manual_seed(0)
+    B, S, H, D, page, block = 2, 3, 2, 64, 32, 16
+    k, v = (torch.randn(B, S, H, D, device="cuda", generator=g).to(dtype) for _ in range(2))
+    q = torch.randn(B, S, 4, D, device="cuda", generator=g).to(dtype)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    table, starts, lens = torch.tensor([[0, 1], [2, 3]], **i32), torch.tensor([0, 0], **i32), torch.tensor([3, 2], **i32)
+    want, got = (KV8.allocate(4, H, page, D, block, "cuda") for _ in range(2))
+    kv8_append(want, k, v, table, starts, lens)
+    kv8_append(got, _off(k), _off(v, 3), table, starts, lens)
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and want.k.any()
+    assert torch.equal(kv8_attention(_off(q), want, table, lens), kv8_attention(q, want, table, lens))
+    one = torch.zeros(1, 1, 4 * D + 3, device="cuda", dtype=dtype)  # one token cut from a wider odd buffer
+    one[..., 1: -2] = q[:1, :1].flatten(2)
+    cut = one[..., 1: -2].unflatten(-1, (4, D))
+    assert torch.equal(kv8_attention(cut, want, table[:1], lens[:1]), kv8_attention(q[:1, :1], want, table[:1], lens[:1]))
