@@ -63,10 +63,12 @@ def scaled_rope_table(dim: int, max_len: int, base: float = 10000.0, method: str
 
     * ``linear``: position interpolation, every angle divided by ``factor``.
     * ``yarn`` (Peng et al., "YaRN: Efficient Context Window Extension of Large Language Models", 2023):
-      a pair that turns r times over ``original_max_len`` positions is interpolated if r <= ``beta_slow``,
-      left alone if r >= ``beta_fast``, and mixed linearly in r between; (cos, sin) are multiplied by
-      ``attention_factor`` (None: ``0.1 ln(factor) + 1``, and 1 for factors up to 1), which scales the
-      scores by its square. The table is then no pure rotation.
+      pairs up to the one that turns ``beta_fast`` times over ``original_max_len`` positions are left alone,
+      those from the one that turns ``beta_slow`` times on are interpolated. Between the two, rounded
+      outwards to whole pairs and clamped to [0, dim - 1], the mix is linear in the pair's index, as in the
+      tables that published checkpoints run with (the paper's text has it linear in the number of turns).
+      (cos, sin) are multiplied by ``attention_factor`` (None: ``0.1 ln(factor) + 1``, and 1 for factors up
+      to 1), which scales the scores by its square. The table is then no pure rotation.
     """
     if method not in ROPE_SCALING_METHODS:
         raise ValueError(f"method must be one of {ROPE_SCALING_METHODS}, got {method!r}")
@@ -77,10 +79,16 @@ def scaled_rope_table(dim: int, max_len: int, base: float = 10000.0, method: str
     if method == "linear":
         inv = inv / factor
     else:
-        if not original_max_len or beta_fast <= beta_slow:
-            raise ValueError("yarn needs original_max_len and beta_fast > beta_slow")
-        turns = original_max_len * inv / (2 * math.pi)
-        keep = ((turns - beta_slow) / (beta_fast - beta_slow)).clamp(0, 1)
+        if not original_max_len or original_max_len < 0 or not beta_fast > beta_slow > 0 or base <= 1:
+            raise ValueError("yarn needs original_max_len, beta_fast > beta_slow > 0 and a base above 1")
+
+        def pair_of(turns):  # where original_max_len * base^(-2i / dim) / (2 pi) = turns
+            return dim * math.log(original_max_len / (2 * math.pi * turns)) / (2 * math.log(base))
+
+        low = min(max(math.floor(pair_of(beta_fast)), 0), dim - 1)
+        high = min(max(math.ceil(pair_of(beta_slow)), 0), dim - 1)
+        pair = torch.arange(dim // 2, dtype=torch.float64, device=device)
+        keep = 1 - ((pair - low) / max(high - low, 1e-3)).clamp(0, 1)
         inv = inv / factor * (1 - keep) + inv * keep
         gain = attention_factor if attention_factor is not None else 0.1 * math.log(factor) + 1 if factor > 1 else 1.0
     ang = torch.outer(torch.arange(max_len, dtype=torch.float64, device=device), inv)
