@@ -15,7 +15,7 @@ the reference behaviour:
 * ``rope_layout``        - ``"interleaved"`` (reference) or ``"half"``: channel i
                             rotates with i + rotated channels / 2;
 * ``rope_fraction``      - share of each head's channels that is rotated, the
-                            first ones (1.0);
+                            first ones (1.0): a multiple of 8 channels;
 * ``rope_scaling_method`` - ``"linear"`` or ``"yarn"``: long-context scaling of
                             the angle table with ``rope_scaling``'s ``factor``,
                             ``original_max_position_embeddings``,
@@ -26,7 +26,9 @@ the reference behaviour:
 * ``fused_qk_norm``      - QK-norm and rotation in one pass over the projection
                             output, rounded once. Any of ``rope_layout="half"``,
                             ``rope_fraction < 1`` and ``qk_norm_first`` implies
-                            it. These five apply to ``attn_type="gqa"``.
+                            it. Head sizes that are multiples of 8, at most 256.
+                            ``rope_layout``, ``rope_fraction`` and the last two
+                            apply to ``attn_type="gqa"``.
 """
 
 from __future__ import annotations

@@ -79,8 +79,8 @@ class GQA(nn.Module):
         assert dim % n_heads == 0 and n_heads % n_kv_heads == 0
         if rope_layout not in (None, "interleaved", "half"):
             raise ValueError(f"rope_layout must be 'interleaved' or 'half', got {rope_layout!r}")
+        turned = dim // n_heads * (1.0 if rope_fraction is None else rope_fraction)
         if rope_fraction is not None:
-            turned = dim // n_heads * rope_fraction
             if not 0 < rope_fraction <= 1 or abs(turned - round(turned)) > 1e-6 or round(turned) % 2:
                 raise ValueError(f"rope_fraction must be an even number of a head's {dim // n_heads} channels, "
                                  f"got {rope_fraction}")
@@ -93,6 +93,10 @@ class GQA(nn.Module):
         self.qk_norm_first = bool(qk_norm_first)
         self.one_pass = (self.rope_layout == "half" or (rope_fraction or 1.0) < 1 or self.qk_norm_first
                          or bool(fused_qk_norm))
+        if self.one_pass and (self.head_dim % 8 or self.head_dim > 256 or round(turned) % 8):
+            raise ValueError("norm and rotation in one pass (rope_layout='half', rope_fraction < 1, qk_norm_first, "
+                             "fused_qk_norm) need a head size of at most 256 that is a multiple of 8, and a multiple of 8 "
+                             f"rotated channels, got {self.head_dim} and {round(turned)}")
         self.q_proj = Linear(dim, n_heads * self.head_dim)
         self.k_proj = Linear(dim, n_kv_heads * self.head_dim)
         self.v_proj = Linear(dim, n_kv_heads * self.head_dim)
