@@ -28,7 +28,7 @@ the reference behaviour:
                             ``rope_fraction < 1`` and ``qk_norm_first`` implies
                             it. Head sizes that are multiples of 8, at most 256.
                             ``rope_layout``, ``rope_fraction`` and the last two
-                            apply to ``attn_type="gqa"``.
+                            apply to ``attn_type="gqa"``; MLA refuses them.
 """
 
 from __future__ import annotations

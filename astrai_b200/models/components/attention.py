@@ -215,8 +215,16 @@ class MLA(nn.Module):
 
     def __init__(self, dim: int, n_heads: int, n_kv_heads: int, kv_lora_rank: int, qk_nope_head_dim: int,
                  qk_rope_head_dim: int, norm_eps: float = 1e-6, use_qk_norm: bool = False,
-                 use_gated_attention: bool = False, layer_id: int = 0, n_layers: int = 1):
+                 use_gated_attention: bool = False, layer_id: int = 0, n_layers: int = 1,
+                 rope_layout: Optional[str] = None, rope_fraction: Optional[float] = None,
+                 qk_norm_first: Optional[bool] = None, fused_qk_norm: Optional[bool] = None):
         super().__init__()
+        for name, given in (("rope_layout", rope_layout not in (None, "interleaved")),
+                            ("rope_fraction", rope_fraction not in (None, 1)),
+                            ("qk_norm_first", qk_norm_first), ("fused_qk_norm", fused_qk_norm)):
+            if given:
+                raise ValueError(f"{name} is an option of attn_type='gqa': MLA rotates the rope part of each head in the "
+                                 "interleaved layout and normalises it afterwards")
         self.dim, self.n_heads, self.n_kv_heads = dim, n_heads, n_kv_heads
         self.kv_lora_rank = kv_lora_rank
         self.qk_nope_head_dim, self.qk_rope_head_dim = qk_nope_head_dim, qk_rope_head_dim
