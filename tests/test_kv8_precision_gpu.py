@@ -64,3 +64,25 @@ def test_a_tail_far_behind_one_key_keeps_its_bits(n, S, Hq, Hkv, D, ahead, dtype
             tol = HALF_SPACING[dtype] * want + (2.0 ** -17 + 2.0 ** -20 * reach) * want \
                 + m * 2.0 ** -32 * prob.max() * 0.75
             assert ((got[0, i, h] - want).abs() <= tol).all(), ((got[0, i, h] - want).abs() / tol).max().item()
+
+
+def test_a_block_that_reads_as_nan_reaches_only_the_queries_that_see_it():
+    from astrai_b200.ops.kv8 import KV8, kv8_append, kv8_attention
+
+    B, H, D, page, block, n, S = 2, 2, 64, 32, 16, 34, 4
+    g = torch.Generator(device="cuda").manual_seed(0)
+    k, v = (torch.randn(B, n, H, D, device="cuda", generator=g).bfloat16() for _ in range(2))
+    i32 = dict(dtype=torch.int32, device="cuda")
+    table, zero, lens = torch.tensor([[0, 1], [2, 3]], **i32), torch.zeros(B, **i32), torch.full((B,), n, **i32)
+    clean, dirty = (KV8.allocate(4, H, page, D, block, "cuda") for _ in range(2))
+    kv8_append(clean, k, v, table, zero, lens)
+    for x in (k, v):
+        x[0, 33, 1] = float("nan")  # token 33 shares its block with token 32 alone
+    kv8_append(dirty, k, v, table, zero, lens)
+    for heads in (2, 4, 16):  # two, four and sixteen query rows of a KV head
+        q = torch.randn(B, S, heads, D, device="cuda", generator=g).bfloat16()
+        want, got = kv8_attention(q, clean, table, lens), kv8_attention(q, dirty, table, lens)
+        bad = torch.zeros(B, S, heads, dtype=torch.bool, device="cuda")
+        bad[0, 2:, heads // 2:] = True  # tokens 32 and 33, the query heads of KV head 1
+        assert torch.equal(got.isnan().all(-1), bad) and torch.equal(got.isnan().any(-1), bad)
+        assert torch.equal(got[~bad], want[~bad])
