@@ -406,14 +406,15 @@ struct Piece {       // of a segment, on one CTA
 // own near the maximum of s + log2 absmax_v, so as fp16 they keep their precision whatever the
 // magnitudes of the blocks. out = sum w v / l * 2^(M - m) / 127.
 //
-// Bound by HBM on long rows (4 x 131072 tokens of 4 heads of 128: 94 us, 0.87 of the copy rate), by its start (1.7 us
-// to the first copy), merge (2 us) and join (3 us) on short ones (32 x 4096: 31.6 us, 0.65). Two CTAs of 8 warps per
-// SM: with 4 or 16 warps per CTA the long case takes 114 or 96 us.
+// Bound by HBM on long rows (4 x 131072 tokens of 4 heads of 128: 94 us, 0.88 of the copy rate), by its start (1.7 us
+// to the first copy), merge (2 us) and join (3 us) on short ones (32 x 4096: 31.9 us, 0.65). Two CTAs of 8 warps per
+// SM: with 4 or 16 warps per CTA the long case took 114 or 96 us.
 //
-// A weight is held as two fp16 numbers, itself and what that leaves, 22 bits in all: rounded once, the weights put
-// errors of up to 3.3e-4 in norm into outputs whose own rounding is 2.1e-4 (fp16) and moved 7e-4 of bfloat16 ones to
-// the next value; now both are below 2e-4. TWIN: at most four query rows, each in two columns, one of which takes
-// what the other's weights leave (32 x 4096: 32.3 us); otherwise a second product does (34.5 us for the same).
+// A weight is held as two fp16 numbers, itself and what that leaves, 22 bits in all. Rounded once, the weights put
+// errors of up to 3.3e-4 in norm into fp16 outputs, whose own rounding is 2.1e-4, and bfloat16 outputs differed by
+// 6e-4 to 8e-4 from those of weights in fp32; as two numbers by less than 2e-4. TWIN: at most four query rows, each
+// in two columns, one of which takes what the other's weights leave (32 x 4096 tokens: 32.3 us); otherwise a second
+// product does (34.5 us for the same).
 template <typename T, int D, int NT, int STAGES, bool TWIN>
 __global__ void __launch_bounds__(kWarps * 32, NT == 1 ? 2 : 1) kv8_attend_kernel(const AttendParams p) {
   constexpr int KS = D / 16;     // k-steps of S^T = K Q^T
@@ -1002,8 +1003,9 @@ struct AttendPlan {
 // Splitting rows over CTAs evens the work out but costs the join, a second piece for many CTAs and, with
 // that, about kJoinUs; whole rows cost the idle slots of the last wave and, if they are few, the rate that one
 // CTA reaches alone. Both sides are estimated from rates measured on B200 (cache bytes: 6 TB/s in all, 36 GB/s
-// for one CTA): at 64 rows of 1024 tokens of 4 heads of 128 whole rows take 18.5 us and split ones 24.0, at 4
-// rows 11.4 and 8.9.
+// for one CTA): at 64 rows of 1024 tokens of 4 heads of 128 whole rows take 18.8 us and split ones 24.6, at 4 rows of
+// 1000 11.7 and 9.0. The estimate is of full tables: 32 rows of 500 tokens in tables of 4096 are split (13.1 us, whole
+// 8.5), and 64 rows of 1 to 8192 tokens, most of them short, in tables of 8192 are whole (69 us, split 25).
 constexpr double kAllRate = 6e6, kOneRate = 3.6e4, kJoinUs = 3.3;  // bytes per us
 
 AttendPlan attend_plan(int B, int S, int Hq, int Hkv, int D, int page_size, int max_pages, int sms) {

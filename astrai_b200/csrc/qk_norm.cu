@@ -353,8 +353,10 @@ __global__ void __launch_bounds__(384, 2) qk_norm_fwd_kernel(const QkNormParams 
 // depend on registers or occupancy; the other warps take their heads of each row out of it. CTA c has the
 // chunks c, c + grid, ... In the backward the sums of g u stay in registers and go to the CTA's own row of dw_part,
 // so the result does not depend on any order in time.
-// Bound by instructions (105 per two heads forward, 190 backward) and, forward, nearly by HBM: 8192 rows of 20 heads
-// of 128 in bfloat16 take 15.5 us forward (84 MB, 0.83 of the copy rate) and 29 us backward (126 MB, 0.66).
+// Forward nearly bound by HBM, backward by latency: 8192 rows of 20 heads of 128 in bfloat16 take 15.5 us forward (84
+// MB, 0.83 of the copy rate) and 29 us backward (126 MB, 0.66), where 30 % of the warps an SM can hold issue in 54 %
+// of its slots, waiting for the instruction before (105 per two heads forward, 190 backward), for the two sums over
+// a head's lanes and for shared memory.
 constexpr int kStages = 4;
 // consumer warps of a CTA at most: 10 leave the backward of 16-bit types enough registers not to spill (33.7 -> 30 us at
 // 8192 rows of 20 heads of 128), 4-byte rows are so wide that often only one is in a chunk and all warps share it

@@ -45,9 +45,11 @@ _MASK64 = 0xFFFFFFFFFFFFFFFF
 HEAD_DIM = 128
 KERNEL_HEAD_DIMS = (64, 128)  # head sizes the cache kernels (write, gather, decode) support
 # Query rows of a KV head (new tokens x query heads per KV head) up to which new tokens attend over an int8 cache in
-# place; past that its values are gathered for the prefill kernel. Measured on B200, 16 / 4 heads of 128: 8 rows of
-# 2048 tokens with 16 new ones each 20.8 us in place and 45.2 gathered, with 32 new ones 48.9 and 45.2; 8 rows of 8192
-# with 32 new ones 118.9 and 162.5; 1 row of 8192 with 128 new ones 64 and 128.
+# place; past that its values are gathered for the prefill kernel, so that a long prompt reads the cache once and not
+# once for every 16 query rows. Measured on B200, 16 / 4 heads of 128, in place and gathered: 8 rows of 2048 tokens with
+# 16 new ones each 22.9 and 45.6 us, with 32 new ones 51.5 and 46.2; 8 rows of 8192 with 32 new ones 137 and 164; 1 row
+# of 2048 with 128 new ones 22.8 and 38.2, 1 row of 8192 72 and 128. Where both are near each other depends on the batch
+# and the lengths as well: the second of these is 11 % slower in place, and single rows would gain in place past it.
 INT8_ROWS = 128
 
 
