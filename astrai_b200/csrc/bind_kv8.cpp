@@ -1,11 +1,11 @@
 // Python bindings of the 8-bit paged KV cache kernels (kv8.cu): every tensor check is here.
-#include <ATen/cuda/CUDAContext.h>
-#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
 #include <cuda_runtime.h>
+
+#include "bind_util.h"
 
 namespace astrai_host {
 bool kv8_block_supported(int block);
@@ -24,13 +24,7 @@ void kv8_attend(const void* q, const long long* qs, const void* kc, const void* 
 
 namespace {
 
-using OptTensor = c10::optional<at::Tensor>;
-
-// Uninitialised memory straight from the caching allocator: a call of a few microseconds feels the dispatcher's share
-// of at::empty.
-at::Tensor new_like(const at::Tensor& t, at::IntArrayRef sizes, at::ScalarType dtype) {
-  return at::Tensor(at::detail::empty_cuda(sizes, dtype, t.device(), c10::nullopt));
-}
+using namespace astrai_bind;
 
 // Numbers enter messages as text made here: a build whose compiler links its own static libstdc++ must not
 // stream them through the locale of the one that torch loaded.
@@ -62,7 +56,7 @@ Cache check_cache(const at::Tensor& kc, const at::Tensor& vc, const at::Tensor& 
   TORCH_CHECK(astrai_host::kv8_block_supported((int)block), "kv8: block must be 16, 32, 64 or 128 tokens, got ", text(block));
   TORCH_CHECK(kc.size(0) < (1LL << 31) && kc.size(1) < 65536 && kc.size(2) < (1LL << 30), "kv8: cache too large");
   for (const auto* t : {&kc, &vc})
-    TORCH_CHECK(reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0, "kv8: the caches must be 16-byte aligned");
+    TORCH_CHECK(on_grid(*t), "kv8: the caches must be 16-byte aligned");
   return {(int)kc.size(0), (int)kc.size(1), (int)kc.size(2), (int)kc.size(3), (int)block};
 }
 
@@ -91,7 +85,7 @@ int dtype_code(const at::Tensor& t, const char* name) {
 // copied if it is not (contiguous() would return a contiguous tensor as it is, wherever it starts)
 at::Tensor heads_of(const at::Tensor& t) {
   if (t.dim() != 4) return t;  // refused by check_heads
-  bool ok = t.stride(3) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
+  bool ok = t.stride(3) == 1 && on_grid(t);
   for (int i = 0; i < 3; ++i) ok = ok && (t.size(i) <= 1 || t.stride(i) % 8 == 0);
   return ok ? t : t.clone(at::MemoryFormat::Contiguous);
 }
@@ -103,15 +97,13 @@ at::Tensor int32_of(const at::Tensor& t) {
 void check_heads(const at::Tensor& t, const at::Tensor& like, const char* name, long long* strides) {
   TORCH_CHECK(t.is_cuda() && t.device() == like.device() && t.dim() == 4, "kv8: ", name,
               " must be a CUDA [batch, tokens, heads, head_dim] tensor on the cache's device");
-  TORCH_CHECK(t.stride(3) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0, "kv8: ", name,
+  TORCH_CHECK(t.stride(3) == 1 && on_grid(t), "kv8: ", name,
               " needs a contiguous last dimension and a 16-byte aligned start");
   for (int i = 0; i < 3; ++i) {
     TORCH_CHECK(t.size(i) <= 1 || t.stride(i) % 8 == 0, "kv8: ", name, " rows must be 16-byte aligned");
     strides[i] = t.stride(i);
   }
 }
-
-cudaStream_t stream() { return at::cuda::getCurrentCUDAStream().stream(); }
 
 void kv8_append(const at::Tensor& k_in, const at::Tensor& v_in, at::Tensor& kc, at::Tensor& vc, at::Tensor& ka,
                 at::Tensor& va, const at::Tensor& table_in, const at::Tensor& starts_in, const at::Tensor& lens_in) {
@@ -150,7 +142,7 @@ std::pair<at::Tensor, at::Tensor> kv8_gather(const at::Tensor& kc, const at::Ten
   const int mp = check_table(table, kc, B, c);
   at::Tensor starts;
   const int* st = nullptr;
-  if (starts_in.has_value() && starts_in->defined()) {
+  if (given(starts_in)) {
     starts = int32_of(*starts_in);
     st = check_i32(starts, kc, B, "starts");
   }
@@ -193,7 +185,7 @@ at::Tensor kv8_attend(const at::Tensor& q_in, const at::Tensor& kc, const at::Te
   const int* ln = check_i32(lens, kc, B, "lens");
   at::Tensor starts;
   const int* st = nullptr;
-  if (starts_in.has_value() && starts_in->defined()) {
+  if (given(starts_in)) {
     starts = int32_of(*starts_in);
     st = check_i32(starts, kc, B, "starts");
   }
@@ -207,10 +199,10 @@ at::Tensor kv8_attend(const at::Tensor& q_in, const at::Tensor& kc, const at::Te
   at::Tensor ws;
   float* wp = nullptr;
   if (need > 0) {
-    if (workspace.has_value() && workspace->defined()) {
+    if (given(workspace)) {
       ws = *workspace;
       TORCH_CHECK(ws.device() == q.device() && ws.scalar_type() == at::kFloat && ws.is_contiguous() && ws.numel() >= need &&
-                      reinterpret_cast<uintptr_t>(ws.data_ptr()) % 16 == 0,
+                      on_grid(ws),
                   "kv8_attention: workspace must be contiguous fp32 of at least ", text(need), " elements");
     } else {
       ws = new_like(q, {need}, at::kFloat);

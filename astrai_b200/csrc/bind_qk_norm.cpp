@@ -1,6 +1,4 @@
 // Python bindings of the per-head norm + rotation kernels (qk_norm.cu): every tensor check is here.
-#include <ATen/cuda/CUDAContext.h>
-#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/function.h>
@@ -9,6 +7,8 @@
 #include <torch/extension.h>
 
 #include <cuda_runtime.h>
+
+#include "bind_util.h"
 
 namespace astrai_host {
 void qk_norm_fwd(const void* x, long long ldx, void* y, long long ldy, int rows, int hq, int hkv, int D,
@@ -24,15 +24,7 @@ void qk_norm_bwd(const void* dy, long long lddy, const void* x, long long ldx, v
 
 namespace {
 
-using OptTensor = c10::optional<at::Tensor>;
-
-bool given(const OptTensor& t) { return t.has_value() && t->defined(); }
-
-// Uninitialised memory straight from the caching allocator: a call of a few microseconds feels the dispatcher's share
-// of at::empty.
-at::Tensor new_like(const at::Tensor& t, at::IntArrayRef sizes, at::ScalarType dtype) {
-  return at::Tensor(at::detail::empty_cuda(sizes, dtype, t.device(), c10::nullopt));
-}
+using namespace astrai_bind;
 
 int dtype_code(const at::Tensor& t) {
   switch (t.scalar_type()) {
@@ -44,7 +36,6 @@ int dtype_code(const at::Tensor& t) {
   return -1;
 }
 
-bool on_grid(const at::Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
 bool rows_on_grid(const at::Tensor& t) {
   return t.stride(1) == 1 && (t.size(0) <= 1 || (t.stride(0) * t.element_size()) % 16 == 0) && on_grid(t);
 }
@@ -117,8 +108,6 @@ struct Options {
   bool half_layout;
   double eps;
 };
-
-cudaStream_t stream() { return at::cuda::getCurrentCUDAStream().stream(); }
 
 // y may be x itself
 void forward_into(const at::Tensor& x, const at::Tensor& y, const at::Tensor& table, const OptTensor& pos,
