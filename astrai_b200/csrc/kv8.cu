@@ -289,8 +289,8 @@ constexpr int kPad = 4;                  // units that a segment's start weighs 
 constexpr int kMaxBatch = 1024;        // rows of a launch
 // Running maxima start here: below every score, and finite, so that no difference of maxima is NaN.
 constexpr float kNone = -1.7e38f;
-// A running maximum follows the scores only when they pass it by this much (powers of two): weights then
-// reach 2^8, far inside fp16, and most tiles need no reduction over lanes and no rescaling.
+// A running maximum follows the scores only when they pass it by this much (powers of two): most tiles then need no
+// reduction over lanes and no rescaling.
 constexpr float kSlack = 8.f;
 // The weights' reference stays this far below their largest, which is then 2^kLift to 2^(kLift + kSlack) as fp16, half
 // its range: a weight of 2^-32 of the largest still reaches its last place.
@@ -403,8 +403,8 @@ struct Piece {       // of a segment, on one CTA
 //
 // Softmax per query row: a reference m near the maximum of the scores s (within kSlack) and
 // l = sum 2^(s - m). The weights of the integers v are 2^s * absmax_v; they have a reference M of their
-// own near the maximum of s + log2 absmax_v, so as fp16 they keep their precision whatever the
-// magnitudes of the blocks. out = sum w v / l * 2^(M - m) / 127.
+// own, kLift below the maximum of s + log2 absmax_v (within kSlack), so as fp16 they keep their precision whatever
+// the magnitudes of the blocks. out = sum w v / l * 2^(M - m) / 127.
 //
 // Bound by HBM on long rows (4 x 131072 tokens of 4 heads of 128: 94 us, 0.88 of the copy rate), by its start (1.7 us
 // to the first copy), merge (2 us) and join (3 us) on short ones (32 x 4096: 31.9 us, 0.65). Two CTAs of 8 warps per
