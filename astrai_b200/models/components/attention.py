@@ -164,14 +164,15 @@ class GQA(nn.Module):
         B, S, _ = x.shape
         Hq, Hkv, D = self.n_heads, self.n_kv_heads, self.head_dim
         rotary = self.rotary(ctx)
+        positions = None if ctx.positions is None else ctx.positions.expand(B, S)  # one row may stand for the batch
         qkv = self.qkv_proj(x).reshape(B * S, (Hq + 2 * Hkv) * D)
         if ctx.cache is None and ctx.dense_mask is None:
-            o = attention_qk_norm(qkv, rotary, B, S, Hq, Hkv, ctx.positions, ctx.causal, ctx.seg)
+            o = attention_qk_norm(qkv, rotary, B, S, Hq, Hkv, positions, ctx.causal, ctx.seg)
         elif ctx.cache is not None and getattr(ctx.cache, "supports_qkv", False) and x.is_cuda \
                 and x.dtype == torch.bfloat16:
             o = ctx.cache.attend_qkv(self.layer_id, qkv, B, S, Hq, Hkv, ctx.table, rotary=rotary)
         else:
-            qk = rotary.apply(qkv, Hq, Hkv, D, positions=ctx.positions, seq_len=S).view(B, S, Hq + Hkv, D)
+            qk = rotary.apply(qkv, Hq, Hkv, D, positions=positions, seq_len=S).view(B, S, Hq + Hkv, D)
             q, k, v = qk[:, :, :Hq], qk[:, :, Hq:], qkv.view(B, S, Hq + 2 * Hkv, D)[:, :, Hq + Hkv:]
             if ctx.cache is not None:
                 o = ctx.cache.attend(self.layer_id, q, k, v)

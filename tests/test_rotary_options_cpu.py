@@ -45,3 +45,21 @@ def test_mla_takes_defaults_and_scaled_tables():
     m = _mla(rope_scaling_method="linear", rope_scaling=dict(factor=2.0))
     plain = _mla()
     assert torch.allclose(m.rotary_embedding.table()[2], plain.rotary_embedding.table()[1], atol=1e-6)
+
+
+@pytest.mark.parametrize("shape", [(1, 9), (3, 9)])
+def test_one_pass_takes_the_positions_that_the_separate_path_takes(shape):
+    """One row of positions for the whole batch."""
+    def model(**kw):
+        torch.manual_seed(0)
+        return AutoRegressiveLM(AutoRegressiveLMConfig(
+            vocab_size=50, hidden_size=64, num_hidden_layers=2, rms_norm_eps=1e-5, intermediate_size=64,
+            tie_word_embeddings=False, max_position_embeddings=64, rope_theta=1e4, num_attention_heads=4,
+            num_key_value_heads=2, use_qk_norm=True, **kw)).eval()
+
+    ids = torch.arange(27).view(3, 9)
+    pos = (torch.arange(9) + 4).expand(*shape)
+    mask = torch.ones(3, 9, 9, dtype=torch.bool).tril()
+    for kw in ({}, dict(input_mask=mask)):
+        a, b = (model(fused_qk_norm=f)(ids, position_ids=pos, **kw)["logits"] for f in (False, True))
+        assert torch.allclose(a, b, atol=1e-5)
