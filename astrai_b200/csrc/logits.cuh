@@ -1,0 +1,139 @@
+// Rows of logits as 16-byte vectors: what the kernels over [rows, vocab] share.
+//
+// A row may start at any element. Its vectors lie on the 16-byte grid of memory: vector i holds the row's elements
+// i * E - head .. i * E - head + E - 1 (E elements in 16 bytes, head the elements between the grid and the row's start),
+// so that every vector but the first and the last is one aligned access; those two are read and written by element.
+#pragma once
+#include <cuda_fp16.h>
+
+#include "common.cuh"
+
+namespace astrai {
+
+template <typename T>
+struct LogitType;
+template <>
+struct LogitType<__nv_bfloat16> {
+  static constexpr int E = 8;
+  static constexpr uint32_t kNegInf = 0xFF80u;
+  __device__ static float one(__nv_bfloat16 v) { return __bfloat162float(v); }
+  __device__ static __nv_bfloat16 round(float v) { return __float2bfloat16_rn(v); }
+  __device__ static float2 pair(uint32_t u) { return unpack_bf16(u); }
+  __device__ static uint32_t pack(float a, float b) { return pack_bf16(a, b); }
+};
+template <>
+struct LogitType<__half> {
+  static constexpr int E = 8;
+  static constexpr uint32_t kNegInf = 0xFC00u;
+  __device__ static float one(__half v) { return __half2float(v); }
+  __device__ static __half round(float v) { return __float2half_rn(v); }
+  __device__ static float2 pair(uint32_t u) { return __half22float2(*reinterpret_cast<const __half2*>(&u)); }
+  __device__ static uint32_t pack(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+};
+template <>
+struct LogitType<float> {
+  static constexpr int E = 4;
+  static constexpr uint32_t kNegInf = 0xFF800000u;
+  __device__ static float one(float v) { return v; }
+  __device__ static float round(float v) { return v; }
+};
+
+// The E elements of a vector as floats.
+template <typename T>
+__device__ __forceinline__ void vec_floats(const uint4& u, float (&f)[LogitType<T>::E]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if constexpr (LogitType<T>::E == 4) {
+      f[j] = __uint_as_float(w[j]);
+    } else {
+      const float2 p = LogitType<T>::pair(w[j]);
+      f[2 * j] = p.x;
+      f[2 * j + 1] = p.y;
+    }
+  }
+}
+
+template <typename T>
+__device__ __forceinline__ uint4 vec_round(const float (&f)[LogitType<T>::E]) {
+  uint32_t w[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if constexpr (LogitType<T>::E == 4)
+      w[j] = __float_as_uint(f[j]);
+    else
+      w[j] = LogitType<T>::pack(f[2 * j], f[2 * j + 1]);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+template <typename T>
+__device__ __forceinline__ uint4 vec_neg_inf() {
+  const uint32_t w = LogitType<T>::E == 4 ? LogitType<T>::kNegInf : LogitType<T>::kNegInf * 0x10001u;
+  return make_uint4(w, w, w, w);
+}
+
+// Elements of `u` whose bit of `bits` is set become -inf.
+template <typename T>
+__device__ __forceinline__ void vec_mask(uint4& u, uint32_t bits) {
+  uint32_t* const w[4] = {&u.x, &u.y, &u.z, &u.w};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if constexpr (LogitType<T>::E == 4) {
+      if (bits >> j & 1) *w[j] = LogitType<T>::kNegInf;
+    } else {
+      if (bits >> (2 * j) & 1) *w[j] = (*w[j] & 0xFFFF0000u) | LogitType<T>::kNegInf;
+      if (bits >> (2 * j + 1) & 1) *w[j] = (*w[j] & 0x0000FFFFu) | (LogitType<T>::kNegInf << 16);
+    }
+  }
+}
+
+// The vectors of one row.
+template <typename T>
+struct RowVecs {
+  static constexpr int E = LogitType<T>::E;
+  const T* row;
+  int V, head, n;  // elements, elements before the row on the 16-byte grid, vectors
+  __device__ RowVecs(const T* x, int vocab) : row(x), V(vocab) {
+    head = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
+    n = (V + head + E - 1) / E;
+  }
+  __device__ int first(int vec) const { return vec * E - head; }  // its first element (negative: before the row)
+  __device__ bool whole(int vec) const { return first(vec) >= 0 && first(vec) + E <= V; }
+  // Elements outside the row read as -inf.
+  __device__ uint4 load(int vec) const {
+    const int at = first(vec);
+    if (at >= 0 && at + E <= V) return __ldg(reinterpret_cast<const uint4*>(row + at));
+    return load_edge(at);
+  }
+  __device__ __noinline__ uint4 load_edge(int at) const {
+    float f[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) f[e] = at + e >= 0 && at + e < V ? LogitType<T>::one(row[at + e]) : -INFINITY;
+    return vec_round<T>(f);
+  }
+  // `out` is a row with the same head.
+  __device__ void store(T* out, int vec, const uint4& u) const {
+    const int at = first(vec);
+    if (at >= 0 && at + E <= V) {
+      *reinterpret_cast<uint4*>(out + at) = u;
+    } else {
+      float f[E];
+      vec_floats<T>(u, f);
+#pragma unroll
+      for (int e = 0; e < E; ++e)
+        if (at + e >= 0 && at + e < V) out[at + e] = LogitType<T>::round(f[e]);
+    }
+  }
+};
+
+__device__ __forceinline__ float exp2_fast(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+}  // namespace astrai
