@@ -1,4 +1,4 @@
-// Python bindings of the kernels over rows of logits (distill.cu): every tensor check is here.
+// Python bindings of the kernels over rows of logits (distill.cu, top_logits.cu): every tensor check is here.
 #include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/function.h>
@@ -8,6 +8,7 @@
 
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 
 #include "bind_util.h"
@@ -19,6 +20,10 @@ void distill(const void* x, long long ldx, void* dx, long long lddx, const void*
              int values_type, const float* rest, const long long* target, long long ignore, int rows, int V, int K,
              float tau, float hard, const float* grad, float expected, bool unless_expected, float* row_loss,
              float* count, bool have_count, float* loss, int dtype, cudaStream_t s);
+int top_logits_max_k();
+int top_logits_max_vocab(int elem);
+void top_logits(const void* x, long long ldx, int rows, int V, int k, float tau, int* ids, void* values, float* rest,
+                int dtype, cudaStream_t s);
 }  // namespace astrai_host
 
 namespace {
@@ -49,6 +54,39 @@ at::Tensor rows_of(const at::Tensor& t) {
   return r.stride(1) == 1 || r.size(1) == 1 ? r : r.contiguous();
 }
 long long row_stride(const at::Tensor& t) { return t.size(0) > 1 ? t.stride(0) : t.size(1); }
+
+// ------------------------------------------------------------------------------------------ top logits
+std::tuple<at::Tensor, at::Tensor, at::Tensor> top_logits(const at::Tensor& logits, int64_t k, double tau) {
+  TORCH_CHECK_VALUE(logits.dim() >= 1 && logits.size(-1) >= 1, "top_logits: logits must be [..., vocab]");
+  const int64_t V = logits.size(-1);
+  TORCH_CHECK_VALUE(k >= 1 && k <= V && k <= astrai_host::top_logits_max_k(), "top_logits: k must be in 1 .. ",
+                    std::to_string(std::min<int64_t>(V, astrai_host::top_logits_max_k())), ", got ", std::to_string(k));
+  TORCH_CHECK_VALUE(tau > 0. && std::isfinite(tau), "top_logits: temperature must be positive");
+  const int code = dtype_code(logits, "top_logits: logits");
+  TORCH_CHECK_VALUE(V <= astrai_host::top_logits_max_vocab((int)logits.element_size()), "top_logits: a vocabulary of ",
+                    std::to_string(V), " is too large for this type");
+  no_tangent(logits, "top_logits");
+  TORCH_CHECK(!(at::GradMode::is_enabled() && logits.requires_grad()), "top_logits has no gradient: call it under no_grad");
+  const c10::cuda::CUDAGuard guard(logits.device());
+  const at::Tensor x = rows_of(logits);
+  const int64_t rows = x.size(0);
+  TORCH_CHECK_VALUE(rows < (1LL << 27), "top_logits: too many rows");
+  auto lead = logits.sizes().vec();
+  lead.pop_back();
+  auto ids = new_like(x, {rows, k}, at::kInt), values = new_like(x, {rows, k}, x.scalar_type()),
+       rest = new_like(x, {rows}, at::kFloat);
+  if (rows > 0) {
+    astrai_host::top_logits(x.data_ptr(), row_stride(x), (int)rows, (int)V, (int)k, (float)tau, ids.data_ptr<int>(),
+                            values.data_ptr(), rest.data_ptr<float>(), code, stream());
+    C10_CUDA_KERNEL_LAUNCH_CHECK();
+  }
+  if (logits.dim() != 2) {
+    rest = rest.view(lead);
+    lead.push_back(k);
+    ids = ids.view(lead), values = values.view(lead);
+  }
+  return {ids, values, rest};
+}
 
 // ------------------------------------------------------------------------------------------ distillation
 struct Distill {
@@ -189,6 +227,7 @@ at::Tensor distill_loss(const at::Tensor& logits, const at::Tensor& ids_in, cons
 
 void register_logits(pybind11::module& m) {
   namespace py = pybind11;
+  m.def("top_logits", &top_logits, py::arg("logits"), py::arg("k"), py::arg("temperature"));
   m.def("distill_loss", &distill_loss, py::arg("logits"), py::arg("ids"), py::arg("values"), py::arg("rest"),
         py::arg("temperature"), py::arg("target"), py::arg("hard_weight"), py::arg("ignore_index"),
         py::arg("expected_grad"));

@@ -92,17 +92,17 @@ __device__ __forceinline__ float teacher_value(const DistillArgs& a, long long i
 // a finite reference for a maximum
 __device__ __forceinline__ float ref_of(float m) { return m == -INFINITY ? 0.f : m; }
 
-// The student's mass at one temperature: outside J and on J as sums of 2^(x c - off), joined. With d = offset of J - offset
-// outside and m = max(d, 0), `sum` is all of it relative to the offset outside + m, so that neither part overflows.
+// The student's mass at one temperature: outside J and on J as sums of 2^((x - ref) c), joined. With d = (J's reference -
+// that outside) c and m = max(d, 0), `sum` is all of it relative to 2^m at the reference outside: neither part overflows.
 struct Mass {
   float outside, d, m, sum;
   __device__ Mass(float outside_, float on, float d_) : outside(outside_), d(d_), m(fmaxf(d_, 0.f)) {
     sum = outside * exp2_fast(-m) + on * exp2_fast(d - m);
   }
   __device__ float log2_all_over_outside() const { return m + log2f(sum) - log2f(outside); }  // -log2 q_0
-  __device__ float log2_rel_outside() const { return m + log2f(sum); }  // of all of it, relative to each offset
+  __device__ float log2_rel_outside() const { return m + log2f(sum); }  // of all of it, relative to each reference
   __device__ float log2_rel_on() const { return m - d + log2f(sum); }
-  __device__ float inv_rel_outside() const { return exp2_fast(-m) / sum; }  // 1 / all of it, relative to each offset
+  __device__ float inv_rel_outside() const { return exp2_fast(-m) / sum; }  // 1 / all of it, relative to each reference
   __device__ float inv_rel_on() const { return exp2_fast(d - m) / sum; }
 };
 
@@ -218,21 +218,29 @@ __global__ void __launch_bounds__(DST_THREADS, 2) distill_kernel(const DistillAr
       if constexpr (TWO) sum[3] += exp2_fast((xj[i] - mj) * LOG2E);
     }
   }
-  float mo = mr, off = mo * c, off1 = mo * LOG2E;  // the logit that the sums outside J are relative to, its exponents
+  float mo = mr;  // the logit that the sums outside J are relative to
+  const Pair c2(c, c), log2e2(LOG2E, LOG2E);
+  {
+    const Pair ref2(-mo, -mo);
+    Pair s2(0.f, 0.f), s1(0.f, 0.f);
 #pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    float f[E];
-    vec_floats<T>(u[i], f);
+    for (int i = 0; i < NV; ++i) {
+      Pair p[E / 2];
+      vec_pairs<T>(u[i], p);
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      sum[4] += exp2_fast(fmaf(f[e], c, -off));
-      if constexpr (TWO) sum[5] += exp2_fast(fmaf(f[e], LOG2E, -off1));
+      for (int e = 0; e < E / 2; ++e) {
+        const Pair d = p[e] + ref2;
+        s2 = s2 + exp2_fast(d * c2);
+        if constexpr (TWO) s1 = s1 + exp2_fast(d * log2e2);
+      }
     }
+    sum[4] = s2.sum();
+    if constexpr (TWO) sum[5] = s1.sum();
   }
   block_reduce<6, false>(sum, part_sum);
 
   float on = sum[2], on1 = sum[3], out = sum[4], out1 = sum[5];
-  if (cs > 1) {  // the sums of all CTAs, those outside J relative to this one's offset
+  if (cs > 1) {  // the sums of all CTAs, those outside J relative to this one's reference
     cg::cluster_group cl = cg::this_cluster();
     if (t == 0) {
       mine[0] = mx[2];
@@ -245,22 +253,17 @@ __global__ void __launch_bounds__(DST_THREADS, 2) distill_kernel(const DistillAr
     const int lane = t & 31;
     const float* theirs = cl.map_shared_rank(mine, lane < cs ? lane : 0);
     const float m = lane < cs ? theirs[0] : -INFINITY;
-    if (mx[2] == -INFINITY) {  // none of its own: any offset that others have
-      mo = ref_of(warp_max(m));
-      off = mo * c;
-      off1 = mo * LOG2E;
-    }
+    if (mx[2] == -INFINITY) mo = ref_of(warp_max(m));  // none of its own: one that others have
     const bool some = m != -INFINITY;
-    out = warp_sum(some ? theirs[1] * exp2_fast(m * c - off) : 0.f);
-    if constexpr (TWO) out1 = warp_sum(some ? theirs[2] * exp2_fast(m * LOG2E - off1) : 0.f);
+    out = warp_sum(some ? theirs[1] * exp2_fast((m - mo) * c) : 0.f);
+    if constexpr (TWO) out1 = warp_sum(some ? theirs[2] * exp2_fast((m - mo) * LOG2E) : 0.f);
     on = warp_sum(lane < cs ? theirs[3] : 0.f);
     if constexpr (TWO) on1 = warp_sum(lane < cs ? theirs[4] : 0.f);
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   }
-  const float offj = mj * c, offj1 = mj * LOG2E;
-  if (out == 0.f) mo = mj, off = offj, off1 = offj1;  // nothing outside J
-  const Mass z(out, on, on == 0.f ? -INFINITY : offj - off);
-  const Mass z1(TWO ? out1 : out, TWO ? on1 : on, on == 0.f ? -INFINITY : (TWO ? offj1 - off1 : offj - off));
+  if (out == 0.f) mo = mj;  // nothing outside J
+  const Mass z(out, on, on == 0.f ? -INFINITY : (mj - mo) * c);
+  const Mass z1(TWO ? out1 : out, TWO ? on1 : on, on == 0.f ? -INFINITY : (mj - mo) * (TWO ? LOG2E : c));
   // the teacher's share outside J
   const float pr = rest == -INFINITY ? 0.f : exp2_fast((rest - mt) * LOG2E);
   const float mass = sum[0] + pr, inv = mass != 0.f ? 1.f / mass : 0.f;
@@ -285,20 +288,22 @@ __global__ void __launch_bounds__(DST_THREADS, 2) distill_kernel(const DistillAr
     const float share = out != 0.f ? p0 / out : 0.f;
     const float base = kl * (all * z.inv_rel_outside() - share) + (TWO ? 0.f : ce * z.inv_rel_outside());
     const float base1 = TWO ? ce * z1.inv_rel_outside() : 0.f;
-    const auto outside = [&](float f) {
-      float d = base * exp2_fast(fmaf(f, c, -off));
-      if constexpr (TWO) d = fmaf(base1, exp2_fast(fmaf(f, LOG2E, -off1)), d);
+    const Pair ref2(-mo, -mo), base2(base, base), base12(base1, base1);
+    const auto outside = [&](Pair p) {
+      p = p + ref2;
+      const Pair d = base2 * exp2_fast(p * c2);
+      if constexpr (TWO) return fma2(base12, exp2_fast(p * log2e2), d);
       return d;
     };
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
       const int v = v0 + t + i * DST_THREADS;
       if (v >= v1) break;
-      float f[E];
-      vec_floats<T>(u[i], f);
+      Pair p[E / 2];
+      vec_pairs<T>(u[i], p);
 #pragma unroll
-      for (int e = 0; e < E; ++e) f[e] = outside(f[e]);
-      vecs.store(dx, v, vec_round<T>(f));
+      for (int e = 0; e < E / 2; ++e) p[e] = outside(p[e]);
+      vecs.store(dx, v, pairs_round<T>(p));
     }
     __syncthreads();  // the base gradient lies before the entries' gradients
 #pragma unroll 1
@@ -311,13 +316,13 @@ __global__ void __launch_bounds__(DST_THREADS, 2) distill_kernel(const DistillAr
           if (id_at(l) == id[i])
             p += exp2_fast((teacher_value(a, (long long)row * a.K + l) * a.inv_tau - mt) * LOG2E) * inv;
       }
-      const float q = exp2_fast(fmaf(xj[i], c, -offj)) * z.inv_rel_on();
-      const float q1 = TWO ? exp2_fast(fmaf(xj[i], LOG2E, -offj1)) * z1.inv_rel_on() : q;
+      const float q = exp2_fast((xj[i] - mj) * c) * z.inv_rel_on();
+      const float q1 = TWO ? exp2_fast((xj[i] - mj) * LOG2E) * z1.inv_rel_on() : q;
       dx[id[i]] = LogitType<T>::round(kl * (q * all - p) + ce * (q1 - (id[i] == y ? 1.f : 0.f)));
     }
     if (t == 0 && y >= 0 && ce != 0.f) {
       const int v = ((int)y + vecs.head) / E, bit = ((int)y + vecs.head) % E;
-      if (v >= v0 && v < v1 && !(mask[v - v0] >> bit & 1)) dx[y] = LogitType<T>::round(outside(xy) - ce);
+      if (v >= v0 && v < v1 && !(mask[v - v0] >> bit & 1)) dx[y] = LogitType<T>::round(outside(Pair(xy, xy)).get().x - ce);
     }
   }
   if (cs > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // others may still read `mine`

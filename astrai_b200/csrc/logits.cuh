@@ -136,4 +136,65 @@ __device__ __forceinline__ float exp2_fast(float x) {
   return y;
 }
 
+// Two floats in one register pair: one instruction works on both.
+struct Pair {
+  unsigned long long v;
+  __device__ Pair() = default;
+  __device__ Pair(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+  __device__ explicit Pair(float2 f) : Pair(f.x, f.y) {}
+  __device__ float2 get() const {
+    float2 f;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+    return f;
+  }
+  __device__ float sum() const {
+    const float2 f = get();
+    return f.x + f.y;
+  }
+};
+__device__ __forceinline__ Pair operator+(Pair a, Pair b) {
+  Pair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Pair operator*(Pair a, Pair b) {
+  Pair r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+  Pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+__device__ __forceinline__ Pair exp2_fast(Pair p) {
+  const float2 f = p.get();
+  return Pair(exp2_fast(f.x), exp2_fast(f.y));
+}
+
+// The E elements of a vector as pairs.
+template <typename T>
+__device__ __forceinline__ void vec_pairs(const uint4& u, Pair (&p)[LogitType<T>::E / 2]) {
+  if constexpr (LogitType<T>::E == 4) {
+    p[0] = Pair(__uint_as_float(u.x), __uint_as_float(u.y));
+    p[1] = Pair(__uint_as_float(u.z), __uint_as_float(u.w));
+  } else {
+    p[0] = Pair(LogitType<T>::pair(u.x));
+    p[1] = Pair(LogitType<T>::pair(u.y));
+    p[2] = Pair(LogitType<T>::pair(u.z));
+    p[3] = Pair(LogitType<T>::pair(u.w));
+  }
+}
+template <typename T>
+__device__ __forceinline__ uint4 pairs_round(const Pair (&p)[LogitType<T>::E / 2]) {
+  float f[LogitType<T>::E];
+#pragma unroll
+  for (int j = 0; j < LogitType<T>::E / 2; ++j) {
+    const float2 g = p[j].get();
+    f[2 * j] = g.x;
+    f[2 * j + 1] = g.y;
+  }
+  return vec_round<T>(f);
+}
+
 }  // namespace astrai

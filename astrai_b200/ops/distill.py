@@ -1,14 +1,15 @@
-"""Distillation from a teacher's top logits: the loss of a student's logits and their gradient.
+"""Distillation from a teacher's top logits: taking them, and the loss of a student's logits with their gradient.
 
 The reference trains on hard labels, preferences and rewards (astrai/trainer/strategy.py) and has no distillation. Here
 a teacher is given as :class:`TopLogits`: for each position the ids and logits of its most likely tokens and, if wanted,
 the log-sum-exp of all its other logits, a few hundred bytes where its whole row takes ``vocab`` numbers.
 
+* :func:`top_logits`   a teacher's rows of logits as :class:`TopLogits`
 * :func:`distill_loss` the mean over positions of ``(1 - hard_weight) * temperature**2 * KL(teacher | student)``
   ``+ hard_weight * cross_entropy(target)``
 
-On CUDA the kernels of ``csrc/distill.cu`` run (bfloat16, float16 and float32 logits): the logits are read once, and the
-same pass writes their gradient. CPU tensors take the plain PyTorch functions below.
+On CUDA the kernels of ``csrc/distill.cu`` and ``csrc/top_logits.cu`` run (bfloat16, float16 and float32 logits): the
+logits are read once, and the loss writes their gradient in the same pass. CPU tensors take the plain PyTorch functions below.
 """
 
 from __future__ import annotations
@@ -27,6 +28,26 @@ class TopLogits(NamedTuple):
     ids: torch.Tensor                     # int32 or int64 [..., k]; an id outside the vocabulary: no entry
     values: torch.Tensor                  # their logits [..., k], bfloat16, float16 or float32
     rest: Optional[torch.Tensor] = None   # fp32 [...]: log sum exp(logit / temperature) over all other tokens
+
+
+# ----------------------------------------------------------------------------- the teacher's side
+def top_logits(logits: torch.Tensor, k: int, temperature: float = 1.0) -> TopLogits:
+    """The ``k`` (at most 256) largest of each row of ``logits [..., vocab]`` in descending order, of equal ones the
+    lowest id first, and ``rest``: log sum exp(logit / temperature) over all others (-inf where there are none).
+
+    A NaN counts as larger than every number. There is no gradient: under grad mode logits that require one are refused.
+    """
+    if logits.is_cuda:
+        return TopLogits(*native().top_logits(logits, int(k), float(temperature)))
+    if logits.dim() < 1 or not 1 <= k <= min(256, logits.shape[-1]):
+        raise ValueError(f"top_logits: k must be in 1 .. min(256, vocab), got {k}")
+    if not 0 < temperature < math.inf:
+        raise ValueError("top_logits: temperature must be positive")
+    if torch.is_grad_enabled() and logits.requires_grad:
+        raise RuntimeError("top_logits has no gradient: call it under no_grad")
+    values, ids = torch.sort(logits, dim=-1, descending=True, stable=True)
+    rest = torch.logsumexp(values[..., k:].float() / temperature, -1)
+    return TopLogits(ids[..., :k].int(), values[..., :k].contiguous(), rest)
 
 
 # ----------------------------------------------------------------------------- loss

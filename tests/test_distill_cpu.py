@@ -75,3 +75,19 @@ def test_refusals():
             distill_loss(**{"logits": x, "teacher": ok, **bad})
     with pytest.raises(RuntimeError, match="gradient of the teacher"):
         distill_loss(x, TopLogits(ids, values.requires_grad_(), rest))
+
+
+def test_top_logits():
+    from astrai_b200.ops.distill import top_logits
+
+    x = torch.tensor([[1.0, 3.0, 3.0, -math.inf, 2.0], [0.0, 0.0, 0.0, 0.0, 0.0]])
+    top = top_logits(x, 2, 2.0)
+    assert top.ids.tolist() == [[1, 2], [0, 1]] and top.values.tolist() == [[3.0, 3.0], [0.0, 0.0]]
+    want = torch.tensor([math.log(math.exp(0.5) + math.exp(1.0)), math.log(3.0)])
+    assert (top.rest - want).abs().max() < 1e-6
+    assert (top_logits(x, 5).rest == -math.inf).all()
+    for k, tau in ((0, 1.0), (6, 1.0), (1, 0.0)):
+        with pytest.raises(ValueError):
+            top_logits(x, k, tau)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        top_logits(x.requires_grad_(), 2)
