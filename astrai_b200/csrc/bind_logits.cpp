@@ -1,4 +1,4 @@
-// Python bindings of the kernels over rows of logits (distill.cu, top_logits.cu): every tensor check is here.
+// Python bindings of the kernels over rows of logits (distill.cu, top_logits.cu, sample_given.cu): every tensor check is here.
 #include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/csrc/autograd/function.h>
@@ -24,6 +24,10 @@ int top_logits_max_k();
 int top_logits_max_vocab(int elem);
 void top_logits(const void* x, long long ldx, int rows, int V, int k, float tau, int* ids, void* values, float* rest,
                 int dtype, cudaStream_t s);
+int sample_given_max_vocab(int elem);
+void sample_given(const void* x, long long ldx, int rows, int V, const void* uniform, bool uniform64,
+                  const float* temperature, const int* top_k, const float* top_p, const float* min_p, long long* token,
+                  float* logprob, int dtype, cudaStream_t s);
 }  // namespace astrai_host
 
 namespace {
@@ -86,6 +90,45 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> top_logits(const at::Tensor& logi
     ids = ids.view(lead), values = values.view(lead);
   }
   return {ids, values, rest};
+}
+
+// ------------------------------------------------------------------------------------------ sampling
+std::pair<at::Tensor, OptTensor> sample_given(const at::Tensor& logits, const at::Tensor& uniform_in,
+                                              const at::Tensor& temperature_in, const at::Tensor& top_k_in,
+                                              const at::Tensor& top_p_in, const at::Tensor& min_p_in, bool logprobs) {
+  TORCH_CHECK_VALUE(logits.dim() == 2 && logits.size(1) >= 1, "sample_given: logits must be [batch, vocab]");
+  const int64_t rows = logits.size(0), V = logits.size(1);
+  const int code = dtype_code(logits, "sample_given: logits");
+  TORCH_CHECK_VALUE(V <= astrai_host::sample_given_max_vocab((int)logits.element_size()), "sample_given: a vocabulary of ",
+                    std::to_string(V), " is too large for this type");
+  TORCH_CHECK_VALUE(rows < (1LL << 27), "sample_given: too many rows");
+  TORCH_CHECK(uniform_in.scalar_type() == at::kFloat || uniform_in.scalar_type() == at::kDouble,
+              "sample_given: uniform must be float32 or float64, got ", uniform_in.scalar_type());
+  const c10::cuda::CUDAGuard guard(logits.device());
+  // one number per row, or one for all
+  const auto per_row = [&](const at::Tensor& t, at::ScalarType type, const char* name) {
+    TORCH_CHECK_VALUE(t.numel() == rows || t.numel() == 1, "sample_given: ", name, " must have one number or one per row");
+    TORCH_CHECK(t.is_cuda() && t.device() == logits.device(), "sample_given: ", name, " must be on the logits' device");
+    if (t.scalar_type() == type && t.numel() == rows && t.is_contiguous()) return t;
+    return t.to(type).reshape({-1}).expand({rows}).contiguous();
+  };
+  const at::NoGradGuard off;
+  const at::Tensor uniform = per_row(uniform_in, uniform_in.scalar_type(), "uniform"),
+                   temperature = per_row(temperature_in, at::kFloat, "temperature"),
+                   top_k = per_row(top_k_in, at::kInt, "top_k"), top_p = per_row(top_p_in, at::kFloat, "top_p"),
+                   min_p = per_row(min_p_in, at::kFloat, "min_p");
+  const at::Tensor x = rows_of(logits);
+  auto token = new_like(x, {rows}, at::kLong);
+  OptTensor logprob;
+  if (logprobs) logprob = new_like(x, {rows}, at::kFloat);
+  if (rows > 0) {
+    astrai_host::sample_given(x.data_ptr(), row_stride(x), (int)rows, (int)V, uniform.data_ptr(),
+                              uniform.scalar_type() == at::kDouble, temperature.data_ptr<float>(), top_k.data_ptr<int>(),
+                              top_p.data_ptr<float>(), min_p.data_ptr<float>(), (long long*)token.data_ptr<int64_t>(),
+                              logprobs ? logprob->data_ptr<float>() : nullptr, code, stream());
+    C10_CUDA_KERNEL_LAUNCH_CHECK();
+  }
+  return {token, logprob};
 }
 
 // ------------------------------------------------------------------------------------------ distillation
@@ -228,6 +271,8 @@ at::Tensor distill_loss(const at::Tensor& logits, const at::Tensor& ids_in, cons
 void register_logits(pybind11::module& m) {
   namespace py = pybind11;
   m.def("top_logits", &top_logits, py::arg("logits"), py::arg("k"), py::arg("temperature"));
+  m.def("sample_given", &sample_given, py::arg("logits"), py::arg("uniform"), py::arg("temperature"), py::arg("top_k"),
+        py::arg("top_p"), py::arg("min_p"), py::arg("return_logprobs"));
   m.def("distill_loss", &distill_loss, py::arg("logits"), py::arg("ids"), py::arg("values"), py::arg("rest"),
         py::arg("temperature"), py::arg("target"), py::arg("hard_weight"), py::arg("ignore_index"),
         py::arg("expected_grad"));

@@ -6,6 +6,8 @@
 #pragma once
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace astrai {
@@ -139,7 +141,7 @@ __device__ __forceinline__ float exp2_fast(float x) {
 // Two floats in one register pair: one instruction works on both.
 struct Pair {
   unsigned long long v;
-  __device__ Pair() = default;
+  Pair() = default;
   __device__ Pair(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
   __device__ explicit Pair(float2 f) : Pair(f.x, f.y) {}
   __device__ float2 get() const {
@@ -195,6 +197,35 @@ __device__ __forceinline__ uint4 pairs_round(const Pair (&p)[LogitType<T>::E / 2
     f[2 * j + 1] = g.y;
   }
   return vec_round<T>(f);
+}
+
+// Greater logits have greater keys; -0 and 0 the same one, a NaN the greatest.
+__device__ __forceinline__ uint32_t key_of(float x) {
+  if (x != x) return 0xFFFFFFFFu;
+  const uint32_t u = __float_as_uint(x + 0.f);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+__device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k); }
+
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+// largest element, NaN if there is one
+template <typename T>
+__device__ __forceinline__ float vec_max(const uint4& u) {
+  if constexpr (LogitType<T>::E == 4) {
+    return max_nan(max_nan(__uint_as_float(u.x), __uint_as_float(u.y)), max_nan(__uint_as_float(u.z), __uint_as_float(u.w)));
+  } else if constexpr (std::is_same<T, __half>::value) {
+    const __half2* h = reinterpret_cast<const __half2*>(&u);
+    const float2 f = __half22float2(__hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3])));
+    return max_nan(f.x, f.y);
+  } else {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
+    const float2 f = __bfloat1622float2(__hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3])));
+    return max_nan(f.x, f.y);
+  }
 }
 
 }  // namespace astrai

@@ -34,35 +34,6 @@ struct TopArgs {
   float* rest;   // [rows]
 };
 
-// Greater logits have greater keys; -0 and 0 the same one, a NaN the greatest.
-__device__ __forceinline__ uint32_t key_of(float x) {
-  if (x != x) return 0xFFFFFFFFu;
-  const uint32_t u = __float_as_uint(x + 0.f);
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
-}
-__device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k); }
-
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
-// largest element, NaN if there is one
-template <typename T>
-__device__ __forceinline__ float vec_max(const uint4& u) {
-  if constexpr (LogitType<T>::E == 4) {
-    return max_nan(max_nan(__uint_as_float(u.x), __uint_as_float(u.y)), max_nan(__uint_as_float(u.z), __uint_as_float(u.w)));
-  } else if constexpr (std::is_same<T, __half>::value) {
-    const __half2* h = reinterpret_cast<const __half2*>(&u);
-    const float2 f = __half22float2(__hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3])));
-    return max_nan(f.x, f.y);
-  } else {
-    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
-    const float2 f = __bfloat1622float2(__hmax2_nan(__hmax2_nan(h[0], h[1]), __hmax2_nan(h[2], h[3])));
-    return max_nan(f.x, f.y);
-  }
-}
-
 struct TopShared {
   unsigned long long list[TOP_CAP];  // key, then the id's complement: greater ranks first
   float left[TOP_CAP];                     // logits of candidates that are not among the k

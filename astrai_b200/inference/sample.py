@@ -220,3 +220,97 @@ def sample(logits: Tensor, temperature: Scalar = 1.0, top_k: Scalar = 0, top_p: 
     pipe = SamplingPipeline([TemperatureStrategy(temperature), TopKStrategy(top_k), TopPStrategy(top_p),
                              FrequencyPenaltyStrategy(frequency_penalty)])
     return pipe.sample(logits, filter_value, input_ids, input_mask, return_logprobs)
+
+
+# ----------------------------------------------------------------------------- from given numbers
+def _given_reference(x: Tensor, uniform: Tensor, temperature: Tensor, top_k: Tensor, top_p: Tensor, min_p: Tensor):
+    rows, vocab = x.shape
+    tokens = torch.zeros(rows, dtype=torch.long)
+    logprobs = torch.full((rows,), float("nan"))
+    settings = zip(uniform.double().tolist(), temperature.tolist(), top_k.tolist(), top_p.double().tolist(),
+                   min_p.double().tolist())
+    for r, (u, t, k, p, m) in enumerate(settings):
+        row = x[r].double()
+        top = float(row.max())
+        if not abs(top) < float("inf"):  # also a NaN
+            number = row.masked_fill(row.isnan(), -float("inf"))
+            if not row.isnan().all():
+                tokens[r] = int(((row == number.max()) & ~row.isnan()).nonzero()[0])
+            continue
+        greedy = not t > 0
+        t = 1.0 if greedy else max(t, 1e-8)
+        w = torch.where(row == -float("inf"), 0.0, ((row - top) / t).exp())
+        if greedy:
+            tokens[r] = int((row == top).nonzero()[0])
+            logprobs[r] = -float(w.sum().log())
+            continue
+        value, place = torch.unique(row, return_inverse=True)  # ascending
+        count = torch.bincount(place, minlength=value.numel())
+        mass = torch.zeros_like(value).index_add_(0, place, w)
+        above = count.flip(0).cumsum(0).flip(0) - count        # tokens of larger value
+        kept = above < k if 0 < k < vocab else torch.ones_like(above, dtype=torch.bool)
+        if p < 1:
+            mass = torch.where(kept, mass, 0.0)
+            larger = mass.flip(0).cumsum(0).flip(0) - mass
+            larger[-1] = 0.0
+            kept &= larger <= max(p, 0.0) * mass.sum()
+        w = torch.where(kept[place], w, 0.0)
+        if m > 0:
+            w = torch.where(w >= min(m, 1.0), w, 0.0)
+        sums = w.cumsum(0)
+        u = min(max(u, 0.0), 1.0) if u == u else 0.0
+        hit = ((sums > u * sums[-1]) & (w > 0)).nonzero()
+        tokens[r] = int(hit[0]) if hit.numel() else int((w > 0).nonzero()[-1])
+        logprobs[r] = float((w[tokens[r]] / sums[-1]).log())
+    return tokens, logprobs
+
+
+def _setting(name: str, v: Scalar, low: float, high: float, device, dtype) -> Tensor:
+    if isinstance(v, Tensor):
+        return v if v.device == device else v.to(device)
+    if not low <= v <= high:
+        raise ValueError(f"sample_given: {name} must be in [{low}, {high}], got {v}")
+    return torch.full((1,), v, device=device, dtype=dtype)
+
+
+@torch.no_grad()
+def sample_given(logits: Tensor, uniform: Tensor, temperature: Scalar = 1.0, top_k: Scalar = 0, top_p: Scalar = 1.0,
+                 min_p: Scalar = 0.0, return_logprobs: bool = False) -> Union[Tensor, Tuple[Tensor, Tensor]]:
+    """One token per row of ``logits [batch, vocab]`` from a given number of each row, so that a draw can be repeated.
+
+    ``uniform [batch]`` holds fp32 or fp64 numbers in [0, 1) (others count as the nearer end, NaN as 0). The settings are
+    numbers or tensors of one entry per row. With ``w = exp((logit - max) / temperature)`` a row keeps
+
+    * ``top_k`` (0 or at least ``vocab``: off): the logits not below the k-th largest;
+    * ``top_p`` (1: off): those whose strictly larger ones hold at most ``top_p`` of what top-k kept;
+    * ``min_p`` (0: off): those with ``w >= min_p``, a share of the largest probability
+
+    (tokens of equal logits together), and takes the first id at which the running sum of ``w`` over the kept ids exceeds
+    ``uniform`` times the whole, as 64-bit arithmetic has it. Temperature 0 takes the largest logit, of equal ones the
+    lowest id; temperatures below 1e-8 count as that. ``return_logprobs`` also gives the token's fp32 log-probability
+    among the kept (greedy: among all). A row with a NaN, an infinity or nothing but -inf has no distribution: it gives
+    its largest number's id, and NaN for the log-probability.
+
+    :func:`sample` draws its own numbers and knows a frequency penalty, but no ``min_p``.
+    """
+    if logits.dim() != 2 or logits.shape[1] < 1:
+        raise ValueError("sample_given: logits must be [batch, vocab]")
+    dev, rows = logits.device, logits.shape[0]
+    if uniform.numel() != rows:
+        raise ValueError("sample_given: uniform must have one number per row")
+    settings = [_setting("temperature", temperature, 0.0, float("inf"), dev, torch.float32),
+                _setting("top_k", top_k, 0, 2 ** 31 - 1, dev, torch.int32),
+                _setting("top_p", top_p, 0.0, 1.0, dev, torch.float32),
+                _setting("min_p", min_p, 0.0, 1.0, dev, torch.float32)]
+    if logits.is_cuda:
+        from astrai_b200.ops._ext import native
+
+        token, logprob = native().sample_given(logits, uniform, *settings, return_logprobs)
+    else:
+        for s in settings:
+            if s.numel() not in (1, rows):
+                raise ValueError("sample_given: a setting must have one number or one per row")
+        kinds = (torch.float32, torch.int32, torch.float32, torch.float32)
+        rowwise = [s.reshape(-1).to(kind).expand(rows) for s, kind in zip(settings, kinds)]
+        token, logprob = _given_reference(logits, uniform.reshape(-1), *rowwise)
+    return (token, logprob) if return_logprobs else token
