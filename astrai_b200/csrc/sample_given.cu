@@ -12,9 +12,10 @@
 // 64 bits. Sums over a whole row are taken in 32 bits first, with a bound on their error; a row whose answer lies within it
 // is summed again in 64 bits.
 //
-// A row is read once, into shared memory: a CTA of 512 threads holds up to 64 KB of it, a longer row is shared by a cluster. The
-// bound that gathers the candidates is the one of the top logits: the smallest, over the row's warps, of each warp's j-th
-// largest thread maximum.
+// A row is read once, into shared memory: a CTA of 512 threads holds up to 64 KB of it, a longer row is shared by a cluster.
+// The bound that gathers the candidates is the one of the top logits: the smallest, over the row's warps, of each warp's j-th
+// largest thread maximum. Where top-p reaches below them (flat rows) or k is large, a histogram of the logits over 4096 equal
+// steps shows in which steps the bound must lie, and the few logits there are ordered and decided exactly.
 #include <cooperative_groups.h>
 
 #include "launch.cuh"
@@ -29,6 +30,7 @@ constexpr int SG_WARPS = SG_THREADS / 32;
 constexpr int SG_VECS = 8;  // 16-byte vectors of a thread
 constexpr int SG_LIST_K = 256;  // top-k up to here, and the largest logits looked at for top-p, go by the list
 constexpr int SG_CAP = 1024;
+constexpr int SG_BINS = 4096;
 constexpr int SG_MAX_CLUSTER = 16;
 
 struct SampleGivenArgs {
@@ -50,19 +52,27 @@ enum Verdict { kDone = 0, kAmbiguous = 1, kIncomplete = 2 };
 struct SampleShared {
   unsigned long long list[SG_CAP];    // candidates: key, then the id's complement
   unsigned long long sorted[SG_CAP];  // greatest first
-  double weight[SG_CAP];              // of the sorted ones
-  double before[SG_CAP];              // mass of those before it
-  double warp_sum[2][SG_WARPS];
-  double sums[2];                     // of this CTA
-  uint32_t warp_key[SG_WARPS];
-  int warp_count[SG_WARPS];
-  uint32_t key;  // of this CTA
-  int count;     // of this CTA
+  union {
+    struct {
+      double weight[SG_CAP];  // of the sorted ones
+      double before[SG_CAP];  // mass of those before it
+    };
+    uint32_t bins[SG_BINS];
+  };
+  double warp_sum[2][SG_WARPS];  // two of each: a reduction writes one while the last one's may still be read
+  double sums[2];                // of this CTA
+  uint32_t warp_key[2][SG_WARPS], key[2];
   int n;         // the leader's: candidates of the row
   int verdict;   // the leader's
+  uint32_t low;  // the least key that min-p keeps; the leader's: the least key that the row keeps
+  uint32_t scan[SG_WARPS];
+  double scan64[SG_WARPS];
+  int found;
+  uint32_t found_above;
 };
 
-// What the rows' settings say, and the sums over threads, CTAs and the cluster.
+// What the row's settings say, and the reductions over warps, CTAs and the cluster: their results are the same in all
+// threads of the row.
 struct SampleRow {
   SampleShared& sh;
   int cs, rank, t, lane, w;
@@ -70,37 +80,42 @@ struct SampleRow {
   double T64, p, m, draw;
   bool use_k, use_p, use_m;
   int k;
+  int turn = 0;
 
   __device__ void sync() const {
     if (cs > 1) cg::this_cluster().sync();
     else __syncthreads();
   }
-  // The results of these are the same in all threads of the row.
-  __device__ uint32_t max_key(uint32_t key) const {
-    key = __reduce_max_sync(0xffffffff, key);
+  template <typename F>
+  __device__ uint32_t reduce(uint32_t v, F f) {
+    const int at = turn ^= 1;
+    v = f(v);
+    if (lane == 0) sh.warp_key[at][w] = v;
     __syncthreads();
-    if (lane == 0) sh.warp_key[w] = key;
-    __syncthreads();
-    key = __reduce_max_sync(0xffffffff, sh.warp_key[lane & (SG_WARPS - 1)]);
+    v = f(sh.warp_key[at][lane & (SG_WARPS - 1)]);
     if (cs > 1) {
-      if (t == 0) sh.key = key;
+      if (t == 0) sh.key[at] = v;
       cg::this_cluster().sync();
-      key = __reduce_max_sync(0xffffffff, *cg::this_cluster().map_shared_rank(&sh.key, lane < cs ? lane : 0));
-      cg::this_cluster().sync();
+      v = f(*cg::this_cluster().map_shared_rank(&sh.key[at], lane < cs ? lane : 0));
     }
-    return key;
+    return v;
   }
-  __device__ int count(int n) const {
+  __device__ uint32_t max_key(uint32_t v) {
+    return reduce(v, [](uint32_t x) { return __reduce_max_sync(0xffffffff, x); });
+  }
+  __device__ uint32_t min_key(uint32_t v) {
+    return reduce(v, [](uint32_t x) { return __reduce_min_sync(0xffffffff, x); });
+  }
+  __device__ int count(int n) {
+    const int at = turn ^= 1;
     n = __reduce_add_sync(0xffffffff, n);
+    if (lane == 0) sh.warp_key[at][w] = n;
     __syncthreads();
-    if (lane == 0) sh.warp_count[w] = n;
-    __syncthreads();
-    n = __reduce_add_sync(0xffffffff, lane < SG_WARPS ? sh.warp_count[lane] : 0);
+    n = __reduce_add_sync(0xffffffff, lane < SG_WARPS ? (int)sh.warp_key[at][lane] : 0);
     if (cs > 1) {
-      if (t == 0) sh.count = n;
+      if (t == 0) sh.key[at] = n;
       cg::this_cluster().sync();
-      n = __reduce_add_sync(0xffffffff, lane < cs ? *cg::this_cluster().map_shared_rank(&sh.count, lane) : 0);
-      cg::this_cluster().sync();
+      n = __reduce_add_sync(0xffffffff, lane < cs ? (int)*cg::this_cluster().map_shared_rank(&sh.key[at], lane) : 0);
     }
     return n;
   }
@@ -109,33 +124,45 @@ struct SampleRow {
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffff, v, o);
     return v;
   }
-  // Two sums. The first one's parts: before this CTA, in it, and whether CTAs after it have any; its warps' parts stay in
-  // sh.warp_sum[0].
+  // A sum and its parts: before this CTA, in it, and whether no CTA after it has any; in this warp and the warps before it in
+  // the CTA, and whether no warp after it has any.
   struct Part {
-    double before, here;
-    bool last;
+    double total, before, here, warp_before, warp;
+    bool last, warp_last;
   };
-  __device__ Part sum(double& s0, double& s1) const {
-    s0 = warp_add(s0);
-    s1 = warp_add(s1);
+  __device__ Part sum(double s) {
+    const int at = turn ^= 1;
+    Part part;
+    part.warp = s = warp_add(s);
+    if (lane == 0) sh.warp_sum[at][w] = s;
     __syncthreads();
-    if (lane == 0) sh.warp_sum[0][w] = s0, sh.warp_sum[1][w] = s1;
-    __syncthreads();
-    s0 = s1 = 0.;
-    for (int i = 0; i < SG_WARPS; ++i) s0 += sh.warp_sum[0][i], s1 += sh.warp_sum[1][i];
-    Part part{0., s0, true};
+    const double theirs = sh.warp_sum[at][lane & (SG_WARPS - 1)];
+    double scan = theirs;
+#pragma unroll
+    for (int o = 1; o < SG_WARPS; o <<= 1) {
+      const double up = __shfl_up_sync(0xffffffff, scan, o, SG_WARPS);
+      if ((lane & (SG_WARPS - 1)) >= o) scan += up;
+    }
+    part.total = part.here = __shfl_sync(0xffffffff, scan, SG_WARPS - 1);
+    part.warp_before = __shfl_sync(0xffffffff, scan, max(w - 1, 0));
+    if (w == 0) part.warp_before = 0.;
+    part.warp_last = (__ballot_sync(0xffffffff, theirs > 0.) & ((1u << SG_WARPS) - 1)) >> (w + 1) == 0;
+    part.before = 0.;
+    part.last = true;
     if (cs > 1) {
-      if (t == 0) sh.sums[0] = s0, sh.sums[1] = s1;
+      if (t == 0) sh.sums[at] = part.here;
       cg::this_cluster().sync();
-      s0 = s1 = 0.;
-      for (int i = 0; i < cs; ++i) {
-        const double* theirs = cg::this_cluster().map_shared_rank(sh.sums, i);
-        if (i == rank) part.before = s0;
-        if (i > rank && theirs[0] > 0.) part.last = false;
-        s0 += theirs[0];
-        s1 += theirs[1];
+      const double others = lane < cs ? *cg::this_cluster().map_shared_rank(&sh.sums[at], lane) : 0.;
+      scan = others;
+#pragma unroll
+      for (int o = 1; o < SG_MAX_CLUSTER; o <<= 1) {
+        const double up = __shfl_up_sync(0xffffffff, scan, o);
+        if (lane >= o) scan += up;
       }
-      cg::this_cluster().sync();
+      part.total = __shfl_sync(0xffffffff, scan, SG_MAX_CLUSTER - 1);
+      part.before = __shfl_sync(0xffffffff, scan, max(rank - 1, 0));
+      if (rank == 0) part.before = 0.;
+      part.last = __ballot_sync(0xffffffff, others > 0.) >> (rank + 1) == 0;
     }
     return part;
   }
@@ -182,10 +209,22 @@ __device__ void order_list(const SampleRow& r, int n) {
   __syncthreads();
 }
 
+// Where the value of the sorted candidate i begins.
+__device__ __forceinline__ int first_of_value(const SampleShared& sh, int i) {
+  int first = 0, last = i;
+  const uint32_t key = key_part(sh.sorted[i]);
+  while (first < last) {
+    const int mid = (first + last) / 2;
+    if (key_part(sh.sorted[mid]) == key) last = mid;
+    else first = mid + 1;
+  }
+  return first;
+}
+
 // The leader's answer from its candidates. `total` +- `error` is the mass of the row that top-p takes a share of, where top-k
 // is off; `complete`: no token below the candidates can be kept.
-__device__ void answer_from_list(const SampleRow& r, int n, bool complete, double total, double error, long long* token,
-                                 float* logprob) {
+__device__ void answer_from_list(SampleRow& r, int n, bool complete, uint32_t low_m, double total, double error,
+                                 long long* token, float* logprob) {
   SampleShared& sh = r.sh;
   const uint32_t kth = r.use_k && r.k <= n ? key_part(sh.sorted[r.k - 1]) : 0;
   int nk = n;
@@ -202,17 +241,11 @@ __device__ void answer_from_list(const SampleRow& r, int n, bool complete, doubl
     const int i = i0 + r.t;
     bool keep = i < nk;
     if (keep && r.use_p) {
-      int first = 0, last = i;  // where its value begins
-      const uint32_t key = key_part(sh.sorted[i]);
-      while (first < last) {
-        const int mid = (first + last) / 2;
-        if (key_part(sh.sorted[mid]) == key) last = mid;
-        else first = mid + 1;
-      }
+      const int first = first_of_value(sh, i);
       keep = !(sh.before[first] > share);
       unsure |= first > 0 && blur > 0. && fabs(sh.before[first] - share) <= blur;
     }
-    if (keep && r.use_m) keep = sh.weight[i] >= r.m;
+    if (keep && r.use_m) keep = key_part(sh.sorted[i]) >= low_m;
     kept += __syncthreads_count(keep);
   }
   int verdict = kDone;
@@ -241,13 +274,13 @@ __device__ void answer_from_list(const SampleRow& r, int n, bool complete, doubl
         if (sh.weight[i] > 0.) last = max(last, id);
       }
     }
+    const int at = r.turn;
     best = __reduce_max_sync(0xffffffff, best);
     last = __reduce_max_sync(0xffffffff, last);
+    if (r.lane == 0) sh.warp_key[at][r.w] = best, sh.scan[r.w] = (uint32_t)last;
     __syncthreads();
-    if (r.lane == 0) sh.warp_key[r.w] = best, sh.warp_count[r.w] = last;
-    __syncthreads();
-    best = __reduce_max_sync(0xffffffff, sh.warp_key[r.lane & (SG_WARPS - 1)]);
-    last = __reduce_max_sync(0xffffffff, sh.warp_count[r.lane & (SG_WARPS - 1)]);
+    best = __reduce_max_sync(0xffffffff, sh.warp_key[at][r.lane & (SG_WARPS - 1)]);
+    last = __reduce_max_sync(0xffffffff, (int)sh.scan[r.lane & (SG_WARPS - 1)]);
     const int id = best ? (int)~best : last;
     for (int i = r.t; i < kept; i += SG_THREADS)
       if (id_part(sh.sorted[i]) == id) {
@@ -256,6 +289,32 @@ __device__ void answer_from_list(const SampleRow& r, int n, bool complete, doubl
       }
   }
   if (r.t == 0) sh.verdict = verdict;
+}
+
+// The leader's bound of top-p among the candidates of a few steps of the histogram, above which lies `above` +- `error`; `end`:
+// no logit lies below them. The mass of strictly larger logits must be known to lie below or above the share.
+__device__ void bound_from_list(const SampleRow& r, int n, bool end, double above, double error, double share, double blur) {
+  SampleShared& sh = r.sh;
+  const double doubt = error + blur;
+  bool unsure = false;
+  int kept = 0;
+  for (int i0 = 0; i0 < n; i0 += SG_THREADS) {
+    const int i = i0 + r.t;
+    bool keep = i < n;
+    if (keep) {
+      const double larger = above + sh.before[first_of_value(sh, i)];
+      keep = !(larger > share);
+      unsure |= larger > 0. && doubt > 0. && fabs(larger - share) <= doubt;
+    }
+    kept += __syncthreads_count(keep);
+  }
+  const double all = above + (n > 0 ? sh.before[n - 1] + sh.weight[n - 1] : 0.);
+  unsure |= !end && doubt > 0. && fabs(all - share) <= doubt;
+  unsure = __syncthreads_or(unsure);
+  if (r.t == 0) {
+    sh.verdict = unsure ? kAmbiguous : (kept == 0 || (!end && !(all > share)) ? kIncomplete : kDone);
+    sh.low = kept > 0 ? key_part(sh.sorted[kept - 1]) : 0;
+  }
 }
 
 template <typename T>
@@ -299,10 +358,11 @@ __global__ void __launch_bounds__(SG_THREADS, 2) sample_given_kernel(const Sampl
   r.m = r.use_m ? fmin((double)m, 1.) : 0.;
   r.draw = a.uniform64 ? static_cast<const double*>(a.uniform)[row] : (double)static_cast<const float*>(a.uniform)[row];
   r.draw = fmin(fmax(r.draw, 0.), 1.);  // a NaN becomes 0
+  long long* const token = a.token + row;
+  float* const logprob = a.logprob ? a.logprob + row : nullptr;
   SampleShared* lead = &sh;
   if (cs > 1) lead = cg::this_cluster().map_shared_rank(&sh, 0);
   if (t == 0) sh.n = 0;
-
   const float c = (float)(1.4426950408889634 / r.T64);
   r.max_x = of_key(r.max_key(key_of(nan ? of_key(0xFFFFFFFFu) : top)));
 
@@ -318,90 +378,68 @@ __global__ void __launch_bounds__(SG_THREADS, 2) sample_given_kernel(const Sampl
         if (at + e >= 0 && at + e < a.V) f(x[e], at + e);
     }
   };
-  const bool none = !(fabsf(r.max_x) < INFINITY);
-  if (none) {  // a NaN, an infinity or nothing allowed: no distribution; the largest logit that is a number
-    uint32_t key = 0;
-    each([&](float x, int) { if (x == x) key = max(key, key_of(x)); });
-    key = r.max_key(key);
-    uint32_t first = 0;
-    each([&](float x, int id) { if (x == x && key_of(x) == key) first = max(first, ~(uint32_t)id); });
-    first = r.max_key(first);
-    if (rank == 0 && t == 0) {
-      a.token[row] = key ? (int)~first : 0;
-      if (a.logprob) a.logprob[row] = __int_as_float(0x7FC00000);
-    }
-    return;
-  }
-
-  // Mass of what `keep` leaves of a vector, and its sum of w |t|. In 32 bits each exponential is within 2^-22 of itself and
-  // 3 |t| 2^-24 ln 2 for the roundings of t = (x - max) c, and eight of them are added in a tree.
-  const auto vec_mass = [&](int i, bool precise, auto keep, float& spread) {
-    float x[E];
-    vec_floats<T>(held[i * SG_THREADS + t], x);
+  // Mass of a vector's logits from `low` on. In 32 bits each exponential is within 2^-22 of itself and 3 |t| 2^-24 ln 2 for
+  // the roundings of t = (x - max) c, and eight of them are added in a tree.
+  const auto vec_mass = [&](int i, bool precise, float low) -> double {
+    const uint4 u = held[i * SG_THREADS + t];
     if (precise) {
+      float x[E];
+      vec_floats<T>(u, x);
       double s = 0.;
 #pragma unroll 1
       for (int e = 0; e < E; ++e)
-        if (x[e] > -INFINITY && keep(x[e])) s += r.weight(x[e]);
+        if (x[e] >= low) s += r.weight(x[e]);
       return s;
     }
-    float s[E];
+    const Pair ref2(-r.max_x, -r.max_x), c2(c, c);
+    float x[E];
+    vec_floats<T>(u, x);
+    Pair q[E / 2];
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const float arg = (x[e] - r.max_x) * c;
-      s[e] = x[e] > -INFINITY && keep(x[e]) ? exp2_fast(arg) : 0.f;
-      if (s[e] > 0.f) spread -= s[e] * arg;
-    }
+    for (int e = 0; e < E / 2; ++e)
+      q[e] = exp2_fast((Pair(x[2 * e] >= low ? x[2 * e] : -INFINITY, x[2 * e + 1] >= low ? x[2 * e + 1] : -INFINITY) + ref2) * c2);
 #pragma unroll
-    for (int o = E / 2; o > 0; o >>= 1)
+    for (int o = E / 4; o > 0; o >>= 1)
 #pragma unroll
-      for (int e = 0; e < o; ++e) s[e] += s[e + o];
-    return (double)s[0];
+      for (int e = 0; e < o; ++e) q[e] = q[e] + q[e + o];
+    return (double)q[0].sum();
   };
-  SampleRow::Part part;
-  const auto masses = [&](bool precise, auto keep, double& total, double& error) {
-    double spread = 0.;
-    total = 0.;
+  // Over the row, with a bound on its error: the mass' average |t| is the entropy of its shares less log2 of it (the largest
+  // weight is 1), at most log2 V - log2 total.
+  double error = 0.;
+  const float log_v = log2f((float)a.V);
+  const auto masses = [&](bool precise, float low) {
+    double s = 0.;
 #pragma unroll 1
-    for (int i = 0; i < mine; ++i) {
-      float d = 0.f;
-      total += vec_mass(i, precise, keep, d);
-      spread += d;
-    }
-    part = r.sum(total, spread);
-    error = precise ? 0. : 4.5e-7 * total + 1.3e-7 * spread;
+    for (int i = 0; i < mine; ++i) s += vec_mass(i, precise, low);
+    const SampleRow::Part part = r.sum(s);
+    error = precise ? 0. : part.total * (4.5e-7 + 1.3e-7 * fmaxf(log_v - log2f((float)part.total), 0.f));
+    return part;
   };
-  // Draws among what `keep` leaves.
-  const auto draw = [&](auto keep) {
+  // Draws among the logits from `low` on.
+  const auto draw = [&](float low) {
 #pragma unroll 1
     for (int precise = 0; precise < 2; ++precise) {
       if (rank == 0 && t == 0) sh.verdict = kDone;
-      double total, error;
-      masses(precise, keep, total, error);
+      const SampleRow::Part part = masses(precise, low);
       // The CTA in whose part the target lies, and there, counted from its start, the warp. Should rounding leave the
       // target at the very end, the last one with any mass takes it.
-      double target = r.draw * total;
+      double target = r.draw * part.total;
       const bool here = part.here > 0. && part.before <= target && (target < part.before + part.here || part.last);
       target -= part.before;
-      double before = 0.;
-      for (int i = 0; i < w; ++i) before += sh.warp_sum[0][i];
-      bool last = true;
-      for (int i = w + 1; i < SG_WARPS; ++i) last &= !(sh.warp_sum[0][i] > 0.);
-      const double hi = before + sh.warp_sum[0][w];
-      if (here && before < hi && before <= target && (target < hi || last)) {
+      double before = part.warp_before;
+      if (here && part.warp > 0. && before <= target && (target < before + part.warp || part.warp_last)) {
         int at_i = 0, last_i = 0;
         double at_before = -1., last_before = before, s;
 #pragma unroll 1
         for (int i = 0; i < chunk / 32; ++i) {
-          float d = 0.f;
-          s = SampleRow::warp_add(i < mine ? vec_mass(i, precise, keep, d) : 0.);
+          s = SampleRow::warp_add(i < mine ? vec_mass(i, precise, low) : 0.);
           if (s > 0.) last_i = i, last_before = before;
           if (at_before < 0. && before + s > target) at_i = i, at_before = before;
           before += s;
         }
         if (at_before < 0.) at_i = last_i, at_before = last_before;
-        float d = 0.f;
-        s = at_i < mine ? vec_mass(at_i, precise, keep, d) : 0.;
+        s = at_i < mine ? vec_mass(at_i, precise, low) : 0.;
         double scan = s;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -419,7 +457,7 @@ __global__ void __launch_bounds__(SG_THREADS, 2) sample_given_kernel(const Sampl
           const int at = vecs.first(w0 + at_i * 32 + lane);
 #pragma unroll
           for (int e = 0; e < E; ++e) {
-            if (!(x[e] > -INFINITY) || !keep(x[e])) continue;
+            if (!(x[e] >= low)) continue;
             const double one = precise ? r.weight(x[e]) : (double)exp2_fast((x[e] - r.max_x) * c);
             if (one > 0. && (id < 0 || !(c1 > target))) {  // the first above the target, or the last with any mass
               id = at + e;
@@ -432,8 +470,8 @@ __global__ void __launch_bounds__(SG_THREADS, 2) sample_given_kernel(const Sampl
           if (!precise && (target - c0 <= 2. * error || c1 - target <= 2. * error)) {
             lead->verdict = kAmbiguous;
           } else {
-            a.token[row] = id;
-            if (a.logprob) a.logprob[row] = (float)log(r.weight(chosen) / total);
+            *token = id;
+            if (logprob) *logprob = (float)log(r.weight(chosen) / part.total);
           }
         }
       }
@@ -443,35 +481,83 @@ __global__ void __launch_bounds__(SG_THREADS, 2) sample_given_kernel(const Sampl
       if (verdict == kDone) return;
     }
   };
-
-  double total = 0., error = 0.;
-  if (greedy) {
-    uint32_t first = 0;
-    each([&](float x, int id) { if (x == r.max_x) first = max(first, ~(uint32_t)id); });
-    first = r.max_key(first);
-    masses(false, [](float) { return true; }, total, error);
-    if (rank == 0 && t == 0) {
-      a.token[row] = (int)~first;
-      if (a.logprob) a.logprob[row] = (float)-log(total);
+  // Candidates: logits for which `in` holds, into the leader's list.
+  const auto gather = [&](float low, auto in) {
+#pragma unroll 1
+    for (int i = 0; i < mine; ++i) {
+      const uint4 u = held[i * SG_THREADS + t];
+      if (!(vec_max<T>(u) >= low)) continue;
+      const int at = vecs.first(w0 + i * 32 + lane);
+      float x[E];
+      vec_floats<T>(u, x);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        if (!(x[e] >= low) || !in(x[e]) || at + e < 0 || at + e >= a.V) continue;
+        const int slot = atomicAdd(&lead->n, 1);
+        if (slot < SG_CAP) lead->list[slot] = (unsigned long long)key_of(x[e]) << 32 | (uint32_t)~(at + e);
+      }
     }
-    return;
-  }
+    r.sync();
+    return lead->n;
+  };
 
-  const auto all = [](float) { return true; };
-  const bool by_k = r.use_k && r.k <= SG_LIST_K;
-  if (by_k || (!r.use_k && (r.use_p || r.use_m))) {
-    // A bound that all candidates reach.
-    uint32_t bound = 0;
-    if (r.use_m && !(by_k && r.use_p)) {
-      const double x = r.max_x + r.T64 * log(r.m);
-      bound = key_of((float)(x - 1e-6 * (fabs(x) + fabs(r.max_x) + r.T64)));
+  const auto run = [&] {
+    if (!(fabsf(r.max_x) < INFINITY)) {  // a NaN, an infinity or nothing allowed: no distribution; the largest number
+      uint32_t key = 0;
+      each([&](float x, int) { if (x == x) key = max(key, key_of(x)); });
+      key = r.max_key(key);
+      uint32_t first = 0;
+      each([&](float x, int id) { if (x == x && key_of(x) == key) first = max(first, ~(uint32_t)id); });
+      first = r.max_key(first);
+      if (rank == 0 && t == 0) {
+        *token = key ? (int)~first : 0;
+        if (logprob) *logprob = __int_as_float(0x7FC00000);
+      }
+      return;
     }
-    bool complete = by_k || r.use_m;
-    if (by_k || r.use_p) {
-      const auto full = [&](int n) { return n < 32 ? 0 : min((n - 32) / chunk + 1, SG_WARPS); };
+    if (greedy) {
+      uint32_t first = 0;
+      if (top == r.max_x) each([&](float x, int id) { if (x == r.max_x) first = max(first, ~(uint32_t)id); });
+      first = r.max_key(first);
+      const double total = logprob ? masses(false, -INFINITY).total : 1.;
+      if (rank == 0 && t == 0) {
+        *token = (int)~first;
+        if (logprob) *logprob = (float)-log(total);
+      }
+      return;
+    }
+
+    // min-p as a bound on the key: the least whose weight reaches it, among the 32 around max + T ln m, or where that window
+    // lies above it (temperatures at which neighbours have the same weight) by a search in 32 parts.
+    if (r.use_m && w == 0) {
+      const uint32_t max_key = key_of(r.max_x);
+      const auto reaches = [&](uint32_t key) {
+        return __ballot_sync(0xffffffff, key == max_key || (key < max_key && r.weight(of_key(key)) >= r.m));
+      };
+      uint32_t lo = key_of(-3.4028235e38f), step = 1;
+      uint32_t from = max(key_of((float)fmax(r.max_x + r.T64 * log(r.m), -3.4e38)), lo + 16) - 16;
+      uint32_t ok = reaches(from + lane), hi = ok ? from + __ffs(ok) - 1 : max_key;
+      if (ok & 1) {
+        while (lo < hi) {
+          step = (hi - lo) / 32 + 1;
+          ok = reaches(min(lo + lane * step, hi));  // the last one does
+          const int i = __ffs(ok) - 1;
+          hi = min(lo + i * step, hi);
+          if (i > 0) lo = lo + (i - 1) * step + 1;
+          else break;
+        }
+      }
+      if (lane == 0) sh.low = hi;
+    }
+    const bool by_k = r.use_k && r.k <= SG_LIST_K;
+    const bool by_list = by_k || (!r.use_k && (r.use_p || r.use_m));
+    // A bound that all candidates of top-k, or the SG_LIST_K largest logits, reach.
+    uint32_t low = 0xFFFFFFFFu;
+    if (by_k || (r.use_p && !r.use_k)) {
+      const auto full = [&](int n) { return n < 32 ? 0 : min((n - 32) / chunk + 1, SG_WARPS); };  // warps without an idle lane
       const int warps = (cs - 1) * full(per) + full(vecs.n - (cs - 1) * per);
       const int j = warps > 0 ? ((by_k ? r.k : SG_LIST_K) + warps - 1) / warps : 33;
-      uint32_t key = key_of(top), low = 0xFFFFFFFFu;
+      uint32_t key = key_of(top);
       if (j > 32) {
         low = 0;
       } else if (w < full(v1 - v0)) {
@@ -481,76 +567,203 @@ __global__ void __launch_bounds__(SG_THREADS, 2) sample_given_kernel(const Sampl
           if (lane == __ffs(__ballot_sync(0xffffffff, key == low)) - 1) key = 0;
         }
       }
-      low = ~r.max_key(~low);
-      if (low > bound) {
-        complete = by_k || low == 0;
-        bound = low;
-      }
-      complete |= low == 0;
     }
-    if (r.use_p && !by_k) masses(false, all, total, error);
-    each([&](float x, int id) {
-      const uint32_t key = key_of(x);
-      if (key < bound) return;
-      const int slot = atomicAdd(&lead->n, 1);
-      if (slot < SG_CAP) lead->list[slot] = (unsigned long long)key << 32 | (uint32_t)~id;
-    });
-    r.sync();
-    const int n = lead->n;
-    if (n <= SG_CAP) {
-      if (rank == 0) order_list(r, n);
-      for (int precise = 0;; ++precise) {
-        if (rank == 0) answer_from_list(r, n, complete, total, error, a.token + row, a.logprob ? a.logprob + row : nullptr);
-        r.sync();
-        const int verdict = lead->verdict;
-        r.sync();
-        if (verdict == kDone) return;
-        if (verdict == kIncomplete) break;
-        masses(true, all, total, error);
+    low = r.min_key(low);  // and its barrier for sh.low
+    const uint32_t low_m = r.use_m ? sh.low : 0;
+    double total = 0.;
+    if (r.use_p && !by_k && !r.use_k) total = masses(false, -INFINITY).total;
+    double total_error = error;
+    if (by_list) {
+      uint32_t bound = by_k || r.use_p ? low : 0;
+      bool complete = by_k || bound == 0;
+      if (r.use_m && !(by_k && r.use_p) && low_m >= bound) bound = low_m, complete = true;
+      // below all numbers: -inf and the padding have no mass
+      const int n = gather(bound <= key_of(-INFINITY) ? -3.4028235e38f : of_key(bound), [](float) { return true; });
+      if (n <= SG_CAP) {
+        if (rank == 0) order_list(r, n);
+        for (int precise = 0;; ++precise) {
+          if (rank == 0) answer_from_list(r, n, complete, low_m, total, total_error, token, logprob);
+          r.sync();
+          const int verdict = lead->verdict;
+          r.sync();
+          if (verdict == kDone) return;
+          if (verdict == kIncomplete) break;
+          total = masses(true, -INFINITY).total;
+          total_error = 0.;
+        }
+      } else {
+        r.sync();  // the leader's count has been read
       }
-    } else {
-      r.sync();  // the leader's count has been read
     }
-  }
 
-  // Many tokens stay: the bounds of top-k and top-p by bisection of the key.
-  uint32_t kth = 0;
-  if (r.use_k) {
-#pragma unroll 1
-    for (int b = 31; b >= 0; --b) {
-      const uint32_t next = kth | 1u << b;
-      int n = 0;
-      each([&](float x, int) { n += key_of(x) >= next; });
-      if (r.count(n) >= r.k) kth = next;
-    }
-  }
-  uint32_t low = kth;
-  if (r.use_p) {
-#pragma unroll 1
-    for (int precise = 0; precise < 2; ++precise) {
-      bool unsure = false;
-      masses(precise, [&](float x) { return key_of(x) >= kth; }, total, error);
-      const double share = r.p * total, blur = r.p * error;
-      uint32_t cut = 0;  // the largest key such that it and those above hold more than the share
-#pragma unroll 1
-      for (int b = 31; b >= 0; --b) {
-        const uint32_t next = cut | 1u << b;
-        double s, e;
-        masses(precise, [&](float x) { return key_of(x) >= kth && key_of(x) >= next; }, s, e);
-        unsure |= fabs(s - share) <= e + blur;
-        if (s > share) cut = next;
+    // Many tokens stay. A histogram of the logits over equal steps down from the largest.
+    float least = INFINITY;
+    each([&](float x, int) { if (x > -INFINITY) least = fminf(least, x); });
+    least = of_key(r.min_key(key_of(least)));
+    float range = r.max_x - least;
+    if (r.use_p && !r.use_k) range = fminf(range, 24.f * (float)r.T64);
+    const bool flat = !(range > 0.f);  // all numbers are equal
+    const float scale = flat ? 0.f : (SG_BINS - 1) / range;
+    const auto bin_of = [&](float x) { return min((int)((r.max_x - x) * scale), SG_BINS - 1); };
+    constexpr int kEach = SG_BINS / SG_THREADS;
+    uint32_t count[kEach];  // of this thread's bins, over the row
+    const bool by_bins = scale > 0.f && isfinite(scale) && (r.use_p || r.use_k);
+    if (by_bins) {
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) sh.bins[t * kEach + i] = 0;
+      __syncthreads();
+      each([&](float x, int) { if (x > -INFINITY) atomicAdd(&sh.bins[bin_of(x)], 1u); });
+      r.sync();
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) count[i] = 0;
+      for (int o = 0; o < cs; ++o) {
+        const uint32_t* theirs = cs > 1 ? cg::this_cluster().map_shared_rank(sh.bins, o) : sh.bins;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) count[i] += theirs[t * kEach + i];
       }
-      low = max(kth, cut);
-      if (!unsure) break;
+      r.sync();  // the bins give way to the list's weights
     }
-  }
-  const float near = r.use_m ? r.max_x + (float)r.T64 * logf((float)r.m) : -INFINITY;
-  const float slack = 1e-4f * (fabsf(r.max_x) + fabsf(near) + (float)r.T64);
-  draw([&](float x) {
-    if (key_of(x) < low) return false;
-    if (!r.use_m || x > near + slack) return true;
-    return x >= near - slack && r.weight(x) >= r.m;
-  });
+    // The first bin at which the running sum of `of`(bin, count) exceeds `share`, SG_BINS if none does; `above`: the sum
+    // before it.
+    const auto find_bin = [&](double share, auto of, double& above) {
+      double s = 0.;
+#pragma unroll
+      for (int i = 0; i < kEach; ++i) s += of(t * kEach + i, count[i]);
+      double scan = s;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const double up = __shfl_up_sync(0xffffffff, scan, o);
+        if (lane >= o) scan += up;
+      }
+      if (t == 0) sh.found = SG_BINS;
+      if (lane == 31) sh.scan64[w] = scan;
+      __syncthreads();
+      double base = 0.;
+      for (int i = 0; i < w; ++i) base += sh.scan64[i];
+      double before = base + scan - s;
+      if (before <= share && base + scan > share) {
+        bool done = false;
+        for (int i = 0; i < kEach; ++i) {
+          const double one = of(t * kEach + i, count[i]);
+          if (!done && before + one > share) {
+            atomicMin(&sh.found, t * kEach + i);
+            done = true;
+          }
+          if (!done) before += one;
+        }
+      }
+      __syncthreads();
+      const int bin = sh.found;
+      if (bin / kEach == t) sh.scan64[0] = before;
+      __syncthreads();
+      above = sh.scan64[0];
+      __syncthreads();
+      return bin;
+    };
+
+    uint32_t kth = 0;  // top-k's bound
+    if (r.use_k && flat) {
+      kth = key_of(r.max_x);
+    } else if (r.use_k) {
+      bool found = false;
+      if (by_bins) {
+        double above;
+        const int bin = find_bin(r.k - 0.5, [](int, uint32_t n) { return (double)n; }, above);
+        if (bin == SG_BINS) {
+          found = true;  // fewer numbers than k
+        } else {
+          if (rank == 0 && t == 0) sh.n = 0;
+          r.sync();
+          const int n = gather(-3.4028235e38f, [&](float x) { return bin_of(x) == bin; });
+          if (n <= SG_CAP) {
+            if (rank == 0) {
+              order_list(r, n);
+              if (t == 0) sh.low = key_part(sh.sorted[min(max(r.k - (int)above - 1, 0), n - 1)]);
+            }
+            found = true;
+          }
+          r.sync();
+          kth = lead->low;
+          r.sync();
+          if (!found) kth = 0;
+        }
+      }
+      if (!found) {  // ties, or outliers that leave too few steps for the rest: bisection of the key
+#pragma unroll 1
+        for (int b = 31; b >= 0; --b) {
+          const uint32_t next = kth | 1u << b;
+          int n = 0;
+          each([&](float x, int) { n += key_of(x) >= next; });
+          if (r.count(n) >= r.k) kth = next;
+        }
+      }
+    }
+    const auto from = [&](uint32_t key) { return key <= key_of(-3.4028235e38f) ? -3.4028235e38f : of_key(key); };
+    uint32_t cut = 0;  // top-p's bound
+    if (r.use_p && flat) {
+      cut = key_of(r.max_x);
+    } else if (r.use_p) {
+      bool found = false;
+      if (r.use_k) {
+        total = masses(false, from(kth)).total;
+        total_error = error;
+      }
+      int first = 0, last = -1, n = 0;
+      if (by_bins) {
+        // the steps around the one that the weights at their middles point to
+        double above;
+        const int bin = find_bin(r.p * total, [&](int b, uint32_t n) {
+          return n ? n * (double)exp2_fast(-((float)b + 0.5f) / scale * c) : 0.;
+        }, above);
+        first = max(bin - 2, 0);
+        last = min(bin + 2, SG_BINS - 1);
+        if (rank == 0 && t == 0) sh.n = 0;
+        r.sync();
+        n = gather(from(kth), [&](float x) {
+          const int b = bin_of(x);
+          return b >= first && b <= last;
+        });
+        if (n <= SG_CAP && rank == 0) order_list(r, n);
+        r.sync();
+      }
+#pragma unroll 1
+      for (int precise = 0; precise < 2 && !found; ++precise) {
+        if (precise) {
+          total = masses(true, from(kth)).total;
+          total_error = 0.;
+        }
+        const double share = r.p * total, blur = r.p * total_error;
+        if (by_bins && n <= SG_CAP) {
+          // the least number of the steps above: a bound between them and those gathered
+          float edge = INFINITY;
+          each([&](float x, int) { if (x > -INFINITY && bin_of(x) < first) edge = fminf(edge, x); });
+          edge = of_key(r.min_key(key_of(edge)));
+          const double above = edge < INFINITY ? masses(precise, fmaxf(edge, from(kth))).total : (error = 0., 0.);
+          if (rank == 0) bound_from_list(r, n, last == SG_BINS - 1, above, error, share, blur);
+          r.sync();
+          const int verdict = lead->verdict;
+          cut = lead->low;
+          r.sync();
+          if (verdict == kDone) break;
+          if (verdict == kAmbiguous) continue;
+        }
+        // Bisection: the largest key such that it and those above hold more than the share.
+        bool unsure = false;
+        cut = 0;
+#pragma unroll 1
+        for (int b = 31; b >= 0; --b) {
+          const uint32_t next = cut | 1u << b;
+          const double s = next > key_of(r.max_x) ? (error = 0., 0.) : masses(precise, from(max(next, kth))).total;
+          unsure |= error + blur > 0. && fabs(s - share) <= error + blur;
+          if (s > share) cut = next;
+        }
+        found = !unsure;
+      }
+    }
+    draw(from(max(max(kth, cut), low_m)));
+  };
+  run();
+  if (cs > 1) cg::this_cluster().sync();  // no CTA leaves while others read its memory
 }
 
 template <typename T>
