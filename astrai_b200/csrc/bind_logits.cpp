@@ -24,10 +24,9 @@ int top_logits_max_k();
 int top_logits_max_vocab(int elem);
 void top_logits(const void* x, long long ldx, int rows, int V, int k, float tau, int* ids, void* values, float* rest,
                 int dtype, cudaStream_t s);
-int sample_given_max_vocab(int elem);
 void sample_given(const void* x, long long ldx, int rows, int V, const void* uniform, bool uniform64,
                   const float* temperature, const int* top_k, const float* top_p, const float* min_p, long long* token,
-                  float* logprob, int dtype, cudaStream_t s);
+                  float* logprob, int dtype, int device, cudaStream_t s);
 }  // namespace astrai_host
 
 namespace {
@@ -99,8 +98,7 @@ std::pair<at::Tensor, OptTensor> sample_given(const at::Tensor& logits, const at
   TORCH_CHECK_VALUE(logits.dim() == 2 && logits.size(1) >= 1, "sample_given: logits must be [batch, vocab]");
   const int64_t rows = logits.size(0), V = logits.size(1);
   const int code = dtype_code(logits, "sample_given: logits");
-  TORCH_CHECK_VALUE(V <= astrai_host::sample_given_max_vocab((int)logits.element_size()), "sample_given: a vocabulary of ",
-                    std::to_string(V), " is too large for this type");
+  TORCH_CHECK_VALUE(V < (1LL << 30), "sample_given: vocabulary too large");
   TORCH_CHECK_VALUE(rows < (1LL << 27), "sample_given: too many rows");
   TORCH_CHECK(uniform_in.scalar_type() == at::kFloat || uniform_in.scalar_type() == at::kDouble,
               "sample_given: uniform must be float32 or float64, got ", uniform_in.scalar_type());
@@ -125,7 +123,7 @@ std::pair<at::Tensor, OptTensor> sample_given(const at::Tensor& logits, const at
     astrai_host::sample_given(x.data_ptr(), row_stride(x), (int)rows, (int)V, uniform.data_ptr(),
                               uniform.scalar_type() == at::kDouble, temperature.data_ptr<float>(), top_k.data_ptr<int>(),
                               top_p.data_ptr<float>(), min_p.data_ptr<float>(), (long long*)token.data_ptr<int64_t>(),
-                              logprobs ? logprob->data_ptr<float>() : nullptr, code, stream());
+                              logprobs ? logprob->data_ptr<float>() : nullptr, code, logits.get_device(), stream());
     C10_CUDA_KERNEL_LAUNCH_CHECK();
   }
   return {token, logprob};

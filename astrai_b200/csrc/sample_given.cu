@@ -12,11 +12,14 @@
 // 64 bits. Sums over a whole row are taken in 32 bits first, with a bound on their error; a row whose answer lies within it
 // is summed again in 64 bits.
 //
-// A row is read once, into shared memory: a CTA of 512 threads holds up to 64 KB of it, a longer row is shared by a cluster.
+// A CTA of 512 threads takes a row, or where the rows are too few for the SMs a cluster of CTAs does. Up to 64 KB of logits
+// stay in the CTA's shared memory between the passes over them, more than that come from L2 again.
 // The bound that gathers the candidates is the one of the top logits: the smallest, over the row's warps, of each warp's j-th
 // largest thread maximum. Where top-p reaches below them (flat rows) or k is large, a histogram of the logits over 4096 equal
 // steps shows in which steps the bound must lie, and the few logits there are ordered and decided exactly.
 #include <cooperative_groups.h>
+
+#include <cstdlib>
 
 #include "launch.cuh"
 #include "logits.cuh"
@@ -31,7 +34,7 @@ constexpr int SG_VECS = 8;  // 16-byte vectors of a thread
 constexpr int SG_LIST_K = 256;  // top-k up to here, and the largest logits looked at for top-p, go by the list
 constexpr int SG_CAP = 1024;
 constexpr int SG_BINS = 4096;
-constexpr int SG_MAX_CLUSTER = 16;
+constexpr int SG_MAX_CLUSTER = 8;
 
 struct SampleGivenArgs {
   const void* x;
@@ -47,11 +50,33 @@ struct SampleGivenArgs {
   float* logprob;    // [rows] or null
 };
 
+// 2^t for t <= 0 in 64 bits, within 2^-46 of itself (below 2^-1000: zero): e^z = sum z^n / n! at |z| <= ln 2 / 2, whose 13th
+// term is below 2^-53, times a power of two.
+__device__ __forceinline__ double exp2_64(double t) {
+  constexpr double kRound = 6755399441055744.;  // 1.5 * 2^52: adding it rounds to a whole number
+  const double n = t + kRound, z = (t - (n - kRound)) * 0.6931471805599453;
+  double e = 1. / 479001600.;
+  e = fma(e, z, 1. / 39916800.);
+  e = fma(e, z, 1. / 3628800.);
+  e = fma(e, z, 1. / 362880.);
+  e = fma(e, z, 1. / 40320.);
+  e = fma(e, z, 1. / 5040.);
+  e = fma(e, z, 1. / 720.);
+  e = fma(e, z, 1. / 120.);
+  e = fma(e, z, 1. / 24.);
+  e = fma(e, z, 1. / 6.);
+  e = fma(e, z, 0.5);
+  e = fma(e, z, 1.);
+  e = fma(e, z, 1.);
+  return t > -1000. ? __hiloint2double(__double2hiint(e) + (__double2loint(n) << 20), __double2loint(e)) : 0.;
+}
+
 enum Verdict { kDone = 0, kAmbiguous = 1, kIncomplete = 2 };
 
 struct SampleShared {
   unsigned long long list[SG_CAP];    // candidates: key, then the id's complement
   unsigned long long sorted[SG_CAP];  // greatest first
+  uint16_t by_id[SG_CAP];             // places among the sorted ones, in the order of ids
   union {
     struct {
       double weight[SG_CAP];  // of the sorted ones
@@ -77,7 +102,7 @@ struct SampleRow {
   SampleShared& sh;
   int cs, rank, t, lane, w;
   float max_x;
-  double T64, p, m, draw;
+  double T64, c64, p, m, draw;  // c64: log2(e) / T
   bool use_k, use_p, use_m;
   int k;
   int turn = 0;
@@ -166,13 +191,13 @@ struct SampleRow {
     }
     return part;
   }
-  __device__ double weight(float x) const { return x == -INFINITY ? 0. : exp(((double)x - (double)max_x) / T64); }
+  __device__ double weight(float x) const { return exp2_64(((double)x - (double)max_x) * c64); }
 };
 
 __device__ __forceinline__ uint32_t key_part(unsigned long long e) { return (uint32_t)(e >> 32); }
 __device__ __forceinline__ int id_part(unsigned long long e) { return (int)~(uint32_t)e; }
 
-// The leader's candidates in order, their weights and running mass.
+// The leader's candidates in order of value, their weights, and their places in the order of ids.
 __device__ void order_list(const SampleRow& r, int n) {
   SampleShared& sh = r.sh;
   const int quarter = r.t & 3;
@@ -180,33 +205,46 @@ __device__ void order_list(const SampleRow& r, int n) {
   for (int i0 = 0; i0 < n; i0 += SG_THREADS / 4) {
     const int i = i0 + r.t / 4;
     const unsigned long long mine = i < n ? sh.list[i] : 0;
-    int above = 0;
-    for (int l = quarter; l < n; l += 4) above += sh.list[l] > mine;
+    int above = 0, earlier = 0;
+#pragma unroll 4
+    for (int l = quarter; l < n; l += 4) {
+      const unsigned long long other = sh.list[l];
+      above += other > mine;
+      earlier += (uint32_t)other > (uint32_t)mine;  // complements of ids
+    }
     above += __shfl_xor_sync(0xffffffff, above, 1);
     above += __shfl_xor_sync(0xffffffff, above, 2);
+    earlier += __shfl_xor_sync(0xffffffff, earlier, 1);
+    earlier += __shfl_xor_sync(0xffffffff, earlier, 2);
     if (i < n && quarter == 0) {
       sh.sorted[above] = mine;
       sh.weight[above] = r.weight(of_key(key_part(mine)));
+      sh.by_id[earlier] = (uint16_t)above;
     }
   }
   __syncthreads();
-  if (r.w == 0) {
-    const int each = (n + 31) / 32, a = min(n, r.lane * each), b = min(n, a + each);
-    double s = 0.;
-    for (int i = a; i < b; ++i) s += sh.weight[i];
-    double run = s;
+}
+
+// For warp 0 of the leader: the running sums of v(i), i < n, each lane its own part of them; before(i, sum before i, v(i)).
+template <typename V, typename F>
+__device__ __forceinline__ double running_sums(int lane, int n, V v, F before) {
+  const int each = (n + 31) / 32, a = min(n, lane * each), b = min(n, a + each);
+  double s = 0.;
+  for (int i = a; i < b; ++i) s += v(i);
+  double scan = s;
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const double up = __shfl_up_sync(0xffffffff, run, o);
-      if (r.lane >= o) run += up;
-    }
-    run -= s;
-    for (int i = a; i < b; ++i) {
-      sh.before[i] = run;
-      run += sh.weight[i];
-    }
+  for (int o = 1; o < 32; o <<= 1) {
+    const double up = __shfl_up_sync(0xffffffff, scan, o);
+    if (lane >= o) scan += up;
   }
-  __syncthreads();
+  const double total = __shfl_sync(0xffffffff, scan, 31);
+  double run = scan - s;
+  for (int i = a; i < b; ++i) {
+    const double one = v(i);
+    before(i, run, one);
+    run += one;
+  }
+  return total;
 }
 
 // Where the value of the sorted candidate i begins.
@@ -221,103 +259,88 @@ __device__ __forceinline__ int first_of_value(const SampleShared& sh, int i) {
   return first;
 }
 
-// The leader's answer from its candidates. `total` +- `error` is the mass of the row that top-p takes a share of, where top-k
-// is off; `complete`: no token below the candidates can be kept.
-__device__ void answer_from_list(SampleRow& r, int n, bool complete, uint32_t low_m, double total, double error,
+// The leader's answer from its candidates, by its first warp. `total` +- `error` is the mass of the row that top-p takes a
+// share of, where top-k is off; `complete`: no token below the candidates can be kept.
+__device__ void answer_from_list(const SampleRow& r, int n, bool complete, uint32_t low_m, double total, double error,
                                  long long* token, float* logprob) {
   SampleShared& sh = r.sh;
-  const uint32_t kth = r.use_k && r.k <= n ? key_part(sh.sorted[r.k - 1]) : 0;
+  const int lane = r.lane;
+  const double all = running_sums(lane, n, [&](int i) { return sh.weight[i]; },
+                                  [&](int i, double run, double) { sh.before[i] = run; });
+  __syncwarp();
   int nk = n;
   if (r.use_k) {
+    const uint32_t kth = r.k <= n ? key_part(sh.sorted[r.k - 1]) : 0;
     nk = 0;
-    for (int i0 = 0; i0 < n; i0 += SG_THREADS) nk += __syncthreads_count(i0 + r.t < n && key_part(sh.sorted[i0 + r.t]) >= kth);
-    total = nk > 0 ? sh.before[nk - 1] + sh.weight[nk - 1] : 0.;
+    for (int i = lane; i < n; i += 32) nk += key_part(sh.sorted[i]) >= kth;
+    nk = __reduce_add_sync(0xffffffff, nk);
+    total = nk < n ? sh.before[nk] : all;
     error = 0.;
   }
   const double share = r.p * total, blur = r.p * error;
   bool unsure = false;
   int kept = 0;
-  for (int i0 = 0; i0 < n; i0 += SG_THREADS) {
-    const int i = i0 + r.t;
-    bool keep = i < nk;
-    if (keep && r.use_p) {
+  for (int i = lane; i < nk; i += 32) {
+    bool keep = !r.use_m || key_part(sh.sorted[i]) >= low_m;
+    if (r.use_p && i > 0) {
       const int first = first_of_value(sh, i);
-      keep = !(sh.before[first] > share);
       unsure |= first > 0 && blur > 0. && fabs(sh.before[first] - share) <= blur;
+      keep &= first == 0 || !(sh.before[first] > share);
     }
-    if (keep && r.use_m) keep = key_part(sh.sorted[i]) >= low_m;
-    kept += __syncthreads_count(keep);
+    kept += keep;
   }
+  kept = __reduce_add_sync(0xffffffff, kept);
   int verdict = kDone;
   if (!complete && r.use_p) {  // is the bound of top-p among the candidates?
-    const double all = sh.before[n - 1] + sh.weight[n - 1];
     unsure |= blur > 0. && fabs(all - share) <= blur;
     if (!(all > share)) verdict = kIncomplete;
   }
-  if (__syncthreads_or(unsure)) verdict = kAmbiguous;
+  if (__any_sync(0xffffffff, unsure)) verdict = kAmbiguous;
   if (verdict == kDone) {
-    const double mass = sh.before[kept - 1] + sh.weight[kept - 1], target = r.draw * mass;
-    const int quarter = r.t & 3;
-    uint32_t best = 0;   // complement of the id: the first at which the running sum in the order of ids is above the target
-    int last = -1;       // and the last with any mass
-#pragma unroll 1
-    for (int i0 = 0; i0 < kept; i0 += SG_THREADS / 4) {
-      const int i = i0 + r.t / 4;
-      const int id = i < kept ? id_part(sh.sorted[i]) : -1;
-      double s = 0.;
-      for (int l = quarter; l < kept; l += 4)
-        if (id_part(sh.sorted[l]) <= id) s += sh.weight[l];
-      s += __shfl_xor_sync(0xffffffff, s, 1);
-      s += __shfl_xor_sync(0xffffffff, s, 2);
-      if (i < kept) {
-        if (s > target) best = max(best, ~(uint32_t)id);
-        if (sh.weight[i] > 0.) last = max(last, id);
-      }
-    }
-    const int at = r.turn;
-    best = __reduce_max_sync(0xffffffff, best);
+    const double mass = kept < n ? sh.before[kept] : all, target = r.draw * mass;
+    int hit = n, last = -1;  // in the order of ids: the first at which the running sum is above the target, the last with mass
+    running_sums(lane, n, [&](int q) { return sh.by_id[q] < kept ? sh.weight[sh.by_id[q]] : 0.; },
+                 [&](int q, double run, double one) {
+                   if (one > 0.) last = q;
+                   if (one > 0. && run + one > target) hit = min(hit, q);
+                 });
+    hit = __reduce_min_sync(0xffffffff, hit);
     last = __reduce_max_sync(0xffffffff, last);
-    if (r.lane == 0) sh.warp_key[at][r.w] = best, sh.scan[r.w] = (uint32_t)last;
-    __syncthreads();
-    best = __reduce_max_sync(0xffffffff, sh.warp_key[at][r.lane & (SG_WARPS - 1)]);
-    last = __reduce_max_sync(0xffffffff, (int)sh.scan[r.lane & (SG_WARPS - 1)]);
-    const int id = best ? (int)~best : last;
-    for (int i = r.t; i < kept; i += SG_THREADS)
-      if (id_part(sh.sorted[i]) == id) {
-        *token = id;
-        if (logprob) *logprob = (float)log(sh.weight[i] / mass);
-      }
+    if (lane == 0) {
+      const int i = sh.by_id[hit < n ? hit : last];
+      *token = id_part(sh.sorted[i]);
+      if (logprob) *logprob = (float)log(sh.weight[i] / mass);
+    }
   }
-  if (r.t == 0) sh.verdict = verdict;
+  if (lane == 0) sh.verdict = verdict;
 }
 
-// The leader's bound of top-p among the candidates of a few steps of the histogram, above which lies `above` +- `error`; `end`:
-// no logit lies below them. The mass of strictly larger logits must be known to lie below or above the share.
+// The leader's bound of top-p, by its first warp, among the candidates of a few steps of the histogram, above which lies
+// `above` +- `error`; `end`: no logit lies below them. The mass of strictly larger logits must be known to lie below or above
+// the share.
 __device__ void bound_from_list(const SampleRow& r, int n, bool end, double above, double error, double share, double blur) {
   SampleShared& sh = r.sh;
   const double doubt = error + blur;
-  bool unsure = false;
+  const double all = above + running_sums(r.lane, n, [&](int i) { return sh.weight[i]; },
+                                          [&](int i, double run, double) { sh.before[i] = run; });
+  __syncwarp();
+  bool unsure = !end && doubt > 0. && fabs(all - share) <= doubt;
   int kept = 0;
-  for (int i0 = 0; i0 < n; i0 += SG_THREADS) {
-    const int i = i0 + r.t;
-    bool keep = i < n;
-    if (keep) {
-      const double larger = above + sh.before[first_of_value(sh, i)];
-      keep = !(larger > share);
-      unsure |= larger > 0. && doubt > 0. && fabs(larger - share) <= doubt;
-    }
-    kept += __syncthreads_count(keep);
+  for (int i = r.lane; i < n; i += 32) {
+    const double larger = above + sh.before[first_of_value(sh, i)];
+    kept += !(larger > share);
+    unsure |= larger > 0. && doubt > 0. && fabs(larger - share) <= doubt;
   }
-  const double all = above + (n > 0 ? sh.before[n - 1] + sh.weight[n - 1] : 0.);
-  unsure |= !end && doubt > 0. && fabs(all - share) <= doubt;
-  unsure = __syncthreads_or(unsure);
-  if (r.t == 0) {
+  kept = __reduce_add_sync(0xffffffff, kept);
+  unsure = __any_sync(0xffffffff, unsure);
+  if (r.lane == 0) {
     sh.verdict = unsure ? kAmbiguous : (kept == 0 || (!end && !(all > share)) ? kIncomplete : kDone);
     sh.low = kept > 0 ? key_part(sh.sorted[kept - 1]) : 0;
   }
 }
 
-template <typename T>
+// HELD: the CTA's part of the row lies in shared memory.
+template <typename T, bool HELD>
 __global__ void __launch_bounds__(SG_THREADS, 2) sample_given_kernel(const SampleGivenArgs a) {
   constexpr int E = LogitType<T>::E;
   extern __shared__ uint4 held[];  // vector i of thread t at i * 512 + t
@@ -333,18 +356,35 @@ __global__ void __launch_bounds__(SG_THREADS, 2) sample_given_kernel(const Sampl
   const int mine = max(0, min(chunk / 32, (w1 - w0 - lane + 31) / 32));  // vectors of this thread
   float top = -INFINITY;
   bool nan = false;
-  {
+#pragma unroll 1
+  for (int i0 = 0; i0 < mine; i0 += SG_VECS) {
     uint4 u[SG_VECS];
 #pragma unroll
-    for (int i = 0; i < SG_VECS; ++i) u[i] = i < mine ? vecs.load(w0 + i * 32 + lane) : vec_neg_inf<T>();
+    for (int i = 0; i < SG_VECS; ++i) u[i] = i0 + i < mine ? vecs.load(w0 + (i0 + i) * 32 + lane) : vec_neg_inf<T>();
 #pragma unroll
     for (int i = 0; i < SG_VECS; ++i) {
-      if (i < mine) held[i * SG_THREADS + t] = u[i];
+      if (HELD && i0 + i < mine) held[(i0 + i) * SG_THREADS + t] = u[i];
       const float most = vec_max<T>(u[i]);
       nan |= most != most;
       top = fmaxf(top, most);
     }
   }
+  const auto vec = [&](int i) { return HELD ? held[i * SG_THREADS + t] : vecs.load(w0 + i * 32 + lane); };
+  // f(vector, its number) over this thread's vectors, several in flight
+  const auto for_vecs = [&](auto f) {
+    constexpr int kBatch = HELD ? 2 : 4;
+    int i = 0;
+#pragma unroll 1
+    for (; i + kBatch <= mine; i += kBatch) {
+      uint4 u[kBatch];
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) u[j] = vec(i + j);
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) f(u[j], i + j);
+    }
+#pragma unroll 1
+    for (; i < mine; ++i) f(vec(i), i);
+  };
   SampleRow r{sh, cs, rank, t, lane, w};
   const float temperature = a.temperature[row];
   const bool greedy = !(temperature > 0.f);
@@ -363,37 +403,33 @@ __global__ void __launch_bounds__(SG_THREADS, 2) sample_given_kernel(const Sampl
   SampleShared* lead = &sh;
   if (cs > 1) lead = cg::this_cluster().map_shared_rank(&sh, 0);
   if (t == 0) sh.n = 0;
-  const float c = (float)(1.4426950408889634 / r.T64);
+  r.c64 = 1.4426950408889634 / r.T64;
+  const float c = (float)r.c64;
   r.max_x = of_key(r.max_key(key_of(nan ? of_key(0xFFFFFFFFu) : top)));
 
   // f(element, id) over this thread's elements
   const auto each = [&](auto f) {
-#pragma unroll 1
-    for (int i = 0; i < mine; ++i) {
+    for_vecs([&](const uint4& u, int i) {
       const int at = vecs.first(w0 + i * 32 + lane);
       float x[E];
-      vec_floats<T>(held[i * SG_THREADS + t], x);
+      vec_floats<T>(u, x);
 #pragma unroll
       for (int e = 0; e < E; ++e)
         if (at + e >= 0 && at + e < a.V) f(x[e], at + e);
-    }
+    });
   };
   // Mass of a vector's logits from `low` on. In 32 bits each exponential is within 2^-22 of itself and 3 |t| 2^-24 ln 2 for
   // the roundings of t = (x - max) c, and eight of them are added in a tree.
-  const auto vec_mass = [&](int i, bool precise, float low) -> double {
-    const uint4 u = held[i * SG_THREADS + t];
-    if (precise) {
-      float x[E];
-      vec_floats<T>(u, x);
-      double s = 0.;
-#pragma unroll 1
-      for (int e = 0; e < E; ++e)
-        if (x[e] >= low) s += r.weight(x[e]);
-      return s;
-    }
-    const Pair ref2(-r.max_x, -r.max_x), c2(c, c);
+  const Pair ref2(-r.max_x, -r.max_x), c2(c, c);
+  const auto vec_mass = [&](const uint4& u, bool precise, float low) -> double {
     float x[E];
     vec_floats<T>(u, x);
+    if (precise) {
+      double s = 0.;
+#pragma unroll
+      for (int e = 0; e < E; ++e) s += x[e] >= low ? r.weight(x[e]) : 0.;
+      return s;
+    }
     Pair q[E / 2];
 #pragma unroll
     for (int e = 0; e < E / 2; ++e)
@@ -410,8 +446,12 @@ __global__ void __launch_bounds__(SG_THREADS, 2) sample_given_kernel(const Sampl
   const float log_v = log2f((float)a.V);
   const auto masses = [&](bool precise, float low) {
     double s = 0.;
+    if (precise) {
 #pragma unroll 1
-    for (int i = 0; i < mine; ++i) s += vec_mass(i, precise, low);
+      for (int i = 0; i < mine; ++i) s += vec_mass(vec(i), true, low);
+    } else {
+      for_vecs([&](const uint4& u, int) { s += vec_mass(u, false, low); });
+    }
     const SampleRow::Part part = r.sum(s);
     error = precise ? 0. : part.total * (4.5e-7 + 1.3e-7 * fmaxf(log_v - log2f((float)part.total), 0.f));
     return part;
@@ -432,14 +472,23 @@ __global__ void __launch_bounds__(SG_THREADS, 2) sample_given_kernel(const Sampl
         int at_i = 0, last_i = 0;
         double at_before = -1., last_before = before, s;
 #pragma unroll 1
-        for (int i = 0; i < chunk / 32; ++i) {
-          s = SampleRow::warp_add(i < mine ? vec_mass(i, precise, low) : 0.);
-          if (s > 0.) last_i = i, last_before = before;
-          if (at_before < 0. && before + s > target) at_i = i, at_before = before;
-          before += s;
+        for (int i0 = 0; i0 < chunk / 32; i0 += 4) {
+          double part4[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) part4[i] = i0 + i < mine ? vec_mass(vec(i0 + i), precise, low) : 0.;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) part4[i] = SampleRow::warp_add(part4[i]);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            s = part4[i];
+            if (s > 0.) last_i = i0 + i, last_before = before;
+            if (at_before < 0. && before + s > target) at_i = i0 + i, at_before = before;
+            before += s;
+          }
+          if (at_before >= 0.) break;
         }
         if (at_before < 0.) at_i = last_i, at_before = last_before;
-        s = at_i < mine ? vec_mass(at_i, precise, low) : 0.;
+        s = at_i < mine ? vec_mass(vec(at_i), precise, low) : 0.;
         double scan = s;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -453,7 +502,7 @@ __global__ void __launch_bounds__(SG_THREADS, 2) sample_given_kernel(const Sampl
           double run = at_before + (scan - s), c0 = run, c1 = run;
           int id = -1;
           float chosen = 0.f, x[E];
-          vec_floats<T>(held[at_i * SG_THREADS + t], x);
+          vec_floats<T>(vec(at_i), x);
           const int at = vecs.first(w0 + at_i * 32 + lane);
 #pragma unroll
           for (int e = 0; e < E; ++e) {
@@ -481,22 +530,20 @@ __global__ void __launch_bounds__(SG_THREADS, 2) sample_given_kernel(const Sampl
       if (verdict == kDone) return;
     }
   };
-  // Candidates: logits for which `in` holds, into the leader's list.
+  // Candidates: logits from `low` on for which `in` holds, into the leader's list.
   const auto gather = [&](float low, auto in) {
-#pragma unroll 1
-    for (int i = 0; i < mine; ++i) {
-      const uint4 u = held[i * SG_THREADS + t];
-      if (!(vec_max<T>(u) >= low)) continue;
+    for_vecs([&](const uint4& u, int i) {
+      if (!(vec_max<T>(u) >= low)) return;
       const int at = vecs.first(w0 + i * 32 + lane);
       float x[E];
       vec_floats<T>(u, x);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        if (!(x[e] >= low) || !in(x[e]) || at + e < 0 || at + e >= a.V) continue;
+        if (!(x[e] >= low) || !in(x[e])) continue;
         const int slot = atomicAdd(&lead->n, 1);
         if (slot < SG_CAP) lead->list[slot] = (unsigned long long)key_of(x[e]) << 32 | (uint32_t)~(at + e);
       }
-    }
+    });
     r.sync();
     return lead->n;
   };
@@ -578,11 +625,13 @@ __global__ void __launch_bounds__(SG_THREADS, 2) sample_given_kernel(const Sampl
       bool complete = by_k || bound == 0;
       if (r.use_m && !(by_k && r.use_p) && low_m >= bound) bound = low_m, complete = true;
       // below all numbers: -inf and the padding have no mass
-      const int n = gather(bound <= key_of(-INFINITY) ? -3.4028235e38f : of_key(bound), [](float) { return true; });
+      const float reach = bound <= key_of(-INFINITY) ? -3.4028235e38f : of_key(bound);
+      const bool hopeless = !complete && masses(false, reach).total < 0.999 * r.p * total;
+      const int n = hopeless ? SG_CAP + 1 : gather(reach, [](float) { return true; });
       if (n <= SG_CAP) {
         if (rank == 0) order_list(r, n);
         for (int precise = 0;; ++precise) {
-          if (rank == 0) answer_from_list(r, n, complete, low_m, total, total_error, token, logprob);
+          if (rank == 0 && w == 0) answer_from_list(r, n, complete, low_m, total, total_error, token, logprob);
           r.sync();
           const int verdict = lead->verdict;
           r.sync();
@@ -598,7 +647,12 @@ __global__ void __launch_bounds__(SG_THREADS, 2) sample_given_kernel(const Sampl
 
     // Many tokens stay. A histogram of the logits over equal steps down from the largest.
     float least = INFINITY;
-    each([&](float x, int) { if (x > -INFINITY) least = fminf(least, x); });
+    for_vecs([&](const uint4& u, int) {
+      float x[E];
+      vec_floats<T>(u, x);
+#pragma unroll
+      for (int e = 0; e < E; ++e) least = fminf(least, x[e] > -INFINITY ? x[e] : least);
+    });
     least = of_key(r.min_key(key_of(least)));
     float range = r.max_x - least;
     if (r.use_p && !r.use_k) range = fminf(range, 24.f * (float)r.T64);
@@ -612,7 +666,13 @@ __global__ void __launch_bounds__(SG_THREADS, 2) sample_given_kernel(const Sampl
 #pragma unroll
       for (int i = 0; i < kEach; ++i) sh.bins[t * kEach + i] = 0;
       __syncthreads();
-      each([&](float x, int) { if (x > -INFINITY) atomicAdd(&sh.bins[bin_of(x)], 1u); });
+      for_vecs([&](const uint4& u, int) {
+        float x[E];
+        vec_floats<T>(u, x);
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+          if (x[e] > -INFINITY) atomicAdd(&sh.bins[bin_of(x[e])], 1u);
+      });
       r.sync();
 #pragma unroll
       for (int i = 0; i < kEach; ++i) count[i] = 0;
@@ -739,7 +799,7 @@ __global__ void __launch_bounds__(SG_THREADS, 2) sample_given_kernel(const Sampl
           each([&](float x, int) { if (x > -INFINITY && bin_of(x) < first) edge = fminf(edge, x); });
           edge = of_key(r.min_key(key_of(edge)));
           const double above = edge < INFINITY ? masses(precise, fmaxf(edge, from(kth))).total : (error = 0., 0.);
-          if (rank == 0) bound_from_list(r, n, last == SG_BINS - 1, above, error, share, blur);
+          if (rank == 0 && w == 0) bound_from_list(r, n, last == SG_BINS - 1, above, error, share, blur);
           r.sync();
           const int verdict = lead->verdict;
           cut = lead->low;
@@ -766,15 +826,19 @@ __global__ void __launch_bounds__(SG_THREADS, 2) sample_given_kernel(const Sampl
   if (cs > 1) cg::this_cluster().sync();  // no CTA leaves while others read its memory
 }
 
-template <typename T>
-void sample_given_launch(const SampleGivenArgs& a, int smem, cudaStream_t s) {
-  auto* kernel = sample_given_kernel<T>;
+template <typename T, bool HELD>
+void sample_given_launch(const SampleGivenArgs& a, int smem, int device, cudaStream_t s) {
+  auto* kernel = sample_given_kernel<T, HELD>;
+  static bool ready[64] = {};  // per device
+  if (device < 0 || device >= 64 || !ready[device]) {
+    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SG_VECS * SG_THREADS * 16);
+    if (device >= 0 && device < 64) ready[device] = true;
+  }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)a.rows * a.cluster);
   cfg.blockDim = dim3(SG_THREADS);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
-  cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SG_VECS * SG_THREADS * 16);
   cudaLaunchAttribute at[2]{};
   at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[0].val.programmaticStreamSerializationAllowed = 1;
@@ -783,20 +847,23 @@ void sample_given_launch(const SampleGivenArgs& a, int smem, cudaStream_t s) {
   at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
   cfg.attrs = at;
   cfg.numAttrs = a.cluster > 1 ? 2 : 1;
-  if (a.cluster > 8) cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
   note_launch();
   cudaLaunchKernelEx(&cfg, kernel, a);
 }
 
 template <typename T>
-void sample_given_sized(SampleGivenArgs a, cudaStream_t s) {
+void sample_given_sized(SampleGivenArgs a, int device, cudaStream_t s) {
   constexpr int E = LogitType<T>::E;
   const int vecs = (a.V + E - 1) / E + 1;  // one more where a row starts off the grid
+  const int sms = astrai_host::num_sms(device);
+  const char* env = getenv("SG_CS");
   int cs = 1;
-  while ((vecs + cs - 1) / cs > SG_THREADS * SG_VECS) cs *= 2;
+  while (cs < SG_MAX_CLUSTER && (long long)a.rows * cs * 2 <= sms && vecs >= cs * 2 * SG_THREADS) cs *= 2;
+  if (env) cs = atoi(env);
   a.cluster = cs;
-  const int per = (vecs + cs - 1) / cs;
-  sample_given_launch<T>(a, (per + SG_THREADS - 1) / SG_THREADS * SG_THREADS * 16, s);
+  const int each = ((vecs + cs - 1) / cs + SG_THREADS - 1) / SG_THREADS;  // vectors of a thread
+  if (each <= SG_VECS) sample_given_launch<T, true>(a, each * SG_THREADS * 16, device, s);
+  else sample_given_launch<T, false>(a, 0, device, s);
 }
 
 }  // namespace astrai
@@ -804,16 +871,13 @@ void sample_given_sized(SampleGivenArgs a, cudaStream_t s) {
 namespace astrai_host {
 using namespace astrai;
 
-// longest row for elements of this size
-int sample_given_max_vocab(int elem) { return SG_MAX_CLUSTER * SG_THREADS * SG_VECS * (16 / elem) - 16 / elem; }
-
 void sample_given(const void* x, long long ldx, int rows, int V, const void* uniform, bool uniform64,
                   const float* temperature, const int* top_k, const float* top_p, const float* min_p, long long* token,
-                  float* logprob, int dtype, cudaStream_t s) {
+                  float* logprob, int dtype, int device, cudaStream_t s) {
   const SampleGivenArgs a{x, ldx, rows, V, 1, uniform, uniform64, temperature, top_k, top_p, min_p, token, logprob};
-  if (dtype == 0) sample_given_sized<__nv_bfloat16>(a, s);
-  else if (dtype == 1) sample_given_sized<__half>(a, s);
-  else sample_given_sized<float>(a, s);
+  if (dtype == 0) sample_given_sized<__nv_bfloat16>(a, device, s);
+  else if (dtype == 1) sample_given_sized<__half>(a, device, s);
+  else sample_given_sized<float>(a, device, s);
 }
 
 }  // namespace astrai_host

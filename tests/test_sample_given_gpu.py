@@ -63,10 +63,10 @@ SETTINGS = [dict(), dict(t=0.0), dict(t=0.7, k=50, p=0.95), dict(k=1), dict(k=40
 
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
-@pytest.mark.parametrize("V", [1, 2, 9, 100, 1000, 1025, 4097, 32000, 32003, 50021, 131072])
+@pytest.mark.parametrize("V", [1, 2, 9, 100, 1000, 1025, 4097, 32000, 32003, 50021, 131072, 300001])
 def test_sizes_and_settings(dtype, V):
     x, u = _logits(8, V, dtype, V)
-    for s in SETTINGS if V < 40000 else SETTINGS[::2]:
+    for s in SETTINGS if V < 40000 else SETTINGS[V % 3::3]:
         _check(x, u, **s)
 
 
@@ -252,7 +252,5 @@ def test_refusals():
     for bad in (dict(logits=x.double()), dict(uniform=u.half()), dict(uniform=u.cpu())):
         with pytest.raises(RuntimeError):
             sample_given(**{"logits": x, "uniform": u, **bad})
-    with pytest.raises(ValueError, match="too large"):
-        sample_given(torch.zeros(1, 300000, device="cuda"), u[:1])
     assert sample_given(x[:0], u[:0]).shape == (0,)
     assert not sample_given(x.requires_grad_(), u, return_logprobs=True)[1].requires_grad
