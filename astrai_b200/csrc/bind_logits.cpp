@@ -98,7 +98,7 @@ std::pair<at::Tensor, OptTensor> sample_given(const at::Tensor& logits, const at
   TORCH_CHECK_VALUE(logits.dim() == 2 && logits.size(1) >= 1, "sample_given: logits must be [batch, vocab]");
   const int64_t rows = logits.size(0), V = logits.size(1);
   const int code = dtype_code(logits, "sample_given: logits");
-  TORCH_CHECK_VALUE(V < (1LL << 30), "sample_given: vocabulary too large");
+  TORCH_CHECK_VALUE(V <= (1LL << 22), "sample_given: a vocabulary of at most 2^22");
   TORCH_CHECK_VALUE(rows < (1LL << 27), "sample_given: too many rows");
   TORCH_CHECK(uniform_in.scalar_type() == at::kFloat || uniform_in.scalar_type() == at::kDouble,
               "sample_given: uniform must be float32 or float64, got ", uniform_in.scalar_type());

@@ -12,34 +12,32 @@
 // 64 bits. Sums over a whole row are taken in 32 bits first, with a bound on their error; a row whose answer lies within it
 // is summed again in 64 bits.
 //
-// A CTA of 512 threads takes a row, or where the rows are too few for the SMs a cluster of CTAs does. Up to 64 KB of logits
-// stay in the CTA's shared memory between the passes over them, more than that come from L2 again.
-// The bound that gathers the candidates is the one of the top logits: the smallest, over the row's warps, of each warp's j-th
-// largest thread maximum. Where top-p reaches below them (flat rows) or k is large, a histogram of the logits over 4096 equal
-// steps shows in which steps the bound must lie, and the few logits there are ordered and decided exactly.
-#include <cooperative_groups.h>
-
-#include <cstdlib>
-
+// A CTA of 512 threads takes a row, two on an SM. Logits that fit stay in its shared memory between the passes over them,
+// others come from L2 again. (A cluster of two to eight CTAs for a row, or 1024 threads, took as long or longer: 64 rows of
+// 32000 with k = 50 16.6 and 21.8 us against 15.4 and 13.9; the barriers cost what the shorter passes save.) The bound that gathers the candidates is the one of
+// the top logits: the smallest, over the warps, of each warp's j-th largest thread maximum. Where top-p reaches below them
+// (flat rows) or k is large, a histogram over 4096 equal steps of the logits shows in which steps the bound must lie, and the
+// few logits there are ordered and decided exactly.
+//
+// A row takes each step once, so that the time to fetch instructions counts: inlined into each other, the passes were 430 KB
+// of code, a third of all stalls waited for it (64 rows of 32000, k = 50: 15 us), hence functions that are called.
 #include "launch.cuh"
 #include "logits.cuh"
 
 namespace astrai {
 
-namespace cg = cooperative_groups;
-
 constexpr int SG_THREADS = 512;
-constexpr int SG_WARPS = SG_THREADS / 32;
-constexpr int SG_VECS = 8;  // 16-byte vectors of a thread
+constexpr int SG_VECS = 8;      // 16-byte vectors that a thread loads at once
 constexpr int SG_LIST_K = 256;  // top-k up to here, and the largest logits looked at for top-p, go by the list
-constexpr int SG_CAP = 1024;
+constexpr int SG_CAP = 2 * SG_THREADS;  // candidates
 constexpr int SG_BINS = 4096;
-constexpr int SG_MAX_CLUSTER = 8;
+constexpr int SG_GROUPS = 8;    // of a thread's vectors: each with its maximum
+constexpr uint32_t kLowest = 0x00800000u;  // the key of the lowest finite number
 
 struct SampleGivenArgs {
   const void* x;
   long long ldx;
-  int rows, V, cluster;
+  int rows, V;
   const void* uniform;  // [rows] fp32 or fp64
   int uniform64;
   const float* temperature;  // [rows]
@@ -50,386 +48,201 @@ struct SampleGivenArgs {
   float* logprob;    // [rows] or null
 };
 
-// 2^t for t <= 0 in 64 bits, within 2^-46 of itself (below 2^-1000: zero): e^z = sum z^n / n! at |z| <= ln 2 / 2, whose 13th
-// term is below 2^-53, times a power of two.
-__device__ __forceinline__ double exp2_64(double t) {
+// 2^(k / 16), in shared memory: a warp's 32 reads of these 16 words meet no bank twice.
+struct Powers {
+  double at[16];
+};
+// 2^(t / 16) for N values t <= 0 in 64 bits, within 2^-42 of themselves (below 2^-1000: zero): a power of two, one of `pow`
+// and e^z = sum z^n / n! at |z| <= ln 2 / 32, whose sixth term is below 2^-42. Step by step for all of them, as each step
+// waits for the last.
+template <int N>
+__device__ __forceinline__ void exp2_16th(double (&t)[N], const Powers& pow) {
   constexpr double kRound = 6755399441055744.;  // 1.5 * 2^52: adding it rounds to a whole number
-  const double n = t + kRound, z = (t - (n - kRound)) * 0.6931471805599453;
-  double e = 1. / 479001600.;
-  e = fma(e, z, 1. / 39916800.);
-  e = fma(e, z, 1. / 3628800.);
-  e = fma(e, z, 1. / 362880.);
-  e = fma(e, z, 1. / 40320.);
-  e = fma(e, z, 1. / 5040.);
-  e = fma(e, z, 1. / 720.);
-  e = fma(e, z, 1. / 120.);
-  e = fma(e, z, 1. / 24.);
-  e = fma(e, z, 1. / 6.);
-  e = fma(e, z, 0.5);
-  e = fma(e, z, 1.);
-  e = fma(e, z, 1.);
-  return t > -1000. ? __hiloint2double(__double2hiint(e) + (__double2loint(n) << 20), __double2loint(e)) : 0.;
+  constexpr double a = 0.6931471805599453 / 16.;
+  constexpr double kTerms[] = {a * a * a * a / 24., a * a * a / 6., a * a / 2., a, 1.};
+  int n[N], live[N];
+  double e[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    live[i] = t[i] > -16000. ? -1 : 0;
+    const double whole = t[i] + kRound;
+    n[i] = __double2loint(whole);
+    t[i] -= whole - kRound;
+    e[i] = a * a * a * a * a / 120.;
+  }
+#pragma unroll
+  for (const double term : kTerms)
+#pragma unroll
+    for (int i = 0; i < N; ++i) e[i] = fma(e[i], t[i], term);
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    e[i] *= pow.at[n[i] & 15];
+    t[i] = __hiloint2double((__double2hiint(e[i]) + (n[i] >> 4 << 20)) & live[i], __double2loint(e[i]) & live[i]);
+  }
+}
+
+// The least key in lo .. hi for which `reaches` holds, in all lanes: it holds from some key on, at hi at the latest.
+template <typename F>
+__device__ __forceinline__ uint32_t least_key(int lane, uint32_t lo, uint32_t hi, F reaches) {
+#pragma unroll 1
+  while (lo < hi) {
+    const uint32_t step = (hi - lo + 30) / 31;  // the last lane takes hi
+    const int i = __ffs(__ballot_sync(0xffffffff, reaches(min(lo + lane * step, hi)))) - 1;
+    hi = min(lo + i * step, hi);
+    if (i == 0) break;
+    lo += (i - 1) * step + 1;
+  }
+  return hi;
 }
 
 enum Verdict { kDone = 0, kAmbiguous = 1, kIncomplete = 2 };
 
 struct SampleShared {
-  unsigned long long list[SG_CAP];    // candidates: key, then the id's complement
-  unsigned long long sorted[SG_CAP];  // greatest first
-  uint16_t by_id[SG_CAP];             // places among the sorted ones, in the order of ids
+  // candidates in no order; some of their numbers in descending order
+  uint32_t key[SG_CAP], id[SG_CAP], sorted[SG_CAP];
   union {
-    struct {
-      double weight[SG_CAP];  // of the sorted ones
-      double before[SG_CAP];  // mass of those before it
-    };
+    double before[SG_CAP];     // mass before a sorted one
+    uint32_t swap[2][SG_CAP];  // for sorting
     uint32_t bins[SG_BINS];
   };
-  double warp_sum[2][SG_WARPS];  // two of each: a reduction writes one while the last one's may still be read
-  double sums[2];                // of this CTA
-  uint32_t warp_key[2][SG_WARPS], key[2];
-  int n;         // the leader's: candidates of the row
-  int verdict;   // the leader's
-  uint32_t low;  // the least key that min-p keeps; the leader's: the least key that the row keeps
-  uint32_t scan[SG_WARPS];
-  double scan64[SG_WARPS];
-  int found;
-  uint32_t found_above;
+  double warp_sum[SG_THREADS / 32];
+  double group_sum[SG_THREADS / 32][SG_GROUPS];  // a warp's mass by groups of vectors
+  uint32_t warp_key[SG_THREADS / 32];
+  // the row and its settings
+  const void* row;
+  int V, chunk, group;  // chunk: vectors of a warp, one after another, so that sums over warps are sums over ids
+  float max_x, c;       // c = log2(e) / T
+  double T64, c64, p, m, draw;  // c64 = 16 log2(e) / T
+  Powers pow;
+  int k;
+  bool use_k, use_p, use_m;
+  long long* token;
+  float* logprob;
+  // results
+  int n;           // candidates
+  uint32_t low;    // the least key that min-p keeps, later of a bound
+  int hit, last;
+  int bin;
+  float above;     // the histogram's sum before `bin`
 };
 
-// What the row's settings say, and the reductions over warps, CTAs and the cluster: their results are the same in all
-// threads of the row.
-struct SampleRow {
-  SampleShared& sh;
-  int cs, rank, t, lane, w;
-  float max_x;
-  double T64, c64, p, m, draw;  // c64: log2(e) / T
-  bool use_k, use_p, use_m;
-  int k;
-  int turn = 0;
+template <typename T, bool HELD>
+struct Sampler {
+  static constexpr int E = LogitType<T>::E, NT = SG_THREADS, kWarps = NT / 32;
 
-  __device__ void sync() const {
-    if (cs > 1) cg::this_cluster().sync();
-    else __syncthreads();
+  static __device__ __forceinline__ SampleShared& shared() {
+    extern __shared__ __align__(16) unsigned char sample_smem[];
+    return *reinterpret_cast<SampleShared*>(sample_smem);
+  }
+  // the held vectors: i of thread t at i * NT + t; if they are not held, the maxima of their groups
+  static __device__ __forceinline__ uint4* held() {
+    extern __shared__ __align__(16) unsigned char sample_smem[];
+    return reinterpret_cast<uint4*>(sample_smem + (sizeof(SampleShared) + 15) / 16 * 16);
+  }
+  static __device__ __forceinline__ float* tops() { return reinterpret_cast<float*>(held()); }
+
+  // This thread's vectors: w0 + i * 32 + lane, i < mine.
+  struct Mine {
+    RowVecs<T> vecs;
+    int w0, mine;
+    __device__ Mine(const SampleShared& sh) : vecs(static_cast<const T*>(sh.row), sh.V) {
+      const int t = threadIdx.x;
+      w0 = t / 32 * sh.chunk;
+      mine = max(0, min(sh.chunk / 32, (min(w0 + sh.chunk, vecs.n) - w0 - (t & 31) + 31) / 32));
+    }
+    __device__ __forceinline__ int first(int i) const { return vecs.first(w0 + i * 32 + (threadIdx.x & 31)); }
+    __device__ __forceinline__ uint4 vec(int i) const {
+      if (i >= mine) return vec_neg_inf<T>();
+      return HELD ? held()[i * NT + threadIdx.x] : vecs.load(w0 + i * 32 + (threadIdx.x & 31));
+    }
+  };
+  // f(vector, its number) over this thread's vectors of the groups that reach `low`, four in flight (with some behind the
+  // last that read as -inf); g(group) after each
+  template <typename F, typename G>
+  static __device__ __forceinline__ void for_vecs(const SampleShared& sh, const Mine& me, float low, F f, G g) {
+#pragma unroll 1
+    for (int i0 = 0, at = 0; i0 < sh.chunk / 32; i0 += sh.group, ++at) {
+      const int end = min(i0 + sh.group, me.mine);
+      if (i0 < end && tops()[at * NT + threadIdx.x + (HELD ? sh.chunk / 32 * NT * 4 : 0)] >= low) {
+#pragma unroll 1
+        for (int i = i0; i < end; i += 4) {
+          uint4 u[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) u[j] = me.vec(i + j);
+#pragma unroll
+          for (int j = 0; j < 4; ++j) f(u[j], i + j);
+        }
+      }
+      g(at);
+    }
   }
   template <typename F>
-  __device__ uint32_t reduce(uint32_t v, F f) {
-    const int at = turn ^= 1;
+  static __device__ __forceinline__ void for_vecs(const SampleShared& sh, const Mine& me, float low, F f) {
+    for_vecs(sh, me, low, f, [](int) {});
+  }
+
+  // ---------------------------------------------------------------- reductions: the same result in all threads
+  template <typename F>
+  static __device__ __forceinline__ uint32_t reduce(uint32_t v, uint32_t none, F f) {
+    SampleShared& sh = shared();
     v = f(v);
-    if (lane == 0) sh.warp_key[at][w] = v;
     __syncthreads();
-    v = f(sh.warp_key[at][lane & (SG_WARPS - 1)]);
-    if (cs > 1) {
-      if (t == 0) sh.key[at] = v;
-      cg::this_cluster().sync();
-      v = f(*cg::this_cluster().map_shared_rank(&sh.key[at], lane < cs ? lane : 0));
-    }
-    return v;
-  }
-  __device__ uint32_t max_key(uint32_t v) {
-    return reduce(v, [](uint32_t x) { return __reduce_max_sync(0xffffffff, x); });
-  }
-  __device__ uint32_t min_key(uint32_t v) {
-    return reduce(v, [](uint32_t x) { return __reduce_min_sync(0xffffffff, x); });
-  }
-  __device__ int count(int n) {
-    const int at = turn ^= 1;
-    n = __reduce_add_sync(0xffffffff, n);
-    if (lane == 0) sh.warp_key[at][w] = n;
+    if ((threadIdx.x & 31) == 0) sh.warp_key[threadIdx.x / 32] = v;
     __syncthreads();
-    n = __reduce_add_sync(0xffffffff, lane < SG_WARPS ? (int)sh.warp_key[at][lane] : 0);
-    if (cs > 1) {
-      if (t == 0) sh.key[at] = n;
-      cg::this_cluster().sync();
-      n = __reduce_add_sync(0xffffffff, lane < cs ? (int)*cg::this_cluster().map_shared_rank(&sh.key[at], lane) : 0);
-    }
-    return n;
+    return f((threadIdx.x & 31) < kWarps ? sh.warp_key[threadIdx.x & 31] : none);
   }
-  __device__ static double warp_add(double v) {
+  static __device__ __noinline__ uint32_t max_of(uint32_t v) {
+    return reduce(v, 0, [](uint32_t x) { return __reduce_max_sync(0xffffffff, x); });
+  }
+  static __device__ __noinline__ uint32_t min_of(uint32_t v) { return ~max_of(~v); }
+  static __device__ __noinline__ uint32_t sum_of(uint32_t v) {
+    return reduce(v, 0, [](uint32_t x) { return __reduce_add_sync(0xffffffff, x); });
+  }
+  static __device__ __forceinline__ double warp_add(double v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffff, v, o);
     return v;
   }
-  // A sum and its parts: before this CTA, in it, and whether no CTA after it has any; in this warp and the warps before it in
-  // the CTA, and whether no warp after it has any.
-  struct Part {
-    double total, before, here, warp_before, warp;
-    bool last, warp_last;
-  };
-  __device__ Part sum(double s) {
-    const int at = turn ^= 1;
-    Part part;
-    part.warp = s = warp_add(s);
-    if (lane == 0) sh.warp_sum[at][w] = s;
+  static __device__ __forceinline__ double lanes_before(double v) {  // running sum over the lanes, v included
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const double up = __shfl_up_sync(0xffffffff, v, o);
+      if ((threadIdx.x & 31) >= o) v += up;
+    }
+    return v;
+  }
+  // The sum over the threads before this one, and over all. The warps' sums stay in sh.warp_sum.
+  static __device__ __noinline__ double2 scan(double s) {
+    SampleShared& sh = shared();
+    const int lane = threadIdx.x & 31, w = threadIdx.x / 32;
+    const double run = lanes_before(s);
     __syncthreads();
-    const double theirs = sh.warp_sum[at][lane & (SG_WARPS - 1)];
-    double scan = theirs;
-#pragma unroll
-    for (int o = 1; o < SG_WARPS; o <<= 1) {
-      const double up = __shfl_up_sync(0xffffffff, scan, o, SG_WARPS);
-      if ((lane & (SG_WARPS - 1)) >= o) scan += up;
-    }
-    part.total = part.here = __shfl_sync(0xffffffff, scan, SG_WARPS - 1);
-    part.warp_before = __shfl_sync(0xffffffff, scan, max(w - 1, 0));
-    if (w == 0) part.warp_before = 0.;
-    part.warp_last = (__ballot_sync(0xffffffff, theirs > 0.) & ((1u << SG_WARPS) - 1)) >> (w + 1) == 0;
-    part.before = 0.;
-    part.last = true;
-    if (cs > 1) {
-      if (t == 0) sh.sums[at] = part.here;
-      cg::this_cluster().sync();
-      const double others = lane < cs ? *cg::this_cluster().map_shared_rank(&sh.sums[at], lane) : 0.;
-      scan = others;
-#pragma unroll
-      for (int o = 1; o < SG_MAX_CLUSTER; o <<= 1) {
-        const double up = __shfl_up_sync(0xffffffff, scan, o);
-        if (lane >= o) scan += up;
-      }
-      part.total = __shfl_sync(0xffffffff, scan, SG_MAX_CLUSTER - 1);
-      part.before = __shfl_sync(0xffffffff, scan, max(rank - 1, 0));
-      if (rank == 0) part.before = 0.;
-      part.last = __ballot_sync(0xffffffff, others > 0.) >> (rank + 1) == 0;
-    }
-    return part;
+    if (lane == 31) sh.warp_sum[w] = run;
+    __syncthreads();
+    const double warps = lanes_before(lane < kWarps ? sh.warp_sum[lane] : 0.);
+    const double base = __shfl_sync(0xffffffff, warps, max(w - 1, 0));
+    return make_double2((w > 0 ? base : 0.) + (run - s), __shfl_sync(0xffffffff, warps, 31));
   }
-  __device__ double weight(float x) const { return exp2_64(((double)x - (double)max_x) * c64); }
-};
 
-__device__ __forceinline__ uint32_t key_part(unsigned long long e) { return (uint32_t)(e >> 32); }
-__device__ __forceinline__ int id_part(unsigned long long e) { return (int)~(uint32_t)e; }
-
-// The leader's candidates in order of value, their weights, and their places in the order of ids.
-__device__ void order_list(const SampleRow& r, int n) {
-  SampleShared& sh = r.sh;
-  const int quarter = r.t & 3;
-#pragma unroll 1
-  for (int i0 = 0; i0 < n; i0 += SG_THREADS / 4) {
-    const int i = i0 + r.t / 4;
-    const unsigned long long mine = i < n ? sh.list[i] : 0;
-    int above = 0, earlier = 0;
-#pragma unroll 4
-    for (int l = quarter; l < n; l += 4) {
-      const unsigned long long other = sh.list[l];
-      above += other > mine;
-      earlier += (uint32_t)other > (uint32_t)mine;  // complements of ids
-    }
-    above += __shfl_xor_sync(0xffffffff, above, 1);
-    above += __shfl_xor_sync(0xffffffff, above, 2);
-    earlier += __shfl_xor_sync(0xffffffff, earlier, 1);
-    earlier += __shfl_xor_sync(0xffffffff, earlier, 2);
-    if (i < n && quarter == 0) {
-      sh.sorted[above] = mine;
-      sh.weight[above] = r.weight(of_key(key_part(mine)));
-      sh.by_id[earlier] = (uint16_t)above;
-    }
+  // ---------------------------------------------------------------- passes over the row
+  static __device__ __noinline__ double weight(float x) {
+    const SampleShared& sh = shared();
+    double t[1] = {((double)x - (double)sh.max_x) * sh.c64};
+    exp2_16th(t, sh.pow);
+    return t[0];
   }
-  __syncthreads();
-}
-
-// For warp 0 of the leader: the running sums of v(i), i < n, each lane its own part of them; before(i, sum before i, v(i)).
-template <typename V, typename F>
-__device__ __forceinline__ double running_sums(int lane, int n, V v, F before) {
-  const int each = (n + 31) / 32, a = min(n, lane * each), b = min(n, a + each);
-  double s = 0.;
-  for (int i = a; i < b; ++i) s += v(i);
-  double scan = s;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const double up = __shfl_up_sync(0xffffffff, scan, o);
-    if (lane >= o) scan += up;
+  // ln x within 2^-40, for x >= 1: the fp32 logarithm and one step of Newton's method for e^y = x.
+  static __device__ __forceinline__ double log_64(double x) {
+    const double y = (double)logf((float)x);
+    double t[1] = {-y * (16. * 1.4426950408889634)};
+    exp2_16th(t, shared().pow);
+    return y + (x * t[0] - 1.);
   }
-  const double total = __shfl_sync(0xffffffff, scan, 31);
-  double run = scan - s;
-  for (int i = a; i < b; ++i) {
-    const double one = v(i);
-    before(i, run, one);
-    run += one;
-  }
-  return total;
-}
-
-// Where the value of the sorted candidate i begins.
-__device__ __forceinline__ int first_of_value(const SampleShared& sh, int i) {
-  int first = 0, last = i;
-  const uint32_t key = key_part(sh.sorted[i]);
-  while (first < last) {
-    const int mid = (first + last) / 2;
-    if (key_part(sh.sorted[mid]) == key) last = mid;
-    else first = mid + 1;
-  }
-  return first;
-}
-
-// The leader's answer from its candidates, by its first warp. `total` +- `error` is the mass of the row that top-p takes a
-// share of, where top-k is off; `complete`: no token below the candidates can be kept.
-__device__ void answer_from_list(const SampleRow& r, int n, bool complete, uint32_t low_m, double total, double error,
-                                 long long* token, float* logprob) {
-  SampleShared& sh = r.sh;
-  const int lane = r.lane;
-  const double all = running_sums(lane, n, [&](int i) { return sh.weight[i]; },
-                                  [&](int i, double run, double) { sh.before[i] = run; });
-  __syncwarp();
-  int nk = n;
-  if (r.use_k) {
-    const uint32_t kth = r.k <= n ? key_part(sh.sorted[r.k - 1]) : 0;
-    nk = 0;
-    for (int i = lane; i < n; i += 32) nk += key_part(sh.sorted[i]) >= kth;
-    nk = __reduce_add_sync(0xffffffff, nk);
-    total = nk < n ? sh.before[nk] : all;
-    error = 0.;
-  }
-  const double share = r.p * total, blur = r.p * error;
-  bool unsure = false;
-  int kept = 0;
-  for (int i = lane; i < nk; i += 32) {
-    bool keep = !r.use_m || key_part(sh.sorted[i]) >= low_m;
-    if (r.use_p && i > 0) {
-      const int first = first_of_value(sh, i);
-      unsure |= first > 0 && blur > 0. && fabs(sh.before[first] - share) <= blur;
-      keep &= first == 0 || !(sh.before[first] > share);
-    }
-    kept += keep;
-  }
-  kept = __reduce_add_sync(0xffffffff, kept);
-  int verdict = kDone;
-  if (!complete && r.use_p) {  // is the bound of top-p among the candidates?
-    unsure |= blur > 0. && fabs(all - share) <= blur;
-    if (!(all > share)) verdict = kIncomplete;
-  }
-  if (__any_sync(0xffffffff, unsure)) verdict = kAmbiguous;
-  if (verdict == kDone) {
-    const double mass = kept < n ? sh.before[kept] : all, target = r.draw * mass;
-    int hit = n, last = -1;  // in the order of ids: the first at which the running sum is above the target, the last with mass
-    running_sums(lane, n, [&](int q) { return sh.by_id[q] < kept ? sh.weight[sh.by_id[q]] : 0.; },
-                 [&](int q, double run, double one) {
-                   if (one > 0.) last = q;
-                   if (one > 0. && run + one > target) hit = min(hit, q);
-                 });
-    hit = __reduce_min_sync(0xffffffff, hit);
-    last = __reduce_max_sync(0xffffffff, last);
-    if (lane == 0) {
-      const int i = sh.by_id[hit < n ? hit : last];
-      *token = id_part(sh.sorted[i]);
-      if (logprob) *logprob = (float)log(sh.weight[i] / mass);
-    }
-  }
-  if (lane == 0) sh.verdict = verdict;
-}
-
-// The leader's bound of top-p, by its first warp, among the candidates of a few steps of the histogram, above which lies
-// `above` +- `error`; `end`: no logit lies below them. The mass of strictly larger logits must be known to lie below or above
-// the share.
-__device__ void bound_from_list(const SampleRow& r, int n, bool end, double above, double error, double share, double blur) {
-  SampleShared& sh = r.sh;
-  const double doubt = error + blur;
-  const double all = above + running_sums(r.lane, n, [&](int i) { return sh.weight[i]; },
-                                          [&](int i, double run, double) { sh.before[i] = run; });
-  __syncwarp();
-  bool unsure = !end && doubt > 0. && fabs(all - share) <= doubt;
-  int kept = 0;
-  for (int i = r.lane; i < n; i += 32) {
-    const double larger = above + sh.before[first_of_value(sh, i)];
-    kept += !(larger > share);
-    unsure |= larger > 0. && doubt > 0. && fabs(larger - share) <= doubt;
-  }
-  kept = __reduce_add_sync(0xffffffff, kept);
-  unsure = __any_sync(0xffffffff, unsure);
-  if (r.lane == 0) {
-    sh.verdict = unsure ? kAmbiguous : (kept == 0 || (!end && !(all > share)) ? kIncomplete : kDone);
-    sh.low = kept > 0 ? key_part(sh.sorted[kept - 1]) : 0;
-  }
-}
-
-// HELD: the CTA's part of the row lies in shared memory.
-template <typename T, bool HELD>
-__global__ void __launch_bounds__(SG_THREADS, 2) sample_given_kernel(const SampleGivenArgs a) {
-  constexpr int E = LogitType<T>::E;
-  extern __shared__ uint4 held[];  // vector i of thread t at i * 512 + t
-  __shared__ SampleShared sh;
-  const int t = threadIdx.x, lane = t & 31, w = t >> 5;
-  const int cs = a.cluster, rank = cs > 1 ? (int)cg::this_cluster().block_rank() : 0;
-  const int row = blockIdx.x / cs;
-  begin_early();
-  const RowVecs<T> vecs(static_cast<const T*>(a.x) + (long long)row * a.ldx, a.V);
-  const int per = (vecs.n + cs - 1) / cs, v0 = rank * per, v1 = min(v0 + per, vecs.n);
-  // every warp holds vectors one after another, so that sums over warps are sums over ids
-  const int chunk = (per + SG_THREADS - 1) / SG_THREADS * 32, w0 = v0 + w * chunk, w1 = min(w0 + chunk, v1);
-  const int mine = max(0, min(chunk / 32, (w1 - w0 - lane + 31) / 32));  // vectors of this thread
-  float top = -INFINITY;
-  bool nan = false;
-#pragma unroll 1
-  for (int i0 = 0; i0 < mine; i0 += SG_VECS) {
-    uint4 u[SG_VECS];
-#pragma unroll
-    for (int i = 0; i < SG_VECS; ++i) u[i] = i0 + i < mine ? vecs.load(w0 + (i0 + i) * 32 + lane) : vec_neg_inf<T>();
-#pragma unroll
-    for (int i = 0; i < SG_VECS; ++i) {
-      if (HELD && i0 + i < mine) held[(i0 + i) * SG_THREADS + t] = u[i];
-      const float most = vec_max<T>(u[i]);
-      nan |= most != most;
-      top = fmaxf(top, most);
-    }
-  }
-  const auto vec = [&](int i) { return HELD ? held[i * SG_THREADS + t] : vecs.load(w0 + i * 32 + lane); };
-  // f(vector, its number) over this thread's vectors, several in flight
-  const auto for_vecs = [&](auto f) {
-    constexpr int kBatch = HELD ? 2 : 4;
-    int i = 0;
-#pragma unroll 1
-    for (; i + kBatch <= mine; i += kBatch) {
-      uint4 u[kBatch];
-#pragma unroll
-      for (int j = 0; j < kBatch; ++j) u[j] = vec(i + j);
-#pragma unroll
-      for (int j = 0; j < kBatch; ++j) f(u[j], i + j);
-    }
-#pragma unroll 1
-    for (; i < mine; ++i) f(vec(i), i);
-  };
-  SampleRow r{sh, cs, rank, t, lane, w};
-  const float temperature = a.temperature[row];
-  const bool greedy = !(temperature > 0.f);
-  r.T64 = (double)(greedy ? 1.f : fminf(fmaxf(temperature, 1e-8f), 3.4e38f));
-  r.k = a.top_k[row];
-  r.use_k = !greedy && r.k > 0 && r.k < a.V;
-  const float p = a.top_p[row], m = a.min_p[row];
-  r.use_p = !greedy && p < 1.f;
-  r.use_m = !greedy && m > 0.f;
-  r.p = r.use_p ? fmax((double)p, 0.) : 1.;
-  r.m = r.use_m ? fmin((double)m, 1.) : 0.;
-  r.draw = a.uniform64 ? static_cast<const double*>(a.uniform)[row] : (double)static_cast<const float*>(a.uniform)[row];
-  r.draw = fmin(fmax(r.draw, 0.), 1.);  // a NaN becomes 0
-  long long* const token = a.token + row;
-  float* const logprob = a.logprob ? a.logprob + row : nullptr;
-  SampleShared* lead = &sh;
-  if (cs > 1) lead = cg::this_cluster().map_shared_rank(&sh, 0);
-  if (t == 0) sh.n = 0;
-  r.c64 = 1.4426950408889634 / r.T64;
-  const float c = (float)r.c64;
-  r.max_x = of_key(r.max_key(key_of(nan ? of_key(0xFFFFFFFFu) : top)));
-
-  // f(element, id) over this thread's elements
-  const auto each = [&](auto f) {
-    for_vecs([&](const uint4& u, int i) {
-      const int at = vecs.first(w0 + i * 32 + lane);
-      float x[E];
-      vec_floats<T>(u, x);
-#pragma unroll
-      for (int e = 0; e < E; ++e)
-        if (at + e >= 0 && at + e < a.V) f(x[e], at + e);
-    });
-  };
   // Mass of a vector's logits from `low` on. In 32 bits each exponential is within 2^-22 of itself and 3 |t| 2^-24 ln 2 for
   // the roundings of t = (x - max) c, and eight of them are added in a tree.
-  const Pair ref2(-r.max_x, -r.max_x), c2(c, c);
-  const auto vec_mass = [&](const uint4& u, bool precise, float low) -> double {
+  static __device__ __forceinline__ double vec_mass(const uint4& u, float low, Pair ref2, Pair c2) {
     float x[E];
     vec_floats<T>(u, x);
-    if (precise) {
-      double s = 0.;
-#pragma unroll
-      for (int e = 0; e < E; ++e) s += x[e] >= low ? r.weight(x[e]) : 0.;
-      return s;
-    }
     Pair q[E / 2];
 #pragma unroll
     for (int e = 0; e < E / 2; ++e)
@@ -439,175 +252,554 @@ __global__ void __launch_bounds__(SG_THREADS, 2) sample_given_kernel(const Sampl
 #pragma unroll
       for (int e = 0; e < o; ++e) q[e] = q[e] + q[e + o];
     return (double)q[0].sum();
-  };
-  // Over the row, with a bound on its error: the mass' average |t| is the entropy of its shares less log2 of it (the largest
-  // weight is 1), at most log2 V - log2 total.
-  double error = 0.;
-  const float log_v = log2f((float)a.V);
-  const auto masses = [&](bool precise, float low) {
+  }
+  static __device__ __forceinline__ double vec_mass_64(const uint4& u, float low, double max_x, double c64) {
+    float x[E];
+    vec_floats<T>(u, x);
+    double sum = 0.;
+#pragma unroll
+    for (int e0 = 0; e0 < E; e0 += 4) {
+      double s[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[e] = x[e0 + e] >= low ? ((double)x[e0 + e] - max_x) * c64 : -INFINITY;
+      exp2_16th(s, shared().pow);
+      sum += (s[0] + s[1]) + (s[2] + s[3]);
+    }
+    return sum;
+  }
+  // This warp's mass of vectors i .. i + 3 each.
+  static __device__ __noinline__ void warp_masses(bool precise, float low, int i, int end, double (&s)[4], double& mine, int which) {
+    const SampleShared& sh = shared();
+    const Mine me(sh);
+    const Pair ref2(-sh.max_x, -sh.max_x), c2(sh.c, sh.c);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint4 u = i + j < end ? me.vec(i + j) : vec_neg_inf<T>();
+      s[j] = precise ? vec_mass_64(u, low, sh.max_x, sh.c64) : vec_mass(u, low, ref2, c2);
+      if (j == which) mine = s[j];
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s[j] = warp_add(s[j]);
+  }
+  // The row's mass from `low` on; by warps in sh.warp_sum, by their groups in sh.group_sum.
+  static __device__ __noinline__ double mass_64(float low) {
+    SampleShared& sh = shared();
+    const Mine me(sh);
+    const double max_x = sh.max_x, c64 = sh.c64;
     double s = 0.;
-    if (precise) {
 #pragma unroll 1
-      for (int i = 0; i < mine; ++i) s += vec_mass(vec(i), true, low);
-    } else {
-      for_vecs([&](const uint4& u, int) { s += vec_mass(u, false, low); });
-    }
-    const SampleRow::Part part = r.sum(s);
-    error = precise ? 0. : part.total * (4.5e-7 + 1.3e-7 * fmaxf(log_v - log2f((float)part.total), 0.f));
-    return part;
-  };
-  // Draws among the logits from `low` on.
-  const auto draw = [&](float low) {
+    for (int i0 = 0, at = 0; i0 < sh.chunk / 32; i0 += sh.group, ++at) {
+      double part = 0.;
 #pragma unroll 1
-    for (int precise = 0; precise < 2; ++precise) {
-      if (rank == 0 && t == 0) sh.verdict = kDone;
-      const SampleRow::Part part = masses(precise, low);
-      // The CTA in whose part the target lies, and there, counted from its start, the warp. Should rounding leave the
-      // target at the very end, the last one with any mass takes it.
-      double target = r.draw * part.total;
-      const bool here = part.here > 0. && part.before <= target && (target < part.before + part.here || part.last);
-      target -= part.before;
-      double before = part.warp_before;
-      if (here && part.warp > 0. && before <= target && (target < before + part.warp || part.warp_last)) {
-        int at_i = 0, last_i = 0;
-        double at_before = -1., last_before = before, s;
-#pragma unroll 1
-        for (int i0 = 0; i0 < chunk / 32; i0 += 4) {
-          double part4[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) part4[i] = i0 + i < mine ? vec_mass(vec(i0 + i), precise, low) : 0.;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) part4[i] = SampleRow::warp_add(part4[i]);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            s = part4[i];
-            if (s > 0.) last_i = i0 + i, last_before = before;
-            if (at_before < 0. && before + s > target) at_i = i0 + i, at_before = before;
-            before += s;
-          }
-          if (at_before >= 0.) break;
-        }
-        if (at_before < 0.) at_i = last_i, at_before = last_before;
-        s = at_i < mine ? vec_mass(vec(at_i), precise, low) : 0.;
-        double scan = s;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const double up = __shfl_up_sync(0xffffffff, scan, o);
-          if (lane >= o) scan += up;
-        }
-        const uint32_t above = __ballot_sync(0xffffffff, s > 0. && at_before + scan > target);
-        const uint32_t some = __ballot_sync(0xffffffff, s > 0.);
-        const int who = above ? __ffs(above) - 1 : 31 - __clz(some);
-        if (lane == who) {
-          double run = at_before + (scan - s), c0 = run, c1 = run;
-          int id = -1;
-          float chosen = 0.f, x[E];
-          vec_floats<T>(vec(at_i), x);
-          const int at = vecs.first(w0 + at_i * 32 + lane);
-#pragma unroll
-          for (int e = 0; e < E; ++e) {
-            if (!(x[e] >= low)) continue;
-            const double one = precise ? r.weight(x[e]) : (double)exp2_fast((x[e] - r.max_x) * c);
-            if (one > 0. && (id < 0 || !(c1 > target))) {  // the first above the target, or the last with any mass
-              id = at + e;
-              chosen = x[e];
-              c0 = run;
-              c1 = run + one;
-            }
-            run += one;
-          }
-          if (!precise && (target - c0 <= 2. * error || c1 - target <= 2. * error)) {
-            lead->verdict = kAmbiguous;
-          } else {
-            *token = id;
-            if (logprob) *logprob = (float)log(r.weight(chosen) / part.total);
-          }
-        }
+      for (int i = i0; i < min(i0 + sh.group, me.mine); ++i) part += vec_mass_64(me.vec(i), low, max_x, c64);
+      s += part;
+      if (!HELD) {
+        part = warp_add(part);
+        if ((threadIdx.x & 31) == 0) sh.group_sum[threadIdx.x / 32][at] = part;
       }
-      r.sync();
-      const int verdict = lead->verdict;
-      r.sync();
-      if (verdict == kDone) return;
     }
-  };
-  // Candidates: logits from `low` on for which `in` holds, into the leader's list.
-  const auto gather = [&](float low, auto in) {
-    for_vecs([&](const uint4& u, int i) {
+    return scan(s).y;
+  }
+  static __device__ __noinline__ double mass_32(float low) {
+    SampleShared& sh = shared();
+    const Mine me(sh);
+    const Pair ref2(-sh.max_x, -sh.max_x), c2(sh.c, sh.c);
+    double s = 0., part = 0.;
+    for_vecs(sh, me, low, [&](const uint4& u, int) { part += vec_mass(u, low, ref2, c2); },
+             [&](int at) {
+               s += part;
+               if (!HELD) {
+                 part = warp_add(part);
+                 if ((threadIdx.x & 31) == 0) sh.group_sum[threadIdx.x / 32][at] = part;
+               }
+               part = 0.;
+             });
+    return scan(s).y;
+  }
+  // With a bound on its error: the mass' average |t| is the entropy of its shares less log2 of it (the largest weight is 1),
+  // at most log2 V - log2 total.
+  static __device__ __forceinline__ double mass(bool precise, float low, double& error) {
+    const double total = precise ? mass_64(low) : mass_32(low);
+    error = precise || total == 0. ? 0. : total * (4.5e-7 + 1.3e-7 * fmaxf(log2f((float)shared().V) - log2f((float)total), 0.f));
+    return total;
+  }
+  // Candidates: the logits in low .. high (exclusive), if they are not too many; their number.
+  static __device__ __noinline__ int gather(float low, float high) {
+    SampleShared& sh = shared();
+    const Mine me(sh);
+    __syncthreads();
+    if (threadIdx.x == 0) sh.n = 0;
+    __syncthreads();
+    for_vecs(sh, me, low, [&](const uint4& u, int i) {
       if (!(vec_max<T>(u) >= low)) return;
-      const int at = vecs.first(w0 + i * 32 + lane);
+      float x[E];
+      vec_floats<T>(u, x);
+      uint32_t bits = 0;
+#pragma unroll
+      for (int e = 0; e < E; ++e) bits |= (uint32_t)(x[e] >= low && x[e] < high) << e;
+      if (!bits) return;
+      int to = atomicAdd(&sh.n, __popc(bits));
+      const int at = me.first(i);
+#pragma unroll 1
+      for (; bits; bits &= bits - 1, ++to) {
+        const int e = __ffs(bits) - 1;
+        float one = x[0];
+#pragma unroll
+        for (int j = 1; j < E; ++j) one = e == j ? x[j] : one;
+        if (to < SG_CAP) sh.key[to] = key_of(one), sh.id[to] = at + e;
+      }
+    });
+    __syncthreads();
+    return sh.n;
+  }
+  // The number of logits from `low` on by steps down from the largest; those in the last step, or beyond it, are not counted.
+  static __device__ __forceinline__ int bin_of(float x, float max_x, float scale) {
+    return min((int)((max_x - x) * scale), SG_BINS - 1);
+  }
+  static __device__ __noinline__ void histogram(float scale, float low) {
+    SampleShared& sh = shared();
+    const Mine me(sh);
+    __syncthreads();
+    for (int i = threadIdx.x; i < SG_BINS; i += NT) sh.bins[i] = 0;
+    __syncthreads();
+    const float max_x = sh.max_x;
+    for_vecs(sh, me, low, [&](const uint4& u, int) {
       float x[E];
       vec_floats<T>(u, x);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        if (!(x[e] >= low) || !in(x[e])) continue;
-        const int slot = atomicAdd(&lead->n, 1);
-        if (slot < SG_CAP) lead->list[slot] = (unsigned long long)key_of(x[e]) << 32 | (uint32_t)~(at + e);
+        const int bin = bin_of(x[e], max_x, scale);
+        if (x[e] >= low && bin < SG_BINS - 1) atomicAdd(&sh.bins[bin], 1u);
       }
     });
-    r.sync();
-    return lead->n;
-  };
-
-  const auto run = [&] {
-    if (!(fabsf(r.max_x) < INFINITY)) {  // a NaN, an infinity or nothing allowed: no distribution; the largest number
-      uint32_t key = 0;
-      each([&](float x, int) { if (x == x) key = max(key, key_of(x)); });
-      key = r.max_key(key);
-      uint32_t first = 0;
-      each([&](float x, int id) { if (x == x && key_of(x) == key) first = max(first, ~(uint32_t)id); });
-      first = r.max_key(first);
-      if (rank == 0 && t == 0) {
-        *token = key ? (int)~first : 0;
-        if (logprob) *logprob = __int_as_float(0x7FC00000);
-      }
-      return;
+    __syncthreads();
+  }
+  // The first bin at which the running sum exceeds `target` (SG_BINS: none) and the sum before it: of the logits' number, or
+  // of their mass with each taken at the middle of its step (fp32, sums of whole numbers up to 2^22 are exact).
+  static __device__ __noinline__ int find_bin(float target, float scale, bool mass, float& above) {
+    SampleShared& sh = shared();
+    constexpr int kEach = SG_BINS / NT;
+    const int t = threadIdx.x, lane = t & 31, w = t / 32;
+    float bins[kEach], s = 0.f;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      bins[i] = (float)sh.bins[t * kEach + i];
+      if (mass) bins[i] *= exp2_fast(-((float)(t * kEach + i) + 0.5f) / scale * sh.c);
+      s += bins[i];
     }
-    if (greedy) {
-      uint32_t first = 0;
-      if (top == r.max_x) each([&](float x, int id) { if (x == r.max_x) first = max(first, ~(uint32_t)id); });
-      first = r.max_key(first);
-      const double total = logprob ? masses(false, -INFINITY).total : 1.;
-      if (rank == 0 && t == 0) {
-        *token = (int)~first;
-        if (logprob) *logprob = (float)-log(total);
-      }
-      return;
+    float run = s;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const float up = __shfl_up_sync(0xffffffff, run, o);
+      if (lane >= o) run += up;
     }
+    __syncthreads();
+    if (lane == 31) sh.warp_key[w] = __float_as_uint(run);
+    if (t == 0) sh.bin = SG_BINS;
+    __syncthreads();
+    float warps = lane < kWarps ? __uint_as_float(sh.warp_key[lane]) : 0.f;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const float up = __shfl_up_sync(0xffffffff, warps, o);
+      if (lane >= o) warps += up;
+    }
+    const float base = __shfl_sync(0xffffffff, warps, max(w - 1, 0));
+    float before = (w > 0 ? base : 0.f) + (run - s);
+    if (before <= target && before + s > target) {  // two threads where rounding lets their parts overlap: the first
+      int i = 0;
+#pragma unroll
+      for (int b = 0; b < kEach; ++b)
+        if (i == b && b + 1 < kEach && before + bins[b] <= target) before += bins[b], ++i;
+      atomicMin(&sh.bin, t * kEach + i);
+    }
+    __syncthreads();
+    const int bin = sh.bin;
+    if (bin / kEach == t) sh.above = before;
+    __syncthreads();
+    above = sh.above;
+    return bin;
+  }
+  // That running sum before bin `end`.
+  static __device__ __noinline__ double mass_of_bins(int end, float scale) {
+    const SampleShared& sh = shared();
+    float s = 0.f;
+    for (int i = threadIdx.x; i < end; i += NT) s += (float)sh.bins[i] * exp2_fast(-((float)i + 0.5f) / scale * sh.c);
+    return scan((double)s).y;
+  }
+  // The least key in a bin before this one.
+  static __device__ __noinline__ uint32_t edge_of(int bin, float scale) {
+    const float max_x = shared().max_x;
+    const auto before = [&](uint32_t key) { return bin_of(of_key(key), max_x, scale) < bin; };
+    uint32_t lo = kLowest, hi = key_of(max_x);
+    const float x = max_x - (float)bin / scale, near = 1e-6f * (fabsf(max_x) + fabsf(x));  // a window around it
+    const uint32_t a = key_of(x - near), b = key_of(x + near);
+    if (a > lo && b < hi && !before(a) && before(b)) lo = a, hi = b;
+    return least_key(threadIdx.x & 31, lo, hi, before);
+  }
+  static __device__ __noinline__ float least() {
+    const SampleShared& sh = shared();
+    const Mine me(sh);
+    float least = INFINITY;
+    for_vecs(sh, me, -INFINITY, [&](const uint4& u, int) {
+      float x[E];
+      vec_floats<T>(u, x);
+#pragma unroll
+      for (int e = 0; e < E; ++e) least = fminf(least, x[e] > -INFINITY ? x[e] : least);
+    });
+    return of_key(min_of(key_of(least)));
+  }
+  static __device__ __noinline__ int count_from(float low) {
+    const SampleShared& sh = shared();
+    const Mine me(sh);
+    int n = 0;
+    for_vecs(sh, me, low, [&](const uint4& u, int) {
+      float x[E];
+      vec_floats<T>(u, x);
+#pragma unroll
+      for (int e = 0; e < E; ++e) n += x[e] >= low;
+    });
+    return sum_of(n);
+  }
+  // The lowest id of a number equal to `value`.
+  static __device__ __noinline__ uint32_t first_id(float value) {
+    const SampleShared& sh = shared();
+    const Mine me(sh);
+    uint32_t first = 0;  // complement
+    for_vecs(sh, me, value, [&](const uint4& u, int i) {
+      float x[E];
+      vec_floats<T>(u, x);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const int id = me.first(i) + e;
+        if (i < me.mine && x[e] == value && id >= 0 && id < sh.V) first = max(first, ~(uint32_t)id);
+      }
+    });
+    return ~max_of(first);
+  }
 
-    // min-p as a bound on the key: the least whose weight reaches it, among the 32 around max + T ln m, or where that window
-    // lies above it (temperatures at which neighbours have the same weight) by a search in 32 parts.
-    if (r.use_m && w == 0) {
-      const uint32_t max_key = key_of(r.max_x);
-      const auto reaches = [&](uint32_t key) {
-        return __ballot_sync(0xffffffff, key == max_key || (key < max_key && r.weight(of_key(key)) >= r.m));
-      };
-      uint32_t lo = key_of(-3.4028235e38f), step = 1;
-      uint32_t from = max(key_of((float)fmax(r.max_x + r.T64 * log(r.m), -3.4e38)), lo + 16) - 16;
-      uint32_t ok = reaches(from + lane), hi = ok ? from + __ffs(ok) - 1 : max_key;
-      if (ok & 1) {
-        while (lo < hi) {
-          step = (hi - lo) / 32 + 1;
-          ok = reaches(min(lo + lane * step, hi));  // the last one does
-          const int i = __ffs(ok) - 1;
-          hi = min(lo + i * step, hi);
-          if (i > 0) lo = lo + (i - 1) * step + 1;
-          else break;
+  // ---------------------------------------------------------------- candidates
+  // `n` numbers of sh (at `from`) in descending order into sh.sorted: a bitonic sort, one or two numbers a thread,
+  // within a warp by shuffles. Written out: as a loop its branches took most of the time (128 numbers: 7000 clocks, now 1500).
+  template <bool TWO>
+  static __device__ __noinline__ void sort_by(int n, uint32_t v0, uint32_t v1) {
+    SampleShared& sh = shared();
+    const int t = threadIdx.x;
+    int turn = 0;
+#pragma unroll
+    for (int k = 2; k <= (TWO ? 2 * SG_THREADS : SG_THREADS); k <<= 1) {
+      if (k / 2 >= n) break;
+#pragma unroll
+      for (int j = k >> 1; j > 0; j >>= 1) {
+        if (j == SG_THREADS) {  // the two numbers of a thread
+          const uint32_t a = max(v0, v1);
+          v1 = min(v0, v1);
+          v0 = a;
+          continue;
+        }
+        uint32_t o0, o1 = 0;
+        if (j >= 32) {
+          sh.swap[turn][t] = v0;
+          if (TWO) sh.swap[turn][t + SG_THREADS] = v1;
+          __syncthreads();
+          o0 = sh.swap[turn][t ^ j];
+          if (TWO) o1 = sh.swap[turn][(t ^ j) + SG_THREADS];
+          turn ^= 1;
+        } else {
+          o0 = __shfl_xor_sync(0xffffffff, v0, j);
+          if (TWO) o1 = __shfl_xor_sync(0xffffffff, v1, j);
+        }
+        const bool lower = (t & j) == 0;
+        v0 = ((t & k) == 0) == lower ? max(v0, o0) : min(v0, o0);
+        if (TWO) v1 = (((t + SG_THREADS) & k) == 0) == lower ? max(v1, o1) : min(v1, o1);
+      }
+    }
+    if (t < n) sh.sorted[t] = v0;
+    if (TWO && t + SG_THREADS < n) sh.sorted[t + SG_THREADS] = v1;
+  }
+  static __device__ __noinline__ void sort(int n, const uint32_t* from) {
+    const int t = threadIdx.x;
+    const uint32_t v0 = t < n ? from[t] : 0, v1 = t + SG_THREADS < n ? from[t + SG_THREADS] : 0;
+    __syncthreads();
+    if (n > SG_THREADS) sort_by<true>(n, v0, v1);
+    else sort_by<false>(n, v0, v1);
+    __syncthreads();
+  }
+  // Where the value of the sorted candidate i begins.
+  static __device__ __forceinline__ int first_of_value(const SampleShared& sh, int i) {
+    const uint32_t key = sh.sorted[i];
+    if (i == 0 || sh.sorted[i - 1] != key) return i;
+    int first = 0, last = i - 1;
+#pragma unroll 1
+    while (first < last) {
+      const int mid = (first + last) / 2;
+      if (sh.sorted[mid] == key) last = mid;
+      else first = mid + 1;
+    }
+    return first;
+  }
+  // The mass before each of the sorted candidates, and of all.
+  static __device__ __noinline__ double mass_before(int n) {
+    SampleShared& sh = shared();
+    const int each = n > NT ? 2 : 1, i = threadIdx.x * each;
+    double a = 0., b = 0.;
+    if (i < n) a = weight(of_key(sh.sorted[i]));
+    if (each == 2 && i + 1 < n) b = weight(of_key(sh.sorted[i + 1]));
+    const double2 run = scan(a + b);
+    if (i < n) sh.before[i] = run.x;
+    if (each == 2 && i + 1 < n) sh.before[i + 1] = run.x + a;
+    __syncthreads();
+    return run.y;
+  }
+  // Top-p's bound among the sorted candidates, above which lies the mass `above`: keeps those whose strictly larger logits
+  // hold at most `share`; `doubt`: how near to it that is not known; `end`: no logit that could be kept lies below them.
+  // The least key that is kept in sh.low.
+  static __device__ __noinline__ Verdict bound(int n, double above, double share, double doubt, bool end) {
+    SampleShared& sh = shared();
+    const double all = above + mass_before(n);
+    bool unsure = !end && doubt > 0. && fabs(all - share) <= doubt;
+    int kept = 0;
+#pragma unroll 1
+    for (int i = threadIdx.x; i - (int)threadIdx.x < n; i += NT) {
+      bool keep = false;
+      if (i < n) {
+        const double larger = above + sh.before[first_of_value(sh, i)];
+        keep = larger == 0. || !(larger > share);
+        unsure |= larger > 0. && doubt > 0. && fabs(larger - share) <= doubt;
+      }
+      kept += __syncthreads_count(keep);
+    }
+    unsure = __syncthreads_or(unsure);
+    if (threadIdx.x == 0) sh.low = kept > 0 ? sh.sorted[kept - 1] : 0;
+    __syncthreads();
+    return unsure ? kAmbiguous : kept == 0 || (!end && !(all > share)) ? kIncomplete : kDone;
+  }
+  // The draw among the candidates from the key `low` on, in the order of ids: an id and a place in the list make one number.
+  static __device__ __noinline__ void draw_from_list(int n, uint32_t low) {
+    SampleShared& sh = shared();
+    const int t = threadIdx.x;
+    __syncthreads();
+    for (int i = t; i < n; i += NT) sh.swap[1][i] = ~(sh.id[i] << 10 | i);
+    __syncthreads();
+    sort(n, sh.swap[1]);
+    if (t == 0) sh.hit = SG_CAP, sh.last = -1;
+    const int each = n > NT ? 2 : 1, i = t * each;
+    double w0 = 0., w1 = 0.;
+    if (i < n && sh.key[~sh.sorted[i] & 1023] >= low) w0 = weight(of_key(sh.key[~sh.sorted[i] & 1023]));
+    if (each == 2 && i + 1 < n && sh.key[~sh.sorted[i + 1] & 1023] >= low) w1 = weight(of_key(sh.key[~sh.sorted[i + 1] & 1023]));
+    const double2 run = scan(w0 + w1);  // with its barriers for hit and last
+    const double target = sh.draw * run.y;
+    int hit = SG_CAP;  // the first at which the running sum is above the target, or the last with any mass
+    if (w1 > 0. && run.x + w0 + w1 > target) hit = i + 1;
+    if (w0 > 0. && run.x + w0 > target) hit = i;
+    hit = __reduce_min_sync(0xffffffff, hit);
+    const int last = __reduce_max_sync(0xffffffff, w1 > 0. ? i + 1 : w0 > 0. ? i : -1);
+    if ((t & 31) == 0 && hit < SG_CAP) atomicMin(&sh.hit, hit);
+    if ((t & 31) == 0 && last >= 0) atomicMax(&sh.last, last);
+    __syncthreads();
+    if (t == 0) answer(~sh.sorted[sh.hit < n ? sh.hit : sh.last] & 1023, run.y);
+  }
+  static __device__ __noinline__ void answer(int place, double total) { answer(shared().id[place], of_key(shared().key[place]), total); }
+  static __device__ __noinline__ void answer(int id, float x, double total) {
+    const SampleShared& sh = shared();
+    *sh.token = id;
+    if (sh.logprob) *sh.logprob = (float)(((double)x - (double)sh.max_x) / sh.T64 - log_64(total));
+  }
+  // The draw among all logits from `low` on.
+  static __device__ __noinline__ void draw(float low) {
+    SampleShared& sh = shared();
+    const int lane = threadIdx.x & 31, w = threadIdx.x / 32;
+#pragma unroll 1
+    for (int precise = 0; precise < 2; ++precise) {
+      double error;
+      const double total = mass(precise, low, error), target = sh.draw * total;
+      if (threadIdx.x == 0) sh.hit = kDone;
+      // The warp in whose part the target lies. Should rounding leave the target at the very end, the last one with any mass
+      // takes it.
+      const double theirs = lane < kWarps ? sh.warp_sum[lane] : 0., upto = lanes_before(theirs);
+      const double here = __shfl_sync(0xffffffff, theirs, w);
+      double before = __shfl_sync(0xffffffff, upto, max(w - 1, 0));
+      if (w == 0) before = 0.;
+      const bool last = (__ballot_sync(0xffffffff, theirs > 0.) & ~(0xffffffffu >> (31 - w))) == 0;
+      __syncthreads();
+      if (here > 0. && before <= target && (target < before + here || last)) {
+        int begin = 0, end = sh.chunk / 32;
+        if (!HELD) {  // the group
+          double run = before;
+          bool found = false;
+          for (int g = 0; g * sh.group < sh.chunk / 32; ++g) {
+            const double one = sh.group_sum[w][g];
+            if (!found && one > 0.) begin = g * sh.group, before = run, found = run + one > target;
+            run += one;
+          }
+          end = min(begin + sh.group, sh.chunk / 32);
+        }
+        // four rows of vectors at a time, then the row
+        int at_i = -1, last_i = begin;
+        double at_before = 0., last_before = before, s[4], mine;
+#pragma unroll 1
+        for (int i0 = begin; i0 < end && at_i < 0; i0 += 4) {
+          warp_masses(precise, low, i0, end, s, mine, -1);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if (s[i] > 0.) last_i = i0 + i, last_before = before;
+            if (at_i < 0 && s[i] > 0. && before + s[i] > target) at_i = i0 + i, at_before = before;
+            before += s[i];
+          }
+        }
+        if (at_i < 0) at_i = last_i, at_before = last_before;
+        warp_masses(precise, low, at_i, at_i + 1, s, mine, 0);
+        const double run = lanes_before(mine);
+        const uint32_t above = __ballot_sync(0xffffffff, mine > 0. && at_before + run > target);
+        const uint32_t some = __ballot_sync(0xffffffff, mine > 0.);
+        if (lane == (above ? __ffs(above) - 1 : 31 - __clz(some))) {
+          const Mine me(sh);
+          double upto = at_before + (run - mine), c0 = upto, c1 = upto;
+          int id = -1;
+          float chosen = 0.f, x[E];
+          vec_floats<T>(me.vec(at_i), x);
+#pragma unroll 1
+          for (int e = 0; e < E; ++e) {
+            float one_x = x[0];
+#pragma unroll
+            for (int j = 1; j < E; ++j) one_x = e == j ? x[j] : one_x;
+            if (!(one_x >= low)) continue;
+            const double one = precise ? weight(one_x) : (double)exp2_fast((one_x - sh.max_x) * sh.c);
+            if (one > 0. && (id < 0 || !(c1 > target))) {  // the first above the target, or the last with any mass
+              id = me.first(at_i) + e;
+              chosen = one_x;
+              c0 = upto;
+              c1 = upto + one;
+            }
+            upto += one;
+          }
+          if (!precise && (target - c0 <= 2. * error || c1 - target <= 2. * error)) sh.hit = kAmbiguous;
+          else answer(id, chosen, total);
         }
       }
-      if (lane == 0) sh.low = hi;
+      __syncthreads();
+      if (sh.hit == kDone) return;
     }
-    const bool by_k = r.use_k && r.k <= SG_LIST_K;
-    const bool by_list = by_k || (!r.use_k && (r.use_p || r.use_m));
+  }
+
+  // ---------------------------------------------------------------- bounds where many tokens stay
+  static __device__ __forceinline__ float from(uint32_t key) { return of_key(max(key, kLowest)); }
+  static __device__ __forceinline__ bool usable(float range) {
+    return range > 0.f && range < 1e37f && (SG_BINS - 1) / range < 1e37f;
+  }
+  // The histogram's range is `near` first (four times from the largest to a logit that SG_LIST_K logits reach); if that is too
+  // short, down to the least.
+  static __device__ __noinline__ uint32_t top_k_bound(int k, float near) {
+    SampleShared& sh = shared();
+#pragma unroll 1
+    for (int attempt = 0; attempt < 2; ++attempt) {
+      const float range = attempt == 0 ? near : sh.max_x - least();
+      if (!usable(range)) continue;
+      const float scale = (SG_BINS - 1) / range;
+      histogram(scale, of_key(kLowest));
+      float above;
+      const int bin = find_bin((float)(k - 1), scale, false, above);
+      if (bin == SG_BINS && attempt == 1 && count_from(of_key(kLowest)) < k) return 0;  // fewer numbers than k
+      if (bin == SG_BINS) continue;
+      const float high = bin > 0 ? of_key(edge_of(bin, scale)) : INFINITY;
+      const int n = gather(of_key(edge_of(bin + 1, scale)), high);
+      if (n > SG_CAP) continue;
+      sort(n, sh.key);
+      return sh.sorted[min(max(k - (int)above - 1, 0), n - 1)];
+    }
+    // ties, or outliers that leave too few steps for the rest: bisection of the key
+    uint32_t kth = 0;
+#pragma unroll 1
+    for (int b = 31; b >= 0; --b) {
+      const uint32_t next = kth | 1u << b;
+      if (next <= key_of(sh.max_x) && (next < kLowest || count_from(of_key(next)) >= k)) kth = next;
+    }
+    return kth < kLowest ? 0 : kth;
+  }
+  // `total` +- `error`: the mass from top-k's bound `kth` on.
+  static __device__ __noinline__ uint32_t top_p_bound(uint32_t kth, double total, double error, float near) {
+    SampleShared& sh = shared();
+    int precise = 0;
+#pragma unroll 1
+    for (int attempt = 0; attempt < 2; ++attempt) {
+      const float range = fminf(24.f * (float)sh.T64, attempt == 0 ? near : sh.max_x - least());
+      if (!usable(range)) continue;
+      const float scale = (SG_BINS - 1) / range;
+      double off = 0.;
+      // Where the steps' masses point to; if the bound does not lie there, as far on as their sum was off.
+#pragma unroll 1
+      for (int turn = 0; turn < 4; ++turn) {
+        histogram(scale, from(kth));
+        float unused;
+        const int bin = find_bin((float)fmax(sh.p * total - off, 0.), scale, true, unused);
+        if (bin >= SG_BINS - 1 && attempt == 0) break;
+        const int first = min(max(bin - 2, 0), SG_BINS - 1), last = min(bin + 2, SG_BINS - 1);
+        const double guess = mass_of_bins(first, scale);
+        const float high = first > 0 ? of_key(edge_of(first, scale)) : INFINITY;
+        const uint32_t low = max(last == SG_BINS - 1 ? kLowest : edge_of(last + 1, scale), kth);
+        const int n = gather(from(low), high);
+        if (n > SG_CAP) break;
+        if (n > 0) sort(n, sh.key);
+        Verdict verdict;
+        double above;
+#pragma unroll 1
+        for (;; precise = 1) {
+          if (precise && error > 0.) total = mass(true, from(kth), error);
+          double blur = 0.;
+          above = first > 0 ? mass(precise, fmaxf(high, from(kth)), blur) : 0.;
+          verdict = bound(n, above, sh.p * total, blur + sh.p * error, last == SG_BINS - 1 || low == kth);
+          if (verdict != kAmbiguous) break;
+        }
+        if (verdict == kDone) return sh.low;
+        off = above - guess;
+      }
+    }
+#pragma unroll 1
+    for (;; precise = 1) {  // bisection: the largest key such that it and those above hold more than the share
+      if (precise && error > 0.) total = mass(true, from(kth), error);
+      const double share = sh.p * total;
+      bool unsure = false;
+      uint32_t cut = 0;
+#pragma unroll 1
+      for (int b = 31; b >= 0; --b) {
+        const uint32_t next = cut | 1u << b;
+        double blur = 0., s = 0.;
+        if (next <= key_of(sh.max_x)) s = mass(precise, from(max(next, kth)), blur);
+        blur += sh.p * error;
+        unsure |= blur > 0. && fabs(s - share) <= blur;
+        if (s > share) cut = next;
+      }
+      if (!unsure) return cut;
+    }
+  }
+
+  // ---------------------------------------------------------------- the row
+  static __device__ __forceinline__ void run(float top) {
+    SampleShared& sh = shared();
+    const int t = threadIdx.x, lane = t & 31, w = t / 32;
+    const float max_x = sh.max_x;
+    // min-p as a bound on the key: the least whose weight reaches it, among the 32 around max + T ln m, or where that window
+    // lies above it (temperatures at which neighbours have the same weight) by a search.
+    if (sh.use_m && w == 0) {
+      const uint32_t max_key = key_of(max_x);
+      const auto reaches = [&](uint32_t key) { return weight(of_key(key)) >= sh.m || key >= max_key; };
+      const uint32_t mid = key_of((float)fmax(max_x + sh.T64 * log(sh.m), -3.4e38)), low = max(mid, kLowest + 16) - 16;
+      const uint32_t ok = __ballot_sync(0xffffffff, reaches(low + lane));
+      uint32_t key = ok ? min(low + __ffs(ok) - 1, max_key) : max_key;
+      if (ok & 1) key = least_key(lane, kLowest, key, reaches);
+      if (lane == 0) sh.low = key;
+    }
+    const bool by_k = sh.use_k && sh.k <= SG_LIST_K;
     // A bound that all candidates of top-k, or the SG_LIST_K largest logits, reach.
     uint32_t low = 0xFFFFFFFFu;
-    if (by_k || (r.use_p && !r.use_k)) {
-      const auto full = [&](int n) { return n < 32 ? 0 : min((n - 32) / chunk + 1, SG_WARPS); };  // warps without an idle lane
-      const int warps = (cs - 1) * full(per) + full(vecs.n - (cs - 1) * per);
-      const int j = warps > 0 ? ((by_k ? r.k : SG_LIST_K) + warps - 1) / warps : 33;
+    if (sh.use_k || sh.use_p) {
+      const int chunk = sh.chunk, n = RowVecs<T>(static_cast<const T*>(sh.row), sh.V).n;
+      const int warps = n < 32 ? 0 : min((n - 32) / chunk + 1, kWarps);  // without an idle lane
+      const int j = warps > 0 ? ((by_k ? sh.k : SG_LIST_K) + warps - 1) / warps : 33;
       uint32_t key = key_of(top);
       if (j > 32) {
         low = 0;
-      } else if (w < full(v1 - v0)) {
+      } else if (w < warps) {
+#pragma unroll 1
         for (int i = 0;; ++i) {
           low = __reduce_max_sync(0xffffffff, key);
           if (i == j - 1) break;
@@ -615,255 +807,159 @@ __global__ void __launch_bounds__(SG_THREADS, 2) sample_given_kernel(const Sampl
         }
       }
     }
-    low = r.min_key(low);  // and its barrier for sh.low
-    const uint32_t low_m = r.use_m ? sh.low : 0;
-    double total = 0.;
-    if (r.use_p && !by_k && !r.use_k) total = masses(false, -INFINITY).total;
-    double total_error = error;
-    if (by_list) {
-      uint32_t bound = by_k || r.use_p ? low : 0;
-      bool complete = by_k || bound == 0;
-      if (r.use_m && !(by_k && r.use_p) && low_m >= bound) bound = low_m, complete = true;
-      // below all numbers: -inf and the padding have no mass
-      const float reach = bound <= key_of(-INFINITY) ? -3.4028235e38f : of_key(bound);
-      const bool hopeless = !complete && masses(false, reach).total < 0.999 * r.p * total;
-      const int n = hopeless ? SG_CAP + 1 : gather(reach, [](float) { return true; });
-      if (n <= SG_CAP) {
-        if (rank == 0) order_list(r, n);
-        for (int precise = 0;; ++precise) {
-          if (rank == 0 && w == 0) answer_from_list(r, n, complete, low_m, total, total_error, token, logprob);
-          r.sync();
-          const int verdict = lead->verdict;
-          r.sync();
-          if (verdict == kDone) return;
-          if (verdict == kIncomplete) break;
-          total = masses(true, -INFINITY).total;
-          total_error = 0.;
-        }
-      } else {
-        r.sync();  // the leader's count has been read
+    low = min_of(low);  // and its barrier for sh.low
+    const uint32_t low_m = sh.use_m ? sh.low : 0;
+    double total = 0., error = 0.;
+    if (sh.use_p && !sh.use_k) total = mass(false, -INFINITY, error);
+    if (by_k || (!sh.use_k && (sh.use_p || sh.use_m))) {
+      uint32_t least = by_k || sh.use_p ? low : 0;
+      bool complete = by_k || least == 0;  // no token below the candidates can be kept
+      if (sh.use_m && !(by_k && sh.use_p) && low_m >= least) least = low_m, complete = true;
+      const int n = gather(from(least), INFINITY);
+      bool may = n <= SG_CAP;
+      if (may && !complete) {  // where the candidates' mass cannot reach top-p's bound they need no order
+        float s = 0.f;
+        for (int i = t; i < n; i += NT) s += exp2_fast((of_key(sh.key[i]) - max_x) * sh.c);
+        may = !(scan((double)s).y < 0.999 * sh.p * total);
       }
-    }
-
-    // Many tokens stay. A histogram of the logits over equal steps down from the largest.
-    float least = INFINITY;
-    for_vecs([&](const uint4& u, int) {
-      float x[E];
-      vec_floats<T>(u, x);
-#pragma unroll
-      for (int e = 0; e < E; ++e) least = fminf(least, x[e] > -INFINITY ? x[e] : least);
-    });
-    least = of_key(r.min_key(key_of(least)));
-    float range = r.max_x - least;
-    if (r.use_p && !r.use_k) range = fminf(range, 24.f * (float)r.T64);
-    const bool flat = !(range > 0.f);  // all numbers are equal
-    const float scale = flat ? 0.f : (SG_BINS - 1) / range;
-    const auto bin_of = [&](float x) { return min((int)((r.max_x - x) * scale), SG_BINS - 1); };
-    constexpr int kEach = SG_BINS / SG_THREADS;
-    uint32_t count[kEach];  // of this thread's bins, over the row
-    const bool by_bins = scale > 0.f && isfinite(scale) && (r.use_p || r.use_k);
-    if (by_bins) {
-#pragma unroll
-      for (int i = 0; i < kEach; ++i) sh.bins[t * kEach + i] = 0;
-      __syncthreads();
-      for_vecs([&](const uint4& u, int) {
-        float x[E];
-        vec_floats<T>(u, x);
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-          if (x[e] > -INFINITY) atomicAdd(&sh.bins[bin_of(x[e])], 1u);
-      });
-      r.sync();
-#pragma unroll
-      for (int i = 0; i < kEach; ++i) count[i] = 0;
-      for (int o = 0; o < cs; ++o) {
-        const uint32_t* theirs = cs > 1 ? cg::this_cluster().map_shared_rank(sh.bins, o) : sh.bins;
-#pragma unroll
-        for (int i = 0; i < kEach; ++i) count[i] += theirs[t * kEach + i];
-      }
-      r.sync();  // the bins give way to the list's weights
-    }
-    // The first bin at which the running sum of `of`(bin, count) exceeds `share`, SG_BINS if none does; `above`: the sum
-    // before it.
-    const auto find_bin = [&](double share, auto of, double& above) {
-      double s = 0.;
-#pragma unroll
-      for (int i = 0; i < kEach; ++i) s += of(t * kEach + i, count[i]);
-      double scan = s;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const double up = __shfl_up_sync(0xffffffff, scan, o);
-        if (lane >= o) scan += up;
-      }
-      if (t == 0) sh.found = SG_BINS;
-      if (lane == 31) sh.scan64[w] = scan;
-      __syncthreads();
-      double base = 0.;
-      for (int i = 0; i < w; ++i) base += sh.scan64[i];
-      double before = base + scan - s;
-      if (before <= share && base + scan > share) {
-        bool done = false;
-        for (int i = 0; i < kEach; ++i) {
-          const double one = of(t * kEach + i, count[i]);
-          if (!done && before + one > share) {
-            atomicMin(&sh.found, t * kEach + i);
-            done = true;
+      if (may) {
+        if (sh.use_k || sh.use_p) sort(n, sh.key);
+        uint32_t cut = low_m;
+        Verdict verdict = kDone;
+        int members = n;
+        if (by_k) {
+          const uint32_t kth = sh.k <= n ? sh.sorted[sh.k - 1] : 0;
+          cut = max(cut, kth);
+          if (sh.use_p) {
+            members = 0;
+#pragma unroll 1
+            for (int i = t; i - t < n; i += NT) members += __syncthreads_count(i < n && sh.sorted[i] >= kth);
           }
-          if (!done) before += one;
         }
-      }
-      __syncthreads();
-      const int bin = sh.found;
-      if (bin / kEach == t) sh.scan64[0] = before;
-      __syncthreads();
-      above = sh.scan64[0];
-      __syncthreads();
-      return bin;
-    };
-
-    uint32_t kth = 0;  // top-k's bound
-    if (r.use_k && flat) {
-      kth = key_of(r.max_x);
-    } else if (r.use_k) {
-      bool found = false;
-      if (by_bins) {
-        double above;
-        const int bin = find_bin(r.k - 0.5, [](int, uint32_t n) { return (double)n; }, above);
-        if (bin == SG_BINS) {
-          found = true;  // fewer numbers than k
-        } else {
-          if (rank == 0 && t == 0) sh.n = 0;
-          r.sync();
-          const int n = gather(-3.4028235e38f, [&](float x) { return bin_of(x) == bin; });
-          if (n <= SG_CAP) {
-            if (rank == 0) {
-              order_list(r, n);
-              if (t == 0) sh.low = key_part(sh.sorted[min(max(r.k - (int)above - 1, 0), n - 1)]);
-            }
-            found = true;
+        if (sh.use_p) {
+#pragma unroll 1
+          for (;;) {
+            if (by_k) total = mass_before(members);
+            verdict = bound(members, 0., sh.p * total, sh.p * error, complete);
+            if (verdict != kAmbiguous) break;
+            total = mass(true, -INFINITY, error);
           }
-          r.sync();
-          kth = lead->low;
-          r.sync();
-          if (!found) kth = 0;
+          cut = max(cut, sh.low);
         }
-      }
-      if (!found) {  // ties, or outliers that leave too few steps for the rest: bisection of the key
-#pragma unroll 1
-        for (int b = 31; b >= 0; --b) {
-          const uint32_t next = kth | 1u << b;
-          int n = 0;
-          each([&](float x, int) { n += key_of(x) >= next; });
-          if (r.count(n) >= r.k) kth = next;
+        if (verdict == kDone) {
+          draw_from_list(n, cut);
+          return;
         }
       }
     }
-    const auto from = [&](uint32_t key) { return key <= key_of(-3.4028235e38f) ? -3.4028235e38f : of_key(key); };
-    uint32_t cut = 0;  // top-p's bound
-    if (r.use_p && flat) {
-      cut = key_of(r.max_x);
-    } else if (r.use_p) {
-      bool found = false;
-      if (r.use_k) {
-        total = masses(false, from(kth)).total;
-        total_error = error;
-      }
-      int first = 0, last = -1, n = 0;
-      if (by_bins) {
-        // the steps around the one that the weights at their middles point to
-        double above;
-        const int bin = find_bin(r.p * total, [&](int b, uint32_t n) {
-          return n ? n * (double)exp2_fast(-((float)b + 0.5f) / scale * c) : 0.;
-        }, above);
-        first = max(bin - 2, 0);
-        last = min(bin + 2, SG_BINS - 1);
-        if (rank == 0 && t == 0) sh.n = 0;
-        r.sync();
-        n = gather(from(kth), [&](float x) {
-          const int b = bin_of(x);
-          return b >= first && b <= last;
-        });
-        if (n <= SG_CAP && rank == 0) order_list(r, n);
-        r.sync();
-      }
-#pragma unroll 1
-      for (int precise = 0; precise < 2 && !found; ++precise) {
-        if (precise) {
-          total = masses(true, from(kth)).total;
-          total_error = 0.;
-        }
-        const double share = r.p * total, blur = r.p * total_error;
-        if (by_bins && n <= SG_CAP) {
-          // the least number of the steps above: a bound between them and those gathered
-          float edge = INFINITY;
-          each([&](float x, int) { if (x > -INFINITY && bin_of(x) < first) edge = fminf(edge, x); });
-          edge = of_key(r.min_key(key_of(edge)));
-          const double above = edge < INFINITY ? masses(precise, fmaxf(edge, from(kth))).total : (error = 0., 0.);
-          if (rank == 0 && w == 0) bound_from_list(r, n, last == SG_BINS - 1, above, error, share, blur);
-          r.sync();
-          const int verdict = lead->verdict;
-          cut = lead->low;
-          r.sync();
-          if (verdict == kDone) break;
-          if (verdict == kAmbiguous) continue;
-        }
-        // Bisection: the largest key such that it and those above hold more than the share.
-        bool unsure = false;
-        cut = 0;
-#pragma unroll 1
-        for (int b = 31; b >= 0; --b) {
-          const uint32_t next = cut | 1u << b;
-          const double s = next > key_of(r.max_x) ? (error = 0., 0.) : masses(precise, from(max(next, kth))).total;
-          unsure |= error + blur > 0. && fabs(s - share) <= error + blur;
-          if (s > share) cut = next;
-        }
-        found = !unsure;
-      }
+    const float near = low < kLowest || low > key_of(max_x) ? 0.f : 4.f * (max_x - of_key(low));
+    uint32_t cut = low_m;
+    if (sh.use_k) {
+      const uint32_t kth = top_k_bound(sh.k, near);
+      if (sh.use_p) total = mass(false, from(kth), error);
+      cut = max(cut, sh.use_p ? max(kth, top_p_bound(kth, total, error, near)) : kth);
+    } else if (sh.use_p) {
+      cut = max(cut, top_p_bound(0, total, error, near));
     }
-    draw(from(max(max(kth, cut), low_m)));
-  };
-  run();
-  if (cs > 1) cg::this_cluster().sync();  // no CTA leaves while others read its memory
+    draw(from(cut));
+  }
+};
+
+// HELD: the logits stay in shared memory.
+template <typename T, bool HELD>
+__global__ void __launch_bounds__(SG_THREADS, 2) sample_given_kernel(const SampleGivenArgs a) {
+  constexpr int NT = SG_THREADS;
+  using S = Sampler<T, HELD>;
+  SampleShared& sh = S::shared();
+  const int t = threadIdx.x, lane = t & 31, row = blockIdx.x;
+  begin_early();
+  const T* x = static_cast<const T*>(a.x) + (long long)row * a.ldx;
+  const RowVecs<T> vecs(x, a.V);
+  const int chunk = (vecs.n + NT - 1) / NT * 32;
+  const int group = HELD ? chunk / 32 : ((chunk / 32 + SG_GROUPS - 1) / SG_GROUPS + SG_VECS - 1) / SG_VECS * SG_VECS;
+  const int w0 = t / 32 * chunk, mine = max(0, min(chunk / 32, (min(w0 + chunk, vecs.n) - w0 - lane + 31) / 32));
+  float top = -INFINITY, top_here = -INFINITY;
+  bool nan = false;
+#pragma unroll 1
+  for (int i0 = 0; i0 < mine; i0 += SG_VECS) {
+    uint4 u[SG_VECS];
+#pragma unroll
+    for (int i = 0; i < SG_VECS; ++i) u[i] = i0 + i < mine ? vecs.load(w0 + (i0 + i) * 32 + lane) : vec_neg_inf<T>();
+#pragma unroll
+    for (int i = 0; i < SG_VECS; ++i) {
+      if (HELD && i0 + i < mine) S::held()[(i0 + i) * NT + t] = u[i];
+      const float most = vec_max<T>(u[i]);
+      nan |= most != most;
+      top_here = fmaxf(top_here, most);
+    }
+    if (!HELD && ((i0 + SG_VECS) % group == 0 || i0 + SG_VECS >= mine)) {
+      S::tops()[i0 / group * NT + t] = top_here;
+      top = fmaxf(top, top_here);
+      top_here = -INFINITY;
+    }
+  }
+  if (HELD) S::tops()[chunk / 32 * NT * 4 + t] = top = top_here;  // behind the vectors
+  const float temperature = a.temperature[row];
+  const bool greedy = !(temperature > 0.f);
+  if (t == 0) {
+    sh.row = x;
+    sh.V = a.V, sh.chunk = chunk, sh.group = group;
+    sh.T64 = (double)(greedy ? 1.f : fminf(fmaxf(temperature, 1e-8f), 3.4e38f));
+    sh.c64 = 16. * 1.4426950408889634 / sh.T64;
+    sh.c = (float)(1.4426950408889634 / sh.T64);
+    sh.k = a.top_k[row];
+    sh.use_k = !greedy && sh.k > 0 && sh.k < a.V;
+    const float p = a.top_p[row], m = a.min_p[row];
+    sh.use_p = !greedy && p < 1.f;
+    sh.use_m = !greedy && m > 0.f;
+    sh.p = sh.use_p ? fmax((double)p, 0.) : 1.;
+    sh.m = sh.use_m ? fmin((double)m, 1.) : 0.;
+    const double u = a.uniform64 ? static_cast<const double*>(a.uniform)[row] : (double)static_cast<const float*>(a.uniform)[row];
+    sh.draw = fmin(fmax(u, 0.), 1.);  // a NaN becomes 0
+    sh.token = a.token + row;
+    sh.logprob = a.logprob ? a.logprob + row : nullptr;
+  }
+  if (t >= 32 && t < 48) sh.pow.at[t - 32] = exp2((t - 32) / 16.);
+  const uint32_t max_key = S::max_of(key_of(nan ? of_key(0xFFFFFFFFu) : top));
+  if (t == 0) sh.max_x = of_key(max_key);
+  __syncthreads();
+  if (!(fabsf(of_key(max_key)) < INFINITY)) {  // a NaN, an infinity or nothing allowed: no distribution; the largest number
+    const float most = of_key(S::max_of(key_of(top)));  // -inf where there is none but NaN
+    const uint32_t id = S::first_id(most);
+    if (t == 0) {
+      *sh.token = id < (uint32_t)a.V ? id : 0;
+      if (sh.logprob) *sh.logprob = __int_as_float(0x7FC00000);
+    }
+  } else if (greedy) {
+    const uint32_t id = S::first_id(of_key(max_key));
+    const double total = sh.logprob ? S::mass_32(-INFINITY) : 1.;
+    if (t == 0) S::answer((int)id, of_key(max_key), total);
+  } else {
+    S::run(top);
+  }
 }
+
+constexpr int SG_MAX_SMEM = 113 * 1024;  // two CTAs on an SM
 
 template <typename T, bool HELD>
 void sample_given_launch(const SampleGivenArgs& a, int smem, int device, cudaStream_t s) {
   auto* kernel = sample_given_kernel<T, HELD>;
   static bool ready[64] = {};  // per device
   if (device < 0 || device >= 64 || !ready[device]) {
-    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SG_VECS * SG_THREADS * 16);
+    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SG_MAX_SMEM);
     if (device >= 0 && device < 64) ready[device] = true;
   }
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)a.rows * a.cluster);
-  cfg.blockDim = dim3(SG_THREADS);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute at[2]{};
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  at[1].id = cudaLaunchAttributeClusterDimension;
-  at[1].val.clusterDim.x = a.cluster;
-  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = a.cluster > 1 ? 2 : 1;
-  note_launch();
-  cudaLaunchKernelEx(&cfg, kernel, a);
+  launch_early(kernel, dim3((unsigned)a.rows), dim3(SG_THREADS), smem, s, a);
 }
 
 template <typename T>
-void sample_given_sized(SampleGivenArgs a, int device, cudaStream_t s) {
+void sample_given_typed(const SampleGivenArgs& a, int device, cudaStream_t s) {
   constexpr int E = LogitType<T>::E;
   const int vecs = (a.V + E - 1) / E + 1;  // one more where a row starts off the grid
-  const int sms = astrai_host::num_sms(device);
-  const char* env = getenv("SG_CS");
-  int cs = 1;
-  while (cs < SG_MAX_CLUSTER && (long long)a.rows * cs * 2 <= sms && vecs >= cs * 2 * SG_THREADS) cs *= 2;
-  if (env) cs = atoi(env);
-  a.cluster = cs;
-  const int each = ((vecs + cs - 1) / cs + SG_THREADS - 1) / SG_THREADS;  // vectors of a thread
-  if (each <= SG_VECS) sample_given_launch<T, true>(a, each * SG_THREADS * 16, device, s);
-  else sample_given_launch<T, false>(a, 0, device, s);
+  const int state = ((int)sizeof(SampleShared) + 15) / 16 * 16;
+  const int held = (vecs + SG_THREADS - 1) / SG_THREADS * SG_THREADS * 16 + SG_THREADS * 4;
+  if (held <= SG_MAX_SMEM - state) sample_given_launch<T, true>(a, state + held, device, s);
+  else sample_given_launch<T, false>(a, state + SG_GROUPS * SG_THREADS * 4, device, s);
 }
 
 }  // namespace astrai
@@ -874,10 +970,10 @@ using namespace astrai;
 void sample_given(const void* x, long long ldx, int rows, int V, const void* uniform, bool uniform64,
                   const float* temperature, const int* top_k, const float* top_p, const float* min_p, long long* token,
                   float* logprob, int dtype, int device, cudaStream_t s) {
-  const SampleGivenArgs a{x, ldx, rows, V, 1, uniform, uniform64, temperature, top_k, top_p, min_p, token, logprob};
-  if (dtype == 0) sample_given_sized<__nv_bfloat16>(a, device, s);
-  else if (dtype == 1) sample_given_sized<__half>(a, device, s);
-  else sample_given_sized<float>(a, device, s);
+  const SampleGivenArgs a{x, ldx, rows, V, uniform, uniform64, temperature, top_k, top_p, min_p, token, logprob};
+  if (dtype == 0) sample_given_typed<__nv_bfloat16>(a, device, s);
+  else if (dtype == 1) sample_given_typed<__half>(a, device, s);
+  else sample_given_typed<float>(a, device, s);
 }
 
 }  // namespace astrai_host
