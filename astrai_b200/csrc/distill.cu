@@ -11,12 +11,18 @@
 // and the loss is the mean over the rows that count; s is the gradient of the loss over their number.
 //
 // The sums run over the tokens outside J and over J apart: q_0 as 1 - sum q_jk would lose what a good student leaves to
-// the others. The tokens of J are marked in shared memory and read as -inf in the pass over the row, which leaves their
-// base gradient at zero; one thread for each entry then writes its gradient over it.
+// the others. The tokens of J are overwritten with -inf in the CTA's copy of the row, which leaves their base gradient at
+// zero; their own gradients are written over it.
 //
-// A row is read once, into registers: a CTA of 512 threads holds up to 64 KB of it (NV vectors of 16 bytes a thread),
-// a longer row is shared by a cluster of CTAs that exchange their maxima and sums through distributed shared memory.
+// Persistent CTAs take row after row: a bulk copy brings the row into shared memory, NT threads take the maximum, the sum and
+// the gradient from there, and one more warp does what is small: J and its sums, the row's coefficients and loss, the copy of
+// the next row. Three CTAs share an SM, so that one row is copied or written while others are computed. (With the row in
+// registers and J spread over 512 threads, 60 % of the instructions were the same few for every thread: 8192 rows of 32000
+// took 373 us, forward only 220.) A row that does not fit is shared by a cluster, whose extra warps exchange the sums through
+// distributed shared memory.
 #include <cooperative_groups.h>
+
+#include <algorithm>
 
 #include "launch.cuh"
 #include "logits.cuh"
@@ -25,11 +31,10 @@ namespace astrai {
 
 namespace cg = cooperative_groups;
 
-constexpr int DST_THREADS = 512;
-constexpr int DST_WARPS = DST_THREADS / 32;
 constexpr int DST_MAX_K = 1024;
-constexpr int DST_KI = DST_MAX_K / DST_THREADS;  // entries of a thread
 constexpr int DST_MAX_CLUSTER = 16;
+constexpr int DST_VECS = 4352;  // vectors of a row in one CTA: 68 KB, three CTAs on an SM
+constexpr int DST_MAX_SMEM = 224 * 1024;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 
 struct DistillArgs {
@@ -51,6 +56,7 @@ struct DistillArgs {
   float expected;
   int unless_expected;    // nothing is done if *grad == expected
   float* row_loss;        // null: not wanted
+  int* err;
 };
 
 __device__ __forceinline__ bool row_counts(const long long* target, long long ignore, int row, int V, long long& y) {
@@ -58,29 +64,6 @@ __device__ __forceinline__ bool row_counts(const long long* target, long long ig
   if (!target) return true;
   y = target[row];
   return y != ignore && y >= 0 && y < V;
-}
-
-// Several values of every thread reduced over the CTA, the same result in all threads: MAX of them as maxima, the others as
-// sums in a fixed order. `part` holds N floats per warp; a barrier separates two uses of it.
-template <int N, bool MAX>
-__device__ __forceinline__ void block_reduce(float (&v)[N], float* part) {
-  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
-#pragma unroll
-  for (int i = 0; i < N; ++i) v[i] = MAX ? warp_max(v[i]) : warp_sum(v[i]);
-  if (lane == 0) {
-#pragma unroll
-    for (int i = 0; i < N; ++i) part[i * DST_WARPS + w] = v[i];
-  }
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < N; ++i) {
-    v[i] = part[i * DST_WARPS + (lane & (DST_WARPS - 1))];
-#pragma unroll
-    for (int o = DST_WARPS / 2; o > 0; o >>= 1) {
-      const float u = __shfl_xor_sync(0xffffffff, v[i], o);
-      v[i] = MAX ? fmaxf(v[i], u) : v[i] + u;
-    }
-  }
 }
 
 __device__ __forceinline__ float teacher_value(const DistillArgs& a, long long i) {
@@ -106,226 +89,368 @@ struct Mass {
   __device__ float inv_rel_on() const { return exp2_fast(d - m) / sum; }
 };
 
-template <typename T, int NV, bool TRAIN, bool TWO>
-__global__ void __launch_bounds__(DST_THREADS, 2) distill_kernel(const DistillArgs a) {
-  constexpr int E = LogitType<T>::E;
-  __shared__ __align__(4) uint8_t mask[DST_THREADS * NV];
-  __shared__ float part_max[3 * DST_WARPS], part_sum[6 * DST_WARPS];
-  __shared__ float mine[6];
-  __shared__ int twice;
-  const int t = threadIdx.x;
+// One entry of the teacher in shared memory.
+struct Entry {
+  int id;       // -1: none
+  float value;  // over tau; then its mass
+  float x;      // the student's logit
+  int here;     // in this CTA's part of the row
+};
+
+// What the extra warp tells the others about a row: gradients outside J are sum of base 2^((x - ref) c).
+struct Coefficients {
+  float ref, base, base1;
+};
+
+constexpr int DST_AHEAD = 4;  // entries of a lane that are read one row ahead
+
+__device__ __forceinline__ uint32_t remote(const void* p, int rank) {  // the same place in another CTA of the cluster
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ bool wait_cluster(uint64_t* bar, uint32_t parity, int* err) {
+  const uint64_t t0 = globaltimer();
+  for (;;) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity), "r"(0x989680u)
+        : "memory");
+    if (ok) return true;
+    if (globaltimer() - t0 > ASTRAI_WAIT_NS) {
+      set_error(err, kErrWaitPeer);
+      return false;
+    }
+  }
+}
+
+// f(vector number) for this thread's vectors, four at a time
+template <int NT, typename F>
+__device__ __forceinline__ void each_vec(int n, F f) {
+  int v = threadIdx.x;
+#pragma unroll 1
+  for (; v + 3 * NT < n; v += 4 * NT) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f(v + i * NT);
+  }
+#pragma unroll 1
+  for (; v < n; v += NT) f(v);
+}
+
+template <typename T, int NT, bool TRAIN, bool TWO>
+__global__ void __launch_bounds__(NT + 32) distill_kernel(const DistillArgs a, int held) {
+  constexpr int E = LogitType<T>::E, W = NT / 32;
+  using Bits = typename std::conditional<E == 4, uint32_t, uint16_t>::type;
+  extern __shared__ __align__(128) unsigned char distill_smem[];  // the row's vectors, then the entries
+  uint4* const buffer = reinterpret_cast<uint4*>(distill_smem);
+  Bits* const elements = reinterpret_cast<Bits*>(distill_smem);
+  Entry* const entries = reinterpret_cast<Entry*>(distill_smem + held);
+  __shared__ float part_max[W], part_sum[2 * W];
+  __shared__ Coefficients coefs;
+  __shared__ float theirs[2][DST_MAX_CLUSTER][6];
+  __shared__ uint64_t full, told;
+  const int t = threadIdx.x, lane = t & 31, w = t >> 5;
   const int cs = a.cluster, rank = cs > 1 ? (int)cg::this_cluster().block_rank() : 0;
-  const int row = blockIdx.x / cs;
+  const int stride = gridDim.x / cs;
   begin_early();
   float g = a.expected;
   if (a.grad) {
     g = *a.grad;
     if (a.unless_expected && g == a.expected) return;
   }
-  const T* x = static_cast<const T*>(a.x) + (long long)row * a.ldx;
-  T* dx = TRAIN ? static_cast<T*>(a.dx) + (long long)row * a.lddx : nullptr;
-  const RowVecs<T> vecs(x, a.V);
-  const int per = (vecs.n + cs - 1) / cs, v0 = rank * per, v1 = min(v0 + per, vecs.n);
-  long long y;
-  if (!row_counts(a.target, a.ignore, row, a.V, y)) {  // the same for the whole cluster
-    if constexpr (TRAIN)
-      for (int v = v0 + t; v < v1; v += DST_THREADS) vecs.store(dx, v, make_uint4(0, 0, 0, 0));
-    if (a.row_loss && rank == 0 && t == 0) a.row_loss[row] = 0.f;
-    return;
+  if (t == 0) {
+    mbar_init(&full, 1);
+    mbar_init(&told, cs);
+    fence_mbar_init();
   }
+  if (cs > 1) cg::this_cluster().sync();
+  else __syncthreads();
 
-  uint4 u[NV];
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int v = v0 + t + i * DST_THREADS;
-    u[i] = v < v1 ? vecs.load(v) : vec_neg_inf<T>();
-  }
-  const auto id_at = [&](int k) -> long long {
+  const bool extra = w == W;
+  const float c = a.inv_tau * LOG2E;
+  const float scale = TRAIN ? g / (a.count ? fmaxf(*a.count, 1.f) : (float)max(a.rows, 1)) : 0.f;
+  const auto row_vecs = [&](int row) { return RowVecs<T>(static_cast<const T*>(a.x) + (long long)row * a.ldx, a.V); };
+  // the whole vectors of this CTA's part of a row; a cut first or last one is read by element
+  const auto issue = [&](int row) {
+    const RowVecs<T> v = row_vecs(row);
+    const int per = (v.n + cs - 1) / cs, v0 = rank * per, v1 = min(v0 + per, v.n);
+    const int b = v0 + (v0 < v1 && !v.whole(v0)), e = v1 - (v0 < v1 && !v.whole(v1 - 1));
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // behind the marks in the row before
+    if (b < e) {
+      mbar_expect_tx(&full, (uint32_t)(e - b) * 16);
+      bulk_load(buffer + (b - v0), v.row + v.first(b), (uint32_t)(e - b) * 16, &full);
+    } else {
+      mbar_arrive(&full);
+    }
+  };
+  const auto counts = [&](int row, long long& y) { return row < a.rows && row_counts(a.target, a.ignore, row, a.V, y); };
+  const auto id_at = [&](int row, int k) -> long long {
     const long long at = (long long)row * a.K + k;
     return a.ids64 ? static_cast<const long long*>(a.ids)[at] : static_cast<const int*>(a.ids)[at];
   };
-  int id[DST_KI];
-  float tv[DST_KI], xj[DST_KI];
+  // The extra warp reads a row's small inputs one row ahead, the labels two.
+  long long y, y_next = -1, id_next[DST_AHEAD];
+  float value_next[DST_AHEAD], rest_next = -INFINITY;
+  const auto look_ahead = [&](int row) {
 #pragma unroll
-  for (int i = 0; i < DST_KI; ++i) {
-    const int k = t + i * DST_THREADS;
-    id[i] = -1;
-    tv[i] = xj[i] = -INFINITY;
-    if (k < a.K) {
-      const long long j = id_at(k);
-      if (j >= 0 && j < a.V) {
-        id[i] = (int)j;
-        tv[i] = teacher_value(a, (long long)row * a.K + k) * a.inv_tau;
-        xj[i] = LogitType<T>::one(x[j]);
+    for (int i = 0; i < DST_AHEAD; ++i) {
+      const int k = lane + i * 32;
+      if (k < a.K) {
+        id_next[i] = id_at(row, k);
+        value_next[i] = teacher_value(a, (long long)row * a.K + k);
       }
     }
+    rest_next = a.rest ? a.rest[row] : -INFINITY;
+  };
+  int row = blockIdx.x / cs, turn = 0;
+  uint32_t phase = 0, told_phase = 0;
+  bool counted = counts(row, y);
+  if (extra && counted) {
+    if (lane == 0) issue(row);
+    look_ahead(row);
   }
-  const float rest = a.rest ? a.rest[row] : -INFINITY;
-  const float xy = y >= 0 ? LogitType<T>::one(x[y]) : 0.f;
-  for (int i = t; i < DST_THREADS * NV / 4; i += DST_THREADS) reinterpret_cast<uint32_t*>(mask)[i] = 0;
-  if (t == 0) twice = 0;
-  __syncthreads();
-  // marks of the entries in this CTA's part of the row
-  bool here[DST_KI], first[DST_KI];
-#pragma unroll
-  for (int i = 0; i < DST_KI; ++i) {
-    const int v = (id[i] + vecs.head) / E;
-    first[i] = here[i] = id[i] >= 0 && v >= v0 && v < v1;
-    if (here[i]) {
-      const uint32_t b = 1u << (8 * ((v - v0) & 3) + (id[i] + vecs.head) % E);
-      if (atomicOr(reinterpret_cast<uint32_t*>(mask) + (v - v0) / 4, b) & b) twice = 1;
-    }
-  }
-  __syncthreads();
-  if (twice) {  // an id that comes again: the student's mass there counts once, with the first of them
+  bool counted_next = counts(row + stride, y_next);
+
 #pragma unroll 1
-    for (int i = 0; i < DST_KI; ++i)
-      for (int l = 0; first[i] && l < t + i * DST_THREADS; ++l)
-        if (id_at(l) == id[i]) first[i] = false;
-  }
-
-  const float c = a.inv_tau * LOG2E;
-  float mx[3] = {rest, -INFINITY, -INFINITY};  // teacher; student on J, outside J
-#pragma unroll
-  for (int i = 0; i < DST_KI; ++i) {
-    mx[0] = fmaxf(mx[0], tv[i]);
-    mx[1] = fmaxf(mx[1], xj[i]);
-  }
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const uint32_t bits = mask[t + i * DST_THREADS];
-    if (bits) vec_mask<T>(u[i], bits);
-    float f[E];
-    vec_floats<T>(u[i], f);
-#pragma unroll
-    for (int e = 0; e < E; ++e) mx[2] = fmaxf(mx[2], f[e]);
-  }
-  block_reduce<3, true>(mx, part_max);
-  const float mt = ref_of(mx[0]), mj = ref_of(mx[1]), mr = ref_of(mx[2]);
-
-  // teacher's mass on J; sum of its mass * (log p - log q) up to constants; student's sums on J and outside, over tau and
-  // at 1
-  float sum[6] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-  float pe[DST_KI];
-#pragma unroll
-  for (int i = 0; i < DST_KI; ++i) {
-    const float th = tv[i] - mt, zh = (xj[i] - mj) * a.inv_tau;
-    pe[i] = id[i] >= 0 ? exp2_fast(th * LOG2E) : 0.f;
-    sum[0] += pe[i];
-    if (pe[i] != 0.f) sum[1] += pe[i] * (th - zh);
-    if (first[i]) {
-      sum[2] += exp2_fast(zh * LOG2E);
-      if constexpr (TWO) sum[3] += exp2_fast((xj[i] - mj) * LOG2E);
-    }
-  }
-  float mo = mr;  // the logit that the sums outside J are relative to
-  const Pair c2(c, c), log2e2(LOG2E, LOG2E);
-  {
-    const Pair ref2(-mo, -mo);
-    Pair s2(0.f, 0.f), s1(0.f, 0.f);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      Pair p[E / 2];
-      vec_pairs<T>(u[i], p);
-#pragma unroll
-      for (int e = 0; e < E / 2; ++e) {
-        const Pair d = p[e] + ref2;
-        s2 = s2 + exp2_fast(d * c2);
-        if constexpr (TWO) s1 = s1 + exp2_fast(d * log2e2);
+  for (; row < a.rows; row += stride, counted = counted_next, y = y_next, counted_next = counts(row + stride, y_next)) {
+    const RowVecs<T> vecs = row_vecs(row);
+    T* const dx = TRAIN ? static_cast<T*>(a.dx) + (long long)row * a.lddx : nullptr;
+    const int per = (vecs.n + cs - 1) / cs, v0 = rank * per, v1 = min(v0 + per, vecs.n), nv = max(v1 - v0, 0);
+    if (!counted) {  // the same for the whole cluster
+      if constexpr (TRAIN)
+        for (int v = v0 + t; v < v1; v += NT + 32) vecs.store(dx, v, make_uint4(0, 0, 0, 0));
+      if (a.row_loss && rank == 0 && t == 0) a.row_loss[row] = 0.f;
+      if (extra && counted_next) {
+        if (lane == 0) issue(row + stride);
+        look_ahead(row + stride);
       }
+      continue;
     }
-    sum[4] = s2.sum();
-    if constexpr (TWO) sum[5] = s1.sum();
-  }
-  block_reduce<6, false>(sum, part_sum);
+    if (!mbar_wait(&full, phase, a.err, kErrWaitFull)) return;  // (then all threads run out of time)
+    phase ^= 1;
+    // ---- the extra warp: cut vectors, the entries and their logits, -inf in their place
+    const int base_id = vecs.first(v0);  // the id of the buffer's first element
+    float rest = 0.f, xy = 0.f, mt = -INFINITY, mj = -INFINITY;
+    bool repeated = false;
+    if (extra) {
+      if (nv > 0 && lane < 2) {
+        const int v = lane == 0 ? v0 : v1 - 1;
+        if (!vecs.whole(v)) buffer[v - v0] = vecs.load(v);
+      }
+      __syncwarp();
+      rest = rest_next;
+      xy = y >= 0 ? LogitType<T>::one(vecs.row[y]) : 0.f;
+#pragma unroll 1
+      for (int k = lane, i = 0; k < a.K; k += 32, ++i) {
+        long long j = id_next[0];
+        float value = value_next[0];
+#pragma unroll
+        for (int q = 1; q < DST_AHEAD; ++q)
+          if (i == q) j = id_next[q], value = value_next[q];
+        if (i >= DST_AHEAD) {
+          j = id_at(row, k);
+          value = teacher_value(a, (long long)row * a.K + k);
+        }
+        Entry n{-1, -INFINITY, -INFINITY, 0};
+        if (j >= 0 && j < a.V) {
+          n.id = (int)j;
+          n.value = value * a.inv_tau;
+          const int at = n.id - base_id;
+          n.here = at >= 0 && at < nv * E;
+          n.x = LogitType<T>::one(n.here ? reinterpret_cast<const T*>(elements)[at] : vecs.row[j]);
+        }
+        entries[k] = n;
+        mt = fmaxf(mt, n.value);
+        mj = fmaxf(mj, n.x);
+      }
+      __syncwarp();
+      // every entry leaves its number; one that finds another's has an id that comes again
+      for (int k = lane; k < a.K; k += 32)
+        if (entries[k].here) elements[entries[k].id - base_id] = (Bits)k;
+      __syncwarp();
+      for (int k = lane; k < a.K; k += 32) repeated |= entries[k].here && elements[entries[k].id - base_id] != (Bits)k;
+      repeated = __any_sync(0xffffffff, repeated);
+      for (int k = lane; k < a.K; k += 32)
+        if (entries[k].here) elements[entries[k].id - base_id] = (Bits)LogitType<T>::kNegInf;
+    }
+    __syncthreads();
 
-  float on = sum[2], on1 = sum[3], out = sum[4], out1 = sum[5];
-  if (cs > 1) {  // the sums of all CTAs, those outside J relative to this one's reference
-    cg::cluster_group cl = cg::this_cluster();
-    if (t == 0) {
-      mine[0] = mx[2];
-      mine[1] = out;
-      mine[2] = out1;
-      mine[3] = on;
-      mine[4] = on1;
+    // ---- the largest logit outside J
+    if (!extra) {
+      float m0 = -INFINITY;
+      each_vec<NT>(nv, [&](int v) { m0 = fmaxf(m0, vec_max_number<T>(buffer[v])); });
+      m0 = of_key(__reduce_max_sync(0xffffffff, key_of(m0)));
+      if (lane == 0) part_max[w] = m0;
     }
-    cl.sync();
-    const int lane = t & 31;
-    const float* theirs = cl.map_shared_rank(mine, lane < cs ? lane : 0);
-    const float m = lane < cs ? theirs[0] : -INFINITY;
-    if (mx[2] == -INFINITY) mo = ref_of(warp_max(m));  // none of its own: one that others have
-    const bool some = m != -INFINITY;
-    out = warp_sum(some ? theirs[1] * exp2_fast((m - mo) * c) : 0.f);
-    if constexpr (TWO) out1 = warp_sum(some ? theirs[2] * exp2_fast((m - mo) * LOG2E) : 0.f);
-    on = warp_sum(lane < cs ? theirs[3] : 0.f);
-    if constexpr (TWO) on1 = warp_sum(lane < cs ? theirs[4] : 0.f);
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  }
-  if (out == 0.f) mo = mj;  // nothing outside J
-  const Mass z(out, on, on == 0.f ? -INFINITY : (mj - mo) * c);
-  const Mass z1(TWO ? out1 : out, TWO ? on1 : on, on == 0.f ? -INFINITY : (mj - mo) * (TWO ? LOG2E : c));
-  // the teacher's share outside J
-  const float pr = rest == -INFINITY ? 0.f : exp2_fast((rest - mt) * LOG2E);
-  const float mass = sum[0] + pr, inv = mass != 0.f ? 1.f / mass : 0.f;
-  const float p0 = pr * inv;
+    // teacher's mass on J; sum of its mass * (log p - log q) up to constants; the student's sums on J, over tau and at 1
+    float teach = 0.f, cross = 0.f, on = 0.f, on1 = 0.f;
+    if (extra) {
+      mt = ref_of(fmaxf(warp_max(mt), rest));
+      const float top = warp_max(mj);
+      mj = ref_of(top);
+#pragma unroll 1
+      for (int k = lane; k < a.K; k += 32) {
+        const Entry n = entries[k];
+        const float th = n.value - mt, zh = (n.x - mj) * a.inv_tau, e = n.id >= 0 ? exp2_fast(th * LOG2E) : 0.f;
+        entries[k].value = e;
+        teach += e;
+        if (e != 0.f) cross += e * (th - zh);
+        bool first = n.here;  // the student's mass at an id that comes again counts once, with the first of them
+        for (int l = 0; repeated && first && l < k; ++l) first = entries[l].id != n.id;
+        if (first) {
+          on += exp2_fast(zh * LOG2E);
+          if constexpr (TWO) on1 += exp2_fast((n.x - mj) * LOG2E);
+        }
+      }
+      teach = warp_sum(teach);
+      cross = warp_sum(cross);
+      on = warp_sum(on);
+      if constexpr (TWO) on1 = warp_sum(on1);
+    }
+    __syncthreads();
 
-  if (a.row_loss && rank == 0 && t == 0) {
-    // sum_k p_k (log p_k - log q_jk) = (sum e_k (th - zh)) / mass + (sum of p_k) (log of q's sum - log mass)
-    float loss = 0.f;
-    if (mass != 0.f) {
-      const float logm = logf(mass);
-      if (sum[0] != 0.f) loss = sum[1] * inv + sum[0] * inv * (z.log2_rel_on() * LN2 - logm);
-      if (p0 != 0.f) loss += p0 * ((rest - mt) - logm + z.log2_all_over_outside() * LN2);
-      loss *= a.kl_loss;
+    // ---- sums outside J, over tau and at 1
+    float most = part_max[lane & (W - 1)];
+#pragma unroll
+    for (int o = W / 2; o > 0; o >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffff, most, o));
+    const Pair c2(c, c), log2e2(LOG2E, LOG2E);
+    if (!extra) {
+      const Pair ref2(-ref_of(most), -ref_of(most));
+      Pair s2(0.f, 0.f), s1(0.f, 0.f);
+      each_vec<NT>(nv, [&](int v) {
+        Pair p[E / 2];
+        vec_pairs<T>(buffer[v], p);
+#pragma unroll
+        for (int e = 0; e < E / 2; ++e) {
+          const Pair d = p[e] + ref2;
+          s2 = s2 + exp2_fast(d * c2);
+          if constexpr (TWO) s1 = s1 + exp2_fast(d * log2e2);
+        }
+      });
+      const float a2 = warp_sum(s2.sum()), a1 = TWO ? warp_sum(s1.sum()) : 0.f;
+      if (lane == 0) part_sum[w] = a2, part_sum[W + w] = a1;
     }
-    if (a.hard > 0.f) loss += a.hard * ((mo - xy) + z1.log2_rel_outside() * LN2);
-    a.row_loss[row] = loss;
-  }
-  if constexpr (TRAIN) {
-    const float s = g / (a.count ? fmaxf(*a.count, 1.f) : (float)max(a.rows, 1));
-    const float all = mass != 0.f ? 1.f : 0.f;
-    const float kl = s * a.kl_grad, ce = s * a.hard;
-    const float share = out != 0.f ? p0 / out : 0.f;
-    const float base = kl * (all * z.inv_rel_outside() - share) + (TWO ? 0.f : ce * z.inv_rel_outside());
-    const float base1 = TWO ? ce * z1.inv_rel_outside() : 0.f;
-    const Pair ref2(-mo, -mo), base2(base, base), base12(base1, base1);
-    const auto outside = [&](Pair p) {
-      p = p + ref2;
-      const Pair d = base2 * exp2_fast(p * c2);
-      if constexpr (TWO) return fma2(base12, exp2_fast(p * log2e2), d);
+    __syncthreads();
+
+    // ---- the extra warp: the row's coefficients and loss
+    float kl = 0.f, ce = 0.f, inv = 0.f, all = 0.f, inv_on = 0.f, inv_on1 = 0.f;
+    if (extra) {
+      float mo = ref_of(most);  // the logit that the sums outside J are relative to
+      float out = warp_sum(lane < W ? part_sum[lane] : 0.f), out1 = TWO ? warp_sum(lane < W ? part_sum[W + lane] : 0.f) : 0.f;
+      if (cs > 1) {  // of all CTAs, those outside J relative to this one's reference
+        if (lane < cs) {
+          const float own[5] = {most, out, out1, on, on1};
+          const uint32_t to = remote(&theirs[turn][rank][0], lane);
+#pragma unroll
+          for (int i = 0; i < 5; ++i)
+            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 4 * i), "f"(own[i]) : "memory");
+          asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote(&told, lane)) : "memory");
+        }
+        __syncwarp();
+        if (!wait_cluster(&told, told_phase, a.err)) return;  // (no copy follows: the others run out of time)
+        told_phase ^= 1;
+        const float* their = theirs[turn][lane < cs ? lane : 0];
+        const float m = lane < cs ? their[0] : -INFINITY;
+        if (most == -INFINITY) mo = ref_of(warp_max(m));  // none of its own: one that others have
+        const bool some = m != -INFINITY;
+        out = warp_sum(some ? their[1] * exp2_fast((m - mo) * c) : 0.f);
+        if constexpr (TWO) out1 = warp_sum(some ? their[2] * exp2_fast((m - mo) * LOG2E) : 0.f);
+        on = warp_sum(lane < cs ? their[3] : 0.f);
+        if constexpr (TWO) on1 = warp_sum(lane < cs ? their[4] : 0.f);
+      }
+      if (out == 0.f) mo = mj;  // nothing outside J
+      const Mass z(out, on, on == 0.f ? -INFINITY : (mj - mo) * c);
+      const Mass z1(TWO ? out1 : out, TWO ? on1 : on, on == 0.f ? -INFINITY : (mj - mo) * (TWO ? LOG2E : c));
+      // the teacher's share outside J
+      const float pr = rest == -INFINITY ? 0.f : exp2_fast((rest - mt) * LOG2E);
+      const float mass = teach + pr;
+      inv = mass != 0.f ? 1.f / mass : 0.f;
+      const float p0 = pr * inv;
+      if constexpr (TRAIN) {
+        all = mass != 0.f ? 1.f : 0.f;
+        kl = scale * a.kl_grad, ce = scale * a.hard;
+        inv_on = z.inv_rel_on();
+        inv_on1 = TWO ? z1.inv_rel_on() : inv_on;
+        const float share = out != 0.f ? p0 / out : 0.f;
+        if (lane == 0) {
+          coefs.ref = mo;
+          coefs.base = kl * (all * z.inv_rel_outside() - share) + (TWO ? 0.f : ce * z.inv_rel_outside());
+          coefs.base1 = TWO ? ce * z1.inv_rel_outside() : 0.f;
+        }
+        __syncthreads();
+      }
+      if (a.row_loss && rank == 0 && lane == 0) {
+        // sum_k p_k (log p_k - log q_jk) = (sum e_k (th - zh)) / mass + (sum of p_k) (log of q's sum - log mass)
+        float loss = 0.f;
+        if (mass != 0.f) {
+          const float logm = logf(mass);
+          if (teach != 0.f) loss = cross * inv + teach * inv * (z.log2_rel_on() * LN2 - logm);
+          if (p0 != 0.f) loss += p0 * ((rest - mt) - logm + z.log2_all_over_outside() * LN2);
+          loss *= a.kl_loss;
+        }
+        if (a.hard > 0.f) loss += a.hard * ((mo - xy) + z1.log2_rel_outside() * LN2);
+        a.row_loss[row] = loss;
+      }
+    } else if constexpr (TRAIN) {
+      __syncthreads();
+    }
+    // ---- the gradient outside J
+    const auto outside = [&](Pair p, const Coefficients& k) {
+      p = p + Pair(-k.ref, -k.ref);
+      const Pair d = Pair(k.base, k.base) * exp2_fast(p * c2);
+      if constexpr (TWO) return fma2(Pair(k.base1, k.base1), exp2_fast(p * log2e2), d);
       return d;
     };
+    if constexpr (TRAIN) {
+      if (!extra) {
+        const Coefficients k = coefs;
+        const int b = v0 < v1 && !vecs.whole(v0) ? 1 : 0, e = nv - (nv > 0 && !vecs.whole(v1 - 1));
+        T* const to = dx + base_id;
+        each_vec<NT>(nv, [&](int v) {
+          Pair p[E / 2];
+          vec_pairs<T>(buffer[v], p);
 #pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int v = v0 + t + i * DST_THREADS;
-      if (v >= v1) break;
-      Pair p[E / 2];
-      vec_pairs<T>(u[i], p);
-#pragma unroll
-      for (int e = 0; e < E / 2; ++e) p[e] = outside(p[e]);
-      vecs.store(dx, v, pairs_round<T>(p));
-    }
-    __syncthreads();  // the base gradient lies before the entries' gradients
-#pragma unroll 1
-    for (int i = 0; i < DST_KI; ++i) {
-      if (!here[i]) continue;
-      float p = pe[i] * inv;
-      if (twice) {  // the teacher's mass of all entries with this id, the same whichever of them writes it
-        p = 0.f;
-        for (int l = 0; l < a.K; ++l)
-          if (id_at(l) == id[i])
-            p += exp2_fast((teacher_value(a, (long long)row * a.K + l) * a.inv_tau - mt) * LOG2E) * inv;
+          for (int e = 0; e < E / 2; ++e) p[e] = outside(p[e], k);
+          const uint4 u = pairs_round<T>(p);
+          if (v >= b && v < e) *reinterpret_cast<uint4*>(to + v * E) = u;
+          else vecs.store(dx, v0 + v, u);
+        });
       }
-      const float q = exp2_fast((xj[i] - mj) * c) * z.inv_rel_on();
-      const float q1 = TWO ? exp2_fast((xj[i] - mj) * LOG2E) * z1.inv_rel_on() : q;
-      dx[id[i]] = LogitType<T>::round(kl * (q * all - p) + ce * (q1 - (id[i] == y ? 1.f : 0.f)));
     }
-    if (t == 0 && y >= 0 && ce != 0.f) {
-      const int v = ((int)y + vecs.head) / E, bit = ((int)y + vecs.head) % E;
-      if (v >= v0 && v < v1 && !(mask[v - v0] >> bit & 1)) dx[y] = LogitType<T>::round(outside(Pair(xy, xy)).get().x - ce);
+    if (extra && counted_next) look_ahead(row + stride);
+    __syncthreads();  // the base gradient lies before the entries'; the buffer has been read
+    if (extra) {
+      if (counted_next && lane == 0) issue(row + stride);
+      if constexpr (TRAIN) {
+        bool label = false;  // is it one of the entries
+#pragma unroll 1
+        for (int k = lane; k < a.K; k += 32) {
+          const Entry n = entries[k];
+          label |= n.id >= 0 && n.id == y;
+          if (!n.here) continue;
+          float p = n.value * inv;
+          if (repeated) {  // the teacher's mass of all entries with this id, the same whichever of them writes it
+            p = 0.f;
+            for (int l = 0; l < a.K; ++l)
+              if (entries[l].id == n.id) p += entries[l].value * inv;
+          }
+          const float q = exp2_fast((n.x - mj) * c) * inv_on;
+          const float q1 = TWO ? exp2_fast((n.x - mj) * LOG2E) * inv_on1 : q;
+          dx[n.id] = LogitType<T>::round(kl * (q * all - p) + ce * (q1 - (n.id == y ? 1.f : 0.f)));
+        }
+        label = __any_sync(0xffffffff, label);
+        if (lane == 0 && y >= 0 && ce != 0.f && !label && y >= base_id && y - base_id < nv * E)
+          dx[y] = LogitType<T>::round(outside(Pair(xy, xy), coefs).get().x - ce);
+      }
+      __syncwarp();
     }
+    turn ^= 1;
   }
-  if (cs > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // others may still read `mine`
+  if (cs > 1) cg::this_cluster().sync();  // others may still write here
 }
 
 // count[0] = rows that count
@@ -364,47 +489,65 @@ __global__ void __launch_bounds__(1024) distill_mean_kernel(const float* row_los
   }
 }
 
-template <typename T, int NV, bool TRAIN, bool TWO>
-void distill_launch(const DistillArgs& a, cudaStream_t s) {
-  auto* kernel = distill_kernel<T, NV, TRAIN, TWO>;
+template <typename T, int NT, bool TRAIN, bool TWO>
+void distill_launch(const DistillArgs& a, int vecs, int device, cudaStream_t s) {
+  auto* kernel = distill_kernel<T, NT, TRAIN, TWO>;
+  const int held = (vecs * 16 + 127) / 128 * 128, smem = held + a.K * (int)sizeof(Entry);
+  static bool ready[64] = {};  // per device
+  if (device < 0 || device >= 64 || !ready[device]) {
+    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, DST_MAX_SMEM);
+    cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+    if (device >= 0 && device < 64) ready[device] = true;
+  }
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)a.rows * a.cluster);
-  cfg.blockDim = dim3(DST_THREADS);
+  cfg.gridDim = dim3(a.cluster);
+  cfg.blockDim = dim3(NT + 32);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cudaLaunchAttribute at[2]{};
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  at[1].id = cudaLaunchAttributeClusterDimension;
-  at[1].val.clusterDim.x = a.cluster;
-  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = a.cluster;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
-  cfg.numAttrs = a.cluster > 1 ? 2 : 1;
-  if (a.cluster > 8) cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+  // as many clusters as run at once, each with rows of its own
+  int most = 0;
+  if (a.cluster > 1) {
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&most, kernel, &cfg) != cudaSuccess) most = 0;
+  } else if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&most, kernel, NT + 32, smem) != cudaSuccess) {
+    most = 0;
+  } else {
+    most *= astrai_host::num_sms(device);
+  }
+  if (most < 1) most = 1;
+  cfg.gridDim = dim3((unsigned)(std::min(a.rows, most) * a.cluster));
+  cfg.numAttrs = 2;
+  if (a.cluster == 1) cfg.attrs = at + 1, cfg.numAttrs = 1;
   note_launch();
-  cudaLaunchKernelEx(&cfg, kernel, a);
+  cudaLaunchKernelEx(&cfg, kernel, a, held);
 }
 
 template <typename T, bool TRAIN, bool TWO>
-void distill_sized(DistillArgs a, cudaStream_t s) {
+void distill_sized(DistillArgs a, int device, cudaStream_t s) {
   constexpr int E = LogitType<T>::E;
   const int vecs = (a.V + E - 1) / E + 1;  // one more where a row starts off the grid
   int cs = 1;
-  while ((vecs + cs - 1) / cs > DST_THREADS * 8) cs *= 2;
+  while ((vecs + cs - 1) / cs > DST_VECS) cs *= 2;
   a.cluster = cs;
   const int per = (vecs + cs - 1) / cs;
-  if (per <= DST_THREADS) return distill_launch<T, 1, TRAIN, TWO>(a, s);
-  if (per <= DST_THREADS * 2) return distill_launch<T, 2, TRAIN, TWO>(a, s);
-  if (per <= DST_THREADS * 4) return distill_launch<T, 4, TRAIN, TWO>(a, s);
-  distill_launch<T, 8, TRAIN, TWO>(a, s);
+  if (per <= 1024) return distill_launch<T, 128, TRAIN, TWO>(a, per, device, s);
+  distill_launch<T, 256, TRAIN, TWO>(a, per, device, s);
 }
 
 template <typename T>
-void distill_typed(const DistillArgs& a, cudaStream_t s) {
+void distill_typed(const DistillArgs& a, int device, cudaStream_t s) {
   const bool two = a.hard > 0.f && a.inv_tau != 1.f;
   if (a.dx)
-    two ? distill_sized<T, true, true>(a, s) : distill_sized<T, true, false>(a, s);
+    two ? distill_sized<T, true, true>(a, device, s) : distill_sized<T, true, false>(a, device, s);
   else
-    two ? distill_sized<T, false, true>(a, s) : distill_sized<T, false, false>(a, s);
+    two ? distill_sized<T, false, true>(a, device, s) : distill_sized<T, false, false>(a, device, s);
 }
 
 }  // namespace astrai
@@ -414,21 +557,21 @@ using namespace astrai;
 
 int distill_max_k() { return DST_MAX_K; }
 // longest row for elements of this size
-int distill_max_vocab(int elem) { return DST_MAX_CLUSTER * DST_THREADS * 8 * (16 / elem) - 16 / elem; }
+int distill_max_vocab(int elem) { return DST_MAX_CLUSTER * DST_VECS * (16 / elem) - 16 / elem; }
 
 void distill(const void* x, long long ldx, void* dx, long long lddx, const void* ids, bool ids64, const void* values,
              int values_type, const float* rest, const long long* target, long long ignore, int rows, int V, int K,
              float tau, float hard, const float* grad, float expected, bool unless_expected, float* row_loss,
-             float* count, bool have_count, float* loss, int dtype, cudaStream_t s) {
+             float* count, bool have_count, float* loss, int dtype, int device, cudaStream_t s) {
   if (target && !have_count)
     launch_early(distill_count_kernel, dim3(1), dim3(1024), 0, s, target, ignore, rows, V, count);
   DistillArgs a{x, ldx, dx, lddx, ids, ids64, values, values_type, rest, target, ignore, rows, V, K, 1, 1.f / tau,
                 (1.f - hard) * tau * tau, (1.f - hard) * tau, hard, target ? count : nullptr, grad, expected,
-                unless_expected, row_loss};
+                unless_expected, row_loss, astrai_host::error_word(device)};
   if (rows > 0) {
-    if (dtype == 0) distill_typed<__nv_bfloat16>(a, s);
-    else if (dtype == 1) distill_typed<__half>(a, s);
-    else distill_typed<float>(a, s);
+    if (dtype == 0) distill_typed<__nv_bfloat16>(a, device, s);
+    else if (dtype == 1) distill_typed<__half>(a, device, s);
+    else distill_typed<float>(a, device, s);
   }
   if (loss)
     launch_early(distill_mean_kernel, dim3(1), dim3(1024), 0, s, (const float*)row_loss, rows,

@@ -93,6 +93,22 @@ __device__ __forceinline__ void vec_mask(uint4& u, uint32_t bits) {
   }
 }
 
+// Largest element, a NaN only if there is nothing else.
+template <typename T>
+__device__ __forceinline__ float vec_max_number(const uint4& u) {
+  if constexpr (LogitType<T>::E == 4) {
+    return fmaxf(fmaxf(__uint_as_float(u.x), __uint_as_float(u.y)), fmaxf(__uint_as_float(u.z), __uint_as_float(u.w)));
+  } else if constexpr (std::is_same<T, __half>::value) {
+    const __half2* h = reinterpret_cast<const __half2*>(&u);
+    const float2 f = __half22float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
+    return fmaxf(f.x, f.y);
+  } else {
+    const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&u);
+    const float2 f = __bfloat1622float2(__hmax2(__hmax2(h[0], h[1]), __hmax2(h[2], h[3])));
+    return fmaxf(f.x, f.y);
+  }
+}
+
 // The vectors of one row.
 template <typename T>
 struct RowVecs {
