@@ -15,8 +15,9 @@
 // zero; their own gradients are written over it.
 //
 // Persistent CTAs take row after row: a bulk copy brings the row into shared memory, NT threads take the maximum, the sum and
-// the gradient from there, and one more warp does what is small: J and its sums, the row's coefficients and loss, the copy of
-// the next row. Three CTAs share an SM, so that one row is copied or written while others are computed. (With the row in
+// the gradient from there, and one more warp does what is small: the sums over J, the row's coefficients and loss, the copy of
+// the next row. A warp that works alone spends about 15 clocks on an instruction, so that the marks and gradients of J are
+// spread over all threads. Three CTAs share an SM, so that one row is copied or written while others are computed. (With the row in
 // registers and J spread over 512 threads, 60 % of the instructions were the same few for every thread: 8192 rows of 32000
 // took 373 us, forward only 220.) A row that does not fit is shared by a cluster, whose extra warps exchange the sums through
 // distributed shared memory.
@@ -59,12 +60,7 @@ struct DistillArgs {
   int* err;
 };
 
-__device__ __forceinline__ bool row_counts(const long long* target, long long ignore, int row, int V, long long& y) {
-  y = -1;
-  if (!target) return true;
-  y = target[row];
-  return y != ignore && y >= 0 && y < V;
-}
+__device__ __forceinline__ bool label_counts(long long y, long long ignore, int V) { return y != ignore && y >= 0 && y < V; }
 
 __device__ __forceinline__ float teacher_value(const DistillArgs& a, long long i) {
   if (a.values_type == 0) return __bfloat162float(static_cast<const __nv_bfloat16*>(a.values)[i]);
@@ -93,16 +89,15 @@ struct Mass {
 struct Entry {
   int id;       // -1: none
   float value;  // over tau; then its mass
-  float x;      // the student's logit
-  int here;     // in this CTA's part of the row
+  float x;      // the student's logit, in this CTA's part of the row
+  int here;     // it lies there
 };
 
-// What the extra warp tells the others about a row: gradients outside J are sum of base 2^((x - ref) c).
+// What the extra warp tells the others about a row: gradients outside J are base 2^((x - ref) c) + base1 2^((x - ref) log2 e).
 struct Coefficients {
   float ref, base, base1;
+  float kl, ce, inv, all, mj, inv_on, inv_on1;
 };
-
-constexpr int DST_AHEAD = 4;  // entries of a lane that are read one row ahead
 
 __device__ __forceinline__ uint32_t remote(const void* p, int rank) {  // the same place in another CTA of the cluster
   uint32_t r;
@@ -148,10 +143,12 @@ __global__ void __launch_bounds__(NT + 32) distill_kernel(const DistillArgs a, i
   extern __shared__ __align__(128) unsigned char distill_smem[];  // the row's vectors, then the entries
   uint4* const buffer = reinterpret_cast<uint4*>(distill_smem);
   Bits* const elements = reinterpret_cast<Bits*>(distill_smem);
-  Entry* const entries = reinterpret_cast<Entry*>(distill_smem + held);
+  Entry* const entries_of[2] = {reinterpret_cast<Entry*>(distill_smem + held),
+                                reinterpret_cast<Entry*>(distill_smem + held) + a.K};
   __shared__ float part_max[W], part_sum[2 * W];
   __shared__ Coefficients coefs;
-  __shared__ float theirs[2][DST_MAX_CLUSTER][6];
+  __shared__ float theirs[2][DST_MAX_CLUSTER][8];
+  __shared__ int twice[2];
   __shared__ uint64_t full, told;
   const int t = threadIdx.x, lane = t & 31, w = t >> 5;
   const int cs = a.cluster, rank = cs > 1 ? (int)cg::this_cluster().block_rank() : 0;
@@ -162,8 +159,9 @@ __global__ void __launch_bounds__(NT + 32) distill_kernel(const DistillArgs a, i
     g = *a.grad;
     if (a.unless_expected && g == a.expected) return;
   }
+  if (t < 2) twice[t] = 0;
   if (t == 0) {
-    mbar_init(&full, 1);
+    mbar_init(&full, 2);  // the copy, and the cut vectors
     mbar_init(&told, cs);
     fence_mbar_init();
   }
@@ -174,49 +172,78 @@ __global__ void __launch_bounds__(NT + 32) distill_kernel(const DistillArgs a, i
   const float c = a.inv_tau * LOG2E;
   const float scale = TRAIN ? g / (a.count ? fmaxf(*a.count, 1.f) : (float)max(a.rows, 1)) : 0.f;
   const auto row_vecs = [&](int row) { return RowVecs<T>(static_cast<const T*>(a.x) + (long long)row * a.ldx, a.V); };
-  // the whole vectors of this CTA's part of a row; a cut first or last one is read by element
-  const auto issue = [&](int row) {
+  // The extra warp: the whole vectors of this CTA's part of a row by the copy, a cut first or last one by element; finish()
+  // has what begin() loaded.
+  const auto begin = [&](int row, uint4& cut) {
     const RowVecs<T> v = row_vecs(row);
     const int per = (v.n + cs - 1) / cs, v0 = rank * per, v1 = min(v0 + per, v.n);
     const int b = v0 + (v0 < v1 && !v.whole(v0)), e = v1 - (v0 < v1 && !v.whole(v1 - 1));
-    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // behind the marks in the row before
-    if (b < e) {
-      mbar_expect_tx(&full, (uint32_t)(e - b) * 16);
-      bulk_load(buffer + (b - v0), v.row + v.first(b), (uint32_t)(e - b) * 16, &full);
-    } else {
-      mbar_arrive(&full);
+    if (lane == 0) {
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // behind the marks in the row before
+      if (b < e) {
+        mbar_expect_tx(&full, (uint32_t)(e - b) * 16);
+        bulk_load(buffer + (b - v0), v.row + v.first(b), (uint32_t)(e - b) * 16, &full);
+      } else {
+        mbar_arrive(&full);
+      }
     }
+    const int mine = lane == 0 ? v0 : v1 - 1;
+    if (lane < 2 && v0 < v1 && !v.whole(mine)) cut = v.load(mine);
   };
-  const auto counts = [&](int row, long long& y) { return row < a.rows && row_counts(a.target, a.ignore, row, a.V, y); };
+  const auto finish = [&](int row, const uint4& cut) {
+    const RowVecs<T> v = row_vecs(row);
+    const int per = (v.n + cs - 1) / cs, v0 = rank * per, v1 = min(v0 + per, v.n), mine = lane == 0 ? v0 : v1 - 1;
+    if (lane < 2 && v0 < v1 && !v.whole(mine)) buffer[mine - v0] = cut;
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&full);
+  };
   const auto id_at = [&](int row, int k) -> long long {
     const long long at = (long long)row * a.K + k;
     return a.ids64 ? static_cast<const long long*>(a.ids)[at] : static_cast<const int*>(a.ids)[at];
   };
-  // The extra warp reads a row's small inputs one row ahead, the labels two.
-  long long y, y_next = -1, id_next[DST_AHEAD];
-  float value_next[DST_AHEAD], rest_next = -INFINITY;
-  const auto look_ahead = [&](int row) {
-#pragma unroll
-    for (int i = 0; i < DST_AHEAD; ++i) {
-      const int k = lane + i * 32;
-      if (k < a.K) {
-        id_next[i] = id_at(row, k);
-        value_next[i] = teacher_value(a, (long long)row * a.K + k);
-      }
+  // Labels are read two rows ahead, the entries one.
+  const auto label_of = [&](int row) -> long long { return a.target && row < a.rows ? a.target[row] : -1; };
+  const auto counts = [&](int row, long long y) { return row < a.rows && (!a.target || label_counts(y, a.ignore, a.V)); };
+  // entry k of a row, the logit left out
+  const auto read_entry = [&](int row, int k, long long j, float value) {
+    Entry n{-1, -INFINITY, -INFINITY, 0};
+    if (j >= 0 && j < a.V) {
+      const RowVecs<T> v = row_vecs(row);
+      const int per = (v.n + cs - 1) / cs, v0 = rank * per, v1 = min(v0 + per, v.n), at = ((int)j + v.head) / E;
+      n.id = (int)j;
+      n.value = value * a.inv_tau;
+      n.here = at >= v0 && at < v1;
     }
-    rest_next = a.rest ? a.rest[row] : -INFINITY;
+    return n;
+  };
+  const auto fill_entries = [&](int row, Entry* entries, int from) {
+    for (int k = from; k < a.K; k += NT) entries[k] = read_entry(row, k, id_at(row, k), teacher_value(a, (long long)row * a.K + k));
   };
   int row = blockIdx.x / cs, turn = 0;
   uint32_t phase = 0, told_phase = 0;
-  bool counted = counts(row, y);
-  if (extra && counted) {
-    if (lane == 0) issue(row);
-    look_ahead(row);
+  long long y = label_of(row), y_next = label_of(row + stride), y_after;
+  uint4 cut = make_uint4(0, 0, 0, 0);
+  if (counts(row, y)) {
+    if (extra) {
+      begin(row, cut);
+      finish(row, cut);
+    } else {
+      fill_entries(row, entries_of[0], t);
+    }
   }
-  bool counted_next = counts(row + stride, y_next);
 
 #pragma unroll 1
-  for (; row < a.rows; row += stride, counted = counted_next, y = y_next, counted_next = counts(row + stride, y_next)) {
+  for (; row < a.rows; row += stride, y = y_next, y_next = y_after) {
+    y_after = label_of(row + 2 * stride);
+    const bool counted = counts(row, y), counted_next = counts(row + stride, y_next);
+    // this thread's first entry of the next row, on its way until the end of this one
+    const bool ahead = counted && counted_next && !extra && t < a.K;
+    long long id_next = -1;
+    float value_next = 0.f;
+    if (ahead) {
+      id_next = id_at(row + stride, t);
+      value_next = teacher_value(a, (long long)(row + stride) * a.K + t);
+    }
     const RowVecs<T> vecs = row_vecs(row);
     T* const dx = TRAIN ? static_cast<T*>(a.dx) + (long long)row * a.lddx : nullptr;
     const int per = (vecs.n + cs - 1) / cs, v0 = rank * per, v1 = min(v0 + per, vecs.n), nv = max(v1 - v0, 0);
@@ -224,60 +251,39 @@ __global__ void __launch_bounds__(NT + 32) distill_kernel(const DistillArgs a, i
       if constexpr (TRAIN)
         for (int v = v0 + t; v < v1; v += NT + 32) vecs.store(dx, v, make_uint4(0, 0, 0, 0));
       if (a.row_loss && rank == 0 && t == 0) a.row_loss[row] = 0.f;
-      if (extra && counted_next) {
-        if (lane == 0) issue(row + stride);
-        look_ahead(row + stride);
+      if (counted_next) {
+        if (extra) {
+          begin(row + stride, cut);
+          finish(row + stride, cut);
+        } else {
+          fill_entries(row + stride, entries_of[turn], t);
+        }
       }
       continue;
     }
+    Entry* const entries = entries_of[turn];
     if (!mbar_wait(&full, phase, a.err, kErrWaitFull)) return;  // (then all threads run out of time)
     phase ^= 1;
-    // ---- the extra warp: cut vectors, the entries and their logits, -inf in their place
+    // ---- the logits of J, and -inf in their places; every entry leaves its number in between: one that does not find it has
+    // an id that comes again
     const int base_id = vecs.first(v0);  // the id of the buffer's first element
-    float rest = 0.f, xy = 0.f, mt = -INFINITY, mj = -INFINITY;
-    bool repeated = false;
-    if (extra) {
-      if (nv > 0 && lane < 2) {
-        const int v = lane == 0 ? v0 : v1 - 1;
-        if (!vecs.whole(v)) buffer[v - v0] = vecs.load(v);
-      }
-      __syncwarp();
-      rest = rest_next;
-      xy = y >= 0 ? LogitType<T>::one(vecs.row[y]) : 0.f;
-#pragma unroll 1
-      for (int k = lane, i = 0; k < a.K; k += 32, ++i) {
-        long long j = id_next[0];
-        float value = value_next[0];
-#pragma unroll
-        for (int q = 1; q < DST_AHEAD; ++q)
-          if (i == q) j = id_next[q], value = value_next[q];
-        if (i >= DST_AHEAD) {
-          j = id_at(row, k);
-          value = teacher_value(a, (long long)row * a.K + k);
+    if (!extra)
+      for (int k = t; k < a.K; k += NT)
+        if (entries[k].here) {
+          const int at = entries[k].id - base_id;
+          entries[k].x = LogitType<T>::one(reinterpret_cast<const T*>(elements)[at]);
+          elements[at] = (Bits)k;
         }
-        Entry n{-1, -INFINITY, -INFINITY, 0};
-        if (j >= 0 && j < a.V) {
-          n.id = (int)j;
-          n.value = value * a.inv_tau;
-          const int at = n.id - base_id;
-          n.here = at >= 0 && at < nv * E;
-          n.x = LogitType<T>::one(n.here ? reinterpret_cast<const T*>(elements)[at] : vecs.row[j]);
-        }
-        entries[k] = n;
-        mt = fmaxf(mt, n.value);
-        mj = fmaxf(mj, n.x);
-      }
-      __syncwarp();
-      // every entry leaves its number; one that finds another's has an id that comes again
-      for (int k = lane; k < a.K; k += 32)
-        if (entries[k].here) elements[entries[k].id - base_id] = (Bits)k;
-      __syncwarp();
-      for (int k = lane; k < a.K; k += 32) repeated |= entries[k].here && elements[entries[k].id - base_id] != (Bits)k;
-      repeated = __any_sync(0xffffffff, repeated);
-      for (int k = lane; k < a.K; k += 32)
-        if (entries[k].here) elements[entries[k].id - base_id] = (Bits)LogitType<T>::kNegInf;
-    }
     __syncthreads();
+    if (!extra)
+      for (int k = t; k < a.K; k += NT)
+        if (entries[k].here) {
+          const int at = entries[k].id - base_id;
+          if (elements[at] != (Bits)k) twice[turn] = 1;
+          elements[at] = (Bits)LogitType<T>::kNegInf;
+        }
+    __syncthreads();
+    const bool repeated = twice[turn];
 
     // ---- the largest logit outside J
     if (!extra) {
@@ -286,33 +292,49 @@ __global__ void __launch_bounds__(NT + 32) distill_kernel(const DistillArgs a, i
       m0 = of_key(__reduce_max_sync(0xffffffff, key_of(m0)));
       if (lane == 0) part_max[w] = m0;
     }
-    // teacher's mass on J; sum of its mass * (log p - log q) up to constants; the student's sums on J, over tau and at 1
-    float teach = 0.f, cross = 0.f, on = 0.f, on1 = 0.f;
+    __syncthreads();
+
+    // ---- the extra warp: the sums over J
+    // the teacher's mass on J; of it that with a logit here; the sum of mass * (log p - log q) up to constants, the first part
+    // with the cluster's first CTA, the second with each one's own; the student's sums here, over tau and at 1
+    float rest = -INFINITY, mt = -INFINITY, mj = -INFINITY, teach = 0.f, own = 0.f, cross = 0.f, on = 0.f, on1 = 0.f;
+    bool label = false;  // it is one of the entries
     if (extra) {
-      mt = ref_of(fmaxf(warp_max(mt), rest));
-      const float top = warp_max(mj);
-      mj = ref_of(top);
-#pragma unroll 1
+      if (a.rest) rest = a.rest[row];
+#pragma unroll 2
       for (int k = lane; k < a.K; k += 32) {
         const Entry n = entries[k];
-        const float th = n.value - mt, zh = (n.x - mj) * a.inv_tau, e = n.id >= 0 ? exp2_fast(th * LOG2E) : 0.f;
+        if (repeated && n.here) entries[k].x = LogitType<T>::one(vecs.row[n.id]);  // another's number may have been read
+        mt = fmaxf(mt, n.value);
+        mj = fmaxf(mj, n.here ? entries[k].x : -INFINITY);
+        label |= n.id >= 0 && n.id == y;
+      }
+      label = __any_sync(0xffffffff, label);
+      mt = ref_of(fmaxf(of_key(__reduce_max_sync(0xffffffff, key_of(mt))), rest));
+      mj = of_key(__reduce_max_sync(0xffffffff, key_of(mj)));
+      const float ref = ref_of(mj);
+#pragma unroll 2
+      for (int k = lane; k < a.K; k += 32) {
+        const Entry n = entries[k];
+        const float th = n.value - mt, zh = (n.x - ref) * a.inv_tau, e = n.id >= 0 ? exp2_fast(th * LOG2E) : 0.f;
         entries[k].value = e;
         teach += e;
-        if (e != 0.f) cross += e * (th - zh);
-        bool first = n.here;  // the student's mass at an id that comes again counts once, with the first of them
+        if (e != 0.f && rank == 0) cross += e * th;
+        if (!n.here) continue;
+        if (e != 0.f) cross -= e * zh, own += e;
+        bool first = true;  // the student's mass at an id that comes again counts once, with the first of its entries
         for (int l = 0; repeated && first && l < k; ++l) first = entries[l].id != n.id;
         if (first) {
           on += exp2_fast(zh * LOG2E);
-          if constexpr (TWO) on1 += exp2_fast((n.x - mj) * LOG2E);
+          if constexpr (TWO) on1 += exp2_fast((n.x - ref) * LOG2E);
         }
       }
       teach = warp_sum(teach);
       cross = warp_sum(cross);
       on = warp_sum(on);
       if constexpr (TWO) on1 = warp_sum(on1);
+      if (cs > 1) own = warp_sum(own);
     }
-    __syncthreads();
-
     // ---- sums outside J, over tau and at 1
     float most = part_max[lane & (W - 1)];
 #pragma unroll
@@ -335,51 +357,54 @@ __global__ void __launch_bounds__(NT + 32) distill_kernel(const DistillArgs a, i
       if (lane == 0) part_sum[w] = a2, part_sum[W + w] = a1;
     }
     __syncthreads();
+    if (!TRAIN && extra && counted_next) begin(row + stride, cut);  // the buffer has been read
 
     // ---- the extra warp: the row's coefficients and loss
-    float kl = 0.f, ce = 0.f, inv = 0.f, all = 0.f, inv_on = 0.f, inv_on1 = 0.f;
     if (extra) {
       float mo = ref_of(most);  // the logit that the sums outside J are relative to
       float out = warp_sum(lane < W ? part_sum[lane] : 0.f), out1 = TWO ? warp_sum(lane < W ? part_sum[W + lane] : 0.f) : 0.f;
-      if (cs > 1) {  // of all CTAs, those outside J relative to this one's reference
+      if (cs > 1) {  // of all CTAs, relative to one reference
         if (lane < cs) {
-          const float own[5] = {most, out, out1, on, on1};
+          const float mine[8] = {most, out, out1, mj, on, on1, cross, own};
           const uint32_t to = remote(&theirs[turn][rank][0], lane);
 #pragma unroll
-          for (int i = 0; i < 5; ++i)
-            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 4 * i), "f"(own[i]) : "memory");
+          for (int i = 0; i < 8; ++i)
+            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 4 * i), "f"(mine[i]) : "memory");
           asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote(&told, lane)) : "memory");
         }
         __syncwarp();
         if (!wait_cluster(&told, told_phase, a.err)) return;  // (no copy follows: the others run out of time)
         told_phase ^= 1;
         const float* their = theirs[turn][lane < cs ? lane : 0];
-        const float m = lane < cs ? their[0] : -INFINITY;
+        const float m = lane < cs ? their[0] : -INFINITY, m_on = lane < cs ? their[3] : -INFINITY;
         if (most == -INFINITY) mo = ref_of(warp_max(m));  // none of its own: one that others have
         const bool some = m != -INFINITY;
         out = warp_sum(some ? their[1] * exp2_fast((m - mo) * c) : 0.f);
         if constexpr (TWO) out1 = warp_sum(some ? their[2] * exp2_fast((m - mo) * LOG2E) : 0.f);
-        on = warp_sum(lane < cs ? their[3] : 0.f);
-        if constexpr (TWO) on1 = warp_sum(lane < cs ? their[4] : 0.f);
+        mj = ref_of(warp_max(m_on));
+        const bool some_on = m_on != -INFINITY;
+        on = warp_sum(some_on ? their[4] * exp2_fast((m_on - mj) * c) : 0.f);
+        if constexpr (TWO) on1 = warp_sum(some_on ? their[5] * exp2_fast((m_on - mj) * LOG2E) : 0.f);
+        cross = warp_sum(lane < cs ? their[6] - (some_on ? their[7] * ((m_on - mj) * a.inv_tau) : 0.f) : 0.f);
+      } else {
+        mj = ref_of(mj);
       }
       if (out == 0.f) mo = mj;  // nothing outside J
       const Mass z(out, on, on == 0.f ? -INFINITY : (mj - mo) * c);
       const Mass z1(TWO ? out1 : out, TWO ? on1 : on, on == 0.f ? -INFINITY : (mj - mo) * (TWO ? LOG2E : c));
       // the teacher's share outside J
       const float pr = rest == -INFINITY ? 0.f : exp2_fast((rest - mt) * LOG2E);
-      const float mass = teach + pr;
-      inv = mass != 0.f ? 1.f / mass : 0.f;
+      const float mass = teach + pr, inv = mass != 0.f ? 1.f / mass : 0.f;
       const float p0 = pr * inv;
       if constexpr (TRAIN) {
-        all = mass != 0.f ? 1.f : 0.f;
-        kl = scale * a.kl_grad, ce = scale * a.hard;
-        inv_on = z.inv_rel_on();
-        inv_on1 = TWO ? z1.inv_rel_on() : inv_on;
+        const float all = mass != 0.f ? 1.f : 0.f, kl = scale * a.kl_grad, ce = scale * a.hard;
         const float share = out != 0.f ? p0 / out : 0.f;
         if (lane == 0) {
           coefs.ref = mo;
           coefs.base = kl * (all * z.inv_rel_outside() - share) + (TWO ? 0.f : ce * z.inv_rel_outside());
           coefs.base1 = TWO ? ce * z1.inv_rel_outside() : 0.f;
+          coefs.kl = kl, coefs.ce = ce, coefs.inv = inv, coefs.all = all;
+          coefs.mj = mj, coefs.inv_on = z.inv_rel_on(), coefs.inv_on1 = TWO ? z1.inv_rel_on() : z.inv_rel_on();
         }
         __syncthreads();
       }
@@ -392,7 +417,7 @@ __global__ void __launch_bounds__(NT + 32) distill_kernel(const DistillArgs a, i
           if (p0 != 0.f) loss += p0 * ((rest - mt) - logm + z.log2_all_over_outside() * LN2);
           loss *= a.kl_loss;
         }
-        if (a.hard > 0.f) loss += a.hard * ((mo - xy) + z1.log2_rel_outside() * LN2);
+        if (a.hard > 0.f) loss += a.hard * ((mo - LogitType<T>::one(vecs.row[y])) + z1.log2_rel_outside() * LN2);
         a.row_loss[row] = loss;
       }
     } else if constexpr (TRAIN) {
@@ -421,33 +446,40 @@ __global__ void __launch_bounds__(NT + 32) distill_kernel(const DistillArgs a, i
         });
       }
     }
-    if (extra && counted_next) look_ahead(row + stride);
-    __syncthreads();  // the base gradient lies before the entries'; the buffer has been read
-    if (extra) {
-      if (counted_next && lane == 0) issue(row + stride);
-      if constexpr (TRAIN) {
-        bool label = false;  // is it one of the entries
-#pragma unroll 1
-        for (int k = lane; k < a.K; k += 32) {
-          const Entry n = entries[k];
-          label |= n.id >= 0 && n.id == y;
+    if constexpr (TRAIN) {
+      __syncthreads();  // the base gradient lies before the entries'; the buffer has been read
+      const Coefficients k = coefs;
+      if (extra) {
+        if (counted_next) begin(row + stride, cut);
+        if (lane == 0 && y >= 0 && k.ce != 0.f && !label && y >= base_id && y - base_id < nv * E) {
+          const float xy = LogitType<T>::one(vecs.row[y]);
+          dx[y] = LogitType<T>::round(outside(Pair(xy, xy), k).get().x - k.ce);
+        }
+      } else {
+        for (int i = t; i < a.K; i += NT) {
+          const Entry n = entries[i];
           if (!n.here) continue;
-          float p = n.value * inv;
+          float p = n.value * k.inv;
           if (repeated) {  // the teacher's mass of all entries with this id, the same whichever of them writes it
             p = 0.f;
             for (int l = 0; l < a.K; ++l)
-              if (entries[l].id == n.id) p += entries[l].value * inv;
+              if (entries[l].id == n.id) p += entries[l].value * k.inv;
           }
-          const float q = exp2_fast((n.x - mj) * c) * inv_on;
-          const float q1 = TWO ? exp2_fast((n.x - mj) * LOG2E) * inv_on1 : q;
-          dx[n.id] = LogitType<T>::round(kl * (q * all - p) + ce * (q1 - (n.id == y ? 1.f : 0.f)));
+          const float q = exp2_fast((n.x - k.mj) * c) * k.inv_on;
+          const float q1 = TWO ? exp2_fast((n.x - k.mj) * LOG2E) * k.inv_on1 : q;
+          dx[n.id] = LogitType<T>::round(k.kl * (q * k.all - p) + k.ce * (q1 - (n.id == y ? 1.f : 0.f)));
         }
-        label = __any_sync(0xffffffff, label);
-        if (lane == 0 && y >= 0 && ce != 0.f && !label && y >= base_id && y - base_id < nv * E)
-          dx[y] = LogitType<T>::round(outside(Pair(xy, xy), coefs).get().x - ce);
       }
-      __syncwarp();
     }
+    if (counted_next) {
+      if (extra) {
+        finish(row + stride, cut);
+      } else {
+        if (ahead) entries_of[turn ^ 1][t] = read_entry(row + stride, t, id_next, value_next);
+        fill_entries(row + stride, entries_of[turn ^ 1], t + NT);
+      }
+    }
+    if (t == 0) twice[turn ^ 1] = 0;  // last read a row ago
     turn ^= 1;
   }
   if (cs > 1) cg::this_cluster().sync();  // others may still write here
@@ -459,8 +491,7 @@ __global__ void __launch_bounds__(1024) distill_count_kernel(const long long* ta
   __shared__ int part[32];
   begin_early();
   int n = 0;
-  long long y;
-  for (int r = threadIdx.x; r < rows; r += 1024) n += row_counts(target, ignore, r, V, y);
+  for (int r = threadIdx.x; r < rows; r += 1024) n += label_counts(target[r], ignore, V);
   n = __reduce_add_sync(0xffffffff, n);
   if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = n;
   __syncthreads();
@@ -492,7 +523,7 @@ __global__ void __launch_bounds__(1024) distill_mean_kernel(const float* row_los
 template <typename T, int NT, bool TRAIN, bool TWO>
 void distill_launch(const DistillArgs& a, int vecs, int device, cudaStream_t s) {
   auto* kernel = distill_kernel<T, NT, TRAIN, TWO>;
-  const int held = (vecs * 16 + 127) / 128 * 128, smem = held + a.K * (int)sizeof(Entry);
+  const int held = (vecs * 16 + 127) / 128 * 128, smem = held + 2 * a.K * (int)sizeof(Entry);
   static bool ready[64] = {};  // per device
   if (device < 0 || device >= 64 || !ready[device]) {
     cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, DST_MAX_SMEM);
