@@ -21,9 +21,8 @@ void distill(const void* x, long long ldx, void* dx, long long lddx, const void*
              float tau, float hard, const float* grad, float expected, bool unless_expected, float* row_loss,
              float* count, bool have_count, float* loss, int dtype, int device, cudaStream_t s);
 int top_logits_max_k();
-int top_logits_max_vocab(int elem);
 void top_logits(const void* x, long long ldx, int rows, int V, int k, float tau, int* ids, void* values, float* rest,
-                int dtype, cudaStream_t s);
+                int dtype, int device, cudaStream_t s);
 void sample_given(const void* x, long long ldx, int rows, int V, const void* uniform, bool uniform64,
                   const float* temperature, const int* top_k, const float* top_p, const float* min_p, long long* token,
                   float* logprob, int dtype, int device, cudaStream_t s);
@@ -66,8 +65,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> top_logits(const at::Tensor& logi
                     std::to_string(std::min<int64_t>(V, astrai_host::top_logits_max_k())), ", got ", std::to_string(k));
   TORCH_CHECK_VALUE(tau > 0. && std::isfinite(tau), "top_logits: temperature must be positive");
   const int code = dtype_code(logits, "top_logits: logits");
-  TORCH_CHECK_VALUE(V <= astrai_host::top_logits_max_vocab((int)logits.element_size()), "top_logits: a vocabulary of ",
-                    std::to_string(V), " is too large for this type");
+  TORCH_CHECK_VALUE(V < (1LL << 30), "top_logits: vocabulary too large");
   no_tangent(logits, "top_logits");
   TORCH_CHECK(!(at::GradMode::is_enabled() && logits.requires_grad()), "top_logits has no gradient: call it under no_grad");
   const c10::cuda::CUDAGuard guard(logits.device());
@@ -80,7 +78,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> top_logits(const at::Tensor& logi
        rest = new_like(x, {rows}, at::kFloat);
   if (rows > 0) {
     astrai_host::top_logits(x.data_ptr(), row_stride(x), (int)rows, (int)V, (int)k, (float)tau, ids.data_ptr<int>(),
-                            values.data_ptr(), rest.data_ptr<float>(), code, stream());
+                            values.data_ptr(), rest.data_ptr<float>(), code, x.get_device(), stream());
     C10_CUDA_KERNEL_LAUNCH_CHECK();
   }
   if (logits.dim() != 2) {

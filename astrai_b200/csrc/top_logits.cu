@@ -3,31 +3,27 @@
 // Equal logits rank by id, the lowest first; a NaN ranks above every number. `rest` is log sum exp(x_v / tau) over the
 // tokens that are not among the k.
 //
-// A row is read once, into registers: a CTA of 512 threads holds up to 64 KB of it, a longer row is shared by a cluster.
-// Nothing is sorted but a few candidates. Every warp finds the j-th largest of its 32 threads' maxima, and the smallest of
-// those over the G warps of the row is a bound that at least G j >= k logits reach: for k = 64 of 32000 about 150 do. Those
-// become candidates in shared memory, ranked by comparing each with all, and read as -inf in the sum over the rest of the
-// row. Where more than TOP_CAP logits reach the bound (ties), the exact k-th largest and the id that cuts its ties are found
-// by bisection, and the row is read again.
-#include <cooperative_groups.h>
-
+// A CTA of 256 threads takes a row, three on an SM; a row of up to 68 KB stays in its shared memory, a longer one comes from L2
+// again. Nothing is sorted but a few candidates: the largest logits of both halves of every thread's part make 64 numbers a
+// warp, and the smallest, over the W warps, of each warp's j-th largest is a bound that at least W j >= k logits reach (for
+// k = 64 of 32000 about 150 do). Those are ranked by comparing each with all; the others, and the candidates that do not make
+// it, give `rest`. Where more than TOP_CAP logits reach the bound (ties), the exact k-th largest and the id that cuts its ties
+// are found by bisection.
 #include "launch.cuh"
 #include "logits.cuh"
 
 namespace astrai {
 
-namespace cg = cooperative_groups;
-
-constexpr int TOP_THREADS = 512;
+constexpr int TOP_THREADS = 256;
 constexpr int TOP_WARPS = TOP_THREADS / 32;
 constexpr int TOP_MAX_K = 256;
 constexpr int TOP_CAP = 1024;
-constexpr int TOP_MAX_CLUSTER = 16;
+constexpr int TOP_HELD = 68 * 1024;
 
 struct TopArgs {
   const void* x;
   long long ldx;
-  int rows, V, k, cluster;
+  int rows, V, k;
   float inv_tau;
   int* ids;      // [rows, k]
   void* values;  // [rows, k]
@@ -35,267 +31,296 @@ struct TopArgs {
 };
 
 struct TopShared {
-  unsigned long long list[TOP_CAP];  // key, then the id's complement: greater ranks first
-  float left[TOP_CAP];                     // logits of candidates that are not among the k
-  uint32_t bound[TOP_WARPS], most[TOP_WARPS];
-  float part[TOP_WARPS];
-  int counts[TOP_WARPS];
-  uint32_t cluster_bound;
-  int cluster_count;
-  int n;                                   // the leader's: candidates of the row
-  float max_of[TOP_MAX_CLUSTER], sum_of[TOP_MAX_CLUSTER];  // the leader's: each CTA's part of the rest
+  unsigned long long list[TOP_CAP + 2];  // key, then the id's complement: greater ranks first
+  float left[TOP_CAP];                   // logits of candidates that are not among the k
+  uint32_t part[2][TOP_WARPS];
+  float sum[TOP_WARPS];
+  int n;
 };
 
-// Sum over the row's threads, the same in all of them.
-__device__ __forceinline__ int row_count(TopShared& sh, int n, int cs) {
-  n = __reduce_add_sync(0xffffffff, n);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) sh.counts[threadIdx.x >> 5] = n;
-  __syncthreads();
-  n = __reduce_add_sync(0xffffffff, (threadIdx.x & 31) < TOP_WARPS ? sh.counts[threadIdx.x & 31] : 0);
-  if (cs == 1) return n;
-  cg::cluster_group cl = cg::this_cluster();
-  if (threadIdx.x == 0) sh.cluster_count = n;
-  cl.sync();
-  n = 0;
-  for (int i = 0; i < cs; ++i) n += *cl.map_shared_rank(&sh.cluster_count, i);
-  cl.sync();
-  return n;
-}
+template <typename T, bool HELD>
+struct TopRow {
+  static constexpr int E = LogitType<T>::E, NT = TOP_THREADS;
+  TopShared& sh;
+  const uint4* held;
+  RowVecs<T> vecs;
+  int chunk, w0, mine;  // a warp's vectors, this thread's: w0 + i * 32 + lane
+  int turn = 0;
 
-template <typename T, int NV>
-__global__ void __launch_bounds__(TOP_THREADS, 2) top_logits_kernel(const TopArgs a) {
-  constexpr int E = LogitType<T>::E;
-  __shared__ TopShared sh;
-  const int t = threadIdx.x, lane = t & 31, w = t >> 5;
-  const int cs = a.cluster, rank = cs > 1 ? (int)cg::this_cluster().block_rank() : 0;
-  const int row = blockIdx.x / cs;
-  begin_early();
-  const RowVecs<T> vecs(static_cast<const T*>(a.x) + (long long)row * a.ldx, a.V);
-  const int per = (vecs.n + cs - 1) / cs, v0 = rank * per, v1 = min(v0 + per, vecs.n);
-  uint4 u[NV];
-  float most[NV];
-  const auto load = [&] {
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      const int v = v0 + t + i * TOP_THREADS;
-      u[i] = v < v1 ? vecs.load(v) : vec_neg_inf<T>();
-    }
-  };
-  load();
-  if (t == 0) sh.n = 0;
-  TopShared* lead = &sh;
-  if (cs > 1) lead = cg::this_cluster().map_shared_rank(&sh, 0);
-
-  // The bound: warps whose lanes all hold logits, the last CTA's may be fewer.
-  float top = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    most[i] = vec_max<T>(u[i]);
-    top = max_nan(top, most[i]);
+  __device__ uint4 vec(int i) const {
+    if (i >= mine) return vec_neg_inf<T>();
+    return HELD ? held[i * NT + threadIdx.x] : vecs.load(w0 + i * 32 + (threadIdx.x & 31));
   }
-  const int tail = vecs.n - (cs - 1) * per;  // vectors of the last CTA
-  const auto full = [&](int n) { return min(max(n, 0) / 32, TOP_WARPS); };
-  const int warps = (cs - 1) * full(per) + full(tail);
-  const int j = warps > 0 ? (a.k + warps - 1) / warps : 33;
-  uint32_t key = key_of(top), bound = 0xFFFFFFFFu;
-  if (j > 32) {
+  __device__ int first(int i) const { return vecs.first(w0 + i * 32 + (threadIdx.x & 31)); }
+  // f(vector, its number), four in flight; some behind the last read as -inf
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {
+#pragma unroll 1
+    for (int i = 0; i < mine; i += 4) {
+      uint4 u[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) u[j] = vec(i + j);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) f(u[j], i + j);
+    }
+  }
+  // over the CTA, the same in all threads
+  template <typename F>
+  __device__ __forceinline__ uint32_t reduce(uint32_t v, F f) {
+    v = f(v);
+    if ((threadIdx.x & 31) == 0) sh.part[turn][threadIdx.x >> 5] = v;
+    __syncthreads();
+    v = f(sh.part[turn][threadIdx.x & (TOP_WARPS - 1)]);
+    turn ^= 1;
+    return v;
+  }
+  __device__ uint32_t max_of(uint32_t v) {
+    return reduce(v, [](uint32_t x) { return __reduce_max_sync(0xffffffff, x); });
+  }
+  __device__ uint32_t min_of(uint32_t v) {
+    return reduce(v, [](uint32_t x) { return __reduce_min_sync(0xffffffff, x); });
+  }
+  __device__ int count_of(int n) {
+    return (int)reduce((uint32_t)n, [](uint32_t x) { return __reduce_add_sync(0xffffffff, x); }) / (32 / TOP_WARPS);
+  }
+  __device__ float sum_of(float s) {
+    s = warp_sum(s);
+    if ((threadIdx.x & 31) == 0) sh.sum[threadIdx.x >> 5] = s;
+    __syncthreads();
+    s = 0.f;
+#pragma unroll
+    for (int i = 0; i < TOP_WARPS; ++i) s += sh.sum[i];
+    __syncthreads();
+    return s;
+  }
+  // Keys above `more_than`, and those equal to it with ids below `below`.
+  __device__ __noinline__ int count(uint32_t more_than, int below) {
+    int n = 0;
+    each([&](const uint4& u, int i) {
+      float x[E];
+      vec_floats<T>(u, x);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const uint32_t key = key_of(x[e]);
+        const int id = first(i) + e;
+        n += i < mine && id >= 0 && id < vecs.V && (key > more_than || (key == more_than && id < below));
+      }
+    });
+    return count_of(n);
+  }
+  // Candidates: keys above `bound`, and those equal to it with ids below `cut`; their number.
+  __device__ __noinline__ int gather(uint32_t bound, int cut) {
+    __syncthreads();
+    if (threadIdx.x == 0) sh.n = 0;
+    __syncthreads();
+    each([&](const uint4& u, int i) {
+      if (key_of(vec_max<T>(u)) < bound || i >= mine) return;
+      float x[E];
+      vec_floats<T>(u, x);
+      const int at = first(i);
+      uint32_t bits = 0;
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const uint32_t key = key_of(x[e]);
+        const int id = at + e;
+        bits |= (uint32_t)(id >= 0 && id < vecs.V && (key > bound || (key == bound && id < cut))) << e;
+      }
+      if (!bits) return;
+      int to = atomicAdd(&sh.n, __popc(bits));
+#pragma unroll 1
+      for (; bits; bits &= bits - 1, ++to) {
+        const int e = __ffs(bits) - 1;
+        float one = x[0];
+#pragma unroll
+        for (int j = 1; j < E; ++j) one = e == j ? x[j] : one;
+        if (to < TOP_CAP) sh.list[to] = (unsigned long long)key_of(one) << 32 | (uint32_t)~(at + e);
+      }
+    });
+    __syncthreads();
+    return sh.n;
+  }
+  // Sum of 2^((x - ref) c) over what gather() left with this bound (a NaN is among them if there are more than k).
+  __device__ __noinline__ float mass_below(uint32_t bound, int cut, float ref, float c) {
+    const Pair ref2(-ref, -ref), c2(c, c);
+    const float edge = of_key(bound);
+    Pair s(0.f, 0.f);
+    if (cut >= vecs.V && edge == edge) {  // all logits equal to the bound are candidates
+      each([&](const uint4& u, int) {
+        float x[E];
+        vec_floats<T>(u, x);
+#pragma unroll
+        for (int e = 0; e < E; e += 2)
+          s = s + exp2_fast((Pair(x[e] < edge ? x[e] : -INFINITY, x[e + 1] < edge ? x[e + 1] : -INFINITY) + ref2) * c2);
+      });
+    } else {
+      each([&](const uint4& u, int i) {
+        float x[E];
+        vec_floats<T>(u, x);
+#pragma unroll
+        for (int e = 0; e < E; e += 2) {
+          float y[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t key = key_of(x[e + h]);
+            y[h] = key > bound || (key == bound && first(i) + e + h < cut) ? -INFINITY : x[e + h];
+          }
+          s = s + exp2_fast((Pair(y[0], y[1]) + ref2) * c2);
+        }
+      });
+    }
+    return sum_of(s.sum());
+  }
+  // The largest of them.
+  __device__ __noinline__ float max_below(uint32_t bound, int cut) {
+    uint32_t most = 0;
+    each([&](const uint4& u, int i) {
+      float x[E];
+      vec_floats<T>(u, x);
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const uint32_t key = key_of(x[e]);
+        const int id = first(i) + e;
+        if (i < mine && id >= 0 && id < vecs.V && (key < bound || (key == bound && id >= cut))) most = max(most, key);
+      }
+    });
+    most = max_of(most);
+    return most ? of_key(most) : -INFINITY;
+  }
+};
+
+template <typename T, bool HELD>
+__global__ void __launch_bounds__(TOP_THREADS, 3) top_logits_kernel(const TopArgs a) {
+  constexpr int NT = TOP_THREADS;
+  extern __shared__ uint4 top_held[];  // vector i of thread t at i * NT + t
+  __shared__ __align__(16) TopShared sh;
+  const int t = threadIdx.x, lane = t & 31, w = t >> 5, row = blockIdx.x;
+  begin_early();
+  TopRow<T, HELD> r{sh, top_held, RowVecs<T>(static_cast<const T*>(a.x) + (long long)row * a.ldx, a.V)};
+  r.chunk = (r.vecs.n + NT - 1) / NT * 32;
+  r.w0 = w * r.chunk;
+  r.mine = max(0, min(r.chunk / 32, (min(r.w0 + r.chunk, r.vecs.n) - r.w0 - lane + 31) / 32));
+
+  // the largest of the thread's first and second half
+  float top[2] = {-INFINITY, -INFINITY};
+  const int half = (r.mine + 1) / 2;
+#pragma unroll 1
+  for (int i0 = 0; i0 < r.mine; i0 += 8) {
+    uint4 u[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) u[i] = i0 + i < r.mine ? r.vecs.load(r.w0 + (i0 + i) * 32 + lane) : vec_neg_inf<T>();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (HELD && i0 + i < r.mine) top_held[(i0 + i) * NT + t] = u[i];
+      const float most = vec_max<T>(u[i]);
+      if (i0 + i < half) top[0] = max_nan(top[0], most);
+      else top[1] = max_nan(top[1], most);
+    }
+  }
+  // The bound, from the warps whose lanes all hold logits.
+  const int warps = r.vecs.n < 32 ? 0 : min((r.vecs.n - 32) / r.chunk + 1, TOP_WARPS);
+  const int j = warps > 0 ? (a.k + warps - 1) / warps : 65;
+  uint32_t key = key_of(top[0]), second = r.mine > 1 ? key_of(top[1]) : 0, bound = 0xFFFFFFFFu;
+  if (second > key) {
+    const uint32_t swap = key;
+    key = second;
+    second = swap;
+  }
+  if (j > 64 || a.V <= a.k) {
     bound = 0;
-  } else if (w < full(v1 - v0)) {
+  } else if (w < warps) {
+#pragma unroll 1
     for (int i = 0;; ++i) {
       bound = __reduce_max_sync(0xffffffff, key);
       if (i == j - 1) break;
-      if (lane == __ffs(__ballot_sync(0xffffffff, key == bound)) - 1) key = 0;
+      if (lane == __ffs(__ballot_sync(0xffffffff, key == bound)) - 1) key = second, second = 0;
     }
   }
-  if (lane == 0) sh.bound[w] = bound;
-  __syncthreads();
-  bound = __reduce_min_sync(0xffffffff, sh.bound[lane & (TOP_WARPS - 1)]);
-  if (cs > 1) {
-    cg::cluster_group cl = cg::this_cluster();
-    if (t == 0) sh.cluster_bound = bound;
-    cl.sync();
-    bound = __reduce_min_sync(0xffffffff, *cl.map_shared_rank(&sh.cluster_bound, lane < cs ? lane : 0));
-  }
-
+  bound = r.min_of(bound);
   int cut = a.V;  // of the logits equal to the bound, those with smaller ids
-  for (int attempt = 0;; ++attempt) {
-    // Candidates out of the row; the largest logit that stays, and its sum.
-    float mx = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      if (key_of(most[i]) >= bound) {
-        const int v = v0 + t + i * TOP_THREADS, at = vecs.first(v);
-        float f[E];
-        vec_floats<T>(u[i], f);
-        uint32_t out = 0;
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const uint32_t ke = key_of(f[e]);
-          const int id = at + e;
-          if (ke < bound || (ke == bound && id >= cut) || id < 0 || id >= a.V || v >= v1) continue;
-          out |= 1u << e;
-          const int slot = atomicAdd(&lead->n, 1);
-          if (slot < TOP_CAP) lead->list[slot] = (unsigned long long)ke << 32 | (uint32_t)~id;
-        }
-        vec_mask<T>(u[i], out);
-        mx = max_nan(mx, vec_max<T>(u[i]));
-      } else {
-        mx = fmaxf(mx, most[i]);
-      }
-    }
-    uint32_t km = __reduce_max_sync(0xffffffff, key_of(mx));
-    if (lane == 0) sh.most[w] = km;
-    __syncthreads();
-    km = __reduce_max_sync(0xffffffff, sh.most[lane & (TOP_WARPS - 1)]);
-    mx = of_key(km);
-    const float c = a.inv_tau * 1.4426950408889634f, ref = mx == -INFINITY ? 0.f : mx;
-    const Pair c2(c, c), ref2(-ref, -ref);
-    Pair s2(0.f, 0.f);
-#pragma unroll
-    for (int i = 0; i < NV; ++i) {
-      Pair p[E / 2];
-      vec_pairs<T>(u[i], p);
-#pragma unroll
-      for (int e = 0; e < E / 2; ++e) s2 = s2 + exp2_fast((p[e] + ref2) * c2);
-    }
-    float s = warp_sum(s2.sum());
-    if (lane == 0) sh.part[w] = s;
-    __syncthreads();
-    if (t == 0) {
-      s = 0.f;
-      for (int i = 0; i < TOP_WARPS; ++i) s += sh.part[i];
-      lead->max_of[rank] = mx;
-      lead->sum_of[rank] = s;
-    }
-    if (cs > 1) cg::this_cluster().sync();
-    else __syncthreads();
-    const int n = lead->n;
-    if (n <= TOP_CAP) break;
-    // Too many. The exact k-th largest key, and the id up to which the logits equal to it are taken.
-    const auto count = [&](uint32_t more_than, uint32_t equal, int below) {  // keys above, and equal ones with ids below
-      int got = 0;
-#pragma unroll 1
-      for (int v = v0 + t; v < v1; v += TOP_THREADS) {
-        const int at = vecs.first(v);
-        float f[E];
-        vec_floats<T>(vecs.load(v), f);
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          const uint32_t ke = key_of(f[e]);
-          const int id = at + e;
-          got += id >= 0 && id < a.V && (ke > more_than || (ke == equal && id < below));
-        }
-      }
-      return row_count(sh, got, cs);
-    };
+  int n = r.gather(bound, cut);
+  if (n > TOP_CAP) {
+    // The exact k-th largest key, and the id up to which the logits equal to it are taken.
     uint32_t kth = 0;
 #pragma unroll 1
     for (int b = 31; b >= 0; --b) {
       const uint32_t next = kth | 1u << b;
-      if (count(next, next, a.V) >= a.k) kth = next;
+      if (r.count(next, a.V) >= a.k) kth = next;
     }
     int low = 0;  // fewer than k are above, or equal with an id below `low`
 #pragma unroll 1
     for (int b = 31 - __clz(a.V); b >= 0; --b)
-      if (low + (1 << b) <= a.V && count(kth, kth, low + (1 << b)) < a.k) low += 1 << b;
+      if (low + (1 << b) <= a.V && r.count(kth, low + (1 << b)) < a.k) low += 1 << b;
     bound = kth;
     cut = low + 1;
-    load();
-#pragma unroll
-    for (int i = 0; i < NV; ++i) most[i] = of_key(0xFFFFFFFFu);  // every vector may hold a candidate
-    if (rank == 0 && t == 0) sh.n = 0;
-    if (cs > 1) cg::this_cluster().sync();
-    else __syncthreads();
+    n = r.gather(bound, cut);
   }
-  if (rank > 0) {  // the leader stays until its memory has been read
-    asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-    return;
-  }
-  if (cs > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
 
-  // Ranks: four threads for each candidate compare it with a quarter of the others.
-  const int n = sh.n, quarter = t & 3;
-  float mx = -INFINITY, s = 0.f;
-  for (int i = 0; i < cs; ++i) {
-    if (sh.max_of[i] == -INFINITY) continue;
-    const float m = max_nan(mx, sh.max_of[i]);
-    s = s * exp2_fast((mx - m) * a.inv_tau * 1.4426950408889634f) +
-        sh.sum_of[i] * exp2_fast((sh.max_of[i] - m) * a.inv_tau * 1.4426950408889634f);
-    mx = m;
-  }
+  // Ranks: each candidate against all, two at a time.
   float left_max = -INFINITY;
+  if (t == 0) sh.list[n] = 0;
+  __syncthreads();
 #pragma unroll 1
-  for (int i0 = 0; i0 < n; i0 += TOP_THREADS / 4) {
-    const int i = i0 + t / 4;
-    const unsigned long long mine = i < n ? sh.list[i] : 0;
-    int r = 0;
-    for (int l = quarter; l < n; l += 4) r += sh.list[l] > mine;
-    r += __shfl_xor_sync(0xffffffff, r, 1);
-    r += __shfl_xor_sync(0xffffffff, r, 2);
-    if (i >= n || quarter != 0) continue;
+  for (int i = t; i < n; i += NT) {
+    const unsigned long long mine = sh.list[i];
+    int rank = 0;
+    const ulonglong2* two = reinterpret_cast<const ulonglong2*>(sh.list);
+#pragma unroll 4
+    for (int l = 0; l < n; l += 2) {
+      const ulonglong2 other = two[l / 2];
+      rank += (other.x > mine) + (other.y > mine);
+    }
     const float value = of_key((uint32_t)(mine >> 32));
-    if (r < a.k) {
-      const long long at = (long long)row * a.k + r;
+    if (rank < a.k) {
+      const long long at = (long long)row * a.k + rank;
       a.ids[at] = (int)~(uint32_t)mine;
       static_cast<T*>(a.values)[at] = LogitType<T>::round(value);
     } else {
-      sh.left[r - a.k] = value;  // by rank: the order in which candidates came must not reach the sum
+      sh.left[rank - a.k] = value;  // by rank: the order in which candidates came must not reach the sum
       left_max = max_nan(left_max, value);
     }
   }
-  // the candidates that are not among the k
-  uint32_t kl = __reduce_max_sync(0xffffffff, key_of(left_max));
-  if (lane == 0) sh.bound[w] = kl;
-  __syncthreads();
-  left_max = of_key(__reduce_max_sync(0xffffffff, sh.bound[lane & (TOP_WARPS - 1)]));
-  const float m = max_nan(mx, left_max), ref = m == -INFINITY ? 0.f : m;
+  // The rest relative to the bound or to the largest candidate in it; where that is too far above the others, to its largest.
   const float c = a.inv_tau * 1.4426950408889634f;
-  float sl = 0.f;
-  for (int i = t; i < n - a.k; i += TOP_THREADS) sl += exp2_fast((sh.left[i] - ref) * c);
-  sl = warp_sum(sl);
-  if (lane == 0) sh.part[w] = sl;
-  __syncthreads();
-  if (t == 0) {
-    s *= exp2_fast((mx - ref) * c);
-    for (int i = 0; i < TOP_WARPS; ++i) s += sh.part[i];
-    a.rest[row] = isinf(m) ? m : fmaf(ref, a.inv_tau, logf(s));
+  left_max = of_key(r.max_of(key_of(left_max)));  // and its barrier for `left`
+  float ref = max_nan(of_key(bound), left_max);
+  if (bound <= key_of(-INFINITY) || !(fabsf(ref) < INFINITY)) ref = max_nan(r.max_below(bound, cut), left_max);
+#pragma unroll 1
+  for (int attempt = 0;; ++attempt) {
+    const float from = ref == -INFINITY ? 0.f : ref;
+    float s = r.mass_below(bound, cut, from, c);
+    float sl = 0.f;
+    for (int i = t; i < n - a.k; i += NT) sl += exp2_fast((sh.left[i] - from) * c);
+    s += r.sum_of(sl);
+    if (attempt == 0 && s < 1e-24f && n < a.V) {
+      const float most = max_nan(r.max_below(bound, cut), left_max);
+      if (most != ref) {
+        ref = most;
+        continue;
+      }
+    }
+    if (t == 0) a.rest[row] = isinf(ref) ? ref : s == 0.f ? -INFINITY : fmaf(ref, a.inv_tau, logf(s));
+    return;
   }
-  if (cs > 1) asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 
-template <typename T, int NV>
-void top_launch(const TopArgs& a, cudaStream_t s) {
-  auto* kernel = top_logits_kernel<T, NV>;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)a.rows * a.cluster);
-  cfg.blockDim = dim3(TOP_THREADS);
-  cfg.stream = s;
-  cudaLaunchAttribute at[2]{};
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  at[1].id = cudaLaunchAttributeClusterDimension;
-  at[1].val.clusterDim.x = a.cluster;
-  at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = a.cluster > 1 ? 2 : 1;
-  if (a.cluster > 8) cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-  note_launch();
-  cudaLaunchKernelEx(&cfg, kernel, a);
+template <typename T, bool HELD>
+void top_launch(const TopArgs& a, int smem, int device, cudaStream_t s) {
+  auto* kernel = top_logits_kernel<T, HELD>;
+  static bool ready[64] = {};  // per device
+  if (device < 0 || device >= 64 || !ready[device]) {
+    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TOP_HELD);
+    if (device >= 0 && device < 64) ready[device] = true;
+  }
+  launch_early(kernel, dim3((unsigned)a.rows), dim3(TOP_THREADS), smem, s, a);
 }
 
 template <typename T>
-void top_sized(TopArgs a, cudaStream_t s) {
+void top_typed(const TopArgs& a, int device, cudaStream_t s) {
   constexpr int E = LogitType<T>::E;
   const int vecs = (a.V + E - 1) / E + 1;  // one more where a row starts off the grid
-  int cs = 1;
-  while ((vecs + cs - 1) / cs > TOP_THREADS * 8) cs *= 2;
-  a.cluster = cs;
-  const int per = (vecs + cs - 1) / cs;
-  if (per <= TOP_THREADS) return top_launch<T, 1>(a, s);
-  if (per <= TOP_THREADS * 2) return top_launch<T, 2>(a, s);
-  if (per <= TOP_THREADS * 4) return top_launch<T, 4>(a, s);
-  top_launch<T, 8>(a, s);
+  const int held = (vecs + TOP_THREADS - 1) / TOP_THREADS * TOP_THREADS * 16;
+  if (held <= TOP_HELD) top_launch<T, true>(a, held, device, s);
+  else top_launch<T, false>(a, 0, device, s);
 }
 
 }  // namespace astrai
@@ -304,15 +329,13 @@ namespace astrai_host {
 using namespace astrai;
 
 int top_logits_max_k() { return TOP_MAX_K; }
-// longest row for elements of this size
-int top_logits_max_vocab(int elem) { return TOP_MAX_CLUSTER * TOP_THREADS * 8 * (16 / elem) - 16 / elem; }
 
 void top_logits(const void* x, long long ldx, int rows, int V, int k, float tau, int* ids, void* values, float* rest,
-                int dtype, cudaStream_t s) {
-  const TopArgs a{x, ldx, rows, V, k, 1, 1.f / tau, ids, values, rest};
-  if (dtype == 0) top_sized<__nv_bfloat16>(a, s);
-  else if (dtype == 1) top_sized<__half>(a, s);
-  else top_sized<float>(a, s);
+                int dtype, int device, cudaStream_t s) {
+  const TopArgs a{x, ldx, rows, V, k, 1.f / tau, ids, values, rest};
+  if (dtype == 0) top_typed<__nv_bfloat16>(a, device, s);
+  else if (dtype == 1) top_typed<__half>(a, device, s);
+  else top_typed<float>(a, device, s);
 }
 
 }  // namespace astrai_host
