@@ -37,6 +37,8 @@ def main(argv: Optional[List[str]] = None) -> None:
     p.add_argument("--cache_len", type=int, default=2048)
     p.add_argument("--frequency_penalty", type=float, default=0.0)
     p.add_argument("--rep_window", type=int, default=64)
+    p.add_argument("--min_p", type=float, default=0.0)
+    p.add_argument("--seed", type=int, default=None, help="Same answers on every run; the samples of all prompts have seeds from here on.")
     a = p.parse_args(argv)
     t0 = time.time()
     model = AutoModel.from_pretrained(a.param_path).to(device="cuda", dtype=torch.bfloat16).eval()
@@ -52,7 +54,8 @@ def main(argv: Optional[List[str]] = None) -> None:
             chunk = prompts[i:i + n]
             flat = [q for q in chunk for _ in range(a.num_samples)]
             res = eng.generate(flat, max_tokens=max_tokens, temperature=a.temperature, top_p=a.top_p, top_k=a.top_k,
-                               frequency_penalty=a.frequency_penalty, rep_window=a.rep_window)
+                               frequency_penalty=a.frequency_penalty, rep_window=a.rep_window, min_p=a.min_p,
+                               seed=None if a.seed is None else a.seed + i * a.num_samples)
             for j, q in enumerate(chunk):
                 r = res[j * a.num_samples:(j + 1) * a.num_samples]
                 r = r if a.num_samples > 1 else r[0]

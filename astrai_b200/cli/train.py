@@ -8,7 +8,8 @@ steps and warmup from the dataset length; scheduler kwargs per schedule
 type; DecoderBlock checkpointing with --gradient_checkpointing). Added
 flags: ``--comm_backend fused`` (NVLink peer-memory gradient all-reduce for
 ddp), ``--expert_parallel`` (shard MoE experts over the ranks),
-``--profile_dir``, ``--shard_muon`` (owner-sharded Muon: each rank runs
+``--profile_dir``, ``--rollout_min_p``, ``--train_type distill`` with
+``--teacher_path`` and ``--distill_*``, ``--shard_muon`` (owner-sharded Muon: each rank runs
 Newton-Schulz on 1/world of the matrices and writes the updated weights into
 every replica over NVLink).
 """
@@ -26,7 +27,7 @@ import torch
 def parse_args(argv: Optional[List[str]] = None) -> argparse.Namespace:
     p = argparse.ArgumentParser(description="Train a model with astrai_b200.")
     a = p.add_argument
-    a("--train_type", type=str, required=True, choices=["seq", "sft", "dpo", "grpo", "online_grpo", "online_dpo"])
+    a("--train_type", type=str, required=True, choices=["seq", "sft", "dpo", "grpo", "online_grpo", "online_dpo", "distill"])
     a("--data_root_path", type=str, required=True, help="Dataset root (bin / h5 / jsonl).")
     a("--param_path", type=str, required=True, help="Model directory: config.json, tokenizer, weights.")
     a("--resume", action="store_true", help="Resume from the checkpoint in --param_path.")
@@ -86,6 +87,11 @@ def parse_args(argv: Optional[List[str]] = None) -> argparse.Namespace:
     a("--shard_muon", action="store_true",
       help="ddp: each rank orthogonalises 1/world of the Muon matrices and writes the update into every replica.")
     a("--profile_dir", type=str, default=None)
+    a("--rollout_min_p", type=float, default=0.0)
+    a("--teacher_path", type=str, default=None, help="distill: model directory of the teacher (same vocabulary).")
+    a("--distill_top_k", type=int, default=64, help="distill: the teacher's tokens that are told apart.")
+    a("--distill_temperature", type=float, default=1.0)
+    a("--distill_hard_weight", type=float, default=0.0, help="distill: share of the labels' cross entropy.")
     return p.parse_args(argv)
 
 
@@ -118,7 +124,7 @@ def scheduler_kwargs(schedule_type: str, total_steps: int, warmup_ratio: float, 
 def build_config(args: argparse.Namespace):
     from astrai_b200.config import AutoRegressiveLMConfig, TrainConfig
     from astrai_b200.dataset import DatasetFactory, dpo_collate_fn, grpo_collate_fn
-    from astrai_b200.models import AutoRegressiveLM, DecoderBlock
+    from astrai_b200.models import AutoModel, AutoRegressiveLM, DecoderBlock
     from astrai_b200.optim import MuonMix
     from astrai_b200.trainer import SchedulerFactory
 
@@ -126,6 +132,8 @@ def build_config(args: argparse.Namespace):
         raise FileNotFoundError(args.param_path)
     if args.nprocs > 1 and args.parallel_mode == "none":
         raise ValueError("--nprocs > 1 requires --parallel_mode to be 'ddp', 'fsdp', or 'fsdp2'")
+    if args.train_type == "distill" and args.teacher_path is None:
+        raise ValueError("--train_type distill requires --teacher_path")
     config = AutoRegressiveLMConfig.from_file(os.path.join(args.param_path, "config.json"))
     config.neftune_alpha = args.neftune_alpha
     window = args.window_size or config.max_position_embeddings
@@ -156,11 +164,15 @@ def build_config(args: argparse.Namespace):
         gradient_checkpointing_modules=[DecoderBlock] if args.gradient_checkpointing else [],
         executor_kwargs=executor_kwargs,
         extra_kwargs={"beta": args.dpo_beta, "label_smoothing": args.label_smoothing, "clip_eps": args.grpo_clip_eps,
-                      "kl_coef": args.grpo_kl_coef, "group_size": args.group_size},
+                      "kl_coef": args.grpo_kl_coef, "group_size": args.group_size,
+                      **({"distill_top_k": args.distill_top_k, "distill_temperature": args.distill_temperature,
+                          "distill_hard_weight": args.distill_hard_weight} if args.train_type == "distill" else {})},
         neftune_alpha=args.neftune_alpha, collate_fn=collate, rollout_interval=args.rollout_interval,
         rollout_temperature=args.rollout_temperature, rollout_top_k=args.rollout_top_k,
         rollout_top_p=args.rollout_top_p, rollout_max_tokens=args.rollout_max_tokens,
-        comm_backend=args.comm_backend, profile_dir=args.profile_dir,
+        comm_backend=args.comm_backend, profile_dir=args.profile_dir, rollout_min_p=args.rollout_min_p,
+        teacher_fn=partial(AutoModel.from_pretrained, args.teacher_path, dtype=torch.bfloat16) if args.teacher_path
+        else None,
     )
 
 

@@ -6,7 +6,9 @@ checkpoint ``meta.json`` (which embeds ``to_dict()``) and user scripts depend
 on them. Fields added here: ``comm_backend`` (``"nccl"`` or ``"fused"``: who
 moves gradients between GPUs), ``cuda_graph`` (replay each micro-step's forward
 and backward from a CUDA graph, for fixed-shape batches on the seq / sft
-strategies) and ``profile_dir`` (torch.profiler trace output).
+strategies), ``profile_dir`` (torch.profiler trace output), ``rollout_min_p``
+(min-p of online rollouts) and ``teacher_fn`` (builds the teacher of the
+distill strategy).
 """
 
 from __future__ import annotations
@@ -69,6 +71,8 @@ class TrainConfig(BaseConfig):
     comm_backend: str = "nccl"
     cuda_graph: bool = False
     profile_dir: Optional[str] = None
+    rollout_min_p: float = 0.0
+    teacher_fn: Optional[Callable] = None
 
     def __post_init__(self):
         self.validate()

@@ -323,6 +323,61 @@ struct Sampler {
     error = precise || total == 0. ? 0. : total * (4.5e-7 + 1.3e-7 * fmaxf(log2f((float)shared().V) - log2f((float)total), 0.f));
     return total;
   }
+  // Numbers at the lanes for which `some` holds, behind those that a list has.
+  static __device__ __forceinline__ int place(int* n, bool some) {
+    const uint32_t lanes = __ballot_sync(0xffffffff, some);
+    int at = 0;
+    if ((threadIdx.x & 31) == 0 && lanes) at = atomicAdd(n, __popc(lanes));
+    return __shfl_sync(0xffffffff, at, 0) + __popc(lanes & ((1u << (threadIdx.x & 31)) - 1));
+  }
+  // Candidates: the logits from `low` on, if they are not too many; their number. First the vectors that hold any, then those
+  // vectors' elements, one a thread: a warp in which a few lanes look at eight elements each takes as long as if all did.
+  static __device__ __noinline__ int gather_top(float low) {
+    SampleShared& sh = shared();
+    const Mine me(sh);
+    const int t = threadIdx.x;
+    __syncthreads();
+    if (t == 0) sh.n = sh.hit = 0;
+    __syncthreads();
+#pragma unroll 1
+    for (int i0 = 0, at = 0; i0 < sh.chunk / 32; i0 += sh.group, ++at) {
+      const int end = min(i0 + sh.group, me.mine);
+      const bool may = i0 < end && tops()[at * NT + t + (HELD ? sh.chunk / 32 * NT * 4 : 0)] >= low;
+      if (!__any_sync(0xffffffff, may)) continue;
+#pragma unroll 1
+      for (int i = i0; i < min(i0 + sh.group, sh.chunk / 32); i += 4) {
+        uint4 u[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) u[j] = may && i + j < end ? me.vec(i + j) : vec_neg_inf<T>();
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const bool some = vec_max<T>(u[j]) >= low;
+          if (!__any_sync(0xffffffff, some)) continue;
+          const int to = place(&sh.hit, some);
+          if (some && to < SG_CAP) sh.sorted[to] = (i + j) * NT + t;
+        }
+      }
+    }
+    __syncthreads();
+    const int vecs = sh.hit, all = vecs * E;
+    if (vecs > SG_CAP) return SG_CAP + 1;
+#pragma unroll 1
+    for (int q0 = 0; q0 < all; q0 += NT) {
+      const int q = q0 + t;
+      int id = -1;
+      float x = -INFINITY;
+      if (q < all) {
+        const int v = sh.sorted[q / E], of = v % NT;
+        id = me.vecs.first(of / 32 * sh.chunk + v / NT * 32 + of % 32) + q % E;
+        if (id >= 0 && id < sh.V) x = LogitType<T>::one(HELD ? reinterpret_cast<const T*>(held())[v * E + q % E] : me.vecs.row[id]);
+      }
+      const bool some = x >= low;
+      const int to = place(&sh.n, some);
+      if (some && to < SG_CAP) sh.key[to] = key_of(x), sh.id[to] = id;
+    }
+    __syncthreads();
+    return sh.n;
+  }
   // Candidates: the logits in low .. high (exclusive), if they are not too many; their number.
   static __device__ __noinline__ int gather(float low, float high) {
     SampleShared& sh = shared();
@@ -815,7 +870,7 @@ struct Sampler {
       uint32_t least = by_k || sh.use_p ? low : 0;
       bool complete = by_k || least == 0;  // no token below the candidates can be kept
       if (sh.use_m && !(by_k && sh.use_p) && low_m >= least) least = low_m, complete = true;
-      const int n = gather(from(least), INFINITY);
+      const int n = gather_top(from(least));
       bool may = n <= SG_CAP;
       if (may && !complete) {  // where the candidates' mass cannot reach top-p's bound they need no order
         float s = 0.f;

@@ -3,8 +3,9 @@
 // Equal logits rank by id, the lowest first; a NaN ranks above every number. `rest` is log sum exp(x_v / tau) over the
 // tokens that are not among the k.
 //
-// A CTA of 256 threads takes a row, three on an SM; a row of up to 68 KB stays in its shared memory, a longer one comes from L2
-// again. Nothing is sorted but a few candidates: the largest logits of both halves of every thread's part make 64 numbers a
+// A CTA takes a row: 256 threads, three on an SM, where it is no longer than 68 KB, else 512 threads that have an SM to
+// themselves. A row of up to 200 KB stays in shared memory, a longer one comes from L2 again (three such rows on every SM would
+// not fit there: 768 rows of 131072 bf16 took 211 us). Nothing is sorted but a few candidates: the largest logits of both halves of every thread's part make 64 numbers a
 // warp, and the smallest, over the W warps, of each warp's j-th largest is a bound that at least W j >= k logits reach (for
 // k = 64 of 32000 about 150 do). Those are ranked by comparing each with all; the others, and the candidates that do not make
 // it, give `rest`. Where more than TOP_CAP logits reach the bound (ties), the exact k-th largest and the id that cuts its ties
@@ -14,11 +15,9 @@
 
 namespace astrai {
 
-constexpr int TOP_THREADS = 256;
-constexpr int TOP_WARPS = TOP_THREADS / 32;
 constexpr int TOP_MAX_K = 256;
 constexpr int TOP_CAP = 1024;
-constexpr int TOP_HELD = 68 * 1024;
+constexpr int TOP_HELD = 68 * 1024, TOP_HELD_ALONE = 200 * 1024;
 
 struct TopArgs {
   const void* x;
@@ -33,14 +32,15 @@ struct TopArgs {
 struct TopShared {
   unsigned long long list[TOP_CAP + 2];  // key, then the id's complement: greater ranks first
   float left[TOP_CAP];                   // logits of candidates that are not among the k
-  uint32_t part[2][TOP_WARPS];
-  float sum[TOP_WARPS];
-  int n;
+  uint32_t vecs[TOP_CAP];                // vectors that hold candidates
+  uint32_t part[2][16];
+  float sum[16];
+  int n, n_vecs;
 };
 
-template <typename T, bool HELD>
+template <typename T, bool HELD, int NT>
 struct TopRow {
-  static constexpr int E = LogitType<T>::E, NT = TOP_THREADS;
+  static constexpr int E = LogitType<T>::E, W = NT / 32;
   TopShared& sh;
   const uint4* held;
   RowVecs<T> vecs;
@@ -50,6 +50,13 @@ struct TopRow {
   __device__ uint4 vec(int i) const {
     if (i >= mine) return vec_neg_inf<T>();
     return HELD ? held[i * NT + threadIdx.x] : vecs.load(w0 + i * 32 + (threadIdx.x & 31));
+  }
+  // Numbers at the lanes for which `some` holds, behind those that a list has.
+  static __device__ __forceinline__ int place(int* n, bool some) {
+    const uint32_t lanes = __ballot_sync(0xffffffff, some);
+    int at = 0;
+    if ((threadIdx.x & 31) == 0 && lanes) at = atomicAdd(n, __popc(lanes));
+    return __shfl_sync(0xffffffff, at, 0) + __popc(lanes & ((1u << (threadIdx.x & 31)) - 1));
   }
   __device__ int first(int i) const { return vecs.first(w0 + i * 32 + (threadIdx.x & 31)); }
   // f(vector, its number), four in flight; some behind the last read as -inf
@@ -70,7 +77,7 @@ struct TopRow {
     v = f(v);
     if ((threadIdx.x & 31) == 0) sh.part[turn][threadIdx.x >> 5] = v;
     __syncthreads();
-    v = f(sh.part[turn][threadIdx.x & (TOP_WARPS - 1)]);
+    v = f(sh.part[turn][threadIdx.x & (W - 1)]);
     turn ^= 1;
     return v;
   }
@@ -81,7 +88,7 @@ struct TopRow {
     return reduce(v, [](uint32_t x) { return __reduce_min_sync(0xffffffff, x); });
   }
   __device__ int count_of(int n) {
-    return (int)reduce((uint32_t)n, [](uint32_t x) { return __reduce_add_sync(0xffffffff, x); }) / (32 / TOP_WARPS);
+    return (int)reduce((uint32_t)n, [](uint32_t x) { return __reduce_add_sync(0xffffffff, x); }) / (32 / W);
   }
   __device__ float sum_of(float s) {
     s = warp_sum(s);
@@ -89,7 +96,7 @@ struct TopRow {
     __syncthreads();
     s = 0.f;
 #pragma unroll
-    for (int i = 0; i < TOP_WARPS; ++i) s += sh.sum[i];
+    for (int i = 0; i < W; ++i) s += sh.sum[i];
     __syncthreads();
     return s;
   }
@@ -108,8 +115,50 @@ struct TopRow {
     });
     return count_of(n);
   }
+  // Candidates: keys from `bound` on; their number, or more than TOP_CAP. First the vectors that hold any, then those vectors'
+  // elements, one a thread: a warp in which a few lanes look at eight elements each takes as long as if all did.
+  __device__ __noinline__ int gather(uint32_t bound) {
+    const int t = threadIdx.x;
+    __syncthreads();
+    if (t == 0) sh.n = sh.n_vecs = 0;
+    __syncthreads();
+    const float edge = of_key(bound);
+#pragma unroll 1
+    for (int i = 0; i < chunk / 32; i += 4) {
+      uint4 u[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) u[j] = vec(i + j);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const bool some = i + j < mine && !(vec_max<T>(u[j]) < edge);  // a NaN too
+        if (!__any_sync(0xffffffff, some)) continue;
+        const int to = place(&sh.n_vecs, some);
+        if (some && to < TOP_CAP) sh.vecs[to] = (i + j) * NT + t;
+      }
+    }
+    __syncthreads();
+    const int all = sh.n_vecs * E;
+    if (sh.n_vecs > TOP_CAP) return TOP_CAP + 1;
+#pragma unroll 1
+    for (int q0 = 0; q0 < all; q0 += NT) {
+      const int q = q0 + t;
+      int id = -1;
+      uint32_t key = 0;
+      if (q < all) {
+        const int v = sh.vecs[q / E], i = v / NT, of = v % NT;
+        id = vecs.first(of / 32 * chunk + i * 32 + of % 32) + q % E;
+        if (id >= 0 && id < vecs.V) key = key_of(LogitType<T>::one(HELD ? reinterpret_cast<const T*>(held)[v * E + q % E] : vecs.row[id]));
+        else id = -1;
+      }
+      const bool some = id >= 0 && key >= bound;
+      const int to = place(&sh.n, some);
+      if (some && to < TOP_CAP) sh.list[to] = (unsigned long long)key << 32 | (uint32_t)~id;
+    }
+    __syncthreads();
+    return sh.n;
+  }
   // Candidates: keys above `bound`, and those equal to it with ids below `cut`; their number.
-  __device__ __noinline__ int gather(uint32_t bound, int cut) {
+  __device__ __noinline__ int gather_cut(uint32_t bound, int cut) {
     __syncthreads();
     if (threadIdx.x == 0) sh.n = 0;
     __syncthreads();
@@ -188,14 +237,14 @@ struct TopRow {
   }
 };
 
-template <typename T, bool HELD>
-__global__ void __launch_bounds__(TOP_THREADS, 3) top_logits_kernel(const TopArgs a) {
-  constexpr int NT = TOP_THREADS;
+template <typename T, bool HELD, int NT>
+__global__ void __launch_bounds__(NT, NT == 256 ? 3 : 1) top_logits_kernel(const TopArgs a) {
+  constexpr int W = NT / 32;
   extern __shared__ uint4 top_held[];  // vector i of thread t at i * NT + t
   __shared__ __align__(16) TopShared sh;
   const int t = threadIdx.x, lane = t & 31, w = t >> 5, row = blockIdx.x;
   begin_early();
-  TopRow<T, HELD> r{sh, top_held, RowVecs<T>(static_cast<const T*>(a.x) + (long long)row * a.ldx, a.V)};
+  TopRow<T, HELD, NT> r{sh, top_held, RowVecs<T>(static_cast<const T*>(a.x) + (long long)row * a.ldx, a.V)};
   r.chunk = (r.vecs.n + NT - 1) / NT * 32;
   r.w0 = w * r.chunk;
   r.mine = max(0, min(r.chunk / 32, (min(r.w0 + r.chunk, r.vecs.n) - r.w0 - lane + 31) / 32));
@@ -217,7 +266,7 @@ __global__ void __launch_bounds__(TOP_THREADS, 3) top_logits_kernel(const TopArg
     }
   }
   // The bound, from the warps whose lanes all hold logits.
-  const int warps = r.vecs.n < 32 ? 0 : min((r.vecs.n - 32) / r.chunk + 1, TOP_WARPS);
+  const int warps = r.vecs.n < 32 ? 0 : min((r.vecs.n - 32) / r.chunk + 1, W);
   const int j = warps > 0 ? (a.k + warps - 1) / warps : 65;
   uint32_t key = key_of(top[0]), second = r.mine > 1 ? key_of(top[1]) : 0, bound = 0xFFFFFFFFu;
   if (second > key) {
@@ -237,7 +286,7 @@ __global__ void __launch_bounds__(TOP_THREADS, 3) top_logits_kernel(const TopArg
   }
   bound = r.min_of(bound);
   int cut = a.V;  // of the logits equal to the bound, those with smaller ids
-  int n = r.gather(bound, cut);
+  int n = r.gather(bound);
   if (n > TOP_CAP) {
     // The exact k-th largest key, and the id up to which the logits equal to it are taken.
     uint32_t kth = 0;
@@ -252,7 +301,7 @@ __global__ void __launch_bounds__(TOP_THREADS, 3) top_logits_kernel(const TopArg
       if (low + (1 << b) <= a.V && r.count(kth, low + (1 << b)) < a.k) low += 1 << b;
     bound = kth;
     cut = low + 1;
-    n = r.gather(bound, cut);
+    n = r.gather_cut(bound, cut);
   }
 
   // Ranks: each candidate against all, two at a time.
@@ -303,24 +352,25 @@ __global__ void __launch_bounds__(TOP_THREADS, 3) top_logits_kernel(const TopArg
   }
 }
 
-template <typename T, bool HELD>
+template <typename T, bool HELD, int NT>
 void top_launch(const TopArgs& a, int smem, int device, cudaStream_t s) {
-  auto* kernel = top_logits_kernel<T, HELD>;
+  auto* kernel = top_logits_kernel<T, HELD, NT>;
   static bool ready[64] = {};  // per device
   if (device < 0 || device >= 64 || !ready[device]) {
-    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, TOP_HELD);
+    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, NT == 256 ? TOP_HELD : TOP_HELD_ALONE);
     if (device >= 0 && device < 64) ready[device] = true;
   }
-  launch_early(kernel, dim3((unsigned)a.rows), dim3(TOP_THREADS), smem, s, a);
+  launch_early(kernel, dim3((unsigned)a.rows), dim3(NT), smem, s, a);
 }
 
 template <typename T>
 void top_typed(const TopArgs& a, int device, cudaStream_t s) {
   constexpr int E = LogitType<T>::E;
   const int vecs = (a.V + E - 1) / E + 1;  // one more where a row starts off the grid
-  const int held = (vecs + TOP_THREADS - 1) / TOP_THREADS * TOP_THREADS * 16;
-  if (held <= TOP_HELD) top_launch<T, true>(a, held, device, s);
-  else top_launch<T, false>(a, 0, device, s);
+  const auto held = [&](int threads) { return (vecs + threads - 1) / threads * threads * 16; };
+  if (held(256) <= TOP_HELD) top_launch<T, true, 256>(a, held(256), device, s);
+  else if (held(512) <= TOP_HELD_ALONE) top_launch<T, true, 512>(a, held(512), device, s);
+  else top_launch<T, false, 512>(a, TOP_HELD_ALONE / 2 + 32 * 1024, device, s);  // (asked for to be alone)
 }
 
 }  // namespace astrai

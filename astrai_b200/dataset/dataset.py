@@ -1,7 +1,7 @@
 """Training datasets: a :class:`Store` plus the key mapping of one training type.
 
 Public names kept from the reference (astrai/dataset/dataset.py:43-506): ``BaseDataset``,
-``DatasetFactory`` (keys ``seq``, ``sft``, ``dpo``, ``grpo``), the four dataset classes,
+``DatasetFactory`` (keys ``seq``, ``sft``, ``dpo``, ``grpo``; ``distill`` reads as ``sft``), the four dataset classes,
 ``dpo_tokenize``, ``dpo_processor``, ``dpo_collate_fn`` and ``grpo_collate_fn``.
 
 Each dataset class is declarative:
@@ -211,7 +211,7 @@ class DatasetFactory(Registry["BaseDataset"]):
 
                 kw["processor"] = partial(dpo_processor, tokenizer=AutoTokenizer.from_pretrained(tokenizer_path),
                                           max_len=max_len)
-            elif train_type in ("seq", "sft"):
+            elif train_type in ("seq", "sft", "distill"):
                 kw.setdefault("tokenizer_path", tokenizer_path)
         st.load(load_path, **kw)
         return st
@@ -226,6 +226,9 @@ class SEQDataset(_WindowDataset):
 class SFTDataset(_WindowDataset):
     fields = (("input_ids", "sequence", 0, torch.long), ("target_ids", "sequence", 1, torch.long),
               ("position_ids", "position_ids", 0, torch.long), ("loss_mask", "loss_mask", 1, torch.bool))
+
+
+DatasetFactory.alias("distill", "sft")
 
 
 @DatasetFactory.register("dpo")

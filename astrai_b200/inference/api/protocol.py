@@ -102,10 +102,14 @@ class ProtocolHandler:
 
     def _agen(self, prompt: str) -> AsyncGenerator[str, None]:
         r = self.request
+        penalty = getattr(r, "frequency_penalty", 0.0) or 0.0
+        given = {"min_p": getattr(r, "min_p", 0.0) or 0.0, "seed": getattr(r, "seed", None)}
+        if penalty or not (given["min_p"] or given["seed"] is not None):
+            given = {}  # a request with a penalty is answered as if it had neither
         return self.engine.generate_async(
             prompt, max_tokens=r.max_tokens, temperature=r.temperature if r.temperature is not None else 1.0,
             top_p=r.top_p if r.top_p is not None else 1.0, top_k=r.top_k if r.top_k is not None else 50,
-            frequency_penalty=getattr(r, "frequency_penalty", 0.0) or 0.0)
+            frequency_penalty=penalty, **given)
 
     def _count(self, text: str) -> int:
         return len(self.engine.tokenizer.encode(text)) if text else 0

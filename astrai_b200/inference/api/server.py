@@ -60,6 +60,8 @@ class ChatCompletionRequest(BaseModel):
     frequency_penalty: Optional[float] = Field(default=0.0, ge=-2.0, le=2.0)
     logit_bias: Optional[Dict[int, float]] = None
     user: Optional[str] = None
+    min_p: Optional[float] = Field(default=0.0, ge=0.0, le=1.0)
+    seed: Optional[int] = None
     tools: Optional[List[ToolDef]] = None
     tool_choice: Optional[Union[str, Dict[str, Any]]] = "auto"
 
@@ -79,6 +81,7 @@ class MessagesRequest(BaseModel):
     top_k: Optional[int] = Field(default=50, ge=0)
     stream: Optional[bool] = False
     stop_sequences: Optional[List[str]] = None
+    min_p: Optional[float] = Field(default=0.0, ge=0.0, le=1.0)
 
 
 def _create_engine(param_path, device: str = "cuda", dtype: torch.dtype = torch.bfloat16, max_batch_size: int = 16,

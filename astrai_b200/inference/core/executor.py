@@ -15,19 +15,23 @@ Differences, all on the device side:
   three H2D copies; with ``use_cuda_graph`` the whole decode forward +
   sampling for a batch-size bucket is replayed from a captured CUDA graph
   (rows whose frequency penalty is non-zero take the eager path, which also
-  ships the history window).
+  ships the history window);
+* rows with a seed of their own or min-p are drawn by ``sample_given`` from
+  numbers that the host sends, on the eager path; the other rows of the batch
+  keep the sampler that draws its own.
 """
 
 from __future__ import annotations
 
 import logging
+import random
 from typing import Dict, List, Optional, Tuple
 
 import torch
 
 from astrai_b200.inference.core.cache import KVCache, PageCacheView
 from astrai_b200.inference.core.task import Task
-from astrai_b200.inference.sample import DeviceRNG, fused_sample, sample
+from astrai_b200.inference.sample import DeviceRNG, fused_sample, sample, sample_given
 
 logger = logging.getLogger(__name__)
 
@@ -157,6 +161,7 @@ class Executor:
         self.n_heads = cfg.num_attention_heads
         self.rng = DeviceRNG(self.device, seed) if self.device.type == "cuda" else None
         self._cpu_gen = torch.Generator().manual_seed(seed) if seed is not None else None
+        self._numbers = random.Random(seed)  # for rows with min-p and no seed
         self._graphs: Optional[_DecodeGraphs] = None
         if use_cuda_graph and self.device.type == "cuda":
             page = getattr(kv_cache, "page_size", max_seq_len)
@@ -164,6 +169,29 @@ class Executor:
 
     # ----------------------------------------------------------------- helpers
     def _sample(self, logits: torch.Tensor, tasks: List[Task]) -> Tuple[List[int], List[float]]:
+        given = [i for i, t in enumerate(tasks) if t.given]
+        if not given:
+            return self._sample_own(logits, tasks)
+        toks, lps = [0] * len(tasks), [0.0] * len(tasks)
+        for rows, draw in ((given, self._sample_given),
+                           ([i for i, t in enumerate(tasks) if not t.given], self._sample_own)):
+            if rows:
+                part = logits if len(rows) == len(tasks) else logits[torch.tensor(rows, device=logits.device)]
+                for i, tok, lp in zip(rows, *draw(part, [tasks[i] for i in rows])):
+                    toks[i], lps[i] = tok, lp
+        return toks, lps
+
+    def _sample_given(self, logits: torch.Tensor, tasks: List[Task]) -> Tuple[List[int], List[float]]:
+        numbers = [t.uniform() if t.seed is not None else self._numbers.random() for t in tasks]
+        host = torch.tensor([numbers, *([getattr(t, name) for t in tasks] for name in ("temperature", "top_p", "min_p"))],
+                            dtype=torch.float64)
+        u, temperature, top_p, min_p = host.to(logits.device, non_blocking=True)
+        top_k = torch.tensor([t.top_k for t in tasks], dtype=torch.int32).to(logits.device, non_blocking=True)
+        tok, lp = sample_given(logits, u, temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p,
+                               return_logprobs=True)
+        return tok.tolist(), lp.tolist()
+
+    def _sample_own(self, logits: torch.Tensor, tasks: List[Task]) -> Tuple[List[int], List[float]]:
         dev = logits.device
         n = len(tasks)
         pen_on = any(t.frequency_penalty != 0.0 for t in tasks)
@@ -215,7 +243,7 @@ class Executor:
         if not tasks:
             return []
         if self._graphs is not None and len(tasks) <= self._graphs.max_batch and not any(
-                t.frequency_penalty != 0.0 for t in tasks):
+                t.frequency_penalty != 0.0 or t.given for t in tasks):
             toks, lps = self._graphs.run(tasks)
             return self._append(tasks, toks, lps, return_logprobs)
         dev = self.device

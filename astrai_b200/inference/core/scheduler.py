@@ -190,21 +190,25 @@ class InferenceScheduler:
     # ------------------------------------------------------------------ synchronous batch (RL rollout)
     def run_batch(self, prompt_ids_list: List[List[int]], *, max_tokens: Optional[int] = None,
                   temperature: float = 1.0, top_p: float = 1.0, top_k: int = 50, frequency_penalty: float = 0.0,
-                  rep_window: int = 64, return_logprobs: bool = False) -> List[Any]:
+                  rep_window: int = 64, return_logprobs: bool = False, min_p: float = 0.0,
+                  seeds: Optional[List[int]] = None) -> List[Any]:
         """Generate for already-tokenised prompts on the calling thread.
 
         Prompts run in waves of at most ``max_batch_size``; a prompt that does
         not fit ``max_seq_len`` (or the cache) yields an empty result.
+        ``seeds`` has one for each prompt; its tokens then repeat in any batch.
         """
+        if seeds is not None and len(seeds) != len(prompt_ids_list):
+            raise ValueError("run_batch: seeds must have one for each prompt")
         cap = self.max_seq_len
         tasks: List[Optional[Task]] = []
-        for ids in prompt_ids_list:
+        for i, ids in enumerate(prompt_ids_list):
             if not ids or len(ids) >= cap:
                 tasks.append(None)
                 continue
             mt = cap - len(ids) if max_tokens is None else min(max_tokens, cap - len(ids))
             tasks.append(Task(f"batch_{uuid.uuid4().hex[:8]}", list(ids), mt, temperature, top_p, top_k,
-                              frequency_penalty, rep_window))
+                              frequency_penalty, rep_window, min_p=min_p, seed=seeds[i] if seeds else None))
         live_all = [t for t in tasks if t is not None]
         wave = max(1, self._task_mgr.max_batch_size)
         for i in range(0, len(live_all), wave):

@@ -95,6 +95,8 @@ class Task:
     output_tokens: int = 0
     arrival_time: float = field(default_factory=time.time)
     finish_time: Optional[float] = None
+    min_p: float = 0.0
+    seed: Optional[int] = None
     _detok: Optional[StreamDecoder] = field(default=None, repr=False)
 
     def __post_init__(self):
@@ -102,6 +104,25 @@ class Task:
         self.temperature, self.top_p = float(self.temperature), float(self.top_p)
         self.top_k, self.rep_window = int(self.top_k), int(self.rep_window)
         self.frequency_penalty = float(self.frequency_penalty)
+        self.min_p = float(self.min_p)
+        if self.given and self.frequency_penalty:
+            raise ValueError("min_p and seed do not go together with a frequency penalty")
+
+    # ------------------------------------------------------------------ sampling
+    @property
+    def given(self) -> bool:
+        """Whether its tokens are drawn by ``sample_given`` (a seed of its own, or min-p)."""
+        return self.seed is not None or self.min_p > 0.0
+
+    def uniform(self) -> Optional[float]:
+        """The number in [0, 1) that the next token is drawn from: a hash of the task's seed and the token's index
+        (the SplitMix64 finaliser), so that a seeded request repeats in any batch. None without a seed."""
+        if self.seed is None:
+            return None
+        z = (self.seed * 0xD1342543DE82EF95 + (len(self.output_ids) + 1) * 0x9E3779B97F4A7C15) & 0xFFFFFFFFFFFFFFFF
+        z = ((z ^ (z >> 30)) * 0xBF58476D1CE4E5B9) & 0xFFFFFFFFFFFFFFFF
+        z = ((z ^ (z >> 27)) * 0x94D049BB133111EB) & 0xFFFFFFFFFFFFFFFF
+        return ((z ^ (z >> 31)) >> 11) * 2.0 ** -53
 
     # ------------------------------------------------------------------ streaming text
     def decode_new_token(self, tokenizer) -> str:
@@ -163,12 +184,13 @@ class TaskManager:
 
     def add_task(self, prompt: str, max_tokens: Optional[int] = None, temperature: float = 1.0, top_p: float = 1.0,
                  top_k: int = 50, frequency_penalty: float = 0.0, rep_window: int = 64,
-                 stream_callback: Optional[Callback] = None, prompt_ids: Optional[List[int]] = None) -> str:
+                 stream_callback: Optional[Callback] = None, prompt_ids: Optional[List[int]] = None,
+                 min_p: float = 0.0, seed: Optional[int] = None) -> str:
         """Queue a request; returns its id. A prompt that leaves no room to generate is answered
         with ``STOP`` at once (its id is still returned, and refers to nothing)."""
         ids = self.tokenizer.encode(prompt) if prompt_ids is None else prompt_ids
         task = self.make_task(ids, max_tokens, temperature=temperature, top_p=top_p, top_k=top_k,
-                              frequency_penalty=frequency_penalty, rep_window=rep_window)
+                              frequency_penalty=frequency_penalty, rep_window=rep_window, min_p=min_p, seed=seed)
         if task is None:
             if stream_callback is not None:
                 stream_callback(STOP)

@@ -79,7 +79,7 @@ class GenerateResult:
         return ["".join(p) for p in self._pieces]
 
 
-def _check_sampling(top_k, top_p, temperature, frequency_penalty, rep_window) -> None:
+def _check_sampling(top_k, top_p, temperature, frequency_penalty, rep_window, min_p=0.0, seed=None) -> None:
     problems = []
     if not isinstance(top_k, int) or isinstance(top_k, bool) or top_k < 0:
         problems.append(f"top_k={top_k!r} (want an int >= 0; 0 disables the cut)")
@@ -91,6 +91,12 @@ def _check_sampling(top_k, top_p, temperature, frequency_penalty, rep_window) ->
         problems.append(f"frequency_penalty={frequency_penalty!r} (want a number in [-2, 2])")
     if not isinstance(rep_window, int) or rep_window <= 0:
         problems.append(f"rep_window={rep_window!r} (want an int > 0)")
+    if not isinstance(min_p, (int, float)) or not 0.0 <= min_p <= 1.0:
+        problems.append(f"min_p={min_p!r} (want a number in [0, 1]; 0 disables the cut)")
+    if seed is not None and (not isinstance(seed, int) or isinstance(seed, bool)):
+        problems.append(f"seed={seed!r} (want an int or None)")
+    if frequency_penalty and (min_p or seed is not None):
+        problems.append("frequency_penalty (goes with neither min_p nor a seed)")
     if problems:
         raise ValueError("invalid sampling parameters: " + "; ".join(problems))
 
@@ -101,8 +107,8 @@ class GenerationRequest:
 
     def __init__(self, messages: List[Dict[str, str]], top_k: int = 50, top_p: float = 1.0,
                  temperature: float = 1.0, max_tokens: Optional[int] = None, frequency_penalty: float = 0.0,
-                 rep_window: int = 64, stream: bool = False):
-        _check_sampling(top_k, top_p, temperature, frequency_penalty, rep_window)
+                 rep_window: int = 64, stream: bool = False, min_p: float = 0.0, seed: Optional[int] = None):
+        _check_sampling(top_k, top_p, temperature, frequency_penalty, rep_window, min_p, seed)
         self.messages = messages
         self.top_k = top_k
         self.top_p = top_p
@@ -111,10 +117,13 @@ class GenerationRequest:
         self.frequency_penalty = frequency_penalty
         self.rep_window = rep_window
         self.stream = stream
+        self.min_p = min_p
+        self.seed = seed
 
     def sampling(self) -> Dict[str, Any]:
         return {"max_tokens": self.max_tokens, "temperature": self.temperature, "top_p": self.top_p,
-                "top_k": self.top_k, "frequency_penalty": self.frequency_penalty, "rep_window": self.rep_window}
+                "top_k": self.top_k, "frequency_penalty": self.frequency_penalty, "rep_window": self.rep_window,
+                "min_p": self.min_p, "seed": self.seed}
 
 
 def _text_only(events: Iterator[Tuple[int, str]]) -> Iterator[str]:
@@ -166,7 +175,9 @@ class InferenceEngine:
     # ------------------------------------------------------------------ submission
     def _launch(self, prompts: Sequence[str], sampling: Dict[str, Any]) -> Tuple[GenerateResult, List[str]]:
         res = GenerateResult(len(prompts))
-        tasks = [self.scheduler.add_task(text, stream_callback=lambda piece, i=i: res.append(piece, i), **sampling)
+        seed = sampling.get("seed")
+        each = [sampling if seed is None else {**sampling, "seed": seed + i} for i in range(len(prompts))]
+        tasks = [self.scheduler.add_task(text, stream_callback=lambda piece, i=i: res.append(piece, i), **each[i])
                  for i, text in enumerate(prompts)]
         return res, tasks
 
@@ -186,13 +197,21 @@ class InferenceEngine:
     # ------------------------------------------------------------------ public API
     def generate(self, prompt: Union[str, List[str]], stream: bool = False, max_tokens: Optional[int] = None,
                  temperature: float = 1.0, top_p: float = 1.0, top_k: int = 50, frequency_penalty: float = 0.0,
-                 rep_window: int = 64) -> Union[Iterator, str, List[str]]:
+                 rep_window: int = 64, min_p: float = 0.0, seed: Optional[int] = None) -> Union[Iterator, str, List[str]]:
         """Blocking: the generated text (a list of texts for a list of prompts). Streaming: an
-        iterator of text pieces (of ``(prompt index, piece)`` pairs for a list of prompts)."""
+        iterator of text pieces (of ``(prompt index, piece)`` pairs for a list of prompts).
+
+        ``min_p`` drops tokens less likely than that share of the likeliest; with a ``seed`` a prompt's
+        tokens are drawn from numbers of its own, the same in any batch and on every call (prompt ``i`` of
+        a list has ``seed + i``; the model's logits may round differently in a batch of another size). Neither goes with a frequency penalty (``ValueError``)."""
+        if min_p or seed is not None:
+            _check_sampling(top_k, top_p, temperature, frequency_penalty, rep_window, min_p, seed)
         as_list = isinstance(prompt, list)
         prompts = prompt if as_list else [prompt]
         sampling = {"max_tokens": max_tokens, "temperature": temperature, "top_p": top_p, "top_k": top_k,
                     "frequency_penalty": frequency_penalty, "rep_window": rep_window}
+        if min_p or seed is not None:
+            sampling.update(min_p=min_p, seed=seed)
         if stream:
             events = self._drain(prompts, sampling, None)
             return events if as_list else _text_only(events)
@@ -204,11 +223,12 @@ class InferenceEngine:
 
     def generate_async(self, prompt: str, max_tokens: Optional[int] = None, temperature: float = 1.0,
                        top_p: float = 1.0, top_k: int = 50, frequency_penalty: float = 0.0,
-                       rep_window: int = 64) -> AsyncIterator[str]:
+                       rep_window: int = 64, min_p: float = 0.0, seed: Optional[int] = None) -> AsyncIterator[str]:
         """Async iterator of text pieces for one prompt. The blocking queue reads run in the event
         loop's default executor; closing the iterator early cancels the task."""
         pieces = self.generate(prompt, stream=True, max_tokens=max_tokens, temperature=temperature, top_p=top_p,
-                               top_k=top_k, frequency_penalty=frequency_penalty, rep_window=rep_window)
+                               top_k=top_k, frequency_penalty=frequency_penalty, rep_window=rep_window, min_p=min_p,
+                               seed=seed)
         end = object()
 
         def pull():

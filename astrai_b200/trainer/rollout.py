@@ -47,7 +47,8 @@ class BaseRewardModel(ABC):
 
 class RolloutGenerator:
     def __init__(self, scheduler, tokenizer, max_tokens: int = 1024, group_size: int = 8, temperature: float = 1.0,
-                 top_k: int = 0, top_p: float = 1.0, frequency_penalty: float = 0.0, rep_window: int = 64):
+                 top_k: int = 0, top_p: float = 1.0, frequency_penalty: float = 0.0, rep_window: int = 64,
+                 min_p: float = 0.0):
         self.scheduler = scheduler
         self.tokenizer = tokenizer
         self.max_tokens = max_tokens
@@ -57,6 +58,7 @@ class RolloutGenerator:
         self.top_p = top_p
         self.frequency_penalty = frequency_penalty
         self.rep_window = rep_window
+        self.min_p = min_p
 
     @torch.no_grad()
     def generate(self, batch: Dict) -> RawRollout:
@@ -75,7 +77,7 @@ class RolloutGenerator:
         results = self.scheduler.run_batch(flat, max_tokens=self.max_tokens, temperature=self.temperature,
                                            top_k=self.top_k, top_p=self.top_p,
                                            frequency_penalty=self.frequency_penalty, rep_window=self.rep_window,
-                                           return_logprobs=True)
+                                           return_logprobs=True, **({"min_p": self.min_p} if self.min_p else {}))
         if len(results) != B * G:
             raise RuntimeError(f"Rollout scheduler returned {len(results)} results, expected {B * G}")
         dev = self.scheduler.device

@@ -1,4 +1,4 @@
-"""Training strategies: seq / sft / dpo / grpo (+ online_dpo / online_grpo).
+"""Training strategies: seq / sft / dpo / grpo (+ online_dpo / online_grpo) and distill.
 
 Loss definitions follow the reference (astrai/trainer/strategy.py):
 * seq:  mean CE over all targets with label smoothing;
@@ -8,7 +8,9 @@ Loss definitions follow the reference (astrai/trainer/strategy.py):
         response-token log-prob sums (``reduction="sum"`` by default);
 * grpo: group-normalised advantages ``(r - mean) / (std_biased + 1e-8)``,
         token-level PPO clip, k1 KL ``exp(ref-pol) - (ref-pol) - 1`` against a
-        frozen reference, token mean over response tokens.
+        frozen reference, token mean over response tokens;
+* distill (not in the reference): KL to a teacher's top logits, with a share of
+        the CE on the labels, over the tokens that sft counts.
 
 Differences that matter for speed: CE and token log-probs run in the fused
 kernels on bf16 logits (no fp32 [tokens, vocab] copy); document and padding
@@ -27,6 +29,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 
 from astrai_b200.factory import Registry
+from astrai_b200.ops.distill import TopLogits, distill_loss, top_logits
 from astrai_b200.ops.loss import cross_entropy, token_logprobs
 
 
@@ -167,6 +170,54 @@ class SFTStrategy(BaseStrategy):
         target = batch["target_ids"].masked_fill(~batch["loss_mask"].bool(), -100)
         out = self.model(input_ids=batch["input_ids"], position_ids=pos, seg_ids=doc_ids_from_positions(pos))
         loss = cross_entropy(out["logits"], target, label_smoothing=self.label_smoothing, ignore_index=-100)
+        return self._add_aux(out, loss)
+
+
+@StrategyFactory.register("distill")
+class DistillStrategy(BaseStrategy):
+    """A student learns a teacher's distribution over its top tokens and all others
+    (:func:`astrai_b200.ops.distill.distill_loss`), and the labels with ``distill_hard_weight``.
+
+    The teacher is a frozen ``teacher_model`` with the student's vocabulary, or its rows come with the batch:
+    ``teacher_ids`` and ``teacher_logits [B, S, k]`` and, if wanted, ``teacher_rest [B, S]``, the log-sum-exp of
+    its other logits over the temperature. ``position_ids`` (packed documents) and ``loss_mask`` are used as by
+    sft if the batch has them.
+    """
+
+    cuda_graph_safe = True
+
+    def __init__(self, model, device, teacher_model=None, distill_top_k: int = 64, distill_temperature: float = 1.0,
+                 distill_hard_weight: float = 0.0, **kwargs):
+        super().__init__(model, device, **kwargs)
+        self.teacher_model = teacher_model
+        self.top_k = distill_top_k
+        self.temperature = distill_temperature
+        self.hard_weight = distill_hard_weight
+
+    def _teacher(self, batch, inputs) -> TopLogits:
+        if "teacher_ids" in batch:
+            return TopLogits(batch["teacher_ids"], batch["teacher_logits"], batch.get("teacher_rest"))
+        if self.teacher_model is None:
+            raise ValueError("distill needs a teacher_model (TrainConfig.teacher_fn), or batches with teacher_ids and "
+                             "teacher_logits")
+        with torch.no_grad():
+            logits = self.teacher_model(**inputs)["logits"]
+            return top_logits(logits, min(self.top_k, logits.shape[-1]), self.temperature)
+
+    def compute_loss(self, batch):
+        batch = move_to_device(batch, self.device)
+        inputs = {"input_ids": batch["input_ids"]}
+        if "position_ids" in batch:
+            inputs.update(position_ids=batch["position_ids"], seg_ids=doc_ids_from_positions(batch["position_ids"]))
+        target = batch["target_ids"]
+        if "loss_mask" in batch:
+            target = target.masked_fill(~batch["loss_mask"].bool(), -100)
+        teacher = self._teacher(batch, inputs)
+        out = self.model(**inputs)
+        # the gradient that the trainer sends back, which divides the loss by the accumulation steps
+        steps = getattr(self.executor, "grad_accum_steps", 1)
+        loss = distill_loss(out["logits"], teacher, self.temperature, target, self.hard_weight, ignore_index=-100,
+                            expected_grad=1.0 / steps)
         return self._add_aux(out, loss)
 
 

@@ -4,7 +4,8 @@ The builder creates the executor, loads a checkpoint (``param_path``; with
 ``resume`` also epoch / consumed samples rounded down to an optimizer-step
 multiple, and optimizer / scheduler state), injects LoRA before wrapping,
 builds the resumable ``RDSampler`` + DataLoader (optional validation split),
-creates frozen reference / old-policy models for dpo / grpo, the strategy,
+creates frozen reference / old-policy models for dpo / grpo, the teacher for
+distill, the strategy,
 and for ``online_*`` strategies the rollout generator + runner on top of the
 inference scheduler.
 
@@ -169,6 +170,8 @@ class TrainContextBuilder:
             skw["ref_model"] = create_ref_model(cfg.model_fn, executor.unwrap_model(ctx.model)).to(device=device)
         if cfg.strategy in ("grpo", "online_grpo"):
             skw["old_model"] = create_ref_model(cfg.model_fn, executor.unwrap_model(ctx.model)).to(device=device)
+        if cfg.strategy == "distill" and cfg.teacher_fn is not None:
+            skw["teacher_model"] = cfg.teacher_fn().requires_grad_(False).eval().to(device=device)
         ctx.strategy = StrategyFactory.create(cfg.strategy, model=ctx.model, device=device, executor=executor, **skw)
 
         if cfg.strategy.startswith("online_"):
@@ -188,7 +191,7 @@ class TrainContextBuilder:
                                        max_seq_len=max_len, max_prompt_len=max_len or 4096)
             gen = RolloutGenerator(scheduler=sched, tokenizer=tok, max_tokens=cfg.rollout_max_tokens, group_size=group,
                                    temperature=cfg.rollout_temperature, top_k=cfg.rollout_top_k,
-                                   top_p=cfg.rollout_top_p)
+                                   top_p=cfg.rollout_top_p, min_p=cfg.rollout_min_p)
             ctx.strategy.set_rollout_runner(RolloutRunner(generator=gen, reward_model=cfg.reward_model_fn(),
                                                           rollout_interval=cfg.rollout_interval))
         return ctx
