@@ -51,12 +51,18 @@ struct TopRow {
     if (i >= mine) return vec_neg_inf<T>();
     return HELD ? held[i * NT + threadIdx.x] : vecs.load(w0 + i * 32 + (threadIdx.x & 31));
   }
-  // Numbers at the lanes for which `some` holds, behind those that a list has.
-  static __device__ __forceinline__ int place(int* n, bool some) {
-    const uint32_t lanes = __ballot_sync(0xffffffff, some);
+  // The place in a list of each lane's `mine` entries, behind those that the list has.
+  static __device__ __forceinline__ int place(int* n, int mine) {
+    const int lane = threadIdx.x & 31;
+    int before = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const int other = __shfl_up_sync(0xffffffff, before, d);
+      if (lane >= d) before += other;
+    }
     int at = 0;
-    if ((threadIdx.x & 31) == 0 && lanes) at = atomicAdd(n, __popc(lanes));
-    return __shfl_sync(0xffffffff, at, 0) + __popc(lanes & ((1u << (threadIdx.x & 31)) - 1));
+    if (lane == 31 && before) at = atomicAdd(n, before);
+    return __shfl_sync(0xffffffff, at, 31) + before - mine;
   }
   __device__ int first(int i) const { return vecs.first(w0 + i * 32 + (threadIdx.x & 31)); }
   // f(vector, its number), four in flight; some behind the last read as -inf
@@ -116,7 +122,8 @@ struct TopRow {
     return count_of(n);
   }
   // Candidates: keys from `bound` on; their number, or more than TOP_CAP. First the vectors that hold any, then those vectors'
-  // elements, one a thread: a warp in which a few lanes look at eight elements each takes as long as if all did.
+  // elements: a warp in which a few lanes look at eight elements each takes as long as if all did. A thread marks its vectors
+  // in a word first, and a warp takes its places in the list at once: at 64 of 32000 nearly every warp has some in every turn.
   __device__ __noinline__ int gather(uint32_t bound) {
     const int t = threadIdx.x;
     __syncthreads();
@@ -124,35 +131,46 @@ struct TopRow {
     __syncthreads();
     const float edge = of_key(bound);
 #pragma unroll 1
-    for (int i = 0; i < chunk / 32; i += 4) {
-      uint4 u[4];
+    for (int i0 = 0; i0 < chunk / 32; i0 += 32) {
+      uint32_t marks = 0;
+#pragma unroll 1
+      for (int i = i0; i < min(i0 + 32, chunk / 32); i += 4) {
+        uint4 u[4];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) u[j] = vec(i + j);
+        for (int j = 0; j < 4; ++j) u[j] = vec(i + j);
+        uint32_t four = 0;
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const bool some = i + j < mine && !(vec_max<T>(u[j]) < edge);  // a NaN too
-        if (!__any_sync(0xffffffff, some)) continue;
-        const int to = place(&sh.n_vecs, some);
-        if (some && to < TOP_CAP) sh.vecs[to] = (i + j) * NT + t;
+        for (int j = 0; j < 4; ++j) four |= (uint32_t)!(vec_max<T>(u[j]) < edge) << j;  // a NaN too
+        marks |= four << (i - i0);
       }
+      if (mine - i0 < 32) marks &= (1u << max(mine - i0, 0)) - 1;
+      int to = place(&sh.n_vecs, __popc(marks));
+#pragma unroll 1
+      for (; marks && to < TOP_CAP; marks &= marks - 1) sh.vecs[to++] = (i0 + __ffs(marks) - 1) * NT + t;
     }
     __syncthreads();
-    const int all = sh.n_vecs * E;
     if (sh.n_vecs > TOP_CAP) return TOP_CAP + 1;
 #pragma unroll 1
-    for (int q0 = 0; q0 < all; q0 += NT) {
+    for (int q0 = 0; q0 < sh.n_vecs; q0 += NT) {
       const int q = q0 + t;
-      int id = -1;
-      uint32_t key = 0;
-      if (q < all) {
-        const int v = sh.vecs[q / E], i = v / NT, of = v % NT;
-        id = vecs.first(of / 32 * chunk + i * 32 + of % 32) + q % E;
-        if (id >= 0 && id < vecs.V) key = key_of(LogitType<T>::one(HELD ? reinterpret_cast<const T*>(held)[v * E + q % E] : vecs.row[id]));
-        else id = -1;
+      uint32_t marks = 0;
+      int at = 0, v = 0;
+      if (q < sh.n_vecs) {
+        v = sh.vecs[q];
+        const int of = v % NT, number = of / 32 * chunk + v / NT * 32 + of % 32;
+        at = vecs.first(number);
+        float x[E];
+        vec_floats<T>(HELD ? held[v] : vecs.load(number), x);
+#pragma unroll
+        for (int e = 0; e < E; ++e) marks |= (uint32_t)(at + e >= 0 && at + e < vecs.V && key_of(x[e]) >= bound) << e;
       }
-      const bool some = id >= 0 && key >= bound;
-      const int to = place(&sh.n, some);
-      if (some && to < TOP_CAP) sh.list[to] = (unsigned long long)key << 32 | (uint32_t)~id;
+      int to = place(&sh.n, __popc(marks));
+#pragma unroll 1
+      for (; marks && to < TOP_CAP; marks &= marks - 1) {
+        const int e = __ffs(marks) - 1;
+        const T one = HELD ? reinterpret_cast<const T*>(held)[v * E + e] : vecs.row[at + e];
+        sh.list[to++] = (unsigned long long)key_of(LogitType<T>::one(one)) << 32 | (uint32_t)~(at + e);
+      }
     }
     __syncthreads();
     return sh.n;
