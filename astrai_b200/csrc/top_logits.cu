@@ -35,7 +35,7 @@ struct TopShared {
   uint32_t vecs[TOP_CAP];                // vectors that hold candidates
   uint32_t part[2][16];
   float sum[16];
-  int n, n_vecs;
+  int n;
 };
 
 template <typename T, bool HELD, int NT>
@@ -46,23 +46,11 @@ struct TopRow {
   RowVecs<T> vecs;
   int chunk, w0, mine;  // a warp's vectors, this thread's: w0 + i * 32 + lane
   int turn = 0;
+  float below = 0.f;  // this thread's sum of 2^((x - bound) c) over the logits below gather()'s bound
 
   __device__ uint4 vec(int i) const {
     if (i >= mine) return vec_neg_inf<T>();
     return HELD ? held[i * NT + threadIdx.x] : vecs.load(w0 + i * 32 + (threadIdx.x & 31));
-  }
-  // The place in a list of each lane's `mine` entries, behind those that the list has.
-  static __device__ __forceinline__ int place(int* n, int mine) {
-    const int lane = threadIdx.x & 31;
-    int before = mine;
-#pragma unroll
-    for (int d = 1; d < 32; d *= 2) {
-      const int other = __shfl_up_sync(0xffffffff, before, d);
-      if (lane >= d) before += other;
-    }
-    int at = 0;
-    if (lane == 31 && before) at = atomicAdd(n, before);
-    return __shfl_sync(0xffffffff, at, 31) + before - mine;
   }
   __device__ int first(int i) const { return vecs.first(w0 + i * 32 + (threadIdx.x & 31)); }
   // f(vector, its number), four in flight; some behind the last read as -inf
@@ -96,6 +84,23 @@ struct TopRow {
   __device__ int count_of(int n) {
     return (int)reduce((uint32_t)n, [](uint32_t x) { return __reduce_add_sync(0xffffffff, x); }) / (32 / W);
   }
+  // The place in a list of this thread's `mine` entries, by thread; `n`, what the list has, counts on.
+  __device__ __forceinline__ int place(int& n, int mine) {
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    int before = mine;
+#pragma unroll
+    for (int d = 1; d < 32; d *= 2) {
+      const int other = __shfl_up_sync(0xffffffff, before, d);
+      if (lane >= d) before += other;
+    }
+    if (lane == 31) sh.part[turn][w] = before;
+    __syncthreads();
+    const int of_warp = lane < W ? (int)sh.part[turn][lane] : 0;
+    turn ^= 1;
+    const int at = n + before - mine + __reduce_add_sync(0xffffffff, lane < w ? of_warp : 0);
+    n += __reduce_add_sync(0xffffffff, of_warp);
+    return at;
+  }
   __device__ float sum_of(float s) {
     s = warp_sum(s);
     if ((threadIdx.x & 31) == 0) sh.sum[threadIdx.x >> 5] = s;
@@ -123,13 +128,14 @@ struct TopRow {
   }
   // Candidates: keys from `bound` on; their number, or more than TOP_CAP. First the vectors that hold any, then those vectors'
   // elements: a warp in which a few lanes look at eight elements each takes as long as if all did. A thread marks its vectors
-  // in a word first, and a warp takes its places in the list at once: at 64 of 32000 nearly every warp has some in every turn.
-  __device__ __noinline__ int gather(uint32_t bound) {
+  // in a word first, and the CTA takes its places in the list at once: at 64 of 32000 nearly every warp has some in every turn.
+  // Both steps sum what is below the bound. The lists are in the threads' order, so that the sum's order is always the same.
+  __device__ __noinline__ int gather(uint32_t bound, float c) {
     const int t = threadIdx.x;
-    __syncthreads();
-    if (t == 0) sh.n = sh.n_vecs = 0;
-    __syncthreads();
     const float edge = of_key(bound);
+    const Pair edge2(-edge, -edge), c2(c, c);
+    Pair sum(0.f, 0.f);
+    int n_vecs = 0, n = 0;
 #pragma unroll 1
     for (int i0 = 0; i0 < chunk / 32; i0 += 32) {
       uint32_t marks = 0;
@@ -140,31 +146,46 @@ struct TopRow {
         for (int j = 0; j < 4; ++j) u[j] = vec(i + j);
         uint32_t four = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) four |= (uint32_t)!(vec_max<T>(u[j]) < edge) << j;  // a NaN too
+        for (int j = 0; j < 4; ++j) {
+          const bool some = !(vec_max<T>(u[j]) < edge);  // a NaN too
+          four |= (uint32_t)some << j;
+          Pair x[E / 2];
+          vec_pairs<T>(u[j], x);
+          Pair s = exp2_fast((x[0] + edge2) * c2);
+#pragma unroll
+          for (int e = 1; e < E / 2; ++e) s = s + exp2_fast((x[e] + edge2) * c2);
+          if (!some) sum = sum + s;
+        }
         marks |= four << (i - i0);
       }
       if (mine - i0 < 32) marks &= (1u << max(mine - i0, 0)) - 1;
-      int to = place(&sh.n_vecs, __popc(marks));
+      int to = place(n_vecs, __popc(marks));
 #pragma unroll 1
       for (; marks && to < TOP_CAP; marks &= marks - 1) sh.vecs[to++] = (i0 + __ffs(marks) - 1) * NT + t;
     }
+    if (n_vecs > TOP_CAP) return TOP_CAP + 1;
     __syncthreads();
-    if (sh.n_vecs > TOP_CAP) return TOP_CAP + 1;
 #pragma unroll 1
-    for (int q0 = 0; q0 < sh.n_vecs; q0 += NT) {
+    for (int q0 = 0; q0 < n_vecs; q0 += NT) {
       const int q = q0 + t;
       uint32_t marks = 0;
       int at = 0, v = 0;
-      if (q < sh.n_vecs) {
+      if (q < n_vecs) {
         v = sh.vecs[q];
         const int of = v % NT, number = of / 32 * chunk + v / NT * 32 + of % 32;
         at = vecs.first(number);
         float x[E];
         vec_floats<T>(HELD ? held[v] : vecs.load(number), x);
 #pragma unroll
-        for (int e = 0; e < E; ++e) marks |= (uint32_t)(at + e >= 0 && at + e < vecs.V && key_of(x[e]) >= bound) << e;
+        for (int e = 0; e < E; ++e) {
+          const bool some = key_of(x[e]) >= bound;
+          marks |= (uint32_t)(some && at + e >= 0 && at + e < vecs.V) << e;
+          if (some) x[e] = -INFINITY;
+        }
+#pragma unroll
+        for (int e = 0; e < E; e += 2) sum = sum + exp2_fast((Pair(x[e], x[e + 1]) + edge2) * c2);
       }
-      int to = place(&sh.n, __popc(marks));
+      int to = place(n, __popc(marks));
 #pragma unroll 1
       for (; marks && to < TOP_CAP; marks &= marks - 1) {
         const int e = __ffs(marks) - 1;
@@ -172,8 +193,8 @@ struct TopRow {
         sh.list[to++] = (unsigned long long)key_of(LogitType<T>::one(one)) << 32 | (uint32_t)~(at + e);
       }
     }
-    __syncthreads();
-    return sh.n;
+    below = sum.sum();
+    return n;
   }
   // Candidates: keys above `bound`, and those equal to it with ids below `cut`; their number.
   __device__ __noinline__ int gather_cut(uint32_t bound, int cut) {
@@ -206,36 +227,19 @@ struct TopRow {
     __syncthreads();
     return sh.n;
   }
-  // Sum of 2^((x - ref) c) over what gather() left with this bound (a NaN is among them if there are more than k).
+  // This thread's sum of 2^((x - ref) c) over the logits below the bound, and those equal to it with ids from `cut` on.
   __device__ __noinline__ float mass_below(uint32_t bound, int cut, float ref, float c) {
-    const Pair ref2(-ref, -ref), c2(c, c);
-    const float edge = of_key(bound);
-    Pair s(0.f, 0.f);
-    if (cut >= vecs.V && edge == edge) {  // all logits equal to the bound are candidates
-      each([&](const uint4& u, int) {
-        float x[E];
-        vec_floats<T>(u, x);
+    float s = 0.f;
+    each([&](const uint4& u, int i) {
+      float x[E];
+      vec_floats<T>(u, x);
 #pragma unroll
-        for (int e = 0; e < E; e += 2)
-          s = s + exp2_fast((Pair(x[e] < edge ? x[e] : -INFINITY, x[e + 1] < edge ? x[e + 1] : -INFINITY) + ref2) * c2);
-      });
-    } else {
-      each([&](const uint4& u, int i) {
-        float x[E];
-        vec_floats<T>(u, x);
-#pragma unroll
-        for (int e = 0; e < E; e += 2) {
-          float y[2];
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint32_t key = key_of(x[e + h]);
-            y[h] = key > bound || (key == bound && first(i) + e + h < cut) ? -INFINITY : x[e + h];
-          }
-          s = s + exp2_fast((Pair(y[0], y[1]) + ref2) * c2);
-        }
-      });
-    }
-    return sum_of(s.sum());
+      for (int e = 0; e < E; ++e) {
+        const uint32_t key = key_of(x[e]);
+        s += exp2_fast(((key > bound || (key == bound && first(i) + e < cut) ? -INFINITY : x[e]) - ref) * c);
+      }
+    });
+    return s;
   }
   // The largest of them.
   __device__ __noinline__ float max_below(uint32_t bound, int cut) {
@@ -304,7 +308,9 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 3 : 1) top_logits_kernel(const
   }
   bound = r.min_of(bound);
   int cut = a.V;  // of the logits equal to the bound, those with smaller ids
-  int n = r.gather(bound);
+  const float c = a.inv_tau * 1.4426950408889634f;
+  int n = r.gather(bound, c);
+  bool usual = n <= TOP_CAP && bound > key_of(-INFINITY);
   if (n > TOP_CAP) {
     // The exact k-th largest key, and the id up to which the logits equal to it are taken.
     uint32_t kth = 0;
@@ -346,28 +352,22 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 3 : 1) top_logits_kernel(const
       left_max = max_nan(left_max, value);
     }
   }
-  // The rest relative to the bound or to the largest candidate in it; where that is too far above the others, to its largest.
-  const float c = a.inv_tau * 1.4426950408889634f;
+  // The rest relative to the bound or to the largest candidate in it; where that is too far above the others or is not a
+  // number, to its largest.
   left_max = of_key(r.max_of(key_of(left_max)));  // and its barrier for `left`
-  float ref = max_nan(of_key(bound), left_max);
-  if (bound <= key_of(-INFINITY) || !(fabsf(ref) < INFINITY)) ref = max_nan(r.max_below(bound, cut), left_max);
-#pragma unroll 1
-  for (int attempt = 0;; ++attempt) {
-    const float from = ref == -INFINITY ? 0.f : ref;
-    float s = r.mass_below(bound, cut, from, c);
+  float ref = max_nan(of_key(bound), left_max), s = 0.f;
+  usual = usual && fabsf(ref) < INFINITY;
+  const auto left = [&] {
     float sl = 0.f;
-    for (int i = t; i < n - a.k; i += NT) sl += exp2_fast((sh.left[i] - from) * c);
-    s += r.sum_of(sl);
-    if (attempt == 0 && s < 1e-24f && n < a.V) {
-      const float most = max_nan(r.max_below(bound, cut), left_max);
-      if (most != ref) {
-        ref = most;
-        continue;
-      }
-    }
-    if (t == 0) a.rest[row] = isinf(ref) ? ref : s == 0.f ? -INFINITY : fmaf(ref, a.inv_tau, logf(s));
-    return;
+    for (int i = t; i < n - a.k; i += NT) sl += exp2_fast((sh.left[i] - ref) * c);
+    return sl;
+  };
+  if (usual) s = r.sum_of(r.below * exp2_fast((of_key(bound) - ref) * c) + left());
+  if (!usual || (s < 1e-24f && n < a.V)) {
+    ref = max_nan(r.max_below(bound, cut), left_max);
+    if (fabsf(ref) < INFINITY) s = r.sum_of(r.mass_below(bound, cut, ref, c) + left());
   }
+  if (t == 0) a.rest[row] = !(fabsf(ref) < INFINITY) ? ref : s == 0.f ? -INFINITY : fmaf(ref, a.inv_tau, logf(s));
 }
 
 template <typename T, bool HELD, int NT>
