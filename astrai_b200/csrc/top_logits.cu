@@ -30,7 +30,7 @@ struct TopArgs {
 };
 
 struct TopShared {
-  unsigned long long list[TOP_CAP + 2];  // key, then the id's complement: greater ranks first
+  unsigned long long list[TOP_CAP];  // key, then the id's complement: greater ranks first
   float left[TOP_CAP];                   // logits of candidates that are not among the k
   uint32_t vecs[TOP_CAP];                // vectors that hold candidates
   uint32_t part[2][16];
@@ -328,19 +328,36 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 3 : 1) top_logits_kernel(const
     n = r.gather_cut(bound, cut);
   }
 
-  // Ranks: each candidate against all, two at a time.
+  // Ranks: each warp sorts 32 candidates at a time; one's rank is its place there and, by bisection, how many of each other 32
+  // are greater.
   float left_max = -INFINITY;
-  if (t == 0) sh.list[n] = 0;
+  const int runs = (n + 31) / 32;
+  __syncthreads();
+#pragma unroll 1
+  for (int i = t; i < runs * 32; i += NT) {
+    unsigned long long v = i < n ? sh.list[i] : 0;
+#pragma unroll
+    for (int of = 2; of <= 32; of *= 2)
+#pragma unroll
+      for (int d = of / 2; d; d /= 2) {
+        const unsigned long long other = __shfl_xor_sync(0xffffffff, v, d);
+        if ((other > v) == (((lane & d) == 0) == ((lane & of) == 0))) v = other;
+      }
+    sh.list[i] = v;
+  }
   __syncthreads();
 #pragma unroll 1
   for (int i = t; i < n; i += NT) {
     const unsigned long long mine = sh.list[i];
-    int rank = 0;
-    const ulonglong2* two = reinterpret_cast<const ulonglong2*>(sh.list);
-#pragma unroll 4
-    for (int l = 0; l < n; l += 2) {
-      const ulonglong2 other = two[l / 2];
-      rank += (other.x > mine) + (other.y > mine);
+    int rank = lane;
+#pragma unroll 2
+    for (int run = 0; run < runs; ++run) {
+      const unsigned long long* const sorted = sh.list + run * 32;
+      int greater = 0;
+#pragma unroll
+      for (int step = 16; step; step /= 2) greater += sorted[greater + step - 1] > mine ? step : 0;
+      greater += sorted[greater] > mine;
+      rank += run == i / 32 ? 0 : greater;
     }
     const float value = of_key((uint32_t)(mine >> 32));
     if (rank < a.k) {
