@@ -22,7 +22,7 @@ void distill(const void* x, long long ldx, void* dx, long long lddx, const void*
              float* count, bool have_count, float* loss, int dtype, int device, cudaStream_t s);
 int top_logits_max_k();
 void top_logits(const void* x, long long ldx, int rows, int V, int k, float tau, int* ids, void* values, float* rest,
-                int dtype, int device, cudaStream_t s);
+                int dtype, cudaStream_t s);
 void sample_given(const void* x, long long ldx, int rows, int V, const void* uniform, bool uniform64,
                   const float* temperature, const int* top_k, const float* top_p, const float* min_p, long long* token,
                   float* logprob, int dtype, int device, cudaStream_t s);
@@ -78,7 +78,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> top_logits(const at::Tensor& logi
        rest = new_like(x, {rows}, at::kFloat);
   if (rows > 0) {
     astrai_host::top_logits(x.data_ptr(), row_stride(x), (int)rows, (int)V, (int)k, (float)tau, ids.data_ptr<int>(),
-                            values.data_ptr(), rest.data_ptr<float>(), code, x.get_device(), stream());
+                            values.data_ptr(), rest.data_ptr<float>(), code, stream());
     C10_CUDA_KERNEL_LAUNCH_CHECK();
   }
   if (logits.dim() != 2) {

@@ -3,13 +3,21 @@
 // Equal logits rank by id, the lowest first; a NaN ranks above every number. `rest` is log sum exp(x_v / tau) over the
 // tokens that are not among the k.
 //
-// A CTA takes a row: 256 threads, three on an SM, where it is no longer than 68 KB, else 512 threads that have an SM to
-// themselves. A row of up to 200 KB stays in shared memory, a longer one comes from L2 again (three such rows on every SM would
-// not fit there: 768 rows of 131072 bf16 took 211 us). Nothing is sorted but a few candidates: the largest logits of both halves of every thread's part make 64 numbers a
-// warp, and the smallest, over the W warps, of each warp's j-th largest is a bound that at least W j >= k logits reach (for
-// k = 64 of 32000 about 150 do). Those are ranked by comparing each with all; the others, and the candidates that do not make
-// it, give `rest`. Where more than TOP_CAP logits reach the bound (ties), the exact k-th largest and the id that cuts its ties
-// are found by bisection.
+// A CTA takes a row and reads it twice, from memory and then from L2. Nothing is sorted but a few candidates: in the first
+// reading the largest logits of both halves of every thread's part make 64 numbers a warp, and the smallest, over the W warps,
+// of each warp's j-th largest is a bound that at least W j >= k logits reach (for k = 64 of 32000 about 100 do). The second
+// reading finds those and sums the others, relative to the bound, for `rest`; the candidates that do not make it are added.
+// Where more than TOP_CAP logits reach the bound (ties), the exact k-th largest and the id that cuts its ties are found by
+// bisection.
+//
+// What bounds it is a row's chain of steps with a barrier behind each, so small CTAs of 64 registers a thread, 32 warps of them
+// on an SM, hide most of it: 8192 rows of 32000 bf16, k = 64, take 195 us (2.7 TB/s of what has to be read; the
+// exponentials alone, 16 a clock and SM, 58 us) with 128 threads a row, 225 with 256 and 346 with 512. Rows kept in shared memory
+// between the readings left room for 24 warps and took 261 us. More threads take a row where there are too few rows to fill
+// the GPU, or where the rows of all CTAs at a time would not stay in L2 (2048 rows of 50021 bf16: 128 threads 119 us, 256 threads
+// 107 us; 999 rows of 50021 fp32: 125 us, and 107 with 512).
+#include <algorithm>
+
 #include "launch.cuh"
 #include "logits.cuh"
 
@@ -17,7 +25,7 @@ namespace astrai {
 
 constexpr int TOP_MAX_K = 256;
 constexpr int TOP_CAP = 1024;
-constexpr int TOP_HELD = 68 * 1024, TOP_HELD_ALONE = 200 * 1024;
+constexpr long long TOP_L2 = 96ll << 20;  // bytes of rows that stay in L2 between a row's two readings
 
 struct TopArgs {
   const void* x;
@@ -33,24 +41,32 @@ struct TopShared {
   unsigned long long list[TOP_CAP];  // key, then the id's complement: greater ranks first
   float left[TOP_CAP];                   // logits of candidates that are not among the k
   uint32_t vecs[TOP_CAP];                // vectors that hold candidates
-  uint32_t part[2][16];
-  float sum[16];
+  uint32_t part[2][32];
+  float sum[32];
   int n;
 };
 
-template <typename T, bool HELD, int NT>
+template <typename T, int NT>
 struct TopRow {
   static constexpr int E = LogitType<T>::E, W = NT / 32;
   TopShared& sh;
-  const uint4* held;
   RowVecs<T> vecs;
   int chunk, w0, mine;  // a warp's vectors, this thread's: w0 + i * 32 + lane
   int turn = 0;
   float below = 0.f;  // this thread's sum of 2^((x - bound) c) over the logits below gather()'s bound
 
-  __device__ uint4 vec(int i) const {
-    if (i >= mine) return vec_neg_inf<T>();
-    return HELD ? held[i * NT + threadIdx.x] : vecs.load(w0 + i * 32 + (threadIdx.x & 31));
+  // Vectors i to i + N - 1, -inf behind the last. Without the row's ends, N loads without a branch.
+  template <int N>
+  __device__ __forceinline__ void load(int i, uint4 (&u)[N]) const {
+    const int at = w0 + i * 32, lane = threadIdx.x & 31;
+    if (at > 0 && i + N <= chunk / 32 && at + N * 32 < vecs.n) {
+      const uint4* const from = reinterpret_cast<const uint4*>(vecs.row - vecs.head) + at + lane;
+#pragma unroll
+      for (int j = 0; j < N; ++j) u[j] = __ldg(from + j * 32);
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j) u[j] = i + j < mine ? vecs.load(at + j * 32 + lane) : vec_neg_inf<T>();
+    }
   }
   __device__ int first(int i) const { return vecs.first(w0 + i * 32 + (threadIdx.x & 31)); }
   // f(vector, its number), four in flight; some behind the last read as -inf
@@ -59,8 +75,7 @@ struct TopRow {
 #pragma unroll 1
     for (int i = 0; i < mine; i += 4) {
       uint4 u[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) u[j] = vec(i + j);
+      load(i, u);
 #pragma unroll
       for (int j = 0; j < 4; ++j) f(u[j], i + j);
     }
@@ -142,13 +157,12 @@ struct TopRow {
 #pragma unroll 1
       for (int i = i0; i < min(i0 + 32, chunk / 32); i += 4) {
         uint4 u[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) u[j] = vec(i + j);
-        uint32_t four = 0;
+        load(i, u);
+        uint32_t some4 = 0;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           const bool some = !(vec_max<T>(u[j]) < edge);  // a NaN too
-          four |= (uint32_t)some << j;
+          some4 |= (uint32_t)some << j;
           Pair x[E / 2];
           vec_pairs<T>(u[j], x);
           Pair s = exp2_fast((x[0] + edge2) * c2);
@@ -156,7 +170,7 @@ struct TopRow {
           for (int e = 1; e < E / 2; ++e) s = s + exp2_fast((x[e] + edge2) * c2);
           if (!some) sum = sum + s;
         }
-        marks |= four << (i - i0);
+        marks |= some4 << (i - i0);
       }
       if (mine - i0 < 32) marks &= (1u << max(mine - i0, 0)) - 1;
       int to = place(n_vecs, __popc(marks));
@@ -169,13 +183,12 @@ struct TopRow {
     for (int q0 = 0; q0 < n_vecs; q0 += NT) {
       const int q = q0 + t;
       uint32_t marks = 0;
-      int at = 0, v = 0;
+      int at = 0;
       if (q < n_vecs) {
-        v = sh.vecs[q];
-        const int of = v % NT, number = of / 32 * chunk + v / NT * 32 + of % 32;
+        const int v = sh.vecs[q], of = v % NT, number = of / 32 * chunk + v / NT * 32 + of % 32;
         at = vecs.first(number);
         float x[E];
-        vec_floats<T>(HELD ? held[v] : vecs.load(number), x);
+        vec_floats<T>(vecs.load(number), x);
 #pragma unroll
         for (int e = 0; e < E; ++e) {
           const bool some = key_of(x[e]) >= bound;
@@ -189,8 +202,7 @@ struct TopRow {
 #pragma unroll 1
       for (; marks && to < TOP_CAP; marks &= marks - 1) {
         const int e = __ffs(marks) - 1;
-        const T one = HELD ? reinterpret_cast<const T*>(held)[v * E + e] : vecs.row[at + e];
-        sh.list[to++] = (unsigned long long)key_of(LogitType<T>::one(one)) << 32 | (uint32_t)~(at + e);
+        sh.list[to++] = (unsigned long long)key_of(LogitType<T>::one(vecs.row[at + e])) << 32 | (uint32_t)~(at + e);
       }
     }
     below = sum.sum();
@@ -259,14 +271,13 @@ struct TopRow {
   }
 };
 
-template <typename T, bool HELD, int NT>
-__global__ void __launch_bounds__(NT, NT == 256 ? 3 : 1) top_logits_kernel(const TopArgs a) {
+template <typename T, int NT>
+__global__ void __launch_bounds__(NT, 1024 / NT) top_logits_kernel(const TopArgs a) {
   constexpr int W = NT / 32;
-  extern __shared__ uint4 top_held[];  // vector i of thread t at i * NT + t
   __shared__ __align__(16) TopShared sh;
   const int t = threadIdx.x, lane = t & 31, w = t >> 5, row = blockIdx.x;
   begin_early();
-  TopRow<T, HELD, NT> r{sh, top_held, RowVecs<T>(static_cast<const T*>(a.x) + (long long)row * a.ldx, a.V)};
+  TopRow<T, NT> r{sh, RowVecs<T>(static_cast<const T*>(a.x) + (long long)row * a.ldx, a.V)};
   r.chunk = (r.vecs.n + NT - 1) / NT * 32;
   r.w0 = w * r.chunk;
   r.mine = max(0, min(r.chunk / 32, (min(r.w0 + r.chunk, r.vecs.n) - r.w0 - lane + 31) / 32));
@@ -275,13 +286,11 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 3 : 1) top_logits_kernel(const
   float top[2] = {-INFINITY, -INFINITY};
   const int half = (r.mine + 1) / 2;
 #pragma unroll 1
-  for (int i0 = 0; i0 < r.mine; i0 += 8) {
-    uint4 u[8];
+  for (int i0 = 0; i0 < r.mine; i0 += 4) {
+    uint4 u[4];
+    r.load(i0, u);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) u[i] = i0 + i < r.mine ? r.vecs.load(r.w0 + (i0 + i) * 32 + lane) : vec_neg_inf<T>();
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      if (HELD && i0 + i < r.mine) top_held[(i0 + i) * NT + t] = u[i];
+    for (int i = 0; i < 4; ++i) {
       const float most = vec_max<T>(u[i]);
       if (i0 + i < half) top[0] = max_nan(top[0], most);
       else top[1] = max_nan(top[1], most);
@@ -372,40 +381,37 @@ __global__ void __launch_bounds__(NT, NT == 256 ? 3 : 1) top_logits_kernel(const
   // The rest relative to the bound or to the largest candidate in it; where that is too far above the others or is not a
   // number, to its largest.
   left_max = of_key(r.max_of(key_of(left_max)));  // and its barrier for `left`
-  float ref = max_nan(of_key(bound), left_max), s = 0.f;
-  usual = usual && fabsf(ref) < INFINITY;
+  float ref = n < a.V ? max_nan(of_key(bound), left_max) : left_max, s = 0.f;
   const auto left = [&] {
     float sl = 0.f;
     for (int i = t; i < n - a.k; i += NT) sl += exp2_fast((sh.left[i] - ref) * c);
     return sl;
   };
-  if (usual) s = r.sum_of(r.below * exp2_fast((of_key(bound) - ref) * c) + left());
-  if (!usual || (s < 1e-24f && n < a.V)) {
+  if (n == a.V) {
+    if (fabsf(ref) < INFINITY) s = r.sum_of(left());
+  } else if (usual && fabsf(ref) < INFINITY) {
+    s = r.sum_of(r.below * exp2_fast((of_key(bound) - ref) * c) + left());
+  }
+  if (n < a.V && !(s >= 1e-24f)) {
     ref = max_nan(r.max_below(bound, cut), left_max);
     if (fabsf(ref) < INFINITY) s = r.sum_of(r.mass_below(bound, cut, ref, c) + left());
   }
   if (t == 0) a.rest[row] = !(fabsf(ref) < INFINITY) ? ref : s == 0.f ? -INFINITY : fmaf(ref, a.inv_tau, logf(s));
 }
 
-template <typename T, bool HELD, int NT>
-void top_launch(const TopArgs& a, int smem, int device, cudaStream_t s) {
-  auto* kernel = top_logits_kernel<T, HELD, NT>;
-  static bool ready[64] = {};  // per device
-  if (device < 0 || device >= 64 || !ready[device]) {
-    cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, NT == 256 ? TOP_HELD : TOP_HELD_ALONE);
-    if (device >= 0 && device < 64) ready[device] = true;
-  }
-  launch_early(kernel, dim3((unsigned)a.rows), dim3(NT), smem, s, a);
-}
-
 template <typename T>
-void top_typed(const TopArgs& a, int device, cudaStream_t s) {
-  constexpr int E = LogitType<T>::E;
-  const int vecs = (a.V + E - 1) / E + 1;  // one more where a row starts off the grid
-  const auto held = [&](int threads) { return (vecs + threads - 1) / threads * threads * 16; };
-  if (held(256) <= TOP_HELD) top_launch<T, true, 256>(a, held(256), device, s);
-  else if (held(512) <= TOP_HELD_ALONE) top_launch<T, true, 512>(a, held(512), device, s);
-  else top_launch<T, false, 512>(a, TOP_HELD_ALONE / 2 + 32 * 1024, device, s);  // (asked for to be alone)
+void top_typed(const TopArgs& a, cudaStream_t s) {
+  const auto launch = [&](auto* kernel, int threads) { launch_early(kernel, dim3((unsigned)a.rows), dim3(threads), 0, s, a); };
+  constexpr int SMS = 148;
+  const long long vecs = (a.V + LogitType<T>::E - 1) / LogitType<T>::E;
+  int threads = 128;
+  const auto rows = [&](int n) { return std::min<long long>(a.rows, SMS * (1024 / n)); };  // at a time
+  while (threads < 1024 && ((rows(threads) == rows(2 * threads) && vecs >= 16 * threads) || rows(threads) * vecs * 16 > TOP_L2))
+    threads *= 2;
+  if (threads == 128) launch(top_logits_kernel<T, 128>, 128);
+  else if (threads == 256) launch(top_logits_kernel<T, 256>, 256);
+  else if (threads == 512) launch(top_logits_kernel<T, 512>, 512);
+  else launch(top_logits_kernel<T, 1024>, 1024);
 }
 
 }  // namespace astrai
@@ -416,11 +422,11 @@ using namespace astrai;
 int top_logits_max_k() { return TOP_MAX_K; }
 
 void top_logits(const void* x, long long ldx, int rows, int V, int k, float tau, int* ids, void* values, float* rest,
-                int dtype, int device, cudaStream_t s) {
+                int dtype, cudaStream_t s) {
   const TopArgs a{x, ldx, rows, V, k, 1.f / tau, ids, values, rest};
-  if (dtype == 0) top_typed<__nv_bfloat16>(a, device, s);
-  else if (dtype == 1) top_typed<__half>(a, device, s);
-  else top_typed<float>(a, device, s);
+  if (dtype == 0) top_typed<__nv_bfloat16>(a, s);
+  else if (dtype == 1) top_typed<__half>(a, s);
+  else top_typed<float>(a, s);
 }
 
 }  // namespace astrai_host
