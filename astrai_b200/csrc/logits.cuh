@@ -78,21 +78,6 @@ __device__ __forceinline__ uint4 vec_neg_inf() {
   return make_uint4(w, w, w, w);
 }
 
-// Elements of `u` whose bit of `bits` is set become -inf.
-template <typename T>
-__device__ __forceinline__ void vec_mask(uint4& u, uint32_t bits) {
-  uint32_t* const w[4] = {&u.x, &u.y, &u.z, &u.w};
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    if constexpr (LogitType<T>::E == 4) {
-      if (bits >> j & 1) *w[j] = LogitType<T>::kNegInf;
-    } else {
-      if (bits >> (2 * j) & 1) *w[j] = (*w[j] & 0xFFFF0000u) | LogitType<T>::kNegInf;
-      if (bits >> (2 * j + 1) & 1) *w[j] = (*w[j] & 0x0000FFFFu) | (LogitType<T>::kNegInf << 16);
-    }
-  }
-}
-
 // Largest element, a NaN only if there is nothing else.
 template <typename T>
 __device__ __forceinline__ float vec_max_number(const uint4& u) {
@@ -126,6 +111,20 @@ struct RowVecs {
     const int at = first(vec);
     if (at >= 0 && at + E <= V) return __ldg(reinterpret_cast<const uint4*>(row + at));
     return load_edge(at);
+  }
+  // This lane's vectors at + lane, at + 32 + lane, .., of which the warp has `rows` and this lane `mine` before its part ends
+  // (-inf from there). Away from the row's ends they are N loads without a branch.
+  template <int N>
+  __device__ __forceinline__ void load(int at, int rows, int mine, uint4 (&u)[N]) const {
+    const int lane = threadIdx.x & 31;
+    if (at > 0 && N <= rows && at + N * 32 < n) {
+      const uint4* const from = reinterpret_cast<const uint4*>(row - head) + at + lane;
+#pragma unroll
+      for (int j = 0; j < N; ++j) u[j] = __ldg(from + j * 32);
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j) u[j] = j < mine ? load(at + j * 32 + lane) : vec_neg_inf<T>();
+    }
   }
   __device__ __noinline__ uint4 load_edge(int at) const {
     float f[E];

@@ -155,6 +155,14 @@ struct Sampler {
       if (i >= mine) return vec_neg_inf<T>();
       return HELD ? held()[i * NT + threadIdx.x] : vecs.load(w0 + i * 32 + (threadIdx.x & 31));
     }
+    __device__ __forceinline__ void four(int i, uint4 (&u)[4]) const {
+      if constexpr (HELD) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) u[j] = vec(i + j);
+      } else {
+        vecs.load(w0 + i * 32, shared().chunk / 32 - i, mine - i, u);
+      }
+    }
   };
   // f(vector, its number) over this thread's vectors of the groups that reach `low`, four in flight (with some behind the
   // last that read as -inf); g(group) after each
@@ -167,8 +175,7 @@ struct Sampler {
 #pragma unroll 1
         for (int i = i0; i < end; i += 4) {
           uint4 u[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) u[j] = me.vec(i + j);
+          me.four(i, u);
 #pragma unroll
           for (int j = 0; j < 4; ++j) f(u[j], i + j);
         }
@@ -323,15 +330,22 @@ struct Sampler {
     error = precise || total == 0. ? 0. : total * (4.5e-7 + 1.3e-7 * fmaxf(log2f((float)shared().V) - log2f((float)total), 0.f));
     return total;
   }
-  // Numbers at the lanes for which `some` holds, behind those that a list has.
-  static __device__ __forceinline__ int place(int* n, bool some) {
-    const uint32_t lanes = __ballot_sync(0xffffffff, some);
+  // The place of this lane's `mine` entries in a list, behind those that it has: one atomic a warp.
+  static __device__ __forceinline__ int place(int* n, int mine) {
+    const int lane = threadIdx.x & 31;
+    int upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int up = __shfl_up_sync(0xffffffff, upto, o);
+      if (lane >= o) upto += up;
+    }
     int at = 0;
-    if ((threadIdx.x & 31) == 0 && lanes) at = atomicAdd(n, __popc(lanes));
-    return __shfl_sync(0xffffffff, at, 0) + __popc(lanes & ((1u << (threadIdx.x & 31)) - 1));
+    if (lane == 31 && upto > 0) at = atomicAdd(n, upto);
+    return __shfl_sync(0xffffffff, at, 31) + upto - mine;
   }
-  // Candidates: the logits from `low` on, if they are not too many; their number. First the vectors that hold any, then those
-  // vectors' elements, one a thread: a warp in which a few lanes look at eight elements each takes as long as if all did.
+  // Candidates: the logits from `low` on, if they are not too many; their number. First the vectors that hold any, marked in a
+  // word for up to 32 of a thread's, then those vectors' elements, a vector a thread: a warp in which a few lanes look at eight
+  // elements each takes as long as if all did.
   static __device__ __noinline__ int gather_top(float low) {
     SampleShared& sh = shared();
     const Mine me(sh);
@@ -345,35 +359,52 @@ struct Sampler {
       const bool may = i0 < end && tops()[at * NT + t + (HELD ? sh.chunk / 32 * NT * 4 : 0)] >= low;
       if (!__any_sync(0xffffffff, may)) continue;
 #pragma unroll 1
-      for (int i = i0; i < min(i0 + sh.group, sh.chunk / 32); i += 4) {
-        uint4 u[4];
+      for (int i1 = i0; i1 < min(i0 + sh.group, sh.chunk / 32); i1 += 32) {
+        uint32_t marks = 0;
+        if (may) {
+#pragma unroll 1
+          for (int i = i1; i < min(i1 + 32, end); i += 4) {
+            uint4 u[4];
+            me.four(i, u);
+            uint32_t some = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) u[j] = may && i + j < end ? me.vec(i + j) : vec_neg_inf<T>();
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const bool some = vec_max<T>(u[j]) >= low;
-          if (!__any_sync(0xffffffff, some)) continue;
-          const int to = place(&sh.hit, some);
-          if (some && to < SG_CAP) sh.sorted[to] = (i + j) * NT + t;
+            for (int j = 0; j < 4; ++j) some |= (uint32_t)(i + j < end && vec_max<T>(u[j]) >= low) << j;
+            marks |= some << (i - i1);
+          }
         }
+        __syncwarp();
+        int to = place(&sh.hit, __popc(marks));
+#pragma unroll 1
+        for (; marks && to < SG_CAP; marks &= marks - 1) sh.sorted[to++] = (i1 + __ffs(marks) - 1) * NT + t;
       }
     }
     __syncthreads();
-    const int vecs = sh.hit, all = vecs * E;
-    if (vecs > SG_CAP) return SG_CAP + 1;
+    const int n = sh.hit;
+    if (n > SG_CAP) return SG_CAP + 1;
 #pragma unroll 1
-    for (int q0 = 0; q0 < all; q0 += NT) {
+    for (int q0 = 0; q0 < n; q0 += NT) {
       const int q = q0 + t;
-      int id = -1;
-      float x = -INFINITY;
-      if (q < all) {
-        const int v = sh.sorted[q / E], of = v % NT;
-        id = me.vecs.first(of / 32 * sh.chunk + v / NT * 32 + of % 32) + q % E;
-        if (id >= 0 && id < sh.V) x = LogitType<T>::one(HELD ? reinterpret_cast<const T*>(held())[v * E + q % E] : me.vecs.row[id]);
+      uint32_t marks = 0;
+      int first = 0;
+      float x[E];
+      if (q < n) {
+        const int v = sh.sorted[q], of = v % NT, number = of / 32 * sh.chunk + v / NT * 32 + of % 32;
+        first = me.vecs.first(number);
+        vec_floats<T>(HELD ? held()[v] : me.vecs.load(number), x);
+#pragma unroll
+        for (int e = 0; e < E; ++e) marks |= (uint32_t)(x[e] >= low && first + e >= 0 && first + e < sh.V) << e;
       }
-      const bool some = x >= low;
-      const int to = place(&sh.n, some);
-      if (some && to < SG_CAP) sh.key[to] = key_of(x), sh.id[to] = id;
+      __syncwarp();
+      int to = place(&sh.n, __popc(marks));
+#pragma unroll 1
+      for (; marks && to < SG_CAP; marks &= marks - 1, ++to) {
+        const int e = __ffs(marks) - 1;
+        float one = x[0];
+#pragma unroll
+        for (int j = 1; j < E; ++j) one = e == j ? x[j] : one;
+        sh.key[to] = key_of(one);
+        sh.id[to] = first + e;
+      }
     }
     __syncthreads();
     return sh.n;
@@ -938,8 +969,7 @@ __global__ void __launch_bounds__(SG_THREADS, 2) sample_given_kernel(const Sampl
 #pragma unroll 1
   for (int i0 = 0; i0 < mine; i0 += SG_VECS) {
     uint4 u[SG_VECS];
-#pragma unroll
-    for (int i = 0; i < SG_VECS; ++i) u[i] = i0 + i < mine ? vecs.load(w0 + (i0 + i) * 32 + lane) : vec_neg_inf<T>();
+    vecs.load(w0 + i0 * 32, chunk / 32 - i0, mine - i0, u);
 #pragma unroll
     for (int i = 0; i < SG_VECS; ++i) {
       if (HELD && i0 + i < mine) S::held()[(i0 + i) * NT + t] = u[i];

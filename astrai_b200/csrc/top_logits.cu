@@ -55,19 +55,7 @@ struct TopRow {
   int turn = 0;
   float below = 0.f;  // this thread's sum of 2^((x - bound) c) over the logits below gather()'s bound
 
-  // Vectors i to i + N - 1, -inf behind the last. Without the row's ends, N loads without a branch.
-  template <int N>
-  __device__ __forceinline__ void load(int i, uint4 (&u)[N]) const {
-    const int at = w0 + i * 32, lane = threadIdx.x & 31;
-    if (at > 0 && i + N <= chunk / 32 && at + N * 32 < vecs.n) {
-      const uint4* const from = reinterpret_cast<const uint4*>(vecs.row - vecs.head) + at + lane;
-#pragma unroll
-      for (int j = 0; j < N; ++j) u[j] = __ldg(from + j * 32);
-    } else {
-#pragma unroll
-      for (int j = 0; j < N; ++j) u[j] = i + j < mine ? vecs.load(at + j * 32 + lane) : vec_neg_inf<T>();
-    }
-  }
+  __device__ __forceinline__ void load(int i, uint4 (&u)[4]) const { vecs.load(w0 + i * 32, chunk / 32 - i, mine - i, u); }
   __device__ int first(int i) const { return vecs.first(w0 + i * 32 + (threadIdx.x & 31)); }
   // f(vector, its number), four in flight; some behind the last read as -inf
   template <typename F>
