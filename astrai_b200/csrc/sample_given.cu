@@ -260,7 +260,8 @@ struct Sampler {
       for (int e = 0; e < o; ++e) q[e] = q[e] + q[e + o];
     return (double)q[0].sum();
   }
-  static __device__ __forceinline__ double vec_mass_64(const uint4& u, float low, double max_x, double c64) {
+  // In 64 bits, and that of the logits from `high` on added to `above`.
+  static __device__ __forceinline__ double vec_mass_64(const uint4& u, float low, double max_x, double c64, float high, double& above) {
     float x[E];
     vec_floats<T>(u, x);
     double sum = 0.;
@@ -271,6 +272,9 @@ struct Sampler {
       for (int e = 0; e < 4; ++e) s[e] = x[e0 + e] >= low ? ((double)x[e0 + e] - max_x) * c64 : -INFINITY;
       exp2_16th(s, shared().pow);
       sum += (s[0] + s[1]) + (s[2] + s[3]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (x[e0 + e] >= high) above += s[e];
     }
     return sum;
   }
@@ -279,32 +283,35 @@ struct Sampler {
     const SampleShared& sh = shared();
     const Mine me(sh);
     const Pair ref2(-sh.max_x, -sh.max_x), c2(sh.c, sh.c);
+    double none = 0.;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       const uint4 u = i + j < end ? me.vec(i + j) : vec_neg_inf<T>();
-      s[j] = precise ? vec_mass_64(u, low, sh.max_x, sh.c64) : vec_mass(u, low, ref2, c2);
+      s[j] = precise ? vec_mass_64(u, low, sh.max_x, sh.c64, INFINITY, none) : vec_mass(u, low, ref2, c2);
       if (j == which) mine = s[j];
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j) s[j] = warp_add(s[j]);
   }
-  // The row's mass from `low` on; by warps in sh.warp_sum, by their groups in sh.group_sum.
-  static __device__ __noinline__ double mass_64(float low) {
+  // The row's mass from `low` on; by warps in sh.warp_sum, by their groups in sh.group_sum. That from `high` on in `above`: both
+  // in one pass, as 13 operations of 64 bits a logit bound it (32000 logits: 12000 clocks).
+  static __device__ __noinline__ double mass_64(float low, float high, double& above) {
     SampleShared& sh = shared();
     const Mine me(sh);
     const double max_x = sh.max_x, c64 = sh.c64;
-    double s = 0.;
+    double s = 0., s_high = 0.;
 #pragma unroll 1
     for (int i0 = 0, at = 0; i0 < sh.chunk / 32; i0 += sh.group, ++at) {
       double part = 0.;
 #pragma unroll 1
-      for (int i = i0; i < min(i0 + sh.group, me.mine); ++i) part += vec_mass_64(me.vec(i), low, max_x, c64);
+      for (int i = i0; i < min(i0 + sh.group, me.mine); ++i) part += vec_mass_64(me.vec(i), low, max_x, c64, high, s_high);
       s += part;
       if (!HELD) {
         part = warp_add(part);
         if ((threadIdx.x & 31) == 0) sh.group_sum[threadIdx.x / 32][at] = part;
       }
     }
+    if (high < INFINITY) above = scan(s_high).y;
     return scan(s).y;
   }
   static __device__ __noinline__ double mass_32(float low) {
@@ -326,7 +333,8 @@ struct Sampler {
   // With a bound on its error: the mass' average |t| is the entropy of its shares less log2 of it (the largest weight is 1),
   // at most log2 V - log2 total.
   static __device__ __forceinline__ double mass(bool precise, float low, double& error) {
-    const double total = precise ? mass_64(low) : mass_32(low);
+    double none;
+    const double total = precise ? mass_64(low, INFINITY, none) : mass_32(low);
     error = precise || total == 0. ? 0. : total * (4.5e-7 + 1.3e-7 * fmaxf(log2f((float)shared().V) - log2f((float)total), 0.f));
     return total;
   }
@@ -829,9 +837,10 @@ struct Sampler {
         double above;
 #pragma unroll 1
         for (;; precise = 1) {
-          if (precise && error > 0.) total = mass(true, from(kth), error);
           double blur = 0.;
-          above = first > 0 ? mass(precise, fmaxf(high, from(kth)), blur) : 0.;
+          above = 0.;
+          if (precise) total = mass_64(from(kth), fmaxf(high, from(kth)), above), error = 0.;
+          else if (first > 0) above = mass(false, fmaxf(high, from(kth)), blur);
           verdict = bound(n, above, sh.p * total, blur + sh.p * error, last == SG_BINS - 1 || low == kth);
           if (verdict != kAmbiguous) break;
         }
