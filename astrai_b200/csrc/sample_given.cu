@@ -819,7 +819,7 @@ struct Sampler {
       if (!usable(range)) continue;
       const float scale = (SG_BINS - 1) / range;
       double off = 0.;
-      // Where the steps' masses point to; if the bound does not lie there, as far on as their sum was off.
+      // Where the steps' masses point to; if the bound does not lie there, as far on as their sum was off at that side.
 #pragma unroll 1
       for (int turn = 0; turn < 4; ++turn) {
         histogram(scale, from(kth));
@@ -828,6 +828,8 @@ struct Sampler {
         if (bin >= SG_BINS - 1 && attempt == 0) break;
         const int first = min(max(bin - 2, 0), SG_BINS - 1), last = min(bin + 2, SG_BINS - 1);
         const double guess = mass_of_bins(first, scale);
+        double guess_last = guess;
+        for (int i = first; i <= last; ++i) guess_last += (double)((float)sh.bins[i] * exp2_fast(-((float)i + 0.5f) / scale * sh.c));
         const float high = first > 0 ? of_key(edge_of(first, scale)) : INFINITY;
         const uint32_t low = max(last == SG_BINS - 1 ? kLowest : edge_of(last + 1, scale), kth);
         const int n = gather(from(low), high);
@@ -845,7 +847,9 @@ struct Sampler {
           if (verdict != kAmbiguous) break;
         }
         if (verdict == kDone) return sh.low;
-        off = above - guess;
+        // The next turn's target is then below what the steps hold before `first`, or not below what they hold up to `last`.
+        if (above > sh.p * total || n == 0) off = above - guess;
+        else off = above + mass_before(n) - guess_last;
       }
     }
 #pragma unroll 1
