@@ -18,9 +18,12 @@
 // the gradient from there, and one more warp does what is small: the sums over J, the row's coefficients and loss, the copy of
 // the next row. A warp that works alone spends about 15 clocks on an instruction, so that the marks and gradients of J are
 // spread over all threads. Three CTAs share an SM, so that one row is copied or written while others are computed. (With the row in
-// registers and J spread over 512 threads, 60 % of the instructions were the same few for every thread: 8192 rows of 32000
-// took 373 us, forward only 220.) A row that does not fit is shared by a cluster, whose extra warps exchange the sums through
-// distributed shared memory.
+// registers and J spread over 512 threads, 60 % of the instructions were the same few for every thread.) A row that does not fit
+// is shared by a cluster, whose extra warps exchange the sums through distributed shared memory.
+//
+// Measured: 8192 rows of 32000 bf16, k = 64: loss and gradient 230 us (4.6 TB/s of what has to be read and written), the loss
+// alone 124 us (4.2 TB/s). With tau other than 1 and h > 0 a logit takes two exponentials for the sums and two for the gradient:
+// 349 us, of which 233 are 16 exponentials a clock and SM. 768 rows of 131072 fp32 on clusters: 204 us (3.9 TB/s).
 #include <cooperative_groups.h>
 
 #include <algorithm>

@@ -13,11 +13,16 @@
 // is summed again in 64 bits.
 //
 // A CTA of 512 threads takes a row, two on an SM. Logits that fit stay in its shared memory between the passes over them,
-// others come from L2 again. (A cluster of two to eight CTAs for a row, or 1024 threads, took as long or longer: 64 rows of
-// 32000 with k = 50 16.6 and 21.8 us against 15.4 and 13.9; the barriers cost what the shorter passes save.) The bound that gathers the candidates is the one of
-// the top logits: the smallest, over the warps, of each warp's j-th largest thread maximum. Where top-p reaches below them
+// others come from L2 again. (In an earlier form 64 rows of 32000 with k = 50 took 13.9 us, 15.4 with 1024 threads and more with
+// clusters of CTAs for a row; the barriers cost what the shorter passes save.) The bound that gathers the candidates is the one
+// of the top logits: the smallest, over the warps, of each warp's j-th largest thread maximum. Where top-p reaches below them
 // (flat rows) or k is large, a histogram over 4096 equal steps of the logits shows in which steps the bound must lie, and the
 // few logits there are ordered and decided exactly.
+//
+// What bounds it is the chain of a row's steps, of 1000 to 5000 clocks each with their barriers (64 rows of 32000, k = 50:
+// load 2100, largest 1400, bound 1600, gather 3800, sort 2800, draw 5600), and for flat rows the 13 operations in 64 bits a logit
+// where the 32-bit sums leave doubt: 64 rows of 32000 take 10 us with k = 50, 12.5 with k = 50 and p = 0.95, 50 to 65 with
+// p = 0.9 or 0.98 alone, 27 with no filter at all.
 //
 // A row takes each step once, so that the time to fetch instructions counts: inlined into each other, the passes were 430 KB
 // of code, a third of all stalls waited for it (64 rows of 32000, k = 50: 15 us), hence functions that are called.
@@ -573,7 +578,7 @@ struct Sampler {
 
   // ---------------------------------------------------------------- candidates
   // `n` numbers of sh (at `from`) in descending order into sh.sorted: a bitonic sort, one or two numbers a thread,
-  // within a warp by shuffles. Written out: as a loop its branches took most of the time (128 numbers: 7000 clocks, now 1500).
+  // within a warp by shuffles. Written out: as a loop its branches took most of the time (128 numbers: 7000 clocks, now about 2700).
   template <bool TWO>
   static __device__ __noinline__ void sort_by(int n, uint32_t v0, uint32_t v1) {
     SampleShared& sh = shared();

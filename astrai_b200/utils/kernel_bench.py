@@ -1,6 +1,6 @@
 """Device-timed micro-benchmarks of the framework's kernels.
 
-    python -m astrai_b200.utils.kernel_bench [gemm [case]|gemm_shapes|swiglu_gemm|rope_gemm|elementwise|ns|attn|norm|skinny|sample|decode|prefill|all]
+    python -m astrai_b200.utils.kernel_bench [gemm [case]|gemm_shapes|swiglu_gemm|rope_gemm|elementwise|ns|attn|norm|logits|skinny|sample|decode|prefill|all]
     torchrun --nproc-per-node N -m astrai_b200.utils.kernel_bench allreduce|ep|tpgather|tprow
 
 Each case is timed with CUDA events on the launching stream after warm-up,
@@ -808,6 +808,34 @@ def bench_qk_norm():
                               "gbs": round(by / ms / 1e6, 1), "frac_of_copy": round(by / ms / 1e6 / hbm, 3), "peak_src": src}))
 
 
+def bench_logits():
+    """Operators on rows of logits: a teacher's largest, the distillation loss with and without its gradient, a token from a
+    given number; bytes: the logits once, and once more for their gradient."""
+    from astrai_b200.inference.sample import sample_given
+    from astrai_b200.ops.distill import distill_loss, top_logits
+
+    hbm, _, src = peaks()
+
+    def report(name, x, fn, copies=1, **more):
+        ms = time_flushed(fn)
+        by = copies * x.numel() * x.element_size()
+        print(json.dumps({"kernel": name, "rows": x.shape[0], "vocab": x.shape[1], **more, "ms": round(ms, 4),
+                          "gbs": round(by / ms / 1e6, 1), "frac_of_copy": round(by / ms / 1e6 / hbm, 3), "peak_src": src}))
+
+    for rows, V, k in ((8192, 32000, 64), (768, 131072, 128), (16, 32000, 16)):
+        x = (2 * torch.randn(rows, V, device="cuda")).to(torch.bfloat16)
+        teacher = top_logits((2 * torch.randn(rows, V, device="cuda")).to(torch.bfloat16), k)
+        report("top_logits", x, lambda: top_logits(x, k), k=k)
+        report("distill_loss", x, lambda: distill_loss(x, teacher), k=k)
+        leaf = x.detach().requires_grad_()
+        report("distill_loss fwd+bwd", x, lambda: torch.autograd.grad(distill_loss(leaf, teacher), leaf), 2, k=k)
+    for rows, V in ((64, 32000), (512, 131072)):
+        x, u = (2 * torch.randn(rows, V, device="cuda")).to(torch.bfloat16), torch.rand(rows, device="cuda")
+        for setting in (dict(top_k=50), dict(top_k=50, top_p=0.95), dict(top_p=0.9), dict(min_p=0.05), dict()):
+            given = {name: torch.full((rows,), value, device="cuda") for name, value in {"temperature": 1.0, **setting}.items()}
+            report("sample_given", x, lambda: sample_given(x, u, **given, return_logprobs=True), **setting)
+
+
 def bench_kv8():
     """8-bit paged KV cache: attention of one new token per row, an append of 512 tokens per row, read-back."""
     from astrai_b200.ops.kv8 import KV8, kv8_append, kv8_attention, kv8_gather
@@ -883,6 +911,8 @@ def main(argv=None):
         bench_norm()
     if which in ("qk_norm", "all"):
         bench_qk_norm()
+    if which in ("logits", "all"):
+        bench_logits()
     if which in ("kv8", "all"):
         bench_kv8()
     if which in ("attn", "all"):

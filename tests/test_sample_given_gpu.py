@@ -134,6 +134,14 @@ def test_ends_of_the_unit_interval():
                 assert int(end[r]) == ids[np.nonzero(w > 0)[0][-1]]
 
 
+@pytest.mark.parametrize("p", [0.9, 0.98, 0.999])
+def test_top_p_of_many_equal_logits(p):
+    """Few distinct logits, each the steps of several others apart: the bound may lie far from where their steps point."""
+    x, u = _logits(48, 60000, torch.bfloat16, 21)
+    _check((x.float() * 3).bfloat16(), u, p=p)
+    _check((x.float() * 3).round().bfloat16(), u, p=p)
+
+
 @pytest.mark.parametrize("V", [300, 5000, 40000])
 def test_ties(V):
     """Equal logits are kept or dropped together; all of a flat row is drawn from."""

@@ -119,6 +119,14 @@ def test_many_rows_same_each_time():
     _check(x, 64, 2.0, got=first)
 
 
+@pytest.mark.parametrize("rows,V,dtype", [(1500, 300, torch.bfloat16), (1300, 9001, torch.float16), (700, 33000, torch.bfloat16),
+                                          (400, 70000, torch.float32)])
+def test_more_rows_than_run_at_a_time(rows, V, dtype):
+    x = (torch.randn(rows, V, device="cuda") * 3).to(dtype)
+    x[rows // 2] = 1.0
+    _check(x, 33, 0.7)
+
+
 def test_captured_and_on_another_stream():
     from astrai_b200.ops.distill import top_logits
 
