@@ -545,18 +545,23 @@ void distill_launch(const DistillArgs& a, int vecs, int device, cudaStream_t s) 
   at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   at[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = at;
-  // as many clusters as run at once, each with rows of its own
-  int most = 0;
-  if (a.cluster > 1) {
-    cfg.numAttrs = 1;
-    if (cudaOccupancyMaxActiveClusters(&most, kernel, &cfg) != cudaSuccess) most = 0;
-  } else if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&most, kernel, NT + 32, smem) != cudaSuccess) {
-    most = 0;
-  } else {
-    most *= astrai_host::num_sms(device);
+  // as many clusters as run at once, each with rows of its own; asked again when the sizes change
+  static thread_local struct {
+    int device = -1, smem, cluster, most;
+  } fit;
+  if (fit.device != device || fit.smem != (int)smem || fit.cluster != a.cluster) {
+    int most = 0;
+    if (a.cluster > 1) {
+      cfg.numAttrs = 1;
+      if (cudaOccupancyMaxActiveClusters(&most, kernel, &cfg) != cudaSuccess) most = 0;
+    } else if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&most, kernel, NT + 32, smem) != cudaSuccess) {
+      most = 0;
+    } else {
+      most *= astrai_host::num_sms(device);
+    }
+    fit.device = device, fit.smem = (int)smem, fit.cluster = a.cluster, fit.most = std::max(most, 1);
   }
-  if (most < 1) most = 1;
-  cfg.gridDim = dim3((unsigned)(std::min(a.rows, most) * a.cluster));
+  cfg.gridDim = dim3((unsigned)(std::min(a.rows, fit.most) * a.cluster));
   cfg.numAttrs = 2;
   if (a.cluster == 1) cfg.attrs = at + 1, cfg.numAttrs = 1;
   note_launch();
