@@ -380,7 +380,7 @@ __global__ void __launch_bounds__(NT + 32) distill_kernel(const DistillArgs a, i
         told_phase ^= 1;
         const float* their = theirs[turn][lane < cs ? lane : 0];
         const float m = lane < cs ? their[0] : -INFINITY, m_on = lane < cs ? their[3] : -INFINITY;
-        if (most == -INFINITY) mo = ref_of(warp_max(m));  // none of its own: one that others have
+        mo = ref_of(warp_max(m));  // the row's: another part's sum may be any distance above this one's own largest
         const bool some = m != -INFINITY;
         out = warp_sum(some ? their[1] * exp2_fast((m - mo) * c) : 0.f);
         if constexpr (TWO) out1 = warp_sum(some ? their[2] * exp2_fast((m - mo) * LOG2E) : 0.f);
@@ -388,7 +388,8 @@ __global__ void __launch_bounds__(NT + 32) distill_kernel(const DistillArgs a, i
         const bool some_on = m_on != -INFINITY;
         on = warp_sum(some_on ? their[4] * exp2_fast((m_on - mj) * c) : 0.f);
         if constexpr (TWO) on1 = warp_sum(some_on ? their[5] * exp2_fast((m_on - mj) * LOG2E) : 0.f);
-        cross = warp_sum(lane < cs ? their[6] - (some_on ? their[7] * ((m_on - mj) * a.inv_tau) : 0.f) : 0.f);
+        // (m_on - mj may be out of range where this part gives the teacher's tokens no mass)
+        cross = warp_sum(lane < cs ? their[6] - (some_on && their[7] != 0.f ? their[7] * ((m_on - mj) * a.inv_tau) : 0.f) : 0.f);
       } else {
         mj = ref_of(mj);
       }

@@ -331,3 +331,42 @@ def test_refusals():
     big = torch.zeros(1, 300000, device="cuda")
     with pytest.raises(ValueError, match="too large"):
         distill_loss(big, TopLogits(ids[:1], values[:1], rest[:1]))
+
+
+# The largest distance in base-2 exponents that a weight is taken at is 126, beyond it the weight is zero. Where the exponent
+# comes from a subtraction and a product with a rounded factor, it is off by three roundings: 3 * 126 * ln 2 * 2^-24 + 2^-22 =
+# 1.59e-5 of a weight, and a sum of at most 100 terms one after another by 100 * 2^-24 = 6e-6 more: 2^-15 = 3.05e-5 still
+# covers both together.
+@pytest.mark.parametrize("V,dtype,parts", [(50000, torch.float32, 4), (131072, torch.bfloat16, 4), (40000, torch.bfloat16, 2)])
+@pytest.mark.parametrize("low", [-60.0, -100.0, -1e4, "least"])
+def test_parts_of_a_row_far_below_the_others(V, dtype, parts, low):
+    """Each part of a row in turn masked with a large finite number: all that one CTA of a cluster has."""
+    value = torch.finfo(dtype).min if low == "least" else low
+    x, ids, values, _, y = _inputs(4, V, 24, dtype, labels=True, seed=11)
+    size = V // parts
+    for r in range(4):
+        at = r % parts * size
+        masked = slice(max(at - 16, 0), min(at + size + 16, V))  # the parts end on a vector
+        other = (r + 1) % parts * size + 100
+        if low == "least":
+            x[r, masked] = value
+        else:
+            x[r, masked] += value
+        ids[r, :4] = torch.arange(4, device="cuda") + at     # of the teacher's tokens, some lie there
+        ids[r, 4:] = torch.arange(20, device="cuda") + other  # and some parts have none
+        if low == "least":
+            values[r, :4] = -math.inf  # with mass there the loss would be 1e38
+            y[r] = ids[r, 5] + 100 * (r % 2)
+    rest = torch.randn(4, device="cuda")
+    for tau, hard in ((1.0, 0.0), (2.0, 0.3), (0.5, 0.3), (1.0, 0.3)):
+        _check(x, ids, values, rest, tau, y, hard)
+        _check(x, ids, values, None, tau, y, hard)
+
+
+@pytest.mark.parametrize("high", [150.0, 1e4])
+def test_parts_of_a_row_far_above_the_others(high):
+    x, ids, values, rest, y = _inputs(8, 50000, 24, torch.float32, seed=12)
+    for r in range(8):
+        x[r, r * 6250: (r + 1) * 6250] += high
+    for tau in (1.0, 2.0):
+        _check(x, ids, values, rest, tau, y, 0.4)
