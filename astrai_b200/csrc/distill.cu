@@ -39,7 +39,7 @@ constexpr int DST_MAX_K = 1024;
 constexpr int DST_MAX_CLUSTER = 16;
 constexpr int DST_VECS = 4352;  // vectors of a row in one CTA: 68 KB, three CTAs on an SM
 constexpr int DST_MAX_SMEM = 224 * 1024;
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+constexpr float LOG2E = 1.4426950408889634f;
 
 struct DistillArgs {
   const void* x;
@@ -74,18 +74,21 @@ __device__ __forceinline__ float teacher_value(const DistillArgs& a, long long i
 // a finite reference for a maximum
 __device__ __forceinline__ float ref_of(float m) { return m == -INFINITY ? 0.f : m; }
 
-// The student's mass at one temperature: outside J and on J as sums of 2^((x - ref) c), joined. With d = (J's reference -
-// that outside) c and m = max(d, 0), `sum` is all of it relative to 2^m at the reference outside: neither part overflows.
+// The student's mass at one temperature: outside J and on J as sums of 2^((x - ref) c), joined. `gap` is J's reference less
+// that outside (-inf: nothing on J), c log2(e) over the temperature, `per` one over it. `sum` is all of it relative to the greater
+// reference, so that neither part overflows; logarithms relative to the lesser one add the distance in units of e. The
+// distance may be out of range (everything outside J masked with the type's lowest value): only what is at the lesser reference
+// is then infinitely far away.
 struct Mass {
-  float outside, d, m, sum;
-  __device__ Mass(float outside_, float on, float d_) : outside(outside_), d(d_), m(fmaxf(d_, 0.f)) {
-    sum = outside * exp2_fast(-m) + on * exp2_fast(d - m);
+  float outside, down, up, low, sum;  // exponents of J's reference and of that outside relative to the greater; the distance
+  __device__ Mass(float outside_, float on, float gap, float c, float per) : outside(outside_) {
+    down = fminf(gap * c, 0.f), up = fminf(-gap * c, 0.f), low = gap * per;
+    sum = outside * exp2_fast(up) + on * exp2_fast(down);
   }
-  __device__ float log2_all_over_outside() const { return m + log2f(sum) - log2f(outside); }  // -log2 q_0
-  __device__ float log2_rel_outside() const { return m + log2f(sum); }  // of all of it, relative to each reference
-  __device__ float log2_rel_on() const { return m - d + log2f(sum); }
-  __device__ float inv_rel_outside() const { return exp2_fast(-m) / sum; }  // 1 / all of it, relative to each reference
-  __device__ float inv_rel_on() const { return exp2_fast(d - m) / sum; }
+  __device__ float log_all_over_outside() const { return fmaxf(low, 0.f) + (logf(sum) - logf(outside)); }  // -ln q_0
+  __device__ float log_rel_on() const { return fmaxf(-low, 0.f) + logf(sum); }  // of all of it, relative to J's reference
+  __device__ float inv_rel_outside() const { return exp2_fast(up) / sum; }  // 1 / all of it, relative to each reference
+  __device__ float inv_rel_on() const { return exp2_fast(down) / sum; }
 };
 
 // One entry of the teacher in shared memory.
@@ -394,8 +397,9 @@ __global__ void __launch_bounds__(NT + 32) distill_kernel(const DistillArgs a, i
         mj = ref_of(mj);
       }
       if (out == 0.f) mo = mj;  // nothing outside J
-      const Mass z(out, on, on == 0.f ? -INFINITY : (mj - mo) * c);
-      const Mass z1(TWO ? out1 : out, TWO ? on1 : on, on == 0.f ? -INFINITY : (mj - mo) * (TWO ? LOG2E : c));
+      const float gap = on == 0.f ? -INFINITY : mj - mo;
+      const Mass z(out, on, gap, c, a.inv_tau);
+      const Mass z1(TWO ? out1 : out, TWO ? on1 : on, gap, TWO ? LOG2E : c, TWO ? 1.f : a.inv_tau);
       // the teacher's share outside J
       const float pr = rest == -INFINITY ? 0.f : exp2_fast((rest - mt) * LOG2E);
       const float mass = teach + pr, inv = mass != 0.f ? 1.f / mass : 0.f;
@@ -417,11 +421,12 @@ __global__ void __launch_bounds__(NT + 32) distill_kernel(const DistillArgs a, i
         float loss = 0.f;
         if (mass != 0.f) {
           const float logm = logf(mass);
-          if (teach != 0.f) loss = cross * inv + teach * inv * (z.log2_rel_on() * LN2 - logm);
-          if (p0 != 0.f) loss += p0 * ((rest - mt) - logm + z.log2_all_over_outside() * LN2);
+          if (teach != 0.f) loss = cross * inv + teach * inv * (z.log_rel_on() - logm);
+          if (p0 != 0.f) loss += p0 * ((rest - mt) - logm + z.log_all_over_outside());
           loss *= a.kl_loss;
         }
-        if (a.hard > 0.f) loss += a.hard * ((mo - LogitType<T>::one(vecs.row[y])) + z1.log2_rel_outside() * LN2);
+        // relative to the greater reference: the label lies there unless its logit is far below, so that nothing large cancels
+        if (a.hard > 0.f) loss += a.hard * (((gap > 0.f ? mj : mo) - LogitType<T>::one(vecs.row[y])) + logf(z1.sum));
         a.row_loss[row] = loss;
       }
     } else if constexpr (TRAIN) {

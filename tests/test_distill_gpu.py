@@ -370,3 +370,27 @@ def test_parts_of_a_row_far_above_the_others(high):
         x[r, r * 6250: (r + 1) * 6250] += high
     for tau in (1.0, 2.0):
         _check(x, ids, values, rest, tau, y, 0.4)
+
+
+@pytest.mark.parametrize("V,dtype", [(600, torch.float32), (9000, torch.bfloat16), (50000, torch.float32)])
+@pytest.mark.parametrize("low", [-1e3, -1e5, "least"])
+def test_all_others_far_below_the_teachers_tokens(V, dtype, low):
+    """Every token but the teacher's masked with a large finite number: the label's part is the difference of two logits near
+    each other, whatever lies between them and the others."""
+    x, ids, values, _, y = _inputs(3, V, 24, dtype, seed=13)
+    x = torch.full_like(x, torch.finfo(dtype).min if low == "least" else low).scatter_(1, ids.long(), values)
+    y[:] = ids[:, 3].long()
+    rest = torch.full((3,), -20.0, device="cuda")
+    rest[1] = -math.inf
+    for tau, hard in ((1.0, 0.0), (2.0, 0.3), (1.0, 0.5), (2.0, 1.0)):
+        _check(x, ids, values, rest, tau, y, hard)
+        _check(x, ids, values, None, tau, y, hard)
+
+
+@pytest.mark.parametrize("V,dtype", [(600, torch.float32), (9000, torch.bfloat16), (50000, torch.float32)])
+def test_teachers_tokens_far_below_all_others(V, dtype):
+    x, ids, values, rest, y = _inputs(3, V, 24, dtype, seed=14)
+    x.scatter_add_(1, ids.long(), torch.full(ids.shape, -1e5, device="cuda", dtype=dtype))
+    y[0] = ids[0, 3]
+    for tau, hard in ((1.0, 0.0), (2.0, 0.3), (1.0, 0.5)):
+        _check(x, ids, values, rest, tau, y, hard)
