@@ -559,12 +559,20 @@ struct Sampler {
     });
     return sum_of(n);
   }
-  // The lowest id of a number equal to `value`.
-  static __device__ __noinline__ uint32_t first_id(float value) {
+  // The largest number of a row with NaN (`tops` leave out the vectors that hold one); -inf where there is none.
+  static __device__ __noinline__ float largest_number() {
+    const SampleShared& sh = shared();
+    const Mine me(sh);
+    float most = -INFINITY;
+    for_vecs(sh, me, -INFINITY, [&](const uint4& u, int) { most = fmaxf(most, vec_max_number<T>(u)); });
+    return of_key(max_of(key_of(most)));
+  }
+  // The lowest id of a number equal to `value`, looked for where `tops` reach `from`.
+  static __device__ __noinline__ uint32_t first_id(float value, float from) {
     const SampleShared& sh = shared();
     const Mine me(sh);
     uint32_t first = 0;  // complement
-    for_vecs(sh, me, value, [&](const uint4& u, int i) {
+    for_vecs(sh, me, from, [&](const uint4& u, int i) {
       float x[E];
       vec_floats<T>(u, x);
 #pragma unroll
@@ -1027,14 +1035,14 @@ __global__ void __launch_bounds__(SG_THREADS, 2) sample_given_kernel(const Sampl
   if (t == 0) sh.max_x = of_key(max_key);
   __syncthreads();
   if (!(fabsf(of_key(max_key)) < INFINITY)) {  // a NaN, an infinity or nothing allowed: no distribution; the largest number
-    const float most = of_key(S::max_of(key_of(top)));  // -inf where there is none but NaN
-    const uint32_t id = S::first_id(most);
+    const float most = S::largest_number();
+    const uint32_t id = S::first_id(most, -INFINITY);
     if (t == 0) {
       *sh.token = id < (uint32_t)a.V ? id : 0;
       if (sh.logprob) *sh.logprob = __int_as_float(0x7FC00000);
     }
   } else if (greedy) {
-    const uint32_t id = S::first_id(of_key(max_key));
+    const uint32_t id = S::first_id(of_key(max_key), of_key(max_key));
     const double total = sh.logprob ? S::mass_32(-INFINITY) : 1.;
     if (t == 0) S::answer((int)id, of_key(max_key), total);
   } else {

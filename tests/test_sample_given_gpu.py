@@ -262,3 +262,35 @@ def test_refusals():
             sample_given(**{"logits": x, "uniform": u, **bad})
     assert sample_given(x[:0], u[:0]).shape == (0,)
     assert not sample_given(x.requires_grad_(), u, return_logprobs=True)[1].requires_grad
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("V", [5, 50, 3001, 40000, 70001])
+def test_largest_number_beside_a_nan(dtype, V):
+    """It may share a 16-byte vector with the NaN, at any place of the vector and of the row."""
+    from astrai_b200.inference.sample import sample_given
+
+    for off in (0, 3):
+        wide = torch.full((24, V + 11), math.inf, dtype=dtype, device="cuda")
+        x = wide[:, off: off + V]
+        x.copy_(torch.randn(24, V, device="cuda"))
+        want = []
+        for r in range(24):
+            best = (r * V // 24) if r % 2 else V - 1 - r * V // 48
+            x[r, best] = 9.0 if r % 3 else math.inf
+            x[r, best + 1 if best + 1 < V else best - 1] = math.nan
+            if r % 5 == 0:
+                x[r, max(best - 1, 0) if best + 1 < V else max(best - 2, 0)] = math.nan
+            row = x[r].float().nan_to_num(nan=-math.inf, posinf=math.inf, neginf=-math.inf)
+            want.append(int((row == row.max()).nonzero()[0]))
+        for s in (dict(), dict(temperature=0.0), dict(top_k=5), dict(top_p=0.5), dict(min_p=0.5)):
+            token, logprob = sample_given(x, torch.rand(24, device="cuda"), return_logprobs=True, **s)
+            assert token.tolist() == want and logprob.isnan().all()
+    # the rows of the CPU's test
+    x = torch.zeros(4, 5, device="cuda", dtype=dtype)
+    x[0] = -math.inf
+    x[1, 0], x[1, 3] = math.nan, 2.0
+    x[2] = math.nan
+    x[3, 2] = math.inf
+    token, logprob = sample_given(x, torch.rand(4, device="cuda"), return_logprobs=True)
+    assert token.tolist() == [0, 3, 0, 2] and logprob.isnan().all()
