@@ -889,8 +889,9 @@ struct Sampler {
     SampleShared& sh = shared();
     const int t = threadIdx.x, lane = t & 31, w = t / 32;
     const float max_x = sh.max_x;
-    // min-p as a bound on the key: the least whose weight reaches it, among the 32 around max + T ln m, or where that window
-    // lies above it (temperatures at which neighbours have the same weight) by a search.
+    // min-p as a bound on the key: the least whose weight reaches it, among the 32 around max + T ln m, or by a search where
+    // that window lies above it (temperatures at which neighbours have the same weight) or below it (next to zero, where 32
+    // keys are less apart than the weight's error of 2^-42).
     if (sh.use_m && w == 0) {
       const uint32_t max_key = key_of(max_x);
       const auto reaches = [&](uint32_t key) { return weight(of_key(key)) >= sh.m || key >= max_key; };
@@ -898,6 +899,7 @@ struct Sampler {
       const uint32_t ok = __ballot_sync(0xffffffff, reaches(low + lane));
       uint32_t key = ok ? min(low + __ffs(ok) - 1, max_key) : max_key;
       if (ok & 1) key = least_key(lane, kLowest, key, reaches);
+      if (!ok) key = least_key(lane, low + 32, max_key, reaches);
       if (lane == 0) sh.low = key;
     }
     const bool by_k = sh.use_k && sh.k <= SG_LIST_K;

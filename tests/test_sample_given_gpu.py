@@ -294,3 +294,31 @@ def test_largest_number_beside_a_nan(dtype, V):
     x[3, 2] = math.inf
     token, logprob = sample_given(x, torch.rand(4, device="cuda"), return_logprobs=True)
     assert token.tolist() == [0, 3, 0, 2] and logprob.isnan().all()
+
+
+@pytest.mark.parametrize("V", [2, 3000, 40000])
+def test_min_p_whose_bound_lies_next_to_zero(V):
+    """Logits near zero lie so close together that a search among the neighbours of max + T ln m alone may end below all that
+    reach it. Apart from the largest each row has one token 0.02 T above the bound and one as far below."""
+    top, t, m = [], [], []
+    for temperature in (1.0, 0.7, 1.3):
+        for share in (0.9, 0.5, 0.1, 0.02):
+            tr, mr = float(np.float32(temperature)), float(np.float32(share))
+            at = np.float32(-tr * math.log(mr))
+            for step in (-2, -1, 0, 1, 2):
+                value = at
+                for _ in range(abs(step)):
+                    value = np.nextafter(value, np.float32(math.inf if step > 0 else 0))
+                top.append(float(value)), t.append(tr), m.append(mr)
+    top.append(0.10536054521799088), t.append(1.0), m.append(float(np.float32(0.9)))
+    rows = len(top)
+    x = torch.full((rows, V), -30.0, device="cuda")
+    t, m = torch.tensor(t, device="cuda"), torch.tensor(m, device="cuda")
+    x[:, V - 1] = 0.02 * t
+    if V > 2:
+        x[:, V // 2] = -0.02 * t
+    x[:, 0] = torch.tensor(top, device="cuda")
+    for u in (0.001, 0.99):
+        u = torch.full((rows,), u, device="cuda")
+        for k, p in ((0, 1.0), (40, 1.0), (0, 0.9999), (V - 1, 1.0)):
+            _check(x, u, t, k, p, m)
