@@ -720,15 +720,14 @@ struct Sampler {
       double error;
       const double total = mass(precise, low, error), target = sh.draw * total;
       if (threadIdx.x == 0) sh.hit = kDone;
-      // The warp in whose part the target lies. Should rounding leave the target at the very end, the last one with any mass
-      // takes it.
+      // The warp in whose part the target lies: the first whose end in the running sum is above it. Should rounding leave the
+      // target at the very end, the last one with any mass takes it. All warps see the same sums, so that one takes it.
       const double theirs = lane < kWarps ? sh.warp_sum[lane] : 0., upto = lanes_before(theirs);
-      const double here = __shfl_sync(0xffffffff, theirs, w);
+      const uint32_t full = __ballot_sync(0xffffffff, theirs > 0.), ends = __ballot_sync(0xffffffff, theirs > 0. && upto > target);
       double before = __shfl_sync(0xffffffff, upto, max(w - 1, 0));
       if (w == 0) before = 0.;
-      const bool last = (__ballot_sync(0xffffffff, theirs > 0.) & ~(0xffffffffu >> (31 - w))) == 0;
       __syncthreads();
-      if (here > 0. && before <= target && (target < before + here || last)) {
+      if (w == (ends ? __ffs(ends) - 1 : 31 - __clz(full))) {
         int begin = 0, end = sh.chunk / 32;
         if (!HELD) {  // the group
           double run = before;

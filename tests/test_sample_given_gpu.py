@@ -322,3 +322,75 @@ def test_min_p_whose_bound_lies_next_to_zero(V):
         u = torch.full((rows,), u, device="cuda")
         for k, p in ((0, 1.0), (40, 1.0), (0, 0.9999), (V - 1, 1.0)):
             _check(x, u, t, k, p, m)
+
+
+def _running(v, n):
+    """Running sums of `n` numbers as a warp takes them by shuffles."""
+    v = v.copy()
+    o = 1
+    while o < n:
+        up = v[..., :-o].copy()
+        v[..., o:] += up
+        o *= 2
+    return v
+
+
+def _weights(steps, temperature):
+    """2^(t / 16) of logits -0, -1, .. in 64 bits as the kernel computes it, where t is next to a multiple of 16."""
+    from fractions import Fraction
+
+    a = 0.6931471805599453 / 16.0
+    terms = (a * a * a * a / 24.0, a * a * a / 6.0, a * a / 2.0, a, 1.0)
+    out = []
+    for n in range(steps):
+        t = -float(n) * (16.0 * 1.4426950408889634 / temperature)
+        whole = t + 6755399441055744.0 - 6755399441055744.0
+        assert whole == -16 * n
+        t, e = t - whole, a * a * a * a * a / 120.0
+        for term in terms:
+            e = float(Fraction(e) * Fraction(t) + Fraction(term))
+        out.append(e * 2.0 ** -n)
+    return np.array(out)
+
+
+def test_numbers_between_two_roundings_of_a_border():
+    """The sum up to a warp's end, taken by shuffles, and the sum before it and its own part may round differently. A number
+    that falls between the two belongs to one of the tokens at the border, and not to none."""
+    from astrai_b200.inference.sample import sample_given
+
+    V, temperature = 32000, float(np.float32(1.4426950408889634))
+    step = np.random.default_rng(0).integers(0, 12, (40, V))
+    x = torch.from_numpy(-step.astype(np.float32)).cuda().bfloat16()  # rows start on the 16-byte grid
+    weight = np.zeros((40, 16 * 256 * 8))
+    weight[:, :V] = _weights(12, temperature)[step]
+    weight = weight.reshape(40, 16, 8, 32, 8)  # warp, vector of a lane, lane, element
+    vec = (weight[..., 0] + weight[..., 1]) + (weight[..., 2] + weight[..., 3])
+    vec = vec + ((weight[..., 4] + weight[..., 5]) + (weight[..., 6] + weight[..., 7]))
+    lane = np.zeros((40, 16, 32))
+    for i in range(8):
+        lane += vec[:, :, i]
+    theirs = _running(lane, 32)[..., 31]
+    padded = np.zeros((40, 32))
+    padded[:, :16] = theirs
+    upto = _running(padded, 32)
+    rows, numbers, warps = [], [], []
+    for r in range(40):
+        total = upto[r, 31]
+        for w in range(1, 15):
+            if upto[r, w - 1] + theirs[r, w] < upto[r, w]:  # a number there is below neither's end, nor in the next warp's part
+                border = upto[r, w - 1] + theirs[r, w]
+                u = border / total
+                for near in (u, np.nextafter(u, 0), np.nextafter(u, 1)):
+                    if near * total == border:
+                        rows.append(r), numbers.append(near), warps.append(w)
+                        break
+    assert len(rows) >= 20
+    spoiled = torch.full((len(rows),), -7, device="cuda")
+    del spoiled  # memory that the result may get
+    token, logprob = sample_given(x[rows], torch.tensor(numbers, dtype=torch.float64, device="cuda"), temperature=temperature,
+                                  return_logprobs=True)
+    last = (torch.tensor(warps) + 1) * 2048 - 1
+    away = token.cpu() - last
+    assert ((away == 0) | (away == 1)).all(), away.tolist()
+    want = torch.log_softmax(x[rows].double() / temperature, -1).gather(1, token[:, None])[:, 0]
+    assert ((logprob - want).abs() <= 2.0 ** -18 + 2.0 ** -23 * want.abs()).all()
