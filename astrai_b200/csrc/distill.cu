@@ -155,7 +155,10 @@ __global__ void __launch_bounds__(NT + 32) distill_kernel(const DistillArgs a, i
   __shared__ Coefficients coefs;
   __shared__ float theirs[2][DST_MAX_CLUSTER][8];
   __shared__ int twice[2];
-  __shared__ uint64_t full, told;
+  // Two barriers in turn for the exchange of sums: one counts arrivals, not senders, and a CTA that is done with a row might
+  // arrive for the next one before another's arrival for this row has come. For the row after next it cannot: then it has seen
+  // that one's arrival for the next row, which follows the one for this.
+  __shared__ uint64_t full, told[2];
   const int t = threadIdx.x, lane = t & 31, w = t >> 5;
   const int cs = a.cluster, rank = cs > 1 ? (int)cg::this_cluster().block_rank() : 0;
   const int stride = gridDim.x / cs;
@@ -168,7 +171,8 @@ __global__ void __launch_bounds__(NT + 32) distill_kernel(const DistillArgs a, i
   if (t < 2) twice[t] = 0;
   if (t == 0) {
     mbar_init(&full, 2);  // the copy, and the cut vectors
-    mbar_init(&told, cs);
+    mbar_init(&told[0], cs);
+    mbar_init(&told[1], cs);
     fence_mbar_init();
   }
   if (cs > 1) cg::this_cluster().sync();
@@ -376,11 +380,11 @@ __global__ void __launch_bounds__(NT + 32) distill_kernel(const DistillArgs a, i
 #pragma unroll
           for (int i = 0; i < 8; ++i)
             asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 4 * i), "f"(mine[i]) : "memory");
-          asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote(&told, lane)) : "memory");
+          asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote(&told[turn], lane)) : "memory");
         }
         __syncwarp();
-        if (!wait_cluster(&told, told_phase, a.err)) return;  // (no copy follows: the others run out of time)
-        told_phase ^= 1;
+        if (!wait_cluster(&told[turn], told_phase >> turn & 1, a.err)) return;  // (no copy follows: the others run out of time)
+        told_phase ^= 1u << turn;
         const float* their = theirs[turn][lane < cs ? lane : 0];
         const float m = lane < cs ? their[0] : -INFINITY, m_on = lane < cs ? their[3] : -INFINITY;
         mo = ref_of(warp_max(m));  // the row's: another part's sum may be any distance above this one's own largest

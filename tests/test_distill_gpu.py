@@ -394,3 +394,22 @@ def test_teachers_tokens_far_below_all_others(V, dtype):
     y[0] = ids[0, 3]
     for tau, hard in ((1.0, 0.0), (2.0, 0.3), (1.0, 0.5)):
         _check(x, ids, values, rest, tau, y, hard)
+
+
+@pytest.mark.parametrize("rows,V,part", [(4096, 17500, 128), (256, 130000, 16)])
+def test_many_rows_in_turn_on_clusters(rows, V, part):
+    """Rows that follow each other on a cluster give what they give in calls in which each cluster has one."""
+    from astrai_b200.ops.distill import TopLogits, distill_loss
+
+    x, ids, values, rest, y = _inputs(rows, V, 2, torch.float32, seed=15)
+    y[::8] = -100  # as many in each part, so that the means' factors are the same numbers
+
+    def gradient(at, upstream):
+        leaf = x[at].detach().requires_grad_()
+        loss = distill_loss(leaf, TopLogits(ids[at], values[at], rest[at]), 1.0, y[at], expected_grad=upstream)
+        return torch.autograd.grad(loss, leaf, torch.full_like(loss, upstream))[0]
+
+    for _ in range(3):
+        together = gradient(slice(0, rows), 1.0)
+        for i in range(0, rows, part):
+            assert torch.equal(together[i: i + part], gradient(slice(i, i + part), part / rows))
