@@ -156,14 +156,25 @@ at::Tensor grad_like(const at::Tensor& x) {
   return new_like(x, {head + rows * ld}, x.scalar_type()).as_strided({rows, V}, {ld, 1}, head);
 }
 
+// The capture that the current stream is part of; 0: none.
+unsigned long long current_capture() {
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  unsigned long long id = 0;
+  C10_CUDA_CHECK(cudaStreamGetCaptureInfo(stream(), &status, &id));
+  return status == cudaStreamCaptureStatusActive ? id : 0;
+}
+
 // The forward pass leaves the gradient for an upstream gradient of `expected`; the backward hands it out after a launch
 // that does nothing on the device where that came true and computes the pass again where it did not. A second backward
-// through a retained graph computes it into new memory: the first one's belongs to its receiver.
+// through a retained graph computes it into new memory: the first one's belongs to its receiver. A backward that is not in the
+// forward's capture may run again where the forward does not, or before it: it takes neither the gradient nor the rows' number
+// from there.
 struct DistillLossBackward : public torch::autograd::Node {
   torch::autograd::SavedVariable x, ids, values, rest, target;
   at::Tensor count, ready;
   double tau = 1., hard = 0., expected = 1.;
   int64_t ignore = -100;
+  unsigned long long capture = 0;  // the forward's
   std::vector<int64_t> sizes;
   std::string name() const override { return "DistillLossBackward"; }
   void release_variables() override {
@@ -177,13 +188,14 @@ struct DistillLossBackward : public torch::autograd::Node {
     torch::autograd::variable_list out(1);
     if (!grads[0].defined()) return out;
     no_tangent(grads[0], "distill_loss's backward");
-    const Distill d{x.unpack(), ids.unpack(), values.unpack(), rest.unpack(), target.unpack(), count, tau, hard, ignore};
+    Distill d{x.unpack(), ids.unpack(), values.unpack(), rest.unpack(), target.unpack(), count, tau, hard, ignore};
     const c10::cuda::CUDAGuard guard(d.x.device());
     const at::Tensor g = grads[0].to(at::kFloat);
-    const bool given = ready.defined();
+    const bool same = capture == current_capture(), given = ready.defined() && same;
+    if (d.target.defined() && !same) d.count = new_like(d.x, {1}, at::kFloat);
     at::Tensor dx = given ? std::move(ready) : grad_like(d.x);
     ready = at::Tensor();
-    if (d.x.size(0) > 0) launch(d, dx, g.data_ptr<float>(), expected, given, {}, true, {});
+    if (d.x.size(0) > 0) launch(d, dx, g.data_ptr<float>(), expected, given, {}, same, {});
     out[0] = dx.view(sizes);
     return out;
   }
@@ -256,6 +268,7 @@ at::Tensor distill_loss(const at::Tensor& logits, const at::Tensor& ids_in, cons
     node->rest = {d.rest, false}, node->target = {d.target, false};
     node->count = d.count, node->ready = dx;
     node->tau = tau, node->hard = hard, node->expected = expected, node->ignore = ignore;
+    node->capture = current_capture();
     node->sizes = logits.sizes().vec();
     torch::autograd::set_history(loss, node);
   }

@@ -413,3 +413,36 @@ def test_many_rows_in_turn_on_clusters(rows, V, part):
         together = gradient(slice(0, rows), 1.0)
         for i in range(0, rows, part):
             assert torch.equal(together[i: i + part], gradient(slice(i, i + part), part / rows))
+
+
+def test_forward_and_backward_on_two_sides_of_a_capture():
+    """The gradient that the forward leaves belongs to its own run: a captured backward writes its gradient at every replay,
+    and an eager backward does not take what a captured forward has yet to write."""
+    from astrai_b200.ops.distill import TopLogits, distill_loss
+
+    x, ids, values, rest, y = _inputs(5, 5000, 9)
+    top = TopLogits(ids, values, rest)
+    base = x.detach().requires_grad_()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        logits = base * 1
+        one = torch.ones((), device="cuda")
+        loss = distill_loss(logits, top, 2.0, y, 0.5)
+        other = distill_loss(logits, top, 2.0, y, 0.5)
+        torch.autograd.grad(other, logits, one, retain_graph=True)
+        side.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            (dx,) = torch.autograd.grad(loss, logits, one, retain_graph=True)
+        for _ in range(2):
+            dx.zero_()
+            g.replay()
+            _check(x, ids, values, rest, 2.0, y, 0.5, got=(loss.detach(), dx))
+        later = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(later, stream=side):
+            captured = distill_loss(logits, top, 2.0, y, 0.5)
+        (dx,) = torch.autograd.grad(captured, logits, one)
+        later.replay()
+        _check(x, ids, values, rest, 2.0, y, 0.5, got=(captured.detach(), dx))
+    torch.cuda.current_stream().wait_stream(side)
