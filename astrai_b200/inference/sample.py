@@ -267,7 +267,9 @@ def _given_reference(x: Tensor, uniform: Tensor, temperature: Tensor, top_k: Ten
 
 def _setting(name: str, v: Scalar, low: float, high: float, device, dtype) -> Tensor:
     if isinstance(v, Tensor):
-        return v if v.device == device else v.to(device)
+        v = v if v.device == device else v.to(device)
+        # whole numbers are read as 32 bits: those beyond (off, as any from the vocabulary's size on) must not wrap
+        return v.clamp(0, 2 ** 31 - 1) if dtype == torch.int32 and v.dtype == torch.int64 else v
     if not low <= v <= high:
         raise ValueError(f"sample_given: {name} must be in [{low}, {high}], got {v}")
     return torch.full((1,), v, device=device, dtype=dtype)

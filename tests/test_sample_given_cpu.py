@@ -44,3 +44,12 @@ def test_refusals():
                 dict(uniform=u[:2]), dict(top_k=torch.zeros(2)), dict(logits=x[0])):
         with pytest.raises(ValueError):
             sample_given(**{"logits": x, "uniform": u, **bad})
+
+
+def test_top_k_beyond_32_bits_is_off():
+    g = torch.Generator().manual_seed(1)
+    x, u = torch.randn(8, 30, generator=g), torch.rand(8, generator=g)
+    off = sample_given(x, u)
+    for k in (2 ** 31 + 1, 2 ** 32 + 1, 2 ** 40 + 3, -1, -2 ** 32 + 1):
+        for n in (1, 8):
+            assert torch.equal(sample_given(x, u, top_k=torch.full((n,), k)), off)

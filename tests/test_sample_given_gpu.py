@@ -394,3 +394,13 @@ def test_numbers_between_two_roundings_of_a_border():
     assert ((away == 0) | (away == 1)).all(), away.tolist()
     want = torch.log_softmax(x[rows].double() / temperature, -1).gather(1, token[:, None])[:, 0]
     assert ((logprob - want).abs() <= 2.0 ** -18 + 2.0 ** -23 * want.abs()).all()
+
+
+def test_top_k_beyond_32_bits_is_off():
+    from astrai_b200.inference.sample import sample_given
+
+    x, u = _logits(16, 2000, torch.float32, 23)
+    off = sample_given(x, u)
+    for k in (2 ** 31 + 1, 2 ** 32 + 1, 2 ** 40 + 3, -1, -2 ** 32 + 1):
+        for n in (1, 16):
+            assert torch.equal(sample_given(x, u, top_k=torch.full((n,), k, device="cuda")), off)
