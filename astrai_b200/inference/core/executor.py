@@ -17,8 +17,9 @@ Differences, all on the device side:
   (rows whose frequency penalty is non-zero take the eager path, which also
   ships the history window);
 * rows with a seed of their own or min-p are drawn by ``sample_given`` from
-  numbers that the host sends, on the eager path; the other rows of the batch
-  keep the sampler that draws its own.
+  numbers that the host sends, after the replay of the graph, which leaves the
+  step's logits; the other rows of the batch keep the graph and the sampler
+  that draws its own.
 """
 
 from __future__ import annotations
@@ -45,6 +46,10 @@ def _bucket(n: int, cap: int) -> int:
     return cap
 
 
+def _rows(logits: torch.Tensor, rows: List[int]) -> torch.Tensor:
+    return logits if len(rows) == logits.shape[0] else logits[torch.tensor(rows, device=logits.device)]
+
+
 class _DecodeGraphs:
     """Static decode inputs + one captured graph per batch-size bucket."""
 
@@ -63,6 +68,7 @@ class _DecodeGraphs:
         self.out_tok = torch.zeros(B, dtype=torch.int64, device=dev)
         self.out_lp = torch.zeros(B, dtype=torch.float32, device=dev)
         self.graphs: Dict[int, torch.cuda.CUDAGraph] = {}
+        self.logits: Dict[int, torch.Tensor] = {}  # what a graph's last replay left, until the next of any graph
         self.pool = None
 
     def _views(self, b: int):
@@ -111,7 +117,9 @@ class _DecodeGraphs:
         view = PageCacheView(ex.kv_cache.storage, table, lens=lens, n_new=1, positions=pos32,
                              workspace=self.workspace(b), splits=self.splits(b))
         out = ex.model(ids, position_ids=pos, paged_cache=view, logits_to_keep=1)
-        fused_sample(out["logits"][:, -1], temp, topk, topp, pen, None, ex.rng, self.out_tok[:b], self.out_lp[:b])
+        logits = out["logits"][:, -1]
+        fused_sample(logits, temp, topk, topp, pen, None, ex.rng, self.out_tok[:b], self.out_lp[:b])
+        return logits
 
     def splits(self, b: int) -> int:
         from astrai_b200.ops._ext import native
@@ -137,12 +145,19 @@ class _DecodeGraphs:
             torch.cuda.current_stream(self.ex.device).wait_stream(s)
             g = torch.cuda.CUDAGraph()
             with torch.inference_mode(), torch.cuda.graph(g, pool=self.pool):
-                self._forward(b)
+                self.logits[b] = self._forward(b)
             self.pool = g.pool()
             self.graphs[b] = g
         g.replay()
         n = len(tasks)
-        return self.out_tok[:n].tolist(), self.out_lp[:n].tolist()
+        given = [i for i, t in enumerate(tasks) if t.given]
+        if not given:
+            return self.out_tok[:n].tolist(), self.out_lp[:n].tolist()
+        drawn = self.ex._sample_given(_rows(self.logits[b][:n], given), [tasks[i] for i in given])
+        toks, lps = self.out_tok[:n].tolist(), self.out_lp[:n].tolist()
+        for i, tok, lp in zip(given, *drawn):
+            toks[i], lps[i] = tok, lp
+        return toks, lps
 
 
 class Executor:
@@ -176,8 +191,7 @@ class Executor:
         for rows, draw in ((given, self._sample_given),
                            ([i for i, t in enumerate(tasks) if not t.given], self._sample_own)):
             if rows:
-                part = logits if len(rows) == len(tasks) else logits[torch.tensor(rows, device=logits.device)]
-                for i, tok, lp in zip(rows, *draw(part, [tasks[i] for i in rows])):
+                for i, tok, lp in zip(rows, *draw(_rows(logits, rows), [tasks[i] for i in rows])):
                     toks[i], lps[i] = tok, lp
         return toks, lps
 
@@ -243,7 +257,7 @@ class Executor:
         if not tasks:
             return []
         if self._graphs is not None and len(tasks) <= self._graphs.max_batch and not any(
-                t.frequency_penalty != 0.0 or t.given for t in tasks):
+                t.frequency_penalty != 0.0 for t in tasks):
             toks, lps = self._graphs.run(tasks)
             return self._append(tasks, toks, lps, return_logprobs)
         dev = self.device

@@ -105,14 +105,14 @@ class Task:
         self.top_k, self.rep_window = int(self.top_k), int(self.rep_window)
         self.frequency_penalty = float(self.frequency_penalty)
         self.min_p = float(self.min_p)
-        if self.given and self.frequency_penalty:
+        if (self.seed is not None or self.min_p > 0.0) and self.frequency_penalty:
             raise ValueError("min_p and seed do not go together with a frequency penalty")
 
     # ------------------------------------------------------------------ sampling
     @property
     def given(self) -> bool:
-        """Whether its tokens are drawn by ``sample_given`` (a seed of its own, or min-p)."""
-        return self.seed is not None or self.min_p > 0.0
+        """Whether its tokens are drawn by ``sample_given`` (a seed of its own, or min-p; at temperature 0 nothing is drawn)."""
+        return (self.seed is not None or self.min_p > 0.0) and self.temperature > 0.0
 
     def uniform(self) -> Optional[float]:
         """The number in [0, 1) that the next token is drawn from: a hash of the task's seed and the token's index

@@ -140,3 +140,12 @@ def test_server_takes_min_p_and_seed():
     assert sent(ChatCompletionRequest, min_p=0.1)["min_p"] == 0.1
     assert sent(MessagesRequest, min_p=0.1)["min_p"] == 0.1
     assert "seed" not in sent(ChatCompletionRequest, seed=4, frequency_penalty=0.5)
+
+
+def test_a_seed_at_temperature_0_draws_nothing():
+    from astrai_b200.inference.core.task import Task
+
+    assert not Task("a", [1], 4, temperature=0.0, seed=9).given and not Task("b", [1], 4, temperature=0.0, min_p=0.1).given
+    assert Task("c", [1], 4, temperature=0.5, seed=9).given and Task("d", [1], 4, temperature=0.5, min_p=0.1).given
+    with pytest.raises(ValueError, match="penalty"):
+        Task("e", [1], 4, temperature=0.0, seed=9, frequency_penalty=0.2)

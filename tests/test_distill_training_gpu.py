@@ -111,3 +111,31 @@ def test_engine_with_seeds():
         assert eng.generate("5 6 7 8", seed=11, **kw) == first
         greedy = eng.generate("5 6 7 8", max_tokens=6, temperature=0.0)
         assert eng.generate("5 6 7 8", max_tokens=6, temperature=1.0, top_k=0, min_p=1.0) == greedy
+
+
+def test_a_seeded_request_leaves_its_batch_on_the_decode_graph():
+    from astrai_b200.inference.core.scheduler import InferenceScheduler
+    from astrai_b200.inference.core.task import Task
+    from tests.test_inference_gpu import _Tok, _gpu_model
+
+    sch = InferenceScheduler(_gpu_model(), _Tok(), max_batch_size=4, max_seq_len=128, use_cuda_graph=True)
+    replays, graphs = [], sch._executor._graphs
+    run = graphs.run
+    graphs.run = lambda tasks: replays.append(len(tasks)) or run(tasks)
+
+    def generate(*settings):
+        replays.clear()
+        tasks = [Task(str(i), [5 + i, 6, 7 + i], 8, **{"top_k": 0, **s}) for i, s in enumerate(settings)]
+        sch._run_wave(tasks)
+        assert len(replays) == max(len(t.output_ids) for t in tasks) - 1
+        return [(t.output_ids, t.output_logprobs) for t in tasks]
+
+    greedy = dict(temperature=0.0)
+    alone = generate(greedy, greedy, greedy)
+    # min-p of one keeps the largest logit alone: drawn from this step's logits, or it would be another token
+    mixed = generate(greedy, dict(min_p=1.0, seed=4), greedy)
+    assert [ids for ids, _ in mixed] == [ids for ids, _ in alone] and mixed[0] == alone[0] and mixed[2] == alone[2]
+    seeded = generate(dict(seed=11), greedy, dict(seed=12, min_p=0.02))
+    assert seeded[1] == alone[1] and generate(dict(seed=11), greedy, dict(seed=12, min_p=0.02)) == seeded
+    assert generate(dict(temperature=0.0, seed=11), greedy, greedy) == alone
+    assert all(0 <= i < 2048 and lp <= 0.0 for ids, lps in seeded for i, lp in zip(ids, lps))
