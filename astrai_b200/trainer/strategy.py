@@ -22,7 +22,7 @@ concatenated chosen+rejected batch as the reference does.
 from __future__ import annotations
 
 from abc import ABC, abstractmethod
-from typing import Callable, Dict, Optional, Union
+from typing import Callable, Dict, Optional, Tuple, Union
 
 import torch
 import torch.nn as nn
@@ -178,7 +178,8 @@ class DistillStrategy(BaseStrategy):
     """A student learns a teacher's distribution over its top tokens and all others
     (:func:`astrai_b200.ops.distill.distill_loss`), and the labels with ``distill_hard_weight``.
 
-    The teacher is a frozen ``teacher_model`` with the student's vocabulary, or its rows come with the batch:
+    The teacher is a frozen ``teacher_model`` with the student's vocabulary (one whose logits are more is refused: its mass on
+    tokens that the student does not have would be lost without a word), or its rows come with the batch:
     ``teacher_ids`` and ``teacher_logits [B, S, k]`` and, if wanted, ``teacher_rest [B, S]``, the log-sum-exp of
     its other logits over the temperature. ``position_ids`` (packed documents) and ``loss_mask`` are used as by
     sft if the batch has them.
@@ -194,15 +195,17 @@ class DistillStrategy(BaseStrategy):
         self.temperature = distill_temperature
         self.hard_weight = distill_hard_weight
 
-    def _teacher(self, batch, inputs) -> TopLogits:
+    def _teacher(self, batch, inputs) -> Tuple[TopLogits, int]:
+        """The teacher's rows, and its vocabulary where it is known."""
         if "teacher_ids" in batch:
-            return TopLogits(batch["teacher_ids"], batch["teacher_logits"], batch.get("teacher_rest"))
+            return TopLogits(batch["teacher_ids"], batch["teacher_logits"], batch.get("teacher_rest")), 0
         if self.teacher_model is None:
             raise ValueError("distill needs a teacher_model (TrainConfig.teacher_fn), or batches with teacher_ids and "
                              "teacher_logits")
         with torch.no_grad():
             logits = self.teacher_model(**inputs)["logits"]
-            return top_logits(logits, min(self.top_k, logits.shape[-1]), self.temperature)
+            vocab = logits.shape[-1]
+            return top_logits(logits, min(self.top_k, vocab), self.temperature), vocab
 
     def compute_loss(self, batch):
         batch = move_to_device(batch, self.device)
@@ -212,8 +215,11 @@ class DistillStrategy(BaseStrategy):
         target = batch["target_ids"]
         if "loss_mask" in batch:
             target = target.masked_fill(~batch["loss_mask"].bool(), -100)
-        teacher = self._teacher(batch, inputs)
+        teacher, vocab = self._teacher(batch, inputs)
         out = self.model(**inputs)
+        if vocab > out["logits"].shape[-1]:
+            raise ValueError(f"distill: the teacher's vocabulary of {vocab} is larger than the student's of "
+                             f"{out['logits'].shape[-1]}")
         # the gradient that the trainer sends back, which divides the loss by the accumulation steps
         steps = getattr(self.executor, "grad_accum_steps", 1)
         loss = distill_loss(out["logits"], teacher, self.temperature, target, self.hard_weight, ignore_index=-100,

@@ -149,3 +149,21 @@ def test_a_seed_at_temperature_0_draws_nothing():
     assert Task("c", [1], 4, temperature=0.5, seed=9).given and Task("d", [1], 4, temperature=0.5, min_p=0.1).given
     with pytest.raises(ValueError, match="penalty"):
         Task("e", [1], 4, temperature=0.0, seed=9, frequency_penalty=0.2)
+
+
+def test_teacher_with_a_larger_vocabulary_is_refused():
+    from astrai_b200.config import AutoRegressiveLMConfig
+    from astrai_b200.models import AutoRegressiveLM
+    from astrai_b200.trainer.strategy import StrategyFactory
+
+    student = AutoRegressiveLM(AutoRegressiveLMConfig(**TINY_CFG))
+    ids = torch.randint(0, 400, (2, 9))
+    batch = {"input_ids": ids[:, :-1], "target_ids": ids[:, 1:]}
+    for more in (8, -8):
+        teacher = AutoRegressiveLM(AutoRegressiveLMConfig(**{**TINY_CFG, "vocab_size": TINY_CFG["vocab_size"] + more}))
+        strategy = StrategyFactory.create("distill", model=student, device="cpu", teacher_model=teacher)
+        if more > 0:
+            with pytest.raises(ValueError, match="vocabulary"):
+                strategy(batch)
+        else:
+            assert torch.isfinite(strategy(batch))
