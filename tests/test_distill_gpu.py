@@ -446,3 +446,14 @@ def test_forward_and_backward_on_two_sides_of_a_capture():
         later.replay()
         _check(x, ids, values, rest, 2.0, y, 0.5, got=(captured.detach(), dx))
     torch.cuda.current_stream().wait_stream(side)
+
+
+@pytest.mark.parametrize("V,dtype", [(139300, torch.float32), (278524, torch.float32), (278523, torch.float32),
+                                     (300001, torch.bfloat16), (557048, torch.float16), (557047, torch.bfloat16)])
+def test_longest_rows(V, dtype):
+    """Up to the largest vocabulary of each type, on the largest clusters."""
+    up = 64.0 if dtype == torch.float16 else 1.0
+    x, ids, values, rest, y = _inputs(2, V, 64, dtype, tau=2.0, seed=16)
+    y[0] = ids[0, 7]
+    _check(x, ids, values, rest, 2.0, y, 0.3, upstream=up, expected=up)
+    _check(x, ids, values, None, upstream=up, expected=1.0)

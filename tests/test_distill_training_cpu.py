@@ -167,3 +167,38 @@ def test_teacher_with_a_larger_vocabulary_is_refused():
                 strategy(batch)
         else:
             assert torch.isfinite(strategy(batch))
+
+
+def test_cli_trains_towards_a_saved_teacher(tmpdir_path):
+    """The command's own configuration, on sft data, builds the saved teacher and runs steps towards it."""
+    import os
+
+    from astrai_b200.cli.train import build_config, parse_args
+    from astrai_b200.serialization import save_bin
+    from astrai_b200.trainer import Trainer
+
+    student, there, data = (os.path.join(tmpdir_path, n) for n in ("student", "teacher", "data"))
+    teacher = _teacher()
+    teacher.save_pretrained(there)
+    teacher.save_pretrained(student)
+    g = torch.Generator().manual_seed(0)
+    save_bin(data, {"sequence": [torch.randint(0, 512, (200,), generator=g) for _ in range(2)],
+                    "loss_mask": [torch.randint(0, 2, (200,), generator=g) for _ in range(2)],
+                    "position_ids": [torch.arange(200) % 50 for _ in range(2)]})
+    cfg = build_config(parse_args([
+        "--train_type", "distill", "--teacher_path", there, "--param_path", student, "--data_root_path", data,
+        "--window_size", "32", "--batch_per_device", "2", "--grad_accum_steps", "1", "--n_epoch", "1", "--ckpt_dir",
+        os.path.join(tmpdir_path, "ckpt"), "--device_type", "cpu", "--backend", "gloo", "--num_workers", "0",
+        "--distill_top_k", "9", "--distill_temperature", "2.0", "--distill_hard_weight", "0.25"]))
+    built = cfg.teacher_fn()
+    assert all(p.dtype == torch.bfloat16 and torch.equal(p, q.bfloat16()) for p, q in zip(built.parameters(), teacher.parameters()))
+    assert {k: v for k, v in cfg.extra_kwargs.items() if k.startswith("distill")} == {
+        "distill_top_k": 9, "distill_temperature": 2.0, "distill_hard_weight": 0.25}
+    batch = torch.utils.data.default_collate([cfg.dataset[i] for i in range(2)])
+    assert batch["input_ids"].shape == (2, 32) and "loss_mask" in batch and "position_ids" in batch
+    t = Trainer(cfg)
+    t.train()
+    ctx = t.last_context
+    assert math.isfinite(ctx.loss) and ctx.optimizer_step > 0
+    assert (ctx.strategy.top_k, ctx.strategy.temperature, ctx.strategy.hard_weight) == (9, 2.0, 0.25)
+    assert not ctx.strategy.teacher_model.training

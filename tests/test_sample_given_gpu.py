@@ -404,3 +404,28 @@ def test_top_k_beyond_32_bits_is_off():
     for k in (2 ** 31 + 1, 2 ** 32 + 1, 2 ** 40 + 3, -1, -2 ** 32 + 1):
         for n in (1, 16):
             assert torch.equal(sample_given(x, u, top_k=torch.full((n,), k, device="cuda")), off)
+
+
+def test_numbers_beyond_the_unit_interval_count_as_its_ends():
+    from astrai_b200.inference.sample import sample_given
+
+    for V in (5, 3000, 70000):
+        x, _ = _logits(8, V, torch.bfloat16, 25)
+        for s in (dict(), dict(top_k=30), dict(top_p=0.8), dict(min_p=0.05)):
+            first, last = (sample_given(x, torch.full((8,), v, device="cuda", dtype=torch.float64), **s) for v in (0.0, 1.0))
+            for v, same in ((-3.0, first), (-math.inf, first), (math.nan, first), (7.0, last), (math.inf, last)):
+                for kind in (torch.float32, torch.float64):
+                    assert torch.equal(sample_given(x, torch.full((8,), v, device="cuda", dtype=kind), **s), same)
+
+
+@pytest.mark.parametrize("V,dtype", [(2 ** 22, torch.bfloat16), (2 ** 22 - 3, torch.float32)])
+def test_largest_vocabulary(V, dtype):
+    from astrai_b200.inference.sample import sample_given
+
+    x, u = _logits(2, V, dtype, 27, sigma=2.0)
+    x[:, -1] = 12.0  # the last id among the candidates
+    for s in (dict(), dict(k=200), dict(k=5000), dict(m=0.01), dict(p=0.5) if dtype == torch.bfloat16 else dict(k=50, p=0.9)):
+        _check(x, u, **s)
+    _check(x, torch.full((2,), 1.0, device="cuda"), k=40)
+    with pytest.raises(ValueError, match="vocabulary"):
+        sample_given(torch.zeros(1, 2 ** 22 + 1, device="cuda"), u[:1])

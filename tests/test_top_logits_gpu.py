@@ -175,3 +175,12 @@ def test_with_the_loss():
         # equal distributions: zero but for the arithmetic, logarithms of up to 20 within 2^-15
         assert abs(float(loss.detach())) <= tau ** 2 * 2.0 ** -15 * 40
         assert dx.abs().max() <= tau / 9 * 2.0 ** -14
+
+
+@pytest.mark.parametrize("rows,V,dtype", [(700, 4096, torch.bfloat16), (700, 8001, torch.float32), (1300, 32000, torch.float16)])
+def test_largest_k_of_many_rows(rows, V, dtype):
+    """The bound from a small CTA's 256 numbers lets more candidates through than their list holds."""
+    g = torch.Generator("cuda").manual_seed(V)
+    x = (torch.randn(rows, V, generator=g, device="cuda") * 3).to(dtype)
+    for k in (240, 250, 256):
+        _check(x, k, 0.7)
