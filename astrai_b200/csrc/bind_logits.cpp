@@ -18,7 +18,7 @@ int distill_max_k();
 int distill_max_vocab(int elem);
 void distill(const void* x, long long ldx, void* dx, long long lddx, const void* ids, bool ids64, const void* values,
              int values_type, const float* rest, const long long* target, long long ignore, int rows, int V, int K,
-             float tau, float hard, const float* grad, float expected, bool unless_expected, float* row_loss,
+             double tau, double hard, const float* grad, float expected, bool unless_expected, float* row_loss,
              float* count, bool have_count, float* loss, int dtype, int device, cudaStream_t s);
 int top_logits_max_k();
 void top_logits(const void* x, long long ldx, int rows, int V, int k, float tau, int* ids, void* values, float* rest,
@@ -141,7 +141,7 @@ void launch(const Distill& d, const at::Tensor& dx, const float* grad, double ex
                        dx.defined() ? row_stride(dx) : 0, d.ids.data_ptr(), d.ids.scalar_type() == at::kLong,
                        d.values.data_ptr(), dtype_code(d.values, "distill_loss: the teacher's values"), f32(d.rest),
                        d.target.defined() ? (const long long*)d.target.data_ptr<int64_t>() : nullptr, d.ignore,
-                       (int)d.x.size(0), (int)d.x.size(1), (int)d.ids.size(1), (float)d.tau, (float)d.hard, grad,
+                       (int)d.x.size(0), (int)d.x.size(1), (int)d.ids.size(1), d.tau, d.hard, grad,
                        (float)expected, unless_expected, f32(row_loss), f32(d.count), have_count, f32(loss),
                        dtype_code(d.x, "distill_loss: logits"), d.x.get_device(), stream());
   C10_CUDA_KERNEL_LAUNCH_CHECK();

@@ -54,7 +54,9 @@ struct DistillArgs {
   const long long* target;  // [rows] or null
   long long ignore;
   int rows, V, K, cluster;
-  float inv_tau, kl_loss, kl_grad, hard;  // 1 / tau, (1 - h) tau^2, (1 - h) tau, h
+  float inv_tau, inv_tau_rest;       // 1 / tau, and what its rounding left out
+  float c, kl_loss, kl_grad, hard;   // log2(e) / tau, (1 - h) tau^2, (1 - h) tau, h
+  int two;                           // the labels' part has a temperature of its own
   const float* count;     // rows that count, null: all
   const float* grad;      // gradient of the loss, null: `expected`
   float expected;
@@ -75,26 +77,23 @@ __device__ __forceinline__ float teacher_value(const DistillArgs& a, long long i
 __device__ __forceinline__ float ref_of(float m) { return m == -INFINITY ? 0.f : m; }
 
 // The student's mass at one temperature: outside J and on J as sums of 2^((x - ref) c), joined. `gap` is J's reference less
-// that outside (-inf: nothing on J), c log2(e) over the temperature, `per` one over it. `sum` is all of it relative to the greater
-// reference, so that neither part overflows; logarithms relative to the lesser one add the distance in units of e. The
-// distance may be out of range (everything outside J masked with the type's lowest value): only what is at the lesser reference
-// is then infinitely far away.
+// that outside (-inf: nothing on J). `sum` is all of it relative to the greater reference, so that neither part overflows.
 struct Mass {
-  float outside, down, up, low, sum;  // exponents of J's reference and of that outside relative to the greater; the distance
-  __device__ Mass(float outside_, float on, float gap, float c, float per) : outside(outside_) {
-    down = fminf(gap * c, 0.f), up = fminf(-gap * c, 0.f), low = gap * per;
-    sum = outside * exp2_fast(up) + on * exp2_fast(down);
+  float up, down;  // a weight of one at the reference outside J, and at J's, relative to the greater
+  float sum;
+  __device__ Mass(float outside, float on, float gap, float c) {
+    up = exp2_fast(fminf(-gap * c, 0.f));
+    down = exp2_fast(fminf(gap * c, 0.f));
+    sum = outside * up + on * down;
   }
-  __device__ float log_all_over_outside() const { return fmaxf(low, 0.f) + (logf(sum) - logf(outside)); }  // -ln q_0
-  __device__ float log_rel_on() const { return fmaxf(-low, 0.f) + logf(sum); }  // of all of it, relative to J's reference
-  __device__ float inv_rel_outside() const { return exp2_fast(up) / sum; }  // 1 / all of it, relative to each reference
-  __device__ float inv_rel_on() const { return exp2_fast(down) / sum; }
+  __device__ float inv_rel_outside() const { return up / sum; }  // 1 / all of it, relative to each reference
+  __device__ float inv_rel_on() const { return down / sum; }
 };
 
 // One entry of the teacher in shared memory.
 struct Entry {
   int id;       // -1: none
-  float value;  // over tau; then its mass
+  float value;  // the teacher's logit; then its mass
   float x;      // the student's logit, in this CTA's part of the row
   int here;     // it lies there
 };
@@ -142,8 +141,9 @@ __device__ __forceinline__ void each_vec(int n, F f) {
   for (; v < n; v += NT) f(v);
 }
 
+// (3: 72 registers; left to itself the compiler takes 56 for some types, and spills: 245 us for 8192 rows of 32000 instead of 236)
 template <typename T, int NT, bool TRAIN, bool TWO>
-__global__ void __launch_bounds__(NT + 32) distill_kernel(const DistillArgs a, int held) {
+__global__ void __launch_bounds__(NT + 32, NT == 256 && TRAIN ? 3 : 0) distill_kernel(const DistillArgs a, int held) {
   constexpr int E = LogitType<T>::E, W = NT / 32;
   using Bits = typename std::conditional<E == 4, uint32_t, uint16_t>::type;
   extern __shared__ __align__(128) unsigned char distill_smem[];  // the row's vectors, then the entries
@@ -179,7 +179,7 @@ __global__ void __launch_bounds__(NT + 32) distill_kernel(const DistillArgs a, i
   else __syncthreads();
 
   const bool extra = w == W;
-  const float c = a.inv_tau * LOG2E;
+  const float c = a.c;
   const float scale = TRAIN ? g / (a.count ? fmaxf(*a.count, 1.f) : (float)max(a.rows, 1)) : 0.f;
   const auto row_vecs = [&](int row) { return RowVecs<T>(static_cast<const T*>(a.x) + (long long)row * a.ldx, a.V); };
   // The extra warp: the whole vectors of this CTA's part of a row by the copy, a cut first or last one by element; finish()
@@ -221,7 +221,7 @@ __global__ void __launch_bounds__(NT + 32) distill_kernel(const DistillArgs a, i
       const RowVecs<T> v = row_vecs(row);
       const int per = (v.n + cs - 1) / cs, v0 = rank * per, v1 = min(v0 + per, v.n), at = ((int)j + v.head) / E;
       n.id = (int)j;
-      n.value = value * a.inv_tau;
+      n.value = value;
       n.here = at >= v0 && at < v1;
     }
     return n;
@@ -305,9 +305,10 @@ __global__ void __launch_bounds__(NT + 32) distill_kernel(const DistillArgs a, i
     __syncthreads();
 
     // ---- the extra warp: the sums over J
-    // the teacher's mass on J; of it that with a logit here; the sum of mass * (log p - log q) up to constants, the first part
-    // with the cluster's first CTA, the second with each one's own; the student's sums here, over tau and at 1
-    float rest = -INFINITY, mt = -INFINITY, mj = -INFINITY, teach = 0.f, own = 0.f, cross = 0.f, on = 0.f, on1 = 0.f;
+    // the teacher's largest logit and its mass on J relative to that; of it that with a logit here; the sum of mass * (the
+    // teacher's logit - the student's), each relative to its largest (in this CTA): one small number a token, as both logarithms'
+    // sums would be far larger than their difference; the student's sums here, over tau and at 1
+    float rest = -INFINITY, vt = -INFINITY, mj = -INFINITY, teach = 0.f, cross = 0.f, own = 0.f, on = 0.f, on1 = 0.f;
     bool label = false;  // it is one of the entries
     if (extra) {
       if (a.rest) rest = a.rest[row];
@@ -315,28 +316,27 @@ __global__ void __launch_bounds__(NT + 32) distill_kernel(const DistillArgs a, i
       for (int k = lane; k < a.K; k += 32) {
         const Entry n = entries[k];
         if (repeated && n.here) entries[k].x = LogitType<T>::one(vecs.row[n.id]);  // another's number may have been read
-        mt = fmaxf(mt, n.value);
+        vt = fmaxf(vt, n.value);
         mj = fmaxf(mj, n.here ? entries[k].x : -INFINITY);
         label |= n.id >= 0 && n.id == y;
       }
       label = __any_sync(0xffffffff, label);
-      mt = ref_of(fmaxf(of_key(__reduce_max_sync(0xffffffff, key_of(mt))), rest));
+      vt = of_key(__reduce_max_sync(0xffffffff, key_of(vt)));
       mj = of_key(__reduce_max_sync(0xffffffff, key_of(mj)));
-      const float ref = ref_of(mj);
+      const float vref = ref_of(vt), ref = ref_of(mj);
 #pragma unroll 2
       for (int k = lane; k < a.K; k += 32) {
         const Entry n = entries[k];
-        const float th = n.value - mt, zh = (n.x - ref) * a.inv_tau, e = n.id >= 0 ? exp2_fast(th * LOG2E) : 0.f;
+        const float th = n.value - vref, zh = n.x - ref, e = n.id >= 0 ? exp2_fast(th * c) : 0.f;
         entries[k].value = e;
         teach += e;
-        if (e != 0.f && rank == 0) cross += e * th;
         if (!n.here) continue;
-        if (e != 0.f) cross -= e * zh, own += e;
+        if (e != 0.f) cross += e * (th - zh), own += e;
         bool first = true;  // the student's mass at an id that comes again counts once, with the first of its entries
         for (int l = 0; repeated && first && l < k; ++l) first = entries[l].id != n.id;
         if (first) {
-          on += exp2_fast(zh * LOG2E);
-          if constexpr (TWO) on1 += exp2_fast((n.x - ref) * LOG2E);
+          on += exp2_fast(zh * c);
+          if constexpr (TWO) on1 += exp2_fast(zh * LOG2E);
         }
       }
       teach = warp_sum(teach);
@@ -396,18 +396,19 @@ __global__ void __launch_bounds__(NT + 32) distill_kernel(const DistillArgs a, i
         on = warp_sum(some_on ? their[4] * exp2_fast((m_on - mj) * c) : 0.f);
         if constexpr (TWO) on1 = warp_sum(some_on ? their[5] * exp2_fast((m_on - mj) * LOG2E) : 0.f);
         // (m_on - mj may be out of range where this part gives the teacher's tokens no mass)
-        cross = warp_sum(lane < cs ? their[6] - (some_on && their[7] != 0.f ? their[7] * ((m_on - mj) * a.inv_tau) : 0.f) : 0.f);
+        cross = warp_sum(lane < cs ? their[6] - (some_on && their[7] != 0.f ? their[7] * (m_on - mj) : 0.f) : 0.f);
       } else {
         mj = ref_of(mj);
       }
       if (out == 0.f) mo = mj;  // nothing outside J
       const float gap = on == 0.f ? -INFINITY : mj - mo;
-      const Mass z(out, on, gap, c, a.inv_tau);
-      const Mass z1(TWO ? out1 : out, TWO ? on1 : on, gap, TWO ? LOG2E : c, TWO ? 1.f : a.inv_tau);
-      // the teacher's share outside J
-      const float pr = rest == -INFINITY ? 0.f : exp2_fast((rest - mt) * LOG2E);
-      const float mass = teach + pr, inv = mass != 0.f ? 1.f / mass : 0.f;
-      const float p0 = pr * inv;
+      const Mass z(out, on, gap, c);
+      const Mass z1 = TWO ? Mass(out1, on1, gap, LOG2E) : z;
+      // the teacher's share outside J: its logarithm over the largest entry's, and the masses relative to the greater of both
+      const float over = vt == -INFINITY ? rest == -INFINITY ? -INFINITY : rest - rest
+                                         : fmaf(-vt, a.inv_tau_rest, fmaf(-vt, a.inv_tau, rest));
+      const float top = fmaxf(over, 0.f), pr = exp2_fast((over - top) * LOG2E), shrink = exp2_fast(-top * LOG2E);
+      const float mass = teach * shrink + pr, inv = mass != 0.f ? 1.f / mass : 0.f, p0 = pr * inv;
       if constexpr (TRAIN) {
         const float all = mass != 0.f ? 1.f : 0.f, kl = scale * a.kl_grad, ce = scale * a.hard;
         const float share = out != 0.f ? p0 / out : 0.f;
@@ -415,23 +416,38 @@ __global__ void __launch_bounds__(NT + 32) distill_kernel(const DistillArgs a, i
           coefs.ref = mo;
           coefs.base = kl * (all * z.inv_rel_outside() - share) + (TWO ? 0.f : ce * z.inv_rel_outside());
           coefs.base1 = TWO ? ce * z1.inv_rel_outside() : 0.f;
-          coefs.kl = kl, coefs.ce = ce, coefs.inv = inv, coefs.all = all;
+          coefs.kl = kl, coefs.ce = ce, coefs.inv = inv * shrink, coefs.all = all;
           coefs.mj = mj, coefs.inv_on = z.inv_rel_on(), coefs.inv_on1 = TWO ? z1.inv_rel_on() : z.inv_rel_on();
         }
         __syncthreads();
       }
-      if (a.row_loss && rank == 0 && lane == 0) {
-        // sum_k p_k (log p_k - log q_jk) = (sum e_k (th - zh)) / mass + (sum of p_k) (log of q's sum - log mass)
-        float loss = 0.f;
-        if (mass != 0.f) {
-          const float logm = logf(mass);
-          if (teach != 0.f) loss = cross * inv + teach * inv * (z.log_rel_on() - logm);
-          if (p0 != 0.f) loss += p0 * ((rest - mt) - logm + z.log_all_over_outside());
-          loss *= a.kl_loss;
+      if (a.row_loss && rank == 0) {
+        // The divergence may be far smaller than the logarithms of the masses. Of the largest of J (lane 0) and of the share
+        // outside (lane 1) it takes the logarithm of the teacher's probability over the student's, from masses joined in 64 bits.
+        // What the factors up, down, shrink and pr are off by is then in both distributions' sums too, and counts only as much
+        // as the two differ.
+        const bool o = lane == 1;
+        const float part = o ? pr : teach * shrink, apart = gap * a.inv_tau;
+        const double sum = (double)out * z.up + (double)on * z.down, of_teacher = (double)teach * shrink + pr;
+        const double den = of_teacher * (o ? (double)z.up * out : (double)z.down);
+        float ln, more = 0.f;
+        if (fminf(o ? z.up : z.down, o ? pr : shrink) > 1e-30f && den > 0.) {
+          double per = __fdividef(1.f, (float)den);
+          per *= 2. - den * per;
+          const double ratio = sum * (o ? pr : shrink) * per;
+          const float near = (float)ratio;
+          ln = logf(near);
+          more = __fdividef((float)(ratio - near), near);
+        } else {  // far from each other, or nothing there
+          ln = (o ? over - top + fmaxf(apart, 0.f) - logf(out) : fmaxf(-apart, 0.f) - top) + logf(z.sum / mass);
         }
+        const float term = part != 0.f ? part * ln : 0.f, add = part != 0.f ? part * more : 0.f;
+        const float crossed = shrink != 0.f ? cross * shrink * a.inv_tau : 0.f;
+        const float terms = term + __shfl_sync(0xffffffff, term, 1) + crossed + (add + __shfl_sync(0xffffffff, add, 1));
+        float loss = mass != 0.f ? terms * inv * a.kl_loss : 0.f;
         // relative to the greater reference: the label lies there unless its logit is far below, so that nothing large cancels
-        if (a.hard > 0.f) loss += a.hard * (((gap > 0.f ? mj : mo) - LogitType<T>::one(vecs.row[y])) + logf(z1.sum));
-        a.row_loss[row] = loss;
+        if (a.hard > 0.f && lane == 0) loss += a.hard * (((gap > 0.f ? mj : mo) - LogitType<T>::one(vecs.row[y])) + logf(z1.sum));
+        if (lane == 0) a.row_loss[row] = loss;
       }
     } else if constexpr (TRAIN) {
       __syncthreads();
@@ -592,7 +608,7 @@ void distill_sized(DistillArgs a, int device, cudaStream_t s) {
 
 template <typename T>
 void distill_typed(const DistillArgs& a, int device, cudaStream_t s) {
-  const bool two = a.hard > 0.f && a.inv_tau != 1.f;
+  const bool two = a.two;
   if (a.dx)
     two ? distill_sized<T, true, true>(a, device, s) : distill_sized<T, true, false>(a, device, s);
   else
@@ -610,12 +626,14 @@ int distill_max_vocab(int elem) { return DST_MAX_CLUSTER * DST_VECS * (16 / elem
 
 void distill(const void* x, long long ldx, void* dx, long long lddx, const void* ids, bool ids64, const void* values,
              int values_type, const float* rest, const long long* target, long long ignore, int rows, int V, int K,
-             float tau, float hard, const float* grad, float expected, bool unless_expected, float* row_loss,
+             double tau, double hard, const float* grad, float expected, bool unless_expected, float* row_loss,
              float* count, bool have_count, float* loss, int dtype, int device, cudaStream_t s) {
   if (target && !have_count)
     launch_early(distill_count_kernel, dim3(1), dim3(1024), 0, s, target, ignore, rows, V, count);
-  DistillArgs a{x, ldx, dx, lddx, ids, ids64, values, values_type, rest, target, ignore, rows, V, K, 1, 1.f / tau,
-                (1.f - hard) * tau * tau, (1.f - hard) * tau, hard, target ? count : nullptr, grad, expected,
+  const double per = std::min(1. / tau, 1e38), soft = 1. - hard;
+  DistillArgs a{x, ldx, dx, lddx, ids, ids64, values, values_type, rest, target, ignore, rows, V, K, 1, (float)per,
+                (float)(per - (float)per), (float)std::min(1.4426950408889634 * per, 1e38), (float)(soft * tau * tau),
+                (float)(soft * tau), (float)hard, hard > 0. && tau != 1., target ? count : nullptr, grad, expected,
                 unless_expected, row_loss, astrai_host::error_word(device)};
   if (rows > 0) {
     if (dtype == 0) distill_typed<__nv_bfloat16>(a, device, s);

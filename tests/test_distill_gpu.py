@@ -457,3 +457,32 @@ def test_longest_rows(V, dtype):
     y[0] = ids[0, 7]
     _check(x, ids, values, rest, 2.0, y, 0.3, upstream=up, expected=up)
     _check(x, ids, values, None, upstream=up, expected=1.0)
+
+
+@pytest.mark.parametrize("tau", [1.0, 1.3, 2.0])
+@pytest.mark.parametrize("V,dtype", [(1000, torch.float32), (33000, torch.bfloat16), (50000, torch.float32)])
+def test_a_small_divergence_keeps_its_digits(V, dtype, tau):
+    """One token of the teacher and the rest, within 1e-3 of the student's: a divergence of 1e-7 between logarithms of up to 12.
+
+    The token's own weights are one exactly. The sum outside is off by at most 2^-15 of itself, the factors between the two
+    masses by less; being in both distributions' sums, that counts as |p_0 - q_0| of it. The logarithms of the two ratios
+    and what they are multiplied by are fp32: 2^-22 of them."""
+    from astrai_b200.ops.distill import TopLogits, distill_loss
+
+    g = torch.Generator().manual_seed(V)
+    for i in range(24):
+        x = (3 * torch.randn(1, V, generator=g)).to(dtype)
+        j = int(x.argmax()) if i % 2 else int(torch.randint(V, (1,), generator=g))
+        if i % 3 == 0:
+            x[0, j] = 9.0 + i / 8
+        z = x[0].double() / tau
+        q = torch.softmax(z, -1)
+        q0 = float(1 - q[j]) if q[j] < 0.5 else float(torch.cat([q[:j], q[j + 1:]]).sum())
+        rest = (torch.cat([z[:j], z[j + 1:]]).logsumexp(0) + 1e-3 * torch.randn((), generator=g)).float()
+        value = x[:, j: j + 1].clone()
+        log_p = torch.log_softmax(torch.stack([value[0, 0].double() / tau, rest.double()]), 0)
+        log_q = torch.tensor([q[j], q0]).double().log()
+        want = float((log_p.exp() * (log_p - log_q)).sum()) * tau ** 2
+        top = TopLogits(torch.tensor([[j]], device="cuda"), value.cuda(), rest[None].cuda())
+        bound = 2.0 ** -15 * abs(float(log_p[1].exp()) - q0) + 2.0 ** -22 * float((log_p - log_q).abs().sum()) + 2.0 ** -48
+        assert abs(float(distill_loss(x.cuda(), top, tau)) - want) <= tau ** 2 * bound, (i, float(distill_loss(x.cuda(), top, tau)), want, bound)
