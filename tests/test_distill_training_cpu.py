@@ -188,8 +188,9 @@ def test_cli_trains_towards_a_saved_teacher(tmpdir_path):
     cfg = build_config(parse_args([
         "--train_type", "distill", "--teacher_path", there, "--param_path", student, "--data_root_path", data,
         "--window_size", "32", "--batch_per_device", "2", "--grad_accum_steps", "1", "--n_epoch", "1", "--ckpt_dir",
-        os.path.join(tmpdir_path, "ckpt"), "--device_type", "cpu", "--backend", "gloo", "--num_workers", "0",
-        "--distill_top_k", "9", "--distill_temperature", "2.0", "--distill_hard_weight", "0.25"]))
+        os.path.join(tmpdir_path, "ckpt"), "--log_dir", os.path.join(tmpdir_path, "logs"), "--device_type", "cpu",
+        "--backend", "gloo", "--num_workers", "0", "--distill_top_k", "9", "--distill_temperature",
+        "2.0", "--distill_hard_weight", "0.25"]))
     built = cfg.teacher_fn()
     assert all(p.dtype == torch.bfloat16 and torch.equal(p, q.bfloat16()) for p, q in zip(built.parameters(), teacher.parameters()))
     assert {k: v for k, v in cfg.extra_kwargs.items() if k.startswith("distill")} == {
