@@ -13,11 +13,11 @@
 // is summed again in 64 bits.
 //
 // A CTA of 512 threads takes a row, two on an SM. Logits that fit stay in its shared memory between the passes over them,
-// others come from L2 again. (In an earlier form 64 rows of 32000 with k = 50 took 13.9 us, 15.4 with 1024 threads and more with
-// clusters of CTAs for a row; the barriers cost what the shorter passes save.) The bound that gathers the candidates is the one
-// of the top logits: the smallest, over the warps, of each warp's j-th largest thread maximum. Where top-p reaches below them
-// (flat rows) or k is large, a histogram over 4096 equal steps of the logits shows in which steps the bound must lie, and the
-// few logits there are ordered and decided exactly.
+// others come from L2 again. (In an earlier form, whose passes were inlined and waited for their instructions, 64 rows of 32000
+// with k = 50 took 13.9 us, 15.4 with 1024 threads and more with clusters of CTAs for a row; not measured again since.) The
+// bound that gathers the candidates is the one of the top logits: the smallest, over the warps, of each warp's j-th largest
+// thread maximum. Where top-p reaches below them (flat rows) or k is large, a histogram over 4096 equal steps of the logits
+// shows in which steps the bound must lie, and the few logits there are ordered and decided exactly.
 //
 // What bounds it is the chain of a row's steps, of 1000 to 5000 clocks each with their barriers (64 rows of 32000, k = 50:
 // load 2100, largest 1400, bound 1600, gather 3800, sort 2800, draw 5600), and for flat rows the 13 operations in 64 bits a logit

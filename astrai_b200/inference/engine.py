@@ -203,7 +203,8 @@ class InferenceEngine:
 
         ``min_p`` drops tokens less likely than that share of the likeliest; with a ``seed`` a prompt's
         tokens are drawn from numbers of its own, the same in any batch and on every call (prompt ``i`` of
-        a list has ``seed + i``; the model's logits may round differently in a batch of another size). Neither goes with a frequency penalty (``ValueError``)."""
+        a list has ``seed + i``; the model's logits may round differently in a batch of another size).
+        Neither goes with a frequency penalty (``ValueError``)."""
         if min_p or seed is not None:
             _check_sampling(top_k, top_p, temperature, frequency_penalty, rep_window, min_p, seed)
         as_list = isinstance(prompt, list)

@@ -97,12 +97,15 @@ def distill_loss(logits: torch.Tensor, teacher: TopLogits, temperature: float = 
 
     ``target [...]`` holds the labels; positions whose target is ``ignore_index`` or outside the vocabulary do not
     count, and without a target all do. A position without any mass of the teacher adds only its label's part. An id
-    that comes twice stands for the sum of its entries' mass. ``k`` is at most 1024.
+    that comes twice stands for the sum of its entries' mass.
 
-    The forward pass also writes the gradient of the logits, for an upstream gradient of ``expected_grad`` (what
-    ``loss * expected_grad`` or a division by the accumulation steps will send back); any other one costs the backward
-    another pass over the logits, with the same result. There is no gradient of the teacher, no forward-mode and no
-    second derivative: under grad mode each is refused.
+    On CUDA ``k`` is at most 1024 and the vocabulary at most 557048 (16-bit types) or 278524 (float32). The forward
+    pass also writes the gradient of the logits, for an upstream gradient of ``expected_grad`` (what ``loss *
+    expected_grad`` or a division by the accumulation steps will send back); any other one costs the backward
+    another pass over the logits, with the same result, and so does a backward that is not in the forward's capture
+    of a CUDA graph. There is no forward-mode and no second derivative: each is refused. CPU tensors take plain
+    operations of PyTorch, which refuse neither, at any ``k``. There is no gradient of the teacher on either: under
+    grad mode it is refused.
     """
     if logits.is_cuda:
         return native().distill_loss(logits, teacher.ids, teacher.values, teacher.rest, float(temperature), target,
