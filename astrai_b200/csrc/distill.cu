@@ -87,7 +87,7 @@ struct Mass {
   __device__ Mass(float outside, float on, float gap, float c) {
     up = exp2_fast(fminf(-gap * c, 0.f));
     down = exp2_fast(fminf(gap * c, 0.f));
-    sum = outside * up + on * down;
+    sum = fmaf(on, down, outside * up);  // (as below, fused by hand: the loss has the same bits with and without a gradient)
   }
   __device__ float inv_rel_outside() const { return up / sum; }  // 1 / all of it, relative to each reference
   __device__ float inv_rel_on() const { return down / sum; }
@@ -411,7 +411,7 @@ __global__ void __launch_bounds__(NT + 32, NT == 256 && TRAIN ? 3 : 0) distill_k
       const float over = vt == -INFINITY ? rest == -INFINITY ? -INFINITY : rest - rest
                                          : fmaf(-vt, a.inv_tau_rest, fmaf(-vt, a.inv_tau, rest));
       const float top = fmaxf(over, 0.f), pr = exp2_fast((over - top) * LOG2E), shrink = exp2_fast(-top * LOG2E);
-      const float mass = teach * shrink + pr, inv = mass != 0.f ? 1.f / mass : 0.f, p0 = pr * inv;
+      const float on_j = __fmul_rn(teach, shrink), mass = on_j + pr, inv = mass != 0.f ? 1.f / mass : 0.f, p0 = pr * inv;
       if constexpr (TRAIN) {
         const float all = mass != 0.f ? 1.f : 0.f, kl = scale * a.kl_grad, ce = scale * a.hard;
         const float share = out != 0.f ? p0 / out : 0.f;
@@ -430,13 +430,14 @@ __global__ void __launch_bounds__(NT + 32, NT == 256 && TRAIN ? 3 : 0) distill_k
         // What the factors up, down, shrink and pr are off by is then in both distributions' sums too, and counts only as much
         // as the two differ.
         const bool o = lane == 1;
-        const float part = o ? pr : teach * shrink, apart = gap * a.inv_tau;
-        const double sum = (double)out * z.up + (double)on * z.down, of_teacher = (double)teach * shrink + pr;
+        const float part = o ? pr : on_j, apart = __fmul_rn(gap, a.inv_tau);
+        const double sum = fma((double)on, (double)z.down, (double)out * z.up);
+        const double of_teacher = fma((double)teach, (double)shrink, (double)pr);
         const double den = of_teacher * (o ? (double)z.up * out : (double)z.down);
         float ln, more = 0.f;
         if (fminf(o ? z.up : z.down, o ? pr : shrink) > 1e-30f && den > 0.) {
           double per = __fdividef(1.f, (float)den);
-          per *= 2. - den * per;
+          per *= fma(-den, per, 2.);
           const double ratio = sum * (o ? pr : shrink) * per;
           const float near = (float)ratio;
           ln = logf(near);
@@ -444,12 +445,13 @@ __global__ void __launch_bounds__(NT + 32, NT == 256 && TRAIN ? 3 : 0) distill_k
         } else {  // far from each other, or nothing there
           ln = (o ? over - top + fmaxf(apart, 0.f) - logf(out) : fmaxf(-apart, 0.f) - top) + logf(z.sum / mass);
         }
-        const float term = part != 0.f ? part * ln : 0.f, add = part != 0.f ? part * more : 0.f;
-        const float crossed = shrink != 0.f ? cross * shrink * a.inv_tau : 0.f;
+        const float term = part != 0.f ? __fmul_rn(part, ln) : 0.f, add = part != 0.f ? __fmul_rn(part, more) : 0.f;
+        const float crossed = shrink != 0.f ? __fmul_rn(cross * shrink, a.inv_tau) : 0.f;
         const float terms = term + __shfl_sync(0xffffffff, term, 1) + crossed + (add + __shfl_sync(0xffffffff, add, 1));
-        float loss = mass != 0.f ? terms * inv * a.kl_loss : 0.f;
+        float loss = mass != 0.f ? __fmul_rn(terms * inv, a.kl_loss) : 0.f;
         // relative to the greater reference: the label lies there unless its logit is far below, so that nothing large cancels
-        if (a.hard > 0.f && lane == 0) loss += a.hard * (((gap > 0.f ? mj : mo) - LogitType<T>::one(vecs.row[y])) + logf(z1.sum));
+        if (a.hard > 0.f && lane == 0)
+          loss = fmaf(a.hard, ((gap > 0.f ? mj : mo) - LogitType<T>::one(vecs.row[y])) + logf(z1.sum), loss);
         if (lane == 0) a.row_loss[row] = loss;
       }
     } else if constexpr (TRAIN) {

@@ -486,3 +486,19 @@ def test_a_small_divergence_keeps_its_digits(V, dtype, tau):
         top = TopLogits(torch.tensor([[j]], device="cuda"), value.cuda(), rest[None].cuda())
         bound = 2.0 ** -15 * abs(float(log_p[1].exp()) - q0) + 2.0 ** -22 * float((log_p - log_q).abs().sum()) + 2.0 ** -48
         assert abs(float(distill_loss(x.cuda(), top, tau)) - want) <= tau ** 2 * bound, (i, float(distill_loss(x.cuda(), top, tau)), want, bound)
+
+
+@pytest.mark.parametrize("V,dtype,tau", [(17500, torch.bfloat16, 1.3), (50001, torch.bfloat16, 2.0), (17500, torch.float32, 1.3),
+                                         (3000, torch.float16, 2.0)])
+def test_the_loss_is_the_same_with_and_without_a_gradient(V, dtype, tau):
+    """Row by row: in a mean a last bit is lost."""
+    from astrai_b200.ops.distill import TopLogits, distill_loss
+
+    x, ids, values, _, y = _inputs(3000, V, 2, dtype, tau, seed=17, sigma=0.01)
+    rest = 10 * torch.randn(3000, device="cuda")
+    leaf = x.detach().requires_grad_()
+    differ = torch.zeros((), device="cuda")
+    for r in range(3000):
+        top = TopLogits(ids[r], values[r], rest[r])
+        differ += distill_loss(leaf[r], top, tau, y[r], 0.3).detach() != distill_loss(x[r], top, tau, y[r], 0.3)
+    assert differ == 0
